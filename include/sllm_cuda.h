@@ -38,6 +38,10 @@
 extern "C" {
 #endif
 
+/* the types of a KV cache (sllm_cuda_ctx_new_kv, sllm_cuda_kv_pages) */
+#define SLLM_CUDA_KV_F32 0
+#define SLLM_CUDA_KV_F16 1
+
 /* ------------------------------------------------------------------ */
 /* status codes                                                        */
 /* ------------------------------------------------------------------ */
@@ -176,6 +180,189 @@ SLLM_CUDA_API int sllm_cuda_i2s_gemm_silu(const uint8_t * w_gate, const uint8_t 
                             const sllm_cuda_act * acts, float * h, void * stream);
 
 /* ------------------------------------------------------------------ */
+/* attention, paged cache and drafts: device pointers                  */
+/* ------------------------------------------------------------------ */
+/*
+ * Operators for a caller that keeps its own device buffers and runs the
+ * projections with the kernels above: what stands between Q/K/V and O
+ * (attention over whole prompts, and over a paged cache while decoding), the
+ * cache itself, and the choice of the next tokens when a draft is verified.
+ * The reference has one contiguous cache per sequence and greedy choice only
+ * (src/forward.c:466-562, :698-726, :876-883); these are additions beside it,
+ * and they do not keep its summation order: results agree to the rounding of
+ * 32-bit sums, not bit for bit.
+ *
+ * Rules for all of them:
+ *   - head dim 128, as everywhere in this library; types are the cache types
+ *     SLLM_CUDA_KV_F32 / _F16;
+ *   - every array is memory of the current device (anything else is refused
+ *     with SLLM_CUDA_ERR_ARG); `stream` belongs to that device;
+ *   - asynchronous on `stream`, no allocation, no synchronisation: they can
+ *     be captured into a CUDA graph;
+ *   - a workspace is the caller's, 16-byte aligned, and holds nothing between
+ *     calls. Calls (or graphs) that may overlap need workspaces of their own;
+ *   - what only the device can see to be wrong (a slot, a length or a page id
+ *     out of range) is reported in `*status`, a device int that may be NULL:
+ *     set to an SLLM_CUDA_ERR_* code, never cleared. Nothing outside the
+ *     arrays is read or written in that case.
+ */
+
+/*
+ * Causal attention over packed whole prompts. Sequence s holds the tokens
+ * cu_seqlens[s] .. cu_seqlens[s + 1] - 1 (n_seq + 1 ascending device ints, the
+ * last at most n_tokens; empty sequences are allowed); token i of a sequence
+ * sees its tokens 0 .. i:
+ *     out[i][h] = sum_j softmax_j(q[i][h] . k[j][g] / sqrt(128)) v[j][g],
+ * g = h / (n_head / n_head_kv). Token t's heads lie at q + t * q_stride
+ * (elements; at least n_head * 128, rows 16-byte aligned), so the parts of one
+ * Q/K/V array can be passed as they are. Rows of `out` behind the last
+ * sequence are not written. A key that a row does not see leaves no trace in
+ * it, not even as an infinity or a NaN. q, k and v have type `type`; out is
+ * f32 or, from f16, f16. f16 inputs are multiplied on the tensor cores with
+ * f32 sums and softmax; the softmax weights are rounded to f16 there.
+ */
+SLLM_CUDA_API int sllm_cuda_attn_prompt(const void * q, size_t q_stride, const void * k, size_t k_stride,
+                                        const void * v, size_t v_stride, int32_t type,
+                                        const int32_t * cu_seqlens, int32_t n_seq, int32_t n_tokens,
+                                        int32_t n_head, int32_t n_head_kv, void * out, size_t out_stride,
+                                        int32_t out_type, void * stream);
+
+/*
+ * A paged KV cache in the caller's memory. Pools are
+ * [n_pages][n_layer][n_head_kv][page_size][128]; slot (sequence) s holds
+ * lens[s] tokens, token t in row t % page_size of page
+ * tables[s * table_width + t / page_size]. refs[p] is the number of table
+ * entries that name page p; 0 means free. Entries behind a slot's last page
+ * mean nothing. An empty cache is all zeros in refs and lens. Slots may share
+ * pages (kv_fork); only a page with one owner is ever written.
+ */
+typedef struct sllm_cuda_kv_pages {
+    void    * k;
+    void    * v;
+    int32_t * refs;         /* [n_pages], 16-byte aligned */
+    int32_t * tables;       /* [n_slots][table_width] */
+    int32_t * lens;         /* [n_slots] */
+    int32_t   n_pages, n_layer, n_head_kv;
+    int32_t   page_size;    /* 16, 32, 64 or 128 tokens */
+    int32_t   n_slots, table_width;
+    int32_t   kv_type;      /* SLLM_CUDA_KV_F32 or SLLM_CUDA_KV_F16 */
+} sllm_cuda_kv_pages;
+
+/* Bytes of the workspace that the four calls below take; 0 for a bad cache. */
+SLLM_CUDA_API size_t sllm_cuda_kv_work_bytes(const sllm_cuda_kv_pages * p);
+
+/*
+ * Slot dst[i] becomes a copy of what slot src[i] held before the call, for all
+ * i < n at once (so a slot may be a source and a destination, as when beams
+ * are reordered); what it held itself is given up. All pages are shared, none
+ * is copied. A slot named twice in dst, or a wrong slot or table, is
+ * SLLM_CUDA_ERR_ARG in *status, and nothing changes.
+ */
+SLLM_CUDA_API int sllm_cuda_kv_fork(const sllm_cuda_kv_pages * p, const int32_t * src, const int32_t * dst,
+                                    int32_t n, void * work, size_t work_bytes, int32_t * status,
+                                    void * stream);
+
+/*
+ * Room for n_new[i] more tokens in slots[i], whose length moves on by as many:
+ * new pages are the free ones of lowest id, in the order of the slots. A
+ * partly filled last page with other owners is replaced by a copy of its live
+ * rows first (copy on write); of owners that are all named in the call, the
+ * last keeps the page. In *status: SLLM_CUDA_ERR_NOMEM when too few pages are
+ * free, SLLM_CUDA_ERR_TOO_LARGE when a table is too short, SLLM_CUDA_ERR_ARG
+ * for wrong or repeated slots; nothing changes then.
+ */
+SLLM_CUDA_API int sllm_cuda_kv_reserve(const sllm_cuda_kv_pages * p, const int32_t * slots,
+                                       const int32_t * n_new, int32_t n, void * work, size_t work_bytes,
+                                       int32_t * status, void * stream);
+
+/*
+ * slots[i] keeps its first new_len[i] tokens (none where new_len is NULL); the
+ * pages behind them lose an owner, and are free when they have none left.
+ * SLLM_CUDA_ERR_ARG in *status, and nothing changes, for wrong or repeated
+ * slots or a length above the slot's.
+ */
+SLLM_CUDA_API int sllm_cuda_kv_release(const sllm_cuda_kv_pages * p, const int32_t * slots,
+                                       const int32_t * new_len, int32_t n, void * work, size_t work_bytes,
+                                       int32_t * status, void * stream);
+
+/*
+ * Moves the live pages to the lowest ids: with L live pages, the live pages at
+ * or above L, ascending, go into the free ones below L, ascending; tables and
+ * counts follow. A table that names a wrong or free page is
+ * SLLM_CUDA_ERR_ARG in *status, and nothing changes.
+ */
+SLLM_CUDA_API int sllm_cuda_kv_compact(const sllm_cuda_kv_pages * p, void * work, size_t work_bytes,
+                                       int32_t * status, void * stream);
+
+/*
+ * Stores the K and V of n_tokens tokens in one layer of the cache: token t at
+ * position pos[t] of slot slot[t], below the slot's length (kv_reserve first).
+ * q and k are rotated (RoPE NEOX, the decode path's operations,
+ * src/ops.c:529-549) with row pos[t] of the [n_ctx][64] angle tables, then q,
+ * k and v are rounded to the cache's type; q_out [n_tokens][n_head][128] and
+ * k_out, v_out [n_tokens][n_head_kv][128] receive them too (k_out and v_out
+ * may be NULL; q and q_out may both be NULL). Strides are floats from a token
+ * to the next. A token with slot[t] < 0 is padding: nothing of it is read
+ * further or written. A token whose slot, position or page is wrong, or whose
+ * page has other owners, sets SLLM_CUDA_ERR_ARG in *status and is left out.
+ * Two tokens for one place leave either of them.
+ */
+SLLM_CUDA_API int sllm_cuda_kv_append(const sllm_cuda_kv_pages * p, int32_t layer, int32_t n_tokens,
+                                      const int32_t * slot, const int32_t * pos, int32_t n_head,
+                                      const float * q, size_t q_stride, const float * k, size_t k_stride,
+                                      const float * v, size_t v_stride, const float * rope_cos,
+                                      const float * rope_sin, int32_t n_ctx, void * q_out, void * k_out,
+                                      void * v_out, int32_t * status, void * stream);
+
+/*
+ * The angle tables of the decode path (host arrays of n_ctx * 64 floats), by
+ * the reference's recurrence on the host libm (src/ops.c:529-549).
+ */
+SLLM_CUDA_API int sllm_cuda_rope_table(int32_t n_ctx, float rope_freq_base, float * cos_out, float * sin_out);
+
+/*
+ * Decode attention of n sequences whose first prefix_len tokens (whole pages)
+ * are the same pages, as forks of one prompt have them: the prefix is read
+ * and multiplied once for all of them, from slots[0]'s table. Sequence b's
+ * n_q query tokens are the last n_q tokens of slots[b]: query j sees the
+ * slot's first lens - n_q + 1 + j tokens (zeros come out where that is none).
+ * n_q > 1 scores drafted tokens. Every query must see the whole prefix;
+ * prefix_len 0 is plain paged decode attention. q and out are
+ * [n][n_q][n_head][128], q of the cache's type, out f32 or, from an f16
+ * cache, f16. A sequence whose slot, length or table is wrong sets
+ * SLLM_CUDA_ERR_ARG in *status and its rows of out mean nothing (all rows,
+ * where the prefix's pages are wrong). n <= 4096, n_q <= 16.
+ */
+SLLM_CUDA_API size_t sllm_cuda_attn_prefix_work_bytes(const sllm_cuda_kv_pages * p, int32_t n, int32_t n_q,
+                                                      int32_t n_head, int32_t prefix_len);
+SLLM_CUDA_API int sllm_cuda_attn_prefix(const sllm_cuda_kv_pages * p, int32_t layer, const void * q,
+                                        const int32_t * slots, int32_t n, int32_t n_q, int32_t n_head,
+                                        int32_t prefix_len, void * out, int32_t out_type, void * work,
+                                        size_t work_bytes, int32_t * status, void * stream);
+
+/*
+ * Verification of drafted tokens, so that what comes out is distributed as
+ * the target's own samples. p [n][k + 1][n_vocab] are the target's
+ * probabilities after 0 .. k drafted tokens, q [n][k][n_vocab] the draft's
+ * (NULL: the draft was certain of its tokens), draft [n][k] its tokens,
+ * n_draft [n] how many each sequence has (NULL: k). With uniforms in [0, 1):
+ * token t is accepted while u_accept[t] * q_t(x_t) < p_t(x_t); at the first
+ * refusal t the next token is drawn from max(p_t - q_t, 0) (from p_t where
+ * that has no mass), after the last accepted one from p: the first index whose
+ * running sum exceeds u_draw times the sum (64-bit sums; u_draw within their
+ * rounding of a border may take the neighbour). Negative, NaN and infinite
+ * entries count as 0. tokens [n][k + 1] receives the accepted tokens, the
+ * drawn one and -1 behind it, count [n] their number; the drawn token is -1
+ * where p has no mass either. A drafted id out of range is refused, a draft
+ * length out of range clamped, with SLLM_CUDA_ERR_ARG in *status.
+ * k <= 64, n <= 65536.
+ */
+SLLM_CUDA_API int sllm_cuda_spec_verify(const float * p, const float * q, const int32_t * draft,
+                                        const int32_t * n_draft, const float * u_accept, const float * u_draw,
+                                        int32_t n, int32_t k, int32_t n_vocab, int32_t * tokens, int32_t * count,
+                                        int32_t * status, void * stream);
+
+/* ------------------------------------------------------------------ */
 /* model level: host pointers                                          */
 /* ------------------------------------------------------------------ */
 
@@ -257,8 +444,6 @@ SLLM_CUDA_API int  sllm_cuda_ctx_new(const sllm_cuda_model * m, int32_t n_ctx,
  * many greedy tokens still agree. State files stay SLKV v1 with f32 values
  * (export widens exactly, import rounds).
  */
-#define SLLM_CUDA_KV_F32 0
-#define SLLM_CUDA_KV_F16 1
 SLLM_CUDA_API int  sllm_cuda_ctx_new_kv(const sllm_cuda_model * m, int32_t n_ctx, int32_t kv_type,
                                         sllm_cuda_ctx ** out);
 SLLM_CUDA_API void sllm_cuda_ctx_free(sllm_cuda_ctx * c);

@@ -62,4 +62,17 @@ class TpSynthDesc(C.Structure):
     ]
 
 
+class KvPages(C.Structure):
+    """sllm_cuda_kv_pages: a paged KV cache in the caller's device memory."""
+    _fields_ = [
+        ("k", C.c_void_p), ("v", C.c_void_p),
+        ("refs", C.c_void_p), ("tables", C.c_void_p), ("lens", C.c_void_p),
+        ("n_pages", C.c_int32), ("n_layer", C.c_int32), ("n_head_kv", C.c_int32), ("page_size", C.c_int32),
+        ("n_slots", C.c_int32), ("table_width", C.c_int32), ("kv_type", C.c_int32),
+    ]
+
+
+KV_F32, KV_F16 = 0, 1
+HEAD_DIM = 128
+
 TP_ID_BYTES = 128

@@ -780,6 +780,20 @@ void sllm::rope_table(int n_ctx, int n_rot, float base, std::vector<float>& cs, 
     }
 }
 
+extern "C" int sllm_cuda_rope_table(int32_t n_ctx, float rope_freq_base, float* cos_out, float* sin_out) {
+    if (n_ctx < 1 || n_ctx > (1 << 24) || !(rope_freq_base > 0.0f) || cos_out == nullptr || sin_out == nullptr)
+        return fail(SLLM_CUDA_ERR_ARG, "rope_table: %d positions, base %g", n_ctx, (double)rope_freq_base);
+    try {
+        std::vector<float> cs, sn;
+        rope_table(n_ctx, 128, rope_freq_base, cs, sn);
+        std::memcpy(cos_out, cs.data(), cs.size() * sizeof(float));
+        std::memcpy(sin_out, sn.data(), sn.size() * sizeof(float));
+    } catch (const std::bad_alloc&) {
+        return fail(SLLM_CUDA_ERR_NOMEM, "rope_table: %d positions", n_ctx);
+    }
+    return SLLM_CUDA_OK;
+}
+
 extern "C" void sllm_cuda_ctx_free(sllm_cuda_ctx* c) {
     if (c == nullptr) return;
     cudaSetDevice(c->m->device);

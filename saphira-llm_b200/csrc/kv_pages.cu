@@ -1,0 +1,709 @@
+// kv_pages.cu -- the paged KV cache: forking, reserving (with copy on write),
+// releasing and compacting pages, and the store of new tokens.
+//
+// The cache is the caller's memory: pools of pages, one reference count per
+// page (0 = free), one table row and one length per slot (sequence). Every
+// operator first checks all that it will use (slots, lengths, page ids,
+// counts) and changes nothing when something is wrong, so the bookkeeping
+// runs in one CTA or one cluster: a phase ends at a barrier, not at a launch.
+// What it decides to copy goes into a list in the caller's workspace, and a
+// second launch over the whole device (overlapped with the first by
+// programmatic dependent launch) moves the bytes.
+//
+// A page is given out lowest id first, in the order of the call's slots, so
+// the tables a call leaves are the same every time; the reference counts are
+// integer atomics, whose order does not matter.
+
+#include <cooperative_groups.h>
+
+#include "serve.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace sllm {
+namespace {
+
+constexpr int kClCtas = 8;          // CTAs of a bookkeeping cluster
+constexpr int kClThreads = 512;
+constexpr int kResThreads = 1024;   // the reserving CTA
+constexpr int kHead = 16;           // ints before the workspace's arrays; [0] is the number of copies
+
+struct Work {                       // the caller's workspace, as ints
+    int* count;
+    int* mark;                      // [n_slots] how often a slot is named
+    int* slot_page;                 // [n_slots] the last page a slot will write to, or -1
+    int* slot_need;                 // [n_slots] first page of its share of the free list; bit 31: copies
+    int* list;                      // [n_pages] free pages, or compact's map from old to new ids
+    int4* pairs;                    // [max(n_slots, n_pages)] copies: source, destination, rows
+    int* rows;                      // [n_slots][width] tables being forked
+};
+
+__host__ __device__ inline size_t align16(size_t n) { return (n + 15) & ~(size_t)15; }
+
+__host__ __device__ inline size_t work_ints(int n_pages, int n_slots, int width) {
+    const size_t pairs = (size_t)(n_pages > n_slots ? n_pages : n_slots);
+    return kHead + 3 * align16(n_slots) + align16(n_pages) + 4 * pairs + align16((size_t)n_slots * width);
+}
+
+__host__ __device__ inline Work work_of(void* base, int n_pages, int n_slots, int width) {
+    const size_t pairs = (size_t)(n_pages > n_slots ? n_pages : n_slots);
+    Work w;
+    int* p = static_cast<int*>(base);
+    w.count = p;
+    p += kHead;
+    w.mark = p;
+    p += align16(n_slots);
+    w.slot_page = p;
+    p += align16(n_slots);
+    w.slot_need = p;
+    p += align16(n_slots);
+    w.list = p;
+    p += align16(n_pages);
+    w.pairs = reinterpret_cast<int4*>(p);
+    p += 4 * pairs;
+    w.rows = p;
+    return w;
+}
+
+__device__ __forceinline__ int used_of(int len, int page) { return (len + page - 1) / page; }
+
+// the used entries of a slot's table name live pages (threads t, t + nt, ...)
+__device__ __forceinline__ bool row_ok(const PagesDev& p, int slot, int t, int nt) {
+    const int len = p.lens[slot];
+    if (len < 0 || len > p.cap) return false;
+    const int used = used_of(len, p.page);
+    bool ok = true;
+    for (int j = t; j < used; j += nt) {
+        const int id = p.tables[(size_t)slot * p.width + j];
+        ok = ok && id >= 0 && id < p.n_pages && p.refs[id] > 0;
+    }
+    return ok;
+}
+
+// exclusive sum over the block; *total gets the sum. NT threads, all of them.
+template <int NT>
+__device__ __forceinline__ int block_scan(int v, int* total) {
+    __shared__ int part[NT / 32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int x = v;
+    #pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+    }
+    if (lane == 31) part[warp] = x;
+    __syncthreads();
+    int before = 0, all = 0;
+    #pragma unroll
+    for (int w = 0; w < NT / 32; ++w) {
+        const int y = part[w];
+        before += w < warp ? y : 0;
+        all += y;
+    }
+    __syncthreads();
+    *total = all;
+    return before + x - v;
+}
+
+// ---------------------------------------------------------------------------
+// fork: dst[i] becomes what src[i] holds, for all i at once. The tables of
+// the sources are staged first, so a slot may be a source and a destination
+// (a beam search's reordering); every page a destination held loses one
+// reference, every page of a source gains one. No page is copied here: a
+// shared last page is copied when a slot next reserves tokens in it.
+// ---------------------------------------------------------------------------
+__global__ void __cluster_dims__(kClCtas, 1, 1) __launch_bounds__(kClThreads)
+kv_fork_kernel(const PagesDev p, const int32_t* src, const int32_t* dst, int n, void* work, int32_t* status) {
+    cg::cluster_group cl = cg::this_cluster();
+    __shared__ int bad;
+    const Work w = work_of(work, p.n_pages, p.n_slots, p.width);
+    const int rank = (int)cl.block_rank(), t = threadIdx.x;
+    if (t == 0) bad = 0;
+    for (int i = rank * kClThreads + t; i < p.n_slots; i += kClCtas * kClThreads) w.mark[i] = 0;
+    cl.sync();
+    int* const bad0 = cl.map_shared_rank(&bad, 0);
+    for (int i = rank; i < n; i += kClCtas) {
+        const int s = src[i], d = dst[i];
+        bool ok = s >= 0 && s < p.n_slots && d >= 0 && d < p.n_slots;
+        if (ok) ok = row_ok(p, s, t, kClThreads) && row_ok(p, d, t, kClThreads);
+        if (t == 0 && d >= 0 && d < p.n_slots && atomicAdd(&w.mark[d], 1) > 0) ok = false;
+        if (!ok) atomicExch(bad0, 1);
+    }
+    cl.sync();
+    const int any = *bad0;
+    cl.sync();                      // nobody leaves before all have read CTA 0's word
+    if (any != 0) {
+        if (rank == 0 && t == 0) raise(status, SLLM_CUDA_ERR_ARG);
+        return;
+    }
+    for (int i = rank; i < n; i += kClCtas) {
+        const int s = src[i], len = p.lens[s], used = used_of(len, p.page);
+        for (int j = t; j < used; j += kClThreads) {
+            const int id = p.tables[(size_t)s * p.width + j];
+            w.rows[(size_t)i * p.width + j] = id;
+            atomicAdd(&p.refs[id], 1);
+        }
+        if (t == 0) w.slot_page[i] = len;
+    }
+    cl.sync();
+    for (int i = rank; i < n; i += kClCtas) {
+        const int d = dst[i], len = w.slot_page[i], used = used_of(len, p.page);
+        const int was = used_of(p.lens[d], p.page);
+        for (int j = t; j < max(used, was); j += kClThreads) {
+            int32_t* e = p.tables + (size_t)d * p.width + j;
+            if (j < was) atomicSub(&p.refs[*e], 1);
+            if (j < used) *e = w.rows[(size_t)i * p.width + j];
+        }
+        __syncthreads();            // every thread has read the old length
+        if (t == 0) p.lens[d] = len;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// release: slots[i] keeps its first new_len[i] tokens (none without new_len)
+// ---------------------------------------------------------------------------
+__global__ void __cluster_dims__(kClCtas, 1, 1) __launch_bounds__(kClThreads)
+kv_release_kernel(const PagesDev p, const int32_t* slots, const int32_t* new_len, int n, void* work,
+                  int32_t* status) {
+    cg::cluster_group cl = cg::this_cluster();
+    __shared__ int bad;
+    const Work w = work_of(work, p.n_pages, p.n_slots, p.width);
+    const int rank = (int)cl.block_rank(), t = threadIdx.x;
+    if (t == 0) bad = 0;
+    for (int i = rank * kClThreads + t; i < p.n_slots; i += kClCtas * kClThreads) w.mark[i] = 0;
+    cl.sync();
+    int* const bad0 = cl.map_shared_rank(&bad, 0);
+    for (int i = rank; i < n; i += kClCtas) {
+        const int s = slots[i];
+        bool ok = s >= 0 && s < p.n_slots;
+        if (ok) {
+            ok = row_ok(p, s, t, kClThreads);
+            const int nl = new_len != nullptr ? new_len[i] : 0;
+            if (nl < 0 || nl > p.lens[s]) ok = false;
+            if (t == 0 && atomicAdd(&w.mark[s], 1) > 0) ok = false;
+        }
+        if (!ok) atomicExch(bad0, 1);
+    }
+    cl.sync();
+    const int any = *bad0;
+    cl.sync();
+    if (any != 0) {
+        if (rank == 0 && t == 0) raise(status, SLLM_CUDA_ERR_ARG);
+        return;
+    }
+    for (int i = rank; i < n; i += kClCtas) {
+        const int s = slots[i], nl = new_len != nullptr ? new_len[i] : 0;
+        const int keep = used_of(nl, p.page), was = used_of(p.lens[s], p.page);
+        for (int j = keep + t; j < was; j += kClThreads) atomicSub(&p.refs[p.tables[(size_t)s * p.width + j]], 1);
+        __syncthreads();
+        if (t == 0) p.lens[s] = nl;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// reserve: pages for n_new[i] more tokens of slots[i], and its length moved
+// on. A last page that is partly filled, will be written and has other
+// owners is replaced by a copy: slot by slot in the call's order, so of r
+// owners named in one call that are all its owners the last keeps the page.
+// One CTA: the call's slots are few, and the free pages are found by one pass
+// over the counts, 16 per thread in flight.
+// ---------------------------------------------------------------------------
+__global__ void __launch_bounds__(kResThreads)
+kv_reserve_kernel(const PagesDev p, const int32_t* slots, const int32_t* n_new, int n, void* work, int32_t* status) {
+    __shared__ int err, n_pairs;
+    pdl_trigger();
+    const Work w = work_of(work, p.n_pages, p.n_slots, p.width);
+    const int t = threadIdx.x;
+    if (t == 0) {
+        err = 0;
+        n_pairs = 0;
+        *w.count = 0;
+    }
+    for (int i = t; i < n; i += kResThreads) {
+        const int s = slots[i];
+        if (s >= 0 && s < p.n_slots) w.mark[s] = 0;
+    }
+    __syncthreads();
+    int total = 0;
+    for (int base = 0; base < n; base += kResThreads) {
+        const int i = base + t;
+        int fresh = 0, last = -1, owners = 0;
+        if (i < n) {
+            const int s = slots[i], nn = n_new[i];
+            int e = 0;
+            if (s < 0 || s >= p.n_slots || nn < 0 || atomicAdd(&w.mark[s], 1) > 0) {
+                e = SLLM_CUDA_ERR_ARG;
+            } else {
+                const int cur = p.lens[s];
+                if (cur < 0 || cur > p.cap) {
+                    e = SLLM_CUDA_ERR_ARG;
+                } else if (nn > p.cap - cur) {
+                    e = SLLM_CUDA_ERR_TOO_LARGE;
+                } else {
+                    fresh = used_of(cur + nn, p.page) - used_of(cur, p.page);
+                    if (nn > 0 && cur % p.page != 0) {
+                        last = p.tables[(size_t)s * p.width + cur / p.page];
+                        if (last < 0 || last >= p.n_pages || (owners = p.refs[last]) <= 0) {
+                            e = SLLM_CUDA_ERR_ARG;
+                            last = -1;
+                        }
+                    }
+                }
+            }
+            if (e != 0) atomicCAS(&err, 0, e);
+            w.slot_page[i] = last;
+        }
+        __syncthreads();
+        int cow = 0;
+        if (owners > 1) {
+            int before = 0;         // earlier slots of this call that write to the same page
+            for (int j = 0; j < i; ++j) before += w.slot_page[j] == last ? 1 : 0;
+            cow = owners - before > 1 ? 1 : 0;
+        }
+        int sum;
+        const int at = block_scan<kResThreads>(cow + fresh, &sum);
+        if (i < n) w.slot_need[i] = (total + at) | (cow << 31);
+        total += sum;
+    }
+    __syncthreads();
+    if (err != 0) {                 // the same for every thread
+        if (t == 0) raise(status, err);
+        return;
+    }
+    // the `total` lowest free pages
+    constexpr int PER = 16;
+    int found = 0;
+    for (int base = 0; base < p.n_pages && found < total; base += kResThreads * PER) {
+        const int b = base + t * PER;
+        int r[PER];
+        if (b + PER <= p.n_pages) {
+            #pragma unroll
+            for (int k = 0; k < PER / 4; ++k) {
+                const int4 v = *reinterpret_cast<const int4*>(p.refs + b + 4 * k);
+                r[4 * k] = v.x; r[4 * k + 1] = v.y; r[4 * k + 2] = v.z; r[4 * k + 3] = v.w;
+            }
+        } else {
+            #pragma unroll
+            for (int k = 0; k < PER; ++k) r[k] = b + k < p.n_pages ? p.refs[b + k] : 1;
+        }
+        int c = 0;
+        #pragma unroll
+        for (int k = 0; k < PER; ++k) c += r[k] == 0 ? 1 : 0;
+        int sum;
+        int at = found + block_scan<kResThreads>(c, &sum);
+        #pragma unroll
+        for (int k = 0; k < PER; ++k)
+            if (r[k] == 0) {
+                if (at < total) w.list[at] = b + k;
+                ++at;
+            }
+        found += sum;
+    }
+    __syncthreads();
+    if (found < total) {
+        if (t == 0) raise(status, SLLM_CUDA_ERR_NOMEM);
+        return;
+    }
+    // hand them out, one warp per slot
+    const int lane = t & 31;
+    for (int i = t >> 5; i < n; i += kResThreads / 32) {
+        const int s = slots[i], nn = n_new[i], cur = p.lens[s];
+        const int need = w.slot_need[i], cow = need < 0 ? 1 : 0, at = need & 0x7fffffff;
+        const int first = used_of(cur, p.page), fresh = used_of(cur + nn, p.page) - first;
+        int32_t* row = p.tables + (size_t)s * p.width;
+        for (int x = lane; x < fresh; x += 32) {
+            const int id = w.list[at + cow + x];
+            row[first + x] = id;
+            p.refs[id] = 1;
+        }
+        if (lane == 0) {
+            if (cow) {
+                const int id = w.list[at], last = w.slot_page[i];
+                row[cur / p.page] = id;
+                p.refs[id] = 1;
+                atomicSub(&p.refs[last], 1);
+                w.pairs[atomicAdd(&n_pairs, 1)] = make_int4(last, id, cur % p.page, 0);
+            }
+            p.lens[s] = cur + nn;
+        }
+    }
+    __syncthreads();
+    if (t == 0) *w.count = n_pairs;
+}
+
+// ---------------------------------------------------------------------------
+// compact: with L live pages, every live page at or above L moves into a free
+// page below L (both in ascending order). Sources and destinations are
+// disjoint, so the copies need no order among themselves.
+// ---------------------------------------------------------------------------
+__global__ void __cluster_dims__(kClCtas, 1, 1) __launch_bounds__(kClThreads)
+kv_compact_kernel(const PagesDev p, void* work, int32_t* status) {
+    cg::cluster_group cl = cg::this_cluster();
+    __shared__ int bad, live_cnt, src_cnt;
+    pdl_trigger();
+    const Work w = work_of(work, p.n_pages, p.n_slots, p.width);
+    const int rank = (int)cl.block_rank(), t = threadIdx.x;
+    if (t == 0) {
+        bad = 0;
+        live_cnt = 0;
+        src_cnt = 0;
+    }
+    cl.sync();
+    int* const bad0 = cl.map_shared_rank(&bad, 0);
+    // the tables first: nothing moves when one is wrong
+    {
+        const int lane = t & 31;
+        bool ok = true;
+        for (int s = rank * (kClThreads / 32) + (t >> 5); s < p.n_slots; s += kClCtas * (kClThreads / 32))
+            ok = row_ok(p, s, lane, 32) && ok;
+        if (!ok) atomicExch(bad0, 1);
+    }
+    // this CTA's share of the pages: a contiguous run, 512 at a time
+    const int per = ((p.n_pages + kClCtas - 1) / kClCtas + kClThreads - 1) / kClThreads * kClThreads;
+    const int lo = min(rank * per, p.n_pages), hi = min(lo + per, p.n_pages);
+    int c = 0;
+    for (int i = lo + t; i < hi; i += kClThreads) c += p.refs[i] > 0 ? 1 : 0;
+    if (c > 0) atomicAdd(&live_cnt, c);
+    cl.sync();
+    const int any = *bad0;
+    int live = 0;
+    for (int r = 0; r < kClCtas; ++r) live += *cl.map_shared_rank(&live_cnt, r);
+    // sources of this share: live pages at or above `live`
+    int cs = 0;
+    for (int i = max(lo, live) + t; i < hi; i += kClThreads) cs += p.refs[i] > 0 ? 1 : 0;
+    if (cs > 0) atomicAdd(&src_cnt, cs);
+    cl.sync();
+    int src0 = 0, total = 0;        // sources before this share, and all of them
+    for (int r = 0; r < kClCtas; ++r) {
+        const int x = *cl.map_shared_rank(&src_cnt, r);
+        src0 += r < rank ? x : 0;
+        total += x;
+    }
+    // free pages below `live` before this share = pages below it that are not live
+    int live_before = 0;
+    for (int r = 0; r < rank; ++r) live_before += *cl.map_shared_rank(&live_cnt, r);
+    cl.sync();                      // all remote reads are done
+    if (any != 0) {
+        if (rank == 0 && t == 0) {
+            *w.count = 0;
+            raise(status, SLLM_CUDA_ERR_ARG);
+        }
+        return;
+    }
+    int dst0 = min(lo, live) - (live_before - src0);    // live pages below `live` before this share
+    for (int base = lo; base < hi; base += kClThreads) {
+        const int i = base + t;
+        const int ref = i < hi ? p.refs[i] : 0;
+        const int is_src = i < hi && i >= live && ref > 0 ? 1 : 0;
+        const int is_dst = i < hi && i < live && ref <= 0 ? 1 : 0;
+        int sums;                   // both ranks in one scan: 16 bits each suffice for 512 threads
+        const int at = block_scan<kClThreads>(is_src | (is_dst << 16), &sums);
+        if (is_src) {
+            w.pairs[src0 + (at & 0xffff)].x = i;
+            w.pairs[src0 + (at & 0xffff)].w = ref;
+        }
+        if (is_dst) w.pairs[dst0 + (at >> 16)].y = i;
+        if (i < hi) w.list[i] = i;
+        src0 += sums & 0xffff;
+        dst0 += sums >> 16;
+    }
+    cl.sync();
+    for (int i = rank * kClThreads + t; i < total; i += kClCtas * kClThreads) {
+        const int4 m = w.pairs[i];
+        w.pairs[i].z = p.page;
+        w.list[m.x] = m.y;
+        p.refs[m.y] = m.w;
+        p.refs[m.x] = 0;
+    }
+    if (rank == 0 && t == 0) *w.count = total;
+}
+
+// ---------------------------------------------------------------------------
+// the copies: one warp per run of rows (a page's rows of one layer and kv
+// head are contiguous), 4 KB in flight per warp. Only the rows a copy names
+// move. For compact the same launch rewrites the tables.
+// ---------------------------------------------------------------------------
+__global__ void __launch_bounds__(256)
+kv_copy_kernel(const PagesDev p, uint8_t* k, uint8_t* v, int runs, int row_bytes, void* work, int remap) {
+    pdl_wait();
+    const Work w = work_of(work, p.n_pages, p.n_slots, p.width);
+    const int count = *w.count;
+    if (count <= 0) return;
+    const int lane = threadIdx.x & 31;
+    const long long nw = (long long)gridDim.x * 8, w0 = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const long long units = (long long)count * 2 * runs;
+    const size_t run_bytes = (size_t)p.page * row_bytes;
+    for (long long u = w0; u < units; u += nw) {
+        const long long pr = u / (2 * runs);
+        const int r = (int)(u - pr * (2 * runs));
+        const int4 m = w.pairs[pr];
+        uint8_t* const pool = r < runs ? k : v;
+        const size_t off = (size_t)(r < runs ? r : r - runs) * run_bytes;
+        const uint4* a = reinterpret_cast<const uint4*>(pool + (size_t)m.x * runs * run_bytes + off);
+        uint4* b = reinterpret_cast<uint4*>(pool + (size_t)m.y * runs * run_bytes + off);
+        const int nv = m.z * (row_bytes >> 4);
+        for (int x = lane; x < nv; x += 256) {
+            uint4 r8[8];
+            #pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (x + 32 * j < nv) r8[j] = __ldcs(a + x + 32 * j);
+            #pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (x + 32 * j < nv) __stcs(b + x + 32 * j, r8[j]);
+        }
+    }
+    if (remap) {
+        for (long long s = w0; s < p.n_slots; s += nw) {
+            const int used = used_of(p.lens[s], p.page);
+            int32_t* row = p.tables + (size_t)s * p.width;
+            for (int j = lane; j < used; j += 32) row[j] = w.list[row[j]];
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// append: RoPE (the decode path's rotation from the same angle table),
+// conversion and store. One warp per (token, head): lane l holds elements
+// 2l, 2l+1 and 2l+64, 2l+65, which are the rotation's pairs. Bound by HBM:
+// every value is read once and written once (k and v twice).
+// ---------------------------------------------------------------------------
+struct AppendParams {
+    const int32_t* slot;
+    const int32_t* pos;
+    const float* q;
+    const float* k;
+    const float* v;
+    size_t qs, ks, vs;              // floats from a token to the next
+    const float* cs;
+    const float* sn;
+    void* qo;
+    void* ko;
+    void* vo;
+    void* kp;                       // the layer's slice of page 0
+    void* vp;
+    size_t page_stride;             // elements from a page to the next
+    int n_tokens, n_head, n_kv, n_ctx;
+    int32_t* status;
+};
+
+template <class T>
+__device__ __forceinline__ void st2(T* p, float a, float b);
+template <> __device__ __forceinline__ void st2<float>(float* p, float a, float b) {
+    *reinterpret_cast<float2*>(p) = make_float2(a, b);
+}
+template <> __device__ __forceinline__ void st2<__half>(__half* p, float a, float b) {
+    *reinterpret_cast<__half2*>(p) = __floats2half2_rn(a, b);
+}
+
+template <class T>
+__global__ void __launch_bounds__(256)
+kv_append_kernel(const PagesDev p, const __grid_constant__ AppendParams a) {
+    const int lane = threadIdx.x & 31;
+    const int heads = (a.q != nullptr ? a.n_head : 0) + 2 * a.n_kv;
+    const long long u = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int tok = (int)(u / heads);
+    if (tok >= a.n_tokens) return;
+    int h = (int)(u - (long long)tok * heads);
+    const int slot = a.slot[tok], pos = a.pos[tok];
+    if (slot < 0) return;           // a padding token
+    int id = -1;
+    if (slot < p.n_slots && pos >= 0 && pos < a.n_ctx && pos < p.cap && pos < p.lens[slot])
+        id = p.tables[(size_t)slot * p.width + pos / p.page];
+    // a shared page is never written: its other owners would change
+    if (id < 0 || id >= p.n_pages || p.refs[id] != 1) {
+        if (lane == 0) raise(a.status, SLLM_CUDA_ERR_ARG);
+        return;
+    }
+    const int kind = h < 2 * a.n_kv ? (h < a.n_kv ? 1 : 2) : 0;
+    h = kind == 0 ? h - 2 * a.n_kv : kind == 1 ? h : h - a.n_kv;
+    const float* x = (kind == 0 ? a.q + tok * a.qs : kind == 1 ? a.k + tok * a.ks : a.v + tok * a.vs) + h * kServeDim;
+    float2 lo = *reinterpret_cast<const float2*>(x + 2 * lane);
+    float2 hi = *reinterpret_cast<const float2*>(x + 64 + 2 * lane);
+    if (kind != 2) {
+        const float2 c = *reinterpret_cast<const float2*>(a.cs + (size_t)pos * 64 + 2 * lane);
+        const float2 s = *reinterpret_cast<const float2*>(a.sn + (size_t)pos * 64 + 2 * lane);
+        const float2 u0 = lo, u1 = hi;
+        lo.x = __fsub_rn(__fmul_rn(u0.x, c.x), __fmul_rn(u1.x, s.x));
+        lo.y = __fsub_rn(__fmul_rn(u0.y, c.y), __fmul_rn(u1.y, s.y));
+        hi.x = __fadd_rn(__fmul_rn(u0.x, s.x), __fmul_rn(u1.x, c.x));
+        hi.y = __fadd_rn(__fmul_rn(u0.y, s.y), __fmul_rn(u1.y, c.y));
+    }
+    T* out = static_cast<T*>(kind == 0 ? a.qo : kind == 1 ? a.ko : a.vo);
+    if (out != nullptr) {
+        out += ((size_t)tok * (kind == 0 ? a.n_head : a.n_kv) + h) * kServeDim;
+        st2(out + 2 * lane, lo.x, lo.y);
+        st2(out + 64 + 2 * lane, hi.x, hi.y);
+    }
+    if (kind != 0) {
+        T* row = static_cast<T*>(kind == 1 ? a.kp : a.vp) + (size_t)id * a.page_stride +
+                 ((size_t)h * p.page + pos % p.page) * kServeDim;
+        st2(row + 2 * lane, lo.x, lo.y);
+        st2(row + 64 + 2 * lane, hi.x, hi.y);
+    }
+}
+
+int check_call(const sllm_cuda_kv_pages* p, const char* who, int n, const void* work, size_t work_bytes,
+               const void* a, const void* b, const void* status) {
+    int rc = check_pages(p, who);
+    if (rc != SLLM_CUDA_OK) return rc;
+    if (n < 0 || n > p->n_slots) return fail(SLLM_CUDA_ERR_ARG, "%s: %d slots named, the cache has %d", who, n, p->n_slots);
+    if (work == nullptr || !aligned16(work) || work_bytes < sllm_cuda_kv_work_bytes(p))
+        return fail(SLLM_CUDA_ERR_ARG, "%s: workspace of %zu bytes, %zu needed, 16-byte aligned", who, work_bytes,
+                    sllm_cuda_kv_work_bytes(p));
+    const void* ptr[] = {p->k, p->v, p->refs, p->tables, p->lens, work, a, b, status};
+    const char* name[] = {"k", "v", "refs", "tables", "lens", "work", "slots", "slots or lengths", "status"};
+    for (int i = 0; i < 9; ++i)
+        if (ptr[i] != nullptr && (rc = need_device(ptr[i], who, name[i])) != SLLM_CUDA_OK) return rc;
+    return SLLM_CUDA_OK;
+}
+
+cudaError_t launch_copies(const sllm_cuda_kv_pages& p, long long most, void* work, int remap, cudaStream_t st) {
+    int dev = 0;
+    cudaGetDevice(&dev);
+    const int runs = p.n_layer * p.n_head_kv;
+    const long long units = most * 2 * runs + (remap ? p.n_slots : 0);
+    const long long blocks = (units + 7) / 8, cap = 8LL * num_sms_of(dev);
+    return launch(kv_copy_kernel, dim3((unsigned)(blocks < 1 ? 1 : blocks < cap ? blocks : cap)), dim3(256), 0, st, true,
+                  pages_dev(p), static_cast<uint8_t*>(p.k), static_cast<uint8_t*>(p.v), runs,
+                  (int)(kServeDim * kv_elt_bytes(p.kv_type)), work, remap);
+}
+
+}  // namespace
+
+int need_device(const void* p, const char* who, const char* arg) {
+    cudaPointerAttributes at{};
+    const cudaError_t e = cudaPointerGetAttributes(&at, p);
+    if (e != cudaSuccess) return cuda_fail(e, who);
+    int dev = -1;
+    if (cudaGetDevice(&dev) != cudaSuccess) return cuda_fail(cudaGetLastError(), who);
+    if (at.type == cudaMemoryTypeManaged) return SLLM_CUDA_OK;
+    if (at.type != cudaMemoryTypeDevice || at.device != dev)
+        return fail(SLLM_CUDA_ERR_ARG, "%s: %s is not memory of the current device (%d)", who, arg, dev);
+    return SLLM_CUDA_OK;
+}
+
+int check_pages(const sllm_cuda_kv_pages* p, const char* who) {
+    if (p == nullptr || p->k == nullptr || p->v == nullptr || p->refs == nullptr || p->tables == nullptr ||
+        p->lens == nullptr)
+        return fail(SLLM_CUDA_ERR_ARG, "%s: a NULL cache or array", who);
+    if (p->kv_type != SLLM_CUDA_KV_F32 && p->kv_type != SLLM_CUDA_KV_F16)
+        return fail(SLLM_CUDA_ERR_ARG, "%s: unknown cache type %d", who, p->kv_type);
+    if (p->page_size != 16 && p->page_size != 32 && p->page_size != 64 && p->page_size != 128)
+        return fail(SLLM_CUDA_ERR_UNSUPPORTED, "%s: pages of %d tokens (16, 32, 64 or 128)", who, p->page_size);
+    if (p->n_pages < 1 || p->n_pages > (1 << 24) || p->n_layer < 1 || p->n_layer > 1024 || p->n_head_kv < 1 ||
+        p->n_head_kv > 1024 || p->n_slots < 1 || p->n_slots > (1 << 16) || p->table_width < 1 ||
+        p->table_width > (1 << 23) || (long long)p->table_width * p->page_size > 0x7fffff00LL ||
+        (long long)p->n_slots * p->table_width > 0x7fffffffLL)
+        return fail(SLLM_CUDA_ERR_ARG, "%s: cache of %d pages, %d layers, %d kv heads, %d slots, %d entries a table",
+                    who, p->n_pages, p->n_layer, p->n_head_kv, p->n_slots, p->table_width);
+    if (!aligned16(p->k) || !aligned16(p->v) || !aligned16(p->refs))
+        return fail(SLLM_CUDA_ERR_ARG, "%s: k, v and refs must be 16-byte aligned", who);
+    return SLLM_CUDA_OK;
+}
+
+}  // namespace sllm
+
+using namespace sllm;
+
+extern "C" size_t sllm_cuda_kv_work_bytes(const sllm_cuda_kv_pages* p) {
+    if (check_pages(p, "kv_work_bytes") != SLLM_CUDA_OK) return 0;
+    return 4 * work_ints(p->n_pages, p->n_slots, p->table_width);
+}
+
+extern "C" int sllm_cuda_kv_fork(const sllm_cuda_kv_pages* p, const int32_t* src, const int32_t* dst, int32_t n,
+                                 void* work, size_t work_bytes, int32_t* status, void* stream) {
+    if (src == nullptr || dst == nullptr) return fail(SLLM_CUDA_ERR_ARG, "kv_fork: NULL slots");
+    const int rc = check_call(p, "kv_fork", n, work, work_bytes, src, dst, status);
+    if (rc != SLLM_CUDA_OK || n == 0) return rc;
+    kv_fork_kernel<<<kClCtas, kClThreads, 0, (cudaStream_t)stream>>>(pages_dev(*p), src, dst, n, work, status);
+    CK(cudaGetLastError(), "kv_fork launch");
+    count_launches(1);
+    return SLLM_CUDA_OK;
+}
+
+extern "C" int sllm_cuda_kv_release(const sllm_cuda_kv_pages* p, const int32_t* slots, const int32_t* new_len,
+                                    int32_t n, void* work, size_t work_bytes, int32_t* status, void* stream) {
+    if (slots == nullptr) return fail(SLLM_CUDA_ERR_ARG, "kv_release: NULL slots");
+    const int rc = check_call(p, "kv_release", n, work, work_bytes, slots, new_len, status);
+    if (rc != SLLM_CUDA_OK || n == 0) return rc;
+    kv_release_kernel<<<kClCtas, kClThreads, 0, (cudaStream_t)stream>>>(pages_dev(*p), slots, new_len, n, work, status);
+    CK(cudaGetLastError(), "kv_release launch");
+    count_launches(1);
+    return SLLM_CUDA_OK;
+}
+
+extern "C" int sllm_cuda_kv_reserve(const sllm_cuda_kv_pages* p, const int32_t* slots, const int32_t* n_new,
+                                    int32_t n, void* work, size_t work_bytes, int32_t* status, void* stream) {
+    if (slots == nullptr || n_new == nullptr) return fail(SLLM_CUDA_ERR_ARG, "kv_reserve: NULL slots or lengths");
+    const int rc = check_call(p, "kv_reserve", n, work, work_bytes, slots, n_new, status);
+    if (rc != SLLM_CUDA_OK || n == 0) return rc;
+    const cudaStream_t st = (cudaStream_t)stream;
+    kv_reserve_kernel<<<1, kResThreads, 0, st>>>(pages_dev(*p), slots, n_new, n, work, status);
+    CK(cudaGetLastError(), "kv_reserve launch");
+    CK(launch_copies(*p, n, work, 0, st), "kv_reserve copies");
+    count_launches(2);
+    return SLLM_CUDA_OK;
+}
+
+extern "C" int sllm_cuda_kv_compact(const sllm_cuda_kv_pages* p, void* work, size_t work_bytes, int32_t* status,
+                                    void* stream) {
+    const int rc = check_call(p, "kv_compact", 0, work, work_bytes, nullptr, nullptr, status);
+    if (rc != SLLM_CUDA_OK) return rc;
+    const cudaStream_t st = (cudaStream_t)stream;
+    kv_compact_kernel<<<kClCtas, kClThreads, 0, st>>>(pages_dev(*p), work, status);
+    CK(cudaGetLastError(), "kv_compact launch");
+    CK(launch_copies(*p, p->n_pages / 2 + 1, work, 1, st), "kv_compact copies");
+    count_launches(2);
+    return SLLM_CUDA_OK;
+}
+
+extern "C" int sllm_cuda_kv_append(const sllm_cuda_kv_pages* p, int32_t layer, int32_t n_tokens, const int32_t* slot,
+                                   const int32_t* pos, int32_t n_head, const float* q, size_t q_stride,
+                                   const float* k, size_t k_stride, const float* v, size_t v_stride,
+                                   const float* rope_cos, const float* rope_sin, int32_t n_ctx, void* q_out,
+                                   void* k_out, void* v_out, int32_t* status, void* stream) {
+    int rc = check_pages(p, "kv_append");
+    if (rc != SLLM_CUDA_OK) return rc;
+    if (slot == nullptr || pos == nullptr || k == nullptr || v == nullptr || rope_cos == nullptr ||
+        rope_sin == nullptr || (q == nullptr) != (q_out == nullptr))
+        return fail(SLLM_CUDA_ERR_ARG, "kv_append: a NULL array (q and q_out go together)");
+    const size_t kvn = (size_t)p->n_head_kv * kServeDim, qn = (size_t)(n_head > 0 ? n_head : 0) * kServeDim;
+    if (layer < 0 || layer >= p->n_layer || n_tokens < 0 || n_tokens > (1 << 24) || n_ctx < 1 ||
+        (q != nullptr && (n_head < 1 || n_head > 1024 || n_head % p->n_head_kv != 0 || q_stride < qn)) ||
+        k_stride < kvn || v_stride < kvn || q_stride > (1u << 30) || k_stride > (1u << 30) || v_stride > (1u << 30))
+        return fail(SLLM_CUDA_ERR_ARG, "kv_append: layer %d, %d tokens, %d heads, strides %zu %zu %zu", layer, n_tokens,
+                    n_head, q_stride, k_stride, v_stride);
+    if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(q_out) || !aligned16(k_out) || !aligned16(v_out) ||
+        !aligned16(rope_cos) || !aligned16(rope_sin) || (q_stride | k_stride | v_stride) % 4 != 0)
+        return fail(SLLM_CUDA_ERR_ARG, "kv_append: arrays must be 16-byte aligned, strides a multiple of 4 floats");
+    const void* ptr[] = {p->k, p->v, p->refs, p->tables, p->lens, slot, pos, q, k, v, rope_cos, rope_sin, q_out, k_out,
+                         v_out, status};
+    const char* name[] = {"k", "v", "refs", "tables", "lens", "slot", "pos", "q", "k", "v", "rope_cos", "rope_sin",
+                          "q_out", "k_out", "v_out", "status"};
+    for (int i = 0; i < 16; ++i)
+        if (ptr[i] != nullptr && (rc = need_device(ptr[i], "kv_append", name[i])) != SLLM_CUDA_OK) return rc;
+    if (n_tokens == 0) return SLLM_CUDA_OK;
+    AppendParams a{};
+    a.slot = slot; a.pos = pos;
+    a.q = q; a.k = k; a.v = v;
+    a.qs = q_stride; a.ks = k_stride; a.vs = v_stride;
+    a.cs = rope_cos; a.sn = rope_sin;
+    a.qo = q_out; a.ko = k_out; a.vo = v_out;
+    const size_t layer_elts = (size_t)p->n_head_kv * p->page_size * kServeDim;
+    const size_t off = (size_t)layer * layer_elts * kv_elt_bytes(p->kv_type);
+    a.kp = static_cast<uint8_t*>(p->k) + off;
+    a.vp = static_cast<uint8_t*>(p->v) + off;
+    a.page_stride = (size_t)p->n_layer * layer_elts;
+    a.n_tokens = n_tokens; a.n_head = n_head; a.n_kv = p->n_head_kv; a.n_ctx = n_ctx;
+    a.status = status;
+    const long long units = (long long)n_tokens * ((q != nullptr ? n_head : 0) + 2 * p->n_head_kv);
+    if (units > 0x7fffffffLL * 8 - 8) return fail(SLLM_CUDA_ERR_TOO_LARGE, "kv_append: %d tokens", n_tokens);
+    const dim3 grid((unsigned)((units + 7) / 8));
+    if (p->kv_type == SLLM_CUDA_KV_F16)
+        kv_append_kernel<__half><<<grid, 256, 0, (cudaStream_t)stream>>>(pages_dev(*p), a);
+    else
+        kv_append_kernel<float><<<grid, 256, 0, (cudaStream_t)stream>>>(pages_dev(*p), a);
+    CK(cudaGetLastError(), "kv_append launch");
+    count_launches(1);
+    return SLLM_CUDA_OK;
+}

@@ -1,0 +1,87 @@
+// serve.cuh -- shared by the serving operators' files (kv_pages.cu,
+// attn_prompt.cu, attn_prefix.cu, spec_verify.cu): argument checks, the
+// device's view of a paged cache, launches.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <cuda_fp16.h>
+
+#include "backend.cuh"
+#include "common.cuh"
+
+namespace sllm {
+
+constexpr int kServeDim = 128;      // the head dimension of every model the library runs
+
+// OK when p is memory of the current device (a kernel given a host pointer or
+// another device's would fault); the message names the argument.
+int need_device(const void* p, const char* who, const char* arg);
+
+// the fields of a sllm_cuda_kv_pages, checked (no device call)
+int check_pages(const sllm_cuda_kv_pages* p, const char* who);
+
+struct PagesDev {
+    int32_t* refs;
+    int32_t* tables;
+    int32_t* lens;
+    int n_pages, n_slots, width, page;
+    int cap;                        // width * page: the most tokens a slot holds
+};
+
+inline PagesDev pages_dev(const sllm_cuda_kv_pages& p) {
+    return PagesDev{p.refs, p.tables, p.lens, p.n_pages, p.n_slots, p.table_width, p.page_size,
+                    p.table_width * p.page_size};
+}
+
+inline size_t kv_elt_bytes(int type) { return type == SLLM_CUDA_KV_F16 ? 2 : 4; }
+
+// sets *status (nullable) to an error; it is never cleared here
+__device__ __forceinline__ void raise(int32_t* status, int code) {
+    if (status != nullptr) *status = code;
+}
+
+// a kernel launch; pdl: the launch may start while the kernel before it on
+// the stream still runs, and orders itself with griddepcontrol.wait
+template <class... KArgs, class... Args>
+cudaError_t launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, bool pdl,
+                   Args... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = pdl ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...);
+}
+
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
+template <class T> __device__ __forceinline__ T from_f32(float x);
+template <> __device__ __forceinline__ float from_f32<float>(float x) { return x; }
+template <> __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
+
+// four consecutive elements as floats (8- or 16-byte aligned)
+__device__ __forceinline__ float4 ld4(const float* p) { return *reinterpret_cast<const float4*>(p); }
+__device__ __forceinline__ float4 ld4(const __half* p) {
+    const uint2 u = *reinterpret_cast<const uint2*>(p);
+    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&u.x));
+    const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
+    return make_float4(a.x, a.y, b.x, b.y);
+}
+__device__ __forceinline__ void st4(float* p, float4 v) { *reinterpret_cast<float4*>(p) = v; }
+__device__ __forceinline__ void st4(__half* p, float4 v) {
+    const __half2 a = __floats2half2_rn(v.x, v.y), b = __floats2half2_rn(v.z, v.w);
+    uint2 u;
+    u.x = *reinterpret_cast<const uint32_t*>(&a);
+    u.y = *reinterpret_cast<const uint32_t*>(&b);
+    *reinterpret_cast<uint2*>(p) = u;
+}
+
+}  // namespace sllm
