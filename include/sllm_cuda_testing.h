@@ -30,6 +30,8 @@ SLLM_CUDA_API int sllm_cuda_test_fallback_count(void);
  * the device; -1 without a device.
  */
 SLLM_CUDA_API int sllm_cuda_test_gemm_error(void);
+/* The same for the attention kernels on the tensor cores. */
+SLLM_CUDA_API int sllm_cuda_test_attn_error(void);
 /* The prefill GEMM's form: 0 by size (at most 16 tokens: weight rows as the
  * MMA's M operand, tokens as N = 16), 1 the 128-token tiles, 2 the skinny
  * form only. */

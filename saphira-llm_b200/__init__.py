@@ -412,6 +412,11 @@ def spec_verify(p, q, draft, n_draft, u_accept, u_draw, tokens, count, status=No
                                        _ints(count, n, w, "count"), _ints(status, 1, w, "status"), _stream(stream)), w)
 
 
+def attn_error():
+    """The tensor-core attention kernels' device error word, likewise."""
+    return lib().sllm_cuda_test_attn_error()
+
+
 def set_force_fallback(on):
     lib().sllm_cuda_test_set_force_fallback(1 if on else 0)
 

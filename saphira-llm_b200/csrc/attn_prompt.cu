@@ -3,6 +3,11 @@
 // Sequence s holds tokens cu[s] .. cu[s + 1] - 1 of the packed arrays; token i
 // of a sequence sees its tokens 0 .. i.
 
+//
+// f16: attn_prompt_mma_kernel, on the tensor cores. f32: the 32-bit kernel
+// of attn_simt.cuh.
+
+#include "attn_mma.cuh"
 #include "attn_simt.cuh"
 
 namespace sllm {
@@ -90,10 +95,421 @@ cudaError_t launch_simt(const PromptParams& p, cudaStream_t st) {
     return launch(kern, dim3((unsigned)tiles, (unsigned)p.n_head), dim3(kSimtThreads), kSimtSmem, st, false, p);
 }
 
+// ---------------------------------------------------------------------------
+// The f16 kernel. One CTA takes 256 query rows of one head as two tiles of
+// 128 rows that share every key tile. Scores, weights and outputs stay in
+// tensor memory (512 columns: S0 S1 O0 O1, 128 each; a tile's f16 weights
+// overwrite the first 64 columns of its scores).
+//
+//   warps 0-3, 4-7   softmax of tile 0, 1: one thread per row. S from tensor
+//                    memory, mask, running maximum, weights back.
+//   warps 8-11       corrections: scale O where a row's maximum has moved on
+//                    (rarely: kAtLag), and at the end O / l to global memory.
+//   warp 12, 1 lane  tcgen05.mma: S_t = Q_t K^T (both from shared memory) and
+//                    O_t += P_t V (P from tensor memory, V MN-major as it
+//                    lies). The order P0 V, S0', P1 V, S1' lets one tile's
+//                    softmax run under the other tile's products.
+//   warp 13, 1 lane  TMA: Q once, then K and V tiles through a ring of five.
+//
+// Causal: only the last key tile of a row tile is masked. A value row past the
+// end of the sequence is zeroed in shared memory before it meets its zero
+// weight. A value inside the sequence that is no number would leak the same
+// way into rows of the tile that do not see it: the correction warps look for
+// such values in the last key tile, and recompute the rows one by one if
+// there are any.
+//
+// Registers: 512 threads x 128 at launch; 2 x 184 (softmax) + 80
+// (corrections) + 64 (the issuing warps) = 512 = 4 x 128 after the split.
+// ---------------------------------------------------------------------------
+constexpr int kPmRows = 2 * kAtRows;
+constexpr int kPmStages = 5;
+constexpr int kPmThreads = 512;
+constexpr int kPmSmem = (2 + kPmStages) * kAtTile + 1024;
+
+__device__ int g_prompt_error;      // why a bounded wait gave up (0: none did)
+
+// tile x of the call's tiles of R rows in descending order of their position
+// in their sequence (the later, the more keys they see): the longest work
+// first. F(t) = tiles at positions >= t; a binary search for the position,
+// then the sequence among those that long. One warp.
+template <int R>
+__device__ __forceinline__ bool find_long_first(const PromptParams& p, int x, int* start, int* len, int* tile) {
+    const int lane = threadIdx.x & 31;
+    auto seq = [&](int s, int* a) {
+        *a = min(max(p.cu[s], 0), p.n_tokens);
+        return min(max(p.cu[s + 1], *a), p.n_tokens) - *a;
+    };
+    auto at_least = [&](int t) {
+        int f = 0, a;
+        for (int s = lane; s < p.n_seq; s += 32) f += max((seq(s, &a) + R - 1) / R - t, 0);
+        return __reduce_add_sync(0xffffffffu, f);
+    };
+    int lo = 0, hi = (p.n_tokens + R - 1) / R;          // F(lo) > x >= F(hi), if x is a tile at all
+    if (at_least(0) <= x) return false;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (at_least(mid) > x) lo = mid;
+        else hi = mid;
+    }
+    int r = x - at_least(lo + 1);                       // the r-th sequence with a tile at lo
+    for (int s0 = 0; s0 < p.n_seq; s0 += 32) {
+        int a = 0, n = 0;
+        if (s0 + lane < p.n_seq) n = seq(s0 + lane, &a);
+        const unsigned has = __ballot_sync(0xffffffffu, (n + R - 1) / R > lo);
+        const int c = __popc(has);
+        if (r < c) {
+            const int l = __fns(has, 0, r + 1);
+            *start = __shfl_sync(0xffffffffu, a, l);
+            *len = __shfl_sync(0xffffffffu, n, l);
+            *tile = lo;
+            return true;
+        }
+        r -= c;
+    }
+    return false;
+}
+
+// rows [first, first + 128) of a sequence, one warp per row at a time, in
+// 32-bit arithmetic: the way out for values that are no numbers
+template <class O>
+__device__ __forceinline__ void slow_rows(const PromptParams& p, int h, int start, int len, int first, int warp) {
+    const int lane = threadIdx.x & 31, kvh = h / p.group;
+    const __half* K = static_cast<const __half*>(p.k) + (size_t)kvh * kServeDim + 4 * lane;
+    const __half* V = static_cast<const __half*>(p.v) + (size_t)kvh * kServeDim + 4 * lane;
+    for (int r = warp; r < kAtRows; r += 4) {
+        const int i = first + r;
+        if (i >= len) return;
+        const float4 q = ld4(static_cast<const __half*>(p.q) + (size_t)(start + i) * p.qs + (size_t)h * kServeDim + 4 * lane);
+        float m = -INFINITY, l = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int j = 0; j <= i; ++j) {
+            const float4 k = ld4(K + (size_t)(start + j) * p.ks), v = ld4(V + (size_t)(start + j) * p.vs);
+            float s = fmaf(q.x, k.x, fmaf(q.y, k.y, fmaf(q.z, k.z, q.w * k.w)));
+            #pragma unroll
+            for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
+            s *= kServeScale;
+            const float mn = fmaxf(m, s), f = mn == -INFINITY ? 1.f : expf(m - mn), e = expf(s - mn);
+            m = mn;
+            l = fmaf(l, f, e);
+            o.x = fmaf(e, v.x, o.x * f);
+            o.y = fmaf(e, v.y, o.y * f);
+            o.z = fmaf(e, v.z, o.z * f);
+            o.w = fmaf(e, v.w, o.w * f);
+        }
+        const float inv = 1.f / l;
+        st4(static_cast<O*>(p.out) + (size_t)(start + i) * p.os + (size_t)h * kServeDim + 4 * lane,
+            make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+    }
+}
+
+template <class O>
+__global__ void __launch_bounds__(kPmThreads, 1)
+attn_prompt_mma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                       const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ PromptParams p) {
+    extern __shared__ uint8_t pm_raw[];
+    __shared__ uint64_t bar_q[2], bar_full[kPmStages], bar_free[kPmStages], bar_s[2], bar_p[2], bar_c[2], bar_o[2],
+        bar_ready[2], bar_l[2], bar_odd[2], bar_done;
+    __shared__ float s_scale[2][kAtRows];
+    __shared__ uint32_t tmem_slot;
+    __shared__ int abort_flag, s_tile[3], s_odd[2];
+    uint8_t* const sm = pm_raw + ((1024u - (smem_u32(pm_raw) & 1023u)) & 1023u);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int h = blockIdx.x % p.n_head;
+    if (warp == 13) {
+        int a = 0, n = 0, t = -1;
+        if (!find_long_first<kPmRows>(p, blockIdx.x / p.n_head, &a, &n, &t)) t = -1;
+        if (lane == 0) {
+            s_tile[0] = a;
+            s_tile[1] = n;
+            s_tile[2] = t;
+        }
+    }
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&bar_q[i], 1);
+            mbar_init(&bar_s[i], 1);
+            mbar_init(&bar_p[i], 4);
+            mbar_init(&bar_c[i], 4);
+            mbar_init(&bar_o[i], 1);
+            mbar_init(&bar_ready[i], 4);
+            mbar_init(&bar_l[i], 4);
+            mbar_init(&bar_odd[i], 4);
+            s_odd[i] = 0;
+        }
+        for (int i = 0; i < kPmStages; ++i) {
+            mbar_init(&bar_full[i], 1);
+            mbar_init(&bar_free[i], 1);
+        }
+        mbar_init(&bar_done, 1);
+        abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+    const int start = s_tile[0], len = s_tile[1], tile = s_tile[2];
+    if (tile < 0) return;               // the whole CTA: the grid is an upper bound
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
+                     "r"(512u)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    volatile int* const ab = &abort_flag;
+    int* const err = &g_prompt_error;
+    const int r0 = tile * kPmRows;
+    // key tiles of each row tile: up to its diagonal, or the sequence's end
+    const int last_tile = (len - 1) / kAtKeys;
+    const int nt0 = min(2 * tile, last_tile) + 1;
+    const int nt1 = r0 + kAtRows < len ? min(2 * tile + 1, last_tile) + 1 : 0;
+    const int nt = max(nt0, nt1);
+
+    if (warp < 8) {
+        // ---------------- softmax ----------------
+        reg_alloc<184>();
+        const int t = warp >> 2, n = t == 0 ? nt0 : nt1;
+        const int row = 32 * (warp & 3) + lane;
+        const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+        const uint32_t s_tm = tmem + lanes + 128 * t;
+        const int seen = min(r0 + kAtRows * t + row + 1, len);
+        RowState st{-INFINITY, 0.f};
+        int j = 0;
+        for (; j < n; ++j) {
+            if (!at_wait_warp(&bar_s[t], j & 1, ab, err)) break;
+            tc_fence_after();
+            float s[128];
+            load_scores(s_tm, s);
+            const int lim = seen - j * kAtKeys;
+            if (j == n - 1) {
+                #pragma unroll
+                for (int c = 0; c < 128; ++c) s[c] = c < lim ? s[c] : -INFINITY;
+            }
+            const float f = row_step(st, row_max(s));
+            s_scale[t][row] = f;
+            __syncwarp();
+            if (j > 0 && lane == 0) mbar_arrive(&bar_c[t]);
+            row_weights(s, st.m, st.l, s_tm);
+            if (j == n - 1 && (j + 1) * kAtKeys > len) {
+                // the tile's rows behind the sequence: their values become 0
+                const int slot = (2 * j + 1) % kPmStages;
+                if (!at_wait_warp(&bar_full[slot], ((2 * j + 1) / kPmStages) & 1, ab, err)) break;
+                if (j * kAtKeys + row >= len) {
+                    uint8_t* v = sm + (2 + slot) * kAtTile + row * 128;
+                    #pragma unroll
+                    for (int c = 0; c < 8; ++c) {
+                        *reinterpret_cast<uint4*>(v + 16 * c) = make_uint4(0, 0, 0, 0);
+                        *reinterpret_cast<uint4*>(v + kAtHalf + 16 * c) = make_uint4(0, 0, 0, 0);
+                    }
+                }
+                fence_proxy_async_smem();
+            }
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar_p[t]);
+        }
+        if (j == n && n > 0) {
+            // not through s_scale, whose last factor may not have been read
+            // yet: the query tile's place is free after its last product
+            reinterpret_cast<float*>(sm + t * kAtTile)[row] = st.l;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar_l[t]);
+        }
+    } else if (warp < 12) {
+        // ---------------- corrections and epilogue ----------------
+        reg_dealloc<80>();
+        const int row = 32 * (warp & 3) + lane;
+        const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+        bool ok = true;
+        for (int j = 1; j < nt && ok; ++j) {
+            #pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                if (j >= (t == 0 ? nt0 : nt1)) continue;
+                if (!(ok = at_wait_warp(&bar_c[t], (j - 1) & 1, ab, err))) break;
+                const float f = s_scale[t][row];
+                if (__any_sync(0xffffffffu, f != 1.f)) {
+                    if (!(ok = at_wait_warp(&bar_o[t], (j - 1) & 1, ab, err))) break;
+                    tc_fence_after();
+                    #pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t r[32];
+                        const uint32_t at = tmem + lanes + 256 + 128 * t + 32 * c;
+                        tmem_ld32(at, r);
+                        tmem_ld_wait();
+                        #pragma unroll
+                        for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * f);
+                        tmem_st32(at, r);
+                    }
+                    tmem_st_wait();
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bar_ready[t]);
+            }
+        }
+        #pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const int n = t == 0 ? nt0 : nt1;
+            if (n == 0 || !ok) continue;
+            // values of the masked tile that are no numbers, in this thread's row
+            const int slot = (2 * n - 1) % kPmStages;
+            if (!(ok = at_wait_warp(&bar_full[slot], ((2 * n - 1) / kPmStages) & 1, ab, err))) continue;
+            bool odd = false;
+            if ((n - 1) * kAtKeys + row < len) {
+                const uint8_t* v = sm + (2 + slot) * kAtTile + row * 128;
+                #pragma unroll
+                for (int c = 0; c < 16; ++c) {
+                    const uint4 u = *reinterpret_cast<const uint4*>(v + (c >> 3) * kAtHalf + 16 * ((c ^ row) & 7));
+                    odd = odd || odd_half2(u.x) || odd_half2(u.y) || odd_half2(u.z) || odd_half2(u.w);
+                }
+            }
+            if (odd) s_odd[t] = 1;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar_odd[t]);
+            if (!(ok = at_wait_warp(&bar_odd[t], 0, ab, err))) continue;
+            if (!(ok = at_wait_warp(&bar_l[t], 0, ab, err))) continue;
+            const float l = reinterpret_cast<const float*>(sm + t * kAtTile)[row];
+            if (!(ok = at_wait_warp(&bar_o[t], (n - 1) & 1, ab, err))) continue;
+            tc_fence_after();
+            if (s_odd[t] != 0) {
+                slow_rows<O>(p, h, start, len, r0 + kAtRows * t, warp & 3);
+            } else {
+                const int i = r0 + kAtRows * t + row;
+                store_row(tmem + lanes + 256 + 128 * t, 1.f / l, i < len,
+                          static_cast<O*>(p.out) + (size_t)(start + i) * p.os + (size_t)h * kServeDim);
+            }
+        }
+    } else {
+        reg_dealloc<64>();
+        if (warp == 12 && lane == 0) {
+            // ---------------- products ----------------
+            const uint32_t idesc_s = umma_idesc_f16(128, 128, false), idesc_o = umma_idesc_f16(128, 128, true);
+            auto tile_at = [&](int i) { return smem_u32(sm + (size_t)(2 + i % kPmStages) * kAtTile); };
+            auto full = [&](int i) { return at_wait(&bar_full[i % kPmStages], (i / kPmStages) & 1, ab, err); };
+            auto scores = [&](int t, int i) {           // S_t = Q_t (ring tile i)^T
+                const uint32_t q = smem_u32(sm + t * kAtTile), k = tile_at(i);
+                #pragma unroll
+                for (int x = 0; x < 8; ++x) {
+                    const uint32_t off = (x >> 2) * kAtHalf + (x & 3) * 32;
+                    umma_f16_ss(tmem + 128 * t, umma_desc_sw128(q + off), umma_desc_sw128(k + off), idesc_s, x > 0);
+                }
+                umma_commit(&bar_s[t]);
+            };
+            auto outputs = [&](int t, int i, bool add) { // O_t (+)= P_t (ring tile i)
+                const uint32_t v = tile_at(i);
+                #pragma unroll
+                for (int x = 0; x < 8; ++x)
+                    umma_f16_ts(tmem + 256 + 128 * t, tmem + 128 * t + 8 * x, umma_desc_mn_sw128(v + 2048 * x, kAtHalf),
+                                idesc_o, add || x > 0);
+                umma_commit(&bar_o[t]);
+            };
+            bool ok = at_wait(&bar_q[0], 0, ab, err) && full(0);
+            if (ok) {
+                tc_fence_after();
+                scores(0, 0);
+                if (nt1 > 0) {
+                    ok = at_wait(&bar_q[1], 0, ab, err);
+                    if (ok) scores(1, 0);
+                }
+                umma_commit(&bar_free[0]);
+            }
+            for (int j = 0; j < nt && ok; ++j) {
+                const int vi = 2 * j + 1, ki = 2 * j + 2;
+                #pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const int n = t == 0 ? nt0 : nt1;
+                    if (!ok || j >= n) continue;
+                    ok = at_wait(&bar_p[t], j & 1, ab, err) && (j == 0 || at_wait(&bar_ready[t], (j - 1) & 1, ab, err)) &&
+                         full(vi);
+                    if (!ok) continue;
+                    tc_fence_after();
+                    outputs(t, vi, j > 0);
+                    if (j + 1 < n) {
+                        if (!(ok = full(ki))) continue;
+                        scores(t, ki);
+                    }
+                }
+                umma_commit(&bar_free[vi % kPmStages]);
+                if (j + 1 < nt) umma_commit(&bar_free[ki % kPmStages]);
+            }
+            umma_commit(&bar_done);
+            at_drain(&bar_done, 0);
+        } else if (warp == 13 && lane == 0) {
+            // ---------------- loads ----------------
+            const int kvh = h / p.group;
+            auto load = [&](uint8_t* dst, const CUtensorMap* tm, int head, int token, uint64_t* bar) {
+                mbar_expect_tx(bar, kAtTile);
+                tma_load_3d(dst, tm, 0, head, token, bar);
+                tma_load_3d(dst + kAtHalf, tm, 64, head, token, bar);
+            };
+            load(sm, &tm_q, h, start + r0, &bar_q[0]);
+            int i = 0;
+            const int total = 2 * nt;
+            for (; i < total; ++i) {
+                const int s = i % kPmStages, use = i / kPmStages;
+                if (use > 0 && !at_wait(&bar_free[s], (use - 1) & 1, ab, err)) break;
+                load(sm + (size_t)(2 + s) * kAtTile, (i & 1) == 0 ? &tm_k : &tm_v, kvh, start + (i >> 1) * kAtKeys,
+                     &bar_full[s]);
+                if (i == 0 && nt1 > 0) load(sm + kAtTile, &tm_q, h, start + r0 + kAtRows, &bar_q[1]);
+            }
+            // no copy may be in flight when the CTA ends
+            at_drain(&bar_q[0], 0);
+            if (nt1 > 0) at_drain(&bar_q[1], 0);
+            for (int x = max(0, i - kPmStages); x < i; ++x) at_drain(&bar_full[x % kPmStages], (x / kPmStages) & 1);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 12) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+}
+
+// [tokens][heads][128] f16 as (64 dims of a half, head, token) boxes of
+// 128 tokens of one head
+bool encode_heads(CUtensorMap* tm, const void* base, int heads, int tokens, size_t stride) {
+    PFN_cuTensorMapEncodeTiled_v12000 enc = tensor_map_encoder();
+    if (enc == nullptr) return false;
+    const cuuint64_t dims[3] = {(cuuint64_t)kServeDim, (cuuint64_t)heads, (cuuint64_t)tokens};
+    const cuuint64_t strides[2] = {(cuuint64_t)kServeDim * 2, (cuuint64_t)stride * 2};
+    const cuuint32_t box[3] = {64, 1, kAtRows};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    return enc(tm, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <class O>
+cudaError_t launch_mma(const PromptParams& p, cudaStream_t st) {
+    CUtensorMap tq, tk, tv;
+    const int n_kv = p.n_head / p.group;
+    if (!encode_heads(&tq, p.q, p.n_head, p.n_tokens, p.qs) || !encode_heads(&tk, p.k, n_kv, p.n_tokens, p.ks) ||
+        !encode_heads(&tv, p.v, n_kv, p.n_tokens, p.vs))
+        return cudaErrorInvalidValue;
+    auto* kern = attn_prompt_mma_kernel<O>;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kPmSmem);
+    if (e != cudaSuccess) return e;
+    const long long tiles = p.n_tokens / kPmRows + (long long)p.n_seq;
+    return launch(kern, dim3((unsigned)(tiles * p.n_head)), dim3(kPmThreads), kPmSmem, st, false, tq, tk, tv, p);
+}
+
 }  // namespace
 }  // namespace sllm
 
 using namespace sllm;
+
+extern "C" int sllm_cuda_test_attn_error(void) {
+    int v = 0;
+    if (cudaDeviceSynchronize() != cudaSuccess ||
+        cudaMemcpyFromSymbol(&v, g_prompt_error, sizeof v) != cudaSuccess)
+        return -1;
+    const int zero = 0;
+    cudaMemcpyToSymbol(g_prompt_error, &zero, sizeof zero);
+    return v;
+}
 
 extern "C" int sllm_cuda_attn_prompt(const void* q, size_t q_stride, const void* k, size_t k_stride, const void* v,
                                      size_t v_stride, int32_t type, const int32_t* cu_seqlens, int32_t n_seq,
@@ -130,8 +546,8 @@ extern "C" int sllm_cuda_attn_prompt(const void* q, size_t q_stride, const void*
     p.n_seq = n_seq; p.n_tokens = n_tokens; p.n_head = n_head; p.group = n_head / n_head_kv;
     const cudaStream_t st = (cudaStream_t)stream;
     const cudaError_t e = type == SLLM_CUDA_KV_F32 ? launch_simt<float, float>(p, st)
-                          : out_type == SLLM_CUDA_KV_F32 ? launch_simt<__half, float>(p, st)
-                                                         : launch_simt<__half, __half>(p, st);
+                          : out_type == SLLM_CUDA_KV_F32 ? launch_mma<float>(p, st)
+                                                         : launch_mma<__half>(p, st);
     CK(e, "attn_prompt launch");
     count_launches(1);
     return SLLM_CUDA_OK;

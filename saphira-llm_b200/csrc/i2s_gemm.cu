@@ -57,9 +57,6 @@ constexpr int kBK = 128;          // elements (= activation bytes) per k-step
 constexpr int kPK = kBK / 4;      // packed weight bytes per row per k-step
 constexpr int kGmUnpackWarps = 8;
 constexpr int kGmThreads = 64 + 32 * kGmUnpackWarps;   // TMA, MMA, 8 unpack / epilogue warps
-constexpr uint64_t kGmWaitNs = 2000000000ull;
-
-enum GemmError { GM_OK = 0, GM_TIMEOUT = 1 };
 
 template <int BN, bool PAIR, int MT>
 struct GemmCfg {
@@ -94,47 +91,6 @@ struct GemmKParams {
     int* error;
     int tma_out;           // 1: outputs leave through the tensor maps tm_y / tm_d
 };
-
-// bounded wait: false when the phase did not complete in time, or when the
-// CTA is aborting. The first check is inline: the single MMA-issuing thread
-// waits once per k-step, and an out-of-line call there cost ~0.1 us each.
-__device__ __noinline__ bool gm_wait_slow(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* error,
-                                         bool sleep);
-__device__ __forceinline__ bool gm_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* error,
-                                        bool sleep = false) {
-    if (mbar_try_wait(bar, parity)) return true;
-    return gm_wait_slow(bar, parity, abort_flag, error, sleep);
-}
-__device__ __noinline__ bool gm_wait_slow(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* error,
-                                         bool sleep) {
-    const uint64_t t0 = gtimer();
-    while (!mbar_try_wait(bar, parity)) {
-        if (*abort_flag) return false;
-        if (gtimer() - t0 > kGmWaitNs) {
-            *abort_flag = 1;
-            atomicExch(error, GM_TIMEOUT);
-            return false;
-        }
-        // waits off the k-loop's critical path (the epilogue's, the
-        // producer's) poll less often
-        if (sleep) __nanosleep(32);
-    }
-    return true;
-}
-
-// a whole warp's wait, the same answer in every lane
-__device__ __forceinline__ bool gm_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* error,
-                                             bool sleep = false) {
-    return __all_sync(0xffffffffu, gm_wait(bar, parity, abort_flag, error, sleep));
-}
-
-// drain: wait for a phase that must complete (work already in flight);
-// bounded, never looks at the abort flag
-__device__ __noinline__ void gm_drain(uint64_t* bar, uint32_t parity) {
-    const uint64_t t0 = gtimer();
-    while (!mbar_try_wait(bar, parity))
-        if (gtimer() - t0 > kGmWaitNs) return;
-}
 
 // a 2-D TMA tile store from shared memory, tracked by the bulk-group counter
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* tm, const void* src, int x, int y) {
@@ -548,7 +504,6 @@ __device__ __forceinline__ void tmem_st4(uint32_t taddr, uint32_t a, uint32_t b,
                  : "memory");
 }
 
-__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 template <bool PAIR, int SK>
 __global__ void __launch_bounds__(kSkThreads, 2)

@@ -171,6 +171,13 @@ def test_prompt_wrong_offsets_stay_inside(cuda):
         check_prompt(q, k, v, out, [100], dt == "f16")
 
 
+def test_no_bounded_wait_gave_up(cuda):
+    import torch
+    q, k, v = (_rand(s, 3000, 2, 128, dt=torch.float16) for s in (1, 2, 3))
+    cuda.attn_prompt(q, k, v, torch.empty_like(q), _i32([0, 2000, 3000]))
+    assert cuda.attn_error() == 0
+
+
 def test_host_memory_is_refused(cuda):
     import torch
     q = torch.zeros(4, 2, 128)
