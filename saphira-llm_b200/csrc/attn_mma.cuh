@@ -31,16 +31,16 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
     return r;
 }
 
-// two f32 at a time (sm_100's packed pipe): a * b + c, a + b
-__device__ __forceinline__ void fma2(float& x, float& y, float a0, float a1, float b, float c) {
+// two f32 at a time (sm_100's packed pipe): a * b + c, x += a
+__device__ __forceinline__ void fma2v(float& x, float& y, float a0, float a1, float b0, float b1, float c0, float c1) {
     asm("{\n\t.reg .b64 a, b, c, d;\n\t"
         "mov.b64 a, {%2, %3};\n\t"
-        "mov.b64 b, {%4, %4};\n\t"
-        "mov.b64 c, {%5, %5};\n\t"
+        "mov.b64 b, {%4, %5};\n\t"
+        "mov.b64 c, {%6, %7};\n\t"
         "fma.rn.f32x2 d, a, b, c;\n\t"
         "mov.b64 {%0, %1}, d;\n\t}"
         : "=f"(x), "=f"(y)
-        : "f"(a0), "f"(a1), "f"(b), "f"(c));
+        : "f"(a0), "f"(a1), "f"(b0), "f"(b1), "f"(c0), "f"(c1));
 }
 __device__ __forceinline__ void add2(float& x, float& y, float a0, float a1) {
     asm("{\n\t.reg .b64 a, d;\n\t"
@@ -83,65 +83,52 @@ __device__ __forceinline__ void at_drain(uint64_t* bar, uint32_t parity) {
         if (gtimer() - t0 > kGmWaitNs) return;
 }
 
-// One row's step over a tile of scores s (raw dots). lim: keys of the tile
-// that the row sees (>= 128: all). Updates m (raw units), l; returns the
-// factor that the row's outputs have to be scaled by (1: none).
-struct RowState {
-    float m, l;
-};
+// (the maxima keep a NaN, so that a row which sees one becomes NaN)
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 __device__ __forceinline__ float row_max(const float (&s)[128]) {
-    float a = fmaxf(s[0], s[1]), b = fmaxf(s[2], s[3]), c = fmaxf(s[4], s[5]), d = fmaxf(s[6], s[7]);
+    float a = max3(s[0], s[1], s[2]), b = max3(s[3], s[4], s[5]), c = max3(s[6], s[7], s[8]), d = s[9];
     #pragma unroll
-    for (int i = 8; i < 128; i += 8) {
-        a = fmaxf(a, fmaxf(s[i], s[i + 1]));
-        b = fmaxf(b, fmaxf(s[i + 2], s[i + 3]));
-        c = fmaxf(c, fmaxf(s[i + 4], s[i + 5]));
-        d = fmaxf(d, fmaxf(s[i + 6], s[i + 7]));
+    for (int i = 10; i < 122; i += 8) {
+        a = max3(a, s[i], s[i + 1]);
+        b = max3(b, s[i + 2], s[i + 3]);
+        c = max3(c, s[i + 4], s[i + 5]);
+        d = max3(d, s[i + 6], s[i + 7]);
     }
-    return fmaxf(fmaxf(a, b), fmaxf(c, d));
+    a = max3(a, s[122], s[123]);
+    b = max3(b, s[124], s[125]);
+    c = max3(c, s[126], s[127]);
+    return max3(a, b, max3(c, d, d));
 }
-__device__ __forceinline__ float row_step(RowState& st, float mx) {
-    float f = 1.f;
-    const float m = fmaxf(st.m, mx);
-    // (the first tile has st.m = -inf; a row that has seen nothing keeps it)
-    if (m > st.m && !((m - st.m) * kAtScale2 <= kAtLag)) {
-        f = ex2((st.m - m) * kAtScale2);
-        st.m = m;
-        st.l *= f;
-    }
-    return f;
-}
-
 // a non-finite f16 in two packed ones
 __device__ __forceinline__ bool odd_half2(uint32_t u) {
     return (u & 0x7c00u) == 0x7c00u || (u & 0x7c000000u) == 0x7c000000u;
 }
 
-// 128 weights of a row, from its scores, into tensor memory as f16; their
-// sum (before the rounding) is added to l
-__device__ __forceinline__ void row_weights(float (&s)[128], float m, float& l, uint32_t p_tmem) {
-    const float mc = m == -INFINITY ? 0.f : -m * kAtScale2;
-    float a0 = 0.f, a1 = 0.f, b0 = 0.f, b1 = 0.f;
+// the weights of 64 of a row's scores: two f16 per word, and their sums
+// before the rounding. All exponentials go through the special-function pipe:
+// moving 1/8, 1/4 or 3/8 of them to a degree-4 polynomial on the multiply-add
+// pipe measured slower (one prompt of 16384 tokens, 16 heads: 871 us without,
+// 889, 898, 919 us).
+__device__ __forceinline__ void half_weights(const float* s, float mc, uint32_t (&u)[32], float (&sum)[4]) {
     #pragma unroll
-    for (int h = 0; h < 4; ++h) {
-        uint32_t u[16];
-        #pragma unroll
-        for (int i = 0; i < 16; i += 2) {
-            float* x = s + 32 * h + 2 * i;
-            fma2(x[0], x[1], x[0], x[1], kAtScale2, mc);
-            fma2(x[2], x[3], x[2], x[3], kAtScale2, mc);
-            x[0] = ex2(x[0]);
-            x[1] = ex2(x[1]);
-            x[2] = ex2(x[2]);
-            x[3] = ex2(x[3]);
-            add2(a0, a1, x[0], x[1]);
-            add2(b0, b1, x[2], x[3]);
-            u[i] = pack_half2(x[0], x[1]);
-            u[i + 1] = pack_half2(x[2], x[3]);
-        }
-        tmem_st16(p_tmem + 16 * h, u);
+    for (int i = 0; i < 32; ++i) {
+        float x0, x1;
+        fma2v(x0, x1, s[2 * i], s[2 * i + 1], kAtScale2, kAtScale2, mc, mc);
+        x0 = ex2(x0);
+        x1 = ex2(x1);
+        if (i & 1) add2(sum[0], sum[1], x0, x1);
+        else add2(sum[2], sum[3], x0, x1);
+        u[i] = pack_half2(x0, x1);
     }
-    l += (a0 + a1) + (b0 + b1);
+}
+// what the scaled scores are offset by: -m in base 2. A row that has only
+// seen -inf has weights 0; one that has seen +inf is no number.
+__device__ __forceinline__ float weight_offset(float m) {
+    return m == -INFINITY ? 0.f : m == INFINITY ? NAN : -m * kAtScale2;
 }
 
 // a row's 128 scores from tensor memory

@@ -7,6 +7,7 @@
 // f16: attn_prompt_mma_kernel, on the tensor cores. f32: the 32-bit kernel
 // of attn_simt.cuh.
 
+#include "../../include/sllm_cuda_testing.h"
 #include "attn_mma.cuh"
 #include "attn_simt.cuh"
 
@@ -96,30 +97,39 @@ cudaError_t launch_simt(const PromptParams& p, cudaStream_t st) {
 }
 
 // ---------------------------------------------------------------------------
-// The f16 kernel. One CTA takes 256 query rows of one head as two tiles of
-// 128 rows that share every key tile. Scores, weights and outputs stay in
-// tensor memory (512 columns: S0 S1 O0 O1, 128 each; a tile's f16 weights
-// overwrite the first 64 columns of its scores).
+// The f16 kernel. One CTA per SM walks items of 256 query rows of one head:
+// two tiles of 128 rows that share every key tile. Scores, weights and outputs
+// stay in tensor memory (512 columns: S0 S1 O0 O1, 128 each; a tile's f16
+// weights overwrite the first 64 columns of its scores).
 //
 //   warps 0-3, 4-7   softmax of tile 0, 1: one thread per row. S from tensor
-//                    memory, mask, running maximum, weights back.
-//   warps 8-11       corrections: scale O where a row's maximum has moved on
-//                    (rarely: kAtLag), and at the end O / l to global memory.
+//                    memory, mask, weights back. The weights stand against the
+//                    running maximum of the tiles before; the tile's own
+//                    maximum is found meanwhile and only checked: where it is
+//                    more than kAtLag doublings higher (rare after the first
+//                    tiles) the warp rescales its rows of O and starts over.
+//   warps 8-11       O / l to global memory, under the next item's products.
 //   warp 12, 1 lane  tcgen05.mma: S_t = Q_t K^T (both from shared memory) and
 //                    O_t += P_t V (P from tensor memory, V MN-major as it
-//                    lies). The order P0 V, S0', P1 V, S1' lets one tile's
+//                    lies), the first 64 keys as soon as their weights are
+//                    there. The order P0 V, S0', P1 V, S1' lets one tile's
 //                    softmax run under the other tile's products.
-//   warp 13, 1 lane  TMA: Q once, then K and V tiles through a ring of five.
+//   warp 13, 1 lane  TMA: Q per item, K and V tiles through a ring of five.
+//   warp 14          the items, longest first, two ahead.
+//
+// What bounds it: per key tile and row tile 1024 clocks of products, and the
+// chain S -> softmax -> P V -> S', whose softmax is 16384 exponentials at 16
+// a clock, shared by the two tiles.
 //
 // Causal: only the last key tile of a row tile is masked. A value row past the
 // end of the sequence is zeroed in shared memory before it meets its zero
 // weight. A value inside the sequence that is no number would leak the same
-// way into rows of the tile that do not see it: the correction warps look for
-// such values in the last key tile, and recompute the rows one by one if
-// there are any.
+// way into rows of the tile that do not see it: the softmax warps look for
+// such values in that last key tile, and if there are any warps 8-11 recompute
+// the tile's rows one by one.
 //
-// Registers: 512 threads x 128 at launch; 2 x 184 (softmax) + 80
-// (corrections) + 64 (the issuing warps) = 512 = 4 x 128 after the split.
+// Registers: 512 threads x 128 at launch; 2 x 192 (softmax) + 64 (outputs) +
+// 64 (the issuing warps) = 512 = 4 x 128 after the split.
 // ---------------------------------------------------------------------------
 constexpr int kPmRows = 2 * kAtRows;
 constexpr int kPmStages = 5;
@@ -202,39 +212,39 @@ __device__ __forceinline__ void slow_rows(const PromptParams& p, int h, int star
     }
 }
 
+struct PromptItem {
+    int start, len, tile, head;         // tile < 0: no more items
+};
+
 template <class O>
 __global__ void __launch_bounds__(kPmThreads, 1)
 attn_prompt_mma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                        const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ PromptParams p) {
     extern __shared__ uint8_t pm_raw[];
-    __shared__ uint64_t bar_q[2], bar_full[kPmStages], bar_free[kPmStages], bar_s[2], bar_p[2], bar_c[2], bar_o[2],
-        bar_ready[2], bar_l[2], bar_odd[2], bar_done;
-    __shared__ float s_scale[2][kAtRows];
+    // [2]: per row tile. q, qf: Q there / free; s: scores there; h, p: the
+    // first half of the weights there, all; l: sums there; o: outputs
+    // complete; of: outputs read
+    __shared__ uint64_t bar_full[kPmStages], bar_free[kPmStages], bar_q[2], bar_qf[2], bar_s[2], bar_h[2], bar_p[2],
+        bar_l[2], bar_o[2], bar_of[2], bar_item[2], bar_itemf[2], bar_done;
+    __shared__ float s_sum[2][kAtRows];
+    __shared__ PromptItem s_item[2];
+    __shared__ int s_odd[2][4];
     __shared__ uint32_t tmem_slot;
-    __shared__ int abort_flag, s_tile[3], s_odd[2];
+    __shared__ int abort_flag;
     uint8_t* const sm = pm_raw + ((1024u - (smem_u32(pm_raw) & 1023u)) & 1023u);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int h = blockIdx.x % p.n_head;
-    if (warp == 13) {
-        int a = 0, n = 0, t = -1;
-        if (!find_long_first<kPmRows>(p, blockIdx.x / p.n_head, &a, &n, &t)) t = -1;
-        if (lane == 0) {
-            s_tile[0] = a;
-            s_tile[1] = n;
-            s_tile[2] = t;
-        }
-    }
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(&bar_q[i], 1);
+            mbar_init(&bar_qf[i], 1);
             mbar_init(&bar_s[i], 1);
+            mbar_init(&bar_h[i], 4);
             mbar_init(&bar_p[i], 4);
-            mbar_init(&bar_c[i], 4);
-            mbar_init(&bar_o[i], 1);
-            mbar_init(&bar_ready[i], 4);
             mbar_init(&bar_l[i], 4);
-            mbar_init(&bar_odd[i], 4);
-            s_odd[i] = 0;
+            mbar_init(&bar_o[i], 1);
+            mbar_init(&bar_of[i], 4);
+            mbar_init(&bar_item[i], 1);
+            mbar_init(&bar_itemf[i], 14);       // 8 softmax, 4 output warps, the MMA's and the loads' lanes
         }
         for (int i = 0; i < kPmStages; ++i) {
             mbar_init(&bar_full[i], 1);
@@ -244,9 +254,6 @@ attn_prompt_mma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    __syncthreads();
-    const int start = s_tile[0], len = s_tile[1], tile = s_tile[2];
-    if (tile < 0) return;               // the whole CTA: the grid is an upper bound
     if (warp == 12) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
                      "r"(512u)
@@ -259,205 +266,304 @@ attn_prompt_mma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     const uint32_t tmem = tmem_slot;
     volatile int* const ab = &abort_flag;
     int* const err = &g_prompt_error;
-    const int r0 = tile * kPmRows;
-    // key tiles of each row tile: up to its diagonal, or the sequence's end
-    const int last_tile = (len - 1) / kAtKeys;
-    const int nt0 = min(2 * tile, last_tile) + 1;
-    const int nt1 = r0 + kAtRows < len ? min(2 * tile + 1, last_tile) + 1 : 0;
-    const int nt = max(nt0, nt1);
+
+    // the i-th item, and its key tiles: up to each row tile's diagonal, or the
+    // sequence's end (none for a second tile without rows)
+    struct Shape {
+        int start, len, r0, head, nt0, nt1, nt;
+    };
+    auto shape = [](const PromptItem& it) {
+        Shape s;
+        s.start = it.start;
+        s.len = it.len;
+        s.r0 = it.tile * kPmRows;
+        s.head = it.head;
+        const int last = (it.len - 1) / kAtKeys;
+        s.nt0 = min(2 * it.tile, last) + 1;
+        s.nt1 = s.r0 + kAtRows < it.len ? min(2 * it.tile + 1, last) + 1 : 0;
+        s.nt = max(s.nt0, s.nt1);
+        return s;
+    };
+    auto next_warp = [&](int i, PromptItem* it) {       // false: no more, or a wait gave up
+        if (!at_wait_warp(&bar_item[i & 1], (i >> 1) & 1, ab, err)) return false;
+        *it = s_item[i & 1];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar_itemf[i & 1]);
+        return it->tile >= 0;
+    };
+    auto next_lane = [&](int i, PromptItem* it) {
+        if (!at_wait(&bar_item[i & 1], (i >> 1) & 1, ab, err)) return false;
+        *it = s_item[i & 1];
+        mbar_arrive(&bar_itemf[i & 1]);
+        return it->tile >= 0;
+    };
 
     if (warp < 8) {
         // ---------------- softmax ----------------
-        reg_alloc<184>();
-        const int t = warp >> 2, n = t == 0 ? nt0 : nt1;
-        const int row = 32 * (warp & 3) + lane;
+        reg_alloc<192>();
+        const int t = warp >> 2, row = 32 * (warp & 3) + lane;
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-        const uint32_t s_tm = tmem + lanes + 128 * t;
-        const int seen = min(r0 + kAtRows * t + row + 1, len);
-        RowState st{-INFINITY, 0.f};
-        int j = 0;
-        for (; j < n; ++j) {
-            if (!at_wait_warp(&bar_s[t], j & 1, ab, err)) break;
-            tc_fence_after();
-            float s[128];
-            load_scores(s_tm, s);
-            const int lim = seen - j * kAtKeys;
-            if (j == n - 1) {
-                #pragma unroll
-                for (int c = 0; c < 128; ++c) s[c] = c < lim ? s[c] : -INFINITY;
-            }
-            const float f = row_step(st, row_max(s));
-            s_scale[t][row] = f;
-            __syncwarp();
-            if (j > 0 && lane == 0) mbar_arrive(&bar_c[t]);
-            row_weights(s, st.m, st.l, s_tm);
-            if (j == n - 1 && (j + 1) * kAtKeys > len) {
-                // the tile's rows behind the sequence: their values become 0
-                const int slot = (2 * j + 1) % kPmStages;
-                if (!at_wait_warp(&bar_full[slot], ((2 * j + 1) / kPmStages) & 1, ab, err)) break;
-                if (j * kAtKeys + row >= len) {
+        const uint32_t s_tm = tmem + lanes + 128 * t, o_tm = s_tm + 256;
+        int steps = 0, uses = 0, ring = 0;              // score tiles, items with this row tile, ring tiles so far
+        bool ok = true;
+        PromptItem it;
+        for (int i = 0; ok && next_warp(i, &it); ++i) {
+            const Shape w = shape(it);
+            const int n = t == 0 ? w.nt0 : w.nt1;
+            const int seen = min(w.r0 + kAtRows * t + row + 1, w.len);
+            float m = -INFINITY, l = 0.f;
+            bool odd = false;
+            #pragma unroll 1
+            for (int j = 0; j < n; ++j, ++steps) {
+                const bool edge = j == n - 1;
+                if (edge) {
+                    // this row of the masked tile's values: zeros behind the
+                    // sequence; no number inside it
+                    const int x = ring + 2 * j + 1, slot = x % kPmStages;
+                    if (!(ok = at_wait_warp(&bar_full[slot], (x / kPmStages) & 1, ab, err))) break;
                     uint8_t* v = sm + (2 + slot) * kAtTile + row * 128;
+                    const bool inside = j * kAtKeys + row < w.len;
                     #pragma unroll
-                    for (int c = 0; c < 8; ++c) {
-                        *reinterpret_cast<uint4*>(v + 16 * c) = make_uint4(0, 0, 0, 0);
-                        *reinterpret_cast<uint4*>(v + kAtHalf + 16 * c) = make_uint4(0, 0, 0, 0);
+                    for (int c = 0; c < 16; ++c) {
+                        uint4* at = reinterpret_cast<uint4*>(v + (c >> 3) * kAtHalf + 16 * ((c ^ row) & 7));
+                        if (inside) {
+                            const uint4 u = *at;
+                            odd = odd || odd_half2(u.x) || odd_half2(u.y) || odd_half2(u.z) || odd_half2(u.w);
+                        } else {
+                            *at = make_uint4(0, 0, 0, 0);
+                        }
+                    }
+                    fence_proxy_async_smem();
+                }
+                if (!(ok = at_wait_warp(&bar_s[t], steps & 1, ab, err))) break;
+                tc_fence_after();
+                float s[128];
+                load_scores(s_tm, s);
+                if (edge) {
+                    const int lim = seen - j * kAtKeys;
+                    #pragma unroll
+                    for (int c = 0; c < 128; ++c) s[c] = c < lim ? s[c] : -INFINITY;
+                }
+                if (j == 0) m = row_max(s);
+                float sum[4];
+                uint32_t u[32];
+                #pragma unroll 1
+                for (int pass = 0;; ++pass) {
+                    sum[0] = sum[1] = sum[2] = sum[3] = 0.f;
+                    half_weights(s, weight_offset(m), u, sum);
+                    const float mx = row_max(s);
+                    const bool fine = (mx - m) * kAtScale2 <= kAtLag;      // (false for a NaN)
+                    if (pass == 1 || __all_sync(0xffffffffu, fine)) break;
+                    // (all of O's earlier products are complete: they precede this tile's scores)
+                    const float m1 = fine ? m : max3(m, mx, mx);
+                    const float f = fine ? 1.f : ex2((m - m1) * kAtScale2);
+                    m = m1;
+                    l *= f;
+                    if (j > 0) {
+                        #pragma unroll 1
+                        for (int c = 0; c < 8; ++c) {
+                            uint32_t r[16];
+                            tmem_ld16(o_tm + 16 * c, r);
+                            tmem_ld_wait();
+                            #pragma unroll
+                            for (int e = 0; e < 16; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * f);
+                            tmem_st16(o_tm + 16 * c, r);
+                        }
                     }
                 }
-                fence_proxy_async_smem();
+                auto arrive = [&](uint64_t* bar) {
+                    tmem_st_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar);
+                };
+                tmem_st32(s_tm, u);
+                arrive(&bar_h[t]);
+                half_weights(s + 64, weight_offset(m), u, sum);
+                tmem_st32(s_tm + 32, u);
+                arrive(&bar_p[t]);
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
             }
-            tmem_st_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&bar_p[t]);
-        }
-        if (j == n && n > 0) {
-            // not through s_scale, whose last factor may not have been read
-            // yet: the query tile's place is free after its last product
-            reinterpret_cast<float*>(sm + t * kAtTile)[row] = st.l;
+            if (!ok) break;
+            ring += 2 * w.nt;
+            if (n == 0) continue;
+            // the sums of the item before have been read
+            if (uses > 0 && !(ok = at_wait_warp(&bar_of[t], (uses - 1) & 1, ab, err))) break;
+            ++uses;
+            s_sum[t][row] = l;
+            odd = __any_sync(0xffffffffu, odd);
+            if (lane == 0) s_odd[t][warp & 3] = odd ? 1 : 0;
             __syncwarp();
             if (lane == 0) mbar_arrive(&bar_l[t]);
         }
     } else if (warp < 12) {
-        // ---------------- corrections and epilogue ----------------
-        reg_dealloc<80>();
+        // ---------------- outputs ----------------
+        reg_dealloc<64>();
         const int row = 32 * (warp & 3) + lane;
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+        int uses[2] = {0, 0};
         bool ok = true;
-        for (int j = 1; j < nt && ok; ++j) {
-            #pragma unroll
+        PromptItem it;
+        for (int i = 0; ok && next_warp(i, &it); ++i) {
+            const Shape w = shape(it);
+            #pragma unroll 1
             for (int t = 0; t < 2; ++t) {
-                if (j >= (t == 0 ? nt0 : nt1)) continue;
-                if (!(ok = at_wait_warp(&bar_c[t], (j - 1) & 1, ab, err))) break;
-                const float f = s_scale[t][row];
-                if (__any_sync(0xffffffffu, f != 1.f)) {
-                    if (!(ok = at_wait_warp(&bar_o[t], (j - 1) & 1, ab, err))) break;
-                    tc_fence_after();
-                    #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t r[32];
-                        const uint32_t at = tmem + lanes + 256 + 128 * t + 32 * c;
-                        tmem_ld32(at, r);
-                        tmem_ld_wait();
-                        #pragma unroll
-                        for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * f);
-                        tmem_st32(at, r);
-                    }
-                    tmem_st_wait();
-                }
+                if (t == 1 && w.nt1 == 0) break;
+                const int par = uses[t] & 1;
+                ++uses[t];
+                if (!(ok = at_wait_warp(&bar_l[t], par, ab, err) && at_wait_warp(&bar_o[t], par, ab, err))) break;
+                tc_fence_after();
+                const int x = w.r0 + kAtRows * t + row;
+                if ((s_odd[t][0] | s_odd[t][1] | s_odd[t][2] | s_odd[t][3]) != 0)
+                    slow_rows<O>(p, w.head, w.start, w.len, w.r0 + kAtRows * t, warp & 3);
+                else
+                    store_row(tmem + lanes + 256 + 128 * t, 1.f / s_sum[t][row], x < w.len,
+                              static_cast<O*>(p.out) + (size_t)(w.start + x) * p.os + (size_t)w.head * kServeDim);
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&bar_ready[t]);
-            }
-        }
-        #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            const int n = t == 0 ? nt0 : nt1;
-            if (n == 0 || !ok) continue;
-            // values of the masked tile that are no numbers, in this thread's row
-            const int slot = (2 * n - 1) % kPmStages;
-            if (!(ok = at_wait_warp(&bar_full[slot], ((2 * n - 1) / kPmStages) & 1, ab, err))) continue;
-            bool odd = false;
-            if ((n - 1) * kAtKeys + row < len) {
-                const uint8_t* v = sm + (2 + slot) * kAtTile + row * 128;
-                #pragma unroll
-                for (int c = 0; c < 16; ++c) {
-                    const uint4 u = *reinterpret_cast<const uint4*>(v + (c >> 3) * kAtHalf + 16 * ((c ^ row) & 7));
-                    odd = odd || odd_half2(u.x) || odd_half2(u.y) || odd_half2(u.z) || odd_half2(u.w);
-                }
-            }
-            if (odd) s_odd[t] = 1;
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&bar_odd[t]);
-            if (!(ok = at_wait_warp(&bar_odd[t], 0, ab, err))) continue;
-            if (!(ok = at_wait_warp(&bar_l[t], 0, ab, err))) continue;
-            const float l = reinterpret_cast<const float*>(sm + t * kAtTile)[row];
-            if (!(ok = at_wait_warp(&bar_o[t], (n - 1) & 1, ab, err))) continue;
-            tc_fence_after();
-            if (s_odd[t] != 0) {
-                slow_rows<O>(p, h, start, len, r0 + kAtRows * t, warp & 3);
-            } else {
-                const int i = r0 + kAtRows * t + row;
-                store_row(tmem + lanes + 256 + 128 * t, 1.f / l, i < len,
-                          static_cast<O*>(p.out) + (size_t)(start + i) * p.os + (size_t)h * kServeDim);
+                if (lane == 0) mbar_arrive(&bar_of[t]);
             }
         }
     } else {
         reg_dealloc<64>();
-        if (warp == 12 && lane == 0) {
-            // ---------------- products ----------------
-            const uint32_t idesc_s = umma_idesc_f16(128, 128, false), idesc_o = umma_idesc_f16(128, 128, true);
-            auto tile_at = [&](int i) { return smem_u32(sm + (size_t)(2 + i % kPmStages) * kAtTile); };
-            auto full = [&](int i) { return at_wait(&bar_full[i % kPmStages], (i / kPmStages) & 1, ab, err); };
-            auto scores = [&](int t, int i) {           // S_t = Q_t (ring tile i)^T
-                const uint32_t q = smem_u32(sm + t * kAtTile), k = tile_at(i);
-                #pragma unroll
-                for (int x = 0; x < 8; ++x) {
-                    const uint32_t off = (x >> 2) * kAtHalf + (x & 3) * 32;
-                    umma_f16_ss(tmem + 128 * t, umma_desc_sw128(q + off), umma_desc_sw128(k + off), idesc_s, x > 0);
+        if (warp == 12) {
+            if (elect_one()) {
+                // ---------------- products ----------------
+                constexpr uint32_t idesc_s = umma_idesc_f16(128, 128, false), idesc_o = umma_idesc_f16(128, 128, true);
+                const uint32_t tiles = smem_u32(sm + 2 * kAtTile), q0 = umma_desc_lo(smem_u32(sm), 16);
+                // the ring's next key and value tiles: slot and parity
+                int ks = 0, kp = 0, vs = 1, vp = 0;
+                auto step = [](int& slot, int& parity, int by) {
+                    slot += by;
+                    if (slot >= kPmStages) {
+                        slot -= kPmStages;
+                        parity ^= 1;
+                    }
+                };
+                auto scores = [&](int t) {                       // S_t = Q_t K^T
+                    const uint32_t q = q0 + t * (kAtTile >> 4), k = umma_desc_lo(tiles + ks * kAtTile, 16);
+                    #pragma unroll
+                    for (int x = 0; x < 8; ++x) {
+                        const uint32_t off = (x >> 2) * (kAtHalf >> 4) + (x & 3) * 2;
+                        umma_f16_ss(tmem + 128 * t, q + off, k + off, idesc_s, x > 0);
+                    }
+                    umma_commit(&bar_s[t]);
+                };
+                auto outputs = [&](int t, int half, bool add) {  // O_t (+)= P_t V, 64 keys
+                    const uint32_t v = umma_desc_lo(tiles + vs * kAtTile, kAtHalf) + half * (8192 >> 4);
+                    #pragma unroll
+                    for (int x = 0; x < 4; ++x)
+                        umma_f16_ts(tmem + 256 + 128 * t, tmem + 128 * t + 32 * half + 8 * x, v + x * (2048 >> 4),
+                                    idesc_o, add || x > 0);
+                };
+                int steps[2] = {0, 0}, uses[2] = {0, 0};
+                bool ok = true;
+                PromptItem it;
+                for (int i = 0; ok && next_lane(i, &it); ++i) {
+                    const Shape w = shape(it);
+                    ok = at_wait(&bar_q[0], uses[0] & 1, ab, err) && at_wait(&bar_full[ks], kp, ab, err);
+                    if (!ok) break;
+                    scores(0);
+                    if (w.nt0 == 1) umma_commit(&bar_qf[0]);
+                    if (w.nt1 > 0) {
+                        if (!(ok = at_wait(&bar_q[1], uses[1] & 1, ab, err))) break;
+                        scores(1);
+                        if (w.nt1 == 1) umma_commit(&bar_qf[1]);
+                    }
+                    umma_commit(&bar_free[ks]);
+                    step(ks, kp, 2);
+                    #pragma unroll 1
+                    for (int j = 0; j < w.nt && ok; ++j) {
+                        const bool more = j + 1 < w.nt;
+                        ok = at_wait(&bar_full[vs], vp, ab, err) && (!more || at_wait(&bar_full[ks], kp, ab, err));
+                        #pragma unroll
+                        for (int t = 0; t < 2; ++t) {
+                            const int n = t == 0 ? w.nt0 : w.nt1;
+                            if (!ok || j >= n) continue;
+                            // the item before has left O (of) before the first product overwrites it
+                            ok = (j > 0 || uses[t] == 0 || at_wait(&bar_of[t], (uses[t] - 1) & 1, ab, err)) &&
+                                 at_wait(&bar_h[t], steps[t] & 1, ab, err);
+                            if (!ok) continue;
+                            tc_fence_after();
+                            outputs(t, 0, j > 0);
+                            if (!(ok = at_wait(&bar_p[t], steps[t] & 1, ab, err))) continue;
+                            tc_fence_after();
+                            outputs(t, 1, true);
+                            ++steps[t];
+                            if (j + 1 < n) {
+                                scores(t);
+                                if (j + 2 == n) umma_commit(&bar_qf[t]);
+                            } else {
+                                umma_commit(&bar_o[t]);
+                            }
+                        }
+                        umma_commit(&bar_free[vs]);
+                        step(vs, vp, 2);
+                        if (more) {
+                            umma_commit(&bar_free[ks]);
+                            step(ks, kp, 2);
+                        }
+                    }
+                    ++uses[0];
+                    uses[1] += w.nt1 > 0 ? 1 : 0;
                 }
-                umma_commit(&bar_s[t]);
-            };
-            auto outputs = [&](int t, int i, bool add) { // O_t (+)= P_t (ring tile i)
-                const uint32_t v = tile_at(i);
-                #pragma unroll
-                for (int x = 0; x < 8; ++x)
-                    umma_f16_ts(tmem + 256 + 128 * t, tmem + 128 * t + 8 * x, umma_desc_mn_sw128(v + 2048 * x, kAtHalf),
-                                idesc_o, add || x > 0);
-                umma_commit(&bar_o[t]);
-            };
-            bool ok = at_wait(&bar_q[0], 0, ab, err) && full(0);
-            if (ok) {
-                tc_fence_after();
-                scores(0, 0);
-                if (nt1 > 0) {
-                    ok = at_wait(&bar_q[1], 0, ab, err);
-                    if (ok) scores(1, 0);
-                }
-                umma_commit(&bar_free[0]);
+                umma_commit(&bar_done);
+                at_drain(&bar_done, 0);
             }
-            for (int j = 0; j < nt && ok; ++j) {
-                const int vi = 2 * j + 1, ki = 2 * j + 2;
-                #pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    const int n = t == 0 ? nt0 : nt1;
-                    if (!ok || j >= n) continue;
-                    ok = at_wait(&bar_p[t], j & 1, ab, err) && (j == 0 || at_wait(&bar_ready[t], (j - 1) & 1, ab, err)) &&
-                         full(vi);
-                    if (!ok) continue;
-                    tc_fence_after();
-                    outputs(t, vi, j > 0);
-                    if (j + 1 < n) {
-                        if (!(ok = full(ki))) continue;
-                        scores(t, ki);
+            __syncwarp();
+        } else if (warp == 13) {
+            if (elect_one()) {
+                // ---------------- loads ----------------
+                int x = 0, uses[2] = {0, 0};
+                bool ok = true;
+                auto load = [&](uint8_t* dst, const CUtensorMap* tm, int head, int token, uint64_t* bar) {
+                    mbar_expect_tx(bar, kAtTile);
+                    tma_load_3d(dst, tm, 0, head, token, bar);
+                    tma_load_3d(dst + kAtHalf, tm, 64, head, token, bar);
+                };
+                PromptItem it;
+                for (int i = 0; ok && next_lane(i, &it); ++i) {
+                    const Shape w = shape(it);
+                    const int kvh = w.head / p.group;
+                    #pragma unroll 1
+                    for (int j = -1; j < 2 * w.nt; ++j) {
+                        // Q0, K0, Q1, V0, K1, V1, ...
+                        const int t = j < 0 ? 0 : 1;
+                        if (j < 0 || (j == 1 && w.nt1 > 0)) {
+                            if (uses[t] > 0 && !(ok = at_wait(&bar_qf[t], (uses[t] - 1) & 1, ab, err))) break;
+                            ++uses[t];
+                            load(sm + t * kAtTile, &tm_q, w.head, w.start + w.r0 + kAtRows * t, &bar_q[t]);
+                        }
+                        if (j < 0) continue;
+                        const int s = x % kPmStages, use = x / kPmStages;
+                        if (use > 0 && !(ok = at_wait(&bar_free[s], (use - 1) & 1, ab, err))) break;
+                        load(sm + (size_t)(2 + s) * kAtTile, (j & 1) == 0 ? &tm_k : &tm_v, kvh,
+                             w.start + (j >> 1) * kAtKeys, &bar_full[s]);
+                        ++x;
                     }
                 }
-                umma_commit(&bar_free[vi % kPmStages]);
-                if (j + 1 < nt) umma_commit(&bar_free[ki % kPmStages]);
+                // no copy may be in flight when the CTA ends
+                for (int t = 0; t < 2; ++t)
+                    if (uses[t] > 0) at_drain(&bar_q[t], (uses[t] - 1) & 1);
+                for (int y = max(0, x - kPmStages); y < x; ++y) at_drain(&bar_full[y % kPmStages], (y / kPmStages) & 1);
             }
-            umma_commit(&bar_done);
-            at_drain(&bar_done, 0);
-        } else if (warp == 13 && lane == 0) {
-            // ---------------- loads ----------------
-            const int kvh = h / p.group;
-            auto load = [&](uint8_t* dst, const CUtensorMap* tm, int head, int token, uint64_t* bar) {
-                mbar_expect_tx(bar, kAtTile);
-                tma_load_3d(dst, tm, 0, head, token, bar);
-                tma_load_3d(dst + kAtHalf, tm, 64, head, token, bar);
-            };
-            load(sm, &tm_q, h, start + r0, &bar_q[0]);
-            int i = 0;
-            const int total = 2 * nt;
-            for (; i < total; ++i) {
-                const int s = i % kPmStages, use = i / kPmStages;
-                if (use > 0 && !at_wait(&bar_free[s], (use - 1) & 1, ab, err)) break;
-                load(sm + (size_t)(2 + s) * kAtTile, (i & 1) == 0 ? &tm_k : &tm_v, kvh, start + (i >> 1) * kAtKeys,
-                     &bar_full[s]);
-                if (i == 0 && nt1 > 0) load(sm + kAtTile, &tm_q, h, start + r0 + kAtRows, &bar_q[1]);
+            __syncwarp();
+        } else if (warp == 14) {
+            // ---------------- items ----------------
+            #pragma unroll 1
+            for (int i = 0;; ++i) {
+                // every other round backwards: the CTA that got the longest
+                // item of one round gets the shortest of the next
+                const int x = i * (int)gridDim.x + ((i & 1) ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x);
+                PromptItem it{0, 0, -1, x % p.n_head};
+                if (!find_long_first<kPmRows>(p, x / p.n_head, &it.start, &it.len, &it.tile)) it.tile = -1;
+                if (i >= 2 && !at_wait_warp(&bar_itemf[i & 1], ((i >> 1) - 1) & 1, ab, err)) break;
+                if (lane == 0) {
+                    s_item[i & 1] = it;
+                    mbar_arrive(&bar_item[i & 1]);
+                }
+                if (it.tile < 0) break;
             }
-            // no copy may be in flight when the CTA ends
-            at_drain(&bar_q[0], 0);
-            if (nt1 > 0) at_drain(&bar_q[1], 0);
-            for (int x = max(0, i - kPmStages); x < i; ++x) at_drain(&bar_full[x % kPmStages], (x / kPmStages) & 1);
         }
     }
     tc_fence_before();
@@ -492,8 +598,12 @@ cudaError_t launch_mma(const PromptParams& p, cudaStream_t st) {
     auto* kern = attn_prompt_mma_kernel<O>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kPmSmem);
     if (e != cudaSuccess) return e;
-    const long long tiles = p.n_tokens / kPmRows + (long long)p.n_seq;
-    return launch(kern, dim3((unsigned)(tiles * p.n_head)), dim3(kPmThreads), kPmSmem, st, false, tq, tk, tv, p);
+    int dev = 0;
+    if ((e = cudaGetDevice(&dev)) != cudaSuccess) return e;
+    // at most this many items: every sequence may end inside one
+    const long long items = (p.n_tokens / kPmRows + (long long)p.n_seq) * p.n_head;
+    const int grid = (int)(items < num_sms_of(dev) ? items : num_sms_of(dev));
+    return launch(kern, dim3((unsigned)grid), dim3(kPmThreads), kPmSmem, st, false, tq, tk, tv, p);
 }
 
 }  // namespace
