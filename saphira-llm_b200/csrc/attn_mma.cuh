@@ -12,6 +12,9 @@ constexpr int kAtRows = 128;                    // query rows of a tile: the TME
 constexpr int kAtKeys = 128;                    // keys of a tile
 constexpr int kAtHalf = 128 * 128;              // bytes of 128 rows x 64 f16 in the 128-byte swizzle
 constexpr int kAtTile = 2 * kAtHalf;            // ... x 128 f16
+constexpr int kAtStages = 5;                    // key and value tiles in flight
+constexpr int kAtThreads = 512;
+constexpr int kAtSmem = (2 + kAtStages) * kAtTile + 3 * 1024;       // two query tiles, the ring, barriers and sums
 // softmax in base 2: exp(s / sqrt(128)) = 2^(s c)
 constexpr float kAtScale2 = 0.08838834764831845f * 1.4426950408889634f;
 // the running maximum a row's weights stand against may lag behind by this
@@ -144,38 +147,435 @@ __device__ __forceinline__ void load_scores(uint32_t s_tmem, float (&s)[128]) {
 }
 
 // the tensor-memory outputs of one row, scaled, to global memory: f16 or f32
-__device__ __forceinline__ void store_row(uint32_t o_tmem, float f, bool live, __half* out) {
+__device__ __forceinline__ void store16(const uint32_t (&r)[16], float f, __half* out) {
     #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-        uint32_t r[32];
-        tmem_ld32(o_tmem + 32 * c, r);
+    for (int i = 0; i < 2; ++i) {
+        uint4 u;
+        uint32_t* w = &u.x;
+        #pragma unroll
+        for (int e = 0; e < 4; ++e)
+            w[e] = pack_half2(__uint_as_float(r[8 * i + 2 * e]) * f, __uint_as_float(r[8 * i + 2 * e + 1]) * f);
+        *reinterpret_cast<uint4*>(out + 8 * i) = u;
+    }
+}
+__device__ __forceinline__ void store16(const uint32_t (&r)[16], float f, float* out) {
+    #pragma unroll
+    for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<float4*>(out + 4 * i) =
+            make_float4(__uint_as_float(r[4 * i]) * f, __uint_as_float(r[4 * i + 1]) * f,
+                        __uint_as_float(r[4 * i + 2]) * f, __uint_as_float(r[4 * i + 3]) * f);
+}
+template <class O>
+__device__ __forceinline__ void store_row(uint32_t o_tmem, float f, bool live, O* out) {
+    #pragma unroll 2
+    for (int c = 0; c < 8; ++c) {
+        uint32_t r[16];
+        tmem_ld16(o_tmem + 16 * c, r);
         tmem_ld_wait();
-        if (live) {
-            #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                uint4 u;
-                uint32_t* w = &u.x;
-                #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    w[e] = pack_half2(__uint_as_float(r[8 * i + 2 * e]) * f, __uint_as_float(r[8 * i + 2 * e + 1]) * f);
-                *reinterpret_cast<uint4*>(out + 32 * c + 8 * i) = u;
+        if (live) store16(r, f, out + 16 * c);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// The core of the f16 kernels. One CTA per SM walks items: up to two tiles of
+// 128 query rows that share every key tile. Scores, weights and outputs
+// stay in tensor memory (512 columns: S0 S1 O0 O1, 128 each; a tile's f16
+// weights overwrite the first 64 columns of its scores).
+//
+//   warps 0-3, 4-7   softmax of tile 0, 1: one thread per row. S from tensor
+//                    memory, mask, weights back. The weights stand against the
+//                    running maximum of the tiles before; the tile's own
+//                    maximum is found meanwhile and only checked: where it is
+//                    more than kAtLag doublings higher (rare after the first
+//                    tiles) the warp rescales its rows of O and starts over.
+//   warps 8-11       outputs to global memory, under the next item's products.
+//   warp 12, 1 lane  tcgen05.mma: S_t = Q_t K^T (both from shared memory) and
+//                    O_t += P_t V (P from tensor memory, V MN-major as it
+//                    lies), the first 64 keys as soon as their weights are
+//                    there. The order P0 V, S0', P1 V, S1' lets one tile's
+//                    softmax run under the other tile's products.
+//   warp 13          TMA: Q per item, K and V tiles through a ring of five.
+//   warp 14          the items, two ahead.
+//
+// What bounds it: per key tile and row tile 1024 clocks of products, and the
+// chain S -> softmax -> P V -> S', whose softmax is 16384 exponentials at 16
+// a clock, shared by the two tiles.
+//
+// Masks: a row sees the item's first so many keys, so only an item's last key
+// tiles are masked. A value row behind the item's keys is zeroed in shared
+// memory before it meets its zero weight. A value among the keys that is no
+// number would leak the same way into rows of the tile that do not see it: the
+// softmax warps look for such values in the masked tiles, and if there are
+// any warps 8-11 recompute the tile's rows one by one.
+//
+// `W` says what the items are: find(x, item) (false: there is no item x, but
+// later ones may be), tiles(item, t) (0: no such row tile), keys(item),
+// seen(item, t, row) (not above keys, and least for row 0), live(item, t, row)
+// (a row to be written), a Loader, store(...) and slow(...).
+//
+// Registers: 512 threads x 128 at launch; 2 x 192 (softmax) + 64 (outputs) +
+// 64 (the issuing warps) = 512 = 4 x 128 after the split.
+// ---------------------------------------------------------------------------
+// why a bounded wait gave up (0: none did), in each file with such a kernel
+static __device__ int g_attn_error;
+static inline int take_attn_error() {
+    int v = 0;
+    const int zero = 0;
+    if (cudaMemcpyFromSymbol(&v, g_attn_error, sizeof v) != cudaSuccess ||
+        cudaMemcpyToSymbol(g_attn_error, &zero, sizeof zero) != cudaSuccess)
+        return -1;
+    return v;
+}
+
+template <class W>
+__device__ __forceinline__ void attn_core(const W w) {
+    int* const err = &g_attn_error;
+    using Item = typename W::Item;
+    extern __shared__ __align__(1024) uint8_t sm[];
+    // [2]: per row tile. q, qf: Q there / free; s: scores there; h, p: the
+    // first half of the weights there, all; l: sums there; o: outputs
+    // complete; of: outputs read
+    struct Shared {
+        uint64_t bar_full[kAtStages], bar_free[kAtStages], bar_q[2], bar_qf[2], bar_s[2], bar_h[2], bar_p[2], bar_l[2],
+            bar_o[2], bar_of[2], bar_item[2], bar_itemf[2], bar_done;
+        float sum[2][kAtRows], top[2][kAtRows];
+        Item item[2];
+        int odd[2][4];
+        uint32_t tmem;
+        int abort_flag;
+    };
+    static_assert(sizeof(Shared) <= kAtSmem - (2 + kAtStages) * kAtTile, "the part behind the tiles");
+    Shared& sh = *reinterpret_cast<Shared*>(sm + (2 + kAtStages) * kAtTile);
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    if ((smem_u32(sm) & 1023u) != 0) {           // the swizzled layouts need it; the compiler was told to
+        if (threadIdx.x == 0) atomicExch(err, 2);
+        return;
+    }
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&sh.bar_q[i], 1);
+            mbar_init(&sh.bar_qf[i], 1);
+            mbar_init(&sh.bar_s[i], 1);
+            mbar_init(&sh.bar_h[i], 4);
+            mbar_init(&sh.bar_p[i], 4);
+            mbar_init(&sh.bar_l[i], 4);
+            mbar_init(&sh.bar_o[i], 1);
+            mbar_init(&sh.bar_of[i], 4);
+            mbar_init(&sh.bar_item[i], 1);
+            mbar_init(&sh.bar_itemf[i], 14);    // 8 softmax, 4 output warps, the products and the loads
+        }
+        for (int i = 0; i < kAtStages; ++i) {
+            mbar_init(&sh.bar_full[i], 1);
+            mbar_init(&sh.bar_free[i], 1);
+        }
+        mbar_init(&sh.bar_done, 1);
+        sh.abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)),
+                     "r"(512u)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sh.tmem;
+    volatile int* const ab = &sh.abort_flag;
+
+    auto next_warp = [&](int i, Item* it) {       // false: no more, or a wait gave up
+        if (!at_wait_warp(&sh.bar_item[i & 1], (i >> 1) & 1, ab, err)) return false;
+        *it = sh.item[i & 1];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.bar_itemf[i & 1]);
+        return !it->last();
+    };
+    auto next_lane = [&](int i, Item* it) {
+        if (!at_wait(&sh.bar_item[i & 1], (i >> 1) & 1, ab, err)) return false;
+        *it = sh.item[i & 1];
+        mbar_arrive(&sh.bar_itemf[i & 1]);
+        return !it->last();
+    };
+
+    if (warp < 8) {
+        // ---------------- softmax ----------------
+        reg_alloc<192>();
+        const int t = warp >> 2, row = 32 * (warp & 3) + lane;
+        const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+        const uint32_t s_tm = tmem + lanes + 128 * t, o_tm = s_tm + 256;
+        int steps = 0, uses = 0, ring = 0;              // score tiles, items with this row tile, ring tiles so far
+        bool ok = true;
+        Item it;
+        for (int i = 0; ok && next_warp(i, &it); ++i) {
+            const int n0 = w.tiles(it, 0), n1 = w.tiles(it, 1), n = t == 0 ? n0 : n1;
+            const int keys = w.keys(it), seen = w.seen(it, t, row);
+            // all rows of this row tile see the keys below `every`
+            const int every = n > 0 ? w.seen(it, t, 0) : 0;
+            // a warp without rows only keeps the others' pace; a row that is none
+            // (what lies in its place may be anything) never asks for a second pass
+            const bool live = n > 0 && w.live(it, t, row), idle = !__any_sync(0xffffffffu, live);
+            float m = -INFINITY, l = 0.f;
+            bool odd = false;
+            #pragma unroll 1
+            for (int j = 0; j < n; ++j, ++steps) {
+                const bool edge = (j + 1) * kAtKeys > every;
+                if (edge) {
+                    // this row of the masked tile's values: zeros behind the
+                    // sequence; no number inside it
+                    const int x = ring + 2 * j + 1, slot = x % kAtStages;
+                    if (!(ok = at_wait_warp(&sh.bar_full[slot], (x / kAtStages) & 1, ab, err))) break;
+                    uint8_t* v = sm + (2 + slot) * kAtTile + row * 128;
+                    const int key = j * kAtKeys + row;
+                    #pragma unroll
+                    for (int c = 0; c < 16; ++c) {
+                        uint4* at = reinterpret_cast<uint4*>(v + (c >> 3) * kAtHalf + 16 * ((c ^ row) & 7));
+                        if (key < keys) {
+                            const uint4 u = *at;
+                            odd = odd || (key >= every &&
+                                          (odd_half2(u.x) || odd_half2(u.y) || odd_half2(u.z) || odd_half2(u.w)));
+                        } else {
+                            *at = make_uint4(0, 0, 0, 0);
+                        }
+                    }
+                    fence_proxy_async_smem();
+                }
+                if (!(ok = at_wait_warp(&sh.bar_s[t], steps & 1, ab, err))) break;
+                tc_fence_after();
+                if (idle) {
+                    if (lane == 0) {
+                        mbar_arrive(&sh.bar_h[t]);
+                        mbar_arrive(&sh.bar_p[t]);
+                    }
+                    continue;
+                }
+                float s[128];
+                load_scores(s_tm, s);
+                if (edge) {
+                    const int lim = seen - j * kAtKeys;
+                    #pragma unroll
+                    for (int c = 0; c < 128; ++c) s[c] = c < lim ? s[c] : -INFINITY;
+                }
+                if (j == 0) m = row_max(s);
+                float sum[4];
+                uint32_t u[32];
+                #pragma unroll 1
+                for (int pass = 0;; ++pass) {
+                    sum[0] = sum[1] = sum[2] = sum[3] = 0.f;
+                    half_weights(s, weight_offset(m), u, sum);
+                    const float mx = row_max(s);
+                    // (false for a NaN)
+                    const bool fine = (mx - m) * kAtScale2 <= kAtLag || mx == -INFINITY || !live;
+                    if (pass == 1 || __all_sync(0xffffffffu, fine)) break;
+                    // (all of O's earlier products are complete: they precede this tile's scores)
+                    const float m1 = fine ? m : max3(m, mx, mx);
+                    const float f = fine ? 1.f : ex2((m - m1) * kAtScale2);
+                    m = m1;
+                    l *= f;
+                    if (j > 0) {
+                        #pragma unroll 1
+                        for (int c = 0; c < 8; ++c) {
+                            uint32_t r[16];
+                            tmem_ld16(o_tm + 16 * c, r);
+                            tmem_ld_wait();
+                            #pragma unroll
+                            for (int e = 0; e < 16; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * f);
+                            tmem_st16(o_tm + 16 * c, r);
+                        }
+                    }
+                }
+                auto arrive = [&](uint64_t* bar) {
+                    tmem_st_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar);
+                };
+                tmem_st32(s_tm, u);
+                arrive(&sh.bar_h[t]);
+                half_weights(s + 64, weight_offset(m), u, sum);
+                tmem_st32(s_tm + 32, u);
+                arrive(&sh.bar_p[t]);
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            }
+            if (!ok) break;
+            ring += 2 * max(n0, n1);
+            if (n == 0) continue;
+            // the sums of the item before have been read
+            if (uses > 0 && !(ok = at_wait_warp(&sh.bar_of[t], (uses - 1) & 1, ab, err))) break;
+            ++uses;
+            sh.sum[t][row] = l;
+            sh.top[t][row] = m;
+            odd = __any_sync(0xffffffffu, odd);
+            if (lane == 0) sh.odd[t][warp & 3] = odd ? 1 : 0;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.bar_l[t]);
+        }
+    } else if (warp < 12) {
+        // ---------------- outputs ----------------
+        reg_dealloc<64>();
+        const int row = 32 * (warp & 3) + lane;
+        const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+        int uses[2] = {0, 0};
+        bool ok = true;
+        Item it;
+        for (int i = 0; ok && next_warp(i, &it); ++i) {
+            #pragma unroll 1
+            for (int t = 0; t < 2; ++t) {
+                if (w.tiles(it, t) == 0) break;
+                const int par = uses[t] & 1;
+                ++uses[t];
+                if (!(ok = at_wait_warp(&sh.bar_l[t], par, ab, err) && at_wait_warp(&sh.bar_o[t], par, ab, err))) break;
+                tc_fence_after();
+                if ((sh.odd[t][0] | sh.odd[t][1] | sh.odd[t][2] | sh.odd[t][3]) != 0)
+                    w.slow(it, t, warp & 3);
+                else
+                    w.store(it, t, row, tmem + lanes + 256 + 128 * t, sh.top[t][row], sh.sum[t][row]);
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.bar_of[t]);
+            }
+        }
+    } else {
+        reg_dealloc<64>();
+        if (warp == 12) {
+            if (elect_one()) {
+                // ---------------- products ----------------
+                constexpr uint32_t idesc_s = umma_idesc_f16(128, 128, false), idesc_o = umma_idesc_f16(128, 128, true);
+                const uint32_t tiles = smem_u32(sm + 2 * kAtTile), q0 = umma_desc_lo(smem_u32(sm), 16);
+                // the ring's next key and value tiles: slot and parity
+                int ks = 0, kp = 0, vs = 1, vp = 0;
+                auto step = [](int& slot, int& parity, int by) {
+                    slot += by;
+                    if (slot >= kAtStages) {
+                        slot -= kAtStages;
+                        parity ^= 1;
+                    }
+                };
+                auto scores = [&](int t) {                       // S_t = Q_t K^T
+                    const uint32_t q = q0 + t * (kAtTile >> 4), k = umma_desc_lo(tiles + ks * kAtTile, 16);
+                    #pragma unroll
+                    for (int x = 0; x < 8; ++x) {
+                        const uint32_t off = (x >> 2) * (kAtHalf >> 4) + (x & 3) * 2;
+                        umma_f16_ss(tmem + 128 * t, q + off, k + off, idesc_s, x > 0);
+                    }
+                    umma_commit(&sh.bar_s[t]);
+                };
+                auto outputs = [&](int t, int half, bool add) {  // O_t (+)= P_t V, 64 keys
+                    const uint32_t v = umma_desc_lo(tiles + vs * kAtTile, kAtHalf) + half * (8192 >> 4);
+                    #pragma unroll
+                    for (int x = 0; x < 4; ++x)
+                        umma_f16_ts(tmem + 256 + 128 * t, tmem + 128 * t + 32 * half + 8 * x, v + x * (2048 >> 4),
+                                    idesc_o, add || x > 0);
+                };
+                int steps[2] = {0, 0}, uses[2] = {0, 0};
+                bool ok = true;
+                Item it;
+                for (int i = 0; ok && next_lane(i, &it); ++i) {
+                    const int n0 = w.tiles(it, 0), n1 = w.tiles(it, 1), nt = max(n0, n1);
+                    ok = at_wait(&sh.bar_q[0], uses[0] & 1, ab, err) && at_wait(&sh.bar_full[ks], kp, ab, err);
+                    if (!ok) break;
+                    scores(0);
+                    if (n0 == 1) umma_commit(&sh.bar_qf[0]);
+                    if (n1 > 0) {
+                        if (!(ok = at_wait(&sh.bar_q[1], uses[1] & 1, ab, err))) break;
+                        scores(1);
+                        if (n1 == 1) umma_commit(&sh.bar_qf[1]);
+                    }
+                    umma_commit(&sh.bar_free[ks]);
+                    step(ks, kp, 2);
+                    #pragma unroll 1
+                    for (int j = 0; j < nt && ok; ++j) {
+                        const bool more = j + 1 < nt;
+                        ok = at_wait(&sh.bar_full[vs], vp, ab, err) && (!more || at_wait(&sh.bar_full[ks], kp, ab, err));
+                        #pragma unroll
+                        for (int t = 0; t < 2; ++t) {
+                            const int n = t == 0 ? n0 : n1;
+                            if (!ok || j >= n) continue;
+                            // the item before has left O (of) before the first product overwrites it
+                            ok = (j > 0 || uses[t] == 0 || at_wait(&sh.bar_of[t], (uses[t] - 1) & 1, ab, err)) &&
+                                 at_wait(&sh.bar_h[t], steps[t] & 1, ab, err);
+                            if (!ok) continue;
+                            tc_fence_after();
+                            outputs(t, 0, j > 0);
+                            if (!(ok = at_wait(&sh.bar_p[t], steps[t] & 1, ab, err))) continue;
+                            tc_fence_after();
+                            outputs(t, 1, true);
+                            ++steps[t];
+                            if (j + 1 < n) {
+                                scores(t);
+                                if (j + 2 == n) umma_commit(&sh.bar_qf[t]);
+                            } else {
+                                umma_commit(&sh.bar_o[t]);
+                            }
+                        }
+                        umma_commit(&sh.bar_free[vs]);
+                        step(vs, vp, 2);
+                        if (more) {
+                            umma_commit(&sh.bar_free[ks]);
+                            step(ks, kp, 2);
+                        }
+                    }
+                    ++uses[0];
+                    uses[1] += n1 > 0 ? 1 : 0;
+                }
+                umma_commit(&sh.bar_done);
+                at_drain(&sh.bar_done, 0);
+            }
+            __syncwarp();
+        } else if (warp == 13) {
+            // ---------------- loads ----------------
+            int x = 0, uses[2] = {0, 0};
+            bool ok = true;
+            Item it;
+            for (int i = 0; ok && next_warp(i, &it); ++i) {
+                const int n1 = w.tiles(it, 1), nt = max(w.tiles(it, 0), n1);
+                typename W::Loader load;
+                load.start(w, it, lane);
+                #pragma unroll 1
+                for (int j = -1; j < 2 * nt; ++j) {
+                    // Q0, K0, Q1, V0, K1, V1, ...
+                    const int t = j < 0 ? 0 : 1;
+                    if (j < 0 || (j == 1 && n1 > 0)) {
+                        if (uses[t] > 0 && !(ok = at_wait_warp(&sh.bar_qf[t], (uses[t] - 1) & 1, ab, err))) break;
+                        ++uses[t];
+                        load.q(w, it, t, sm + t * kAtTile, &sh.bar_q[t], lane);
+                    }
+                    if (j < 0) continue;
+                    const int s = x % kAtStages, use = x / kAtStages;
+                    if (use > 0 && !(ok = at_wait_warp(&sh.bar_free[s], (use - 1) & 1, ab, err))) break;
+                    load.kv(w, it, j >> 1, (j & 1) != 0, sm + (size_t)(2 + s) * kAtTile, &sh.bar_full[s], lane);
+                    ++x;
+                }
+            }
+            // no copy may be in flight when the CTA ends
+            for (int t = 0; t < 2; ++t)
+                if (uses[t] > 0) at_drain(&sh.bar_q[t], (uses[t] - 1) & 1);
+            for (int y = max(0, x - kAtStages); y < x; ++y) at_drain(&sh.bar_full[y % kAtStages], (y / kAtStages) & 1);
+            __syncwarp();
+        } else if (warp == 14) {
+            // ---------------- items ----------------
+            #pragma unroll 1
+            for (int r = 0, i = 0;; ++r) {
+                // every other round backwards: the CTA that got the longest
+                // item of one round gets the shortest of the next
+                const long long x = (long long)r * gridDim.x + ((r & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+                Item it;
+                if (!w.find(x, &it)) continue;          // no item has this number
+                if (i >= 2 && !at_wait_warp(&sh.bar_itemf[i & 1], ((i >> 1) - 1) & 1, ab, err)) break;
+                if (lane == 0) {
+                    sh.item[i & 1] = it;
+                    mbar_arrive(&sh.bar_item[i & 1]);
+                }
+                if (it.last()) break;
+                ++i;
             }
         }
     }
-}
-__device__ __forceinline__ void store_row(uint32_t o_tmem, float f, bool live, float* out) {
-    #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-        uint32_t r[32];
-        tmem_ld32(o_tmem + 32 * c, r);
-        tmem_ld_wait();
-        if (live) {
-            #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                *reinterpret_cast<float4*>(out + 32 * c + 4 * i) =
-                    make_float4(__uint_as_float(r[4 * i]) * f, __uint_as_float(r[4 * i + 1]) * f,
-                                __uint_as_float(r[4 * i + 2]) * f, __uint_as_float(r[4 * i + 3]) * f);
-        }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 12) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
     }
 }
 

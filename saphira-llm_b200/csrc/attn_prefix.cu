@@ -1,20 +1,48 @@
 // attn_prefix.cu -- decode attention of sequences that share a prefix, over a
 // paged cache.
+//
+// The rows of a kv head are all (sequence, query token, query head of the
+// group). Against the prefix they are one matrix, so each of its keys is read
+// once and multiplied with all of them; against a sequence's own tokens only
+// that sequence's rows are. Both kinds of work are split along the keys into
+// items of about one size; an item leaves, for each of its rows, the softmax's
+// maximum m and sum l over its keys and the unscaled output, and a second
+// launch (overlapped by programmatic dependent launch) joins a row's parts:
+//     M = max m_i,  out = sum_i e^(m_i - M) o_i / sum_i e^(m_i - M) l_i.
+//
+// f16: the tensor-core core of attn_mma.cuh. f32, and groups of more than 128
+// heads: the 32-bit tile of attn_simt.cuh, one item per CTA.
+//
+// Bound: HBM (the keys and values once) for few rows; the products for many
+// (n * n_q * group rows share each key: above about 250 of them).
 
+#include "attn_mma.cuh"
 #include "attn_simt.cuh"
 
 namespace sllm {
 namespace {
+
+// how the work is cut, the same for every kernel of a call
+struct Plan {
+    int key_tile;                   // keys of a tile
+    int rt, per;                    // rows of a row tile, row tiles of an item
+    int sp, ptiles;                 // splits and key tiles of the prefix
+    int cm;                         // most chunks of a sequence's own keys
+    int ri_all, ri_seq;             // row items of all sequences, of one
+};
 
 struct PrefixParams {
     const void* q;                  // [n][n_q][n_head][128]
     void* out;
     const void* kp;                 // the layer's slice of page 0
     const void* vp;
-    size_t page_stride;
+    size_t page_stride;             // elements
     const int32_t* slots;
     int n, n_q, n_head, n_kv, group, prefix;
     int32_t* status;
+    float* part_o;                  // [n_kv][rows][sp + cm][128]
+    float2* part_ml;                // [n_kv][rows][sp + cm]
+    Plan plan;
 };
 
 // the tokens a sequence's slot holds; -1 when the slot or its length is wrong
@@ -28,57 +56,385 @@ __device__ __forceinline__ int seq_len(const PagesDev& pg, const PrefixParams& p
     return len;
 }
 
-template <class T, class O>
-__global__ void __launch_bounds__(kSimtThreads)
-attn_prefix_simt_kernel(const PagesDev pg, const __grid_constant__ PrefixParams p) {
-    extern __shared__ float sm[];
-    const int b = blockIdx.x, kvh = blockIdx.y, rows = p.n_q * p.group, r0 = blockIdx.z * kSimtRows;
-    int slot;
-    const int len = seq_len(pg, p, b, &slot);
-    if (len < 0) {
-        if (threadIdx.x == 0) raise(p.status, SLLM_CUDA_ERR_ARG);
-        return;
-    }
-    // row r is query token r / group, head kvh * group + r % group
-    auto row_off = [&](int r) {
-        return (((size_t)b * p.n_q + r / p.group) * p.n_head + kvh * p.group + r % p.group) * kServeDim;
-    };
-    simt_load_q<T>(sm, [&](int r) {
-        return r0 + r < rows ? static_cast<const T*>(p.q) + row_off(r0 + r) : nullptr;
-    });
-    SimtState st;
-    simt_init(st);
-    const int ty = threadIdx.x >> 4;
-    int lim[4];
-    #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int r = r0 + 4 * ty + i;
-        lim[i] = r < rows ? max(0, len - p.n_q + 1 + r / p.group) : 0;
-    }
-    const int32_t* row = pg.tables + (size_t)slot * pg.width;
-    auto addr = [&](const void* pool, int j) -> const T* {
-        if (j >= len) return nullptr;
-        int id = row[j / pg.page];
-        if (id < 0 || id >= pg.n_pages) {
-            raise(p.status, SLLM_CUDA_ERR_ARG);
-            return nullptr;
-        }
-        return static_cast<const T*>(pool) + (size_t)id * p.page_stride + ((size_t)kvh * pg.page + j % pg.page) * kServeDim;
-    };
-    for (int j0 = 0; j0 < len; j0 += kSimtKeys)
-        simt_tile<T>(sm, st, j0, lim, [&](int j) { return addr(p.kp, j); }, [&](int j) { return addr(p.vp, j); });
-    #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (r0 + 4 * ty + i < rows) simt_store(st, i, static_cast<O*>(p.out) + row_off(r0 + 4 * ty + i));
+// chunks of a sequence's own keys: at least two tiles each
+__device__ __forceinline__ int own_chunks(const PrefixParams& p, int len, int* tiles) {
+    const int own = max(0, len - p.prefix);
+    *tiles = (own + p.plan.key_tile - 1) / p.plan.key_tile;
+    return min(p.plan.cm, (*tiles + 1) / 2);
 }
 
-template <class T, class O>
-cudaError_t launch_simt(const PagesDev& pg, const PrefixParams& p, cudaStream_t st) {
-    auto* kern = attn_prefix_simt_kernel<T, O>;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSimtSmem);
+// Keys a .. a + keys - 1 of `slot` for rows row0 .. of kv head kvh (at most
+// row_end); row r (token r / group) sees lim0 + r / group - tok0 of them.
+struct PrefixItem {
+    int slot, kvh, row0, row_end, a, keys, lim0, tok0, part;    // part < 0: no more items
+    __device__ bool last() const { return part < 0; }
+};
+
+// item x: the prefix's splits first, then the sequences' own chunks; false
+// where a sequence has fewer chunks than its share of numbers
+__device__ __forceinline__ bool find_item(const PagesDev& pg, const PrefixParams& p, long long x, PrefixItem* it) {
+    const Plan& pl = p.plan;
+    const long long pre = (long long)p.n_kv * pl.ri_all * pl.sp;
+    if (x < pre) {
+        const int ri = (int)(x % pl.ri_all), u = (int)(x / pl.ri_all);
+        it->kvh = u % p.n_kv;
+        const int s = u / p.n_kv;
+        const int t0 = (int)((long long)s * pl.ptiles / pl.sp), t1 = (int)((long long)(s + 1) * pl.ptiles / pl.sp);
+        it->slot = p.slots[0];
+        it->row0 = ri * pl.per * pl.rt;
+        it->row_end = p.n * p.n_q * p.group;
+        it->a = t0 * pl.key_tile;
+        it->keys = min(t1 * pl.key_tile, p.prefix) - it->a;
+        it->lim0 = it->keys;
+        it->tok0 = 0;
+        it->part = s;
+        return true;
+    }
+    x -= pre;
+    if (x >= (long long)p.n * pl.cm * p.n_kv * pl.ri_seq) {
+        it->part = -1;
+        return true;
+    }
+    const int ri = (int)(x % pl.ri_seq);
+    x /= pl.ri_seq;
+    it->kvh = (int)(x % p.n_kv);
+    x /= p.n_kv;
+    const int b = (int)(x % p.n), c = (int)(x / p.n);
+    int slot, tiles;
+    const int len = seq_len(pg, p, b, &slot), chunks = own_chunks(p, len, &tiles);
+    if (c >= chunks) return false;
+    const int t0 = (int)((long long)c * tiles / chunks), t1 = (int)((long long)(c + 1) * tiles / chunks);
+    it->slot = slot;
+    it->row0 = (b * p.n_q) * p.group + ri * pl.per * pl.rt;
+    it->row_end = (b + 1) * p.n_q * p.group;
+    it->a = p.prefix + t0 * pl.key_tile;
+    it->keys = min(p.prefix + t1 * pl.key_tile, len) - it->a;
+    it->tok0 = b * p.n_q;
+    it->lim0 = len - p.n_q + 1 - it->a;
+    it->part = pl.sp + c;
+    return true;
+}
+
+__device__ __forceinline__ int row_seen(const PrefixParams& p, const PrefixItem& it, int r) {
+    return min(max(it.lim0 + r / p.group - it.tok0, 0), it.keys);
+}
+
+// a row of q or out: token r / group, head kvh * group + r % group
+__device__ __forceinline__ size_t row_off(const PrefixParams& p, int kvh, int r) {
+    return ((size_t)(r / p.group) * p.n_head + kvh * p.group + r % p.group) * kServeDim;
+}
+
+__device__ __forceinline__ size_t part_at(const PrefixParams& p, const PrefixItem& it, int r) {
+    return ((size_t)it.kvh * p.n * p.n_q * p.group + r) * (p.plan.sp + p.plan.cm) + it.part;
+}
+
+// the page that holds key j of a slot; a wrong one is reported and replaced
+__device__ __forceinline__ int page_of(const PagesDev& pg, const PrefixParams& p, int slot, int index) {
+    int id = -1;
+    if (slot >= 0 && slot < pg.n_slots && index < pg.width) id = pg.tables[(size_t)slot * pg.width + index];
+    if (id < 0 || id >= pg.n_pages) {
+        raise(p.status, SLLM_CUDA_ERR_ARG);
+        id = 0;
+    }
+    return id;
+}
+
+// ---------------------------------------------------------------------------
+// f16 on the tensor cores
+// ---------------------------------------------------------------------------
+struct PrefixWork {
+    using Item = PrefixItem;
+    const PagesDev& pg;
+    const PrefixParams& p;
+    const CUtensorMap &tm_q, &tm_k, &tm_v;
+
+    __device__ __forceinline__ bool find(long long x, Item* it) const { return find_item(pg, p, x, it); }
+    __device__ __forceinline__ int tiles(const Item& it, int t) const {
+        return it.row0 + t * p.plan.rt < it.row_end ? (it.keys + kAtKeys - 1) / kAtKeys : 0;
+    }
+    __device__ __forceinline__ int keys(const Item& it) const { return it.keys; }
+    __device__ __forceinline__ int seen(const Item& it, int t, int row) const {
+        return live(it, t, row) ? row_seen(p, it, it.row0 + t * p.plan.rt + row) : it.keys;
+    }
+    __device__ __forceinline__ bool live(const Item& it, int t, int row) const {
+        return row < p.plan.rt && it.row0 + t * p.plan.rt + row < it.row_end;
+    }
+    // One lane per page of a tile; the ids of 32 pages at a time, the next 32
+    // on their way.
+    struct Loader {
+        int cur, nxt, base;
+        __device__ __forceinline__ int ids(const PrefixWork& w, const Item& it, int at, int lane) {
+            const int pages = (it.keys + w.pg.page - 1) / w.pg.page;
+            return at + lane < pages ? page_of(w.pg, w.p, it.slot, it.a / w.pg.page + at + lane) : 0;
+        }
+        __device__ __forceinline__ void start(const PrefixWork& w, const Item& it, int lane) {
+            base = 0;
+            cur = ids(w, it, 0, lane);
+            nxt = ids(w, it, 32, lane);
+        }
+        __device__ __forceinline__ void q(const PrefixWork& w, const Item& it, int t, uint8_t* dst, uint64_t* bar, int lane) {
+            if (lane == 0) {
+                const int token = it.row0 / w.p.group + t * (w.p.plan.rt / w.p.group);
+                mbar_expect_tx(bar, (uint32_t)w.p.plan.rt * 256u);
+                tma_load_4d(dst, &w.tm_q, 0, 0, it.kvh, token, bar);
+                tma_load_4d(dst + kAtHalf, &w.tm_q, 64, 0, it.kvh, token, bar);
+            }
+        }
+        __device__ __forceinline__ void kv(const PrefixWork& w, const Item& it, int j, bool v, uint8_t* dst, uint64_t* bar,
+                                           int lane) {
+            const int per = kAtKeys / w.pg.page, first = j * per;
+            if (first >= base + 32) {
+                base += 32;
+                cur = nxt;
+                nxt = ids(w, it, base + 32, lane);
+            }
+            const int n = min(per, (it.keys - j * kAtKeys + w.pg.page - 1) / w.pg.page);
+            const int id = __shfl_sync(0xffffffffu, cur, (first - base + lane) & 31);
+            if (lane == 0) mbar_expect_tx(bar, (uint32_t)(n * w.pg.page) * 256u);
+            __syncwarp();
+            if (lane < n) {
+                const CUtensorMap* tm = v ? &w.tm_v : &w.tm_k;
+                uint8_t* at = dst + lane * w.pg.page * 128;
+                tma_load_4d(at, tm, 0, 0, it.kvh, id, bar);
+                tma_load_4d(at + kAtHalf, tm, 64, 0, it.kvh, id, bar);
+            }
+            __syncwarp();
+        }
+    };
+    __device__ __forceinline__ void store(const Item& it, int t, int row, uint32_t o_tm, float m, float l) const {
+        const bool ok = live(it, t, row);
+        const size_t at = ok ? part_at(p, it, it.row0 + t * p.plan.rt + row) : 0;
+        if (ok) p.part_ml[at] = make_float2(m * kServeScale, l);
+        store_row(o_tm, 1.f, ok, p.part_o + at * kServeDim);
+    }
+    // one warp per row, in 32-bit arithmetic
+    __device__ __forceinline__ void slow(const Item& it, int t, int warp) const {
+        const int lane = threadIdx.x & 31;
+        const __half* Q = static_cast<const __half*>(p.q);
+        for (int x = warp; x < p.plan.rt; x += 4) {
+            const int r = it.row0 + t * p.plan.rt + x;
+            if (r >= it.row_end) return;
+            const float4 q = ld4(Q + row_off(p, it.kvh, r) + 4 * lane);
+            float m = -INFINITY, l = 0.f;
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+            const int lim = row_seen(p, it, r);
+            for (int j = 0; j < lim; ++j) {
+                const int id = page_of(pg, p, it.slot, (it.a + j) / pg.page);
+                const size_t at = (size_t)id * p.page_stride +
+                                  ((size_t)it.kvh * pg.page + (it.a + j) % pg.page) * kServeDim + 4 * lane;
+                const float4 k = ld4(static_cast<const __half*>(p.kp) + at), v = ld4(static_cast<const __half*>(p.vp) + at);
+                float s = fmaf(q.x, k.x, fmaf(q.y, k.y, fmaf(q.z, k.z, q.w * k.w)));
+                #pragma unroll
+                for (int y = 16; y > 0; y >>= 1) s += __shfl_xor_sync(0xffffffffu, s, y);
+                s *= kServeScale;
+                const float mn = max3(m, s, s), f = mn == -INFINITY ? 1.f : expf(m - mn);
+                const float e = mn == -INFINITY ? 0.f : expf(s - mn);
+                m = mn;
+                l = fmaf(l, f, e);
+                o.x = fmaf(e, v.x, o.x * f);
+                o.y = fmaf(e, v.y, o.y * f);
+                o.z = fmaf(e, v.z, o.z * f);
+                o.w = fmaf(e, v.w, o.w * f);
+            }
+            const size_t at = part_at(p, it, r);
+            if (lane == 0) p.part_ml[at] = make_float2(m, l);
+            st4(p.part_o + at * kServeDim + 4 * lane, o);
+        }
+    }
+};
+
+__global__ void __launch_bounds__(kAtThreads, 1)
+attn_prefix_mma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                       const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ PagesDev pg,
+                       const __grid_constant__ PrefixParams p) {
+    pdl_trigger();
+    attn_core(PrefixWork{pg, p, tm_q, tm_k, tm_v});
+}
+
+// ---------------------------------------------------------------------------
+// 32-bit: one item per CTA, R rows a thread
+// ---------------------------------------------------------------------------
+template <int R, class T>
+__global__ void __launch_bounds__(kSimtThreads)
+attn_prefix_simt_kernel(const __grid_constant__ PagesDev pg, const __grid_constant__ PrefixParams p) {
+    extern __shared__ float smf[];
+    pdl_trigger();
+    PrefixItem it;
+    if (!find_item(pg, p, blockIdx.x, &it) || it.last()) return;
+    const int r0 = it.row0, ty = threadIdx.x >> 4;
+    simt_load_q<R, T>(smf, [&](int r) -> const T* {
+        return r0 + r < it.row_end ? static_cast<const T*>(p.q) + row_off(p, it.kvh, r0 + r) : nullptr;
+    });
+    SimtState<R> st;
+    simt_init(st);
+    int lim[R];
+    #pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const int r = r0 + R * ty + i;
+        lim[i] = r < it.row_end ? row_seen(p, it, r) : 0;
+    }
+    auto addr = [&](const void* pool, int j) -> const T* {
+        if (j >= it.keys) return nullptr;
+        const int id = page_of(pg, p, it.slot, (it.a + j) / pg.page);
+        return static_cast<const T*>(pool) + (size_t)id * p.page_stride +
+               ((size_t)it.kvh * pg.page + (it.a + j) % pg.page) * kServeDim;
+    };
+    for (int j0 = 0; j0 < it.keys; j0 += kSimtKeys)
+        simt_tile<R, T>(smf, st, j0, lim, [&](int j) { return addr(p.kp, j); }, [&](int j) { return addr(p.vp, j); });
+    const int tx = threadIdx.x & 15;
+    #pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const int r = r0 + R * ty + i;
+        if (r >= it.row_end) continue;
+        const size_t at = part_at(p, it, r);
+        if (tx == 0) p.part_ml[at] = make_float2(st.m[i], st.l[i]);
+        float* o = p.part_o + at * kServeDim;
+        st4(o + 4 * tx, make_float4(st.o[i][0], st.o[i][1], st.o[i][2], st.o[i][3]));
+        st4(o + 64 + 4 * tx, make_float4(st.o[i][4], st.o[i][5], st.o[i][6], st.o[i][7]));
+    }
+}
+
+// ---------------------------------------------------------------------------
+// the join: one warp per row, a lane four dimensions
+// ---------------------------------------------------------------------------
+template <class O>
+__global__ void __launch_bounds__(256)
+attn_prefix_join_kernel(const __grid_constant__ PagesDev pg, const __grid_constant__ PrefixParams p) {
+    const int lane = threadIdx.x & 31;
+    const long long x = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int rows = p.n * p.n_q * p.group;
+    if (x >= (long long)rows * p.n_kv) return;
+    const int kvh = (int)(x / rows), r = (int)(x % rows), b = r / (p.n_q * p.group);
+    int slot, tiles;
+    const int len = seq_len(pg, p, b, &slot), chunks = own_chunks(p, len, &tiles);
+    if (len < 0) {
+        if (lane == 0) raise(p.status, SLLM_CUDA_ERR_ARG);
+        return;
+    }
+    const int parts = p.plan.sp + chunks;
+    pdl_wait();
+    const size_t at = (size_t)x * (p.plan.sp + p.plan.cm);
+    const float2* ml = p.part_ml + at;
+    const float* po = p.part_o + at * kServeDim + 4 * lane;
+    float M = -INFINITY;
+    for (int i = lane; i < parts; i += 32) M = fmaxf(M, ml[i].x);
+    M = warp_max(M);
+    float l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i0 = 0; i0 < parts; i0 += 32) {
+        float f = 0.f, part_l = 0.f;
+        if (i0 + lane < parts) {
+            const float2 v = ml[i0 + lane];
+            f = v.x == -INFINITY ? 0.f : expf(v.x - M);     // a part whose rows saw nothing adds nothing
+            part_l = v.x == -INFINITY ? 0.f : f * v.y;
+        }
+        #pragma unroll
+        for (int y = 16; y > 0; y >>= 1) part_l += __shfl_xor_sync(0xffffffffu, part_l, y);
+        l += part_l;
+        const int n = min(32, parts - i0);
+        #pragma unroll 4
+        for (int i = 0; i < n; ++i) {
+            const float g = __shfl_sync(0xffffffffu, f, i);
+            const float4 v = *reinterpret_cast<const float4*>(po + (size_t)(i0 + i) * kServeDim);
+            if (g != 0.f) {
+                o.x = fmaf(g, v.x, o.x);
+                o.y = fmaf(g, v.y, o.y);
+                o.z = fmaf(g, v.z, o.z);
+                o.w = fmaf(g, v.w, o.w);
+            }
+        }
+    }
+    const float inv = M == -INFINITY && l == 0.f ? 0.f : __fdiv_rn(1.f, l);
+    st4(static_cast<O*>(p.out) + row_off(p, kvh, r) + 4 * lane, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+// The cut. Rows: whole tokens per row tile where TMA gathers them. Splits of
+// the prefix: as many as finish first when each item costs its key tiles plus
+// three for its start and its parts, on one CTA per SM. Chunks of a sequence's
+// own keys: up to two items per SM over all sequences, at most 64 each.
+Plan make_plan(const sllm_cuda_kv_pages& p, int n, int n_q, int n_head, int prefix, int sms) {
+    const int group = n_head / p.n_head_kv, rows = n * n_q * group;
+    const bool mma = p.kv_type == SLLM_CUDA_KV_F16 && group <= kAtRows;
+    Plan pl{};
+    pl.key_tile = mma ? kAtKeys : kSimtKeys;
+    pl.rt = mma ? kAtRows / group * group : rows <= kSimtRows<1> ? kSimtRows<1> : kSimtRows<4>;
+    pl.per = mma ? 2 : 1;
+    auto items = [&](int r) { return (r + pl.rt * pl.per - 1) / (pl.rt * pl.per); };
+    pl.ri_all = items(rows);
+    pl.ri_seq = items(n_q * group);
+    pl.ptiles = (prefix + pl.key_tile - 1) / pl.key_tile;
+    const long long base = (long long)p.n_head_kv * pl.ri_all;
+    long long best = 0;
+    for (int s = 1; s <= 32 && s <= pl.ptiles; ++s) {
+        const long long cost = ((base * s + sms - 1) / sms) * ((pl.ptiles + s - 1) / s + 3);
+        if (pl.sp == 0 || cost < best) {
+            best = cost;
+            pl.sp = s;
+        }
+    }
+    const long long own = (long long)n * p.n_head_kv * pl.ri_seq;
+    const long long cm = own > 0 ? (2LL * sms + own - 1) / own : 1;
+    pl.cm = (int)(cm < 1 ? 1 : cm > 64 ? 64 : cm);
+    return pl;
+}
+
+size_t part_count(const Plan& pl, int n, int n_q, int n_head) {
+    return (size_t)n * n_q * n_head * (pl.sp + pl.cm);
+}
+
+bool encode_q(CUtensorMap* tm, const void* base, int tokens, int n_kv, int group) {
+    PFN_cuTensorMapEncodeTiled_v12000 enc = tensor_map_encoder();
+    if (enc == nullptr) return false;
+    const cuuint64_t row = kServeDim * 2;
+    const cuuint64_t dims[4] = {(cuuint64_t)kServeDim, (cuuint64_t)group, (cuuint64_t)n_kv, (cuuint64_t)tokens};
+    const cuuint64_t strides[3] = {row, row * group, row * group * n_kv};
+    const cuuint32_t box[4] = {64, (cuuint32_t)group, 1, (cuuint32_t)(kAtRows / group)};
+    const cuuint32_t estr[4] = {1, 1, 1, 1};
+    return enc(tm, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// one layer of a pool: a page's rows of one kv head per box
+bool encode_pool(CUtensorMap* tm, const void* base, const sllm_cuda_kv_pages& p) {
+    PFN_cuTensorMapEncodeTiled_v12000 enc = tensor_map_encoder();
+    if (enc == nullptr) return false;
+    const cuuint64_t row = kServeDim * 2, head = row * p.page_size, page = head * p.n_head_kv * p.n_layer;
+    const cuuint64_t dims[4] = {(cuuint64_t)kServeDim, (cuuint64_t)p.page_size, (cuuint64_t)p.n_head_kv,
+                                (cuuint64_t)p.n_pages};
+    const cuuint64_t strides[3] = {row, head, page};
+    const cuuint32_t box[4] = {64, (cuuint32_t)p.page_size, 1, 1};
+    const cuuint32_t estr[4] = {1, 1, 1, 1};
+    return enc(tm, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+long long item_numbers(const PrefixParams& p) {
+    return (long long)p.n_kv * p.plan.ri_all * p.plan.sp + (long long)p.n * p.plan.cm * p.n_kv * p.plan.ri_seq;
+}
+
+cudaError_t launch_mma(const sllm_cuda_kv_pages& pages, const PagesDev& pg, const PrefixParams& p, int sms, cudaStream_t st) {
+    CUtensorMap tq, tk, tv;
+    if (!encode_q(&tq, p.q, p.n * p.n_q, p.n_kv, p.group) || !encode_pool(&tk, p.kp, pages) ||
+        !encode_pool(&tv, p.vp, pages))
+        return cudaErrorInvalidValue;
+    const cudaError_t e = allow_smem<attn_prefix_mma_kernel>(kAtSmem);
     if (e != cudaSuccess) return e;
-    const unsigned z = (unsigned)((p.n_q * p.group + kSimtRows - 1) / kSimtRows);
-    return launch(kern, dim3((unsigned)p.n, (unsigned)p.n_kv, z), dim3(kSimtThreads), kSimtSmem, st, false, pg, p);
+    const long long items = item_numbers(p);
+    return launch(attn_prefix_mma_kernel, dim3((unsigned)(items < sms ? items : sms)), dim3(kAtThreads), kAtSmem, st, false,
+                  tq, tk, tv, pg, p);
+}
+
+template <int R, class T>
+cudaError_t launch_simt(const PagesDev& pg, const PrefixParams& p, cudaStream_t st) {
+    const cudaError_t e = allow_smem<attn_prefix_simt_kernel<R, T>>(kSimtSmem<R>);
+    if (e != cudaSuccess) return e;
+    return launch(attn_prefix_simt_kernel<R, T>, dim3((unsigned)item_numbers(p)), dim3(kSimtThreads), kSimtSmem<R>, st,
+                  false, pg, p);
 }
 
 int check_shape(const sllm_cuda_kv_pages* p, int n, int n_q, int n_head, int prefix, const char* who) {
@@ -96,10 +452,13 @@ int check_shape(const sllm_cuda_kv_pages* p, int n, int n_q, int n_head, int pre
 
 using namespace sllm;
 
+int sllm::take_prefix_error() { return take_attn_error(); }
+
 extern "C" size_t sllm_cuda_attn_prefix_work_bytes(const sllm_cuda_kv_pages* p, int32_t n, int32_t n_q, int32_t n_head,
                                                    int32_t prefix_len) {
     if (check_shape(p, n, n_q, n_head, prefix_len, "attn_prefix_work_bytes") != SLLM_CUDA_OK) return 0;
-    return 16;
+    const size_t parts = part_count(make_plan(*p, n, n_q, n_head, prefix_len, current_sms()), n, n_q, n_head);
+    return parts * (kServeDim * sizeof(float) + sizeof(float2)) + 16;
 }
 
 extern "C" int sllm_cuda_attn_prefix(const sllm_cuda_kv_pages* p, int32_t layer, const void* q, const int32_t* slots,
@@ -133,12 +492,26 @@ extern "C" int sllm_cuda_attn_prefix(const sllm_cuda_kv_pages* p, int32_t layer,
     a.n = n; a.n_q = n_q; a.n_head = n_head; a.n_kv = p->n_head_kv; a.group = n_head / p->n_head_kv;
     a.prefix = prefix_len;
     a.status = status;
+    const int sms = current_sms();
+    a.plan = make_plan(*p, n, n_q, n_head, prefix_len, sms);
+    a.part_o = static_cast<float*>(work);
+    a.part_ml = reinterpret_cast<float2*>(a.part_o + part_count(a.plan, n, n_q, n_head) * kServeDim);
+    if (item_numbers(a) > 0x7fffffffLL) return fail(SLLM_CUDA_ERR_TOO_LARGE, "attn_prefix: %d sequences", n);
     const PagesDev pg = pages_dev(*p);
     const cudaStream_t st = (cudaStream_t)stream;
-    const cudaError_t e = p->kv_type == SLLM_CUDA_KV_F32 ? launch_simt<float, float>(pg, a, st)
-                          : out_type == SLLM_CUDA_KV_F32 ? launch_simt<__half, float>(pg, a, st)
-                                                         : launch_simt<__half, __half>(pg, a, st);
+    const bool few = a.plan.rt == kSimtRows<1>;
+    cudaError_t e;
+    if (p->kv_type == SLLM_CUDA_KV_F32)
+        e = few ? launch_simt<1, float>(pg, a, st) : launch_simt<4, float>(pg, a, st);
+    else if (a.group > kAtRows)
+        e = few ? launch_simt<1, __half>(pg, a, st) : launch_simt<4, __half>(pg, a, st);
+    else
+        e = launch_mma(*p, pg, a, sms, st);
     CK(e, "attn_prefix launch");
-    count_launches(1);
+    const dim3 grid((unsigned)(((long long)n * n_q * n_head + 7) / 8));
+    CK(out_type == SLLM_CUDA_KV_F32 ? launch(attn_prefix_join_kernel<float>, grid, dim3(256), 0, st, true, pg, a)
+                                    : launch(attn_prefix_join_kernel<__half>, grid, dim3(256), 0, st, true, pg, a),
+       "attn_prefix join");
+    count_launches(2);
     return SLLM_CUDA_OK;
 }

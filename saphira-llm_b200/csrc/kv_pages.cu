@@ -16,6 +16,7 @@
 
 #include <cooperative_groups.h>
 
+#include "../../include/sllm_cuda_testing.h"
 #include "serve.cuh"
 
 namespace cg = cooperative_groups;
@@ -558,17 +559,21 @@ int check_call(const sllm_cuda_kv_pages* p, const char* who, int n, const void* 
 }
 
 cudaError_t launch_copies(const sllm_cuda_kv_pages& p, long long most, void* work, int remap, cudaStream_t st) {
-    int dev = 0;
-    cudaGetDevice(&dev);
     const int runs = p.n_layer * p.n_head_kv;
     const long long units = most * 2 * runs + (remap ? p.n_slots : 0);
-    const long long blocks = (units + 7) / 8, cap = 8LL * num_sms_of(dev);
+    const long long blocks = (units + 7) / 8, cap = 8LL * current_sms();
     return launch(kv_copy_kernel, dim3((unsigned)(blocks < 1 ? 1 : blocks < cap ? blocks : cap)), dim3(256), 0, st, true,
                   pages_dev(p), static_cast<uint8_t*>(p.k), static_cast<uint8_t*>(p.v), runs,
                   (int)(kServeDim * kv_elt_bytes(p.kv_type)), work, remap);
 }
 
 }  // namespace
+
+int current_sms() {
+    int dev = 0;
+    cudaGetDevice(&dev);
+    return num_sms_of(dev);
+}
 
 int need_device(const void* p, const char* who, const char* arg) {
     cudaPointerAttributes at{};
@@ -604,6 +609,12 @@ int check_pages(const sllm_cuda_kv_pages* p, const char* who) {
 }  // namespace sllm
 
 using namespace sllm;
+
+extern "C" int sllm_cuda_test_attn_error(void) {
+    if (cudaDeviceSynchronize() != cudaSuccess) return -1;
+    const int a = take_prompt_error(), b = take_prefix_error();
+    return a != 0 ? a : b;
+}
 
 extern "C" size_t sllm_cuda_kv_work_bytes(const sllm_cuda_kv_pages* p) {
     if (check_pages(p, "kv_work_bytes") != SLLM_CUDA_OK) return 0;

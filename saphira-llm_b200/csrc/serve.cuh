@@ -3,6 +3,7 @@
 // device's view of a paged cache, launches.
 #pragma once
 
+#include <atomic>
 #include <cuda_runtime.h>
 #include <cuda_fp16.h>
 
@@ -19,6 +20,26 @@ int need_device(const void* p, const char* who, const char* arg);
 
 // the fields of a sllm_cuda_kv_pages, checked (no device call)
 int check_pages(const sllm_cuda_kv_pages* p, const char* who);
+
+// the error words of the attention kernels' bounded waits, read and cleared
+int take_prompt_error();
+int take_prefix_error();
+
+int current_sms();
+
+// the kernel's shared-memory limit, set once per device
+template <auto Kernel>
+cudaError_t allow_smem(int bytes) {
+    static std::atomic<unsigned long long> done{0};
+    int dev = 0;
+    const cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const unsigned long long bit = dev < 64 ? 1ull << dev : 0;
+    if (bit != 0 && (done.load(std::memory_order_relaxed) & bit) != 0) return cudaSuccess;
+    const cudaError_t r = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (r == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    return r;
+}
 
 struct PagesDev {
     int32_t* refs;
