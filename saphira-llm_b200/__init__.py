@@ -247,37 +247,50 @@ def gemm_error():
 
 # attention, paged cache and drafts (device arrays, asynchronous) ---------------
 # These take torch CUDA tensors (or any array object with the same shape,
-# stride(), dtype and data_ptr()) and read sizes, types and strides from them.
+# stride(), dtype, is_contiguous() and data_ptr()) and read sizes, types and
+# strides from them. A decode step makes several such calls per layer, so they
+# ask each array for each attribute once.
+_DTYPES = {}            # dtype object -> "f32", "f16", "i32" or ""
+
+
+def _kind(dtype):
+    kind = _DTYPES.get(dtype)
+    if kind is None:
+        name = str(dtype).rpartition(".")[2]
+        kind = _DTYPES[dtype] = {"float32": "f32", "float16": "f16", "int32": "i32"}.get(name, "")
+    return kind
+
+
+_FLOATS = {"f32": abi.KV_F32, "f16": abi.KV_F16}
+
+
 def _type(t):
-    name = str(t.dtype)
-    if name.endswith("float16") and "bfloat" not in name:
-        return abi.KV_F16
-    if name.endswith("float32"):
-        return abi.KV_F32
-    raise TypeError(f"dtype {t.dtype}: float32 or float16 expected")
-
-
-def _expect(ok, where, what):
-    if not ok:
-        raise ValueError(f"{where}: {what}")
+    kind = _FLOATS.get(_kind(t.dtype))
+    if kind is None:
+        raise TypeError(f"dtype {t.dtype}: float32 or float16 expected")
+    return kind
 
 
 def _ints(t, n, where, name):
-    """An int32 array of n elements, or None."""
-    if t is not None:
-        _expect(str(t.dtype).endswith("int32") and t.is_contiguous() and t.numel() >= n, where,
-                f"{name} must be {n} contiguous int32 values")
-    return _ptr(t)
+    """The address of an int32 array of at least n elements, or None."""
+    if t is None:
+        return None
+    if _kind(t.dtype) != "i32" or not t.is_contiguous() or t.numel() < n:
+        raise ValueError(f"{where}: {name} must be {n} contiguous int32 values")
+    return t.data_ptr()
 
 
 def _heads(t, where, name):
     """(address, token stride, tokens, heads) of a [tokens][heads][128] array
     whose heads lie together; tokens may be apart."""
-    _expect(t.dim() == 3 and t.shape[2] == abi.HEAD_DIM, where, f"{name} must be [tokens][heads][128]")
-    n, h = int(t.shape[0]), int(t.shape[1])
-    _expect(n == 0 or (t.stride(2) == 1 and (h == 1 or t.stride(1) == abi.HEAD_DIM)), where,
-            f"the heads of a token of {name} must lie together")
-    return _ptr(t), (t.stride(0) if n > 1 else h * abi.HEAD_DIM), n, h
+    shape = t.shape
+    if len(shape) != 3 or shape[2] != abi.HEAD_DIM:
+        raise ValueError(f"{where}: {name} must be [tokens][heads][128]")
+    n, h, _ = shape
+    s0, s1, s2 = t.stride()
+    if n > 0 and (s2 != 1 or (h > 1 and s1 != abi.HEAD_DIM)):
+        raise ValueError(f"{where}: the heads of a token of {name} must lie together")
+    return t.data_ptr(), s0 if n > 1 else h * abi.HEAD_DIM, n, h
 
 
 def attn_prompt(q, k, v, out, cu_seqlens, stream=None):
@@ -285,15 +298,22 @@ def attn_prompt(q, k, v, out, cu_seqlens, stream=None):
     q, out [tokens][heads][128], k, v [tokens][kv heads][128], cu_seqlens
     int32 [sequences + 1]."""
     w = "attn_prompt"
-    (qp, qs, n, h), (kp, ks, nk, hk) = _heads(q, w, "q"), _heads(k, w, "k")
-    (vp_, vs, nv, hv), (op, os_, no, ho) = _heads(v, w, "v"), _heads(out, w, "out")
-    _expect(n == nk == nv == no and h == ho and hk == hv, w, "q, k, v and out disagree in tokens or heads")
-    _expect(_type(q) == _type(k) == _type(v), w, "q, k and v must have one type")
+    qp, qs, n, h = _heads(q, w, "q")
+    kp, ks, nk, hk = _heads(k, w, "k")
+    vp, vs, nv, hv = _heads(v, w, "v")
+    op, os_, no, ho = _heads(out, w, "out")
+    if not (n == nk == nv == no and h == ho and hk == hv):
+        raise ValueError("attn_prompt: q, k, v and out disagree in tokens or heads")
+    t = _type(q)
+    if not t == _type(k) == _type(v):
+        raise ValueError("attn_prompt: q, k and v must have one type")
+    cp = _ints(cu_seqlens, 1, w, "cu_seqlens")
     if n == 0:
         return
-    n_seq = cu_seqlens.numel() - 1
-    _check(lib().sllm_cuda_attn_prompt(qp, qs, kp, ks, vp_, vs, _type(q), _ints(cu_seqlens, 1, w, "cu_seqlens"), n_seq, n,
-                                       h, hk, op, os_, _type(out), _stream(stream)), w)
+    rc = lib().sllm_cuda_attn_prompt(qp, qs, kp, ks, vp, vs, t, cp, cu_seqlens.numel() - 1, n, h, hk, op, os_, _type(out),
+                                     _stream(stream))
+    if rc:
+        _check(rc, w)
 
 
 def rope_table(n_ctx, base):
@@ -311,15 +331,17 @@ class KvPages:
 
     def __init__(self, k, v, refs, tables, lens):
         w = "KvPages"
-        _expect(k.dim() == 5 and k.shape == v.shape and k.shape[4] == abi.HEAD_DIM and k.is_contiguous() and
-                v.is_contiguous() and _type(k) == _type(v), w, "k and v must be [pages][layers][heads][size][128]")
-        _expect(tables.dim() == 2 and tables.shape[0] == lens.numel() and refs.numel() == k.shape[0], w,
-                "refs, tables and lens must match the pools and each other")
+        if not (k.dim() == 5 and k.shape == v.shape and k.shape[4] == abi.HEAD_DIM and k.is_contiguous() and
+                v.is_contiguous() and _type(k) == _type(v)):
+            raise ValueError("KvPages: k and v must be [pages][layers][heads][size][128]")
+        if not (tables.dim() == 2 and tables.shape[0] == lens.numel() and refs.numel() == k.shape[0]):
+            raise ValueError("KvPages: refs, tables and lens must match the pools and each other")
         self._keep = (k, v, refs, tables, lens)
-        self.c = abi.KvPages(_ptr(k), _ptr(v), _ints(refs, refs.numel(), w, "refs"),
+        self.c = abi.KvPages(k.data_ptr(), v.data_ptr(), _ints(refs, refs.numel(), w, "refs"),
                              _ints(tables, tables.numel(), w, "tables"), _ints(lens, lens.numel(), w, "lens"),
                              k.shape[0], k.shape[1], k.shape[2], k.shape[3], tables.shape[0], tables.shape[1], _type(k))
         self._p = C.byref(self.c)
+        self._kv_type, self._kv_heads = self.c.kv_type, self.c.n_head_kv
 
     def _bytes(self, n, where):
         if n == 0:
@@ -330,50 +352,67 @@ class KvPages:
         return self._bytes(lib().sllm_cuda_kv_work_bytes(self._p), "kv_work_bytes")
 
     def fork(self, src, dst, work, status=None, stream=None):
-        n = dst.numel()
-        _expect(src.numel() == n, "kv_fork", "src and dst differ in length")
-        _check(lib().sllm_cuda_kv_fork(self._p, _ints(src, n, "kv_fork", "src"), _ints(dst, n, "kv_fork", "dst"), n,
-                                       _ptr(work), work.nbytes, _ints(status, 1, "kv_fork", "status"),
-                                       _stream(stream)), "kv_fork")
+        w, n = "kv_fork", dst.numel()
+        if src.numel() != n:
+            raise ValueError("kv_fork: src and dst differ in length")
+        rc = lib().sllm_cuda_kv_fork(self._p, _ints(src, n, w, "src"), _ints(dst, n, w, "dst"), n, work.data_ptr(),
+                                     work.nbytes, _ints(status, 1, w, "status"), _stream(stream))
+        if rc:
+            _check(rc, w)
 
     def reserve(self, slots, n_new, work, status=None, stream=None):
-        n = slots.numel()
-        _expect(n_new.numel() == n, "kv_reserve", "slots and n_new differ in length")
-        _check(lib().sllm_cuda_kv_reserve(self._p, _ints(slots, n, "kv_reserve", "slots"),
-                                          _ints(n_new, n, "kv_reserve", "n_new"), n, _ptr(work), work.nbytes,
-                                          _ints(status, 1, "kv_reserve", "status"), _stream(stream)), "kv_reserve")
+        w, n = "kv_reserve", slots.numel()
+        if n_new.numel() != n:
+            raise ValueError("kv_reserve: slots and n_new differ in length")
+        rc = lib().sllm_cuda_kv_reserve(self._p, _ints(slots, n, w, "slots"), _ints(n_new, n, w, "n_new"), n,
+                                        work.data_ptr(), work.nbytes, _ints(status, 1, w, "status"), _stream(stream))
+        if rc:
+            _check(rc, w)
 
     def release(self, slots, new_len, work, status=None, stream=None):
-        n = slots.numel()
-        _expect(new_len is None or new_len.numel() == n, "kv_release", "slots and new_len differ in length")
-        _check(lib().sllm_cuda_kv_release(self._p, _ints(slots, n, "kv_release", "slots"),
-                                          _ints(new_len, n, "kv_release", "new_len"), n, _ptr(work), work.nbytes,
-                                          _ints(status, 1, "kv_release", "status"), _stream(stream)), "kv_release")
+        w, n = "kv_release", slots.numel()
+        if new_len is not None and new_len.numel() != n:
+            raise ValueError("kv_release: slots and new_len differ in length")
+        rc = lib().sllm_cuda_kv_release(self._p, _ints(slots, n, w, "slots"), _ints(new_len, n, w, "new_len"), n,
+                                        work.data_ptr(), work.nbytes, _ints(status, 1, w, "status"), _stream(stream))
+        if rc:
+            _check(rc, w)
 
     def compact(self, work, status=None, stream=None):
-        _check(lib().sllm_cuda_kv_compact(self._p, _ptr(work), work.nbytes, _ints(status, 1, "kv_compact", "status"),
-                                          _stream(stream)), "kv_compact")
+        rc = lib().sllm_cuda_kv_compact(self._p, work.data_ptr(), work.nbytes, _ints(status, 1, "kv_compact", "status"),
+                                        _stream(stream))
+        if rc:
+            _check(rc, "kv_compact")
 
     def append(self, layer, slot, pos, q, k, v, cos, sin, q_out=None, k_out=None, v_out=None, status=None,
                stream=None):
         w = "kv_append"
         kp, ks, n, hk = _heads(k, w, "k")
-        vp_, vs, nv, hv = _heads(v, w, "v")
+        vp, vs, nv, hv = _heads(v, w, "v")
         qp, qs, nq, h = _heads(q, w, "q") if q is not None else (None, 0, n, 0)
-        _expect(n == nv == nq and hk == hv == self.c.n_head_kv, w, "q, k, v disagree in tokens, or with the cache's heads")
-        _expect((q is None) == (q_out is None), w, "q and q_out go together")
-        for t in (q, k, v, cos, sin):
-            _expect(t is None or _type(t) == abi.KV_F32, w, "q, k, v, cos and sin must be float32")
+        if not (n == nv == nq and hk == hv == self._kv_heads):
+            raise ValueError("kv_append: q, k, v disagree in tokens, or with the cache's heads")
+        if (q is None) != (q_out is None):
+            raise ValueError("kv_append: q and q_out go together")
+        if not (_kind(k.dtype) == _kind(v.dtype) == _kind(cos.dtype) == _kind(sin.dtype) == "f32") or (
+                q is not None and _kind(q.dtype) != "f32"):
+            raise ValueError("kv_append: q, k, v, cos and sin must be float32")
+        outs = []
         for t, m in ((q_out, h), (k_out, hk), (v_out, hk)):
-            _expect(t is None or (t.is_contiguous() and tuple(t.shape) == (n, m, abi.HEAD_DIM) and
-                                  _type(t) == self.c.kv_type), w, "outputs must be contiguous, of the cache's type")
-        _expect(cos.is_contiguous() and sin.is_contiguous() and cos.shape == sin.shape and cos.shape[1] == 64, w,
-                "cos and sin must be [positions][64]")
+            if t is not None and (not t.is_contiguous() or t.shape != (n, m, abi.HEAD_DIM) or
+                                  _type(t) != self._kv_type):
+                raise ValueError("kv_append: outputs must be contiguous, of the cache's type")
+            outs.append(None if t is None else t.data_ptr())
+        if not (cos.is_contiguous() and sin.is_contiguous() and cos.shape == sin.shape and cos.dim() == 2 and
+                cos.shape[1] == 64):
+            raise ValueError("kv_append: cos and sin must be [positions][64]")
         if n == 0:
             return
-        _check(lib().sllm_cuda_kv_append(self._p, layer, n, _ints(slot, n, w, "slot"), _ints(pos, n, w, "pos"), h, qp, qs,
-                                         kp, ks, vp_, vs, _ptr(cos), _ptr(sin), cos.shape[0], _ptr(q_out), _ptr(k_out),
-                                         _ptr(v_out), _ints(status, 1, w, "status"), _stream(stream)), w)
+        rc = lib().sllm_cuda_kv_append(self._p, layer, n, _ints(slot, n, w, "slot"), _ints(pos, n, w, "pos"), h, qp, qs,
+                                       kp, ks, vp, vs, cos.data_ptr(), sin.data_ptr(), cos.shape[0], *outs,
+                                       _ints(status, 1, w, "status"), _stream(stream))
+        if rc:
+            _check(rc, w)
 
     def attn_prefix_work_bytes(self, n, n_q, n_head, prefix_len):
         return self._bytes(lib().sllm_cuda_attn_prefix_work_bytes(self._p, n, n_q, n_head, prefix_len),
@@ -381,35 +420,44 @@ class KvPages:
 
     def attn_prefix(self, layer, q, out, slots, prefix_len, work, status=None, stream=None):
         """q, out [sequences][query tokens][heads][128]."""
-        w = "attn_prefix"
-        _expect(q.dim() == 4 and q.shape == out.shape and q.shape[3] == abi.HEAD_DIM and q.is_contiguous() and
-                out.is_contiguous() and _type(q) == self.c.kv_type, w,
-                "q and out must be contiguous [sequences][query tokens][heads][128], q of the cache's type")
-        n, nq, h = int(q.shape[0]), int(q.shape[1]), int(q.shape[2])
+        w, shape = "attn_prefix", q.shape
+        if not (len(shape) == 4 and shape == out.shape and shape[3] == abi.HEAD_DIM and q.is_contiguous() and
+                out.is_contiguous() and _type(q) == self._kv_type):
+            raise ValueError("attn_prefix: q and out must be contiguous [sequences][query tokens][heads][128], "
+                             "q of the cache's type")
+        n, nq, h, _ = shape
         if n == 0:
             return
-        _check(lib().sllm_cuda_attn_prefix(self._p, layer, _ptr(q), _ints(slots, n, w, "slots"), n, nq, h, prefix_len,
-                                           _ptr(out), _type(out), _ptr(work), work.nbytes,
-                                           _ints(status, 1, w, "status"), _stream(stream)), w)
+        rc = lib().sllm_cuda_attn_prefix(self._p, layer, q.data_ptr(), _ints(slots, n, w, "slots"), n, nq, h, prefix_len,
+                                         out.data_ptr(), _type(out), work.data_ptr(), work.nbytes,
+                                         _ints(status, 1, w, "status"), _stream(stream))
+        if rc:
+            _check(rc, w)
 
 
 def spec_verify(p, q, draft, n_draft, u_accept, u_draw, tokens, count, status=None, stream=None):
     """sllm_cuda_spec_verify: p [n][k + 1][vocab], q [n][k][vocab] or None,
     draft int32 [n][k], n_draft int32 [n] or None, uniforms [n][k] and [n];
     tokens int32 [n][k + 1] and count int32 [n] are written."""
-    w = "spec_verify"
-    _expect(p.dim() == 3 and p.is_contiguous() and _type(p) == abi.KV_F32 and draft.dim() == 2, w,
-            "p must be contiguous float32 [n][k + 1][vocab], draft [n][k]")
-    n, k, nv = int(p.shape[0]), int(p.shape[1]) - 1, int(p.shape[2])
-    _expect(tuple(draft.shape) == (n, k) and (q is None or (tuple(q.shape) == (n, k, nv) and q.is_contiguous() and
-                                                            _type(q) == abi.KV_F32)), w, "draft or q do not match p")
+    w, shape = "spec_verify", p.shape
+    if not (len(shape) == 3 and p.is_contiguous() and _kind(p.dtype) == "f32"):
+        raise ValueError("spec_verify: p must be contiguous float32 [n][k + 1][vocab]")
+    n, k, nv = shape
+    k -= 1
+    if draft.shape != (n, k) or (q is not None and (q.shape != (n, k, nv) or not q.is_contiguous() or
+                                                    _kind(q.dtype) != "f32")):
+        raise ValueError("spec_verify: draft or q do not match p")
     for t, m in ((u_accept, n * k), (u_draw, n)):
-        _expect(t.is_contiguous() and t.numel() == m and _type(t) == abi.KV_F32, w, "uniforms must be float32 [n][k], [n]")
+        if not (t.is_contiguous() and t.numel() == m and _kind(t.dtype) == "f32"):
+            raise ValueError("spec_verify: uniforms must be float32 [n][k], [n]")
     if n == 0:
         return
-    _check(lib().sllm_cuda_spec_verify(_ptr(p), _ptr(q), _ints(draft, n * k, w, "draft"), _ints(n_draft, n, w, "n_draft"),
-                                       _ptr(u_accept), _ptr(u_draw), n, k, nv, _ints(tokens, n * (k + 1), w, "tokens"),
-                                       _ints(count, n, w, "count"), _ints(status, 1, w, "status"), _stream(stream)), w)
+    rc = lib().sllm_cuda_spec_verify(p.data_ptr(), None if q is None else q.data_ptr(), _ints(draft, n * k, w, "draft"),
+                                     _ints(n_draft, n, w, "n_draft"), u_accept.data_ptr(), u_draw.data_ptr(), n, k, nv,
+                                     _ints(tokens, n * (k + 1), w, "tokens"), _ints(count, n, w, "count"),
+                                     _ints(status, 1, w, "status"), _stream(stream))
+    if rc:
+        _check(rc, w)
 
 
 def attn_error():

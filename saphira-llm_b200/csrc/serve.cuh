@@ -27,19 +27,24 @@ int take_prefix_error();
 
 int current_sms();
 
-// the kernel's shared-memory limit, set once per device
-template <auto Kernel>
-cudaError_t allow_smem(int bytes) {
+// an attribute of a kernel, set once per device
+template <auto Kernel, cudaFuncAttribute Attr>
+cudaError_t set_once(int value) {
     static std::atomic<unsigned long long> done{0};
     int dev = 0;
     const cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     const unsigned long long bit = dev < 64 ? 1ull << dev : 0;
     if (bit != 0 && (done.load(std::memory_order_relaxed) & bit) != 0) return cudaSuccess;
-    const cudaError_t r = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    const cudaError_t r = cudaFuncSetAttribute(Kernel, Attr, value);
     if (r == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
     return r;
 }
+template <auto Kernel>
+cudaError_t allow_smem(int bytes) { return set_once<Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize>(bytes); }
+// clusters of 16 CTAs
+template <auto Kernel>
+cudaError_t allow_cluster() { return set_once<Kernel, cudaFuncAttributeNonPortableClusterSizeAllowed>(1); }
 
 struct PagesDev {
     int32_t* refs;

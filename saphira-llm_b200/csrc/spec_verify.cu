@@ -9,11 +9,15 @@
 // that lies that close to a border.
 //
 // One cluster of CTAs per sequence, each warp a contiguous run of the
-// vocabulary: one pass over the two rows gives each warp its sums of p and
-// of max(p - q, 0) (the second may have no mass, then p stands in), the
-// cluster exchanges its CTAs' sums through distributed shared memory, and the
-// one warp whose run holds the draw walks it again (from L2). Bound by HBM
-// for many sequences and by this chain of dependent steps for one.
+// vocabulary. One pass over the two rows gives each warp its sum; the cluster
+// exchanges its CTAs' sums through distributed shared memory, and the CTA whose
+// run holds the draw walks that run again.
+// What is rare costs another pass: a residual without mass (p stands in), and
+// infinities, which count as nothing.
+//
+// Bound: HBM for many sequences (64 of 128256 words: 10 us for the two rows
+// that each needs); for one, the chain of dependent reads: lengths and tokens,
+// their probabilities, the rows, the run again.
 
 #include <cooperative_groups.h>
 
@@ -24,7 +28,7 @@ namespace cg = cooperative_groups;
 namespace sllm {
 namespace {
 
-constexpr int kSvThreads = 512;
+constexpr int kSvThreads = 256;
 constexpr int kSvWarps = kSvThreads / 32;
 constexpr int kSvMaxDraft = 64;
 
@@ -42,42 +46,141 @@ struct VerifyParams {
 };
 
 // what an entry counts for: nothing when negative, NaN or infinite
-__device__ __forceinline__ double mass(double x) { return x > 0.0 && x < INFINITY ? x : 0.0; }
-
 __device__ __forceinline__ float prob(float x) { return x > 0.0f && x < INFINITY ? x : 0.0f; }
-
-struct Pair2 {
-    double res, all;
-};
 
 template <bool VEC>
 __device__ __forceinline__ float4 row4(const float* row, int i, int hi) {
-    if (row == nullptr) return make_float4(0.f, 0.f, 0.f, 0.f);
+    if (row == nullptr || i >= hi) return make_float4(0.f, 0.f, 0.f, 0.f);
     if (VEC && i + 4 <= hi) return __ldg(reinterpret_cast<const float4*>(row + i));
     float4 r;
-    r.x = i < hi ? __ldg(row + i) : 0.f;
+    r.x = __ldg(row + i);
     r.y = i + 1 < hi ? __ldg(row + i + 1) : 0.f;
     r.z = i + 2 < hi ? __ldg(row + i + 2) : 0.f;
     r.w = i + 3 < hi ? __ldg(row + i + 3) : 0.f;
     return r;
 }
 
-// the mass of index i: p alone, p - q, or p without the refused token
-__device__ __forceinline__ double mass_at(float p, float q, int i, int refused, bool point, bool residual) {
-    const double a = (double)prob(p);
-    if (!residual || refused < 0) return a;
-    if (point) return i == refused ? 0.0 : a;
-    return mass(a - (double)prob(q));
+// the distribution that is drawn from
+struct Draw {
+    const float* p;
+    const float* q;                 // NULL: nothing is subtracted
+    int skip;                       // an index without mass (the refused token of a certain draft), or -1
+};
+
+__device__ __forceinline__ double mass_at(const Draw& d, float p, float q, int i) {
+    if (i == d.skip) return 0.0;
+    const float a = prob(p), b = prob(q);
+    return a > b ? (double)a - (double)b : 0.0;
+}
+
+// the sum over [lo, hi) by one warp. Quick: negatives and NaN count as
+// nothing; an infinity comes out as a sum that is not finite, or in *odd.
+template <bool VEC, bool QUICK>
+__device__ __forceinline__ double run_sum(const Draw& d, int lo, int hi, bool* odd) {
+    const int lane = threadIdx.x & 31;
+    double s0 = 0.0, s1 = 0.0;
+    float top = 0.f;
+    for (int i0 = lo; i0 < hi; i0 += 512) {
+        float4 pv[4], qv[4];
+        #pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int i = i0 + 128 * j + 4 * lane;
+            pv[j] = row4<VEC>(d.p, i, hi);
+            qv[j] = row4<VEC>(d.q, i, hi);
+        }
+        #pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int i = i0 + 128 * j + 4 * lane;
+            const float pe[4] = {pv[j].x, pv[j].y, pv[j].z, pv[j].w};
+            const float qe[4] = {qv[j].x, qv[j].y, qv[j].z, qv[j].w};
+            #pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                double m;
+                if (QUICK) {
+                    const float a = i + e == d.skip ? 0.f : fmaxf(pe[e], 0.f);
+                    const float b = fmaxf(qe[e], 0.f);
+                    top = fmaxf(top, b);
+                    m = (double)a - (double)fminf(a, b);        // exact where a <= b: 0
+                } else {
+                    m = mass_at(d, pe[e], qe[e], i + e);
+                }
+                if (e & 1) s1 += m;
+                else s0 += m;
+            }
+        }
+    }
+    if (QUICK) *odd = __any_sync(0xffffffffu, top == INFINITY);
+    return warp_sum_d(s0 + s1);
+}
+
+// the last index with mass below hi, by one warp; -1 when there is none
+template <bool VEC>
+__device__ __noinline__ int last_mass(const Draw& d, int hi) {
+    const int lane = threadIdx.x & 31;
+    for (int i0 = (hi - 1) & ~31; i0 >= 0; i0 -= 32) {
+        const int i = i0 + lane;
+        const bool has = i < hi && mass_at(d, d.p[i], d.q != nullptr ? d.q[i] : 0.f, i) > 0.0;
+        const unsigned any = __ballot_sync(0xffffffffu, has);
+        if (any != 0) return i0 + 31 - __clz(any);
+    }
+    return -1;
+}
+
+// the first index of [lo, hi) with mass whose running sum, from `before`,
+// exceeds target, by one warp; -1 when the sums' rounding leaves none
+template <bool VEC>
+__device__ __forceinline__ int find_in_run(const Draw& d, int lo, int hi, double before, double target) {
+    const int lane = threadIdx.x & 31;
+    const int per = ((hi - lo + 31) / 32 + 3) & ~3, a = min(lo + lane * per, hi), z = min(a + per, hi);
+    double own = 0.0;
+    #pragma unroll 4
+    for (int i = a; i < z; i += 4) {
+        const float4 pv = row4<VEC>(d.p, i, z), qv = row4<VEC>(d.q, i, z);
+        own += (mass_at(d, pv.x, qv.x, i) + mass_at(d, pv.y, qv.y, i + 1)) +
+               (mass_at(d, pv.z, qv.z, i + 2) + mass_at(d, pv.w, qv.w, i + 3));
+    }
+    double x = own;
+    #pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const double y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+    }
+    // lanes from the first that may hold it: a border that rounding moved
+    // across a lane's end is found by the next one
+    const unsigned may = __ballot_sync(0xffffffffu, own > 0.0 && before + x > target);
+    if (may == 0) return -1;
+    const int l = __ffs(may) - 1;
+    int found = -1;
+    if (lane == l) {
+        double run = before + (x - own);
+        int last = -1;
+        #pragma unroll 2
+        for (int i = a; i < z && found < 0; i += 4) {
+            const float4 pv = row4<VEC>(d.p, i, z), qv = row4<VEC>(d.q, i, z);
+            const float pe[4] = {pv.x, pv.y, pv.z, pv.w}, qe[4] = {qv.x, qv.y, qv.z, qv.w};
+            #pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const double m = mass_at(d, pe[e], qe[e], i + e);
+                run += m;
+                if (found < 0 && m > 0.0) {         // an entry without mass is never drawn
+                    last = i + e;
+                    if (run > target) found = i + e;
+                }
+            }
+        }
+        if (found < 0) found = last;
+    }
+    return __shfl_sync(0xffffffffu, found, l);
 }
 
 template <bool VEC>
-__global__ void __launch_bounds__(kSvThreads)
+__global__ void __launch_bounds__(kSvThreads, 4)
 spec_verify_kernel(const __grid_constant__ VerifyParams a) {
     cg::cluster_group cl = cg::this_cluster();
     const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank();
     const int b = blockIdx.x / C, t = threadIdx.x, lane = t & 31, warp = t >> 5;
-    __shared__ double s_res[kSvWarps], s_all[kSvWarps], cta_res, cta_all;
-    __shared__ int first_refusal, s_last_res[kSvWarps], s_last_all[kSvWarps], cta_last_res, cta_last_all;
+    __shared__ double s_sum[kSvWarps], cta_sum;
+    __shared__ int first_refusal, s_odd, cta_odd;
     const int V = a.V, k = a.k;
     const int nd_raw = a.n_draft != nullptr ? a.n_draft[b] : k;
     const int nd = min(max(nd_raw, 0), k);
@@ -88,164 +191,120 @@ spec_verify_kernel(const __grid_constant__ VerifyParams a) {
     __syncthreads();
     const float* P = a.p + (size_t)b * (k + 1) * V;
     const float* Q = a.q != nullptr ? a.q + (size_t)b * k * V : nullptr;
-    for (int i = t; i < nd; i += kSvThreads) {
-        const int x = a.draft[(size_t)b * k + i];
+    if (t < nd) {
+        const int x = a.draft[(size_t)b * k + t];
         bool ok = false;
         if (x >= 0 && x < V) {
-            const double px = (double)prob(P[(size_t)i * V + x]);
-            const double qx = Q != nullptr ? (double)prob(Q[(size_t)i * V + x]) : 1.0;
-            ok = (double)a.u_accept[(size_t)b * k + i] * qx < px;     // exact in 64 bits
+            const double px = (double)prob(P[(size_t)t * V + x]);
+            const double qx = Q != nullptr ? (double)prob(Q[(size_t)t * V + x]) : 1.0;
+            ok = (double)a.u_accept[(size_t)b * k + t] * qx < px;     // exact in 64 bits
         } else if (rank == 0) {
             raise(a.status, SLLM_CUDA_ERR_ARG);                       // no such token: refused
         }
-        if (!ok) atomicMin(&first_refusal, i);
+        if (!ok) atomicMin(&first_refusal, t);
     }
     __syncthreads();
     const int r = first_refusal;
-    // the refused token (V: one that is no token), -1 when none was refused
-    int refused = -1;
-    if (r < nd) {
-        const int x = a.draft[(size_t)b * k + r];
-        refused = x >= 0 && x < V ? x : V;
+    Draw d{P + (size_t)r * V, nullptr, -1};
+    bool residual = r < nd;
+    if (residual) {
+        if (Q != nullptr) d.q = Q + (size_t)r * V;
+        else d.skip = a.draft[(size_t)b * k + r];
     }
-    const bool point = Q == nullptr;
-    const float* prow = P + (size_t)r * V;
-    const float* qrow = refused >= 0 && !point ? Q + (size_t)r * V : nullptr;
-
     // this warp's run: a multiple of 128 indices, so that a step of the warp
     // reads 512 contiguous bytes
-    const int runs = C * kSvWarps;
-    const int per = ((V + runs - 1) / runs + 127) / 128 * 128;
-    const long long lo_l = (long long)(rank * kSvWarps + warp) * per;
-    const int lo = (int)(lo_l < V ? lo_l : V), hi = min((long long)V, lo_l + per) > lo ? (int)min((long long)V, lo_l + per) : lo;
-    Pair2 sum{0.0, 0.0};
-    int last_res = -1, last_all = -1;
-    for (int i0 = lo; i0 < hi; i0 += 512) {
-        float4 pv[4], qv[4];
-        #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int i = i0 + 128 * j + 4 * lane;
-            pv[j] = row4<VEC>(i < hi ? prow : nullptr, i, hi);
-            qv[j] = row4<VEC>(i < hi ? qrow : nullptr, i, hi);
+    const int per = ((V + C * kSvWarps - 1) / (C * kSvWarps) + 127) / 128 * 128;
+    const int lo = (int)min((long long)(rank * kSvWarps + warp) * per, (long long)V), hi = min(V, lo + min(per, V - lo));
+    double total, before = 0.0, target;
+    int owner;
+    for (bool quick = true;;) {
+        bool odd = false;
+        const double sum = quick ? run_sum<VEC, true>(d, lo, hi, &odd) : run_sum<VEC, false>(d, lo, hi, &odd);
+        if (t == 0) s_odd = 0;
+        __syncthreads();
+        if (lane == 0) {
+            s_sum[warp] = sum;
+            if (odd) s_odd = 1;
         }
+        __syncthreads();
+        if (t == 0) {
+            double x = 0.0;
+            for (int w = 0; w < kSvWarps; ++w) x += s_sum[w];
+            cta_sum = x;
+            cta_odd = s_odd;
+        }
+        cl.sync();
+        // every warp adds the CTAs' sums in the same way, a lane per CTA, and
+        // finds the one that holds the draw
+        const double part = lane < C ? *cl.map_shared_rank(&cta_sum, lane) : 0.0;
+        const bool odds = __any_sync(0xffffffffu, lane < C && *cl.map_shared_rank(&cta_odd, lane) != 0);
+        double upto = part;
         #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int i = i0 + 128 * j + 4 * lane;
-            const float pe[4] = {pv[j].x, pv[j].y, pv[j].z, pv[j].w};
-            const float qe[4] = {qv[j].x, qv[j].y, qv[j].z, qv[j].w};
-            #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const double all = (double)prob(pe[e]);
-                const double res = mass_at(pe[e], qe[e], i + e, refused, point, true);
-                sum.all += all;
-                sum.res += res;
-                if (all > 0.0) last_all = i + e;
-                if (res > 0.0) last_res = i + e;
+        for (int o = 1; o < 16; o <<= 1) {
+            const double y = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += y;
+        }
+        total = __shfl_sync(0xffffffffu, upto, C - 1);
+        target = fmax((double)a.u_draw[b], 0.0) * total;
+        const unsigned hit = __ballot_sync(0xffffffffu, part > 0.0 && upto > target);
+        owner = __ffs(hit) - 1;
+        before = __shfl_sync(0xffffffffu, upto - part, max(owner, 0));
+        cl.sync();                  // remote reads done: the sums may be replaced, a CTA may leave
+        if (quick && (odds || !(total < INFINITY))) {
+            quick = false;          // the infinities have to be told apart
+        } else if (residual && total <= 0.0) {
+            residual = false;       // p lies below q everywhere: p itself
+            d.q = nullptr;
+            d.skip = -1;
+        } else {
+            break;
+        }
+    }
+    int32_t* const out = a.tokens + (size_t)b * (k + 1);
+    // the accepted tokens, and -1 behind the drawn one
+    if (rank == 0) {
+        if (t <= k && t != r) out[t] = t < r ? a.draft[(size_t)b * k + t] : -1;
+        if (t == 0) {
+            a.count[b] = r + 1;
+            if (total <= 0.0) out[r] = -1;          // no mass at all: no token
+        }
+    }
+    if (total <= 0.0 || (owner >= 0 ? owner != rank : rank != 0)) return;
+    // the run that holds it, then which eighth of that run (a warp each, from
+    // L2), then the index. Where the rounding of the sums leaves no such run,
+    // eighth or index: the last index with mass before the border
+    auto pick = [&](const double* sums) {
+        int at = -1;
+        for (int w = 0; w < kSvWarps && at < 0; ++w) {
+            if (sums[w] > 0.0 && before + sums[w] > target) at = w;
+            else before += sums[w];
+        }
+        return at;
+    };
+    int limit = V, found = -1, leader = 0;
+    if (owner >= 0) {
+        limit = (int)min((long long)V, (long long)(rank + 1) * kSvWarps * per);
+        const int mine = pick(s_sum);
+        if (mine >= 0) {
+            const int first = (rank * kSvWarps + mine) * per, end = min(V, first + per);
+            const int piece = ((end - first + kSvWarps - 1) / kSvWarps + 127) / 128 * 128;
+            const int a0 = min(first + warp * piece, end), a1 = min(a0 + piece, end);
+            const double sum = run_sum<VEC, false>(d, a0, a1, nullptr);
+            __shared__ double s_piece[kSvWarps];
+            if (lane == 0) s_piece[warp] = sum;
+            __syncthreads();
+            const int eighth = pick(s_piece);
+            limit = end;
+            if (eighth >= 0) {
+                leader = eighth;
+                limit = min(first + (eighth + 1) * piece, end);
+                if (warp == leader) found = find_in_run<VEC>(d, a0, a1, before, target);
             }
         }
     }
-    sum.res = warp_sum_d(sum.res);
-    sum.all = warp_sum_d(sum.all);
-    last_res = __reduce_max_sync(0xffffffffu, last_res);
-    last_all = __reduce_max_sync(0xffffffffu, last_all);
-    if (lane == 0) {
-        s_res[warp] = sum.res;
-        s_all[warp] = sum.all;
-        s_last_res[warp] = last_res;
-        s_last_all[warp] = last_all;
-    }
-    __syncthreads();
-    if (t == 0) {
-        double x = 0.0, y = 0.0;
-        int lr = -1, la = -1;
-        for (int w = 0; w < kSvWarps; ++w) {
-            x += s_res[w];
-            y += s_all[w];
-            lr = max(lr, s_last_res[w]);
-            la = max(la, s_last_all[w]);
-        }
-        cta_res = x;
-        cta_all = y;
-        cta_last_res = lr;
-        cta_last_all = la;
-    }
-    cl.sync();
-    // every CTA adds the CTAs' sums in the same order, and finds the one that
-    // holds the draw
-    double total_res = 0.0, total_all = 0.0;
-    int end_res = -1, end_all = -1;
-    for (int c = 0; c < C; ++c) {
-        total_res += *cl.map_shared_rank(&cta_res, c);
-        total_all += *cl.map_shared_rank(&cta_all, c);
-        end_res = max(end_res, *cl.map_shared_rank(&cta_last_res, c));
-        end_all = max(end_all, *cl.map_shared_rank(&cta_last_all, c));
-    }
-    const bool residual = refused >= 0 && total_res > 0.0;
-    const double total = residual ? total_res : total_all;
-    const int end = residual ? end_res : end_all;      // the last index with mass
-    const double target = fmax((double)a.u_draw[b], 0.0) * total;
-    double before = 0.0;
-    int owner = -1;
-    for (int c = 0; c < C; ++c) {
-        const double m = *cl.map_shared_rank(residual ? &cta_res : &cta_all, c);
-        if (owner < 0 && before + m > target) owner = c;
-        if (owner < 0) before += m;
-    }
-    cl.sync();                                          // remote reads done
-    // the accepted tokens, and -1 behind the drawn one
-    if (rank == 0)
-        for (int i = t; i <= k; i += kSvThreads)
-            if (i != r) a.tokens[(size_t)b * (k + 1) + i] = i < r ? a.draft[(size_t)b * k + i] : -1;
-    if (rank == 0 && t == 0) {
-        a.count[b] = r + 1;
-        // no mass at all: no token; no index past the draw: the last with mass
-        if (total <= 0.0 || owner < 0) a.tokens[(size_t)b * (k + 1) + r] = total <= 0.0 ? -1 : end;
-    }
-    if (total <= 0.0 || owner != rank) return;
-    // the warp of this CTA, then the index; a border that moved by the
-    // rounding of the partial sums falls to the last index with mass before it
-    int mine = -1;
-    for (int w = 0; w < kSvWarps; ++w) {
-        const double m = residual ? s_res[w] : s_all[w];
-        if (mine < 0 && before + m > target) mine = w;
-        if (mine < 0) before += m;
-    }
-    if (mine < 0) {
-        if (t == 0) a.tokens[(size_t)b * (k + 1) + r] = residual ? cta_last_res : cta_last_all;
-        return;
-    }
-    if (warp != mine) return;
-    int found = -1;
-    for (int i0 = lo; i0 < hi && found < 0; i0 += 128) {
-        const int i = i0 + 4 * lane;
-        const float4 pv = row4<VEC>(i < hi ? prow : nullptr, i, hi), qv = row4<VEC>(i < hi ? qrow : nullptr, i, hi);
-        const float pe[4] = {pv.x, pv.y, pv.z, pv.w}, qe[4] = {qv.x, qv.y, qv.z, qv.w};
-        double m[4], x = 0.0;
-        #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            m[e] = mass_at(pe[e], qe[e], i + e, refused, point, residual);
-            x += m[e];
-        }
-        const double own = x;
-        #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const double y = __shfl_up_sync(0xffffffffu, x, o);
-            if (lane >= o) x += y;
-        }
-        // an entry without mass is never drawn, whatever the sums' rounding
-        double run = before + (x - own);
-        int hit = -1;
-        #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            run += m[e];
-            if (hit < 0 && m[e] > 0.0 && run > target) hit = e;
-        }
-        const unsigned any = __ballot_sync(0xffffffffu, hit >= 0);
-        if (any != 0) found = __shfl_sync(0xffffffffu, i + hit, __ffs(any) - 1);
-        before += __shfl_sync(0xffffffffu, x, 31);
-    }
-    if (lane == 0)
-        a.tokens[(size_t)b * (k + 1) + r] = found >= 0 ? found : residual ? s_last_res[warp] : s_last_all[warp];
+    if (warp != leader) return;
+    if (found < 0) found = last_mass<VEC>(d, limit);
+    if (lane == 0) out[r] = found;
 }
 
 }  // namespace
@@ -278,9 +337,15 @@ extern "C" int sllm_cuda_spec_verify(const float* p, const float* q, const int32
     a.k = k; a.V = n_vocab;
     a.vec = n_vocab % 4 == 0 && aligned16(p) && (q == nullptr || aligned16(q));
     a.status = status;
-    // few sequences: eight CTAs each, so that the rows are read by many SMs;
-    // a small vocabulary needs no cluster
-    const int C = n_vocab <= 4096 ? 1 : 8;
+    // a cluster per sequence; few sequences get larger ones, so that more SMs
+    // read their rows (one sequence of 128256 words: see the sizes below), and
+    // a small vocabulary none
+    const int sms = current_sms();
+    const int C = n_vocab <= 4096 ? 1 : (long long)n * 16 <= sms ? 16 : 8;
+    if (C == 16) {
+        const cudaError_t e1 = allow_cluster<spec_verify_kernel<true>>(), e2 = allow_cluster<spec_verify_kernel<false>>();
+        CK(e1 != cudaSuccess ? e1 : e2, "spec_verify clusters");
+    }
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(n * C));
     cfg.blockDim = dim3(kSvThreads);
