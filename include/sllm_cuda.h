@@ -302,8 +302,8 @@ SLLM_CUDA_API int sllm_cuda_kv_compact(const sllm_cuda_kv_pages * p, void * work
  * k and v are rounded to the cache's type; q_out [n_tokens][n_head][128] and
  * k_out, v_out [n_tokens][n_head_kv][128] receive them too (k_out and v_out
  * may be NULL; q and q_out may both be NULL). Strides are floats from a token
- * to the next. A token with slot[t] < 0 is padding: nothing of it is read
- * further or written. A token whose slot, position or page is wrong, or whose
+ * to the next. A token with slot[t] < 0 is padding: nothing of it is
+ * written. A token whose slot, position or page is wrong, or whose
  * page has other owners, sets SLLM_CUDA_ERR_ARG in *status and is left out.
  * Two tokens for one place leave either of them.
  */

@@ -464,10 +464,15 @@ kv_copy_kernel(const PagesDev p, uint8_t* k, uint8_t* v, int runs, int row_bytes
 
 // ---------------------------------------------------------------------------
 // append: RoPE (the decode path's rotation from the same angle table),
-// conversion and store. One warp per (token, head): lane l holds elements
-// 2l, 2l+1 and 2l+64, 2l+65, which are the rotation's pairs. Bound by HBM:
-// every value is read once and written once (k and v twice).
+// conversion and store. A warp takes eight rows (heads of k, of v, of q, in
+// that order) of one token, two at a time: lane l of a half-warp holds elements
+// 4l .. 4l + 3 and 64 + 4l .., which are the rotation's pairs, so everything
+// moves in 16-byte pieces (8-byte stores for f16). The rows are read before
+// the slot's table has been walked. Bound by HBM: every value is read once and
+// written once (k and v twice).
 // ---------------------------------------------------------------------------
+constexpr int kApRows = 8;
+
 struct AppendParams {
     const int32_t* slot;
     const int32_t* pos;
@@ -488,24 +493,28 @@ struct AppendParams {
 };
 
 template <class T>
-__device__ __forceinline__ void st2(T* p, float a, float b);
-template <> __device__ __forceinline__ void st2<float>(float* p, float a, float b) {
-    *reinterpret_cast<float2*>(p) = make_float2(a, b);
-}
-template <> __device__ __forceinline__ void st2<__half>(__half* p, float a, float b) {
-    *reinterpret_cast<__half2*>(p) = __floats2half2_rn(a, b);
-}
-
-template <class T>
 __global__ void __launch_bounds__(256)
-kv_append_kernel(const PagesDev p, const __grid_constant__ AppendParams a) {
-    const int lane = threadIdx.x & 31;
-    const int heads = (a.q != nullptr ? a.n_head : 0) + 2 * a.n_kv;
+kv_append_kernel(const __grid_constant__ PagesDev p, const __grid_constant__ AppendParams a) {
+    const int lane = threadIdx.x & 31, l4 = 4 * (lane & 15);
+    const int rows = (a.q != nullptr ? a.n_head : 0) + 2 * a.n_kv, units = (rows + kApRows - 1) / kApRows;
     const long long u = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int tok = (int)(u / heads);
+    const int tok = (int)(u / units);
     if (tok >= a.n_tokens) return;
-    int h = (int)(u - (long long)tok * heads);
+    const int r0 = (int)(u - (long long)tok * units) * kApRows + (lane >> 4);
     const int slot = a.slot[tok], pos = a.pos[tok];
+    // row r: k heads, v heads, q heads
+    float4 lo[kApRows / 2], hi[kApRows / 2];
+    #pragma unroll
+    for (int i = 0; i < kApRows / 2; ++i) {
+        const int r = r0 + 2 * i;
+        if (r < rows) {
+            const float* x = r < a.n_kv       ? a.k + tok * a.ks + r * kServeDim
+                             : r < 2 * a.n_kv ? a.v + tok * a.vs + (r - a.n_kv) * kServeDim
+                                              : a.q + tok * a.qs + (r - 2 * a.n_kv) * kServeDim;
+            lo[i] = __ldcs(reinterpret_cast<const float4*>(x + l4));
+            hi[i] = __ldcs(reinterpret_cast<const float4*>(x + 64 + l4));
+        }
+    }
     if (slot < 0) return;           // a padding token
     int id = -1;
     if (slot < p.n_slots && pos >= 0 && pos < a.n_ctx && pos < p.cap && pos < p.lens[slot])
@@ -515,31 +524,36 @@ kv_append_kernel(const PagesDev p, const __grid_constant__ AppendParams a) {
         if (lane == 0) raise(a.status, SLLM_CUDA_ERR_ARG);
         return;
     }
-    const int kind = h < 2 * a.n_kv ? (h < a.n_kv ? 1 : 2) : 0;
-    h = kind == 0 ? h - 2 * a.n_kv : kind == 1 ? h : h - a.n_kv;
-    const float* x = (kind == 0 ? a.q + tok * a.qs : kind == 1 ? a.k + tok * a.ks : a.v + tok * a.vs) + h * kServeDim;
-    float2 lo = *reinterpret_cast<const float2*>(x + 2 * lane);
-    float2 hi = *reinterpret_cast<const float2*>(x + 64 + 2 * lane);
-    if (kind != 2) {
-        const float2 c = *reinterpret_cast<const float2*>(a.cs + (size_t)pos * 64 + 2 * lane);
-        const float2 s = *reinterpret_cast<const float2*>(a.sn + (size_t)pos * 64 + 2 * lane);
-        const float2 u0 = lo, u1 = hi;
-        lo.x = __fsub_rn(__fmul_rn(u0.x, c.x), __fmul_rn(u1.x, s.x));
-        lo.y = __fsub_rn(__fmul_rn(u0.y, c.y), __fmul_rn(u1.y, s.y));
-        hi.x = __fadd_rn(__fmul_rn(u0.x, s.x), __fmul_rn(u1.x, c.x));
-        hi.y = __fadd_rn(__fmul_rn(u0.y, s.y), __fmul_rn(u1.y, c.y));
-    }
-    T* out = static_cast<T*>(kind == 0 ? a.qo : kind == 1 ? a.ko : a.vo);
-    if (out != nullptr) {
-        out += ((size_t)tok * (kind == 0 ? a.n_head : a.n_kv) + h) * kServeDim;
-        st2(out + 2 * lane, lo.x, lo.y);
-        st2(out + 64 + 2 * lane, hi.x, hi.y);
-    }
-    if (kind != 0) {
-        T* row = static_cast<T*>(kind == 1 ? a.kp : a.vp) + (size_t)id * a.page_stride +
-                 ((size_t)h * p.page + pos % p.page) * kServeDim;
-        st2(row + 2 * lane, lo.x, lo.y);
-        st2(row + 64 + 2 * lane, hi.x, hi.y);
+    const float4 c = ld4(a.cs + (size_t)pos * 64 + l4), s = ld4(a.sn + (size_t)pos * 64 + l4);
+    const size_t place = (size_t)id * a.page_stride + (size_t)(pos % p.page) * kServeDim + l4;
+    #pragma unroll
+    for (int i = 0; i < kApRows / 2; ++i) {
+        const int r = r0 + 2 * i;
+        if (r >= rows) break;
+        const bool is_v = r >= a.n_kv && r < 2 * a.n_kv;
+        if (!is_v) {
+            const float4 x = lo[i], y = hi[i];
+            lo[i].x = __fsub_rn(__fmul_rn(x.x, c.x), __fmul_rn(y.x, s.x));
+            lo[i].y = __fsub_rn(__fmul_rn(x.y, c.y), __fmul_rn(y.y, s.y));
+            lo[i].z = __fsub_rn(__fmul_rn(x.z, c.z), __fmul_rn(y.z, s.z));
+            lo[i].w = __fsub_rn(__fmul_rn(x.w, c.w), __fmul_rn(y.w, s.w));
+            hi[i].x = __fadd_rn(__fmul_rn(x.x, s.x), __fmul_rn(y.x, c.x));
+            hi[i].y = __fadd_rn(__fmul_rn(x.y, s.y), __fmul_rn(y.y, c.y));
+            hi[i].z = __fadd_rn(__fmul_rn(x.z, s.z), __fmul_rn(y.z, c.z));
+            hi[i].w = __fadd_rn(__fmul_rn(x.w, s.w), __fmul_rn(y.w, c.w));
+        }
+        const int h = r < a.n_kv ? r : is_v ? r - a.n_kv : r - 2 * a.n_kv;
+        T* out = static_cast<T*>(r < a.n_kv ? a.ko : is_v ? a.vo : a.qo);
+        if (out != nullptr) {
+            out += ((size_t)tok * (r < 2 * a.n_kv ? a.n_kv : a.n_head) + h) * kServeDim + l4;
+            st4(out, lo[i]);
+            st4(out + 64, hi[i]);
+        }
+        if (r < 2 * a.n_kv) {
+            T* row = static_cast<T*>(is_v ? a.vp : a.kp) + place + (size_t)h * p.page * kServeDim;
+            st4(row, lo[i]);
+            st4(row + 64, hi[i]);
+        }
     }
 }
 
@@ -707,7 +721,8 @@ extern "C" int sllm_cuda_kv_append(const sllm_cuda_kv_pages* p, int32_t layer, i
     a.page_stride = (size_t)p->n_layer * layer_elts;
     a.n_tokens = n_tokens; a.n_head = n_head; a.n_kv = p->n_head_kv; a.n_ctx = n_ctx;
     a.status = status;
-    const long long units = (long long)n_tokens * ((q != nullptr ? n_head : 0) + 2 * p->n_head_kv);
+    const int rows = (q != nullptr ? n_head : 0) + 2 * p->n_head_kv;
+    const long long units = (long long)n_tokens * ((rows + kApRows - 1) / kApRows);
     if (units > 0x7fffffffLL * 8 - 8) return fail(SLLM_CUDA_ERR_TOO_LARGE, "kv_append: %d tokens", n_tokens);
     const dim3 grid((unsigned)((units + 7) / 8));
     if (p->kv_type == SLLM_CUDA_KV_F16)
