@@ -195,7 +195,7 @@ __device__ __forceinline__ void store_row(uint32_t o_tmem, float f, bool live, O
 //                    there. The order P0 V, S0', P1 V, S1' lets one tile's
 //                    softmax run under the other tile's products.
 //   warp 13          TMA: Q per item, K and V tiles through a ring of five.
-//   warp 14          the items, two ahead.
+//   warp 14          the items, one ahead.
 //
 // What bounds it: per key tile and row tile 1024 clocks of products, and the
 // chain S -> softmax -> P V -> S', whose softmax is 16384 exponentials at 16
@@ -208,14 +208,21 @@ __device__ __forceinline__ void store_row(uint32_t o_tmem, float f, bool live, O
 // softmax warps look for such values in the masked tiles, and if there are
 // any warps 8-11 recompute the tile's rows one by one.
 //
-// `W` says what the items are: find(x, item) (false: there is no item x, but
-// later ones may be), tiles(item, t) (0: no such row tile), keys(item),
+// `W` says what the items are: a Finder (number(w, r): the number of the CTA's
+// r-th item; item(w, x, item): false: there is no item x, but later ones may
+// be), tiles(item, t) (0: no such row tile), keys(item),
 // seen(item, t, row) (not above keys, and least for row 0), live(item, t, row)
 // (a row to be written), a Loader, store(...) and slow(...).
 //
 // Registers: 512 threads x 128 at launch; 2 x 192 (softmax) + 64 (outputs) +
 // 64 (the issuing warps) = 512 = 4 x 128 after the split.
 // ---------------------------------------------------------------------------
+// a fixed share of the item numbers: every other round backwards, so that the
+// CTA that got the longest item of one round gets the shortest of the next
+__device__ __forceinline__ long long dealt_number(int r) {
+    return (long long)r * gridDim.x + ((r & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+}
+
 // why a bounded wait gave up (0: none did), in each file with such a kernel
 static __device__ int g_attn_error;
 static inline int take_attn_error() {
@@ -237,9 +244,9 @@ __device__ __forceinline__ void attn_core(const W w) {
     // complete; of: outputs read
     struct Shared {
         uint64_t bar_full[kAtStages], bar_free[kAtStages], bar_q[2], bar_qf[2], bar_s[2], bar_h[2], bar_p[2], bar_l[2],
-            bar_o[2], bar_of[2], bar_item[2], bar_itemf[2], bar_done;
+            bar_o[2], bar_of[2], bar_item, bar_itemf, bar_done;
         float sum[2][kAtRows], top[2][kAtRows];
-        Item item[2];
+        Item item;
         int odd[2][4];
         uint32_t tmem;
         int abort_flag;
@@ -261,13 +268,13 @@ __device__ __forceinline__ void attn_core(const W w) {
             mbar_init(&sh.bar_l[i], 4);
             mbar_init(&sh.bar_o[i], 1);
             mbar_init(&sh.bar_of[i], 4);
-            mbar_init(&sh.bar_item[i], 1);
-            mbar_init(&sh.bar_itemf[i], 14);    // 8 softmax, 4 output warps, the products and the loads
         }
         for (int i = 0; i < kAtStages; ++i) {
             mbar_init(&sh.bar_full[i], 1);
             mbar_init(&sh.bar_free[i], 1);
         }
+        mbar_init(&sh.bar_item, 1);
+        mbar_init(&sh.bar_itemf, 14);           // 8 softmax, 4 output warps, the products and the loads
         mbar_init(&sh.bar_done, 1);
         sh.abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -285,16 +292,16 @@ __device__ __forceinline__ void attn_core(const W w) {
     volatile int* const ab = &sh.abort_flag;
 
     auto next_warp = [&](int i, Item* it) {       // false: no more, or a wait gave up
-        if (!at_wait_warp(&sh.bar_item[i & 1], (i >> 1) & 1, ab, err)) return false;
-        *it = sh.item[i & 1];
+        if (!at_wait_warp(&sh.bar_item, i & 1, ab, err)) return false;
+        *it = sh.item;
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sh.bar_itemf[i & 1]);
+        if (lane == 0) mbar_arrive(&sh.bar_itemf);
         return !it->last();
     };
     auto next_lane = [&](int i, Item* it) {
-        if (!at_wait(&sh.bar_item[i & 1], (i >> 1) & 1, ab, err)) return false;
-        *it = sh.item[i & 1];
-        mbar_arrive(&sh.bar_itemf[i & 1]);
+        if (!at_wait(&sh.bar_item, i & 1, ab, err)) return false;
+        *it = sh.item;
+        mbar_arrive(&sh.bar_itemf);
         return !it->last();
     };
 
@@ -554,17 +561,17 @@ __device__ __forceinline__ void attn_core(const W w) {
             __syncwarp();
         } else if (warp == 14) {
             // ---------------- items ----------------
+            typename W::Finder find;
+            find.start(w);
             #pragma unroll 1
             for (int r = 0, i = 0;; ++r) {
-                // every other round backwards: the CTA that got the longest
-                // item of one round gets the shortest of the next
-                const long long x = (long long)r * gridDim.x + ((r & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+                // every warp has taken the item before
+                if (i > 0 && !at_wait_warp(&sh.bar_itemf, (i - 1) & 1, ab, err)) break;
                 Item it;
-                if (!w.find(x, &it)) continue;          // no item has this number
-                if (i >= 2 && !at_wait_warp(&sh.bar_itemf[i & 1], ((i >> 1) - 1) & 1, ab, err)) break;
+                if (!find.item(w, find.number(w, r), &it)) continue;    // no item has this number
                 if (lane == 0) {
-                    sh.item[i & 1] = it;
-                    mbar_arrive(&sh.bar_item[i & 1]);
+                    sh.item = it;
+                    mbar_arrive(&sh.bar_item);
                 }
                 if (it.last()) break;
                 ++i;

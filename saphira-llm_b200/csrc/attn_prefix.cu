@@ -22,13 +22,14 @@
 namespace sllm {
 namespace {
 
-// how the work is cut, the same for every kernel of a call
+// how the work is cut
 struct Plan {
     int key_tile;                   // keys of a tile
     int rt, per;                    // rows of a row tile, row tiles of an item
-    int sp, ptiles;                 // splits and key tiles of the prefix
-    int cm;                         // most chunks of a sequence's own keys
+    int ptiles, sp;                 // key tiles of the prefix, and its splits
+    int ct, cm;                     // key tiles of a chunk of a sequence's own keys; chunks at most
     int ri_all, ri_seq;             // row items of all sequences, of one
+    int* next;                      // the next item's number, or NULL: numbers are dealt
 };
 
 struct PrefixParams {
@@ -56,11 +57,12 @@ __device__ __forceinline__ int seq_len(const PagesDev& pg, const PrefixParams& p
     return len;
 }
 
-// chunks of a sequence's own keys: at least two tiles each
-__device__ __forceinline__ int own_chunks(const PrefixParams& p, int len, int* tiles) {
-    const int own = max(0, len - p.prefix);
-    *tiles = (own + p.plan.key_tile - 1) / p.plan.key_tile;
-    return min(p.plan.cm, (*tiles + 1) / 2);
+__device__ __forceinline__ int own_tiles(const PrefixParams& p, int len) {
+    return (max(0, len - p.prefix) + p.plan.key_tile - 1) / p.plan.key_tile;
+}
+
+__device__ __forceinline__ int own_chunks(const PrefixParams& p, int tiles) {
+    return min(p.plan.cm, (tiles + p.plan.ct - 1) / p.plan.ct);
 }
 
 // Keys a .. a + keys - 1 of `slot` for rows row0 .. of kv head kvh (at most
@@ -100,8 +102,8 @@ __device__ __forceinline__ bool find_item(const PagesDev& pg, const PrefixParams
     it->kvh = (int)(x % p.n_kv);
     x /= p.n_kv;
     const int b = (int)(x % p.n), c = (int)(x / p.n);
-    int slot, tiles;
-    const int len = seq_len(pg, p, b, &slot), chunks = own_chunks(p, len, &tiles);
+    int slot;
+    const int len = seq_len(pg, p, b, &slot), tiles = own_tiles(p, len), chunks = own_chunks(p, tiles);
     if (c >= chunks) return false;
     const int t0 = (int)((long long)c * tiles / chunks), t1 = (int)((long long)(c + 1) * tiles / chunks);
     it->slot = slot;
@@ -148,7 +150,18 @@ struct PrefixWork {
     const PrefixParams& p;
     const CUtensorMap &tm_q, &tm_k, &tm_v;
 
-    __device__ __forceinline__ bool find(long long x, Item* it) const { return find_item(pg, p, x, it); }
+    struct Finder {
+        __device__ __forceinline__ void start(const PrefixWork&) {}
+        __device__ __forceinline__ long long number(const PrefixWork& w, int r) {
+            if (w.p.plan.next == nullptr) return dealt_number(r);
+            int x = 0;
+            if ((threadIdx.x & 31) == 0) x = atomicAdd(w.p.plan.next, 1);
+            return __shfl_sync(0xffffffffu, x, 0);
+        }
+        __device__ __forceinline__ bool item(const PrefixWork& w, long long x, Item* it) {
+            return find_item(w.pg, w.p, x, it);
+        }
+    };
     __device__ __forceinline__ int tiles(const Item& it, int t) const {
         return it.row0 + t * p.plan.rt < it.row_end ? (it.keys + kAtKeys - 1) / kAtKeys : 0;
     }
@@ -255,7 +268,7 @@ attn_prefix_mma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
 // 32-bit: one item per CTA, R rows a thread
 // ---------------------------------------------------------------------------
 template <int R, class T>
-__global__ void __launch_bounds__(kSimtThreads)
+__global__ void __launch_bounds__(kSimtThreads, 2)
 attn_prefix_simt_kernel(const __grid_constant__ PagesDev pg, const __grid_constant__ PrefixParams p) {
     extern __shared__ float smf[];
     pdl_trigger();
@@ -288,9 +301,7 @@ attn_prefix_simt_kernel(const __grid_constant__ PagesDev pg, const __grid_consta
         if (r >= it.row_end) continue;
         const size_t at = part_at(p, it, r);
         if (tx == 0) p.part_ml[at] = make_float2(st.m[i], st.l[i]);
-        float* o = p.part_o + at * kServeDim;
-        st4(o + 4 * tx, make_float4(st.o[i][0], st.o[i][1], st.o[i][2], st.o[i][3]));
-        st4(o + 64 + 4 * tx, make_float4(st.o[i][4], st.o[i][5], st.o[i][6], st.o[i][7]));
+        simt_store(st, i, 1.f, p.part_o + at * kServeDim);
     }
 }
 
@@ -305,13 +316,13 @@ attn_prefix_join_kernel(const __grid_constant__ PagesDev pg, const __grid_consta
     const int rows = p.n * p.n_q * p.group;
     if (x >= (long long)rows * p.n_kv) return;
     const int kvh = (int)(x / rows), r = (int)(x % rows), b = r / (p.n_q * p.group);
-    int slot, tiles;
-    const int len = seq_len(pg, p, b, &slot), chunks = own_chunks(p, len, &tiles);
+    int slot;
+    const int len = seq_len(pg, p, b, &slot);
     if (len < 0) {
         if (lane == 0) raise(p.status, SLLM_CUDA_ERR_ARG);
         return;
     }
-    const int parts = p.plan.sp + chunks;
+    const int parts = p.plan.sp + own_chunks(p, own_tiles(p, len));
     pdl_wait();
     const size_t at = (size_t)x * (p.plan.sp + p.plan.cm);
     const float2* ml = p.part_ml + at;
@@ -331,16 +342,22 @@ attn_prefix_join_kernel(const __grid_constant__ PagesDev pg, const __grid_consta
         #pragma unroll
         for (int y = 16; y > 0; y >>= 1) part_l += __shfl_xor_sync(0xffffffffu, part_l, y);
         l += part_l;
+        // eight parts' outputs in flight; past the last, its own again with weight 0
         const int n = min(32, parts - i0);
-        #pragma unroll 4
-        for (int i = 0; i < n; ++i) {
-            const float g = __shfl_sync(0xffffffffu, f, i);
-            const float4 v = *reinterpret_cast<const float4*>(po + (size_t)(i0 + i) * kServeDim);
-            if (g != 0.f) {
-                o.x = fmaf(g, v.x, o.x);
-                o.y = fmaf(g, v.y, o.y);
-                o.z = fmaf(g, v.z, o.z);
-                o.w = fmaf(g, v.w, o.w);
+        for (int i = 0; i < n; i += 8) {
+            float4 v[8];
+            #pragma unroll
+            for (int e = 0; e < 8; ++e)
+                v[e] = __ldcg(reinterpret_cast<const float4*>(po + (size_t)(i0 + min(i + e, n - 1)) * kServeDim));
+            #pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float g = __shfl_sync(0xffffffffu, f, (i + e) & 31);
+                if (i + e < n && g != 0.f) {
+                    o.x = fmaf(g, v[e].x, o.x);
+                    o.y = fmaf(g, v[e].y, o.y);
+                    o.z = fmaf(g, v[e].z, o.z);
+                    o.w = fmaf(g, v[e].w, o.w);
+                }
             }
         }
     }
@@ -351,10 +368,13 @@ attn_prefix_join_kernel(const __grid_constant__ PagesDev pg, const __grid_consta
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
-// The cut. Rows: whole tokens per row tile where TMA gathers them. Splits of
-// the prefix: as many as finish first when each item costs its key tiles plus
-// three for its start and its parts, on one CTA per SM. Chunks of a sequence's
-// own keys: up to two items per SM over all sequences, at most 64 each.
+// Rows: whole tokens per row tile where TMA gathers them. Splits of the prefix:
+// with an item of its own keys for each sequence besides, all of it in one
+// round of the SMs where that makes splits of at most eight key tiles. Longer:
+// the number, of those that make up to 32 tiles a split, that ends first on
+// the SMs when a split costs a tile's time for its start and its parts.
+// A sequence's own keys: chunks of as many tiles, at least two; no more than
+// two items per SM over all sequences, and no more than 64 chunks.
 Plan make_plan(const sllm_cuda_kv_pages& p, int n, int n_q, int n_head, int prefix, int sms) {
     const int group = n_head / p.n_head_kv, rows = n * n_q * group;
     const bool mma = p.kv_type == SLLM_CUDA_KV_F16 && group <= kAtRows;
@@ -366,16 +386,24 @@ Plan make_plan(const sllm_cuda_kv_pages& p, int n, int n_q, int n_head, int pref
     pl.ri_all = items(rows);
     pl.ri_seq = items(n_q * group);
     pl.ptiles = (prefix + pl.key_tile - 1) / pl.key_tile;
-    const long long base = (long long)p.n_head_kv * pl.ri_all;
-    long long best = 0;
-    for (int s = 1; s <= 32 && s <= pl.ptiles; ++s) {
-        const long long cost = ((base * s + sms - 1) / sms) * ((pl.ptiles + s - 1) / s + 3);
-        if (pl.sp == 0 || cost < best) {
-            best = cost;
-            pl.sp = s;
+    const long long base = (long long)p.n_head_kv * pl.ri_all, own = (long long)n * p.n_head_kv * pl.ri_seq;
+    const long long room = sms - own > sms / 2 ? sms - own : sms / 2;
+    const long long one = (base * pl.ptiles + room - 1) / room;        // tiles a split in one round
+    if (one <= 8) {
+        pl.ct = one < 1 ? 1 : (int)one;
+        pl.sp = (pl.ptiles + pl.ct - 1) / pl.ct;
+    } else {
+        long long best = 0;
+        for (int s = (pl.ptiles + 31) / 32; s <= pl.ptiles && (s <= 32 || pl.sp == 0); ++s) {
+            const long long tiles = (pl.ptiles + s - 1) / s, cost = ((base * s + sms - 1) / sms) * (tiles + 1);
+            if (pl.sp == 0 || cost < best) {
+                best = cost;
+                pl.sp = s;
+                pl.ct = (int)tiles;
+            }
         }
     }
-    const long long own = (long long)n * p.n_head_kv * pl.ri_seq;
+    if (pl.ct < 2) pl.ct = 2;
     const long long cm = own > 0 ? (2LL * sms + own - 1) / own : 1;
     pl.cm = (int)(cm < 1 ? 1 : cm > 64 ? 64 : cm);
     return pl;
@@ -425,6 +453,10 @@ cudaError_t launch_mma(const sllm_cuda_kv_pages& pages, const PagesDev& pg, cons
     const cudaError_t e = allow_smem<attn_prefix_mma_kernel>(kAtSmem);
     if (e != cudaSuccess) return e;
     const long long items = item_numbers(p);
+    if (p.plan.next != nullptr) {
+        const cudaError_t z = cudaMemsetAsync(p.plan.next, 0, sizeof(int), st);
+        if (z != cudaSuccess) return z;
+    }
     return launch(attn_prefix_mma_kernel, dim3((unsigned)(items < sms ? items : sms)), dim3(kAtThreads), kAtSmem, st, false,
                   tq, tk, tv, pg, p);
 }
@@ -496,7 +528,11 @@ extern "C" int sllm_cuda_attn_prefix(const sllm_cuda_kv_pages* p, int32_t layer,
     a.plan = make_plan(*p, n, n_q, n_head, prefix_len, sms);
     a.part_o = static_cast<float*>(work);
     a.part_ml = reinterpret_cast<float2*>(a.part_o + part_count(a.plan, n, n_q, n_head) * kServeDim);
-    if (item_numbers(a) > 0x7fffffffLL) return fail(SLLM_CUDA_ERR_TOO_LARGE, "attn_prefix: %d sequences", n);
+    // many items per SM: each CTA takes the next one when it is free (one more
+    // launch, to clear the counter); few: they are dealt
+    if (item_numbers(a) > 3LL * sms)
+        a.plan.next = reinterpret_cast<int*>(a.part_ml + part_count(a.plan, n, n_q, n_head));
+    if (item_numbers(a) > 0x3fffffffLL) return fail(SLLM_CUDA_ERR_TOO_LARGE, "attn_prefix: %d sequences", n);
     const PagesDev pg = pages_dev(*p);
     const cudaStream_t st = (cudaStream_t)stream;
     const bool few = a.plan.rt == kSimtRows<1>;

@@ -58,7 +58,7 @@ __device__ __forceinline__ bool find_tile(const PromptParams& p, int x, int* sta
 }
 
 template <class T, class O>
-__global__ void __launch_bounds__(kSimtThreads)
+__global__ void __launch_bounds__(kSimtThreads, 2)
 attn_prompt_simt_kernel(const __grid_constant__ PromptParams p) {
     extern __shared__ float sm[];
     int start, len, tile;
@@ -67,7 +67,7 @@ attn_prompt_simt_kernel(const __grid_constant__ PromptParams p) {
     const T* q = static_cast<const T*>(p.q) + (size_t)h * kServeDim;
     const T* k = static_cast<const T*>(p.k) + (size_t)kvh * kServeDim;
     const T* v = static_cast<const T*>(p.v) + (size_t)kvh * kServeDim;
-    simt_load_q<4, T>(sm, [&](int r) { return r0 + r < len ? q + (size_t)(start + r0 + r) * p.qs : nullptr; });
+    simt_load_q<4, T>(sm, [&](int r) -> const T* { return r0 + r < len ? q + (size_t)(start + r0 + r) * p.qs : nullptr; });
     SimtState<4> st;
     simt_init(st);
     const int ty = threadIdx.x >> 4;
@@ -77,12 +77,13 @@ attn_prompt_simt_kernel(const __grid_constant__ PromptParams p) {
     const int end = min(r0 + kSimtRows<4>, len);
     for (int j0 = 0; j0 < end; j0 += kSimtKeys)
         simt_tile<4, T>(sm, st, j0, lim,
-                     [&](int j) { return j < end ? k + (size_t)(start + j) * p.ks : nullptr; },
-                     [&](int j) { return j < end ? v + (size_t)(start + j) * p.vs : nullptr; });
+                     [&](int j) -> const T* { return j < end ? k + (size_t)(start + j) * p.ks : nullptr; },
+                     [&](int j) -> const T* { return j < end ? v + (size_t)(start + j) * p.vs : nullptr; });
     #pragma unroll
     for (int i = 0; i < 4; ++i)
         if (r0 + 4 * ty + i < len)
-            simt_store(st, i, static_cast<O*>(p.out) + (size_t)(start + r0 + 4 * ty + i) * p.os + (size_t)h * kServeDim);
+            simt_store(st, i, __fdiv_rn(1.f, st.l[i]),
+                       static_cast<O*>(p.out) + (size_t)(start + r0 + 4 * ty + i) * p.os + (size_t)h * kServeDim);
 }
 
 template <class T, class O>
@@ -183,11 +184,15 @@ struct PromptWork {
     const PromptParams& p;
     const CUtensorMap &tm_q, &tm_k, &tm_v;
 
-    __device__ __forceinline__ bool find(long long x, Item* it) const {     // the x-th item, longest first
-        *it = Item{0, 0, -1, (int)(x % p.n_head)};
-        if (!find_long_first<kPmRows>(p, (int)(x / p.n_head), &it->start, &it->len, &it->tile)) it->tile = -1;
-        return true;
-    }
+    struct Finder {
+        __device__ __forceinline__ void start(const PromptWork&) {}
+        __device__ __forceinline__ long long number(const PromptWork&, int r) { return dealt_number(r); }
+        __device__ __forceinline__ bool item(const PromptWork& w, long long x, Item* it) {      // longest first
+            *it = Item{0, 0, -1, (int)(x % w.p.n_head)};
+            if (!find_long_first<kPmRows>(w.p, (int)(x / w.p.n_head), &it->start, &it->len, &it->tile)) it->tile = -1;
+            return true;
+        }
+    };
     // key tiles of row tile t: up to its diagonal, or the sequence's end
     __device__ __forceinline__ int tiles(const Item& it, int t) const {
         if (it.tile * kPmRows + kAtRows * t >= it.len) return 0;
