@@ -12,9 +12,12 @@ constexpr int kAtRows = 128;                    // query rows of a tile: the TME
 constexpr int kAtKeys = 128;                    // keys of a tile
 constexpr int kAtHalf = 128 * 128;              // bytes of 128 rows x 64 f16 in the 128-byte swizzle
 constexpr int kAtTile = 2 * kAtHalf;            // ... x 128 f16
-constexpr int kAtStages = 5;                    // key and value tiles in flight
+constexpr int kAtStages = 4;                    // key and value tiles in flight
 constexpr int kAtThreads = 512;
-constexpr int kAtSmem = (2 + kAtStages) * kAtTile + 3 * 1024;       // two query tiles, the ring, barriers and sums
+constexpr int kAtStageRow = 128 + 16;           // an output warp's staging: 32 rows of 128 bytes, 16 apart
+constexpr int kAtStage = 32 * kAtStageRow;
+// two query tiles, the ring, the staging of four warps, barriers and sums
+constexpr int kAtSmem = (2 + kAtStages) * kAtTile + 4 * kAtStage + 3 * 1024;
 // softmax in base 2: exp(s / sqrt(128)) = 2^(s c)
 constexpr float kAtScale2 = 0.08838834764831845f * 1.4426950408889634f;
 // the running maximum a row's weights stand against may lag behind by this
@@ -146,34 +149,56 @@ __device__ __forceinline__ void load_scores(uint32_t s_tmem, float (&s)[128]) {
     tmem_ld_wait();
 }
 
-// the tensor-memory outputs of one row, scaled, to global memory: f16 or f32
-__device__ __forceinline__ void store16(const uint32_t (&r)[16], float f, __half* out) {
+// One warp's 32 rows of outputs, scaled by each lane's f, to global memory:
+// 128 bytes of every row at a time through the warp's staging, so that a store
+// writes whole lines (row by row, 32 partial sectors a store, a tile of f32
+// rows took 2 us). Row r of the warp starts at base + r * stride; the first n
+// are to be written.
+__device__ __forceinline__ void pack_out(const uint32_t (&r)[32], float f, uint8_t* at, const __half*) {
     #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 4; ++i) {
         uint4 u;
         uint32_t* w = &u.x;
         #pragma unroll
         for (int e = 0; e < 4; ++e)
             w[e] = pack_half2(__uint_as_float(r[8 * i + 2 * e]) * f, __uint_as_float(r[8 * i + 2 * e + 1]) * f);
-        *reinterpret_cast<uint4*>(out + 8 * i) = u;
+        *reinterpret_cast<uint4*>(at + 16 * i) = u;
     }
 }
-__device__ __forceinline__ void store16(const uint32_t (&r)[16], float f, float* out) {
+__device__ __forceinline__ void pack_out(const uint32_t (&r)[32], float f, uint8_t* at, const float*) {
     #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        *reinterpret_cast<float4*>(out + 4 * i) =
+    for (int i = 0; i < 8; ++i)
+        *reinterpret_cast<float4*>(at + 16 * i) =
             make_float4(__uint_as_float(r[4 * i]) * f, __uint_as_float(r[4 * i + 1]) * f,
                         __uint_as_float(r[4 * i + 2]) * f, __uint_as_float(r[4 * i + 3]) * f);
 }
 template <class O>
-__device__ __forceinline__ void store_row(uint32_t o_tmem, float f, bool live, O* out) {
-    #pragma unroll 2
-    for (int c = 0; c < 8; ++c) {
-        uint32_t r[16];
-        tmem_ld16(o_tmem + 16 * c, r);
-        tmem_ld_wait();
-        if (live) store16(r, f, out + 16 * c);
+__device__ __forceinline__ void store_rows(uint32_t o_tmem, float f, uint8_t* stage, O* base, size_t stride, int n) {
+    constexpr int kCols = 128 / (int)sizeof(O);         // of 128 bytes
+    const int lane = threadIdx.x & 31, sub = lane >> 3;
+    uint8_t* to = reinterpret_cast<uint8_t*>(base + (size_t)sub * stride) + 16 * (lane & 7);
+    const size_t four = 4 * stride * sizeof(O);
+    uint32_t r[32];
+    tmem_ld32(o_tmem, r);
+    #pragma unroll 1
+    for (int c = 0; c < kServeDim; c += kCols) {
+        #pragma unroll
+        for (int x = 0; x < kCols; x += 32) {
+            tmem_ld_wait();
+            pack_out(r, f, stage + lane * kAtStageRow + x * (int)sizeof(O), static_cast<const O*>(nullptr));
+            // the next columns come while these leave
+            if (c + x + 32 < kServeDim) tmem_ld32(o_tmem + c + x + 32, r);
+        }
+        __syncwarp();
+        #pragma unroll 4
+        for (int i = 0; i < 8; ++i) {                   // four rows a store
+            const uint4 u = *reinterpret_cast<const uint4*>(stage + (4 * i + sub) * kAtStageRow + 16 * (lane & 7));
+            if (4 * i + sub < n) *reinterpret_cast<uint4*>(to + i * four) = u;
+        }
+        to += 128;
+        __syncwarp();
     }
+    tmem_ld_wait();
 }
 
 // ---------------------------------------------------------------------------
@@ -194,7 +219,7 @@ __device__ __forceinline__ void store_row(uint32_t o_tmem, float f, bool live, O
 //                    lies), the first 64 keys as soon as their weights are
 //                    there. The order P0 V, S0', P1 V, S1' lets one tile's
 //                    softmax run under the other tile's products.
-//   warp 13          TMA: Q per item, K and V tiles through a ring of five.
+//   warp 13          TMA: Q per item, K and V tiles through a ring of four.
 //   warp 14          the items, one ahead.
 //
 // What bounds it: per key tile and row tile 1024 clocks of products, and the
@@ -214,7 +239,7 @@ __device__ __forceinline__ void store_row(uint32_t o_tmem, float f, bool live, O
 // seen(item, t, row) (not above keys, and least for row 0), live(item, t, row)
 // (a row to be written), a Loader, store(...) and slow(...).
 //
-// Registers: 512 threads x 128 at launch; 2 x 192 (softmax) + 64 (outputs) +
+// Registers: 512 threads x 128 at launch; 2 x 184 (softmax) + 80 (outputs) +
 // 64 (the issuing warps) = 512 = 4 x 128 after the split.
 // ---------------------------------------------------------------------------
 // a fixed share of the item numbers: every other round backwards, so that the
@@ -251,8 +276,9 @@ __device__ __forceinline__ void attn_core(const W w) {
         uint32_t tmem;
         int abort_flag;
     };
-    static_assert(sizeof(Shared) <= kAtSmem - (2 + kAtStages) * kAtTile, "the part behind the tiles");
-    Shared& sh = *reinterpret_cast<Shared*>(sm + (2 + kAtStages) * kAtTile);
+    uint8_t* const stages = sm + (2 + kAtStages) * kAtTile;
+    static_assert(sizeof(Shared) <= 3 * 1024, "the part behind the tiles");
+    Shared& sh = *reinterpret_cast<Shared*>(stages + 4 * kAtStage);
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     if ((smem_u32(sm) & 1023u) != 0) {           // the swizzled layouts need it; the compiler was told to
         if (threadIdx.x == 0) atomicExch(err, 2);
@@ -307,7 +333,7 @@ __device__ __forceinline__ void attn_core(const W w) {
 
     if (warp < 8) {
         // ---------------- softmax ----------------
-        reg_alloc<192>();
+        reg_alloc<184>();
         const int t = warp >> 2, row = 32 * (warp & 3) + lane;
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
         const uint32_t s_tm = tmem + lanes + 128 * t, o_tm = s_tm + 256;
@@ -419,7 +445,7 @@ __device__ __forceinline__ void attn_core(const W w) {
         }
     } else if (warp < 12) {
         // ---------------- outputs ----------------
-        reg_dealloc<64>();
+        reg_dealloc<80>();
         const int row = 32 * (warp & 3) + lane;
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
         int uses[2] = {0, 0};
@@ -436,7 +462,8 @@ __device__ __forceinline__ void attn_core(const W w) {
                 if ((sh.odd[t][0] | sh.odd[t][1] | sh.odd[t][2] | sh.odd[t][3]) != 0)
                     w.slow(it, t, warp & 3);
                 else
-                    w.store(it, t, row, tmem + lanes + 256 + 128 * t, sh.top[t][row], sh.sum[t][row]);
+                    w.store(it, t, row, tmem + lanes + 256 + 128 * t, sh.top[t][row], sh.sum[t][row],
+                            stages + (warp & 3) * kAtStage);
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sh.bar_of[t]);

@@ -214,11 +214,15 @@ struct PrefixWork {
             __syncwarp();
         }
     };
-    __device__ __forceinline__ void store(const Item& it, int t, int row, uint32_t o_tm, float m, float l) const {
-        const bool ok = live(it, t, row);
-        const size_t at = ok ? part_at(p, it, it.row0 + t * p.plan.rt + row) : 0;
-        if (ok) p.part_ml[at] = make_float2(m * kServeScale, l);
-        store_row(o_tm, 1.f, ok, p.part_o + at * kServeDim);
+    __device__ __forceinline__ void store(const Item& it, int t, int row, uint32_t o_tm, float m, float l,
+                                          uint8_t* stage) const {
+        const int lane = row & 31, r = it.row0 + t * p.plan.rt + row - lane;        // the warp's first row
+        const int n = min(p.plan.rt - (row - lane), it.row_end - r);
+        if (n <= 0) return;                     // a warp without rows
+        const int parts = p.plan.sp + p.plan.cm;
+        const size_t at = part_at(p, it, r);
+        if (lane < n) p.part_ml[at + (size_t)lane * parts] = make_float2(m * kServeScale, l);
+        store_rows(o_tm, 1.f, stage, p.part_o + at * kServeDim, (size_t)parts * kServeDim, n);
     }
     // one warp per row, in 32-bit arithmetic
     __device__ __forceinline__ void slow(const Item& it, int t, int warp) const {
@@ -372,7 +376,8 @@ attn_prefix_join_kernel(const __grid_constant__ PagesDev pg, const __grid_consta
 // with an item of its own keys for each sequence besides, all of it in one
 // round of the SMs where that makes splits of at most eight key tiles. Longer:
 // the number, of those that make up to 32 tiles a split, that ends first on
-// the SMs when a split costs a tile's time for its start and its parts.
+// the SMs when a split costs three tiles' time for its start and its parts
+// (all SMs write their parts at about one time, 128 KB each).
 // A sequence's own keys: chunks of as many tiles, at least two; no more than
 // two items per SM over all sequences, and no more than 64 chunks.
 Plan make_plan(const sllm_cuda_kv_pages& p, int n, int n_q, int n_head, int prefix, int sms) {
@@ -395,7 +400,7 @@ Plan make_plan(const sllm_cuda_kv_pages& p, int n, int n_q, int n_head, int pref
     } else {
         long long best = 0;
         for (int s = (pl.ptiles + 31) / 32; s <= pl.ptiles && (s <= 32 || pl.sp == 0); ++s) {
-            const long long tiles = (pl.ptiles + s - 1) / s, cost = ((base * s + sms - 1) / sms) * (tiles + 1);
+            const long long tiles = (pl.ptiles + s - 1) / s, cost = ((base * s + sms - 1) / sms) * (tiles + 3);
             if (pl.sp == 0 || cost < best) {
                 best = cost;
                 pl.sp = s;

@@ -23,87 +23,9 @@ struct PromptParams {
     int n_seq, n_tokens, n_head, group;
 };
 
-// the sequence and its tile for linear tile x of tiles of R rows: a warp's
-// scan over the lengths. Bounds are clamped to the arrays, so a wrong cu
-// stays inside them.
-template <int R>
-__device__ __forceinline__ bool find_tile(const PromptParams& p, int x, int* start, int* len, int* tile) {
-    const int lane = threadIdx.x & 31;
-    int before = 0;
-    for (int s0 = 0; s0 < p.n_seq; s0 += 32) {
-        const int s = s0 + lane;
-        int a = 0, n = 0;
-        if (s < p.n_seq) {
-            a = min(max(p.cu[s], 0), p.n_tokens);
-            n = min(max(p.cu[s + 1], a), p.n_tokens) - a;
-        }
-        const int tiles = (n + R - 1) / R;
-        int inc = tiles;
-        #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(0xffffffffu, inc, o);
-            if (lane >= o) inc += y;
-        }
-        const unsigned hit = __ballot_sync(0xffffffffu, x < before + inc);
-        if (hit != 0) {
-            const int l = __ffs(hit) - 1;
-            *start = __shfl_sync(0xffffffffu, a, l);
-            *len = __shfl_sync(0xffffffffu, n, l);
-            *tile = x - before - __shfl_sync(0xffffffffu, inc - tiles, l);
-            return true;
-        }
-        before += __shfl_sync(0xffffffffu, inc, 31);
-    }
-    return false;
-}
-
-template <class T, class O>
-__global__ void __launch_bounds__(kSimtThreads, 2)
-attn_prompt_simt_kernel(const __grid_constant__ PromptParams p) {
-    extern __shared__ float sm[];
-    int start, len, tile;
-    if (!find_tile<kSimtRows<4>>(p, blockIdx.x, &start, &len, &tile)) return;
-    const int h = blockIdx.y, kvh = h / p.group, r0 = tile * kSimtRows<4>;
-    const T* q = static_cast<const T*>(p.q) + (size_t)h * kServeDim;
-    const T* k = static_cast<const T*>(p.k) + (size_t)kvh * kServeDim;
-    const T* v = static_cast<const T*>(p.v) + (size_t)kvh * kServeDim;
-    simt_load_q<4, T>(sm, [&](int r) -> const T* { return r0 + r < len ? q + (size_t)(start + r0 + r) * p.qs : nullptr; });
-    SimtState<4> st;
-    simt_init(st);
-    const int ty = threadIdx.x >> 4;
-    int lim[4];
-    #pragma unroll
-    for (int i = 0; i < 4; ++i) lim[i] = min(r0 + 4 * ty + i + 1, len);
-    const int end = min(r0 + kSimtRows<4>, len);
-    for (int j0 = 0; j0 < end; j0 += kSimtKeys)
-        simt_tile<4, T>(sm, st, j0, lim,
-                     [&](int j) -> const T* { return j < end ? k + (size_t)(start + j) * p.ks : nullptr; },
-                     [&](int j) -> const T* { return j < end ? v + (size_t)(start + j) * p.vs : nullptr; });
-    #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (r0 + 4 * ty + i < len)
-            simt_store(st, i, __fdiv_rn(1.f, st.l[i]),
-                       static_cast<O*>(p.out) + (size_t)(start + r0 + 4 * ty + i) * p.os + (size_t)h * kServeDim);
-}
-
-template <class T, class O>
-cudaError_t launch_simt(const PromptParams& p, cudaStream_t st) {
-    const cudaError_t e = allow_smem<attn_prompt_simt_kernel<T, O>>(kSimtSmem<4>);
-    if (e != cudaSuccess) return e;
-    // every sequence may end inside a tile
-    const long long tiles = (p.n_tokens + kSimtRows<4> - 1) / kSimtRows<4> + (long long)p.n_seq;
-    return launch(attn_prompt_simt_kernel<T, O>, dim3((unsigned)tiles, (unsigned)p.n_head), dim3(kSimtThreads), kSimtSmem<4>, st, false, p);
-}
-
-// ---------------------------------------------------------------------------
-// The f16 kernel: attn_mma.cuh's core over items of 256 query rows of one
-// head, from the start of the sequence to the diagonal.
-// ---------------------------------------------------------------------------
-constexpr int kPmRows = 2 * kAtRows;
-
 // tile x of the call's tiles of R rows in descending order of their position
 // in their sequence (the later, the more keys they see): the longest work
-// first. F(t) = tiles at positions >= t; a binary search for the position,
+// first. Bounds are clamped to the arrays, so a wrong cu stays inside them. F(t) = tiles at positions >= t; a binary search for the position,
 // then the sequence among those that long. One warp.
 template <int R>
 __device__ __forceinline__ bool find_long_first(const PromptParams& p, int x, int* start, int* len, int* tile) {
@@ -141,6 +63,50 @@ __device__ __forceinline__ bool find_long_first(const PromptParams& p, int x, in
     }
     return false;
 }
+
+template <class T, class O>
+__global__ void __launch_bounds__(kSimtThreads, 2)
+attn_prompt_simt_kernel(const __grid_constant__ PromptParams p) {
+    extern __shared__ float sm[];
+    int start, len, tile;
+    if (!find_long_first<kSimtRows<4>>(p, blockIdx.x / p.n_head, &start, &len, &tile)) return;
+    const int h = blockIdx.x % p.n_head, kvh = h / p.group, r0 = tile * kSimtRows<4>;
+    const T* q = static_cast<const T*>(p.q) + (size_t)h * kServeDim;
+    const T* k = static_cast<const T*>(p.k) + (size_t)kvh * kServeDim;
+    const T* v = static_cast<const T*>(p.v) + (size_t)kvh * kServeDim;
+    simt_load_q<4, T>(sm, [&](int r) -> const T* { return r0 + r < len ? q + (size_t)(start + r0 + r) * p.qs : nullptr; });
+    SimtState<4> st;
+    simt_init(st);
+    const int ty = threadIdx.x >> 4;
+    int lim[4];
+    #pragma unroll
+    for (int i = 0; i < 4; ++i) lim[i] = min(r0 + 4 * ty + i + 1, len);
+    const int end = min(r0 + kSimtRows<4>, len);
+    for (int j0 = 0; j0 < end; j0 += kSimtKeys)
+        simt_tile<4, T>(sm, st, j0, lim,
+                     [&](int j) -> const T* { return j < end ? k + (size_t)(start + j) * p.ks : nullptr; },
+                     [&](int j) -> const T* { return j < end ? v + (size_t)(start + j) * p.vs : nullptr; });
+    #pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (r0 + 4 * ty + i < len)
+            simt_store(st, i, __fdiv_rn(1.f, st.l[i]),
+                       static_cast<O*>(p.out) + (size_t)(start + r0 + 4 * ty + i) * p.os + (size_t)h * kServeDim);
+}
+
+template <class T, class O>
+cudaError_t launch_simt(const PromptParams& p, cudaStream_t st) {
+    const cudaError_t e = allow_smem<attn_prompt_simt_kernel<T, O>>(kSimtSmem<4>);
+    if (e != cudaSuccess) return e;
+    // every sequence may end inside a tile
+    const long long tiles = (p.n_tokens + kSimtRows<4> - 1) / kSimtRows<4> + (long long)p.n_seq;
+    return launch(attn_prompt_simt_kernel<T, O>, dim3((unsigned)(tiles * p.n_head)), dim3(kSimtThreads), kSimtSmem<4>, st, false, p);
+}
+
+// ---------------------------------------------------------------------------
+// The f16 kernel: attn_mma.cuh's core over items of 256 query rows of one
+// head, from the start of the sequence to the diagonal.
+// ---------------------------------------------------------------------------
+constexpr int kPmRows = 2 * kAtRows;
 
 // rows [first, first + 128) of a sequence, one warp per row at a time, in
 // 32-bit arithmetic: the way out for values that are no numbers
@@ -223,10 +189,10 @@ struct PromptWork {
             }
         }
     };
-    __device__ __forceinline__ void store(const Item& it, int t, int row, uint32_t o_tm, float, float l) const {
-        const int x = it.tile * kPmRows + kAtRows * t + row;
-        store_row(o_tm, 1.f / l, x < it.len,
-                  static_cast<O*>(p.out) + (size_t)(it.start + x) * p.os + (size_t)it.head * kServeDim);
+    __device__ __forceinline__ void store(const Item& it, int t, int row, uint32_t o_tm, float, float l, uint8_t* stage) const {
+        const int x0 = it.tile * kPmRows + kAtRows * t + (row & ~31);       // the warp's first row
+        store_rows(o_tm, 1.f / l, stage, static_cast<O*>(p.out) + (size_t)(it.start + x0) * p.os + (size_t)it.head * kServeDim,
+                   p.os, it.len - x0);
     }
     __device__ __forceinline__ void slow(const Item& it, int t, int warp) const {
         slow_rows<O>(p, it.head, it.start, it.len, it.tile * kPmRows + kAtRows * t, warp);
