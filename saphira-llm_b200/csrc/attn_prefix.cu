@@ -18,6 +18,7 @@
 
 #include "attn_mma.cuh"
 #include "attn_simt.cuh"
+#include "attn_wide.cuh"
 
 namespace sllm {
 namespace {
@@ -141,6 +142,53 @@ __device__ __forceinline__ int page_of(const PagesDev& pg, const PrefixParams& p
     return id;
 }
 
+// one warp's rows of the row tile at r0, from tensor memory, as parts
+__device__ __forceinline__ void store_parts(const PrefixParams& p, const PrefixItem& it, int r0, int row, uint32_t o_tm,
+                                            float m, float l, uint8_t* stage) {
+    const int lane = row & 31, r = r0 + row - lane;         // the warp's first row
+    const int n = min(p.plan.rt - (row - lane), it.row_end - r);
+    if (n <= 0) return;                                     // a warp without rows
+    const int parts = p.plan.sp + p.plan.cm;
+    const size_t at = part_at(p, it, r);
+    if (lane < n) p.part_ml[at + (size_t)lane * parts] = make_float2(m * kServeScale, l);
+    store_rows(o_tm, 1.f, stage, p.part_o + at * kServeDim, (size_t)parts * kServeDim, n);
+}
+
+// the parts of the row tile at r0, one warp per row, in 32-bit arithmetic
+template <class T>
+__device__ __forceinline__ void slow_parts(const PagesDev& pg, const PrefixParams& p, const PrefixItem& it, int r0, int warp) {
+    const int lane = threadIdx.x & 31;
+    for (int x = warp; x < p.plan.rt; x += 4) {
+        const int r = r0 + x;
+        if (r >= it.row_end) return;
+        const float4 q = ld4(static_cast<const T*>(p.q) + row_off(p, it.kvh, r) + 4 * lane);
+        float m = -INFINITY, l = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        const int lim = row_seen(p, it, r);
+        for (int j = 0; j < lim; ++j) {
+            const int id = page_of(pg, p, it.slot, (it.a + j) / pg.page);
+            const size_t at = (size_t)id * p.page_stride +
+                              ((size_t)it.kvh * pg.page + (it.a + j) % pg.page) * kServeDim + 4 * lane;
+            const float4 k = ld4(static_cast<const T*>(p.kp) + at), v = ld4(static_cast<const T*>(p.vp) + at);
+            float s = fmaf(q.x, k.x, fmaf(q.y, k.y, fmaf(q.z, k.z, q.w * k.w)));
+            #pragma unroll
+            for (int y = 16; y > 0; y >>= 1) s += __shfl_xor_sync(0xffffffffu, s, y);
+            s *= kServeScale;
+            const float mn = max3(m, s, s), f = mn == -INFINITY ? 1.f : expf(m - mn);
+            const float e = mn == -INFINITY ? 0.f : expf(s - mn);
+            m = mn;
+            l = fmaf(l, f, e);
+            o.x = fmaf(e, v.x, o.x * f);
+            o.y = fmaf(e, v.y, o.y * f);
+            o.z = fmaf(e, v.z, o.z * f);
+            o.w = fmaf(e, v.w, o.w * f);
+        }
+        const size_t at = part_at(p, it, r);
+        if (lane == 0) p.part_ml[at] = make_float2(m, l);
+        st4(p.part_o + at * kServeDim + 4 * lane, o);
+    }
+}
+
 // ---------------------------------------------------------------------------
 // f16 on the tensor cores
 // ---------------------------------------------------------------------------
@@ -216,47 +264,10 @@ struct PrefixWork {
     };
     __device__ __forceinline__ void store(const Item& it, int t, int row, uint32_t o_tm, float m, float l,
                                           uint8_t* stage) const {
-        const int lane = row & 31, r = it.row0 + t * p.plan.rt + row - lane;        // the warp's first row
-        const int n = min(p.plan.rt - (row - lane), it.row_end - r);
-        if (n <= 0) return;                     // a warp without rows
-        const int parts = p.plan.sp + p.plan.cm;
-        const size_t at = part_at(p, it, r);
-        if (lane < n) p.part_ml[at + (size_t)lane * parts] = make_float2(m * kServeScale, l);
-        store_rows(o_tm, 1.f, stage, p.part_o + at * kServeDim, (size_t)parts * kServeDim, n);
+        store_parts(p, it, it.row0 + t * p.plan.rt, row, o_tm, m, l, stage);
     }
-    // one warp per row, in 32-bit arithmetic
     __device__ __forceinline__ void slow(const Item& it, int t, int warp) const {
-        const int lane = threadIdx.x & 31;
-        const __half* Q = static_cast<const __half*>(p.q);
-        for (int x = warp; x < p.plan.rt; x += 4) {
-            const int r = it.row0 + t * p.plan.rt + x;
-            if (r >= it.row_end) return;
-            const float4 q = ld4(Q + row_off(p, it.kvh, r) + 4 * lane);
-            float m = -INFINITY, l = 0.f;
-            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-            const int lim = row_seen(p, it, r);
-            for (int j = 0; j < lim; ++j) {
-                const int id = page_of(pg, p, it.slot, (it.a + j) / pg.page);
-                const size_t at = (size_t)id * p.page_stride +
-                                  ((size_t)it.kvh * pg.page + (it.a + j) % pg.page) * kServeDim + 4 * lane;
-                const float4 k = ld4(static_cast<const __half*>(p.kp) + at), v = ld4(static_cast<const __half*>(p.vp) + at);
-                float s = fmaf(q.x, k.x, fmaf(q.y, k.y, fmaf(q.z, k.z, q.w * k.w)));
-                #pragma unroll
-                for (int y = 16; y > 0; y >>= 1) s += __shfl_xor_sync(0xffffffffu, s, y);
-                s *= kServeScale;
-                const float mn = max3(m, s, s), f = mn == -INFINITY ? 1.f : expf(m - mn);
-                const float e = mn == -INFINITY ? 0.f : expf(s - mn);
-                m = mn;
-                l = fmaf(l, f, e);
-                o.x = fmaf(e, v.x, o.x * f);
-                o.y = fmaf(e, v.y, o.y * f);
-                o.z = fmaf(e, v.z, o.z * f);
-                o.w = fmaf(e, v.w, o.w * f);
-            }
-            const size_t at = part_at(p, it, r);
-            if (lane == 0) p.part_ml[at] = make_float2(m, l);
-            st4(p.part_o + at * kServeDim + 4 * lane, o);
-        }
+        slow_parts<__half>(pg, p, it, it.row0 + t * p.plan.rt, warp);
     }
 };
 
@@ -307,6 +318,46 @@ attn_prefix_simt_kernel(const __grid_constant__ PagesDev pg, const __grid_consta
         if (tx == 0) p.part_ml[at] = make_float2(st.m[i], st.l[i]);
         simt_store(st, i, 1.f, p.part_o + at * kServeDim);
     }
+}
+
+// ---------------------------------------------------------------------------
+// 32-bit on the tensor cores: one item of up to 128 rows per CTA. Groups of
+// more than 128 f16 heads come here too.
+// ---------------------------------------------------------------------------
+template <class KV>
+struct PrefixWide {
+    using T = KV;
+    using Item = PrefixItem;
+    const PagesDev& pg;
+    const PrefixParams& p;
+
+    __device__ __forceinline__ bool find(long long x, Item* it) const { return find_item(pg, p, x, it); }
+    __device__ __forceinline__ int keys(const Item& it) const { return it.keys; }
+    __device__ __forceinline__ bool live(const Item& it, int row) const { return it.row0 + row < it.row_end; }
+    __device__ __forceinline__ int seen(const Item& it, int row) const {
+        return live(it, row) ? row_seen(p, it, it.row0 + row) : it.keys;
+    }
+    __device__ __forceinline__ const T* q_row(const Item& it, int row) const {
+        return static_cast<const T*>(p.q) + row_off(p, it.kvh, it.row0 + row);
+    }
+    __device__ __forceinline__ const T* kv_row(const Item& it, const void* pool, int key) const {
+        const int id = page_of(pg, p, it.slot, (it.a + key) / pg.page);
+        return static_cast<const T*>(pool) + (size_t)id * p.page_stride +
+               ((size_t)it.kvh * pg.page + (it.a + key) % pg.page) * kServeDim;
+    }
+    __device__ __forceinline__ const T* k_row(const Item& it, int key) const { return kv_row(it, p.kp, key); }
+    __device__ __forceinline__ const T* v_row(const Item& it, int key) const { return kv_row(it, p.vp, key); }
+    __device__ __forceinline__ void store(const Item& it, int row, uint32_t o_tm, float m, float l, uint8_t* stage) const {
+        store_parts(p, it, it.row0, row, o_tm, m, l, stage);
+    }
+    __device__ __forceinline__ void slow(const Item& it, int warp) const { slow_parts<T>(pg, p, it, it.row0, warp); }
+};
+
+template <class KV>
+__global__ void __launch_bounds__(kWdThreads, 1)
+attn_prefix_wide_kernel(const __grid_constant__ PagesDev pg, const __grid_constant__ PrefixParams p) {
+    pdl_trigger();
+    attn_wide_core(PrefixWide<KV>{pg, p});
 }
 
 // ---------------------------------------------------------------------------
@@ -385,7 +436,7 @@ Plan make_plan(const sllm_cuda_kv_pages& p, int n, int n_q, int n_head, int pref
     const bool mma = p.kv_type == SLLM_CUDA_KV_F16 && group <= kAtRows;
     Plan pl{};
     pl.key_tile = mma ? kAtKeys : kSimtKeys;
-    pl.rt = mma ? kAtRows / group * group : rows <= kSimtRows<1> ? kSimtRows<1> : kSimtRows<4>;
+    pl.rt = mma ? kAtRows / group * group : rows <= kSimtRows<1> ? kSimtRows<1> : kAtRows;
     pl.per = mma ? 2 : 1;
     auto items = [&](int r) { return (r + pl.rt * pl.per - 1) / (pl.rt * pl.per); };
     pl.ri_all = items(rows);
@@ -466,12 +517,17 @@ cudaError_t launch_mma(const sllm_cuda_kv_pages& pages, const PagesDev& pg, cons
                   tq, tk, tv, pg, p);
 }
 
-template <int R, class T>
-cudaError_t launch_simt(const PagesDev& pg, const PrefixParams& p, cudaStream_t st) {
-    const cudaError_t e = allow_smem<attn_prefix_simt_kernel<R, T>>(kSimtSmem<R>);
-    if (e != cudaSuccess) return e;
-    return launch(attn_prefix_simt_kernel<R, T>, dim3((unsigned)item_numbers(p)), dim3(kSimtThreads), kSimtSmem<R>, st,
-                  false, pg, p);
+template <class T>
+cudaError_t launch_32(const PagesDev& pg, const PrefixParams& p, cudaStream_t st) {
+    const dim3 grid((unsigned)item_numbers(p));
+    if (p.plan.rt == kAtRows) {
+        const cudaError_t e = allow_smem<attn_prefix_wide_kernel<T>>(kWdSmem);
+        return e != cudaSuccess ? e
+                                : launch(attn_prefix_wide_kernel<T>, grid, dim3(kWdThreads), kWdSmem, st, false, pg, p);
+    }
+    const cudaError_t e = allow_smem<attn_prefix_simt_kernel<1, T>>(kSimtSmem<1>);
+    return e != cudaSuccess ? e
+                            : launch(attn_prefix_simt_kernel<1, T>, grid, dim3(kSimtThreads), kSimtSmem<1>, st, false, pg, p);
 }
 
 int check_shape(const sllm_cuda_kv_pages* p, int n, int n_q, int n_head, int prefix, const char* who) {
@@ -540,14 +596,9 @@ extern "C" int sllm_cuda_attn_prefix(const sllm_cuda_kv_pages* p, int32_t layer,
     if (item_numbers(a) > 0x3fffffffLL) return fail(SLLM_CUDA_ERR_TOO_LARGE, "attn_prefix: %d sequences", n);
     const PagesDev pg = pages_dev(*p);
     const cudaStream_t st = (cudaStream_t)stream;
-    const bool few = a.plan.rt == kSimtRows<1>;
-    cudaError_t e;
-    if (p->kv_type == SLLM_CUDA_KV_F32)
-        e = few ? launch_simt<1, float>(pg, a, st) : launch_simt<4, float>(pg, a, st);
-    else if (a.group > kAtRows)
-        e = few ? launch_simt<1, __half>(pg, a, st) : launch_simt<4, __half>(pg, a, st);
-    else
-        e = launch_mma(*p, pg, a, sms, st);
+    const cudaError_t e = p->kv_type == SLLM_CUDA_KV_F32 ? launch_32<float>(pg, a, st)
+                          : a.group > kAtRows            ? launch_32<__half>(pg, a, st)
+                                                         : launch_mma(*p, pg, a, sms, st);
     CK(e, "attn_prefix launch");
     const dim3 grid((unsigned)(((long long)n * n_q * n_head + 7) / 8));
     CK(out_type == SLLM_CUDA_KV_F32 ? launch(attn_prefix_join_kernel<float>, grid, dim3(256), 0, st, true, pg, a)

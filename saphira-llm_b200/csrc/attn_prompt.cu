@@ -4,11 +4,11 @@
 // of a sequence sees its tokens 0 .. i.
 
 //
-// f16: attn_prompt_mma_kernel, on the tensor cores. f32: the 32-bit kernel
-// of attn_simt.cuh.
+// f16: attn_prompt_mma_kernel over attn_mma.cuh. f32: attn_prompt_wide_kernel
+// over attn_wide.cuh.
 
 #include "attn_mma.cuh"
-#include "attn_simt.cuh"
+#include "attn_wide.cuh"
 
 namespace sllm {
 namespace {
@@ -64,44 +64,6 @@ __device__ __forceinline__ bool find_long_first(const PromptParams& p, int x, in
     return false;
 }
 
-template <class T, class O>
-__global__ void __launch_bounds__(kSimtThreads, 2)
-attn_prompt_simt_kernel(const __grid_constant__ PromptParams p) {
-    extern __shared__ float sm[];
-    int start, len, tile;
-    if (!find_long_first<kSimtRows<4>>(p, blockIdx.x / p.n_head, &start, &len, &tile)) return;
-    const int h = blockIdx.x % p.n_head, kvh = h / p.group, r0 = tile * kSimtRows<4>;
-    const T* q = static_cast<const T*>(p.q) + (size_t)h * kServeDim;
-    const T* k = static_cast<const T*>(p.k) + (size_t)kvh * kServeDim;
-    const T* v = static_cast<const T*>(p.v) + (size_t)kvh * kServeDim;
-    simt_load_q<4, T>(sm, [&](int r) -> const T* { return r0 + r < len ? q + (size_t)(start + r0 + r) * p.qs : nullptr; });
-    SimtState<4> st;
-    simt_init(st);
-    const int ty = threadIdx.x >> 4;
-    int lim[4];
-    #pragma unroll
-    for (int i = 0; i < 4; ++i) lim[i] = min(r0 + 4 * ty + i + 1, len);
-    const int end = min(r0 + kSimtRows<4>, len);
-    for (int j0 = 0; j0 < end; j0 += kSimtKeys)
-        simt_tile<4, T>(sm, st, j0, lim,
-                     [&](int j) -> const T* { return j < end ? k + (size_t)(start + j) * p.ks : nullptr; },
-                     [&](int j) -> const T* { return j < end ? v + (size_t)(start + j) * p.vs : nullptr; });
-    #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (r0 + 4 * ty + i < len)
-            simt_store(st, i, __fdiv_rn(1.f, st.l[i]),
-                       static_cast<O*>(p.out) + (size_t)(start + r0 + 4 * ty + i) * p.os + (size_t)h * kServeDim);
-}
-
-template <class T, class O>
-cudaError_t launch_simt(const PromptParams& p, cudaStream_t st) {
-    const cudaError_t e = allow_smem<attn_prompt_simt_kernel<T, O>>(kSimtSmem<4>);
-    if (e != cudaSuccess) return e;
-    // every sequence may end inside a tile
-    const long long tiles = (p.n_tokens + kSimtRows<4> - 1) / kSimtRows<4> + (long long)p.n_seq;
-    return launch(attn_prompt_simt_kernel<T, O>, dim3((unsigned)(tiles * p.n_head)), dim3(kSimtThreads), kSimtSmem<4>, st, false, p);
-}
-
 // ---------------------------------------------------------------------------
 // The f16 kernel: attn_mma.cuh's core over items of 256 query rows of one
 // head, from the start of the sequence to the diagonal.
@@ -110,15 +72,15 @@ constexpr int kPmRows = 2 * kAtRows;
 
 // rows [first, first + 128) of a sequence, one warp per row at a time, in
 // 32-bit arithmetic: the way out for values that are no numbers
-template <class O>
+template <class T, class O>
 __device__ __forceinline__ void slow_rows(const PromptParams& p, int h, int start, int len, int first, int warp) {
     const int lane = threadIdx.x & 31, kvh = h / p.group;
-    const __half* K = static_cast<const __half*>(p.k) + (size_t)kvh * kServeDim + 4 * lane;
-    const __half* V = static_cast<const __half*>(p.v) + (size_t)kvh * kServeDim + 4 * lane;
+    const T* K = static_cast<const T*>(p.k) + (size_t)kvh * kServeDim + 4 * lane;
+    const T* V = static_cast<const T*>(p.v) + (size_t)kvh * kServeDim + 4 * lane;
     for (int r = warp; r < kAtRows; r += 4) {
         const int i = first + r;
         if (i >= len) return;
-        const float4 q = ld4(static_cast<const __half*>(p.q) + (size_t)(start + i) * p.qs + (size_t)h * kServeDim + 4 * lane);
+        const float4 q = ld4(static_cast<const T*>(p.q) + (size_t)(start + i) * p.qs + (size_t)h * kServeDim + 4 * lane);
         float m = -INFINITY, l = 0.f;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int j = 0; j <= i; ++j) {
@@ -195,7 +157,7 @@ struct PromptWork {
                    p.os, it.len - x0);
     }
     __device__ __forceinline__ void slow(const Item& it, int t, int warp) const {
-        slow_rows<O>(p, it.head, it.start, it.len, it.tile * kPmRows + kAtRows * t, warp);
+        slow_rows<__half, O>(p, it.head, it.start, it.len, it.tile * kPmRows + kAtRows * t, warp);
     }
 };
 
@@ -204,6 +166,57 @@ __global__ void __launch_bounds__(kAtThreads, 1)
 attn_prompt_mma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                        const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ PromptParams p) {
     attn_core(PromptWork<O>{p, tm_q, tm_k, tm_v});
+}
+
+// ---------------------------------------------------------------------------
+// The f32 kernel: attn_wide.cuh's core, 128 query rows a CTA.
+// ---------------------------------------------------------------------------
+struct PromptWide {
+    using T = float;
+    struct Item {
+        int start, len, tile, head;
+        __device__ bool last() const { return tile < 0; }
+    };
+    const PromptParams& p;
+
+    __device__ __forceinline__ bool find(long long x, Item* it) const {      // longest first
+        it->head = (int)(x % p.n_head);
+        return find_long_first<kAtRows>(p, (int)(x / p.n_head), &it->start, &it->len, &it->tile);
+    }
+    __device__ __forceinline__ int keys(const Item& it) const { return min((it.tile + 1) * kAtRows, it.len); }
+    __device__ __forceinline__ int seen(const Item& it, int row) const { return min(it.tile * kAtRows + row + 1, it.len); }
+    __device__ __forceinline__ bool live(const Item& it, int row) const { return it.tile * kAtRows + row < it.len; }
+    __device__ __forceinline__ const float* q_row(const Item& it, int row) const {
+        return static_cast<const float*>(p.q) + (size_t)(it.start + it.tile * kAtRows + row) * p.qs +
+               (size_t)it.head * kServeDim;
+    }
+    __device__ __forceinline__ const float* k_row(const Item& it, int key) const {
+        return static_cast<const float*>(p.k) + (size_t)(it.start + key) * p.ks + (size_t)(it.head / p.group) * kServeDim;
+    }
+    __device__ __forceinline__ const float* v_row(const Item& it, int key) const {
+        return static_cast<const float*>(p.v) + (size_t)(it.start + key) * p.vs + (size_t)(it.head / p.group) * kServeDim;
+    }
+    __device__ __forceinline__ void store(const Item& it, int row, uint32_t o_tm, float, float l, uint8_t* stage) const {
+        const int x0 = it.tile * kAtRows + (row & ~31);
+        store_rows(o_tm, 1.f / l, stage,
+                   static_cast<float*>(p.out) + (size_t)(it.start + x0) * p.os + (size_t)it.head * kServeDim, p.os,
+                   it.len - x0);
+    }
+    __device__ __forceinline__ void slow(const Item& it, int warp) const {
+        slow_rows<float, float>(p, it.head, it.start, it.len, it.tile * kAtRows, warp);
+    }
+};
+
+__global__ void __launch_bounds__(kWdThreads, 1) attn_prompt_wide_kernel(const __grid_constant__ PromptParams p) {
+    attn_wide_core(PromptWide{p});
+}
+
+cudaError_t launch_wide(const PromptParams& p, cudaStream_t st) {
+    const cudaError_t e = allow_smem<attn_prompt_wide_kernel>(kWdSmem);
+    if (e != cudaSuccess) return e;
+    // every sequence may end inside a tile
+    const long long tiles = p.n_tokens / kAtRows + (long long)p.n_seq;
+    return launch(attn_prompt_wide_kernel, dim3((unsigned)(tiles * p.n_head)), dim3(kWdThreads), kWdSmem, st, false, p);
 }
 
 // [tokens][heads][128] f16 as (64 dims of a half, head, token) boxes of
@@ -277,7 +290,7 @@ extern "C" int sllm_cuda_attn_prompt(const void* q, size_t q_stride, const void*
     p.cu = cu_seqlens;
     p.n_seq = n_seq; p.n_tokens = n_tokens; p.n_head = n_head; p.group = n_head / n_head_kv;
     const cudaStream_t st = (cudaStream_t)stream;
-    const cudaError_t e = type == SLLM_CUDA_KV_F32 ? launch_simt<float, float>(p, st)
+    const cudaError_t e = type == SLLM_CUDA_KV_F32 ? launch_wide(p, st)
                           : out_type == SLLM_CUDA_KV_F32 ? launch_mma<float>(p, st)
                                                          : launch_mma<__half>(p, st);
     CK(e, "attn_prompt launch");

@@ -30,7 +30,6 @@ template <int R> constexpr int kSimtPPad = 16 * R + 4;
 template <int R>
 constexpr int kSimtSmem = 4 * (kSimtRows<R> * kSimtDPad + kSimtKeys * kSimtDPad + kSimtKeys * kServeDim);
 static_assert(kSimtKeys * kSimtPPad<4> <= kSimtKeys * kSimtDPad, "the weights fit the keys' place");
-constexpr float kServeScale = 0.08838834764831845f;     // 1 / sqrt(128)
 
 // two f32 at a time (sm_100's packed pipe): x += a * b
 __device__ __forceinline__ void mad2(float2& x, float a0, float a1, float b0, float b1) {

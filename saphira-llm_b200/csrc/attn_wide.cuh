@@ -1,0 +1,326 @@
+// attn_wide.cuh -- attention of 32-bit operands on the tensor cores.
+//
+// An f32 is the sum of three bf16, 24 bits in all, with f32's range: x = x1 +
+// x2 + x3, x1 = bf16(x), x2 = bf16(x - x1), x3 = bf16(x - x1 - x2) (the
+// differences are exact). A product is the six partial products whose size is
+// above 2^-25 of it,
+//     x y = x1 y1 + x1 y2 + x2 y1 + x2 y2 + x1 y3 + x3 y1,
+// each exact in the tensor core's f32 accumulator: as good as 32-bit
+// multiply-adds, at a sixth of the bf16 rate, which is still four times the
+// ordinary pipe's.
+//
+// One CTA: 128 query rows of one head against 64 keys at a time.
+//
+//   warps 0-3        softmax, one thread per row; at the end the outputs.
+//   warps 4-7, 8-11  the operands: both groups the rows of Q, then one the key
+//                    and one the value tiles: from global memory (the next
+//                    tile waits in registers), split, into shared memory in
+//                    the layouts the products want.
+//   warp 12, 1 lane  tcgen05.mma: 6 x 8 products of N = 64 for a tile's scores,
+//                    6 x 4 of N = 128 for the outputs, with the weights' planes
+//                    from tensor memory. The scores of tile j + 1 are made
+//                    under the softmax of tile j.
+//
+// Products of different shapes are not ordered among themselves, so none
+// touches tensor memory that one of the other shape reads or writes, except
+// across a commit: scores 2 x 64 columns, weights 2 x 96, outputs 128. (One
+// product of N = 192 over a key tile's three planes, the softmax adding the
+// column groups, would need 1664 clocks for the scores instead of 2304, but
+// partial sums of three shapes would lean on an order that is not promised.)
+//
+// Bound by the products: the scores' operands come from shared memory, 6 KB in
+// 48 clocks each; 48 x 48 + 24 x 64 = 3840 clocks a tile of 4.2 MFLOP, 290
+// TFLOP/s over 148 SMs at 1.8 GHz.
+//
+// Masks as in attn_mma.cuh: rows behind the keys are stored as zeros; a value
+// that is no number, among keys that not every row sees, makes the CTA
+// recompute its rows one by one. A key or value that a row does see and that
+// is no finite number makes that row no number.
+#pragma once
+
+#include "attn_mma.cuh"
+
+namespace sllm {
+
+constexpr int kWdKeys = 64;
+constexpr int kWdQPlane = kAtTile;                      // 128 rows x 128 bf16
+constexpr int kWdHalf = kWdKeys * 128, kWdPlane = 2 * kWdHalf;      // 64 rows x 64 bf16, x 128
+constexpr int kWdK = 3 * kWdQPlane, kWdV = kWdK + 3 * kWdPlane, kWdEnd = kWdV + 3 * kWdPlane;
+constexpr int kWdP = 128, kWdO = 320;                   // tensor memory columns: weights, outputs
+constexpr int kWdSmem = kWdEnd + 1024;
+constexpr int kWdThreads = 32 * 13;
+
+__host__ __device__ constexpr uint32_t umma_idesc_bf16(int M, int N, bool b_mn) {
+    return umma_idesc_f16(M, N, b_mn) | (1u << 7) | (1u << 10);
+}
+
+__device__ __forceinline__ uint32_t pack_bf2(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+// two f32 into three words of two bf16 (finite ones; of others only the first
+// word means something)
+__device__ __forceinline__ void split2(float a, float b, uint32_t& p1, uint32_t& p2, uint32_t& p3) {
+    p1 = pack_bf2(a, b);
+    a = __fsub_rn(a, __uint_as_float(p1 << 16));
+    b = __fsub_rn(b, __uint_as_float(p1 & 0xffff0000u));
+    p2 = pack_bf2(a, b);
+    p3 = pack_bf2(__fsub_rn(a, __uint_as_float(p2 << 16)), __fsub_rn(b, __uint_as_float(p2 & 0xffff0000u)));
+}
+
+// false when one of four is no finite number, or one that bf16 would round to
+// infinity
+__device__ __forceinline__ bool plain4(float4 x) {
+    const float t = max3(fabsf(x.x), fabsf(x.y), fabsf(x.z));
+    return max3(t, fabsf(x.w), t) < 0x1.fep127f;
+}
+
+// four elements of a row into its three planes: `at` is the row's 128 bytes of
+// the lane's half in the first plane, r its number in the swizzle. What is no
+// finite number lies in the first plane alone.
+__device__ __forceinline__ void store_planes(uint8_t* at, int r, int lane, int plane, float4 x, bool plain) {
+    uint32_t a[3], b[3];
+    split2(x.x, x.y, a[0], a[1], a[2]);
+    split2(x.z, x.w, b[0], b[1], b[2]);
+    if (!plain) a[1] = a[2] = b[1] = b[2] = 0u;
+    uint8_t* p = at + ((((lane & 15) >> 1) ^ (r & 7)) << 4) + (lane & 1) * 8;
+    #pragma unroll
+    for (int i = 0; i < 3; ++i) *reinterpret_cast<uint2*>(p + i * plane) = make_uint2(a[i], b[i]);
+}
+
+// W: Item; T; find(x, item); keys(item); live(item, row); seen(item, row) (at
+// most keys, least for row 0); q_row(item, row), k_row(item, key),
+// v_row(item, key); store(...), slow(...).
+template <class W>
+__device__ __forceinline__ void attn_wide_core(const W w) {
+    using T = typename W::T;
+    int* const err = &g_attn_error;
+    extern __shared__ __align__(1024) uint8_t sm[];
+    struct Shared {
+        // q: split; k, v: tile split; kf, vf: its products done; s: scores; p: weights; o: all
+        uint64_t bar_q, bar_k, bar_kf, bar_v, bar_vf, bar_s[2], bar_p[2], bar_o;
+        uint32_t tmem;
+        int abort_flag, odd;
+    };
+    static_assert(sizeof(Shared) <= kWdSmem - kWdEnd, "the part behind the planes");
+    Shared& sh = *reinterpret_cast<Shared*>(sm + kWdEnd);
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    typename W::Item it;
+    if (!w.find(blockIdx.x, &it) || it.last()) return;      // the grid is an upper bound
+    if ((smem_u32(sm) & 1023u) != 0) {
+        if (threadIdx.x == 0) atomicExch(err, 2);
+        return;
+    }
+    if (threadIdx.x == 0) {
+        mbar_init(&sh.bar_q, 8);
+        mbar_init(&sh.bar_k, 4);
+        mbar_init(&sh.bar_kf, 1);
+        mbar_init(&sh.bar_v, 4);
+        mbar_init(&sh.bar_vf, 1);
+        mbar_init(&sh.bar_s[0], 1);
+        mbar_init(&sh.bar_s[1], 1);
+        mbar_init(&sh.bar_p[0], 4);
+        mbar_init(&sh.bar_p[1], 4);
+        mbar_init(&sh.bar_o, 1);
+        sh.abort_flag = 0;
+        sh.odd = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)),
+                     "r"(512u)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sh.tmem;
+    volatile int* const ab = &sh.abort_flag;
+    const int keys = w.keys(it), n = (keys + kWdKeys - 1) / kWdKeys;
+
+    if (warp < 4) {
+        // ---------------- softmax ----------------
+        const int row = threadIdx.x;
+        const uint32_t lanes = (uint32_t)(32 * warp) << 16, o_tm = tmem + lanes + kWdO;
+        const bool live = w.live(it, row);
+        const int seen = w.seen(it, row);
+        float m = -INFINITY, l = 0.f;
+        bool ok = true;
+        for (int j = 0; j < n; ++j) {
+            const uint32_t s_tm = tmem + lanes + 64 * (j & 1), p_tm = tmem + lanes + kWdP + 96 * (j & 1);
+            if (!(ok = at_wait_warp(&sh.bar_s[j & 1], (j >> 1) & 1, ab, err))) break;
+            tc_fence_after();
+            float s[64];
+            {
+                uint32_t a[32], b[32];
+                tmem_ld32(s_tm, a);
+                tmem_ld32(s_tm + 32, b);
+                tmem_ld_wait();
+                #pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    s[i] = __uint_as_float(a[i]);
+                    s[32 + i] = __uint_as_float(b[i]);
+                }
+            }
+            const int lim = seen - j * kWdKeys;
+            if (__any_sync(0xffffffffu, lim < kWdKeys)) {
+                #pragma unroll
+                for (int c = 0; c < 64; ++c) s[c] = c < lim ? s[c] : -INFINITY;
+            }
+            float mx = max3(s[0], s[1], s[2]);
+            #pragma unroll
+            for (int c = 3; c < 63; c += 2) mx = max3(mx, s[c], s[c + 1]);
+            mx = max3(mx, s[63], s[63]);
+            // (a row that is none may hold anything: it never asks for more)
+            const bool fine = (mx - m) * kAtScale2 <= kAtLag || mx == -INFINITY || !live;
+            if (!__all_sync(0xffffffffu, fine)) {
+                const float m1 = fine ? m : max3(m, mx, mx);
+                const float f = fine ? 1.f : ex2((m - m1) * kAtScale2);
+                m = m1;
+                l *= f;
+                if (j > 0) {
+                    // the products before are complete when the values' place is free
+                    if (!(ok = at_wait_warp(&sh.bar_vf, (j - 1) & 1, ab, err))) break;
+                    tc_fence_after();
+                    #pragma unroll 1
+                    for (int c = 0; c < 8; ++c) {
+                        uint32_t r[16];
+                        tmem_ld16(o_tm + 16 * c, r);
+                        tmem_ld_wait();
+                        #pragma unroll
+                        for (int e = 0; e < 16; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * f);
+                        tmem_st16(o_tm + 16 * c, r);
+                    }
+                }
+            }
+            const float mc = weight_offset(m);
+            float sum0 = 0.f, sum1 = 0.f;
+            #pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                uint32_t u[3][16];
+                #pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    float x0, x1;
+                    fma2v(x0, x1, s[32 * h + 2 * i], s[32 * h + 2 * i + 1], kAtScale2, kAtScale2, mc, mc);
+                    x0 = ex2(x0);
+                    x1 = ex2(x1);
+                    add2(sum0, sum1, x0, x1);
+                    split2(x0, x1, u[0][i], u[1][i], u[2][i]);
+                }
+                #pragma unroll
+                for (int q = 0; q < 3; ++q) tmem_st16(p_tm + 32 * q + 16 * h, u[q]);
+            }
+            l += sum0 + sum1;
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.bar_p[j & 1]);      // (tile j + 1's may come before tile j's products)
+        }
+        if (ok && at_wait_warp(&sh.bar_o, 0, ab, err)) {
+            tc_fence_after();
+            if (*(volatile int*)&sh.odd != 0) w.slow(it, warp);
+            else w.store(it, row, o_tm, m, l, sm + warp * kAtStage);      // the query planes' place is free
+        }
+    } else if (warp < 12) {
+        // ---------------- operands ----------------
+        const int cw = warp & 3, half = lane >> 4, every = w.seen(it, 0);
+        const bool is_v = warp >= 8;
+        const float4 none = make_float4(0.f, 0.f, 0.f, 0.f);
+        float4 r[16];                   // this warp's rows cw, cw + 4, .. of a tile
+        auto load = [&](int j) {
+            #pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int key = j * kWdKeys + cw + 4 * i;
+                const T* at = key < keys ? (is_v ? w.v_row(it, key) : w.k_row(it, key)) : nullptr;
+                r[i] = at != nullptr ? ld4(at + 4 * lane) : none;
+            }
+        };
+        load(0);
+        #pragma unroll 2
+        for (int i = 0; i < kAtRows / 8; ++i) {
+            const int row = (warp - 4) + 8 * i;
+            const float4 x = w.live(it, row) ? ld4(w.q_row(it, row) + 4 * lane) : none;
+            store_planes(sm + half * kAtHalf + row * 128, row, lane, kWdQPlane, x, plain4(x));
+        }
+        auto arrive = [&](uint64_t* bar) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar);
+        };
+        arrive(&sh.bar_q);
+        uint8_t* const tile = sm + (is_v ? kWdV : kWdK) + half * kWdHalf;
+        #pragma unroll 1
+        for (int j = 0; j < n; ++j) {
+            if (j > 0 && !at_wait_warp(is_v ? &sh.bar_vf : &sh.bar_kf, (j - 1) & 1, ab, err)) break;
+            bool odd = false;
+            #pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int row = cw + 4 * i;
+                const bool plain = plain4(r[i]);
+                store_planes(tile + row * 128, row, lane, kWdPlane, r[i], plain);
+                odd = odd || (!plain && j * kWdKeys + row >= every);
+            }
+            if (is_v && odd) sh.odd = 1;
+            arrive(is_v ? &sh.bar_v : &sh.bar_k);
+            if (j + 1 < n) load(j + 1);
+        }
+    } else {
+        if (elect_one()) {
+            // ---------------- products ----------------
+            const uint32_t q0 = umma_desc_lo(smem_u32(sm), 16), k0 = umma_desc_lo(smem_u32(sm + kWdK), 16),
+                           v0 = umma_desc_lo(smem_u32(sm + kWdV), kWdHalf);
+            constexpr int first[6] = {2, 0, 1, 1, 0, 0}, second[6] = {0, 2, 1, 0, 1, 0};    // the small ones first
+            auto scores = [&](int j) {
+                const uint32_t d = tmem + 64 * (j & 1);
+                #pragma unroll
+                for (int y = 0; y < 6; ++y)
+                    #pragma unroll
+                    for (int x = 0; x < 8; ++x)
+                        umma_f16_ss(d, q0 + ((first[y] * kWdQPlane + (x >> 2) * kAtHalf + (x & 3) * 32) >> 4),
+                                    k0 + ((second[y] * kWdPlane + (x >> 2) * kWdHalf + (x & 3) * 32) >> 4),
+                                    umma_idesc_bf16(128, 64, false), x > 0 || y > 0);
+                umma_commit(&sh.bar_s[j & 1]);
+                umma_commit(&sh.bar_kf);
+            };
+            auto outputs = [&](int j) {
+                const uint32_t p = tmem + kWdP + 96 * (j & 1), d = tmem + kWdO;
+                #pragma unroll
+                for (int y = 0; y < 6; ++y)
+                    #pragma unroll
+                    for (int x = 0; x < 4; ++x)
+                        umma_f16_ts(d, p + 32 * first[y] + 8 * x, v0 + ((second[y] * kWdPlane + x * 2048) >> 4),
+                                    umma_idesc_bf16(128, 128, true), j > 0 || x > 0 || y > 0);
+                umma_commit(&sh.bar_vf);
+            };
+            bool ok = at_wait(&sh.bar_q, 0, ab, err) && at_wait(&sh.bar_k, 0, ab, err);
+            if (ok) {
+                tc_fence_after();
+                scores(0);
+            }
+            #pragma unroll 1
+            for (int j = 0; j < n && ok; ++j) {
+                if (j + 1 < n) {
+                    if (!(ok = at_wait(&sh.bar_k, (j + 1) & 1, ab, err))) break;
+                    tc_fence_after();
+                    scores(j + 1);
+                }
+                if (!(ok = at_wait(&sh.bar_v, j & 1, ab, err) && at_wait(&sh.bar_p[j & 1], (j >> 1) & 1, ab, err))) break;
+                tc_fence_after();
+                outputs(j);
+            }
+            umma_commit(&sh.bar_o);
+            at_drain(&sh.bar_o, 0);
+        }
+        __syncwarp();
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 12) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+}
+
+}  // namespace sllm

@@ -13,6 +13,7 @@
 namespace sllm {
 
 constexpr int kServeDim = 128;      // the head dimension of every model the library runs
+constexpr float kServeScale = 0.08838834764831845f;     // 1 / sqrt(128)
 
 // OK when p is memory of the current device (a kernel given a host pointer or
 // another device's would fault); the message names the argument.

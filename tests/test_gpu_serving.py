@@ -173,8 +173,11 @@ def test_prompt_wrong_offsets_stay_inside(cuda):
 
 def test_no_bounded_wait_gave_up(cuda):
     import torch
-    q, k, v = (_rand(s, 3000, 2, 128, dt=torch.float16) for s in (1, 2, 3))
-    cuda.attn_prompt(q, k, v, torch.empty_like(q), _i32([0, 2000, 3000]))
+    for dt in ("f16", "f32"):
+        q, k, v = (_rand(s, 3000, 2, 128, dt=_dt(dt)) for s in (1, 2, 3))
+        cuda.attn_prompt(q, k, v, torch.empty_like(q), _i32([0, 2000, 3000]))
+        c = shared_cache(cuda, 1024, [300] * 9, 16, (20, 5), dt)
+        run_prefix(cuda, c, list(range(9)), 2, (20, 5), 1024, dt)
     assert cuda.attn_error() == 0
 
 
