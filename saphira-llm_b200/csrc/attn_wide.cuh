@@ -1,8 +1,8 @@
 // attn_wide.cuh -- attention of 32-bit operands on the tensor cores.
 //
 // An f32 is the sum of three bf16, 24 bits in all, with f32's range: x = x1 +
-// x2 + x3, x1 = bf16(x), x2 = bf16(x - x1), x3 = bf16(x - x1 - x2) (the
-// differences are exact). A product is the six partial products whose size is
+// x2 + x3, x1 = x rounded to bf16, x2 = the first eight bits of x - x1, x3 = the
+// rest (the differences are exact). A product is the six partial products whose size is
 // above 2^-25 of it,
 //     x y = x1 y1 + x1 y2 + x2 y1 + x2 y2 + x1 y3 + x3 y1,
 // each exact in the tensor core's f32 accumulator: as good as 32-bit
@@ -12,11 +12,12 @@
 // One CTA: 128 query rows of one head against 64 keys at a time.
 //
 //   warps 0-3        softmax, one thread per row; at the end the outputs.
-//   warps 4-7, 8-11  the operands: both groups the rows of Q, then one the key
+//   warps 4-11, 12-19  the operands: both groups the rows of Q, then one the key
 //                    and one the value tiles: from global memory (the next
 //                    tile waits in registers), split, into shared memory in
-//                    the layouts the products want.
-//   warp 12, 1 lane  tcgen05.mma: 6 x 8 products of N = 64 for a tile's scores,
+//                    the layouts the products want. Sixteen warps: with eight
+//                    the splitting took twice the products' time.
+//   warp 20, 1 lane  tcgen05.mma: 6 x 8 products of N = 64 for a tile's scores,
 //                    6 x 4 of N = 128 for the outputs, with the weights' planes
 //                    from tensor memory. The scores of tile j + 1 are made
 //                    under the softmax of tile j.
@@ -31,6 +32,9 @@
 // Bound by the products: the scores' operands come from shared memory, 6 KB in
 // 48 clocks each; 48 x 48 + 24 x 64 = 3840 clocks a tile of 4.2 MFLOP, 290
 // TFLOP/s over 148 SMs at 1.8 GHz.
+//
+// Registers: 768 threads x 80 at launch; 152 (softmax) + 4 x 72 (operands) + 40
+// = 480 = 6 x 80 after the split.
 //
 // Masks as in attn_mma.cuh: rows behind the keys are stored as zeros; a value
 // that is no number, among keys that not every row sees, makes the CTA
@@ -48,7 +52,7 @@ constexpr int kWdHalf = kWdKeys * 128, kWdPlane = 2 * kWdHalf;      // 64 rows x
 constexpr int kWdK = 3 * kWdQPlane, kWdV = kWdK + 3 * kWdPlane, kWdEnd = kWdV + 3 * kWdPlane;
 constexpr int kWdP = 128, kWdO = 320;                   // tensor memory columns: weights, outputs
 constexpr int kWdSmem = kWdEnd + 1024;
-constexpr int kWdThreads = 32 * 13;
+constexpr int kWdThreads = 32 * 24;
 
 __host__ __device__ constexpr uint32_t umma_idesc_bf16(int M, int N, bool b_mn) {
     return umma_idesc_f16(M, N, b_mn) | (1u << 7) | (1u << 10);
@@ -61,12 +65,16 @@ __device__ __forceinline__ uint32_t pack_bf2(float lo, float hi) {
 }
 // two f32 into three words of two bf16 (finite ones; of others only the first
 // word means something)
+__device__ __forceinline__ uint32_t upper2(float lo, float hi) {
+    return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632);
+}
+__device__ __forceinline__ float upper(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
 __device__ __forceinline__ void split2(float a, float b, uint32_t& p1, uint32_t& p2, uint32_t& p3) {
     p1 = pack_bf2(a, b);
     a = __fsub_rn(a, __uint_as_float(p1 << 16));
     b = __fsub_rn(b, __uint_as_float(p1 & 0xffff0000u));
-    p2 = pack_bf2(a, b);
-    p3 = pack_bf2(__fsub_rn(a, __uint_as_float(p2 << 16)), __fsub_rn(b, __uint_as_float(p2 & 0xffff0000u)));
+    p2 = upper2(a, b);
+    p3 = upper2(__fsub_rn(a, upper(a)), __fsub_rn(b, upper(b)));
 }
 
 // false when one of four is no finite number, or one that bf16 would round to
@@ -98,8 +106,9 @@ __device__ __forceinline__ void attn_wide_core(const W w) {
     int* const err = &g_attn_error;
     extern __shared__ __align__(1024) uint8_t sm[];
     struct Shared {
-        // q: split; k, v: tile split; kf, vf: its products done; s: scores; p: weights; o: all
-        uint64_t bar_q, bar_k, bar_kf, bar_v, bar_vf, bar_s[2], bar_p[2], bar_o;
+        // q: split; k, v: tile split; vf: its products done; s: scores (and the
+        // keys' place free); p: weights; o: all
+        uint64_t bar_q, bar_k, bar_v, bar_vf, bar_s[2], bar_p[2], bar_o;
         uint32_t tmem;
         int abort_flag, odd;
     };
@@ -113,10 +122,9 @@ __device__ __forceinline__ void attn_wide_core(const W w) {
         return;
     }
     if (threadIdx.x == 0) {
-        mbar_init(&sh.bar_q, 8);
-        mbar_init(&sh.bar_k, 4);
-        mbar_init(&sh.bar_kf, 1);
-        mbar_init(&sh.bar_v, 4);
+        mbar_init(&sh.bar_q, 16);
+        mbar_init(&sh.bar_k, 8);
+        mbar_init(&sh.bar_v, 8);
         mbar_init(&sh.bar_vf, 1);
         mbar_init(&sh.bar_s[0], 1);
         mbar_init(&sh.bar_s[1], 1);
@@ -127,7 +135,7 @@ __device__ __forceinline__ void attn_wide_core(const W w) {
         sh.odd = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 12) {
+    if (warp == 20) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)),
                      "r"(512u)
                      : "memory");
@@ -142,6 +150,7 @@ __device__ __forceinline__ void attn_wide_core(const W w) {
 
     if (warp < 4) {
         // ---------------- softmax ----------------
+        reg_alloc<152>();
         const int row = threadIdx.x;
         const uint32_t lanes = (uint32_t)(32 * warp) << 16, o_tm = tmem + lanes + kWdO;
         const bool live = w.live(it, row);
@@ -223,26 +232,35 @@ __device__ __forceinline__ void attn_wide_core(const W w) {
             if (*(volatile int*)&sh.odd != 0) w.slow(it, warp);
             else w.store(it, row, o_tm, m, l, sm + warp * kAtStage);      // the query planes' place is free
         }
-    } else if (warp < 12) {
+    } else if (warp < 20) {
         // ---------------- operands ----------------
-        const int cw = warp & 3, half = lane >> 4, every = w.seen(it, 0);
-        const bool is_v = warp >= 8;
+        reg_dealloc<72>();
+        const int cw = (warp - 4) & 7, half = lane >> 4, every = w.seen(it, 0);
+        const bool is_v = warp >= 12;
         const float4 none = make_float4(0.f, 0.f, 0.f, 0.f);
-        float4 r[16];                   // this warp's rows cw, cw + 4, .. of a tile
+        float4 r[8];                    // this warp's rows cw, cw + 8, .. of a tile
         auto load = [&](int j) {
             #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int key = j * kWdKeys + cw + 4 * i;
+            for (int i = 0; i < 8; ++i) {
+                const int key = j * kWdKeys + cw + 8 * i;
                 const T* at = key < keys ? (is_v ? w.v_row(it, key) : w.k_row(it, key)) : nullptr;
                 r[i] = at != nullptr ? ld4(at + 4 * lane) : none;
             }
         };
         load(0);
-        #pragma unroll 2
-        for (int i = 0; i < kAtRows / 8; ++i) {
-            const int row = (warp - 4) + 8 * i;
-            const float4 x = w.live(it, row) ? ld4(w.q_row(it, row) + 4 * lane) : none;
-            store_planes(sm + half * kAtHalf + row * 128, row, lane, kWdQPlane, x, plain4(x));
+        #pragma unroll 1
+        for (int i0 = 0; i0 < kAtRows / 16; i0 += 4) {
+            float4 x[4];
+            #pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int row = (warp - 4) + 16 * (i0 + i);
+                x[i] = w.live(it, row) ? ld4(w.q_row(it, row) + 4 * lane) : none;
+            }
+            #pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int row = (warp - 4) + 16 * (i0 + i);
+                store_planes(sm + half * kAtHalf + row * 128, row, lane, kWdQPlane, x[i], plain4(x[i]));
+            }
         }
         auto arrive = [&](uint64_t* bar) {
             fence_proxy_async_smem();
@@ -253,11 +271,13 @@ __device__ __forceinline__ void attn_wide_core(const W w) {
         uint8_t* const tile = sm + (is_v ? kWdV : kWdK) + half * kWdHalf;
         #pragma unroll 1
         for (int j = 0; j < n; ++j) {
-            if (j > 0 && !at_wait_warp(is_v ? &sh.bar_vf : &sh.bar_kf, (j - 1) & 1, ab, err)) break;
+            if (j > 0 && !(is_v ? at_wait_warp(&sh.bar_vf, (j - 1) & 1, ab, err)
+                                : at_wait_warp(&sh.bar_s[(j - 1) & 1], ((j - 1) >> 1) & 1, ab, err)))
+                break;
             bool odd = false;
             #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int row = cw + 4 * i;
+            for (int i = 0; i < 8; ++i) {
+                const int row = cw + 8 * i;
                 const bool plain = plain4(r[i]);
                 store_planes(tile + row * 128, row, lane, kWdPlane, r[i], plain);
                 odd = odd || (!plain && j * kWdKeys + row >= every);
@@ -267,31 +287,38 @@ __device__ __forceinline__ void attn_wide_core(const W w) {
             if (j + 1 < n) load(j + 1);
         }
     } else {
-        if (elect_one()) {
+        reg_dealloc<40>();
+        if (warp == 20 && elect_one()) {
             // ---------------- products ----------------
             const uint32_t q0 = umma_desc_lo(smem_u32(sm), 16), k0 = umma_desc_lo(smem_u32(sm + kWdK), 16),
                            v0 = umma_desc_lo(smem_u32(sm + kWdV), kWdHalf);
-            constexpr int first[6] = {2, 0, 1, 1, 0, 0}, second[6] = {0, 2, 1, 0, 1, 0};    // the small ones first
+            // the six pairs of planes, a hex digit each, the small products
+            // first; loops, since unrolled their 72 descriptors leave the registers
+            constexpr uint32_t kFirst = 0x001102u, kSecond = 0x010120u;
             auto scores = [&](int j) {
                 const uint32_t d = tmem + 64 * (j & 1);
-                #pragma unroll
-                for (int y = 0; y < 6; ++y)
+                #pragma unroll 1
+                for (int y = 0; y < 6; ++y) {
+                    const uint32_t q = q0 + (kFirst >> (4 * y) & 15u) * (kWdQPlane >> 4),
+                                   k = k0 + (kSecond >> (4 * y) & 15u) * (kWdPlane >> 4);
                     #pragma unroll
                     for (int x = 0; x < 8; ++x)
-                        umma_f16_ss(d, q0 + ((first[y] * kWdQPlane + (x >> 2) * kAtHalf + (x & 3) * 32) >> 4),
-                                    k0 + ((second[y] * kWdPlane + (x >> 2) * kWdHalf + (x & 3) * 32) >> 4),
-                                    umma_idesc_bf16(128, 64, false), x > 0 || y > 0);
+                        umma_f16_ss(d, q + (((x >> 2) * kAtHalf + (x & 3) * 32) >> 4),
+                                    k + (((x >> 2) * kWdHalf + (x & 3) * 32) >> 4), umma_idesc_bf16(128, 64, false),
+                                    x > 0 || y > 0);
+                }
                 umma_commit(&sh.bar_s[j & 1]);
-                umma_commit(&sh.bar_kf);
             };
             auto outputs = [&](int j) {
-                const uint32_t p = tmem + kWdP + 96 * (j & 1), d = tmem + kWdO;
-                #pragma unroll
-                for (int y = 0; y < 6; ++y)
+                const uint32_t d = tmem + kWdO;
+                #pragma unroll 1
+                for (int y = 0; y < 6; ++y) {
+                    const uint32_t p = tmem + kWdP + 96 * (j & 1) + 32 * (kFirst >> (4 * y) & 15u),
+                                   v = v0 + (kSecond >> (4 * y) & 15u) * (kWdPlane >> 4);
                     #pragma unroll
                     for (int x = 0; x < 4; ++x)
-                        umma_f16_ts(d, p + 32 * first[y] + 8 * x, v0 + ((second[y] * kWdPlane + x * 2048) >> 4),
-                                    umma_idesc_bf16(128, 128, true), j > 0 || x > 0 || y > 0);
+                        umma_f16_ts(d, p + 8 * x, v + (x * 2048 >> 4), umma_idesc_bf16(128, 128, true), j > 0 || x > 0 || y > 0);
+                }
                 umma_commit(&sh.bar_vf);
             };
             bool ok = at_wait(&sh.bar_q, 0, ab, err) && at_wait(&sh.bar_k, 0, ab, err);
@@ -317,7 +344,7 @@ __device__ __forceinline__ void attn_wide_core(const W w) {
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 12) {
+    if (warp == 20) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
     }
