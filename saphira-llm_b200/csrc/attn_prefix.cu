@@ -11,7 +11,8 @@
 //     M = max m_i,  out = sum_i e^(m_i - M) o_i / sum_i e^(m_i - M) l_i.
 //
 // f16: the tensor-core core of attn_mma.cuh. f32, and groups of more than 128
-// heads: the 32-bit tile of attn_simt.cuh, one item per CTA.
+// heads: that of attn_wide.cuh, or with up to 16 rows the ordinary pipes
+// (attn_simt.cuh), one item per CTA.
 //
 // Bound: HBM (the keys and values once) for few rows; the products for many
 // (n * n_q * group rows share each key: above about 250 of them).
@@ -280,27 +281,21 @@ attn_prefix_mma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
 }
 
 // ---------------------------------------------------------------------------
-// 32-bit: one item per CTA, R rows a thread
+// 32-bit, up to 16 rows in all: one item per CTA
 // ---------------------------------------------------------------------------
-template <int R, class T>
+template <class T>
 __global__ void __launch_bounds__(kSimtThreads, 2)
 attn_prefix_simt_kernel(const __grid_constant__ PagesDev pg, const __grid_constant__ PrefixParams p) {
     extern __shared__ float smf[];
     pdl_trigger();
     PrefixItem it;
     if (!find_item(pg, p, blockIdx.x, &it) || it.last()) return;
-    const int r0 = it.row0, ty = threadIdx.x >> 4;
-    simt_load_q<R, T>(smf, [&](int r) -> const T* {
-        return r0 + r < it.row_end ? static_cast<const T*>(p.q) + row_off(p, it.kvh, r0 + r) : nullptr;
+    simt_load_q<T>(smf, [&](int i) -> const T* {
+        return it.row0 + i < it.row_end ? static_cast<const T*>(p.q) + row_off(p, it.kvh, it.row0 + i) : nullptr;
     });
-    SimtState<R> st;
+    SimtState st;
     simt_init(st);
-    int lim[R];
-    #pragma unroll
-    for (int i = 0; i < R; ++i) {
-        const int r = r0 + R * ty + i;
-        lim[i] = r < it.row_end ? row_seen(p, it, r) : 0;
-    }
+    const int r = it.row0 + (threadIdx.x >> 4), lim = r < it.row_end ? row_seen(p, it, r) : 0;
     auto addr = [&](const void* pool, int j) -> const T* {
         if (j >= it.keys) return nullptr;
         const int id = page_of(pg, p, it.slot, (it.a + j) / pg.page);
@@ -308,15 +303,11 @@ attn_prefix_simt_kernel(const __grid_constant__ PagesDev pg, const __grid_consta
                ((size_t)it.kvh * pg.page + (it.a + j) % pg.page) * kServeDim;
     };
     for (int j0 = 0; j0 < it.keys; j0 += kSimtKeys)
-        simt_tile<R, T>(smf, st, j0, lim, [&](int j) { return addr(p.kp, j); }, [&](int j) { return addr(p.vp, j); });
-    const int tx = threadIdx.x & 15;
-    #pragma unroll
-    for (int i = 0; i < R; ++i) {
-        const int r = r0 + R * ty + i;
-        if (r >= it.row_end) continue;
+        simt_tile<T>(smf, st, j0, lim, [&](int j) { return addr(p.kp, j); }, [&](int j) { return addr(p.vp, j); });
+    if (r < it.row_end) {
         const size_t at = part_at(p, it, r);
-        if (tx == 0) p.part_ml[at] = make_float2(st.m[i], st.l[i]);
-        simt_store(st, i, 1.f, p.part_o + at * kServeDim);
+        if ((threadIdx.x & 15) == 0) p.part_ml[at] = make_float2(st.m, st.l);
+        simt_store(st, p.part_o + at * kServeDim);
     }
 }
 
@@ -436,7 +427,7 @@ Plan make_plan(const sllm_cuda_kv_pages& p, int n, int n_q, int n_head, int pref
     const bool mma = p.kv_type == SLLM_CUDA_KV_F16 && group <= kAtRows;
     Plan pl{};
     pl.key_tile = mma ? kAtKeys : kSimtKeys;
-    pl.rt = mma ? kAtRows / group * group : rows <= kSimtRows<1> ? kSimtRows<1> : kAtRows;
+    pl.rt = mma ? kAtRows / group * group : rows <= kSimtRows ? kSimtRows : kAtRows;
     pl.per = mma ? 2 : 1;
     auto items = [&](int r) { return (r + pl.rt * pl.per - 1) / (pl.rt * pl.per); };
     pl.ri_all = items(rows);
@@ -525,9 +516,9 @@ cudaError_t launch_32(const PagesDev& pg, const PrefixParams& p, cudaStream_t st
         return e != cudaSuccess ? e
                                 : launch(attn_prefix_wide_kernel<T>, grid, dim3(kWdThreads), kWdSmem, st, false, pg, p);
     }
-    const cudaError_t e = allow_smem<attn_prefix_simt_kernel<1, T>>(kSimtSmem<1>);
+    const cudaError_t e = allow_smem<attn_prefix_simt_kernel<T>>(kSimtSmem);
     return e != cudaSuccess ? e
-                            : launch(attn_prefix_simt_kernel<1, T>, grid, dim3(kSimtThreads), kSimtSmem<1>, st, false, pg, p);
+                            : launch(attn_prefix_simt_kernel<T>, grid, dim3(kSimtThreads), kSimtSmem, st, false, pg, p);
 }
 
 int check_shape(const sllm_cuda_kv_pages* p, int n, int n_q, int n_head, int prefix, const char* who) {

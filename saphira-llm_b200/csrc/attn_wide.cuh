@@ -24,7 +24,7 @@
 //
 // Products of different shapes are not ordered among themselves, so none
 // touches tensor memory that one of the other shape reads or writes, except
-// across a commit: scores 2 x 64 columns, weights 2 x 96, outputs 128. (One
+// across a commit: scores 2 x 64 columns, weights 96, outputs 2 x 128. (One
 // product of N = 192 over a key tile's three planes, the softmax adding the
 // column groups, would need 1664 clocks for the scores instead of 2304, but
 // partial sums of three shapes would lean on an order that is not promised.)
@@ -50,7 +50,14 @@ constexpr int kWdKeys = 64;
 constexpr int kWdQPlane = kAtTile;                      // 128 rows x 128 bf16
 constexpr int kWdHalf = kWdKeys * 128, kWdPlane = 2 * kWdHalf;      // 64 rows x 64 bf16, x 128
 constexpr int kWdK = 3 * kWdQPlane, kWdV = kWdK + 3 * kWdPlane, kWdEnd = kWdV + 3 * kWdPlane;
-constexpr int kWdP = 128, kWdO = 320;                   // tensor memory columns: weights, outputs
+// tensor memory columns behind the scores: weights, outputs, their total
+constexpr int kWdP = 128, kWdO = 224, kWdT = 352;
+// The tensor core cuts a sum's last bits instead of rounding, always towards
+// zero: 1.3e-7 of an output per key tile, 8e-6 after 4000 keys. So the outputs
+// of every kWdFold key tiles are summed by themselves, and added to their total
+// by ordinary additions (error after 4000 keys 6.6e-7; one tile 3.3e-7 and 3%
+// more time, four 1.2e-6; a plain 32-bit computation is 7.9e-7 off).
+constexpr int kWdFold = 2;
 constexpr int kWdSmem = kWdEnd + 1024;
 constexpr int kWdThreads = 32 * 24;
 
@@ -108,7 +115,7 @@ __device__ __forceinline__ void attn_wide_core(const W w) {
     struct Shared {
         // q: split; k, v: tile split; vf: its products done; s: scores (and the
         // keys' place free); p: weights; o: all
-        uint64_t bar_q, bar_k, bar_v, bar_vf, bar_s[2], bar_p[2], bar_o;
+        uint64_t bar_q, bar_k, bar_v, bar_vf, bar_s[2], bar_p, bar_o;
         uint32_t tmem;
         int abort_flag, odd;
     };
@@ -128,8 +135,7 @@ __device__ __forceinline__ void attn_wide_core(const W w) {
         mbar_init(&sh.bar_vf, 1);
         mbar_init(&sh.bar_s[0], 1);
         mbar_init(&sh.bar_s[1], 1);
-        mbar_init(&sh.bar_p[0], 4);
-        mbar_init(&sh.bar_p[1], 4);
+        mbar_init(&sh.bar_p, 4);
         mbar_init(&sh.bar_o, 1);
         sh.abort_flag = 0;
         sh.odd = 0;
@@ -152,13 +158,33 @@ __device__ __forceinline__ void attn_wide_core(const W w) {
         // ---------------- softmax ----------------
         reg_alloc<152>();
         const int row = threadIdx.x;
-        const uint32_t lanes = (uint32_t)(32 * warp) << 16, o_tm = tmem + lanes + kWdO;
+        const uint32_t lanes = (uint32_t)(32 * warp) << 16, p_tm = tmem + lanes + kWdP, o_tm = tmem + lanes + kWdO,
+                       t_tm = tmem + lanes + kWdT;
         const bool live = w.live(it, row);
         const int seen = w.seen(it, row);
         float m = -INFINITY, l = 0.f;
         bool ok = true;
+        // this row's outputs, all scaled by f: the running ones go into the
+        // total (fold; `total`: there is one), or both are scaled in place
+        auto outputs = [&](bool fold, bool total, float f) {
+            #pragma unroll 1
+            for (int c = 0; c < 8; ++c) {
+                uint32_t a[16], t[16];
+                tmem_ld16(o_tm + 16 * c, a);
+                if (total) tmem_ld16(t_tm + 16 * c, t);
+                tmem_ld_wait();
+                #pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const float x = __uint_as_float(a[e]), y = total ? __uint_as_float(t[e]) : 0.f;
+                    a[e] = __float_as_uint(__fmul_rn(x, f));
+                    t[e] = __float_as_uint(__fmul_rn(fold ? __fadd_rn(x, y) : y, f));
+                }
+                if (!fold) tmem_st16(o_tm + 16 * c, a);
+                if (fold || total) tmem_st16(t_tm + 16 * c, t);
+            }
+        };
         for (int j = 0; j < n; ++j) {
-            const uint32_t s_tm = tmem + lanes + 64 * (j & 1), p_tm = tmem + lanes + kWdP + 96 * (j & 1);
+            const uint32_t s_tm = tmem + lanes + 64 * (j & 1);
             if (!(ok = at_wait_warp(&sh.bar_s[j & 1], (j >> 1) & 1, ab, err))) break;
             tc_fence_after();
             float s[64];
@@ -184,53 +210,48 @@ __device__ __forceinline__ void attn_wide_core(const W w) {
             mx = max3(mx, s[63], s[63]);
             // (a row that is none may hold anything: it never asks for more)
             const bool fine = (mx - m) * kAtScale2 <= kAtLag || mx == -INFINITY || !live;
-            if (!__all_sync(0xffffffffu, fine)) {
-                const float m1 = fine ? m : max3(m, mx, mx);
-                const float f = fine ? 1.f : ex2((m - m1) * kAtScale2);
-                m = m1;
-                l *= f;
-                if (j > 0) {
-                    // the products before are complete when the values' place is free
-                    if (!(ok = at_wait_warp(&sh.bar_vf, (j - 1) & 1, ab, err))) break;
-                    tc_fence_after();
-                    #pragma unroll 1
-                    for (int c = 0; c < 8; ++c) {
-                        uint32_t r[16];
-                        tmem_ld16(o_tm + 16 * c, r);
-                        tmem_ld_wait();
-                        #pragma unroll
-                        for (int e = 0; e < 16; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * f);
-                        tmem_st16(o_tm + 16 * c, r);
-                    }
-                }
-            }
+            const float m1 = fine ? m : max3(m, mx, mx), f = fine ? 1.f : ex2((m - m1) * kAtScale2);
+            m = m1;
+            l *= f;
             const float mc = weight_offset(m);
             float sum0 = 0.f, sum1 = 0.f;
+            uint32_t u[3][32];
             #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                uint32_t u[3][16];
-                #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    float x0, x1;
-                    fma2v(x0, x1, s[32 * h + 2 * i], s[32 * h + 2 * i + 1], kAtScale2, kAtScale2, mc, mc);
-                    x0 = ex2(x0);
-                    x1 = ex2(x1);
-                    add2(sum0, sum1, x0, x1);
-                    split2(x0, x1, u[0][i], u[1][i], u[2][i]);
-                }
-                #pragma unroll
-                for (int q = 0; q < 3; ++q) tmem_st16(p_tm + 32 * q + 16 * h, u[q]);
+            for (int i = 0; i < 32; ++i) {
+                float x0, x1;
+                fma2v(x0, x1, s[2 * i], s[2 * i + 1], kAtScale2, kAtScale2, mc, mc);
+                x0 = ex2(x0);
+                x1 = ex2(x1);
+                add2(sum0, sum1, x0, x1);
+                split2(x0, x1, u[0][i], u[1][i], u[2][i]);
             }
             l += sum0 + sum1;
+            // the products before are complete when the values' place is free:
+            // then the weights' place is, too, and the outputs may be touched
+            if (j > 0) {
+                if (!(ok = at_wait_warp(&sh.bar_vf, (j - 1) & 1, ab, err))) break;
+                tc_fence_after();
+                const bool fold = j % kWdFold == 0;
+                if (fold || __any_sync(0xffffffffu, !fine)) outputs(fold, j > kWdFold, f);
+            }
+            #pragma unroll
+            for (int q = 0; q < 3; ++q) tmem_st32(p_tm + 32 * q, u[q]);
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.bar_p[j & 1]);      // (tile j + 1's may come before tile j's products)
+            if (lane == 0) mbar_arrive(&sh.bar_p);
         }
         if (ok && at_wait_warp(&sh.bar_o, 0, ab, err)) {
             tc_fence_after();
-            if (*(volatile int*)&sh.odd != 0) w.slow(it, warp);
-            else w.store(it, row, o_tm, m, l, sm + warp * kAtStage);      // the query planes' place is free
+            if (*(volatile int*)&sh.odd != 0) {
+                w.slow(it, warp);
+            } else {
+                if (n > kWdFold) {
+                    outputs(true, true, 1.f);
+                    tmem_st_wait();
+                }
+                w.store(it, row, n > kWdFold ? t_tm : o_tm, m, l, sm + warp * kAtStage);     // the query planes' place is free
+            }
         }
     } else if (warp < 20) {
         // ---------------- operands ----------------
@@ -313,11 +334,12 @@ __device__ __forceinline__ void attn_wide_core(const W w) {
                 const uint32_t d = tmem + kWdO;
                 #pragma unroll 1
                 for (int y = 0; y < 6; ++y) {
-                    const uint32_t p = tmem + kWdP + 96 * (j & 1) + 32 * (kFirst >> (4 * y) & 15u),
+                    const uint32_t p = tmem + kWdP + 32 * (kFirst >> (4 * y) & 15u),
                                    v = v0 + (kSecond >> (4 * y) & 15u) * (kWdPlane >> 4);
                     #pragma unroll
                     for (int x = 0; x < 4; ++x)
-                        umma_f16_ts(d, p + 8 * x, v + (x * 2048 >> 4), umma_idesc_bf16(128, 128, true), j > 0 || x > 0 || y > 0);
+                        umma_f16_ts(d, p + 8 * x, v + (x * 2048 >> 4), umma_idesc_bf16(128, 128, true),
+                                    j % kWdFold != 0 || x > 0 || y > 0);
                 }
                 umma_commit(&sh.bar_vf);
             };
@@ -333,7 +355,7 @@ __device__ __forceinline__ void attn_wide_core(const W w) {
                     tc_fence_after();
                     scores(j + 1);
                 }
-                if (!(ok = at_wait(&sh.bar_v, j & 1, ab, err) && at_wait(&sh.bar_p[j & 1], (j >> 1) & 1, ab, err))) break;
+                if (!(ok = at_wait(&sh.bar_v, j & 1, ab, err) && at_wait(&sh.bar_p, j & 1, ab, err))) break;
                 tc_fence_after();
                 outputs(j);
             }

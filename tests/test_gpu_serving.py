@@ -108,18 +108,19 @@ def test_prompt_masked_places_leave_no_trace(cuda, dt):
     assert bool(torch.isnan(got[140, :, 0].float()).all())
 
 
-def test_prompt_offsets_beyond_32_bits(cuda):
+@pytest.mark.parametrize("dt", ["f32", "f16"])
+def test_prompt_offsets_beyond_32_bits(cuda, dt):
     """Tokens 2^26 elements apart: addresses past 2^31 elements (and 2^32 bytes)."""
     import torch
     n, stride = 36, 1 << 26
-    buf = torch.zeros(stride * n, dtype=torch.float16, device="cuda")
+    buf = torch.zeros(stride * n, dtype=_dt(dt), device="cuda")
     q, k, v = (torch.as_strided(buf, (n, 1, 128), (stride, 128, 1), storage_offset=o) for o in (0, 128, 256))
     for i, t in enumerate((q, k, v)):
-        t.copy_(_rand(i, n, 1, 128, dt=torch.float16))
-    out = torch.empty(n, 1, 128, dtype=torch.float16, device="cuda")
+        t.copy_(_rand(i, n, 1, 128, dt=_dt(dt)))
+    out = torch.empty(n, 1, 128, dtype=_dt(dt), device="cuda")
     cuda.attn_prompt(q, k, v, out, _i32([0, n]))
     torch.cuda.synchronize()
-    check_prompt(q, k, v, out, [n], True)
+    check_prompt(q, k, v, out, [n], dt == "f16")
     del buf
     torch.cuda.empty_cache()
 
@@ -485,6 +486,8 @@ PREFIX = [
     (512, [4, 90, 5], 64, (8, 1), 4), (1024, [300] * 9, 16, (20, 5), 1), (192, [16, 17, 31], 64, (6, 2), 16),
     (2048, [1] * 33, 128, (8, 1), 1), (320, [3] * 70, 32, (4, 4), 3), (4096, [257, 1], 64, (64, 8), 2),
     (0, [1500, 700, 3], 16, (20, 5), 1), (0, [5, 3], 16, (4, 2), 4), (640, [200, 300], 128, (20, 5), 8),
+    (192, [40, 9], 64, (64, 1), 8), (128, [17], 32, (128, 1), 1), (64, [30, 1], 16, (256, 1), 2), (0, [700], 16, (129, 1), 1),
+    (32, [1] * 300, 16, (2, 1), 1), (1600, [20, 33], 16, (4, 1), 2),
 ]
 
 
@@ -612,6 +615,76 @@ def test_prefix_offsets_beyond_32_bits(cuda):
     check_prefix(c, q, out, [0, 1], layers - 1)
     del pool, c, small_k, small_v
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16"])
+def test_prefix_many_items_captured(cuda, dt):
+    """Enough items for the counter that hands them out: captured, replayed."""
+    import torch
+    n, heads, prefix = 70, (8, 8), 640
+    c = shared_cache(cuda, prefix, [3 + i % 50 for i in range(n)], 32, heads, dt)
+    q = _rand(9, n, 1, 8, 128, dt=_dt(dt))
+    out = torch.empty_like(q)
+    slots = _i32(list(range(n)))
+    work = torch.empty(c.p.attn_prefix_work_bytes(n, 1, 8, prefix), dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        c.p.attn_prefix(1, q, out, slots, prefix, work, c.status, stream=torch.cuda.current_stream())
+    for _ in range(2):
+        out.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        check_prefix(c, q, out, list(range(n)), 1)
+
+
+def test_first_calls_inside_a_capture():
+    """In a fresh process, with nothing loaded before, every operator's first
+    call is captured."""
+    import subprocess
+    import sys
+    code = """
+import importlib, torch
+pkg = importlib.import_module("saphira-llm_b200")
+i32 = lambda a: torch.tensor(a, dtype=torch.int32, device="cuda")
+k = torch.randn(8, 1, 2, 16, 128, device="cuda").half()
+v = torch.randn(8, 1, 2, 16, 128, device="cuda").half()
+p = pkg.KvPages(k, v, i32([1, 1] + [0] * 6), i32([[0, 1, 0], [0, 0, 0]]), i32([20, 0]))
+work = torch.empty(p.work_bytes(), dtype=torch.uint8, device="cuda")
+q = torch.randn(1, 1, 4, 128, device="cuda").half()
+o = torch.empty_like(q)
+scratch = torch.empty(p.attn_prefix_work_bytes(1, 1, 4, 0), dtype=torch.uint8, device="cuda")
+x = torch.randn(9, 2, 128, device="cuda")
+y = torch.empty_like(x)
+h, ho = x.half(), torch.empty_like(x.half())
+pr = torch.full((1, 2, 6000), 1 / 6000, device="cuda")
+tok, cnt = i32([[0, 0]]), i32([0])
+one, zero, cu, status = i32([1]), i32([0]), i32([0, 9]), i32([0])
+ua, us = torch.rand(1, 1, device="cuda"), torch.rand(1, device="cuda")
+cos = torch.ones(64, 64, device="cuda")
+pos20, tok1 = i32([20]), i32([[0]])
+x4, x1, q4 = torch.randn(1, 4, 128, device="cuda"), x[:1], torch.empty(1, 4, 128, device="cuda").half()
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    s = torch.cuda.current_stream()
+    pkg.attn_prompt(x, x, x, y, cu, stream=s)
+    pkg.attn_prompt(h, h, h, ho, cu, stream=s)
+    p.fork(zero, one, work, status, stream=s)
+    p.reserve(one, one, work, status, stream=s)
+    p.append(0, one, pos20, x4, x1, x1, cos, cos, q4, status=status, stream=s)
+    p.attn_prefix(0, q, o, one, 0, scratch, status, stream=s)
+    p.release(zero, None, work, status, stream=s)
+    p.compact(work, status, stream=s)
+    pkg.spec_verify(pr, None, tok1, None, ua, us, tok, cnt, status, stream=s)
+g.replay()
+torch.cuda.synchronize()
+assert status.item() == 0 and torch.isfinite(o.float()).all() and torch.isfinite(y).all() and torch.isfinite(ho.float()).all()
+assert p.c.n_pages == 8
+print("ok")
+"""
+    run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and run.stdout.strip() == "ok", run.stdout + run.stderr
 
 
 @pytest.mark.parametrize("dt", ["f32", "f16"])
