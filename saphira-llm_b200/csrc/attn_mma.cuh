@@ -82,6 +82,22 @@ __device__ __forceinline__ bool at_wait(uint64_t* bar, uint32_t parity, volatile
 __device__ __forceinline__ bool at_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* error) {
     return __all_sync(0xffffffffu, at_wait(bar, parity, abort_flag, error));
 }
+// ... with something to try meanwhile
+template <class F>
+__device__ __forceinline__ bool at_wait_while(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* error, F f) {
+    const uint64_t t0 = gtimer();
+    #pragma unroll 1
+    while (!mbar_test(bar, parity)) {
+        f();
+        if (*abort_flag) return false;
+        if (gtimer() - t0 > kGmWaitNs) {
+            *abort_flag = 1;
+            atomicExch(error, GM_TIMEOUT);
+            return false;
+        }
+    }
+    return true;
+}
 __device__ __forceinline__ void at_drain(uint64_t* bar, uint32_t parity) {
     const uint64_t t0 = gtimer();
     #pragma unroll 1
@@ -360,16 +376,21 @@ __device__ __forceinline__ void attn_core(const W w) {
                     if (!(ok = at_wait_warp(&sh.bar_full[slot], (x / kAtStages) & 1, ab, err))) break;
                     uint8_t* v = sm + (2 + slot) * kAtTile + row * 128;
                     const int key = j * kAtKeys + row;
-                    #pragma unroll
-                    for (int c = 0; c < 16; ++c) {
-                        uint4* at = reinterpret_cast<uint4*>(v + (c >> 3) * kAtHalf + 16 * ((c ^ row) & 7));
-                        if (key < keys) {
-                            const uint4 u = *at;
-                            odd = odd || (key >= every &&
-                                          (odd_half2(u.x) || odd_half2(u.y) || odd_half2(u.z) || odd_half2(u.w)));
-                        } else {
-                            *at = make_uint4(0, 0, 0, 0);
+                    if (key >= keys) {
+                        #pragma unroll 4
+                        for (int c = 0; c < 16; ++c)
+                            *reinterpret_cast<uint4*>(v + (c >> 3) * kAtHalf + 16 * (c & 7)) = make_uint4(0, 0, 0, 0);
+                    } else if (key >= every) {
+                        // (a short loop: its code runs once an item)
+                        __half2 top = __half2half2(__ushort_as_half(0));
+                        #pragma unroll 4
+                        for (int c = 0; c < 16; ++c) {
+                            const uint4 u = *reinterpret_cast<const uint4*>(v + (c >> 3) * kAtHalf + 16 * ((c ^ row) & 7));
+                            const __half2* x = reinterpret_cast<const __half2*>(&u);
+                            top = __hmax2_nan(top, __hmax2_nan(__hmax2_nan(__habs2(x[0]), __habs2(x[1])),
+                                                               __hmax2_nan(__habs2(x[2]), __habs2(x[3]))));
                         }
+                        odd = odd || odd_half2(*reinterpret_cast<const uint32_t*>(&top));
                     }
                     fence_proxy_async_smem();
                 }
@@ -501,40 +522,66 @@ __device__ __forceinline__ void attn_core(const W w) {
                         umma_f16_ts(tmem + 256 + 128 * t, tmem + 128 * t + 32 * half + 8 * x, v + x * (2048 >> 4),
                                     idesc_o, add || x > 0);
                 };
-                int steps[2] = {0, 0}, uses[2] = {0, 0};
+                int steps0 = 0, steps1 = 0, uses0 = 0, uses1 = 0;
                 bool ok = true;
-                Item it;
-                for (int i = 0; ok && next_lane(i, &it); ++i) {
+                // the next item, and whether its first scores have been issued:
+                // that is tried while the last products of this one wait for
+                // their weights, so that its softmax starts under them
+                Item it, nx;
+                bool known = false, ahead = false;
+                for (int i = 0; ok; ++i) {
+                    if (known) it = nx;
+                    else if (!next_lane(i, &it)) break;
+                    if (it.last()) break;
+                    known = false;
                     const int n0 = w.tiles(it, 0), n1 = w.tiles(it, 1), nt = max(n0, n1);
-                    ok = at_wait(&sh.bar_q[0], uses[0] & 1, ab, err) && at_wait(&sh.bar_full[ks], kp, ab, err);
-                    if (!ok) break;
-                    scores(0);
-                    if (n0 == 1) umma_commit(&sh.bar_qf[0]);
+                    if (!ahead) {
+                        ok = at_wait(&sh.bar_q[0], uses0 & 1, ab, err) && at_wait(&sh.bar_full[ks], kp, ab, err);
+                        if (!ok) break;
+                        scores(0);
+                        if (n0 == 1) umma_commit(&sh.bar_qf[0]);
+                    }
+                    ahead = false;
                     if (n1 > 0) {
-                        if (!(ok = at_wait(&sh.bar_q[1], uses[1] & 1, ab, err))) break;
+                        if (!(ok = at_wait(&sh.bar_q[1], uses1 & 1, ab, err))) break;
                         scores(1);
                         if (n1 == 1) umma_commit(&sh.bar_qf[1]);
                     }
                     umma_commit(&sh.bar_free[ks]);
                     step(ks, kp, 2);
+                    auto look = [&] {
+                        if (!known) {
+                            if (!mbar_test(&sh.bar_item, (i + 1) & 1)) return;
+                            nx = sh.item;
+                            mbar_arrive(&sh.bar_itemf);
+                            known = true;
+                        }
+                        if (ahead || nx.last() || !mbar_test(&sh.bar_q[0], (uses0 + 1) & 1) || !mbar_test(&sh.bar_full[ks], kp))
+                            return;
+                        scores(0);
+                        if (w.tiles(nx, 0) == 1) umma_commit(&sh.bar_qf[0]);
+                        ahead = true;
+                    };
                     #pragma unroll 1
                     for (int j = 0; j < nt && ok; ++j) {
                         const bool more = j + 1 < nt;
                         ok = at_wait(&sh.bar_full[vs], vp, ab, err) && (!more || at_wait(&sh.bar_full[ks], kp, ab, err));
                         #pragma unroll
                         for (int t = 0; t < 2; ++t) {
-                            const int n = t == 0 ? n0 : n1;
+                            const int n = t == 0 ? n0 : n1, uses = t == 0 ? uses0 : uses1;
+                            int& steps = t == 0 ? steps0 : steps1;
                             if (!ok || j >= n) continue;
                             // the item before has left O (of) before the first product overwrites it
-                            ok = (j > 0 || uses[t] == 0 || at_wait(&sh.bar_of[t], (uses[t] - 1) & 1, ab, err)) &&
-                                 at_wait(&sh.bar_h[t], steps[t] & 1, ab, err);
+                            ok = j > 0 || uses == 0 || at_wait(&sh.bar_of[t], (uses - 1) & 1, ab, err);
+                            if (t == 1 && !more) ok = ok && at_wait_while(&sh.bar_h[1], steps & 1, ab, err, look);
+                            else ok = ok && at_wait(&sh.bar_h[t], steps & 1, ab, err);
                             if (!ok) continue;
                             tc_fence_after();
                             outputs(t, 0, j > 0);
-                            if (!(ok = at_wait(&sh.bar_p[t], steps[t] & 1, ab, err))) continue;
+                            if (!(ok = at_wait(&sh.bar_p[t], steps & 1, ab, err))) continue;
                             tc_fence_after();
                             outputs(t, 1, true);
-                            ++steps[t];
+                            ++steps;
                             if (j + 1 < n) {
                                 scores(t);
                                 if (j + 2 == n) umma_commit(&sh.bar_qf[t]);
@@ -549,8 +596,8 @@ __device__ __forceinline__ void attn_core(const W w) {
                             step(ks, kp, 2);
                         }
                     }
-                    ++uses[0];
-                    uses[1] += n1 > 0 ? 1 : 0;
+                    ++uses0;
+                    uses1 += n1 > 0 ? 1 : 0;
                 }
                 umma_commit(&sh.bar_done);
                 at_drain(&sh.bar_done, 0);

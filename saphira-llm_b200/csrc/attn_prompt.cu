@@ -30,6 +30,12 @@ struct PromptParams {
 template <int R>
 __device__ __forceinline__ bool find_long_first(const PromptParams& p, int x, int* start, int* len, int* tile) {
     const int lane = threadIdx.x & 31;
+    if (p.n_seq == 1) {
+        *start = min(max(p.cu[0], 0), p.n_tokens);
+        *len = min(max(p.cu[1], *start), p.n_tokens) - *start;
+        *tile = (*len + R - 1) / R - 1 - x;
+        return *tile >= 0;
+    }
     auto seq = [&](int s, int* a) {
         *a = min(max(p.cu[s], 0), p.n_tokens);
         return min(max(p.cu[s + 1], *a), p.n_tokens) - *a;
