@@ -201,10 +201,14 @@ SLLM_CUDA_API int sllm_cuda_i2s_gemm_silu(const uint8_t * w_gate, const uint8_t 
  *     be captured into a CUDA graph;
  *   - a workspace is the caller's, 16-byte aligned, and holds nothing between
  *     calls. Calls (or graphs) that may overlap need workspaces of their own;
+ *   - outputs and workspaces overlap no other array of the call (kv_append may
+ *     write q_out, k_out and v_out exactly over contiguous f32 q, k and v);
  *   - what only the device can see to be wrong (a slot, a length or a page id
  *     out of range) is reported in `*status`, a device int that may be NULL:
  *     set to an SLLM_CUDA_ERR_* code, never cleared. Nothing outside the
- *     arrays is read or written in that case.
+ *     arrays is read or written in that case. SLLM_CUDA_ERR_TIMEOUT there is a
+ *     bounded wait inside a kernel that ran out: the call's output means
+ *     nothing, the device is fine.
  */
 
 /*

@@ -253,7 +253,8 @@ __device__ __forceinline__ void store_rows(uint32_t o_tmem, float f, uint8_t* st
 // r-th item; item(w, x, item): false: there is no item x, but later ones may
 // be), tiles(item, t) (0: no such row tile), keys(item),
 // seen(item, t, row) (not above keys, and least for row 0), live(item, t, row)
-// (a row to be written), a Loader, store(...) and slow(...).
+// (a row to be written), a Loader, store(...), slow(...) and gave_up() (a wait
+// ran out).
 //
 // Registers: 512 threads x 128 at launch; 2 x 184 (softmax) + 80 (outputs) +
 // 64 (the issuing warps) = 512 = 4 x 128 after the split.
@@ -654,6 +655,7 @@ __device__ __forceinline__ void attn_core(const W w) {
     }
     tc_fence_before();
     __syncthreads();
+    if (threadIdx.x == 0 && sh.abort_flag != 0) w.gave_up();
     if (warp == 12) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");

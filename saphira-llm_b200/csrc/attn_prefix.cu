@@ -211,6 +211,7 @@ struct PrefixWork {
             return find_item(w.pg, w.p, x, it);
         }
     };
+    __device__ __forceinline__ void gave_up() const { raise(p.status, SLLM_CUDA_ERR_TIMEOUT); }
     __device__ __forceinline__ int tiles(const Item& it, int t) const {
         return it.row0 + t * p.plan.rt < it.row_end ? (it.keys + kAtKeys - 1) / kAtKeys : 0;
     }
@@ -322,6 +323,7 @@ struct PrefixWide {
     const PagesDev& pg;
     const PrefixParams& p;
 
+    __device__ __forceinline__ void gave_up() const { raise(p.status, SLLM_CUDA_ERR_TIMEOUT); }
     __device__ __forceinline__ bool find(long long x, Item* it) const { return find_item(pg, p, x, it); }
     __device__ __forceinline__ int keys(const Item& it) const { return it.keys; }
     __device__ __forceinline__ bool live(const Item& it, int row) const { return it.row0 + row < it.row_end; }
@@ -360,11 +362,15 @@ attn_prefix_join_kernel(const __grid_constant__ PagesDev pg, const __grid_consta
     const int lane = threadIdx.x & 31;
     const long long x = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
     const int rows = p.n * p.n_q * p.group;
-    if (x >= (long long)rows * p.n_kv) return;
+    if (x >= (long long)rows * p.n_kv) {
+        pdl_wait();                 // (this grid must not end before the parts' does)
+        return;
+    }
     const int kvh = (int)(x / rows), r = (int)(x % rows), b = r / (p.n_q * p.group);
     int slot;
     const int len = seq_len(pg, p, b, &slot);
     if (len < 0) {
+        pdl_wait();
         if (lane == 0) raise(p.status, SLLM_CUDA_ERR_ARG);
         return;
     }

@@ -127,6 +127,7 @@ struct PromptWork {
             return true;
         }
     };
+    __device__ __forceinline__ void gave_up() const {}
     // key tiles of row tile t: up to its diagonal, or the sequence's end
     __device__ __forceinline__ int tiles(const Item& it, int t) const {
         if (it.tile * kPmRows + kAtRows * t >= it.len) return 0;
@@ -185,6 +186,7 @@ struct PromptWide {
     };
     const PromptParams& p;
 
+    __device__ __forceinline__ void gave_up() const {}
     __device__ __forceinline__ bool find(long long x, Item* it) const {      // longest first
         it->head = (int)(x % p.n_head);
         return find_long_first<kAtRows>(p, (int)(x / p.n_head), &it->start, &it->len, &it->tile);

@@ -106,7 +106,7 @@ __device__ __forceinline__ void store_planes(uint8_t* at, int r, int lane, int p
 
 // W: Item; T; find(x, item); keys(item); live(item, row); seen(item, row) (at
 // most keys, least for row 0); q_row(item, row), k_row(item, key),
-// v_row(item, key); store(...), slow(...).
+// v_row(item, key); store(...), slow(...), gave_up().
 template <class W>
 __device__ __forceinline__ void attn_wide_core(const W w) {
     using T = typename W::T;
@@ -366,6 +366,7 @@ __device__ __forceinline__ void attn_wide_core(const W w) {
     }
     tc_fence_before();
     __syncthreads();
+    if (threadIdx.x == 0 && sh.abort_flag != 0) w.gave_up();
     if (warp == 20) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");

@@ -590,8 +590,13 @@ int current_sms() {
 }
 
 int need_device(const void* p, const char* who, const char* arg) {
+    if (((uintptr_t)p & 3u) != 0) return fail(SLLM_CUDA_ERR_ARG, "%s: %s is not aligned", who, arg);
     cudaPointerAttributes at{};
     const cudaError_t e = cudaPointerGetAttributes(&at, p);
+    if (e == cudaErrorNoDevice || e == cudaErrorInsufficientDriver) {
+        cudaGetLastError();
+        return fail(SLLM_CUDA_ERR_UNSUPPORTED, "%s: no CUDA device", who);
+    }
     if (e != cudaSuccess) return cuda_fail(e, who);
     int dev = -1;
     if (cudaGetDevice(&dev) != cudaSuccess) return cuda_fail(cudaGetLastError(), who);

@@ -425,6 +425,22 @@ def test_append(cuda, dt, page, heads, layers):
     assert c.take_status() == 0 and torch.equal(c.k, k0) and torch.equal(c.v, v0)
 
 
+def test_append_in_place(cuda):
+    """f32 outputs over their inputs."""
+    import torch
+    c = Cache(cuda, 10, 1, 8, 16, 1, 2, "f32")
+    c.m.reserve([0], [40])
+    c.push()
+    q, k, v = _rand(1, 40, 4, 128), _rand(2, 40, 2, 128), _rand(3, 40, 2, 128)
+    cos, sin = (torch.from_numpy(x).cuda() for x in cuda.rope_table(64, 10000.0))
+    outs = [torch.empty_like(t) for t in (q, k, v)]
+    slot, pos = _i32([0] * 40), _i32(list(range(40)))
+    c.p.append(0, slot, pos, q, k, v, cos, sin, *outs, c.status)
+    c.p.append(0, slot, pos, q, k, v, cos, sin, q, k, v, c.status)
+    torch.cuda.synchronize()
+    assert c.take_status() == 0 and all(torch.equal(a, b) for a, b in zip(outs, (q, k, v)))
+
+
 # ---------------------------------------------------------------------------
 # decode attention over a shared prefix
 # ---------------------------------------------------------------------------
@@ -585,6 +601,45 @@ def test_prefix_peaked_rows(cuda, dt):
     c.k[c.m.tables[1][17]] *= 12.0
     q, out = run_prefix(cuda, c, [0, 1], 2, (8, 2), 512, dt)
     check_prefix(c, q, out, [0, 1], 1)
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16"])
+def test_prefix_many_sequences(cuda, dt):
+    """More sequences than a block has threads."""
+    n = 1500
+    c = shared_cache(cuda, 32, [1 + i % 3 for i in range(n)], 16, (2, 1), dt, spare_slots=0)
+    slots = list(range(n))
+    q, out = run_prefix(cuda, c, slots, 1, (2, 1), 32, dt)
+    assert c.take_status() == 0
+    check_prefix(c, q, out, slots, 1, skip=set(range(n)) - set(range(0, n, 37)))
+    # and page calls that name them all
+    import torch
+    new = [1] * n
+    want, copies = c.m.reserve(slots[:100], new[:100])
+    c.p.reserve(_i32(slots[:100]), _i32(new[:100]), c.work, c.status)
+    c.same()
+    assert c.take_status() == want
+    want = c.m.release(slots, None)
+    c.p.release(_i32(slots), None, c.work, c.status)
+    c.same()
+    assert c.take_status() == want == 0 and not any(c.m.refs)
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16"])
+def test_rows_that_see_no_numbers_are_no_numbers(cuda, dt):
+    """A NaN or an infinity in a key or value that a row does see shows in it."""
+    import torch
+    n = 200
+    for bad in (math.nan, math.inf):
+        for which in (0, 1):
+            q, k, v = (_rand(s, n, 2, 128, dt=_dt(dt)) for s in (1, 2, 3))
+            (k, v)[which][50] = bad
+            out = torch.empty_like(q)
+            cuda.attn_prompt(q, k, v, out, _i32([0, n]))
+            torch.cuda.synchronize()
+            assert bool(torch.isfinite(out[:50].float()).all())
+            if which == 1 or math.isnan(bad):
+                assert not bool(torch.isfinite(out[50:].float()).any(-1).any()), (bad, which)
 
 
 def test_prefix_offsets_beyond_32_bits(cuda):

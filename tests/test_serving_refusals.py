@@ -120,6 +120,25 @@ def test_verify_refusals(L):
         assert L.sllm_cuda_spec_verify(*a.values()) == -1, bad
 
 
+def test_misaligned_arrays_are_refused(L):
+    """A pointer that no float or int array has, refused on the host."""
+    good = dict(p=A, q=A, draft=A, nd=A, ua=A, us=A, n=1, k=4, V=100, tokens=A, count=A, status=None, stream=None)
+    a = dict(good, p=A + 2)
+    assert L.sllm_cuda_spec_verify(*a.values()) == -1 and b"aligned" in L.sllm_cuda_last_error()
+    assert L.sllm_cuda_attn_prompt(*prompt_args(q=A, cu=A + 1)) in (-1, -4)
+
+
+def test_no_device_is_unsupported(cuda_absent, L, abi):
+    """Without a device good arguments come back as SLLM_CUDA_ERR_UNSUPPORTED."""
+    p = cache(abi)
+    r, n = C.byref(p), L.sllm_cuda_kv_work_bytes(C.byref(p))
+    assert L.sllm_cuda_attn_prompt(*prompt_args()) == -4
+    assert L.sllm_cuda_kv_fork(r, A, A, 1, A, n, None, None) == -4
+    assert L.sllm_cuda_kv_compact(r, A, n, None, None) == -4
+    assert L.sllm_cuda_attn_prefix(r, 0, A, A, 2, 1, 20, 32, A, 1, A, 1 << 40, None, None) == -4
+    assert L.sllm_cuda_spec_verify(A, A, A, A, A, A, 1, 4, 100, A, A, None, None) == -4
+
+
 def test_rope_table(pkg, L):
     c, s = pkg.rope_table(5, 500000.0)
     f = np.float32(500000.0) ** np.float32(-2.0 / 128)
