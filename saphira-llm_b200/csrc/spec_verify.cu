@@ -307,6 +307,28 @@ spec_verify_kernel(const __grid_constant__ VerifyParams a) {
     if (lane == 0) out[r] = found;
 }
 
+// The CTAs of a sequence. Twice as many halve the time of a row's pass, which
+// is about 0.35 us per 1000 words of a CTA, and cost what the launch of more
+// clusters costs: nothing up to two CTAs per SM, about 2 us up to four, 8 us up
+// to eight; clusters of 16 as much as four times their CTAs. Measured, clusters
+// of 1, 2, 4, 8, 16, us:
+//      1 sequence  of   4096 words   7.7   7.3   7.5   7.3   7.8
+//      1              128256        50.2  28.1  15.6  11.4   8.9
+//     64               32000        16.7  11.6  10.0  10.8  22.6
+//     64              128256        60.6  31.6  20.6  17.2  27.9
+//    256                4096         8.7  10.1  17.1  27.1  66.1
+//    256              128256        82.7  61.8  60.3  60.9  96.0
+int cluster_size(int n, int n_vocab, int sms) {
+    int C = 1;
+    while (C < 16) {
+        const long long ctas = 2LL * C * n * (C == 8 ? 4 : 1);
+        const int worth = ctas <= 2LL * sms ? 6144 : ctas <= 4LL * sms ? 12288 : 40960;     // words of a CTA
+        if (ctas > 8LL * sms || n_vocab / C < worth) break;
+        C *= 2;
+    }
+    return C;
+}
+
 }  // namespace
 }  // namespace sllm
 
@@ -337,11 +359,7 @@ extern "C" int sllm_cuda_spec_verify(const float* p, const float* q, const int32
     a.k = k; a.V = n_vocab;
     a.vec = n_vocab % 4 == 0 && aligned16(p) && (q == nullptr || aligned16(q));
     a.status = status;
-    // a cluster per sequence; few sequences get larger ones, so that more SMs
-    // read their rows (one sequence of 128256 words: see the sizes below), and
-    // a small vocabulary none
-    const int sms = current_sms();
-    const int C = n_vocab <= 4096 ? 1 : (long long)n * 16 <= sms ? 16 : 8;
+    const int C = cluster_size(n, n_vocab, current_sms());
     if (C == 16) {
         const cudaError_t e1 = allow_cluster<spec_verify_kernel<true>>(), e2 = allow_cluster<spec_verify_kernel<false>>();
         CK(e1 != cudaSuccess ? e1 : e2, "spec_verify clusters");
