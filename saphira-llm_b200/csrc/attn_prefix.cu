@@ -11,14 +11,12 @@
 //     M = max m_i,  out = sum_i e^(m_i - M) o_i / sum_i e^(m_i - M) l_i.
 //
 // f16: the tensor-core core of attn_mma.cuh. f32, and groups of more than 128
-// heads: that of attn_wide.cuh, or with up to 16 rows the ordinary pipes
-// (attn_simt.cuh), one item per CTA.
+// heads: that of attn_wide.cuh, one item per CTA.
 //
 // Bound: HBM (the keys and values once) for few rows; the products for many
 // (n * n_q * group rows share each key: above about 250 of them).
 
 #include "attn_mma.cuh"
-#include "attn_simt.cuh"
 #include "attn_wide.cuh"
 
 namespace sllm {
@@ -282,37 +280,6 @@ attn_prefix_mma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
 }
 
 // ---------------------------------------------------------------------------
-// 32-bit, up to 16 rows in all: one item per CTA
-// ---------------------------------------------------------------------------
-template <class T>
-__global__ void __launch_bounds__(kSimtThreads, 2)
-attn_prefix_simt_kernel(const __grid_constant__ PagesDev pg, const __grid_constant__ PrefixParams p) {
-    extern __shared__ float smf[];
-    pdl_trigger();
-    PrefixItem it;
-    if (!find_item(pg, p, blockIdx.x, &it) || it.last()) return;
-    simt_load_q<T>(smf, [&](int i) -> const T* {
-        return it.row0 + i < it.row_end ? static_cast<const T*>(p.q) + row_off(p, it.kvh, it.row0 + i) : nullptr;
-    });
-    SimtState st;
-    simt_init(st);
-    const int r = it.row0 + (threadIdx.x >> 4), lim = r < it.row_end ? row_seen(p, it, r) : 0;
-    auto addr = [&](const void* pool, int j) -> const T* {
-        if (j >= it.keys) return nullptr;
-        const int id = page_of(pg, p, it.slot, (it.a + j) / pg.page);
-        return static_cast<const T*>(pool) + (size_t)id * p.page_stride +
-               ((size_t)it.kvh * pg.page + (it.a + j) % pg.page) * kServeDim;
-    };
-    for (int j0 = 0; j0 < it.keys; j0 += kSimtKeys)
-        simt_tile<T>(smf, st, j0, lim, [&](int j) { return addr(p.kp, j); }, [&](int j) { return addr(p.vp, j); });
-    if (r < it.row_end) {
-        const size_t at = part_at(p, it, r);
-        if ((threadIdx.x & 15) == 0) p.part_ml[at] = make_float2(st.m, st.l);
-        simt_store(st, p.part_o + at * kServeDim);
-    }
-}
-
-// ---------------------------------------------------------------------------
 // 32-bit on the tensor cores: one item of up to 128 rows per CTA. Groups of
 // more than 128 f16 heads come here too.
 // ---------------------------------------------------------------------------
@@ -422,18 +389,23 @@ attn_prefix_join_kernel(const __grid_constant__ PagesDev pg, const __grid_consta
 // ---------------------------------------------------------------------------
 // Rows: whole tokens per row tile where TMA gathers them. Splits of the prefix:
 // with an item of its own keys for each sequence besides, all of it in one
-// round of the SMs where that makes splits of at most eight key tiles. Longer:
+// round of the SMs where that makes splits of at most twelve key tiles, or of
+// at most eight where the sequences' items alone are more than a round. Longer:
 // the number, of those that make up to 32 tiles a split, that ends first on
 // the SMs when a split costs three tiles' time for its start and its parts
 // (all SMs write their parts at about one time, 128 KB each).
+// One round or that number, f16, 32 heads of 8: 4 sequences, prefix 4096 (three
+// tiles a split) 16.7 and 21.6 us, 16384 (nine) 26.2 and 33.2 us, 20480 (twelve)
+// 30.5 and 38.8 us; 32 sequences (256 items of their own), prefix 4096 (four)
+// 26.7 and 28.8 us, 12288 (eleven) 42.2 and 36.9 us.
 // A sequence's own keys: chunks of as many tiles, at least two; no more than
 // two items per SM over all sequences, and no more than 64 chunks.
 Plan make_plan(const sllm_cuda_kv_pages& p, int n, int n_q, int n_head, int prefix, int sms) {
     const int group = n_head / p.n_head_kv, rows = n * n_q * group;
     const bool mma = p.kv_type == SLLM_CUDA_KV_F16 && group <= kAtRows;
     Plan pl{};
-    pl.key_tile = mma ? kAtKeys : kSimtKeys;
-    pl.rt = mma ? kAtRows / group * group : rows <= kSimtRows ? kSimtRows : kAtRows;
+    pl.key_tile = mma ? kAtKeys : kWdKeys;
+    pl.rt = mma ? kAtRows / group * group : kAtRows;
     pl.per = mma ? 2 : 1;
     auto items = [&](int r) { return (r + pl.rt * pl.per - 1) / (pl.rt * pl.per); };
     pl.ri_all = items(rows);
@@ -442,7 +414,7 @@ Plan make_plan(const sllm_cuda_kv_pages& p, int n, int n_q, int n_head, int pref
     const long long base = (long long)p.n_head_kv * pl.ri_all, own = (long long)n * p.n_head_kv * pl.ri_seq;
     const long long room = sms - own > sms / 2 ? sms - own : sms / 2;
     const long long one = (base * pl.ptiles + room - 1) / room;        // tiles a split in one round
-    if (one <= 8) {
+    if (one <= (own <= sms ? 12 : 8)) {
         pl.ct = one < 1 ? 1 : (int)one;
         pl.sp = (pl.ptiles + pl.ct - 1) / pl.ct;
     } else {
@@ -516,15 +488,10 @@ cudaError_t launch_mma(const sllm_cuda_kv_pages& pages, const PagesDev& pg, cons
 
 template <class T>
 cudaError_t launch_32(const PagesDev& pg, const PrefixParams& p, cudaStream_t st) {
-    const dim3 grid((unsigned)item_numbers(p));
-    if (p.plan.rt == kAtRows) {
-        const cudaError_t e = allow_smem<attn_prefix_wide_kernel<T>>(kWdSmem);
-        return e != cudaSuccess ? e
-                                : launch(attn_prefix_wide_kernel<T>, grid, dim3(kWdThreads), kWdSmem, st, false, pg, p);
-    }
-    const cudaError_t e = allow_smem<attn_prefix_simt_kernel<T>>(kSimtSmem);
+    const cudaError_t e = allow_smem<attn_prefix_wide_kernel<T>>(kWdSmem);
     return e != cudaSuccess ? e
-                            : launch(attn_prefix_simt_kernel<T>, grid, dim3(kSimtThreads), kSimtSmem, st, false, pg, p);
+                            : launch(attn_prefix_wide_kernel<T>, dim3((unsigned)item_numbers(p)), dim3(kWdThreads), kWdSmem,
+                                     st, false, pg, p);
 }
 
 int check_shape(const sllm_cuda_kv_pages* p, int n, int n_q, int n_head, int prefix, const char* who) {
@@ -586,8 +553,13 @@ extern "C" int sllm_cuda_attn_prefix(const sllm_cuda_kv_pages* p, int32_t layer,
     a.plan = make_plan(*p, n, n_q, n_head, prefix_len, sms);
     a.part_o = static_cast<float*>(work);
     a.part_ml = reinterpret_cast<float2*>(a.part_o + part_count(a.plan, n, n_q, n_head) * kServeDim);
-    // many items per SM: each CTA takes the next one when it is free (one more
-    // launch, to clear the counter); few: they are dealt
+    // many items per SM: each CTA takes the next one when it is free, for one
+    // more launch, to clear the counter; few: they are dealt. Taken and dealt,
+    // f16, 32 heads of 8, own lengths of 1 to 4096 at random: 16 sequences (256
+    // items) 62 and 57 us, 64 (512) 149 and 156 us, 192 (1536) 336 and 375 us;
+    // lengths up to 1024, so that the items are short: 192 behind a prefix of
+    // 2048 149 and 130 us. (The lengths are the device's, so the rule is on the
+    // number alone.)
     if (item_numbers(a) > 3LL * sms)
         a.plan.next = reinterpret_cast<int*>(a.part_ml + part_count(a.plan, n, n_q, n_head));
     if (item_numbers(a) > 0x3fffffffLL) return fail(SLLM_CUDA_ERR_TOO_LARGE, "attn_prefix: %d sequences", n);
