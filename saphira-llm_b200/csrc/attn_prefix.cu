@@ -300,13 +300,31 @@ struct PrefixWide {
     __device__ __forceinline__ const T* q_row(const Item& it, int row) const {
         return static_cast<const T*>(p.q) + row_off(p, it.kvh, it.row0 + row);
     }
-    __device__ __forceinline__ const T* kv_row(const Item& it, const void* pool, int key) const {
-        const int id = page_of(pg, p, it.slot, (it.a + key) / pg.page);
-        return static_cast<const T*>(pool) + (size_t)id * p.page_stride +
-               ((size_t)it.kvh * pg.page + (it.a + key) % pg.page) * kServeDim;
-    }
-    __device__ __forceinline__ const T* k_row(const Item& it, int key) const { return kv_row(it, p.kp, key); }
-    __device__ __forceinline__ const T* v_row(const Item& it, int key) const { return kv_row(it, p.vp, key); }
+    struct Rows {                   // lane i looks up row i's page
+        const PagesDev& pg;
+        const PrefixParams& p;
+        const T* pool;
+        int slot, a, shift, lane;
+        size_t mine;
+        __device__ __forceinline__ Rows(const PrefixWide& w, const Item& it, bool is_v) : pg(w.pg), p(w.p) {
+            pool = static_cast<const T*>(is_v ? p.vp : p.kp) + (size_t)it.kvh * pg.page * kServeDim;
+            slot = it.slot;
+            a = it.a;
+            shift = __ffs(pg.page) - 1;
+            lane = threadIdx.x & 31;
+            mine = 0;
+        }
+        __device__ __forceinline__ void tile(int key, int n) {
+            const int k = key + 8 * lane;
+            if (lane < 8 && k < n)
+                mine = (size_t)page_of(pg, p, slot, (a + k) >> shift) * p.page_stride +
+                       (size_t)(((a + k) & (pg.page - 1)) * kServeDim);
+            __syncwarp();
+        }
+        __device__ __forceinline__ const T* row(int i) const {
+            return pool + __shfl_sync(0xffffffffu, (unsigned long long)mine, i);
+        }
+    };
     __device__ __forceinline__ void store(const Item& it, int row, uint32_t o_tm, float m, float l, uint8_t* stage) const {
         store_parts(p, it, it.row0, row, o_tm, m, l, stage);
     }

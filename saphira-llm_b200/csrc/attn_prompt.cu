@@ -2,7 +2,6 @@
 //
 // Sequence s holds tokens cu[s] .. cu[s + 1] - 1 of the packed arrays; token i
 // of a sequence sees its tokens 0 .. i.
-
 //
 // f16: attn_prompt_mma_kernel over attn_mma.cuh. f32: attn_prompt_wide_kernel
 // over attn_wide.cuh.
@@ -25,8 +24,9 @@ struct PromptParams {
 
 // tile x of the call's tiles of R rows in descending order of their position
 // in their sequence (the later, the more keys they see): the longest work
-// first. Bounds are clamped to the arrays, so a wrong cu stays inside them. F(t) = tiles at positions >= t; a binary search for the position,
-// then the sequence among those that long. One warp.
+// first. Bounds are clamped to the arrays, so a wrong cu stays inside
+// them. F(t) = tiles at positions >= t; a binary search for the position, then
+// the sequence among those that long. One warp.
 template <int R>
 __device__ __forceinline__ bool find_long_first(const PromptParams& p, int x, int* start, int* len, int* tile) {
     const int lane = threadIdx.x & 31;
@@ -198,12 +198,19 @@ struct PromptWide {
         return static_cast<const float*>(p.q) + (size_t)(it.start + it.tile * kAtRows + row) * p.qs +
                (size_t)it.head * kServeDim;
     }
-    __device__ __forceinline__ const float* k_row(const Item& it, int key) const {
-        return static_cast<const float*>(p.k) + (size_t)(it.start + key) * p.ks + (size_t)(it.head / p.group) * kServeDim;
-    }
-    __device__ __forceinline__ const float* v_row(const Item& it, int key) const {
-        return static_cast<const float*>(p.v) + (size_t)(it.start + key) * p.vs + (size_t)(it.head / p.group) * kServeDim;
-    }
+    struct Rows {
+        const float* base;
+        size_t stride;
+        __device__ __forceinline__ Rows(const PromptWide& w, const Item& it, bool is_v) {
+            stride = is_v ? w.p.vs : w.p.ks;
+            base = static_cast<const float*>(is_v ? w.p.v : w.p.k) + (size_t)it.start * stride +
+                   (size_t)(it.head / w.p.group) * kServeDim;
+            at = base;
+        }
+        const float* at;
+        __device__ __forceinline__ void tile(int key, int) { at = base + (size_t)key * stride; }
+        __device__ __forceinline__ const float* row(int i) const { return at + (size_t)(8 * i) * stride; }
+    };
     __device__ __forceinline__ void store(const Item& it, int row, uint32_t o_tm, float, float l, uint8_t* stage) const {
         const int x0 = it.tile * kAtRows + (row & ~31);
         store_rows(o_tm, 1.f / l, stage,

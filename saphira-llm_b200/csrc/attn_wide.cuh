@@ -49,9 +49,13 @@ namespace sllm {
 constexpr int kWdKeys = 64;
 constexpr int kWdQPlane = kAtTile;                      // 128 rows x 128 bf16
 constexpr int kWdHalf = kWdKeys * 128, kWdPlane = 2 * kWdHalf;      // 64 rows x 64 bf16, x 128
-constexpr int kWdK = 3 * kWdQPlane, kWdV = kWdK + 3 * kWdPlane, kWdEnd = kWdV + 3 * kWdPlane;
-// tensor memory columns behind the scores: weights, outputs, their total
-constexpr int kWdP = 128, kWdO = 224, kWdT = 352;
+// shared memory: the queries' second and third plane, two tiles of keys, one of values
+constexpr int kWdK = 2 * kWdQPlane, kWdV = kWdK + 6 * kWdPlane, kWdEnd = kWdV + 3 * kWdPlane;
+constexpr int kWdStage = kWdK + 3 * kWdPlane;           // where the first plane waits for its way into tensor memory
+static_assert(kWdQPlane <= 3 * kWdPlane, "in the place of the second tile of keys");
+// tensor memory columns behind the scores: the queries' first plane, weights,
+// outputs, their total
+constexpr int kWdQ1 = 64, kWdP = 128, kWdO = 224, kWdT = 352;
 // The tensor core cuts a sum's last bits instead of rounding, always towards
 // zero: 1.3e-7 of an output per key tile, 8e-6 after 4000 keys. So the outputs
 // of every kWdFold key tiles are summed by themselves, and added to their total
@@ -76,46 +80,61 @@ __device__ __forceinline__ uint32_t upper2(float lo, float hi) {
     return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632);
 }
 __device__ __forceinline__ float upper(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
+// (the differences are exact, so a multiply-add by -1 is one)
+__device__ __forceinline__ void minus2(float& a, float& b, float x, float y) { fma2v(a, b, x, y, -1.f, -1.f, a, b); }
 __device__ __forceinline__ void split2(float a, float b, uint32_t& p1, uint32_t& p2, uint32_t& p3) {
     p1 = pack_bf2(a, b);
-    a = __fsub_rn(a, __uint_as_float(p1 << 16));
-    b = __fsub_rn(b, __uint_as_float(p1 & 0xffff0000u));
+    minus2(a, b, __uint_as_float(p1 << 16), __uint_as_float(p1 & 0xffff0000u));
     p2 = upper2(a, b);
-    p3 = upper2(__fsub_rn(a, upper(a)), __fsub_rn(b, upper(b)));
+    minus2(a, b, upper(a), upper(b));
+    p3 = upper2(a, b);
 }
 
-// false when one of four is no finite number, or one that bf16 would round to
-// infinity
-__device__ __forceinline__ bool plain4(float4 x) {
-    const float t = max3(fabsf(x.x), fabsf(x.y), fabsf(x.z));
-    return max3(t, fabsf(x.w), t) < 0x1.fep127f;
+// t, or the largest of |x|; NaN when one is
+__device__ __forceinline__ float top4(float4 x, float t) {
+    return max3(fabsf(x.z), fabsf(x.w), max3(fabsf(x.x), fabsf(x.y), t));
 }
+// no NaN, no infinity, nothing that bf16 would round to one
+__device__ __forceinline__ bool plain(float top) { return top < 0x1.fep127f; }
 
 // four elements of a row into its three planes: `at` is the row's 128 bytes of
-// the lane's half in the first plane, r its number in the swizzle. What is no
-// finite number lies in the first plane alone.
-__device__ __forceinline__ void store_planes(uint8_t* at, int r, int lane, int plane, float4 x, bool plain) {
+// the lane's half in the second plane, `first` in the first, r its number in
+// the swizzle. What is not plain lies in the first plane alone.
+__device__ __forceinline__ void store_planes(uint8_t* at, uint8_t* first, int r, int lane, int plane, float4 x, bool whole) {
     uint32_t a[3], b[3];
     split2(x.x, x.y, a[0], a[1], a[2]);
     split2(x.z, x.w, b[0], b[1], b[2]);
-    if (!plain) a[1] = a[2] = b[1] = b[2] = 0u;
-    uint8_t* p = at + ((((lane & 15) >> 1) ^ (r & 7)) << 4) + (lane & 1) * 8;
+    if (!whole) a[1] = a[2] = b[1] = b[2] = 0u;
+    const int in = ((((lane & 15) >> 1) ^ (r & 7)) << 4) + (lane & 1) * 8;
+    *reinterpret_cast<uint2*>(first + in) = make_uint2(a[0], b[0]);
+    *reinterpret_cast<uint2*>(at + in) = make_uint2(a[1], b[1]);
+    *reinterpret_cast<uint2*>(at + in + plane) = make_uint2(a[2], b[2]);
+}
+
+// r[i] without an index into registers
+__device__ __forceinline__ float4 pick(const float4 (&r)[8], int i) {
+    float4 x = r[0];
     #pragma unroll
-    for (int i = 0; i < 3; ++i) *reinterpret_cast<uint2*>(p + i * plane) = make_uint2(a[i], b[i]);
+    for (int e = 1; e < 8; ++e)
+        if (e == i) x = r[e];
+    return x;
 }
 
 // W: Item; T; find(x, item); keys(item); live(item, row); seen(item, row) (at
-// most keys, least for row 0); q_row(item, row), k_row(item, key),
-// v_row(item, key); store(...), slow(...), gave_up().
+// most keys, least for row 0); q_row(item, row); Rows (one warp's keys or values:
+// tile(key, n): the next are keys key, key + 8, .. below n; row(i): the i-th of
+// them); store(...), slow(...), gave_up().
 template <class W>
 __device__ __forceinline__ void attn_wide_core(const W w) {
     using T = typename W::T;
     int* const err = &g_attn_error;
     extern __shared__ __align__(1024) uint8_t sm[];
     struct Shared {
-        // q: split; k, v: tile split; vf: its products done; s: scores (and the
-        // keys' place free); p: weights; o: all
-        uint64_t bar_q, bar_k, bar_v, bar_vf, bar_s[2], bar_p, bar_o;
+        // q: split; q1: the first plane in tensor memory; k, v: tile split; vf:
+        // its products done; s: scores (and the keys' place free; by tile
+        // parity, since a wait may come two tiles late); sf: scores read; p:
+        // weights; o: all
+        uint64_t bar_q, bar_q1, bar_k[2], bar_v, bar_vf, bar_s[2], bar_sf, bar_p, bar_o;
         uint32_t tmem;
         int abort_flag, odd;
     };
@@ -130,11 +149,14 @@ __device__ __forceinline__ void attn_wide_core(const W w) {
     }
     if (threadIdx.x == 0) {
         mbar_init(&sh.bar_q, 16);
-        mbar_init(&sh.bar_k, 8);
+        mbar_init(&sh.bar_q1, 4);
+        mbar_init(&sh.bar_k[0], 8);
+        mbar_init(&sh.bar_k[1], 8);
         mbar_init(&sh.bar_v, 8);
         mbar_init(&sh.bar_vf, 1);
         mbar_init(&sh.bar_s[0], 1);
         mbar_init(&sh.bar_s[1], 1);
+        mbar_init(&sh.bar_sf, 4);
         mbar_init(&sh.bar_p, 4);
         mbar_init(&sh.bar_o, 1);
         sh.abort_flag = 0;
@@ -163,28 +185,73 @@ __device__ __forceinline__ void attn_wide_core(const W w) {
         const bool live = w.live(it, row);
         const int seen = w.seen(it, row);
         float m = -INFINITY, l = 0.f;
-        bool ok = true;
-        // this row's outputs, all scaled by f: the running ones go into the
-        // total (fold; `total`: there is one), or both are scaled in place
-        auto outputs = [&](bool fold, bool total, float f) {
-            #pragma unroll 1
-            for (int c = 0; c < 8; ++c) {
-                uint32_t a[16], t[16];
-                tmem_ld16(o_tm + 16 * c, a);
-                if (total) tmem_ld16(t_tm + 16 * c, t);
-                tmem_ld_wait();
+        // this row's first plane of Q, from the staging place
+        bool ok = at_wait_warp(&sh.bar_q, 0, ab, err);
+        if (ok) {
+            #pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                uint32_t a[32];
                 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const float x = __uint_as_float(a[e]), y = total ? __uint_as_float(t[e]) : 0.f;
-                    a[e] = __float_as_uint(__fmul_rn(x, f));
-                    t[e] = __float_as_uint(__fmul_rn(fold ? __fadd_rn(x, y) : y, f));
+                for (int c = 0; c < 8; ++c) {
+                    const uint4 x = *reinterpret_cast<const uint4*>(sm + kWdStage + h * kAtHalf + row * 128 +
+                                                                    ((c ^ (row & 7)) << 4));
+                    a[4 * c] = x.x;
+                    a[4 * c + 1] = x.y;
+                    a[4 * c + 2] = x.z;
+                    a[4 * c + 3] = x.w;
                 }
-                if (!fold) tmem_st16(o_tm + 16 * c, a);
-                if (fold || total) tmem_st16(t_tm + 16 * c, t);
+                tmem_st32(tmem + lanes + kWdQ1 + 32 * h, a);
+            }
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.bar_q1);
+        }
+        // this row's outputs go into their total (`total`: there is one), which
+        // is then scaled by f
+        auto fold = [&](bool total, float f) {
+            const bool scale = __any_sync(0xffffffffu, f != 1.f);
+            if (!total && !scale) {
+                #pragma unroll 1
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t a[32];
+                    tmem_ld32(o_tm + 32 * c, a);
+                    tmem_ld_wait();
+                    tmem_st32(t_tm + 32 * c, a);
+                }
+                return;
+            }
+            #pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+                uint32_t a[32], t[32];
+                tmem_ld32(o_tm + 32 * c, a);
+                if (total) tmem_ld32(t_tm + 32 * c, t);
+                tmem_ld_wait();
+                if (total) {
+                    #pragma unroll
+                    for (int e = 0; e < 32; ++e)
+                        a[e] = __float_as_uint(__fadd_rn(__uint_as_float(a[e]), __uint_as_float(t[e])));
+                }
+                if (scale) {
+                    #pragma unroll
+                    for (int e = 0; e < 32; ++e) a[e] = __float_as_uint(__fmul_rn(__uint_as_float(a[e]), f));
+                }
+                tmem_st32(t_tm + 32 * c, a);
             }
         };
-        for (int j = 0; j < n; ++j) {
-            const uint32_t s_tm = tmem + lanes + 64 * (j & 1);
+        auto scale = [&](uint32_t at, float f) {
+            #pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+                uint32_t a[32];
+                tmem_ld32(at + 32 * c, a);
+                tmem_ld_wait();
+                #pragma unroll
+                for (int e = 0; e < 32; ++e) a[e] = __float_as_uint(__fmul_rn(__uint_as_float(a[e]), f));
+                tmem_st32(at + 32 * c, a);
+            }
+        };
+        for (int j = 0; j < n && ok; ++j) {
+            const uint32_t s_tm = tmem + lanes;
             if (!(ok = at_wait_warp(&sh.bar_s[j & 1], (j >> 1) & 1, ab, err))) break;
             tc_fence_after();
             float s[64];
@@ -199,6 +266,9 @@ __device__ __forceinline__ void attn_wide_core(const W w) {
                     s[32 + i] = __uint_as_float(b[i]);
                 }
             }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.bar_sf);
             const int lim = seen - j * kWdKeys;
             if (__any_sync(0xffffffffu, lim < kWdKeys)) {
                 #pragma unroll
@@ -231,11 +301,17 @@ __device__ __forceinline__ void attn_wide_core(const W w) {
             if (j > 0) {
                 if (!(ok = at_wait_warp(&sh.bar_vf, (j - 1) & 1, ab, err))) break;
                 tc_fence_after();
-                const bool fold = j % kWdFold == 0;
-                if (fold || __any_sync(0xffffffffu, !fine)) outputs(fold, j > kWdFold, f);
             }
             #pragma unroll
             for (int q = 0; q < 3; ++q) tmem_st32(p_tm + 32 * q, u[q]);
+            if (j > 0) {
+                if (j % kWdFold == 0) {
+                    fold(j > kWdFold, f);
+                } else if (__any_sync(0xffffffffu, !fine)) {
+                    scale(o_tm, f);
+                    if (j > kWdFold) scale(t_tm, f);
+                }
+            }
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
@@ -247,7 +323,7 @@ __device__ __forceinline__ void attn_wide_core(const W w) {
                 w.slow(it, warp);
             } else {
                 if (n > kWdFold) {
-                    outputs(true, true, 1.f);
+                    fold(true, 1.f);
                     tmem_st_wait();
                 }
                 w.store(it, row, n > kWdFold ? t_tm : o_tm, m, l, sm + warp * kAtStage);     // the query planes' place is free
@@ -260,12 +336,19 @@ __device__ __forceinline__ void attn_wide_core(const W w) {
         const bool is_v = warp >= 12;
         const float4 none = make_float4(0.f, 0.f, 0.f, 0.f);
         float4 r[8];                    // this warp's rows cw, cw + 8, .. of a tile
+        typename W::Rows rows(w, it, is_v);
         auto load = [&](int j) {
-            #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int key = j * kWdKeys + cw + 8 * i;
-                const T* at = key < keys ? (is_v ? w.v_row(it, key) : w.k_row(it, key)) : nullptr;
-                r[i] = at != nullptr ? ld4(at + 4 * lane) : none;
+            const int key = j * kWdKeys + cw;
+            rows.tile(key, keys);
+            if ((j + 1) * kWdKeys <= keys) {
+                #pragma unroll
+                for (int i = 0; i < 8; ++i) r[i] = ld4(rows.row(i) + 4 * lane);
+            } else {
+                #pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const T* at = rows.row(i) + 4 * lane;
+                    r[i] = key + 8 * i < keys ? ld4(at) : none;
+                }
             }
         };
         load(0);
@@ -280,7 +363,8 @@ __device__ __forceinline__ void attn_wide_core(const W w) {
             #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int row = (warp - 4) + 16 * (i0 + i);
-                store_planes(sm + half * kAtHalf + row * 128, row, lane, kWdQPlane, x[i], plain4(x[i]));
+                store_planes(sm + half * kAtHalf + row * 128, sm + kWdStage + half * kAtHalf + row * 128, row, lane,
+                             kWdQPlane, x[i], plain(top4(x[i], 0.f)));
             }
         }
         auto arrive = [&](uint64_t* bar) {
@@ -289,22 +373,36 @@ __device__ __forceinline__ void attn_wide_core(const W w) {
             if (lane == 0) mbar_arrive(bar);
         };
         arrive(&sh.bar_q);
-        uint8_t* const tile = sm + (is_v ? kWdV : kWdK) + half * kWdHalf;
         #pragma unroll 1
         for (int j = 0; j < n; ++j) {
-            if (j > 0 && !(is_v ? at_wait_warp(&sh.bar_vf, (j - 1) & 1, ab, err)
-                                : at_wait_warp(&sh.bar_s[(j - 1) & 1], ((j - 1) >> 1) & 1, ab, err)))
-                break;
-            bool odd = false;
-            #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int row = cw + 8 * i;
-                const bool plain = plain4(r[i]);
-                store_planes(tile + row * 128, row, lane, kWdPlane, r[i], plain);
-                odd = odd || (!plain && j * kWdKeys + row >= every);
+            // the place is free: values when the products before are done, keys
+            // when the scores two tiles before are (the second place: when the
+            // queries' first plane has left it)
+            if (is_v) {
+                if (j > 0 && !at_wait_warp(&sh.bar_vf, (j - 1) & 1, ab, err)) break;
+            } else if (j > 0) {
+                if (!at_wait_warp(j > 1 ? &sh.bar_s[j & 1] : &sh.bar_q1, j > 1 ? ((j >> 1) - 1) & 1 : 0, ab, err)) break;
             }
-            if (is_v && odd) sh.odd = 1;
-            arrive(is_v ? &sh.bar_v : &sh.bar_k);
+            uint8_t* const tile = sm + (is_v ? kWdV : kWdK + (j & 1) * 3 * kWdPlane) + half * kWdHalf;
+            float top = 0.f;
+            #pragma unroll
+            for (int i = 0; i < 8; ++i) top = top4(r[i], top);
+            if (__all_sync(0xffffffffu, plain(top))) {
+                #pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    store_planes(tile + kWdPlane + (cw + 8 * i) * 128, tile + (cw + 8 * i) * 128, cw, lane, kWdPlane, r[i], true);
+            } else {
+                bool odd = false;
+                #pragma unroll 1
+                for (int i = 0; i < 8; ++i) {
+                    const float4 x = pick(r, i);
+                    const bool whole = plain(top4(x, 0.f));
+                    store_planes(tile + kWdPlane + (cw + 8 * i) * 128, tile + (cw + 8 * i) * 128, cw, lane, kWdPlane, x, whole);
+                    odd = odd || (!whole && j * kWdKeys + cw + 8 * i >= every);
+                }
+                if (is_v && odd) sh.odd = 1;
+            }
+            arrive(is_v ? &sh.bar_v : &sh.bar_k[j & 1]);
             if (j + 1 < n) load(j + 1);
         }
     } else {
@@ -317,16 +415,23 @@ __device__ __forceinline__ void attn_wide_core(const W w) {
             // first; loops, since unrolled their 72 descriptors leave the registers
             constexpr uint32_t kFirst = 0x001102u, kSecond = 0x010120u;
             auto scores = [&](int j) {
-                const uint32_t d = tmem + 64 * (j & 1);
+                const uint32_t kj = k0 + (j & 1) * (3 * kWdPlane >> 4);
                 #pragma unroll 1
                 for (int y = 0; y < 6; ++y) {
-                    const uint32_t q = q0 + (kFirst >> (4 * y) & 15u) * (kWdQPlane >> 4),
-                                   k = k0 + (kSecond >> (4 * y) & 15u) * (kWdPlane >> 4);
-                    #pragma unroll
-                    for (int x = 0; x < 8; ++x)
-                        umma_f16_ss(d, q + (((x >> 2) * kAtHalf + (x & 3) * 32) >> 4),
-                                    k + (((x >> 2) * kWdHalf + (x & 3) * 32) >> 4), umma_idesc_bf16(128, 64, false),
-                                    x > 0 || y > 0);
+                    const uint32_t a = kFirst >> (4 * y) & 15u, k = kj + (kSecond >> (4 * y) & 15u) * (kWdPlane >> 4);
+                    if (a == 0) {
+                        #pragma unroll
+                        for (int x = 0; x < 8; ++x)
+                            umma_f16_ts(tmem, tmem + kWdQ1 + 8 * x, k + (((x >> 2) * kWdHalf + (x & 3) * 32) >> 4),
+                                        umma_idesc_bf16(128, 64, false), x > 0 || y > 0);
+                    } else {
+                        const uint32_t q = q0 + (a - 1) * (kWdQPlane >> 4);
+                        #pragma unroll
+                        for (int x = 0; x < 8; ++x)
+                            umma_f16_ss(tmem, q + (((x >> 2) * kAtHalf + (x & 3) * 32) >> 4),
+                                        k + (((x >> 2) * kWdHalf + (x & 3) * 32) >> 4), umma_idesc_bf16(128, 64, false),
+                                        x > 0 || y > 0);
+                    }
                 }
                 umma_commit(&sh.bar_s[j & 1]);
             };
@@ -343,7 +448,8 @@ __device__ __forceinline__ void attn_wide_core(const W w) {
                 }
                 umma_commit(&sh.bar_vf);
             };
-            bool ok = at_wait(&sh.bar_q, 0, ab, err) && at_wait(&sh.bar_k, 0, ab, err);
+            bool ok = at_wait(&sh.bar_q, 0, ab, err) && at_wait(&sh.bar_q1, 0, ab, err) &&
+                      at_wait(&sh.bar_k[0], 0, ab, err);
             if (ok) {
                 tc_fence_after();
                 scores(0);
@@ -351,7 +457,9 @@ __device__ __forceinline__ void attn_wide_core(const W w) {
             #pragma unroll 1
             for (int j = 0; j < n && ok; ++j) {
                 if (j + 1 < n) {
-                    if (!(ok = at_wait(&sh.bar_k, (j + 1) & 1, ab, err))) break;
+                    if (!(ok = at_wait(&sh.bar_k[(j + 1) & 1], ((j + 1) >> 1) & 1, ab, err) &&
+                               at_wait(&sh.bar_sf, j & 1, ab, err)))
+                        break;
                     tc_fence_after();
                     scores(j + 1);
                 }
