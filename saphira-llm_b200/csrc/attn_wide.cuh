@@ -12,26 +12,35 @@
 // One CTA: 128 query rows of one head against 64 keys at a time.
 //
 //   warps 0-3        softmax, one thread per row; at the end the outputs.
-//   warps 4-11, 12-19  the operands: both groups the rows of Q, then one the key
-//                    and one the value tiles: from global memory (the next
-//                    tile waits in registers), split, into shared memory in
-//                    the layouts the products want. Sixteen warps: with eight
-//                    the splitting took twice the products' time.
+//   warps 4-11, 12-19  the operands: the keys' and the values' tiles from
+//                    global memory (the next tile waits in registers), split,
+//                    into shared memory in the layouts the products want.
+//                    Sixteen warps: with eight the splitting took twice the
+//                    products' time. At the start all twenty split Q.
 //   warp 20, 1 lane  tcgen05.mma: 6 x 8 products of N = 64 for a tile's scores,
 //                    6 x 4 of N = 128 for the outputs, with the weights' planes
 //                    from tensor memory. The scores of tile j + 1 are made
-//                    under the softmax of tile j.
+//                    under the softmax of tile j, which reads its own first.
+//
+// Q's first plane, which three of the six products take, lies in tensor memory:
+// those read 2 KB of shared memory instead of 6 (32 clocks instead of 48), and
+// the place it leaves holds a second tile of keys.
 //
 // Products of different shapes are not ordered among themselves, so none
 // touches tensor memory that one of the other shape reads or writes, except
-// across a commit: scores 2 x 64 columns, weights 96, outputs 2 x 128. (One
+// across a commit: scores 64 columns, Q 64, weights 96, outputs 2 x 128. (One
 // product of N = 192 over a key tile's three planes, the softmax adding the
-// column groups, would need 1664 clocks for the scores instead of 2304, but
-// partial sums of three shapes would lean on an order that is not promised.)
+// column groups, would save a quarter of the scores' time, but partial sums of
+// three shapes would lean on an order that is not promised.)
 //
-// Bound by the products: the scores' operands come from shared memory, 6 KB in
-// 48 clocks each; 48 x 48 + 24 x 64 = 3840 clocks a tile of 4.2 MFLOP, 290
-// TFLOP/s over 148 SMs at 1.8 GHz.
+// Bound by the products and, at half their time each, the softmax and the
+// splitting that run beside them: 24 x 32 + 24 x 48 + 24 x 64 = 3456 clocks a
+// tile of 4.2 MFLOP, 323 TFLOP/s over 148 SMs at 1.8 GHz. Measured 2.7 us a
+// tile (4096 tokens, 20 heads: 380 us, 226 TFLOP/s): 2.4 us with the splitting
+// left out, 1.7 us with the products cut to a sixth besides. Four prompts of
+// 320, 1, 777 and 256 tokens: 48 us, of which 38 us are the longest row tile's
+// thirteen key tiles; an item's start and end cost about 6 us. 32 heads of 8
+// against a prefix of 16384: 61 us.
 //
 // Registers: 768 threads x 80 at launch; 152 (softmax) + 4 x 72 (operands) + 40
 // = 480 = 6 x 80 after the split.
@@ -41,6 +50,8 @@
 // recompute its rows one by one. A key or value that a row does see and that
 // is no finite number makes that row no number.
 #pragma once
+
+#include <type_traits>
 
 #include "attn_mma.cuh"
 
@@ -148,7 +159,7 @@ __device__ __forceinline__ void attn_wide_core(const W w) {
         return;
     }
     if (threadIdx.x == 0) {
-        mbar_init(&sh.bar_q, 16);
+        mbar_init(&sh.bar_q, 20);
         mbar_init(&sh.bar_q1, 4);
         mbar_init(&sh.bar_k[0], 8);
         mbar_init(&sh.bar_k[1], 8);
@@ -176,6 +187,31 @@ __device__ __forceinline__ void attn_wide_core(const W w) {
     volatile int* const ab = &sh.abort_flag;
     const int keys = w.keys(it), n = (keys + kWdKeys - 1) / kWdKeys;
 
+    const int half = lane >> 4;
+    auto arrive = [&](uint64_t* bar) {      // what this warp wrote is the products'
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar);
+    };
+    // N rows of Q, all their loads in flight: the softmax warps take the upper
+    // half, the operands' warps the lower
+    auto split_q = [&](auto count, int first, int step) {
+        constexpr int N = decltype(count)::value;
+        float4 x[N];
+        #pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int row = first + i * step;
+            x[i] = w.live(it, row) ? ld4(w.q_row(it, row) + 4 * lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        #pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int row = first + i * step;
+            store_planes(sm + half * kAtHalf + row * 128, sm + kWdStage + half * kAtHalf + row * 128, row, lane, kWdQPlane,
+                         x[i], plain(top4(x[i], 0.f)));
+        }
+        arrive(&sh.bar_q);
+    };
+
     if (warp < 4) {
         // ---------------- softmax ----------------
         reg_alloc<152>();
@@ -185,6 +221,7 @@ __device__ __forceinline__ void attn_wide_core(const W w) {
         const bool live = w.live(it, row);
         const int seen = w.seen(it, row);
         float m = -INFINITY, l = 0.f;
+        split_q(std::integral_constant<int, 16>{}, kAtRows / 2 + 16 * warp, 1);
         // this row's first plane of Q, from the staging place
         bool ok = at_wait_warp(&sh.bar_q, 0, ab, err);
         if (ok) {
@@ -332,7 +369,7 @@ __device__ __forceinline__ void attn_wide_core(const W w) {
     } else if (warp < 20) {
         // ---------------- operands ----------------
         reg_dealloc<72>();
-        const int cw = (warp - 4) & 7, half = lane >> 4, every = w.seen(it, 0);
+        const int cw = (warp - 4) & 7, every = w.seen(it, 0);
         const bool is_v = warp >= 12;
         const float4 none = make_float4(0.f, 0.f, 0.f, 0.f);
         float4 r[8];                    // this warp's rows cw, cw + 8, .. of a tile
@@ -352,27 +389,7 @@ __device__ __forceinline__ void attn_wide_core(const W w) {
             }
         };
         load(0);
-        #pragma unroll 1
-        for (int i0 = 0; i0 < kAtRows / 16; i0 += 4) {
-            float4 x[4];
-            #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int row = (warp - 4) + 16 * (i0 + i);
-                x[i] = w.live(it, row) ? ld4(w.q_row(it, row) + 4 * lane) : none;
-            }
-            #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int row = (warp - 4) + 16 * (i0 + i);
-                store_planes(sm + half * kAtHalf + row * 128, sm + kWdStage + half * kAtHalf + row * 128, row, lane,
-                             kWdQPlane, x[i], plain(top4(x[i], 0.f)));
-            }
-        }
-        auto arrive = [&](uint64_t* bar) {
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar);
-        };
-        arrive(&sh.bar_q);
+        split_q(std::integral_constant<int, 4>{}, warp - 4, 16);
         #pragma unroll 1
         for (int j = 0; j < n; ++j) {
             // the place is free: values when the products before are done, keys
