@@ -240,7 +240,12 @@ __device__ __forceinline__ void store_rows(uint32_t o_tmem, float f, uint8_t* st
 //
 // What bounds it: per key tile and row tile 1024 clocks of products, and the
 // chain S -> softmax -> P V -> S', whose softmax is 16384 exponentials at 16
-// a clock, shared by the two tiles.
+// a clock, shared by the two tiles. Measured: one prompt of 16384 tokens, 16
+// heads, 845 us (1302 TFLOP/s, 78% of a library GEMM's best); 4096 tokens, 36
+// heads, 134 us (1153); 1024 tokens, 64 heads, 30 us (571: an item's start and
+// end are 2-3 us, and here most items have four key tiles); 17 tokens 8 us.
+// Part of the exponentials as polynomials on the ordinary pipes: slower (889 to
+// 919 us against 871 where it was tried).
 //
 // Masks: a row sees the item's first so many keys, so only an item's last key
 // tiles are masked. A value row behind the item's keys is zeroed in shared
