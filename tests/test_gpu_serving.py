@@ -301,6 +301,38 @@ def test_page_operations_in_any_order(cuda, page, dt, n_pages, n_slots, width, s
     assert seen[0] > steps // 4
 
 
+def test_page_operations_on_many_slots(cuda):
+    """More slots than the reserving CTA has threads and the clusters have
+    warps: several rounds of each, pages shared across the rounds."""
+    n_slots = 2100
+    c = Cache(cuda, 9000, n_slots, 6, 16, 1, 1, "f16", seed=3)
+    rng = np.random.default_rng(11)
+
+    def step(op, *args):
+        want = getattr(c.m, op)(*args)
+        want = want[0] if isinstance(want, tuple) else want
+        getattr(c.p, op)(*[None if a is None else _i32(a) for a in args], c.work, c.status)
+        c.same()
+        assert c.take_status() == want
+        return want
+
+    order = [int(x) for x in rng.permutation(n_slots)]
+    assert step("reserve", order[:700], [int(x) for x in rng.integers(1, 40, 700)]) == 0
+    assert step("fork", [order[i % 700] for i in range(1400)], order[700:]) == 0
+    # one token each: shared last pages are copied, the last owner keeps one
+    assert step("reserve", order, [1] * n_slots) == 0
+    again = [int(x) for x in rng.permutation(n_slots)]
+    assert step("reserve", again[:1900], [int(x) for x in rng.integers(0, 30, 1900)]) == 0
+    assert step("reserve", order, [97] * n_slots) == -36
+    keep = [int(rng.integers(0, c.m.lens[s] + 1)) for s in again]
+    assert step("release", again, keep[:-1] + [c.m.lens[again[-1]] + 1]) == -1
+    assert step("release", again, keep) == 0
+    assert step("compact") == 0
+    assert step("fork", order[:2000], again[:2000]) == 0
+    assert step("fork", order[:2000], again[:1999] + again[:1]) == -1
+    assert step("release", order[:1500], None) == 0
+
+
 def test_page_errors_change_nothing(cuda):
     c = Cache(cuda, 20, 4, 4, 16)
     m = c.m
