@@ -265,7 +265,7 @@ _FLOATS = {"f32": abi.KV_F32, "f16": abi.KV_F16}
 
 
 def _type(t):
-    kind = _FLOATS.get(_kind(t.dtype))
+    kind = _FLOATS.get(_DTYPES.get(t.dtype) or _kind(t.dtype))
     if kind is None:
         raise TypeError(f"dtype {t.dtype}: float32 or float16 expected")
     return kind
@@ -275,7 +275,7 @@ def _ints(t, n, where, name):
     """The address of an int32 array of at least n elements, or None."""
     if t is None:
         return None
-    if _kind(t.dtype) != "i32" or not t.is_contiguous() or t.numel() < n:
+    if (_DTYPES.get(t.dtype) or _kind(t.dtype)) != "i32" or not t.is_contiguous() or t.numel() < n:
         raise ValueError(f"{where}: {name} must be {n} contiguous int32 values")
     return t.data_ptr()
 
@@ -384,6 +384,11 @@ class KvPages:
         if rc:
             _check(rc, "kv_compact")
 
+    def _out(self, t, n, h):
+        if t.shape != (n, h, abi.HEAD_DIM) or not t.is_contiguous() or _type(t) != self._kv_type:
+            raise ValueError("kv_append: outputs must be contiguous, of the cache's type")
+        return t.data_ptr()
+
     def append(self, layer, slot, pos, q, k, v, cos, sin, q_out=None, k_out=None, v_out=None, status=None,
                stream=None):
         w = "kv_append"
@@ -394,22 +399,21 @@ class KvPages:
             raise ValueError("kv_append: q, k, v disagree in tokens, or with the cache's heads")
         if (q is None) != (q_out is None):
             raise ValueError("kv_append: q and q_out go together")
-        if not (_kind(k.dtype) == _kind(v.dtype) == _kind(cos.dtype) == _kind(sin.dtype) == "f32") or (
-                q is not None and _kind(q.dtype) != "f32"):
+        f32 = k.dtype
+        if _kind(f32) != "f32" or v.dtype != f32 or cos.dtype != f32 or sin.dtype != f32 or (
+                q is not None and q.dtype != f32):
             raise ValueError("kv_append: q, k, v, cos and sin must be float32")
-        outs = []
-        for t, m in ((q_out, h), (k_out, hk), (v_out, hk)):
-            if t is not None and (not t.is_contiguous() or t.shape != (n, m, abi.HEAD_DIM) or
-                                  _type(t) != self._kv_type):
-                raise ValueError("kv_append: outputs must be contiguous, of the cache's type")
-            outs.append(None if t is None else t.data_ptr())
-        if not (cos.is_contiguous() and sin.is_contiguous() and cos.shape == sin.shape and cos.dim() == 2 and
-                cos.shape[1] == 64):
+        qo = None if q_out is None else self._out(q_out, n, h)
+        ko = None if k_out is None else self._out(k_out, n, hk)
+        vo = None if v_out is None else self._out(v_out, n, hk)
+        shape = cos.shape
+        if not (len(shape) == 2 and shape[1] == 64 and sin.shape == shape and cos.is_contiguous() and
+                sin.is_contiguous()):
             raise ValueError("kv_append: cos and sin must be [positions][64]")
         if n == 0:
             return
         rc = lib().sllm_cuda_kv_append(self._p, layer, n, _ints(slot, n, w, "slot"), _ints(pos, n, w, "pos"), h, qp, qs,
-                                       kp, ks, vp, vs, cos.data_ptr(), sin.data_ptr(), cos.shape[0], *outs,
+                                       kp, ks, vp, vs, cos.data_ptr(), sin.data_ptr(), shape[0], qo, ko, vo,
                                        _ints(status, 1, w, "status"), _stream(stream))
         if rc:
             _check(rc, w)
