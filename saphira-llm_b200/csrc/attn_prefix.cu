@@ -18,8 +18,8 @@
 // 8000 keys the two launches and the chain of dependent reads in them, 12 us.
 // Measured, f16: 16 sequences of up to 300 tokens behind 4096, 20 heads of 5,
 // 19 us; 64 of up to 1000 behind 32768, four query tokens each, 64 heads of 8,
-// 288 us (969 TFLOP/s). f32: two of 64 behind 256, 20 heads of 5, 14 us; four
-// behind 16384, 32 heads of 8, 61 us.
+// 288 us (969 TFLOP/s). f32: two of 64 behind 256, 20 heads of 5, 13.4 us; four
+// behind 16384, 32 heads of 8, 59 us.
 // The cut is made on the host, from sizes alone: made on the device, from the
 // lengths, it put two dependent reads before the first item (27.6 us against
 // 18.0 us for the 16 sequences).
@@ -333,8 +333,14 @@ struct PrefixWide {
             return pool + __shfl_sync(0xffffffffu, (unsigned long long)mine, i);
         }
     };
-    __device__ __forceinline__ void store(const Item& it, int row, uint32_t o_tm, float m, float l, uint8_t* stage) const {
-        store_parts(p, it, it.row0, row, o_tm, m, l, stage);
+    __device__ __forceinline__ float scale(float) const { return 1.f; }
+    __device__ __forceinline__ WideOut out(const Item& it, int row) const {
+        const int parts = p.plan.sp + p.plan.cm;
+        return WideOut{p.part_o + part_at(p, it, it.row0 + row) * kServeDim, (size_t)parts * kServeDim,
+                       it.row_end - (it.row0 + row)};
+    }
+    __device__ __forceinline__ void finish(const Item& it, int row, float m, float l) const {
+        p.part_ml[part_at(p, it, it.row0 + row)] = make_float2(m * kServeScale, l);
     }
     __device__ __forceinline__ void slow(const Item& it, int warp) const { slow_parts<T>(pg, p, it, it.row0, warp); }
 };

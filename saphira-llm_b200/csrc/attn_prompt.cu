@@ -8,7 +8,7 @@
 // per item, the longest launched first. What bounds the two stands there.
 // Measured: prompts of 8192, 1, 300, 1021, 0, 2048, 513 and 64 tokens together,
 // 64 heads of 8, f16: 1.03 ms (1158 TFLOP/s); of 320, 1, 777 and 256, 20 heads of
-// 5, f32: 48 us.
+// 5, f32: 43.6 us.
 
 #include "attn_mma.cuh"
 #include "attn_wide.cuh"
@@ -44,9 +44,12 @@ __device__ __forceinline__ bool find_long_first(const PromptParams& p, int x, in
         *a = min(max(p.cu[s], 0), p.n_tokens);
         return min(max(p.cu[s + 1], *a), p.n_tokens) - *a;
     };
+    // the first 32 sequences' tiles stay in registers
+    int a0;
+    const int t0 = lane < p.n_seq ? (seq(lane, &a0) + R - 1) / R : 0;
     auto at_least = [&](int t) {
-        int f = 0, a;
-        for (int s = lane; s < p.n_seq; s += 32) f += max((seq(s, &a) + R - 1) / R - t, 0);
+        int f = max(t0 - t, 0), a;
+        for (int s = lane + 32; s < p.n_seq; s += 32) f += max((seq(s, &a) + R - 1) / R - t, 0);
         return __reduce_add_sync(0xffffffffu, f);
     };
     int lo = 0, hi = (p.n_tokens + R - 1) / R;          // F(lo) > x >= F(hi), if x is a tile at all
@@ -215,12 +218,13 @@ struct PromptWide {
         __device__ __forceinline__ void tile(int key, int) { at = base + (size_t)key * stride; }
         __device__ __forceinline__ const float* row(int i) const { return at + (size_t)(8 * i) * stride; }
     };
-    __device__ __forceinline__ void store(const Item& it, int row, uint32_t o_tm, float, float l, uint8_t* stage) const {
-        const int x0 = it.tile * kAtRows + (row & ~31);
-        store_rows(o_tm, 1.f / l, stage,
-                   static_cast<float*>(p.out) + (size_t)(it.start + x0) * p.os + (size_t)it.head * kServeDim, p.os,
-                   it.len - x0);
+    __device__ __forceinline__ float scale(float l) const { return 1.f / l; }
+    __device__ __forceinline__ WideOut out(const Item& it, int row) const {
+        const int x0 = it.tile * kAtRows + row;
+        return WideOut{static_cast<float*>(p.out) + (size_t)(it.start + x0) * p.os + (size_t)it.head * kServeDim, p.os,
+                       it.len - x0};
     }
+    __device__ __forceinline__ void finish(const Item&, int, float, float) const {}
     __device__ __forceinline__ void slow(const Item& it, int warp) const {
         slow_rows<float, float>(p, it.head, it.start, it.len, it.tile * kAtRows, warp);
     }

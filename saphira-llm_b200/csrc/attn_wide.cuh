@@ -11,12 +11,13 @@
 //
 // One CTA: 128 query rows of one head against 64 keys at a time.
 //
-//   warps 0-3        softmax, one thread per row; at the end the outputs.
+//   warps 0-3        softmax, one thread per row (warp 0 finds the item first).
 //   warps 4-11, 12-19  the operands: the keys' and the values' tiles from
 //                    global memory (the next tile waits in registers), split,
 //                    into shared memory in the layouts the products want.
 //                    Sixteen warps: with eight the splitting took twice the
-//                    products' time. At the start all twenty split Q.
+//                    products' time. At the start all twenty split Q; at the
+//                    end these sixteen store the outputs, 32 x 32 each.
 //   warp 20, 1 lane  tcgen05.mma: 6 x 8 products of N = 64 for a tile's scores,
 //                    6 x 4 of N = 128 for the outputs, with the weights' planes
 //                    from tensor memory. The scores of tile j + 1 are made
@@ -35,12 +36,14 @@
 //
 // Bound by the products and, at half their time each, the softmax and the
 // splitting that run beside them: 24 x 32 + 24 x 48 + 24 x 64 = 3456 clocks a
-// tile of 4.2 MFLOP, 323 TFLOP/s over 148 SMs at 1.8 GHz. Measured 2.7 us a
-// tile (4096 tokens, 20 heads: 380 us, 226 TFLOP/s): 2.4 us with the splitting
-// left out, 1.7 us with the products cut to a sixth besides. Four prompts of
-// 320, 1, 777 and 256 tokens: 48 us, of which 38 us are the longest row tile's
-// thirteen key tiles; an item's start and end cost about 6 us. 32 heads of 8
-// against a prefix of 16384: 61 us.
+// tile of 4.2 MFLOP, 323 TFLOP/s over 148 SMs at 1.8 GHz. Measured 2.6 us a
+// tile (4096 tokens, 20 heads: 372 us, 231 TFLOP/s); with the splitting left out
+// 2.4 us, with the products cut to a sixth besides 1.7 us. An item's start and
+// end cost about 9 us: 1.2 to find it among several prompts, 2.6 to read and
+// split Q and the first tile, 2.6 for the first scores and softmax, 1.6 for the
+// last products, 1.4 to store. Four prompts of 320, 1, 777 and 256 tokens: 43.6
+// us, the longest row tile's 36 us among them. 32 heads of 8 against a prefix of
+// 16384: 59 us.
 //
 // Registers: 768 threads x 80 at launch; 152 (softmax) + 4 x 72 (operands) + 40
 // = 480 = 6 x 80 after the split.
@@ -134,7 +137,47 @@ __device__ __forceinline__ float4 pick(const float4 (&r)[8], int i) {
 // W: Item; T; find(x, item); keys(item); live(item, row); seen(item, row) (at
 // most keys, least for row 0); q_row(item, row); Rows (one warp's keys or values:
 // tile(key, n): the next are keys key, key + 8, .. below n; row(i): the i-th of
-// them); store(...), slow(...), gave_up().
+// them); scale(l) (what the outputs are multiplied by), out(item, row) (where the
+// rows from `row` on go), finish(item, row, m, l) (the rest of a row's result),
+// slow(...), gave_up().
+struct WideOut {
+    float* base;                    // the first row
+    size_t stride;                  // floats from a row to the next
+    int n;                          // rows to be written
+};
+
+// One warp's 32 rows x 32 columns of outputs, plus their total, times each
+// lane's f, to global memory, through the warp's staging: whole lines, four
+// rows a store.
+__device__ __forceinline__ void store_cols(uint32_t o_tm, uint32_t t_tm, bool total, float f, uint8_t* stage,
+                                           const WideOut& to) {
+    const int lane = threadIdx.x & 31, sub = lane >> 3;
+    #pragma unroll
+    for (int c = 0; c < 2; ++c) {
+        uint32_t a[16], t[16];
+        tmem_ld16(o_tm + 16 * c, a);
+        if (total) tmem_ld16(t_tm + 16 * c, t);
+        tmem_ld_wait();
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float x[4];
+            #pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                x[e] = __uint_as_float(a[4 * i + e]);
+                if (total) x[e] = __fadd_rn(x[e], __uint_as_float(t[4 * i + e]));
+                x[e] = __fmul_rn(x[e], f);
+            }
+            *reinterpret_cast<float4*>(stage + lane * kAtStageRow + 64 * c + 16 * i) = make_float4(x[0], x[1], x[2], x[3]);
+        }
+    }
+    __syncwarp();
+    #pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float4 u = *reinterpret_cast<const float4*>(stage + (4 * i + sub) * kAtStageRow + 16 * (lane & 7));
+        if (4 * i + sub < to.n) st4(to.base + (size_t)(4 * i + sub) * to.stride + 4 * (lane & 7), u);
+    }
+}
+
 template <class W>
 __device__ __forceinline__ void attn_wide_core(const W w) {
     using T = typename W::T;
@@ -144,21 +187,29 @@ __device__ __forceinline__ void attn_wide_core(const W w) {
         // q: split; q1: the first plane in tensor memory; k, v: tile split; vf:
         // its products done; s: scores (and the keys' place free; by tile
         // parity, since a wait may come two tiles late); sf: scores read; p:
-        // weights; o: all
-        uint64_t bar_q, bar_q1, bar_k[2], bar_v, bar_vf, bar_s[2], bar_sf, bar_p, bar_o;
+        // weights; f: the rows' factors; o: all
+        uint64_t bar_q, bar_q1, bar_k[2], bar_v, bar_vf, bar_s[2], bar_sf, bar_p, bar_f, bar_o;
+        typename W::Item item;
+        float f[kAtRows];
         uint32_t tmem;
-        int abort_flag, odd;
+        int abort_flag, odd, none;
     };
     static_assert(sizeof(Shared) <= kWdSmem - kWdEnd, "the part behind the planes");
     Shared& sh = *reinterpret_cast<Shared*>(sm + kWdEnd);
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-    typename W::Item it;
-    if (!w.find(blockIdx.x, &it) || it.last()) return;      // the grid is an upper bound
     if ((smem_u32(sm) & 1023u) != 0) {
         if (threadIdx.x == 0) atomicExch(err, 2);
         return;
     }
-    if (threadIdx.x == 0) {
+    if (warp == 0) {                    // (by every warp it took twice as long)
+        typename W::Item it;
+        const bool found = w.find(blockIdx.x, &it) && !it.last();       // the grid is an upper bound
+        if (lane == 0) {
+            sh.item = it;
+            sh.none = !found;
+        }
+    }
+    if (threadIdx.x == 32) {
         mbar_init(&sh.bar_q, 20);
         mbar_init(&sh.bar_q1, 4);
         mbar_init(&sh.bar_k[0], 8);
@@ -169,6 +220,7 @@ __device__ __forceinline__ void attn_wide_core(const W w) {
         mbar_init(&sh.bar_s[1], 1);
         mbar_init(&sh.bar_sf, 4);
         mbar_init(&sh.bar_p, 4);
+        mbar_init(&sh.bar_f, 4);
         mbar_init(&sh.bar_o, 1);
         sh.abort_flag = 0;
         sh.odd = 0;
@@ -184,6 +236,12 @@ __device__ __forceinline__ void attn_wide_core(const W w) {
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sh.tmem;
+    if (sh.none) {
+        if (warp == 20)
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+        return;
+    }
+    const typename W::Item it = sh.item;
     volatile int* const ab = &sh.abort_flag;
     const int keys = w.keys(it), n = (keys + kWdKeys - 1) / kWdKeys;
 
@@ -193,21 +251,39 @@ __device__ __forceinline__ void attn_wide_core(const W w) {
         __syncwarp();
         if (lane == 0) mbar_arrive(bar);
     };
+    // a row without anything
+    auto store_none = [&](uint8_t* at, uint8_t* first, int r, int plane) {
+        const int in = ((((lane & 15) >> 1) ^ (r & 7)) << 4) + (lane & 1) * 8;
+        *reinterpret_cast<uint2*>(first + in) = make_uint2(0u, 0u);
+        *reinterpret_cast<uint2*>(at + in) = make_uint2(0u, 0u);
+        *reinterpret_cast<uint2*>(at + in + plane) = make_uint2(0u, 0u);
+    };
     // N rows of Q, all their loads in flight: the softmax warps take the upper
     // half, the operands' warps the lower
-    auto split_q = [&](auto count, int first, int step) {
+    auto split_q = [&](auto count, int from, int step) {
         constexpr int N = decltype(count)::value;
-        float4 x[N];
-        #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int row = first + i * step;
-            x[i] = w.live(it, row) ? ld4(w.q_row(it, row) + 4 * lane) : make_float4(0.f, 0.f, 0.f, 0.f);
-        }
-        #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int row = first + i * step;
-            store_planes(sm + half * kAtHalf + row * 128, sm + kWdStage + half * kAtHalf + row * 128, row, lane, kWdQPlane,
-                         x[i], plain(top4(x[i], 0.f)));
+        uint8_t* const at = sm + half * kAtHalf;
+        if (w.live(it, from + (N - 1) * step)) {
+            float4 x[N];
+            #pragma unroll
+            for (int i = 0; i < N; ++i) x[i] = ld4(w.q_row(it, from + i * step) + 4 * lane);
+            #pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int row = from + i * step;
+                store_planes(at + row * 128, at + kWdStage + row * 128, row, lane, kWdQPlane, x[i], plain(top4(x[i], 0.f)));
+            }
+        } else {
+            // the rows behind the last are zeros
+            #pragma unroll 2
+            for (int i = 0; i < N; ++i) {
+                const int row = from + i * step;
+                if (w.live(it, row)) {
+                    const float4 x = ld4(w.q_row(it, row) + 4 * lane);
+                    store_planes(at + row * 128, at + kWdStage + row * 128, row, lane, kWdQPlane, x, plain(top4(x, 0.f)));
+                } else {
+                    store_none(at + row * 128, at + kWdStage + row * 128, row, kWdQPlane);
+                }
+            }
         }
         arrive(&sh.bar_q);
     };
@@ -354,17 +430,12 @@ __device__ __forceinline__ void attn_wide_core(const W w) {
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.bar_p);
         }
+        sh.f[row] = w.scale(l);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.bar_f);
         if (ok && at_wait_warp(&sh.bar_o, 0, ab, err)) {
-            tc_fence_after();
-            if (*(volatile int*)&sh.odd != 0) {
-                w.slow(it, warp);
-            } else {
-                if (n > kWdFold) {
-                    fold(true, 1.f);
-                    tmem_st_wait();
-                }
-                w.store(it, row, n > kWdFold ? t_tm : o_tm, m, l, sm + warp * kAtStage);     // the query planes' place is free
-            }
+            if (*(volatile int*)&sh.odd != 0) w.slow(it, warp);
+            else if (live) w.finish(it, row, m, l);
         }
     } else if (warp < 20) {
         // ---------------- operands ----------------
@@ -404,10 +475,19 @@ __device__ __forceinline__ void attn_wide_core(const W w) {
             float top = 0.f;
             #pragma unroll
             for (int i = 0; i < 8; ++i) top = top4(r[i], top);
-            if (__all_sync(0xffffffffu, plain(top))) {
+            const int rows = keys - j * kWdKeys - cw;           // this warp's are those at 8 i < rows
+            const bool ordinary = __all_sync(0xffffffffu, plain(top));
+            if (ordinary && rows > 56) {
                 #pragma unroll
                 for (int i = 0; i < 8; ++i)
                     store_planes(tile + kWdPlane + (cw + 8 * i) * 128, tile + (cw + 8 * i) * 128, cw, lane, kWdPlane, r[i], true);
+            } else if (ordinary) {
+                #pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    uint8_t *const first = tile + (cw + 8 * i) * 128, *const at = first + kWdPlane;
+                    if (8 * i < rows) store_planes(at, first, cw, lane, kWdPlane, r[i], true);
+                    else store_none(at, first, cw, kWdPlane);
+                }
             } else {
                 bool odd = false;
                 #pragma unroll 1
@@ -421,6 +501,17 @@ __device__ __forceinline__ void attn_wide_core(const W w) {
             }
             arrive(is_v ? &sh.bar_v : &sh.bar_k[j & 1]);
             if (j + 1 < n) load(j + 1);
+        }
+        // the outputs: sixteen warps, 32 rows x 32 columns each (the query
+        // planes' place is free)
+        if (at_wait_warp(&sh.bar_f, 0, ab, err) && at_wait_warp(&sh.bar_o, 0, ab, err) &&
+            *(volatile int*)&sh.odd == 0) {
+            tc_fence_after();
+            const int first = 32 * (warp & 3), col = 32 * ((warp - 4) >> 2);
+            const uint32_t at = tmem + ((uint32_t)first << 16) + col;
+            WideOut to = w.out(it, first);
+            to.base += col;
+            if (to.n > 0) store_cols(at + kWdO, at + kWdT, n > kWdFold, sh.f[first + lane], sm + (warp - 4) * kAtStage, to);
         }
     } else {
         reg_dealloc<40>();
