@@ -134,12 +134,6 @@ __device__ __forceinline__ float4 pick(const float4 (&r)[8], int i) {
     return x;
 }
 
-// W: Item; T; find(x, item); keys(item); live(item, row); seen(item, row) (at
-// most keys, least for row 0); q_row(item, row); Rows (one warp's keys or values:
-// tile(key, n): the next are keys key, key + 8, .. below n; row(i): the i-th of
-// them); scale(l) (what the outputs are multiplied by), out(item, row) (where the
-// rows from `row` on go), finish(item, row, m, l) (the rest of a row's result),
-// slow(...), gave_up().
 struct WideOut {
     float* base;                    // the first row
     size_t stride;                  // floats from a row to the next
@@ -178,6 +172,12 @@ __device__ __forceinline__ void store_cols(uint32_t o_tm, uint32_t t_tm, bool to
     }
 }
 
+// W: Item; T; find(x, item); keys(item); live(item, row); seen(item, row) (at
+// most keys, least for row 0); q_row(item, row); Rows (one warp's keys or values:
+// tile(key, n): the next are keys key, key + 8, .. below n; row(i): the i-th of
+// them); scale(l) (what the outputs are multiplied by), out(item, row) (where the
+// rows from `row` on go), finish(item, row, m, l) (the rest of a row's result),
+// slow(...), gave_up().
 template <class W>
 __device__ __forceinline__ void attn_wide_core(const W w) {
     using T = typename W::T;
