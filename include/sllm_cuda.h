@@ -224,6 +224,9 @@ SLLM_CUDA_API int sllm_cuda_i2s_gemm_silu(const uint8_t * w_gate, const uint8_t 
  * it, not even as an infinity or a NaN. q, k and v have type `type`; out is
  * f32 or, from f16, f16. f16 inputs are multiplied on the tensor cores with
  * f32 sums and softmax; the softmax weights are rounded to f16 there.
+ * (There is no status word: nothing in an array can be wrong here, and offsets
+ * that are stay inside the arrays. sllm_cuda_test_attn_error tells whether a
+ * bounded wait ran out.)
  */
 SLLM_CUDA_API int sllm_cuda_attn_prompt(const void * q, size_t q_stride, const void * k, size_t k_stride,
                                         const void * v, size_t v_stride, int32_t type,

@@ -5,7 +5,7 @@
 //
 // f16: attn_prompt_mma_kernel over attn_mma.cuh, one CTA per SM that walks items
 // dealt longest first. f32: attn_prompt_wide_kernel over attn_wide.cuh, one CTA
-// per item, the longest launched first. What bounds the two stands there.
+// per item, the longest launched first where sequences are few. What bounds the two stands there.
 // Measured: prompts of 8192, 1, 300, 1021, 0, 2048, 513 and 64 tokens together,
 // 64 heads of 8, f16: 1.03 ms (1158 TFLOP/s); of 320, 1, 777 and 256, 20 heads of
 // 5, f32: 43.6 us.
@@ -26,55 +26,104 @@ struct PromptParams {
     int n_seq, n_tokens, n_head, group;
 };
 
-// tile x of the call's tiles of R rows in descending order of their position
-// in their sequence (the later, the more keys they see): the longest work
-// first. Bounds are clamped to the arrays, so a wrong cu stays inside
-// them. F(t) = tiles at positions >= t; a binary search for the position, then
-// the sequence among those that long. One warp.
+// sequence s; its bounds are clamped to the arrays, so a wrong cu stays inside
+__device__ __forceinline__ int seq_len(const PromptParams& p, int s, int* start) {
+    *start = min(max(p.cu[s], 0), p.n_tokens);
+    return min(max(p.cu[s + 1], *start), p.n_tokens) - *start;
+}
+
+// The call's tiles of R rows in descending order of their position in their
+// sequence (the later, the more keys they see): the longest work first. One
+// warp; what it asks for only ever rises, so all of a CTA's searches together
+// walk the sequences once per position. (With a search from the start for each
+// item 256 prompts of 100 to 200 tokens, 20 heads, took 270 us instead of 198,
+// 2048 of 32 to 64 tokens 6.0 ms instead of 1.05.)
+template <int R>
+struct LongFirst {
+    int pos;                        // the position
+    int before;                     // tiles at later positions, and at this one in sequences below s0
+    int s0;
+    __device__ __forceinline__ void start(const PromptParams& p) {
+        int most = 0, a;
+        before = s0 = pos = 0;
+        if (p.n_seq == 1) return;
+        for (int s = threadIdx.x & 31; s < p.n_seq; s += 32) most = max(most, (seq_len(p, s, &a) + R - 1) / R);
+        pos = __reduce_max_sync(0xffffffffu, most) - 1;
+    }
+    // tile x; false: there is none, nor any after it
+    __device__ __forceinline__ bool find(const PromptParams& p, int x, int* start, int* len, int* tile) {
+        const int lane = threadIdx.x & 31;
+        if (p.n_seq == 1) {
+            *len = seq_len(p, 0, start);
+            *tile = (*len + R - 1) / R - 1 - x;
+            return *tile >= 0;
+        }
+        if (x >= p.n_tokens / R + p.n_seq) return false;        // ascending offsets have no more
+        for (; pos >= 0; --pos, s0 = 0) {
+            for (; s0 < p.n_seq; s0 += 32) {
+                int a = 0, n = 0;
+                if (s0 + lane < p.n_seq) n = seq_len(p, s0 + lane, &a);
+                const unsigned has = __ballot_sync(0xffffffffu, (n + R - 1) / R > pos);
+                const int c = __popc(has), r = x - before;
+                if (r < c) {
+                    const int l = __fns(has, 0, r + 1);
+                    *start = __shfl_sync(0xffffffffu, a, l);
+                    *len = __shfl_sync(0xffffffffu, n, l);
+                    *tile = pos;
+                    return true;
+                }
+                before += c;
+            }
+        }
+        return false;
+    }
+};
+
+// ... for a single search among up to 32 sequences: F(t) = tiles at positions
+// >= t; a binary search for the position, then the sequence
 template <int R>
 __device__ __forceinline__ bool find_long_first(const PromptParams& p, int x, int* start, int* len, int* tile) {
     const int lane = threadIdx.x & 31;
-    if (p.n_seq == 1) {
-        *start = min(max(p.cu[0], 0), p.n_tokens);
-        *len = min(max(p.cu[1], *start), p.n_tokens) - *start;
-        *tile = (*len + R - 1) / R - 1 - x;
-        return *tile >= 0;
-    }
-    auto seq = [&](int s, int* a) {
-        *a = min(max(p.cu[s], 0), p.n_tokens);
-        return min(max(p.cu[s + 1], *a), p.n_tokens) - *a;
-    };
-    // the first 32 sequences' tiles stay in registers
-    int a0;
-    const int t0 = lane < p.n_seq ? (seq(lane, &a0) + R - 1) / R : 0;
-    auto at_least = [&](int t) {
-        int f = max(t0 - t, 0), a;
-        for (int s = lane + 32; s < p.n_seq; s += 32) f += max((seq(s, &a) + R - 1) / R - t, 0);
-        return __reduce_add_sync(0xffffffffu, f);
-    };
-    int lo = 0, hi = (p.n_tokens + R - 1) / R;          // F(lo) > x >= F(hi), if x is a tile at all
-    if (at_least(0) <= x) return false;
+    int a = 0, n = 0;
+    if (lane < p.n_seq) n = seq_len(p, lane, &a);
+    const int tiles = (n + R - 1) / R;
+    if (__reduce_add_sync(0xffffffffu, tiles) <= x) return false;
+    int lo = 0, hi = __reduce_max_sync(0xffffffffu, tiles), f_hi = 0;      // F(lo) > x >= F(hi) = f_hi
     while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (at_least(mid) > x) lo = mid;
-        else hi = mid;
-    }
-    int r = x - at_least(lo + 1);                       // the r-th sequence with a tile at lo
-    for (int s0 = 0; s0 < p.n_seq; s0 += 32) {
-        int a = 0, n = 0;
-        if (s0 + lane < p.n_seq) n = seq(s0 + lane, &a);
-        const unsigned has = __ballot_sync(0xffffffffu, (n + R - 1) / R > lo);
-        const int c = __popc(has);
-        if (r < c) {
-            const int l = __fns(has, 0, r + 1);
-            *start = __shfl_sync(0xffffffffu, a, l);
-            *len = __shfl_sync(0xffffffffu, n, l);
-            *tile = lo;
-            return true;
+        const int mid = (lo + hi) / 2, f = __reduce_add_sync(0xffffffffu, max(tiles - mid, 0));
+        if (f > x) {
+            lo = mid;
+        } else {
+            hi = mid;
+            f_hi = f;
         }
-        r -= c;
     }
-    return false;
+    const int l = __fns(__ballot_sync(0xffffffffu, tiles > lo), 0, x - f_hi + 1);
+    *start = __shfl_sync(0xffffffffu, a, l);
+    *len = __shfl_sync(0xffffffffu, n, l);
+    *tile = lo;
+    return true;
+}
+
+// Tile x of R rows in the order of the sequences: sequence s has the numbers
+// from cu[s] / R + s on, of which the last may be nobody's (false). One warp,
+// 32 sequences a probe: for a single search among many.
+template <int R>
+__device__ __forceinline__ bool find_in_order(const PromptParams& p, int x, int* start, int* len, int* tile) {
+    const int lane = threadIdx.x & 31;
+    int lo = 0, hi = p.n_seq, first = 0;
+    for (int step = hi; step > 1;) {
+        step = (hi - lo + 31) / 32;
+        const int s = lo + lane * step;
+        first = s < hi ? min(max(p.cu[s], 0), p.n_tokens) / R + s : 0x7fffffff;
+        const unsigned at = __ballot_sync(0xffffffffu, first <= x);
+        if ((at & 1u) == 0) return false;
+        lo += (31 - __clz(at)) * step;
+        hi = min(hi, lo + step);
+    }
+    *len = seq_len(p, lo, start);
+    *tile = x - (*start / R + lo);
+    return *tile >= 0 && *tile < (*len + R - 1) / R;
 }
 
 // ---------------------------------------------------------------------------
@@ -126,11 +175,12 @@ struct PromptWork {
     const CUtensorMap &tm_q, &tm_k, &tm_v;
 
     struct Finder {
-        __device__ __forceinline__ void start(const PromptWork&) {}
+        LongFirst<kPmRows> order;
+        __device__ __forceinline__ void start(const PromptWork& w) { order.start(w.p); }
         __device__ __forceinline__ long long number(const PromptWork&, int r) { return dealt_number(r); }
-        __device__ __forceinline__ bool item(const PromptWork& w, long long x, Item* it) {      // longest first
+        __device__ __forceinline__ bool item(const PromptWork& w, long long x, Item* it) {
             *it = Item{0, 0, -1, (int)(x % w.p.n_head)};
-            if (!find_long_first<kPmRows>(w.p, (int)(x / w.p.n_head), &it->start, &it->len, &it->tile)) it->tile = -1;
+            if (!order.find(w.p, (int)(x / w.p.n_head), &it->start, &it->len, &it->tile)) it->tile = -1;
             return true;
         }
     };
@@ -194,9 +244,15 @@ struct PromptWide {
     const PromptParams& p;
 
     __device__ __forceinline__ void gave_up() const {}
-    __device__ __forceinline__ bool find(long long x, Item* it) const {      // longest first
+    // longest first; of more than 32 sequences in their order, which takes no
+    // walk over all of them and leaves each SM many items to even out (2048
+    // prompts of 32 to 64 tokens, 20 heads: 4.9 ms longest first, 2.9 ms in order;
+    // 256 of 100 to 200: 940 us and 843 us)
+    __device__ __forceinline__ bool find(long long x, Item* it) const {
+        const int t = (int)(x / p.n_head);
         it->head = (int)(x % p.n_head);
-        return find_long_first<kAtRows>(p, (int)(x / p.n_head), &it->start, &it->len, &it->tile);
+        return p.n_seq > 32 ? find_in_order<kAtRows>(p, t, &it->start, &it->len, &it->tile)
+                            : find_long_first<kAtRows>(p, t, &it->start, &it->len, &it->tile);
     }
     __device__ __forceinline__ int keys(const Item& it) const { return min((it.tile + 1) * kAtRows, it.len); }
     __device__ __forceinline__ int seen(const Item& it, int row) const { return min(it.tile * kAtRows + row + 1, it.len); }

@@ -65,6 +65,26 @@ def test_prompt(cuda, heads, lens, types):
     assert bool((out[T:] == 7.0).all())
 
 
+@pytest.mark.parametrize("n_seq,base", [(32, 0), (33, 3), (65, 0), (1030, 5)])
+@pytest.mark.parametrize("dt", ["f32", "f16"])
+def test_prompt_many_sequences(cuda, dt, n_seq, base):
+    """More sequences than a warp has lanes, of which many are empty; offsets
+    that start behind 0."""
+    import torch
+    rng = np.random.default_rng(n_seq)
+    lens = [int(rng.choice([0, 1, 2, 63, 64, 65, 127, 128, 129, 300])) for _ in range(n_seq)]
+    lens[n_seq // 2] = 700
+    lens[-1] = 0 if base else 257
+    T = base + sum(lens)
+    qkv = _rand(n_seq, T + 2, 4, 128, dt=_dt(dt), scale=1.3)
+    q, k, v = qkv[:, :2], qkv[:, 2:3], qkv[:, 3:]
+    out = torch.full((T + 2, 2, 128), 7.0, dtype=_dt(dt), device="cuda")
+    cuda.attn_prompt(q, k, v, out, _i32((base + np.concatenate([[0], np.cumsum(lens)])).tolist()))
+    torch.cuda.synchronize()
+    check_prompt(q, k, v, out, lens, dt == "f16", base)
+    assert bool((out[:base] == 7.0).all()) and bool((out[T:] == 7.0).all())
+
+
 @pytest.mark.parametrize("dt", ["f32", "f16"])
 def test_prompt_large_scores(cuda, dt):
     """Peaked rows: scores up to some hundreds, growing along the keys, so
