@@ -21,9 +21,14 @@ constexpr int kAtSmem = (2 + kAtStages) * kAtTile + 4 * kAtStage + 3 * 1024;
 // softmax in base 2: exp(s / sqrt(128)) = 2^(s c)
 constexpr float kAtScale2 = 0.08838834764831845f * 1.4426950408889634f;
 // the running maximum a row's weights stand against may lag behind by this
-// many doublings before its sums are rescaled: weights stay below 2^8, far
-// from f16's limit, and most tiles need no pass over the outputs
+// many doublings before its sums are rescaled: most tiles need no pass over
+// the outputs
 constexpr float kAtLag = 8.0f;
+// f16 weights stand against 2^-7 of that maximum: up to 2^15 with the lag,
+// within f16's 65504, and a weight keeps its 11 bits down to 2^-21 of the
+// largest, some bits down to 2^-31. (Against the maximum itself a weight 2^-26
+// of the largest, as many keys beside a sink have it, came out as 0.)
+constexpr float kAtShift = 7.0f, kAtBelow = kAtShift / kAtScale2;
 
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -416,7 +421,7 @@ __device__ __forceinline__ void attn_core(const W w) {
                     #pragma unroll
                     for (int c = 0; c < 128; ++c) s[c] = c < lim ? s[c] : -INFINITY;
                 }
-                if (j == 0) m = row_max(s);
+                if (j == 0) m = row_max(s) - kAtBelow;
                 float sum[4];
                 uint32_t u[32];
                 #pragma unroll 1
@@ -425,10 +430,10 @@ __device__ __forceinline__ void attn_core(const W w) {
                     half_weights(s, weight_offset(m), u, sum);
                     const float mx = row_max(s);
                     // (false for a NaN)
-                    const bool fine = (mx - m) * kAtScale2 <= kAtLag || mx == -INFINITY || !live;
+                    const bool fine = (mx - m) * kAtScale2 <= kAtLag + kAtShift || mx == -INFINITY || !live;
                     if (pass == 1 || __all_sync(0xffffffffu, fine)) break;
                     // (all of O's earlier products are complete: they precede this tile's scores)
-                    const float m1 = fine ? m : max3(m, mx, mx);
+                    const float m1 = fine ? m : max3(m, mx - kAtBelow, mx - kAtBelow);
                     const float f = fine ? 1.f : ex2((m - m1) * kAtScale2);
                     m = m1;
                     l *= f;
