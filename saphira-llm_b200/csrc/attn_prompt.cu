@@ -151,7 +151,8 @@ __device__ __forceinline__ void slow_rows(const PromptParams& p, int h, int star
             #pragma unroll
             for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
             s *= kServeScale;
-            const float mn = fmaxf(m, s), f = mn == -INFINITY ? 1.f : expf(m - mn), e = expf(s - mn);
+            const float mn = max3(m, s, s), f = mn == -INFINITY ? 1.f : expf(m - mn);
+            const float e = mn == -INFINITY ? 0.f : expf(s - mn);
             m = mn;
             l = fmaf(l, f, e);
             o.x = fmaf(e, v.x, o.x * f);

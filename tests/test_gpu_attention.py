@@ -68,3 +68,29 @@ def test_prefix_small_weights(cuda, prefix, own):
     for b in range(2):
         k, v = c.rows(b)[:, 1, 0], c.rows(b, c.v)[:, 1, 0]
         _check_small(q[b, 0], k, v, out[b, 0], torch.full((H,), c.m.lens[b], device="cuda"))
+
+
+# ---------------------------------------------------------------------------
+# values that are no numbers
+# ---------------------------------------------------------------------------
+def test_prompt_unseen_value_beside_a_score_of_minus_infinity(cuda):
+    """A key whose score is -inf has weight 0, whether or not a later token
+    that the row does not see holds a NaN."""
+    import torch
+    n = 150
+    q, k, v = (_rand(s, n, 2, 128, dt=torch.float16) for s in (1, 2, 3))
+    q[:, :, 5] = q[:, :, 5].abs() + 0.1
+    k[0, :, 5] = -math.inf
+    out = [torch.empty(n, 2, 128, device="cuda") for _ in range(2)]
+    cuda.attn_prompt(q, k, v, out[0], _i32([0, n]))
+    v[n - 1] = math.nan
+    cuda.attn_prompt(q, k, v, out[1], _i32([0, n]))
+    torch.cuda.synchronize()
+    rows = torch.arange(1, n - 1, device="cuda")            # row i of the keys 1 .. i
+    for o in out:
+        for h in range(2):
+            want, pv, big, va = attention(q[rows, h].double(), k[1:n - 1, h].double(), v[1:n - 1, h].double(), rows)
+            err = (o[rows, h].double() - want).abs()
+            tol = attention_bound(want, pv, big, va, n, True, False)
+            assert bool((err <= tol).all()), float((err / tol).nan_to_num(math.inf).max())
+    assert bool(torch.isnan(out[1][n - 1]).all())
