@@ -1,6 +1,6 @@
 // attn_mma.cuh -- what the tensor-core attention kernels share: barriers'
 // names, the softmax of one 128-key tile of scores held in tensor memory, and
-// the slow path of a tile whose unseen values are no numbers.
+// the way of values that are no numbers around the products.
 #pragma once
 
 #include "serve.cuh"
@@ -134,6 +134,49 @@ __device__ __forceinline__ float row_max(const float (&s)[128]) {
 __device__ __forceinline__ bool odd_half2(uint32_t u) {
     return (u & 0x7c00u) == 0x7c00u || (u & 0x7c000000u) == 0x7c000000u;
 }
+// ... and the two with zeros in such places
+__device__ __forceinline__ uint32_t clean_half2(uint32_t u) {
+    if ((u & 0x7c00u) == 0x7c00u) u &= 0xffff0000u;
+    if ((u & 0x7c000000u) == 0x7c000000u) u &= 0xffffu;
+    return u;
+}
+
+// What counts as no number: NaN, infinities, and what bf16 would round to one.
+__device__ __forceinline__ bool is_odd(float x) { return !(fabsf(x) < 0x1.ffp127f); }
+
+// A value that is no number would reach every row of a tile through its zero
+// weights. So the products meet zeros in the places of those that not every row
+// sees, and the rows that do see one get it here, when this warp has stored
+// them: a weight is positive, so the sum becomes the value itself. Keys `key`
+// .. end - 1 (few: those that a causal mask takes from some rows of a tile),
+// rows 0 .. rows - 1, E dimensions a lane: v(key), out(row): the lane's first.
+template <int E, class V, class S, class O>
+__device__ __forceinline__ void add_odd(int key, int end, int rows, V v, S seen, O out) {
+    __syncwarp();
+    #pragma unroll 1
+    for (; key < end; ++key) {
+        const auto* const at = v(key);
+        float x[E];
+        bool any = false;
+        #pragma unroll
+        for (int e = 0; e < E; ++e) {
+            x[e] = to_f32(at[e]);
+            any = any || is_odd(x[e]);
+        }
+        if (!any) continue;
+        #pragma unroll 1
+        for (int r = 0; r < rows; ++r) {
+            if (seen(r) <= key) continue;
+            auto* const to = out(r);
+            #pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (is_odd(x[e])) {
+                    const float y = to_f32(to[e]) + (x[e] != x[e] ? x[e] : copysignf(INFINITY, x[e]));
+                    from_f32_to(to + e, y);
+                }
+        }
+    }
+}
 
 // the weights of 64 of a row's scores: two f16 per word, and their sums
 // before the rounding. All exponentials go through the special-function pipe:
@@ -256,15 +299,15 @@ __device__ __forceinline__ void store_rows(uint32_t o_tmem, float f, uint8_t* st
 // tiles are masked. A value row behind the item's keys is zeroed in shared
 // memory before it meets its zero weight. A value among the keys that is no
 // number would leak the same way into rows of the tile that do not see it: the
-// softmax warps look for such values in the masked tiles, and if there are
-// any warps 8-11 recompute the tile's rows one by one.
+// softmax warps put zeros in the places of such values in the masked tiles, and
+// warps 8-11 add them to the rows that see them (add_odd).
 //
 // `W` says what the items are: a Finder (number(w, r): the number of the CTA's
 // r-th item; item(w, x, item): false: there is no item x, but later ones may
 // be), tiles(item, t) (0: no such row tile), keys(item),
 // seen(item, t, row) (not above keys, and least for row 0), live(item, t, row)
-// (a row to be written), a Loader, store(...), slow(...) and gave_up() (a wait
-// ran out).
+// (a row to be written), a Loader, store(...), odd(...) (add_odd for a warp's
+// rows) and gave_up() (a wait ran out).
 //
 // Registers: 512 threads x 128 at launch; 2 x 184 (softmax) + 80 (outputs) +
 // 64 (the issuing warps) = 512 = 4 x 128 after the split.
@@ -382,7 +425,7 @@ __device__ __forceinline__ void attn_core(const W w) {
                 const bool edge = (j + 1) * kAtKeys > every;
                 if (edge) {
                     // this row of the masked tile's values: zeros behind the
-                    // sequence; no number inside it
+                    // sequence, and where no number stands inside it
                     const int x = ring + 2 * j + 1, slot = x % kAtStages;
                     if (!(ok = at_wait_warp(&sh.bar_full[slot], (x / kAtStages) & 1, ab, err))) break;
                     uint8_t* v = sm + (2 + slot) * kAtTile + row * 128;
@@ -401,7 +444,15 @@ __device__ __forceinline__ void attn_core(const W w) {
                             top = __hmax2_nan(top, __hmax2_nan(__hmax2_nan(__habs2(x[0]), __habs2(x[1])),
                                                                __hmax2_nan(__habs2(x[2]), __habs2(x[3]))));
                         }
-                        odd = odd || odd_half2(*reinterpret_cast<const uint32_t*>(&top));
+                        if (odd_half2(*reinterpret_cast<const uint32_t*>(&top))) {
+                            odd = true;
+                            #pragma unroll 1
+                            for (int c = 0; c < 16; ++c) {
+                                uint4* const at = reinterpret_cast<uint4*>(v + (c >> 3) * kAtHalf + 16 * (c & 7));
+                                const uint4 u = *at;
+                                *at = make_uint4(clean_half2(u.x), clean_half2(u.y), clean_half2(u.z), clean_half2(u.w));
+                            }
+                        }
                     }
                     fence_proxy_async_smem();
                 }
@@ -484,6 +535,7 @@ __device__ __forceinline__ void attn_core(const W w) {
         bool ok = true;
         Item it;
         for (int i = 0; ok && next_warp(i, &it); ++i) {
+            bool odd = false;               // (tile 1 meets the zeros that tile 0's warps have put)
             #pragma unroll 1
             for (int t = 0; t < 2; ++t) {
                 if (w.tiles(it, t) == 0) break;
@@ -491,11 +543,10 @@ __device__ __forceinline__ void attn_core(const W w) {
                 ++uses[t];
                 if (!(ok = at_wait_warp(&sh.bar_l[t], par, ab, err) && at_wait_warp(&sh.bar_o[t], par, ab, err))) break;
                 tc_fence_after();
-                if ((sh.odd[t][0] | sh.odd[t][1] | sh.odd[t][2] | sh.odd[t][3]) != 0)
-                    w.slow(it, t, warp & 3);
-                else
-                    w.store(it, t, row, tmem + lanes + 256 + 128 * t, sh.top[t][row], sh.sum[t][row],
-                            stages + (warp & 3) * kAtStage);
+                odd = odd || (sh.odd[t][0] | sh.odd[t][1] | sh.odd[t][2] | sh.odd[t][3]) != 0;
+                w.store(it, t, row, tmem + lanes + 256 + 128 * t, sh.top[t][row], sh.sum[t][row],
+                        stages + (warp & 3) * kAtStage);
+                if (odd) w.odd(it, t, 32 * (warp & 3));
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sh.bar_of[t]);

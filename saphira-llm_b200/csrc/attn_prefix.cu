@@ -161,39 +161,12 @@ __device__ __forceinline__ void store_parts(const PrefixParams& p, const PrefixI
     store_rows(o_tm, 1.f, stage, p.part_o + at * kServeDim, (size_t)parts * kServeDim, n);
 }
 
-// the parts of the row tile at r0, one warp per row, in 32-bit arithmetic
+// value row `key` of an item
 template <class T>
-__device__ __forceinline__ void slow_parts(const PagesDev& pg, const PrefixParams& p, const PrefixItem& it, int r0, int warp) {
-    const int lane = threadIdx.x & 31;
-    for (int x = warp; x < p.plan.rt; x += 4) {
-        const int r = r0 + x;
-        if (r >= it.row_end) return;
-        const float4 q = ld4(static_cast<const T*>(p.q) + row_off(p, it.kvh, r) + 4 * lane);
-        float m = -INFINITY, l = 0.f;
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        const int lim = row_seen(p, it, r);
-        for (int j = 0; j < lim; ++j) {
-            const int id = page_of(pg, p, it.slot, (it.a + j) / pg.page);
-            const size_t at = (size_t)id * p.page_stride +
-                              ((size_t)it.kvh * pg.page + (it.a + j) % pg.page) * kServeDim + 4 * lane;
-            const float4 k = ld4(static_cast<const T*>(p.kp) + at), v = ld4(static_cast<const T*>(p.vp) + at);
-            float s = fmaf(q.x, k.x, fmaf(q.y, k.y, fmaf(q.z, k.z, q.w * k.w)));
-            #pragma unroll
-            for (int y = 16; y > 0; y >>= 1) s += __shfl_xor_sync(0xffffffffu, s, y);
-            s *= kServeScale;
-            const float mn = max3(m, s, s), f = mn == -INFINITY ? 1.f : expf(m - mn);
-            const float e = mn == -INFINITY ? 0.f : expf(s - mn);
-            m = mn;
-            l = fmaf(l, f, e);
-            o.x = fmaf(e, v.x, o.x * f);
-            o.y = fmaf(e, v.y, o.y * f);
-            o.z = fmaf(e, v.z, o.z * f);
-            o.w = fmaf(e, v.w, o.w * f);
-        }
-        const size_t at = part_at(p, it, r);
-        if (lane == 0) p.part_ml[at] = make_float2(m, l);
-        st4(p.part_o + at * kServeDim + 4 * lane, o);
-    }
+__device__ __forceinline__ const T* value_row(const PagesDev& pg, const PrefixParams& p, const PrefixItem& it, int key) {
+    const int id = page_of(pg, p, it.slot, (it.a + key) / pg.page);
+    return static_cast<const T*>(p.vp) + (size_t)id * p.page_stride +
+           ((size_t)it.kvh * pg.page + (it.a + key) % pg.page) * kServeDim;
 }
 
 // ---------------------------------------------------------------------------
@@ -274,8 +247,12 @@ struct PrefixWork {
                                           uint8_t* stage) const {
         store_parts(p, it, it.row0 + t * p.plan.rt, row, o_tm, m, l, stage);
     }
-    __device__ __forceinline__ void slow(const Item& it, int t, int warp) const {
-        slow_parts<__half>(pg, p, it, it.row0 + t * p.plan.rt, warp);
+    __device__ __forceinline__ void odd(const Item& it, int t, int row) const {
+        const int lane4 = 4 * (threadIdx.x & 31), r0 = it.row0 + t * p.plan.rt + row;
+        add_odd<4>(row_seen(p, it, it.row0), it.keys, min(min(32, p.plan.rt - row), it.row_end - r0),
+                   [&](int key) { return value_row<__half>(pg, p, it, key) + lane4; },
+                   [&](int r) { return row_seen(p, it, r0 + r); },
+                   [&](int r) { return p.part_o + part_at(p, it, r0 + r) * kServeDim + lane4; });
     }
 };
 
@@ -342,7 +319,7 @@ struct PrefixWide {
     __device__ __forceinline__ void finish(const Item& it, int row, float m, float l) const {
         p.part_ml[part_at(p, it, it.row0 + row)] = make_float2(m * kServeScale, l);
     }
-    __device__ __forceinline__ void slow(const Item& it, int warp) const { slow_parts<T>(pg, p, it, it.row0, warp); }
+    __device__ __forceinline__ const T* value(const Item& it, int key) const { return value_row<T>(pg, p, it, key); }
 };
 
 template <class KV>

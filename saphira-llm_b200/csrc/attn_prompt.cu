@@ -132,40 +132,6 @@ __device__ __forceinline__ bool find_in_order(const PromptParams& p, int x, int*
 // ---------------------------------------------------------------------------
 constexpr int kPmRows = 2 * kAtRows;
 
-// rows [first, first + 128) of a sequence, one warp per row at a time, in
-// 32-bit arithmetic: the way out for values that are no numbers
-template <class T, class O>
-__device__ __forceinline__ void slow_rows(const PromptParams& p, int h, int start, int len, int first, int warp) {
-    const int lane = threadIdx.x & 31, kvh = h / p.group;
-    const T* K = static_cast<const T*>(p.k) + (size_t)kvh * kServeDim + 4 * lane;
-    const T* V = static_cast<const T*>(p.v) + (size_t)kvh * kServeDim + 4 * lane;
-    for (int r = warp; r < kAtRows; r += 4) {
-        const int i = first + r;
-        if (i >= len) return;
-        const float4 q = ld4(static_cast<const T*>(p.q) + (size_t)(start + i) * p.qs + (size_t)h * kServeDim + 4 * lane);
-        float m = -INFINITY, l = 0.f;
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int j = 0; j <= i; ++j) {
-            const float4 k = ld4(K + (size_t)(start + j) * p.ks), v = ld4(V + (size_t)(start + j) * p.vs);
-            float s = fmaf(q.x, k.x, fmaf(q.y, k.y, fmaf(q.z, k.z, q.w * k.w)));
-            #pragma unroll
-            for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-            s *= kServeScale;
-            const float mn = max3(m, s, s), f = mn == -INFINITY ? 1.f : expf(m - mn);
-            const float e = mn == -INFINITY ? 0.f : expf(s - mn);
-            m = mn;
-            l = fmaf(l, f, e);
-            o.x = fmaf(e, v.x, o.x * f);
-            o.y = fmaf(e, v.y, o.y * f);
-            o.z = fmaf(e, v.z, o.z * f);
-            o.w = fmaf(e, v.w, o.w * f);
-        }
-        const float inv = 1.f / l;
-        st4(static_cast<O*>(p.out) + (size_t)(start + i) * p.os + (size_t)h * kServeDim + 4 * lane,
-            make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
-    }
-}
-
 template <class O>
 struct PromptWork {
     struct Item {
@@ -221,8 +187,14 @@ struct PromptWork {
         store_rows(o_tm, 1.f / l, stage, static_cast<O*>(p.out) + (size_t)(it.start + x0) * p.os + (size_t)it.head * kServeDim,
                    p.os, it.len - x0);
     }
-    __device__ __forceinline__ void slow(const Item& it, int t, int warp) const {
-        slow_rows<__half, O>(p, it.head, it.start, it.len, it.tile * kPmRows + kAtRows * t, warp);
+    __device__ __forceinline__ void odd(const Item& it, int t, int row) const {
+        const int lane = threadIdx.x & 31, x0 = it.tile * kPmRows + kAtRows * t + row;
+        const __half* const v = static_cast<const __half*>(p.v) + (size_t)it.start * p.vs +
+                                (size_t)(it.head / p.group) * kServeDim + 4 * lane;
+        O* const out = static_cast<O*>(p.out) + (size_t)(it.start + x0) * p.os + (size_t)it.head * kServeDim + 4 * lane;
+        add_odd<4>(seen(it, 0, 0), min(x0 + 32, it.len), min(32, it.len - x0),
+                   [&](int key) { return v + (size_t)key * p.vs; }, [&](int r) { return x0 + r + 1; },
+                   [&](int r) { return out + (size_t)r * p.os; });
     }
 };
 
@@ -282,8 +254,9 @@ struct PromptWide {
                        it.len - x0};
     }
     __device__ __forceinline__ void finish(const Item&, int, float, float) const {}
-    __device__ __forceinline__ void slow(const Item& it, int warp) const {
-        slow_rows<float, float>(p, it.head, it.start, it.len, it.tile * kAtRows, warp);
+    // value row `key`
+    __device__ __forceinline__ const float* value(const Item& it, int key) const {
+        return static_cast<const float*>(p.v) + (size_t)(it.start + key) * p.vs + (size_t)(it.head / p.group) * kServeDim;
     }
 };
 

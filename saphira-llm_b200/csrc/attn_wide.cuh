@@ -48,10 +48,10 @@
 // Registers: 768 threads x 80 at launch; 152 (softmax) + 4 x 72 (operands) + 40
 // = 480 = 6 x 80 after the split.
 //
-// Masks as in attn_mma.cuh: rows behind the keys are stored as zeros; a value
-// that is no number, among keys that not every row sees, makes the CTA
-// recompute its rows one by one. A key or value that a row does see and that
-// is no finite number makes that row no number.
+// Masks as in attn_mma.cuh: rows behind the keys are stored as zeros, and so is
+// a value that is no number, among keys that not every row sees; add_odd brings
+// it to the rows that do. A key that a row does see and that is no finite number
+// makes that row no number, a value its dimension.
 #pragma once
 
 #include <type_traits>
@@ -109,7 +109,7 @@ __device__ __forceinline__ float top4(float4 x, float t) {
     return max3(fabsf(x.z), fabsf(x.w), max3(fabsf(x.x), fabsf(x.y), t));
 }
 // no NaN, no infinity, nothing that bf16 would round to one
-__device__ __forceinline__ bool plain(float top) { return top < 0x1.fep127f; }
+__device__ __forceinline__ bool plain(float top) { return !is_odd(top); }
 
 // four elements of a row into its three planes: `at` is the row's 128 bytes of
 // the lane's half in the second plane, `first` in the first, r its number in
@@ -123,6 +123,25 @@ __device__ __forceinline__ void store_planes(uint8_t* at, uint8_t* first, int r,
     *reinterpret_cast<uint2*>(first + in) = make_uint2(a[0], b[0]);
     *reinterpret_cast<uint2*>(at + in) = make_uint2(a[1], b[1]);
     *reinterpret_cast<uint2*>(at + in + plane) = make_uint2(a[2], b[2]);
+}
+
+// ... of which some are not plain: those lie in the first plane alone, or, where
+// they are hidden, nowhere; true: something was hidden
+__device__ __forceinline__ bool store_odd(uint8_t* at, uint8_t* first, int r, int lane, int plane, float4 v, bool hidden) {
+    const float x[4] = {v.x, v.y, v.z, v.w};
+    float y[4];
+    #pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = is_odd(x[e]) ? 0.f : x[e];
+    store_planes(at, first, r, lane, plane, make_float4(y[0], y[1], y[2], y[3]), true);
+    const int in = ((((lane & 15) >> 1) ^ (r & 7)) << 4) + (lane & 1) * 8;
+    bool any = false;
+    #pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (is_odd(x[e])) {
+            any = true;
+            if (!hidden) *reinterpret_cast<uint16_t*>(first + in + 2 * e) = (uint16_t)pack_bf2(x[e], 0.f);
+        }
+    return any && hidden;
 }
 
 // r[i] without an index into registers
@@ -177,7 +196,7 @@ __device__ __forceinline__ void store_cols(uint32_t o_tm, uint32_t t_tm, bool to
 // tile(key, n): the next are keys key, key + 8, .. below n; row(i): the i-th of
 // them); scale(l) (what the outputs are multiplied by), out(item, row) (where the
 // rows from `row` on go), finish(item, row, m, l) (the rest of a row's result),
-// slow(...), gave_up().
+// value(item, key) (a row of values), gave_up().
 template <class W>
 __device__ __forceinline__ void attn_wide_core(const W w) {
     using T = typename W::T;
@@ -434,8 +453,7 @@ __device__ __forceinline__ void attn_wide_core(const W w) {
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.bar_f);
         if (ok && at_wait_warp(&sh.bar_o, 0, ab, err)) {
-            if (*(volatile int*)&sh.odd != 0) w.slow(it, warp);
-            else if (live) w.finish(it, row, m, l);
+            if (live) w.finish(it, row, m, l);
         }
     } else if (warp < 20) {
         // ---------------- operands ----------------
@@ -492,26 +510,32 @@ __device__ __forceinline__ void attn_wide_core(const W w) {
                 bool odd = false;
                 #pragma unroll 1
                 for (int i = 0; i < 8; ++i) {
-                    const float4 x = pick(r, i);
-                    const bool whole = plain(top4(x, 0.f));
-                    store_planes(tile + kWdPlane + (cw + 8 * i) * 128, tile + (cw + 8 * i) * 128, cw, lane, kWdPlane, x, whole);
-                    odd = odd || (!whole && j * kWdKeys + cw + 8 * i >= every);
+                    uint8_t* const first = tile + (cw + 8 * i) * 128;
+                    const bool hidden = is_v && j * kWdKeys + cw + 8 * i >= every;
+                    odd = store_odd(first + kWdPlane, first, cw, lane, kWdPlane, pick(r, i), hidden) || odd;
                 }
-                if (is_v && odd) sh.odd = 1;
+                if (odd) sh.odd = 1;
             }
             arrive(is_v ? &sh.bar_v : &sh.bar_k[j & 1]);
             if (j + 1 < n) load(j + 1);
         }
         // the outputs: sixteen warps, 32 rows x 32 columns each (the query
         // planes' place is free)
-        if (at_wait_warp(&sh.bar_f, 0, ab, err) && at_wait_warp(&sh.bar_o, 0, ab, err) &&
-            *(volatile int*)&sh.odd == 0) {
+        if (at_wait_warp(&sh.bar_f, 0, ab, err) && at_wait_warp(&sh.bar_o, 0, ab, err)) {
             tc_fence_after();
             const int first = 32 * (warp & 3), col = 32 * ((warp - 4) >> 2);
             const uint32_t at = tmem + ((uint32_t)first << 16) + col;
             WideOut to = w.out(it, first);
             to.base += col;
-            if (to.n > 0) store_cols(at + kWdO, at + kWdT, n > kWdFold, sh.f[first + lane], sm + (warp - 4) * kAtStage, to);
+            if (to.n > 0) {
+                store_cols(at + kWdO, at + kWdT, n > kWdFold, sh.f[first + lane], sm + (warp - 4) * kAtStage, to);
+                if (*(volatile int*)&sh.odd != 0) {
+                    const typename W::Item o = sh.item;         // (again, so that it takes no registers till then)
+                    add_odd<1>(w.seen(o, 0), w.keys(o), min(32, to.n), [&](int key) { return w.value(o, key) + col + lane; },
+                               [&](int r) { return w.seen(o, first + r); },
+                               [&](int r) { return to.base + (size_t)r * to.stride + lane; });
+                }
+            }
         }
     } else {
         reg_dealloc<40>();

@@ -93,6 +93,7 @@ __device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
 template <class T> __device__ __forceinline__ T from_f32(float x);
 template <> __device__ __forceinline__ float from_f32<float>(float x) { return x; }
 template <> __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
+template <class T> __device__ __forceinline__ void from_f32_to(T* p, float x) { *p = from_f32<T>(x); }
 
 // four consecutive elements as floats (8- or 16-byte aligned)
 __device__ __forceinline__ float4 ld4(const float* p) { return *reinterpret_cast<const float4*>(p); }

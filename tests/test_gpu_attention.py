@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 
 from serving_ref import attention, attention_bound
-from test_gpu_serving import _dt, _i32, _rand, run_prefix, shared_cache
+from test_gpu_serving import Cache, _dt, _i32, _rand, check_prefix, run_prefix, shared_cache
 
 pytestmark = pytest.mark.gpu
 
@@ -94,3 +94,129 @@ def test_prompt_unseen_value_beside_a_score_of_minus_infinity(cuda):
             tol = attention_bound(want, pv, big, va, n, True, False)
             assert bool((err <= tol).all()), float((err / tol).nan_to_num(math.inf).max())
     assert bool(torch.isnan(out[1][n - 1]).all())
+
+
+ODD = [  # token of the 300, dimension, what stands there
+    (3, 7, math.inf), (70, 7, -math.inf), (70, 9, math.nan), (130, 0, -math.inf), (131, 127, math.inf), (255, 64, math.nan),
+    (256, 31, math.inf), (299, 100, math.nan)]
+
+
+@pytest.mark.parametrize("types", [("f32", "f32"), ("f16", "f16"), ("f16", "f32")])
+@pytest.mark.parametrize("heads", [(2, 1), (3, 3)])
+def test_prompt_odd_values_one_by_one(cuda, types, heads):
+    """Single values that are no numbers, in the tiles that a causal mask cuts
+    and before them: a row that sees one has no number in that dimension, and
+    everything else is bit for bit as with zeros in those places."""
+    import torch
+    n, (H, Hkv) = 300, heads
+    q, k, v = (_rand(s, n + 5, h, 128, dt=_dt(types[0])) for s, h in ((1, H), (2, Hkv), (3, Hkv)))
+    for t, d, _ in ODD:
+        v[5 + t, :, d] = 0.0
+    cu = _i32([0, 5, n + 5])
+    out = [torch.empty(n + 5, H, 128, dtype=_dt(types[1]), device="cuda") for _ in range(2)]
+    cuda.attn_prompt(q, k, v, out[0], cu)
+    for t, d, x in ODD:
+        v[5 + t, :, d] = x
+    cuda.attn_prompt(q, k, v, out[1], cu)
+    torch.cuda.synchronize()
+    mask = torch.zeros(n + 5, H, 128, dtype=torch.bool, device="cuda")
+    for t, d, x in ODD:
+        mask[5 + t:, :, d] = True
+    assert torch.equal(torch.where(mask, 0.0, out[0]), torch.where(mask, 0.0, out[1]))
+    assert not bool(torch.isfinite(out[1][mask]).any())
+    # the first rows that see one hold the value itself; both infinities make no number
+    got = out[1][5:].float()
+    for t, d, x in ODD:
+        if (t, d) == (70, 7):
+            assert bool((got[60:70, :, 7] == math.inf).all()) and bool(torch.isnan(got[70:128, :, 7]).all())
+        elif math.isnan(x):
+            assert bool(torch.isnan(got[t:, :, d]).all())
+        elif t % 128 > 0:               # (a value that all rows of a tile see meets the weights' planes: inf or NaN)
+            assert bool((got[t, :, d] == x).all())
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16"])
+@pytest.mark.parametrize("prefix,owns,page,heads,nq", [(128, [5, 37, 64, 131], 64, (8, 2), 4), (0, [3, 130, 16], 16, (64, 1), 8),
+                                                       (64, [129, 9], 32, (256, 1), 3)])
+def test_prefix_odd_values_one_by_one(cuda, dt, prefix, owns, page, heads, nq):
+    """... in the drafted tokens that only some of a sequence's queries see."""
+    import torch
+    c = shared_cache(cuda, prefix, owns, page, heads, dt)
+    slots = list(range(len(owns)))
+    put = []
+    for s in slots:
+        n = c.m.lens[s]
+        for back, d in ((1, 3), (1, 90), (2, 64), (nq, 5)):
+            if back <= owns[s]:
+                pg = c.m.tables[s][(n - back) // page]
+                put.append((s, back, d, pg, (n - back) % page))
+    for s, back, d, pg, r in put:
+        c.v[pg, :, :, r, d] = 0.0
+    q, a = run_prefix(cuda, c, slots, nq, heads, prefix, "f32")
+    check_prefix(c, q, a, slots, 1)
+    for s, back, d, pg, r in put:
+        c.v[pg, :, :, r, d] = math.nan if d == 90 else math.inf
+    _, b = run_prefix(cuda, c, slots, nq, heads, prefix, "f32")
+    assert c.take_status() == 0
+    mask = torch.zeros_like(a, dtype=torch.bool)
+    for s, back, d, pg, r in put:
+        mask[s, nq - back:, :, d] = True
+    assert torch.equal(torch.where(mask, 0.0, a), torch.where(mask, 0.0, b))
+    assert not bool(torch.isfinite(b[mask]).any())
+    assert bool(torch.isnan(b[:, :, :, 90][mask[:, :, :, 90]]).all())
+
+
+def test_prompt_odd_value_at_the_end_of_a_long_sequence(cuda):
+    """No work grows with the sequence where a value is no number: no bounded
+    wait runs out, and the rows before it are those of the run without it."""
+    import torch
+    n = 1 << 18
+    q, k, v = (_rand(s, n, 1, 128, dt=torch.float16) for s in (1, 2, 3))
+    out = [torch.empty(n, 1, 128, dtype=torch.float16, device="cuda") for _ in range(2)]
+    cuda.attn_prompt(q, k, v, out[0], _i32([0, n]))
+    v[n - 2] = math.inf
+    cuda.attn_prompt(q, k, v, out[1], _i32([0, n]))
+    torch.cuda.synchronize()
+    assert cuda.attn_error() == 0
+    assert torch.equal(out[0][:n - 2], out[1][:n - 2]) and not bool(torch.isfinite(out[1][n - 2:]).any())
+    rows = torch.tensor([0, 127, 128, 5000, n - 3], device="cuda")
+    want, pv, big, va = attention(q[rows, 0].double(), k[:, 0].double(), torch.where(v.isinf(), 0.0, v)[:, 0].double(), rows + 1)
+    assert bool(((out[1][rows, 0].double() - want).abs() <= attention_bound(want, pv, big, va, n, True, True)).all())
+
+
+def test_prefix_odd_value_behind_a_long_context(cuda):
+    """... and in a drafted token behind a long context that is one item a
+    kv head, since the sequences fill the device."""
+    import torch
+    page, n, heads, L, nq = 128, 40, (8, 8), 131072, 4
+    c = Cache(cuda, L // page + 1, n, L // page, page, 1, heads[1], "f16")
+    c.m.tables = [list(range(L // page)) for _ in range(n)]
+    c.m.lens = [L] * n
+    c.m.refs = [n] * (L // page) + [0]
+    c.push()
+    q, a = run_prefix(cuda, c, list(range(n)), nq, heads, 0, "f16", layer=0)
+    last = c.m.tables[0][-1]
+    c.v[last, :, :, page - 1] = math.nan
+    _, b = run_prefix(cuda, c, list(range(n)), nq, heads, 0, "f16", layer=0)
+    assert c.take_status() == 0
+    assert torch.equal(a[:, :3], b[:, :3]) and bool(torch.isnan(b[:, 3]).all())
+    for h in (0, 7):
+        k, v = c.k[:L // page, 0, h].reshape(-1, 128).double(), c.v[:L // page, 0, h].reshape(-1, 128).double()
+        v[-1] = 0.0
+        lim = torch.tensor([L - 3, L - 2, L - 1], device="cuda")
+        want, pv, big, va = attention(q[5, :3, h].double(), k, v, lim)
+        assert bool(((b[5, :3, h].double() - want).abs() <= attention_bound(want, pv, big, va, L, True, True)).all())
+
+
+def test_f32_values_next_to_the_largest(cuda):
+    """f32 counts as infinite from where bf16 would round it to that, 2^128 -
+    2^119, on; below, all 24 bits count."""
+    import torch
+    q, k, v = (_rand(s, 1, 1, 128) for s in (1, 2, 3))
+    big = float.fromhex("0x1.fefffep127")
+    v[0, 0, ::3], v[0, 0, 1::3] = big, float.fromhex("-0x1.fe8002p127")
+    out = torch.empty_like(q)
+    cuda.attn_prompt(q, k, v, out, _i32([0, 1]))
+    torch.cuda.synchronize()
+    # one key: the value itself, its planes and the sum's last bits cut
+    assert bool(((out.double() - v.double()).abs() <= v.double().abs() * 4 * 2.0 ** -24).all())
