@@ -221,18 +221,27 @@ SLLM_CUDA_API int sllm_cuda_i2s_gemm_silu(const uint8_t * w_gate, const uint8_t 
  * (elements; at least n_head * 128, rows 16-byte aligned), so the parts of one
  * Q/K/V array can be passed as they are. Rows of `out` behind the last
  * sequence are not written. A key that a row does not see leaves no trace in
- * it, not even as an infinity or a NaN. q, k and v have type `type`; out is
+ * it, not even as an infinity or a NaN; in a row that does see it, a value that
+ * is no finite number leaves no number in its dimension, a key none in all
+ * (in f16 a score of -inf only has weight 0). q, k and v have type `type`; out is
  * f32 or, from f16, f16. f16 inputs are multiplied on the tensor cores with
- * f32 sums and softmax; the softmax weights are rounded to f16 there.
- * (There is no status word: nothing in an array can be wrong here, and offsets
- * that are stay inside the arrays. sllm_cuda_test_attn_error tells whether a
- * bounded wait ran out.)
+ * f32 sums and softmax; the softmax weights are rounded to f16 there (11 bits
+ * down to 2^-21 of a row's largest, fewer down to 2^-31, 0 below). f32 counts as
+ * infinite from 2^128 - 2^119 on.
+ * The first form has no status word: wrong offsets stay inside the arrays, but
+ * nobody hears of them, nor of a bounded wait that ran out. The second reports
+ * both in `*status`.
  */
 SLLM_CUDA_API int sllm_cuda_attn_prompt(const void * q, size_t q_stride, const void * k, size_t k_stride,
                                         const void * v, size_t v_stride, int32_t type,
                                         const int32_t * cu_seqlens, int32_t n_seq, int32_t n_tokens,
                                         int32_t n_head, int32_t n_head_kv, void * out, size_t out_stride,
                                         int32_t out_type, void * stream);
+SLLM_CUDA_API int sllm_cuda_attn_prompt_checked(const void * q, size_t q_stride, const void * k, size_t k_stride,
+                                                const void * v, size_t v_stride, int32_t type,
+                                                const int32_t * cu_seqlens, int32_t n_seq, int32_t n_tokens,
+                                                int32_t n_head, int32_t n_head_kv, void * out, size_t out_stride,
+                                                int32_t out_type, int32_t * status, void * stream);
 
 /*
  * A paged KV cache in the caller's memory. Pools are

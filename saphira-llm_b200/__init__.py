@@ -124,6 +124,9 @@ def lib():
     L.sllm_cuda_test_tp_ctx_last_run_ms.restype = C.c_float
     pg = C.POINTER(abi.KvPages)
     L.sllm_cuda_attn_prompt.argtypes = [vp, sz, vp, sz, vp, sz, i32, vp, i32, i32, i32, i32, vp, sz, i32, vp]
+    L.sllm_cuda_attn_prompt_checked.argtypes = L.sllm_cuda_attn_prompt.argtypes[:-1] + [vp, vp]
+    L.sllm_cuda_test_attn_wait.argtypes = [C.c_ulonglong]
+    L.sllm_cuda_test_attn_wait.restype = None
     L.sllm_cuda_kv_work_bytes.argtypes = [pg]
     L.sllm_cuda_kv_work_bytes.restype = sz
     L.sllm_cuda_kv_fork.argtypes = [pg, vp, vp, i32, vp, sz, vp, vp]
@@ -293,8 +296,9 @@ def _heads(t, where, name):
     return t.data_ptr(), s0 if n > 1 else h * abi.HEAD_DIM, n, h
 
 
-def attn_prompt(q, k, v, out, cu_seqlens, stream=None):
-    """sllm_cuda_attn_prompt: causal attention over packed whole prompts.
+def attn_prompt(q, k, v, out, cu_seqlens, stream=None, status=None):
+    """sllm_cuda_attn_prompt, or with a status word (int32 [1])
+    sllm_cuda_attn_prompt_checked: causal attention over packed whole prompts.
     q, out [tokens][heads][128], k, v [tokens][kv heads][128], cu_seqlens
     int32 [sequences + 1]."""
     w = "attn_prompt"
@@ -308,10 +312,11 @@ def attn_prompt(q, k, v, out, cu_seqlens, stream=None):
     if not t == _type(k) == _type(v):
         raise ValueError("attn_prompt: q, k and v must have one type")
     cp = _ints(cu_seqlens, 1, w, "cu_seqlens")
+    sp = _ints(status, 1, w, "status")
     if n == 0:
         return
-    rc = lib().sllm_cuda_attn_prompt(qp, qs, kp, ks, vp, vs, t, cp, cu_seqlens.numel() - 1, n, h, hk, op, os_, _type(out),
-                                     _stream(stream))
+    rc = lib().sllm_cuda_attn_prompt_checked(qp, qs, kp, ks, vp, vs, t, cp, cu_seqlens.numel() - 1, n, h, hk, op, os_,
+                                             _type(out), sp, _stream(stream))
     if rc:
         _check(rc, w)
 
@@ -467,6 +472,11 @@ def spec_verify(p, q, draft, n_draft, u_accept, u_draw, tokens, count, status=No
 def attn_error():
     """The tensor-core attention kernels' device error word, likewise."""
     return lib().sllm_cuda_test_attn_error()
+
+
+def set_attn_wait(ns):
+    """The limit of the attention kernels' bounded waits, for tests (0: 2 s)."""
+    lib().sllm_cuda_test_attn_wait(ns)
 
 
 def set_force_fallback(on):

@@ -69,40 +69,48 @@ template <int N>
 __device__ __forceinline__ void reg_alloc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 
 // The bounded waits of umma.cuh, in line: a kernel that splits its registers
-// between its warps cannot call functions.
-__device__ __forceinline__ bool at_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* error) {
-    if (mbar_try_wait(bar, parity)) return true;
+// between its warps cannot call functions. Their limit is the launch's: a test
+// sets one that runs out.
+struct WaitEnd {
+    int* error;                     // the file's error word
+    uint64_t ns;                    // the limit
+    __device__ __forceinline__ uint32_t hint() const { return ns < 65536u ? (uint32_t)ns : 65536u; }
+};
+__device__ __forceinline__ bool at_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, const WaitEnd& end) {
+    if (mbar_try_wait_for(bar, parity, end.hint())) return true;
     const uint64_t t0 = gtimer();
     #pragma unroll 1
-    while (!mbar_try_wait(bar, parity)) {
+    while (!mbar_try_wait_for(bar, parity, end.hint())) {
         if (*abort_flag) return false;
-        if (gtimer() - t0 > kGmWaitNs) {
+        if (gtimer() - t0 > end.ns) {
             *abort_flag = 1;
-            atomicExch(error, GM_TIMEOUT);
+            atomicExch(end.error, GM_TIMEOUT);
             return false;
         }
     }
     return true;
 }
-__device__ __forceinline__ bool at_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* error) {
-    return __all_sync(0xffffffffu, at_wait(bar, parity, abort_flag, error));
+__device__ __forceinline__ bool at_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag, const WaitEnd& end) {
+    return __all_sync(0xffffffffu, at_wait(bar, parity, abort_flag, end));
 }
 // ... with something to try meanwhile
 template <class F>
-__device__ __forceinline__ bool at_wait_while(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* error, F f) {
+__device__ __forceinline__ bool at_wait_while(uint64_t* bar, uint32_t parity, volatile int* abort_flag, const WaitEnd& end,
+                                              F f) {
     const uint64_t t0 = gtimer();
     #pragma unroll 1
     while (!mbar_test(bar, parity)) {
         f();
         if (*abort_flag) return false;
-        if (gtimer() - t0 > kGmWaitNs) {
+        if (gtimer() - t0 > end.ns) {
             *abort_flag = 1;
-            atomicExch(error, GM_TIMEOUT);
+            atomicExch(end.error, GM_TIMEOUT);
             return false;
         }
     }
     return true;
 }
+// what must complete (copies and products in flight), whatever the limit
 __device__ __forceinline__ void at_drain(uint64_t* bar, uint32_t parity) {
     const uint64_t t0 = gtimer();
     #pragma unroll 1
@@ -307,7 +315,8 @@ __device__ __forceinline__ void store_rows(uint32_t o_tmem, float f, uint8_t* st
 // be), tiles(item, t) (0: no such row tile), keys(item),
 // seen(item, t, row) (not above keys, and least for row 0), live(item, t, row)
 // (a row to be written), a Loader, store(...), odd(...) (add_odd for a warp's
-// rows) and gave_up() (a wait ran out).
+// rows), check() (one idle warp of each CTA), wait_ns() and gave_up() (a wait ran
+// out).
 //
 // Registers: 512 threads x 128 at launch; 2 x 184 (softmax) + 80 (outputs) +
 // 64 (the issuing warps) = 512 = 4 x 128 after the split.
@@ -331,7 +340,7 @@ static inline int take_attn_error() {
 
 template <class W>
 __device__ __forceinline__ void attn_core(const W w) {
-    int* const err = &g_attn_error;
+    const WaitEnd err{&g_attn_error, w.wait_ns()};
     using Item = typename W::Item;
     extern __shared__ __align__(1024) uint8_t sm[];
     // [2]: per row tile. q, qf: Q there / free; s: scores there; h, p: the
@@ -351,7 +360,7 @@ __device__ __forceinline__ void attn_core(const W w) {
     Shared& sh = *reinterpret_cast<Shared*>(stages + 4 * kAtStage);
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     if ((smem_u32(sm) & 1023u) != 0) {           // the swizzled layouts need it; the compiler was told to
-        if (threadIdx.x == 0) atomicExch(err, 2);
+        if (threadIdx.x == 0) atomicExch(err.error, 2);
         return;
     }
     if (threadIdx.x == 0) {
@@ -712,6 +721,8 @@ __device__ __forceinline__ void attn_core(const W w) {
                 if (it.last()) break;
                 ++i;
             }
+        } else {
+            w.check();
         }
     }
     tc_fence_before();

@@ -48,6 +48,7 @@ struct PrefixParams {
     size_t page_stride;             // elements
     const int32_t* slots;
     int n, n_q, n_head, n_kv, group, prefix;
+    unsigned long long wait_ns;
     int32_t* status;
     float* part_o;                  // [n_kv][rows][sp + cm][128]
     float2* part_ml;                // [n_kv][rows][sp + cm]
@@ -190,6 +191,8 @@ struct PrefixWork {
             return find_item(w.pg, w.p, x, it);
         }
     };
+    __device__ __forceinline__ unsigned long long wait_ns() const { return p.wait_ns; }
+    __device__ __forceinline__ void check() const {}
     __device__ __forceinline__ void gave_up() const { raise(p.status, SLLM_CUDA_ERR_TIMEOUT); }
     __device__ __forceinline__ int tiles(const Item& it, int t) const {
         return it.row0 + t * p.plan.rt < it.row_end ? (it.keys + kAtKeys - 1) / kAtKeys : 0;
@@ -275,6 +278,8 @@ struct PrefixWide {
     const PagesDev& pg;
     const PrefixParams& p;
 
+    __device__ __forceinline__ unsigned long long wait_ns() const { return p.wait_ns; }
+    __device__ __forceinline__ void check() const {}
     __device__ __forceinline__ void gave_up() const { raise(p.status, SLLM_CUDA_ERR_TIMEOUT); }
     __device__ __forceinline__ bool find(long long x, Item* it) const { return find_item(pg, p, x, it); }
     __device__ __forceinline__ int keys(const Item& it) const { return it.keys; }
@@ -558,6 +563,7 @@ extern "C" int sllm_cuda_attn_prefix(const sllm_cuda_kv_pages* p, int32_t layer,
     a.n = n; a.n_q = n_q; a.n_head = n_head; a.n_kv = p->n_head_kv; a.group = n_head / p->n_head_kv;
     a.prefix = prefix_len;
     a.status = status;
+    a.wait_ns = attn_wait_ns();
     const int sms = current_sms();
     a.plan = make_plan(*p, n, n_q, n_head, prefix_len, sms);
     a.part_o = static_cast<float*>(work);

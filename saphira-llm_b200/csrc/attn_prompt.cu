@@ -24,7 +24,21 @@ struct PromptParams {
     size_t qs, ks, vs, os;          // elements from a token to the next
     const int32_t* cu;
     int n_seq, n_tokens, n_head, group;
+    unsigned long long wait_ns;
+    int32_t* status;
 };
+
+// Offsets that descend or leave the arrays are reported; one warp of each CTA, a
+// share each.
+__device__ __forceinline__ void check_offsets(const PromptParams& p) {
+    if (p.status == nullptr) return;
+    bool bad = false;
+    for (long long s = 32LL * blockIdx.x + (threadIdx.x & 31); s <= p.n_seq; s += 32LL * gridDim.x) {
+        const int at = p.cu[s];
+        bad = bad || at < 0 || at > p.n_tokens || (s < p.n_seq && p.cu[s + 1] < at);
+    }
+    if (bad) raise(p.status, SLLM_CUDA_ERR_ARG);
+}
 
 // sequence s; its bounds are clamped to the arrays, so a wrong cu stays inside
 __device__ __forceinline__ int seq_len(const PromptParams& p, int s, int* start) {
@@ -151,7 +165,9 @@ struct PromptWork {
             return true;
         }
     };
-    __device__ __forceinline__ void gave_up() const {}
+    __device__ __forceinline__ unsigned long long wait_ns() const { return p.wait_ns; }
+    __device__ __forceinline__ void check() const { check_offsets(p); }
+    __device__ __forceinline__ void gave_up() const { raise(p.status, SLLM_CUDA_ERR_TIMEOUT); }
     // key tiles of row tile t: up to its diagonal, or the sequence's end
     __device__ __forceinline__ int tiles(const Item& it, int t) const {
         if (it.tile * kPmRows + kAtRows * t >= it.len) return 0;
@@ -216,7 +232,9 @@ struct PromptWide {
     };
     const PromptParams& p;
 
-    __device__ __forceinline__ void gave_up() const {}
+    __device__ __forceinline__ unsigned long long wait_ns() const { return p.wait_ns; }
+    __device__ __forceinline__ void check() const { check_offsets(p); }
+    __device__ __forceinline__ void gave_up() const { raise(p.status, SLLM_CUDA_ERR_TIMEOUT); }
     // longest first; of more than 32 sequences in their order, which takes no
     // walk over all of them and leaves each SM many items to even out (2048
     // prompts of 32 to 64 tokens, 20 heads: 4.9 ms longest first, 2.9 ms in order;
@@ -313,6 +331,14 @@ extern "C" int sllm_cuda_attn_prompt(const void* q, size_t q_stride, const void*
                                      size_t v_stride, int32_t type, const int32_t* cu_seqlens, int32_t n_seq,
                                      int32_t n_tokens, int32_t n_head, int32_t n_head_kv, void* out,
                                      size_t out_stride, int32_t out_type, void* stream) {
+    return sllm_cuda_attn_prompt_checked(q, q_stride, k, k_stride, v, v_stride, type, cu_seqlens, n_seq, n_tokens, n_head,
+                                         n_head_kv, out, out_stride, out_type, nullptr, stream);
+}
+
+extern "C" int sllm_cuda_attn_prompt_checked(const void* q, size_t q_stride, const void* k, size_t k_stride, const void* v,
+                                             size_t v_stride, int32_t type, const int32_t* cu_seqlens, int32_t n_seq,
+                                             int32_t n_tokens, int32_t n_head, int32_t n_head_kv, void* out,
+                                             size_t out_stride, int32_t out_type, int32_t* status, void* stream) {
     if (q == nullptr || k == nullptr || v == nullptr || cu_seqlens == nullptr || out == nullptr)
         return fail(SLLM_CUDA_ERR_ARG, "attn_prompt: a NULL array");
     if ((type != SLLM_CUDA_KV_F32 && type != SLLM_CUDA_KV_F16) ||
@@ -330,9 +356,10 @@ extern "C" int sllm_cuda_attn_prompt(const void* q, size_t q_stride, const void*
         !aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out))
         return fail(SLLM_CUDA_ERR_ARG, "attn_prompt: token strides %zu %zu %zu %zu (at least the heads, rows and arrays "
                     "16-byte aligned)", q_stride, k_stride, v_stride, out_stride);
-    const void* ptr[] = {q, k, v, cu_seqlens, out};
-    const char* name[] = {"q", "k", "v", "cu_seqlens", "out"};
-    for (int i = 0; i < 5; ++i) {
+    const void* ptr[] = {q, k, v, cu_seqlens, out, status};
+    const char* name[] = {"q", "k", "v", "cu_seqlens", "out", "status"};
+    for (int i = 0; i < 6; ++i) {
+        if (ptr[i] == nullptr) continue;
         const int rc = need_device(ptr[i], "attn_prompt", name[i]);
         if (rc != SLLM_CUDA_OK) return rc;
     }
@@ -341,6 +368,8 @@ extern "C" int sllm_cuda_attn_prompt(const void* q, size_t q_stride, const void*
     p.q = q; p.k = k; p.v = v; p.out = out;
     p.qs = q_stride; p.ks = k_stride; p.vs = v_stride; p.os = out_stride;
     p.cu = cu_seqlens;
+    p.wait_ns = attn_wait_ns();
+    p.status = status;
     p.n_seq = n_seq; p.n_tokens = n_tokens; p.n_head = n_head; p.group = n_head / n_head_kv;
     const cudaStream_t st = (cudaStream_t)stream;
     const cudaError_t e = type == SLLM_CUDA_KV_F32 ? launch_wide(p, st)

@@ -196,11 +196,12 @@ __device__ __forceinline__ void store_cols(uint32_t o_tm, uint32_t t_tm, bool to
 // tile(key, n): the next are keys key, key + 8, .. below n; row(i): the i-th of
 // them); scale(l) (what the outputs are multiplied by), out(item, row) (where the
 // rows from `row` on go), finish(item, row, m, l) (the rest of a row's result),
-// value(item, key) (a row of values), gave_up().
+// value(item, key) (a row of values), check() (one warp of each CTA), wait_ns(),
+// gave_up().
 template <class W>
 __device__ __forceinline__ void attn_wide_core(const W w) {
     using T = typename W::T;
-    int* const err = &g_attn_error;
+    const WaitEnd err{&g_attn_error, w.wait_ns()};
     extern __shared__ __align__(1024) uint8_t sm[];
     struct Shared {
         // q: split; q1: the first plane in tensor memory; k, v: tile split; vf:
@@ -217,7 +218,7 @@ __device__ __forceinline__ void attn_wide_core(const W w) {
     Shared& sh = *reinterpret_cast<Shared*>(sm + kWdEnd);
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     if ((smem_u32(sm) & 1023u) != 0) {
-        if (threadIdx.x == 0) atomicExch(err, 2);
+        if (threadIdx.x == 0) atomicExch(err.error, 2);
         return;
     }
     if (warp == 0) {                    // (by every warp it took twice as long)
@@ -228,6 +229,7 @@ __device__ __forceinline__ void attn_wide_core(const W w) {
             sh.none = !found;
         }
     }
+    if (warp == 23) w.check();
     if (threadIdx.x == 32) {
         mbar_init(&sh.bar_q, 20);
         mbar_init(&sh.bar_q1, 4);

@@ -622,6 +622,12 @@ cudaError_t launch_copies(const sllm_cuda_kv_pages& p, long long most, void* wor
 
 }  // namespace
 
+static std::atomic<unsigned long long> g_attn_wait_ns{0};
+unsigned long long attn_wait_ns() {
+    const unsigned long long ns = g_attn_wait_ns.load(std::memory_order_relaxed);
+    return ns != 0 ? ns : 2000000000ull;
+}
+
 int current_sms() {
     int dev = 0;
     cudaGetDevice(&dev);
@@ -673,6 +679,8 @@ extern "C" int sllm_cuda_test_attn_error(void) {
     const int a = take_prompt_error(), b = take_prefix_error();
     return a != 0 ? a : b;
 }
+
+extern "C" void sllm_cuda_test_attn_wait(unsigned long long ns) { g_attn_wait_ns.store(ns, std::memory_order_relaxed); }
 
 extern "C" size_t sllm_cuda_kv_work_bytes(const sllm_cuda_kv_pages* p) {
     if (check_pages(p, "kv_work_bytes") != SLLM_CUDA_OK) return 0;

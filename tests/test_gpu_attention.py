@@ -220,3 +220,55 @@ def test_f32_values_next_to_the_largest(cuda):
     torch.cuda.synchronize()
     # one key: the value itself, its planes and the sum's last bits cut
     assert bool(((out.double() - v.double()).abs() <= v.double().abs() * 4 * 2.0 ** -24).all())
+
+
+# ---------------------------------------------------------------------------
+# what is reported
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dt", ["f32", "f16"])
+def test_prompt_reports_wrong_offsets(cuda, dt):
+    """Offsets that descend or leave the arrays, in *status; right ones, empty
+    sequences and a last one below the array's end among them, leave it alone."""
+    import torch
+    n = 100
+    q, k, v = (_rand(s, n, 2, 128, dt=_dt(dt)) for s in (1, 2, 3))
+    out, status = torch.empty_like(q), _i32([0])
+    for cu in ([0, 100], [0, 0, 40, 40, 99], [7, 100], [0] * 700 + [100] * 700):
+        cuda.attn_prompt(q, k, v, out, _i32(cu), status=status)
+        assert status.item() == 0, cu
+    for cu in ([0, 101], [-1, 100], [60, 20], [0, 100, 50, 100], [0] * 700 + [100] * 700 + [99], [2 ** 31 - 1, -2 ** 31]):
+        status.zero_()
+        cuda.attn_prompt(q, k, v, out, _i32(cu), status=status)
+        assert status.item() == -1, cu
+    with pytest.raises(cuda.SllmCudaError, match="status"):
+        cuda.attn_prompt(q, k, v, out, _i32([0, 100]), status=torch.zeros(1, dtype=torch.int32))
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16"])
+def test_a_wait_that_runs_out_is_reported(cuda, dt):
+    """With a limit of 1 ns every real wait runs out: the kernels end, *status
+    and the error word say so, and the next calls are as good as ever."""
+    import torch
+    n = 1500
+    q, k, v = (_rand(s, n, 4, 128, dt=_dt(dt)) for s in (1, 2, 3))
+    cu, status, ref, out = _i32([0, 300, n]), _i32([0]), torch.empty_like(q), torch.empty_like(q)
+    c = shared_cache(cuda, 1024, [300] * 3, 16, (20, 5), dt)
+    cuda.attn_prompt(q, k, v, ref, cu, status=status)
+    _, a = run_prefix(cuda, c, [0, 1, 2], 2, (20, 5), 1024, dt)
+    assert status.item() == 0 and c.take_status() == 0 and cuda.attn_error() == 0
+    cuda.set_attn_wait(1)
+    try:
+        cuda.attn_prompt(q, k, v, out, cu, status=status)
+        run_prefix(cuda, c, [0, 1, 2], 2, (20, 5), 1024, dt)
+        cuda.attn_prompt(q, k, v, out, cu)              # nobody asks
+        torch.cuda.synchronize()
+    finally:
+        cuda.set_attn_wait(0)
+    assert status.item() == -61 and c.take_status() == -61
+    assert cuda.attn_error() != 0
+    cuda.attn_error()                                   # (one word per file)
+    status.zero_()
+    cuda.attn_prompt(q, k, v, out, cu, status=status)
+    _, b = run_prefix(cuda, c, [0, 1, 2], 2, (20, 5), 1024, dt)
+    assert status.item() == 0 and c.take_status() == 0 and cuda.attn_error() == 0
+    assert torch.equal(out, ref) and torch.equal(a, b)
