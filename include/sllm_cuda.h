@@ -347,7 +347,9 @@ SLLM_CUDA_API int sllm_cuda_rope_table(int32_t n_ctx, float rope_freq_base, floa
  * [n][n_q][n_head][128], q of the cache's type, out f32 or, from an f16
  * cache, f16. A sequence whose slot, length or table is wrong sets
  * SLLM_CUDA_ERR_ARG in *status and its rows of out mean nothing (all rows,
- * where the prefix's pages are wrong). n <= 4096, n_q <= 16.
+ * where the prefix's pages are wrong). n <= 4096, n_q <= 16. A workspace of
+ * work_bytes(n, n_q, n_head, prefix_len) serves every call over this cache with
+ * that n_head and no more sequences, query tokens and prefix.
  */
 SLLM_CUDA_API size_t sllm_cuda_attn_prefix_work_bytes(const sllm_cuda_kv_pages * p, int32_t n, int32_t n_q,
                                                       int32_t n_head, int32_t prefix_len);

@@ -24,6 +24,8 @@
 // lengths, it put two dependent reads before the first item (27.6 us against
 // 18.0 us for the 16 sequences).
 
+#include <algorithm>
+
 #include "attn_mma.cuh"
 #include "attn_wide.cuh"
 
@@ -412,8 +414,15 @@ attn_prefix_join_kernel(const __grid_constant__ PagesDev pg, const __grid_consta
 // tiles a split) 16.7 and 21.6 us, 16384 (nine) 26.2 and 33.2 us, 20480 (twelve)
 // 30.5 and 38.8 us; 32 sequences (256 items of their own), prefix 4096 (four)
 // 26.7 and 28.8 us, 12288 (eleven) 42.2 and 36.9 us.
+// No more splits than eight rounds of the SMs take (f32, with half the rows an
+// item: sixteen), if a split has at most 32 tiles then: that bounds the
+// workspace (work_parts). Shapes that would take more otherwise (one in 30 of
+// those drawn at random), f16, 8 query tokens, with the limit and without: 107
+// sequences, prefix 47872, 32 heads of 8 (12 and 13 splits) 645 and 653 us; 203,
+// 19328 (5 and 7) 519 and 543 us; 59, 35072, 64 heads of 8 (9 and 11) 517 and 508 us.
 // A sequence's own keys: chunks of as many tiles, at least two; no more than
 // two items per SM over all sequences, and no more than 64 chunks.
+int most_rounds(int per) { return per == 2 ? 8 : 16; }
 Plan make_plan(const sllm_cuda_kv_pages& p, int n, int n_q, int n_head, int prefix, int sms) {
     const int group = n_head / p.n_head_kv, rows = n * n_q * group;
     const bool mma = p.kv_type == SLLM_CUDA_KV_F16 && group <= kAtRows;
@@ -433,7 +442,9 @@ Plan make_plan(const sllm_cuda_kv_pages& p, int n, int n_q, int n_head, int pref
         pl.sp = (pl.ptiles + pl.ct - 1) / pl.ct;
     } else {
         long long best = 0;
-        for (int s = (pl.ptiles + 31) / 32; s <= pl.ptiles && (s <= 32 || pl.sp == 0); ++s) {
+        const int least = (pl.ptiles + 31) / 32;
+        const long long most = std::max<long long>((long long)most_rounds(pl.per) * sms / base, least);
+        for (int s = least; s <= pl.ptiles && s <= most && (s <= 32 || pl.sp == 0); ++s) {
             const long long tiles = (pl.ptiles + s - 1) / s, cost = ((base * s + sms - 1) / sms) * (tiles + 3);
             if (pl.sp == 0 || cost < best) {
                 best = cost;
@@ -451,6 +462,21 @@ Plan make_plan(const sllm_cuda_kv_pages& p, int n, int n_q, int n_head, int pref
 size_t part_count(const Plan& pl, int n, int n_q, int n_head) {
     return (size_t)n * n_q * n_head * (pl.sp + pl.cm);
 }
+
+// part_count of this call and of every one with no more sequences, query tokens
+// and prefix, by a form that rises with each (the splits themselves do not: a
+// second tile in a split halves their number). R rows, `item` of a kv head in an
+// item at most. Splits of the prefix: its tiles at most; in one round of the SMs
+// room / base and one more, so R + sms * item; else as many as tiles of 32, or
+// most_rounds' worth. Chunks: 64, or 2 sms / own and one more.
+size_t work_parts(const Plan& pl, int n, int n_q, int n_head, int group, int sms) {
+    const size_t R = (size_t)n * n_q * n_head, item = (size_t)pl.rt * pl.per;
+    const size_t rows = std::min(item, (size_t)n * n_q * group), own = std::min(item, (size_t)n_q * group);
+    const size_t splits = std::min(R * pl.ptiles, std::max({R * ((pl.ptiles + 31) / 32), R + sms * rows, most_rounds(pl.per) * sms * rows}));
+    return splits + std::min(64 * R, R + 2 * sms * own);
+}
+
+size_t part_bytes(size_t parts) { return parts * (kServeDim * sizeof(float) + sizeof(float2)) + 16; }
 
 bool encode_q(CUtensorMap* tm, const void* base, int tokens, int n_kv, int group) {
     PFN_cuTensorMapEncodeTiled_v12000 enc = tensor_map_encoder();
@@ -528,8 +554,8 @@ int sllm::take_prefix_error() { return take_attn_error(); }
 extern "C" size_t sllm_cuda_attn_prefix_work_bytes(const sllm_cuda_kv_pages* p, int32_t n, int32_t n_q, int32_t n_head,
                                                    int32_t prefix_len) {
     if (check_shape(p, n, n_q, n_head, prefix_len, "attn_prefix_work_bytes") != SLLM_CUDA_OK) return 0;
-    const size_t parts = part_count(make_plan(*p, n, n_q, n_head, prefix_len, current_sms()), n, n_q, n_head);
-    return parts * (kServeDim * sizeof(float) + sizeof(float2)) + 16;
+    const int sms = current_sms();
+    return part_bytes(work_parts(make_plan(*p, n, n_q, n_head, prefix_len, sms), n, n_q, n_head, n_head / p->n_head_kv, sms));
 }
 
 extern "C" int sllm_cuda_attn_prefix(const sllm_cuda_kv_pages* p, int32_t layer, const void* q, const int32_t* slots,
@@ -543,10 +569,12 @@ extern "C" int sllm_cuda_attn_prefix(const sllm_cuda_kv_pages* p, int32_t layer,
     if ((out_type != SLLM_CUDA_KV_F32 && out_type != SLLM_CUDA_KV_F16) ||
         (p->kv_type == SLLM_CUDA_KV_F32 && out_type == SLLM_CUDA_KV_F16))
         return fail(SLLM_CUDA_ERR_ARG, "attn_prefix: output type %d (f32, or f16 from an f16 cache)", out_type);
-    if (!aligned16(q) || !aligned16(out) || !aligned16(work) ||
-        work_bytes < sllm_cuda_attn_prefix_work_bytes(p, n, n_q, n_head, prefix_len))
+    const int sms = current_sms();
+    const Plan plan = make_plan(*p, n, n_q, n_head, prefix_len, sms);
+    const size_t parts = part_count(plan, n, n_q, n_head);
+    if (!aligned16(q) || !aligned16(out) || !aligned16(work) || work_bytes < part_bytes(parts))
         return fail(SLLM_CUDA_ERR_ARG, "attn_prefix: workspace of %zu bytes (%zu needed), arrays 16-byte aligned",
-                    work_bytes, sllm_cuda_attn_prefix_work_bytes(p, n, n_q, n_head, prefix_len));
+                    work_bytes, part_bytes(parts));
     const void* ptr[] = {p->k, p->v, p->tables, p->lens, q, slots, out, work, status};
     const char* name[] = {"k", "v", "tables", "lens", "q", "slots", "out", "work", "status"};
     for (int i = 0; i < 9; ++i)
@@ -564,10 +592,9 @@ extern "C" int sllm_cuda_attn_prefix(const sllm_cuda_kv_pages* p, int32_t layer,
     a.prefix = prefix_len;
     a.status = status;
     a.wait_ns = attn_wait_ns();
-    const int sms = current_sms();
-    a.plan = make_plan(*p, n, n_q, n_head, prefix_len, sms);
+    a.plan = plan;
     a.part_o = static_cast<float*>(work);
-    a.part_ml = reinterpret_cast<float2*>(a.part_o + part_count(a.plan, n, n_q, n_head) * kServeDim);
+    a.part_ml = reinterpret_cast<float2*>(a.part_o + parts * kServeDim);
     // many items per SM: each CTA takes the next one when it is free, for one
     // more launch, to clear the counter; few: they are dealt. Taken and dealt,
     // f16, 32 heads of 8, own lengths of 1 to 4096 at random: 16 sequences (256
@@ -576,7 +603,7 @@ extern "C" int sllm_cuda_attn_prefix(const sllm_cuda_kv_pages* p, int32_t layer,
     // 2048 149 and 130 us. (The lengths are the device's, so the rule is on the
     // number alone.)
     if (item_numbers(a) > 3LL * sms)
-        a.plan.next = reinterpret_cast<int*>(a.part_ml + part_count(a.plan, n, n_q, n_head));
+        a.plan.next = reinterpret_cast<int*>(a.part_ml + parts);
     if (item_numbers(a) > 0x3fffffffLL) return fail(SLLM_CUDA_ERR_TOO_LARGE, "attn_prefix: %d sequences", n);
     const PagesDev pg = pages_dev(*p);
     const cudaStream_t st = (cudaStream_t)stream;

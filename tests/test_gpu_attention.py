@@ -272,3 +272,23 @@ def test_a_wait_that_runs_out_is_reported(cuda, dt):
     _, b = run_prefix(cuda, c, [0, 1, 2], 2, (20, 5), 1024, dt)
     assert status.item() == 0 and c.take_status() == 0 and cuda.attn_error() == 0
     assert torch.equal(out, ref) and torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16"])
+def test_prefix_workspace_of_the_largest_call_serves_the_smaller(cuda, dt):
+    """Sequences end one after the other, and the prefix gets shorter, in one
+    workspace of the first call's size; what lies behind it stays."""
+    import torch
+    heads, prefix, n = (8, 1), 4096, 21
+    c = shared_cache(cuda, prefix, [1 + 9 * i for i in range(n)], 16, heads, dt)
+    size = c.p.attn_prefix_work_bytes(n, 2, heads[0], prefix)
+    work = torch.full((size + 4096,), 77, dtype=torch.uint8, device="cuda")
+    for m, nq, pre in ((21, 2, 4096), (20, 2, 4096), (20, 1, 4096), (13, 2, 2048), (7, 1, 1792), (3, 2, 16), (1, 1, 0)):
+        q = _rand(m, m, nq, heads[0], 128, dt=_dt(dt), scale=1.3)
+        out = torch.empty(m, nq, heads[0], 128, device="cuda")
+        slots = list(range(n - m, n))
+        c.p.attn_prefix(1, q, out, _i32(slots), pre, work[:size], c.status)
+        torch.cuda.synchronize()
+        assert c.take_status() == 0
+        check_prefix(c, q, out, slots, 1, skip=range(1, m - 1))
+    assert bool((work[size:] == 77).all())

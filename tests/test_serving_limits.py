@@ -1,6 +1,7 @@
 """The attention and cache entry points without a device: refusals of the
 checked prompt call, and what the workspace sizes promise."""
 import ctypes as C
+import random
 
 import pytest
 
@@ -37,3 +38,55 @@ def test_binding_checks_the_status_word(pkg):
     for status in (torch.zeros(1), torch.zeros(0, dtype=torch.int32), torch.zeros(1, dtype=torch.int64)):
         with pytest.raises(ValueError, match="status"):
             pkg.attn_prompt(w, w, w, w, cu, status=status)
+
+
+HEADS = [(8, 1), (64, 8), (20, 5), (4, 4), (7, 1), (256, 1)]
+
+
+def _wide(abi, kv, f16, page=16):
+    return cache(abi, n_head_kv=kv, kv_type=1 if f16 else 0, page_size=page, table_width=1 << 16, n_slots=4096)
+
+
+def _bytes(L, p, n, nq, h, prefix):
+    return L.sllm_cuda_attn_prefix_work_bytes(C.byref(p), n, nq, h, prefix)
+
+
+@pytest.mark.parametrize("heads", HEADS)
+@pytest.mark.parametrize("f16", [False, True])
+def test_prefix_workspace_never_falls(pkg, L, heads, f16):
+    """More sequences, query tokens or prefix never need less: a buffer of the
+    largest call's size serves the smaller ones."""
+    h, kv = heads
+    p = _wide(pkg.abi, kv, f16)
+    for nq in (1, 3, 16):
+        for prefix in (0, 16, 1792, 2304, 16384, 262144):
+            sizes = [_bytes(L, p, n, nq, h, prefix) for n in list(range(1, 70)) + [100, 128, 129, 500, 1000, 4096]]
+            assert all(sizes) and sizes == sorted(sizes)
+    for n, nq in ((1, 1), (16, 1), (21, 2), (300, 4)):
+        sizes = [_bytes(L, p, n, nq, h, 16 * x) for x in list(range(0, 400)) + [1000, 1024, 2000, 4096, 10000, 65536]]
+        assert all(sizes) and sizes == sorted(sizes)
+        sizes = [_bytes(L, p, n, x, h, 4096) for x in range(1, 17)]
+        assert all(sizes) and sizes == sorted(sizes)
+
+
+def test_prefix_workspace_of_the_largest_call_is_taken(cuda_absent, L, pkg):
+    """... by the call itself, which asks for what its own splits need. Without
+    a device it stops behind that check."""
+    rng = random.Random(4)
+    for _ in range(4000):
+        h, kv = rng.choice(HEADS)
+        f16 = rng.random() < 0.7
+        p = _wide(pkg.abi, kv, f16)
+        most = [int(2 ** rng.uniform(0, 12)), rng.randint(1, 16), 16 * int(2 ** rng.uniform(0, 15))]
+        size = _bytes(L, p, most[0], most[1], h, most[2])
+        for _ in range(3):
+            n, nq, prefix = rng.randint(1, most[0]), rng.randint(1, most[1]), 16 * rng.randint(0, most[2] // 16)
+            rc = L.sllm_cuda_attn_prefix(C.byref(p), 0, A, A, n, nq, h, prefix, A, f16, A, size, None, None)
+            assert rc == -4, (h, kv, f16, most, n, nq, prefix, L.sllm_cuda_last_error())
+
+
+def test_prefix_workspace_is_no_waste(L, pkg):
+    """A bound far above the need would be one too: 64 sequences of four query
+    tokens behind 32768, 64 heads of 8, need ten parts a row."""
+    p = _wide(pkg.abi, 8, True)
+    assert _bytes(L, p, 64, 4, 64, 32768) <= 22 * 64 * 4 * 64 * 520
