@@ -292,3 +292,44 @@ def test_prefix_workspace_of_the_largest_call_serves_the_smaller(cuda, dt):
         assert c.take_status() == 0
         check_prefix(c, q, out, slots, 1, skip=range(1, m - 1))
     assert bool((work[size:] == 77).all())
+
+
+# ---------------------------------------------------------------------------
+# f32 inputs
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("n", [1, 17, 64, 129, 700, 4100])
+def test_prompt_f32_is_as_good_as_32_bits(cuda, n):
+    import torch
+    from precision_ref import as_good_as_32_bits
+    q, k, v = (_rand(s, n + 3, h, 128, scale=1.3) for s, h in ((1, 4), (2, 2), (3, 2)))
+    out = torch.empty_like(q)
+    cuda.attn_prompt(q, k, v, out, _i32([0, 3, n + 3]))
+    torch.cuda.synchronize()
+    for h in range(4):
+        x = q[3:, h], k[3:, h // 2], v[3:, h // 2], torch.arange(1, n + 1, device="cuda")
+        if n == 1:                              # one key: the value, its bits cut at most four times
+            assert bool(((out[3:, h] - x[2]).abs() <= x[2].abs() * 2.0 ** -22).all())
+            continue
+        big, rms = as_good_as_32_bits(out[3:, h], *x)
+        assert big <= 3 and rms <= 3, (h, big, rms)
+
+
+@pytest.mark.parametrize("prefix,owns,nq,heads", [(0, [64, 9], 1, (20, 5)), (0, [4100], 2, (8, 1)), (256, [40, 130], 4, (8, 2)),
+                                                  (4096, [700, 33, 5], 1, (8, 1)), (64, [600], 1, (256, 1))])
+def test_prefix_f32_is_as_good_as_32_bits(cuda, prefix, owns, nq, heads):
+    import torch
+    from precision_ref import as_good_as_32_bits
+    c = shared_cache(cuda, prefix, owns, 16, heads, "f32")
+    slots = list(range(len(owns)))
+    q, out = run_prefix(cuda, c, slots, nq, heads, prefix, "f32")
+    assert c.take_status() == 0
+    group = heads[0] // heads[1]
+    for b in slots:
+        L = c.m.lens[b]
+        for g in range(heads[1]):
+            rows = slice(g * group, (g + 1) * group)
+            lim = torch.tensor([L - nq + 1 + j for j in range(nq)], device="cuda")
+            lim = lim[:, None].expand(nq, group).reshape(-1)
+            x = (q[b, :, rows].reshape(-1, 128), c.rows(b)[:, 1, g], c.rows(b, c.v)[:, 1, g], lim)
+            big, rms = as_good_as_32_bits(out[b, :, rows].reshape(-1, 128), *x)
+            assert big <= 3 and rms <= 3, (b, g, big, rms)

@@ -90,3 +90,24 @@ def test_prefix_workspace_is_no_waste(L, pkg):
     tokens behind 32768, 64 heads of 8, need ten parts a row."""
     p = _wide(pkg.abi, 8, True)
     assert _bytes(L, p, 64, 4, 64, 32768) <= 22 * 64 * 4 * 64 * 520
+
+
+# ---------------------------------------------------------------------------
+# the measure that the f32 attention core is held against
+# ---------------------------------------------------------------------------
+def _rows(n, rows, seed):
+    import torch
+    g = torch.Generator().manual_seed(seed)
+    q, k, v = (torch.randn(m, 128, generator=g) * 1.3 for m in (rows, n, n))
+    return q, k, v, torch.linspace(max(1, n - 4 * rows), n, rows).long()
+
+
+@pytest.mark.parametrize("n", [64, 700, 4100])
+def test_six_partial_products_are_as_good_as_32_bits(n):
+    from precision_ref import PAIRS, as_good_as_32_bits, attention_planes
+    x = _rows(n, 48, n)
+    assert max(as_good_as_32_bits(attention_planes(*x), *x)) <= 3
+    # and with any of them left out they are not
+    for lost in PAIRS:
+        out = attention_planes(*x, [p for p in PAIRS if p != lost])
+        assert min(as_good_as_32_bits(out, *x)) > 3, lost
