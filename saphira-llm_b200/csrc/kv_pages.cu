@@ -228,8 +228,9 @@ kv_release_kernel(const PagesDev p, const int32_t* slots, const int32_t* new_len
 // on. A last page that is partly filled, will be written and has other
 // owners is replaced by a copy: slot by slot in the call's order, so of r
 // owners named in one call that are all its owners the last keeps the page.
-// One CTA: the call's slots are few, and the free pages are found by one pass
-// over the counts, 16 per thread in flight.
+// One CTA: the call's slots are few as a rule, and the free pages are found by
+// one pass over the counts, 16 per thread in flight. A page's writers are counted
+// in the page's own words of the workspace.
 // ---------------------------------------------------------------------------
 __global__ void __launch_bounds__(kResThreads)
 kv_reserve_kernel(const PagesDev p, const int32_t* slots, const int32_t* n_new, int n, void* work, int32_t* status) {
@@ -247,10 +248,13 @@ kv_reserve_kernel(const PagesDev p, const int32_t* slots, const int32_t* n_new, 
         if (s >= 0 && s < p.n_slots) w.mark[s] = 0;
     }
     __syncthreads();
-    int total = 0;
+    // what each slot asks for: its new pages, and its last page if it writes there
+    int fresh = 0, last = -1, owners = 0;       // of this thread's last slot
+    bool shared = false;
     for (int base = 0; base < n; base += kResThreads) {
         const int i = base + t;
-        int fresh = 0, last = -1, owners = 0;
+        fresh = owners = 0;
+        last = -1;
         if (i < n) {
             const int s = slots[i], nn = n_new[i];
             int e = 0;
@@ -274,14 +278,41 @@ kv_reserve_kernel(const PagesDev p, const int32_t* slots, const int32_t* n_new, 
                 }
             }
             if (e != 0) atomicCAS(&err, 0, e);
+            if (owners > 1) {       // x: how many slots of this call write to the page, y: the last of them
+                shared = true;
+                w.pairs[last].x = 0;
+                w.pairs[last].y = -1;
+            }
             w.slot_page[i] = last;
+            w.slot_need[i] = fresh;
         }
+    }
+    const bool one = n <= kResThreads;          // this thread's slot is still at hand
+    if (__syncthreads_or(shared)) {
+        for (int i = t; i < n; i += kResThreads) {
+            const int page = one ? last : w.slot_page[i];
+            if (page >= 0 && (one ? owners : p.refs[page]) > 1) {
+                atomicAdd(&w.pairs[page].x, 1);
+                atomicMax(&w.pairs[page].y, i);
+            }
+        }
+        shared = true;
         __syncthreads();
+    }
+    int total = 0;
+    for (int base = 0; base < n; base += kResThreads) {
+        const int i = base + t;
+        if (!one) {
+            last = i < n ? w.slot_page[i] : -1;
+            fresh = i < n ? w.slot_need[i] : 0;
+            owners = shared && last >= 0 ? p.refs[last] : 0;
+        }
+        // where all owners write, the last of them keeps the page
         int cow = 0;
         if (owners > 1) {
-            int before = 0;         // earlier slots of this call that write to the same page
-            for (int j = 0; j < i; ++j) before += w.slot_page[j] == last ? 1 : 0;
-            cow = owners - before > 1 ? 1 : 0;
+            const int writers = w.pairs[last].x;
+            cow = writers == owners && w.pairs[last].y == i ? 0 : 1;
+            if (writers > owners) atomicCAS(&err, 0, SLLM_CUDA_ERR_ARG);        // more entries than the count says
         }
         int sum;
         const int at = block_scan<kResThreads>(cow + fresh, &sum);
