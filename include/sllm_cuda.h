@@ -201,6 +201,7 @@ SLLM_CUDA_API int sllm_cuda_i2s_gemm_silu(const uint8_t * w_gate, const uint8_t 
  *     be captured into a CUDA graph;
  *   - a workspace is the caller's, 16-byte aligned, and holds nothing between
  *     calls. Calls (or graphs) that may overlap need workspaces of their own;
+ *   - a kv_* call that names no slot (n = 0) does nothing; its lists may be NULL;
  *   - outputs and workspaces overlap no other array of the call (kv_append may
  *     write q_out, k_out and v_out exactly over contiguous f32 q, k and v);
  *   - what only the device can see to be wrong (a slot, a length or a page id

@@ -720,7 +720,7 @@ extern "C" size_t sllm_cuda_kv_work_bytes(const sllm_cuda_kv_pages* p) {
 
 extern "C" int sllm_cuda_kv_fork(const sllm_cuda_kv_pages* p, const int32_t* src, const int32_t* dst, int32_t n,
                                  void* work, size_t work_bytes, int32_t* status, void* stream) {
-    if (src == nullptr || dst == nullptr) return fail(SLLM_CUDA_ERR_ARG, "kv_fork: NULL slots");
+    if (n != 0 && (src == nullptr || dst == nullptr)) return fail(SLLM_CUDA_ERR_ARG, "kv_fork: NULL slots");
     const int rc = check_call(p, "kv_fork", n, work, work_bytes, src, dst, status);
     if (rc != SLLM_CUDA_OK || n == 0) return rc;
     kv_fork_kernel<<<kClCtas, kClThreads, 0, (cudaStream_t)stream>>>(pages_dev(*p), src, dst, n, work, status);
@@ -731,7 +731,7 @@ extern "C" int sllm_cuda_kv_fork(const sllm_cuda_kv_pages* p, const int32_t* src
 
 extern "C" int sllm_cuda_kv_release(const sllm_cuda_kv_pages* p, const int32_t* slots, const int32_t* new_len,
                                     int32_t n, void* work, size_t work_bytes, int32_t* status, void* stream) {
-    if (slots == nullptr) return fail(SLLM_CUDA_ERR_ARG, "kv_release: NULL slots");
+    if (n != 0 && slots == nullptr) return fail(SLLM_CUDA_ERR_ARG, "kv_release: NULL slots");
     const int rc = check_call(p, "kv_release", n, work, work_bytes, slots, new_len, status);
     if (rc != SLLM_CUDA_OK || n == 0) return rc;
     kv_release_kernel<<<kClCtas, kClThreads, 0, (cudaStream_t)stream>>>(pages_dev(*p), slots, new_len, n, work, status);
@@ -742,7 +742,8 @@ extern "C" int sllm_cuda_kv_release(const sllm_cuda_kv_pages* p, const int32_t* 
 
 extern "C" int sllm_cuda_kv_reserve(const sllm_cuda_kv_pages* p, const int32_t* slots, const int32_t* n_new,
                                     int32_t n, void* work, size_t work_bytes, int32_t* status, void* stream) {
-    if (slots == nullptr || n_new == nullptr) return fail(SLLM_CUDA_ERR_ARG, "kv_reserve: NULL slots or lengths");
+    if (n != 0 && (slots == nullptr || n_new == nullptr))
+        return fail(SLLM_CUDA_ERR_ARG, "kv_reserve: NULL slots or lengths");
     const int rc = check_call(p, "kv_reserve", n, work, work_bytes, slots, n_new, status);
     if (rc != SLLM_CUDA_OK || n == 0) return rc;
     const cudaStream_t st = (cudaStream_t)stream;

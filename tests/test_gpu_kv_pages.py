@@ -67,3 +67,18 @@ def test_reserve_refuses_a_count_below_the_entries(cuda):
     c.p.reserve(_i32([0, 1, 2]), _i32([1, 1, 1]), c.work, c.status)
     c.same()
     assert c.take_status() == -1
+
+
+def test_calls_that_name_no_slot(cuda):
+    """A step in which nobody forks, grows or ends: nothing to do, no error
+    (an empty tensor has no address)."""
+    c = Cache(cuda, 20, 4, 4, 16)
+    c.m.reserve([0], [21])
+    c.push()
+    none = _i32([])
+    c.p.fork(none, none, c.work, c.status)
+    c.p.reserve(none, none, c.work, c.status)
+    c.p.release(none, None, c.work, c.status)
+    c.p.release(none, none, c.work, c.status)
+    c.same()
+    assert c.take_status() == 0

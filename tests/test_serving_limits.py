@@ -111,3 +111,14 @@ def test_six_partial_products_are_as_good_as_32_bits(n):
     for lost in PAIRS:
         out = attention_planes(*x, [p for p in PAIRS if p != lost])
         assert min(as_good_as_32_bits(out, *x)) > 3, lost
+
+
+def test_no_slots_need_no_arrays(cuda_absent, pkg, L):
+    """n = 0: NULL arrays are passed over (and the call goes on to look for a
+    device); a negative n, or NULL with slots named, is refused as before."""
+    r = C.byref(cache(pkg.abi))
+    size = L.sllm_cuda_kv_work_bytes(r)
+    for n, rc in ((0, -4), (1, -1), (-1, -1)):
+        assert L.sllm_cuda_kv_fork(r, None, None, n, A, size, None, None) == rc
+        assert L.sllm_cuda_kv_reserve(r, None, None, n, A, size, None, None) == rc
+        assert L.sllm_cuda_kv_release(r, None, None, n, A, size, None, None) == rc
