@@ -34,7 +34,7 @@ SLLM_CUDA_API int sllm_cuda_test_gemm_error(void);
 SLLM_CUDA_API int sllm_cuda_test_attn_error(void);
 /* The limit of the attention kernels' bounded waits, in ns, for the calls that
  * follow; 0: the usual 2 s. A call whose wait runs out ends, and says so. */
-SLLM_CUDA_API void sllm_cuda_test_attn_wait(unsigned long long ns);
+SLLM_CUDA_API void sllm_cuda_test_attn_wait(uint32_t ns);
 /* The prefill GEMM's form: 0 by size (at most 16 tokens: weight rows as the
  * MMA's M operand, tokens as N = 16), 1 the 128-token tiles, 2 the skinny
  * form only. */

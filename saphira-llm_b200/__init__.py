@@ -125,7 +125,7 @@ def lib():
     pg = C.POINTER(abi.KvPages)
     L.sllm_cuda_attn_prompt.argtypes = [vp, sz, vp, sz, vp, sz, i32, vp, i32, i32, i32, i32, vp, sz, i32, vp]
     L.sllm_cuda_attn_prompt_checked.argtypes = L.sllm_cuda_attn_prompt.argtypes[:-1] + [vp, vp]
-    L.sllm_cuda_test_attn_wait.argtypes = [C.c_ulonglong]
+    L.sllm_cuda_test_attn_wait.argtypes = [C.c_uint32]
     L.sllm_cuda_test_attn_wait.restype = None
     L.sllm_cuda_kv_work_bytes.argtypes = [pg]
     L.sllm_cuda_kv_work_bytes.restype = sz

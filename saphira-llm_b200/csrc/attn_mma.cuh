@@ -68,43 +68,52 @@ __device__ __forceinline__ void reg_dealloc() { asm volatile("setmaxnreg.dec.syn
 template <int N>
 __device__ __forceinline__ void reg_alloc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 
+// why a bounded wait gave up (0: none did), in each file with such a kernel
+static __device__ int g_attn_error;
+
 // The bounded waits of umma.cuh, in line: a kernel that splits its registers
 // between its warps cannot call functions. Their limit is the launch's: a test
-// sets one that runs out.
-struct WaitEnd {
-    int* error;                     // the file's error word
-    uint64_t ns;                    // the limit
-    __device__ __forceinline__ uint32_t hint() const { return ns < 65536u ? (uint32_t)ns : 65536u; }
-};
-__device__ __forceinline__ bool at_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, const WaitEnd& end) {
-    if (mbar_try_wait_for(bar, parity, end.hint())) return true;
+// sets one that runs out. For it to do so, one wait of each item (at_wait_start)
+// takes the length of a try's sleep from the launch, too; in all of them that
+// cost 2% of many short prompts.
+// (`w`: the launch, asked where a wait goes on.)
+template <class W>
+__device__ __forceinline__ bool at_wait_on(uint64_t* bar, uint32_t parity, volatile int* abort_flag, const W& w, uint32_t nap) {
     const uint64_t t0 = gtimer();
     #pragma unroll 1
-    while (!mbar_try_wait_for(bar, parity, end.hint())) {
+    while (!mbar_try_wait_for(bar, parity, nap)) {
         if (*abort_flag) return false;
-        if (gtimer() - t0 > end.ns) {
+        if (gtimer() - t0 > w.wait_limit().ns) {
             *abort_flag = 1;
-            atomicExch(end.error, GM_TIMEOUT);
+            atomicExch(&g_attn_error, GM_TIMEOUT);
             return false;
         }
     }
     return true;
 }
-__device__ __forceinline__ bool at_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag, const WaitEnd& end) {
-    return __all_sync(0xffffffffu, at_wait(bar, parity, abort_flag, end));
+template <class W>
+__device__ __forceinline__ bool at_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, const W& w) {
+    return mbar_try_wait(bar, parity) || at_wait_on(bar, parity, abort_flag, w, 65536u);
+}
+template <class W>
+__device__ __forceinline__ bool at_wait_start(uint64_t* bar, uint32_t parity, volatile int* abort_flag, const W& w) {
+    return at_wait_on(bar, parity, abort_flag, w, w.wait_limit().nap);
+}
+template <class W>
+__device__ __forceinline__ bool at_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag, const W& w) {
+    return __all_sync(0xffffffffu, at_wait(bar, parity, abort_flag, w));
 }
 // ... with something to try meanwhile
-template <class F>
-__device__ __forceinline__ bool at_wait_while(uint64_t* bar, uint32_t parity, volatile int* abort_flag, const WaitEnd& end,
-                                              F f) {
+template <class W, class F>
+__device__ __forceinline__ bool at_wait_while(uint64_t* bar, uint32_t parity, volatile int* abort_flag, const W& w, F f) {
     const uint64_t t0 = gtimer();
     #pragma unroll 1
     while (!mbar_test(bar, parity)) {
         f();
         if (*abort_flag) return false;
-        if (gtimer() - t0 > end.ns) {
+        if (gtimer() - t0 > w.wait_limit().ns) {
             *abort_flag = 1;
-            atomicExch(end.error, GM_TIMEOUT);
+            atomicExch(&g_attn_error, GM_TIMEOUT);
             return false;
         }
     }
@@ -315,7 +324,7 @@ __device__ __forceinline__ void store_rows(uint32_t o_tmem, float f, uint8_t* st
 // be), tiles(item, t) (0: no such row tile), keys(item),
 // seen(item, t, row) (not above keys, and least for row 0), live(item, t, row)
 // (a row to be written), a Loader, store(...), odd(...) (add_odd for a warp's
-// rows), check() (one idle warp of each CTA), wait_ns() and gave_up() (a wait ran
+// rows), check() (one idle warp of each CTA), wait_limit() and gave_up() (a wait ran
 // out).
 //
 // Registers: 512 threads x 128 at launch; 2 x 184 (softmax) + 80 (outputs) +
@@ -327,8 +336,6 @@ __device__ __forceinline__ long long dealt_number(int r) {
     return (long long)r * gridDim.x + ((r & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
 }
 
-// why a bounded wait gave up (0: none did), in each file with such a kernel
-static __device__ int g_attn_error;
 static inline int take_attn_error() {
     int v = 0;
     const int zero = 0;
@@ -340,7 +347,6 @@ static inline int take_attn_error() {
 
 template <class W>
 __device__ __forceinline__ void attn_core(const W w) {
-    const WaitEnd err{&g_attn_error, w.wait_ns()};
     using Item = typename W::Item;
     extern __shared__ __align__(1024) uint8_t sm[];
     // [2]: per row tile. q, qf: Q there / free; s: scores there; h, p: the
@@ -360,9 +366,10 @@ __device__ __forceinline__ void attn_core(const W w) {
     Shared& sh = *reinterpret_cast<Shared*>(stages + 4 * kAtStage);
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     if ((smem_u32(sm) & 1023u) != 0) {           // the swizzled layouts need it; the compiler was told to
-        if (threadIdx.x == 0) atomicExch(err.error, 2);
+        if (threadIdx.x == 0) atomicExch(&g_attn_error, 2);
         return;
     }
+    if (warp == 15) w.check();
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(&sh.bar_q[i], 1);
@@ -397,14 +404,14 @@ __device__ __forceinline__ void attn_core(const W w) {
     volatile int* const ab = &sh.abort_flag;
 
     auto next_warp = [&](int i, Item* it) {       // false: no more, or a wait gave up
-        if (!at_wait_warp(&sh.bar_item, i & 1, ab, err)) return false;
+        if (!at_wait_warp(&sh.bar_item, i & 1, ab, w)) return false;
         *it = sh.item;
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.bar_itemf);
         return !it->last();
     };
     auto next_lane = [&](int i, Item* it) {
-        if (!at_wait(&sh.bar_item, i & 1, ab, err)) return false;
+        if (!at_wait(&sh.bar_item, i & 1, ab, w)) return false;
         *it = sh.item;
         mbar_arrive(&sh.bar_itemf);
         return !it->last();
@@ -436,7 +443,7 @@ __device__ __forceinline__ void attn_core(const W w) {
                     // this row of the masked tile's values: zeros behind the
                     // sequence, and where no number stands inside it
                     const int x = ring + 2 * j + 1, slot = x % kAtStages;
-                    if (!(ok = at_wait_warp(&sh.bar_full[slot], (x / kAtStages) & 1, ab, err))) break;
+                    if (!(ok = at_wait_warp(&sh.bar_full[slot], (x / kAtStages) & 1, ab, w))) break;
                     uint8_t* v = sm + (2 + slot) * kAtTile + row * 128;
                     const int key = j * kAtKeys + row;
                     if (key >= keys) {
@@ -465,7 +472,7 @@ __device__ __forceinline__ void attn_core(const W w) {
                     }
                     fence_proxy_async_smem();
                 }
-                if (!(ok = at_wait_warp(&sh.bar_s[t], steps & 1, ab, err))) break;
+                if (!(ok = at_wait_warp(&sh.bar_s[t], steps & 1, ab, w))) break;
                 tc_fence_after();
                 if (idle) {
                     if (lane == 0) {
@@ -526,7 +533,7 @@ __device__ __forceinline__ void attn_core(const W w) {
             ring += 2 * max(n0, n1);
             if (n == 0) continue;
             // the sums of the item before have been read
-            if (uses > 0 && !(ok = at_wait_warp(&sh.bar_of[t], (uses - 1) & 1, ab, err))) break;
+            if (uses > 0 && !(ok = at_wait_warp(&sh.bar_of[t], (uses - 1) & 1, ab, w))) break;
             ++uses;
             sh.sum[t][row] = l;
             sh.top[t][row] = m;
@@ -550,7 +557,7 @@ __device__ __forceinline__ void attn_core(const W w) {
                 if (w.tiles(it, t) == 0) break;
                 const int par = uses[t] & 1;
                 ++uses[t];
-                if (!(ok = at_wait_warp(&sh.bar_l[t], par, ab, err) && at_wait_warp(&sh.bar_o[t], par, ab, err))) break;
+                if (!(ok = at_wait_warp(&sh.bar_l[t], par, ab, w) && at_wait_warp(&sh.bar_o[t], par, ab, w))) break;
                 tc_fence_after();
                 odd = odd || (sh.odd[t][0] | sh.odd[t][1] | sh.odd[t][2] | sh.odd[t][3]) != 0;
                 w.store(it, t, row, tmem + lanes + 256 + 128 * t, sh.top[t][row], sh.sum[t][row],
@@ -607,14 +614,14 @@ __device__ __forceinline__ void attn_core(const W w) {
                     known = false;
                     const int n0 = w.tiles(it, 0), n1 = w.tiles(it, 1), nt = max(n0, n1);
                     if (!ahead) {
-                        ok = at_wait(&sh.bar_q[0], uses0 & 1, ab, err) && at_wait(&sh.bar_full[ks], kp, ab, err);
+                        ok = at_wait_start(&sh.bar_q[0], uses0 & 1, ab, w) && at_wait(&sh.bar_full[ks], kp, ab, w);
                         if (!ok) break;
                         scores(0);
                         if (n0 == 1) umma_commit(&sh.bar_qf[0]);
                     }
                     ahead = false;
                     if (n1 > 0) {
-                        if (!(ok = at_wait(&sh.bar_q[1], uses1 & 1, ab, err))) break;
+                        if (!(ok = at_wait(&sh.bar_q[1], uses1 & 1, ab, w))) break;
                         scores(1);
                         if (n1 == 1) umma_commit(&sh.bar_qf[1]);
                     }
@@ -636,20 +643,20 @@ __device__ __forceinline__ void attn_core(const W w) {
                     #pragma unroll 1
                     for (int j = 0; j < nt && ok; ++j) {
                         const bool more = j + 1 < nt;
-                        ok = at_wait(&sh.bar_full[vs], vp, ab, err) && (!more || at_wait(&sh.bar_full[ks], kp, ab, err));
+                        ok = at_wait(&sh.bar_full[vs], vp, ab, w) && (!more || at_wait(&sh.bar_full[ks], kp, ab, w));
                         #pragma unroll
                         for (int t = 0; t < 2; ++t) {
                             const int n = t == 0 ? n0 : n1, uses = t == 0 ? uses0 : uses1;
                             int& steps = t == 0 ? steps0 : steps1;
                             if (!ok || j >= n) continue;
                             // the item before has left O (of) before the first product overwrites it
-                            ok = j > 0 || uses == 0 || at_wait(&sh.bar_of[t], (uses - 1) & 1, ab, err);
-                            if (t == 1 && !more) ok = ok && at_wait_while(&sh.bar_h[1], steps & 1, ab, err, look);
-                            else ok = ok && at_wait(&sh.bar_h[t], steps & 1, ab, err);
+                            ok = j > 0 || uses == 0 || at_wait(&sh.bar_of[t], (uses - 1) & 1, ab, w);
+                            if (t == 1 && !more) ok = ok && at_wait_while(&sh.bar_h[1], steps & 1, ab, w, look);
+                            else ok = ok && at_wait(&sh.bar_h[t], steps & 1, ab, w);
                             if (!ok) continue;
                             tc_fence_after();
                             outputs(t, 0, j > 0);
-                            if (!(ok = at_wait(&sh.bar_p[t], steps & 1, ab, err))) continue;
+                            if (!(ok = at_wait(&sh.bar_p[t], steps & 1, ab, w))) continue;
                             tc_fence_after();
                             outputs(t, 1, true);
                             ++steps;
@@ -688,13 +695,13 @@ __device__ __forceinline__ void attn_core(const W w) {
                     // Q0, K0, Q1, V0, K1, V1, ...
                     const int t = j < 0 ? 0 : 1;
                     if (j < 0 || (j == 1 && n1 > 0)) {
-                        if (uses[t] > 0 && !(ok = at_wait_warp(&sh.bar_qf[t], (uses[t] - 1) & 1, ab, err))) break;
+                        if (uses[t] > 0 && !(ok = at_wait_warp(&sh.bar_qf[t], (uses[t] - 1) & 1, ab, w))) break;
                         ++uses[t];
                         load.q(w, it, t, sm + t * kAtTile, &sh.bar_q[t], lane);
                     }
                     if (j < 0) continue;
                     const int s = x % kAtStages, use = x / kAtStages;
-                    if (use > 0 && !(ok = at_wait_warp(&sh.bar_free[s], (use - 1) & 1, ab, err))) break;
+                    if (use > 0 && !(ok = at_wait_warp(&sh.bar_free[s], (use - 1) & 1, ab, w))) break;
                     load.kv(w, it, j >> 1, (j & 1) != 0, sm + (size_t)(2 + s) * kAtTile, &sh.bar_full[s], lane);
                     ++x;
                 }
@@ -711,7 +718,7 @@ __device__ __forceinline__ void attn_core(const W w) {
             #pragma unroll 1
             for (int r = 0, i = 0;; ++r) {
                 // every warp has taken the item before
-                if (i > 0 && !at_wait_warp(&sh.bar_itemf, (i - 1) & 1, ab, err)) break;
+                if (i > 0 && !at_wait_warp(&sh.bar_itemf, (i - 1) & 1, ab, w)) break;
                 Item it;
                 if (!find.item(w, find.number(w, r), &it)) continue;    // no item has this number
                 if (lane == 0) {
@@ -721,8 +728,6 @@ __device__ __forceinline__ void attn_core(const W w) {
                 if (it.last()) break;
                 ++i;
             }
-        } else {
-            w.check();
         }
     }
     tc_fence_before();

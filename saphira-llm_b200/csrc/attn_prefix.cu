@@ -50,7 +50,7 @@ struct PrefixParams {
     size_t page_stride;             // elements
     const int32_t* slots;
     int n, n_q, n_head, n_kv, group, prefix;
-    unsigned long long wait_ns;
+    WaitLimit wait;
     int32_t* status;
     float* part_o;                  // [n_kv][rows][sp + cm][128]
     float2* part_ml;                // [n_kv][rows][sp + cm]
@@ -193,7 +193,7 @@ struct PrefixWork {
             return find_item(w.pg, w.p, x, it);
         }
     };
-    __device__ __forceinline__ unsigned long long wait_ns() const { return p.wait_ns; }
+    __device__ __forceinline__ WaitLimit wait_limit() const { return p.wait; }
     __device__ __forceinline__ void check() const {}
     __device__ __forceinline__ void gave_up() const { raise(p.status, SLLM_CUDA_ERR_TIMEOUT); }
     __device__ __forceinline__ int tiles(const Item& it, int t) const {
@@ -280,7 +280,7 @@ struct PrefixWide {
     const PagesDev& pg;
     const PrefixParams& p;
 
-    __device__ __forceinline__ unsigned long long wait_ns() const { return p.wait_ns; }
+    __device__ __forceinline__ WaitLimit wait_limit() const { return p.wait; }
     __device__ __forceinline__ void check() const {}
     __device__ __forceinline__ void gave_up() const { raise(p.status, SLLM_CUDA_ERR_TIMEOUT); }
     __device__ __forceinline__ bool find(long long x, Item* it) const { return find_item(pg, p, x, it); }
@@ -591,7 +591,7 @@ extern "C" int sllm_cuda_attn_prefix(const sllm_cuda_kv_pages* p, int32_t layer,
     a.n = n; a.n_q = n_q; a.n_head = n_head; a.n_kv = p->n_head_kv; a.group = n_head / p->n_head_kv;
     a.prefix = prefix_len;
     a.status = status;
-    a.wait_ns = attn_wait_ns();
+    a.wait = attn_wait_limit();
     a.plan = plan;
     a.part_o = static_cast<float*>(work);
     a.part_ml = reinterpret_cast<float2*>(a.part_o + parts * kServeDim);

@@ -24,7 +24,7 @@ struct PromptParams {
     size_t qs, ks, vs, os;          // elements from a token to the next
     const int32_t* cu;
     int n_seq, n_tokens, n_head, group;
-    unsigned long long wait_ns;
+    WaitLimit wait;
     int32_t* status;
 };
 
@@ -165,7 +165,7 @@ struct PromptWork {
             return true;
         }
     };
-    __device__ __forceinline__ unsigned long long wait_ns() const { return p.wait_ns; }
+    __device__ __forceinline__ WaitLimit wait_limit() const { return p.wait; }
     __device__ __forceinline__ void check() const { check_offsets(p); }
     __device__ __forceinline__ void gave_up() const { raise(p.status, SLLM_CUDA_ERR_TIMEOUT); }
     // key tiles of row tile t: up to its diagonal, or the sequence's end
@@ -232,7 +232,7 @@ struct PromptWide {
     };
     const PromptParams& p;
 
-    __device__ __forceinline__ unsigned long long wait_ns() const { return p.wait_ns; }
+    __device__ __forceinline__ WaitLimit wait_limit() const { return p.wait; }
     __device__ __forceinline__ void check() const { check_offsets(p); }
     __device__ __forceinline__ void gave_up() const { raise(p.status, SLLM_CUDA_ERR_TIMEOUT); }
     // longest first; of more than 32 sequences in their order, which takes no
@@ -368,7 +368,7 @@ extern "C" int sllm_cuda_attn_prompt_checked(const void* q, size_t q_stride, con
     p.q = q; p.k = k; p.v = v; p.out = out;
     p.qs = q_stride; p.ks = k_stride; p.vs = v_stride; p.os = out_stride;
     p.cu = cu_seqlens;
-    p.wait_ns = attn_wait_ns();
+    p.wait = attn_wait_limit();
     p.status = status;
     p.n_seq = n_seq; p.n_tokens = n_tokens; p.n_head = n_head; p.group = n_head / n_head_kv;
     const cudaStream_t st = (cudaStream_t)stream;

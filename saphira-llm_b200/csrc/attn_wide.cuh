@@ -196,12 +196,11 @@ __device__ __forceinline__ void store_cols(uint32_t o_tm, uint32_t t_tm, bool to
 // tile(key, n): the next are keys key, key + 8, .. below n; row(i): the i-th of
 // them); scale(l) (what the outputs are multiplied by), out(item, row) (where the
 // rows from `row` on go), finish(item, row, m, l) (the rest of a row's result),
-// value(item, key) (a row of values), check() (one warp of each CTA), wait_ns(),
+// value(item, key) (a row of values), check() (one warp of each CTA), wait_limit(),
 // gave_up().
 template <class W>
 __device__ __forceinline__ void attn_wide_core(const W w) {
     using T = typename W::T;
-    const WaitEnd err{&g_attn_error, w.wait_ns()};
     extern __shared__ __align__(1024) uint8_t sm[];
     struct Shared {
         // q: split; q1: the first plane in tensor memory; k, v: tile split; vf:
@@ -218,7 +217,7 @@ __device__ __forceinline__ void attn_wide_core(const W w) {
     Shared& sh = *reinterpret_cast<Shared*>(sm + kWdEnd);
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     if ((smem_u32(sm) & 1023u) != 0) {
-        if (threadIdx.x == 0) atomicExch(err.error, 2);
+        if (threadIdx.x == 0) atomicExch(&g_attn_error, 2);
         return;
     }
     if (warp == 0) {                    // (by every warp it took twice as long)
@@ -320,7 +319,7 @@ __device__ __forceinline__ void attn_wide_core(const W w) {
         float m = -INFINITY, l = 0.f;
         split_q(std::integral_constant<int, 16>{}, kAtRows / 2 + 16 * warp, 1);
         // this row's first plane of Q, from the staging place
-        bool ok = at_wait_warp(&sh.bar_q, 0, ab, err);
+        bool ok = at_wait_warp(&sh.bar_q, 0, ab, w);
         if (ok) {
             #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -386,7 +385,7 @@ __device__ __forceinline__ void attn_wide_core(const W w) {
         };
         for (int j = 0; j < n && ok; ++j) {
             const uint32_t s_tm = tmem + lanes;
-            if (!(ok = at_wait_warp(&sh.bar_s[j & 1], (j >> 1) & 1, ab, err))) break;
+            if (!(ok = at_wait_warp(&sh.bar_s[j & 1], (j >> 1) & 1, ab, w))) break;
             tc_fence_after();
             float s[64];
             {
@@ -433,7 +432,7 @@ __device__ __forceinline__ void attn_wide_core(const W w) {
             // the products before are complete when the values' place is free:
             // then the weights' place is, too, and the outputs may be touched
             if (j > 0) {
-                if (!(ok = at_wait_warp(&sh.bar_vf, (j - 1) & 1, ab, err))) break;
+                if (!(ok = at_wait_warp(&sh.bar_vf, (j - 1) & 1, ab, w))) break;
                 tc_fence_after();
             }
             #pragma unroll
@@ -454,7 +453,7 @@ __device__ __forceinline__ void attn_wide_core(const W w) {
         sh.f[row] = w.scale(l);
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.bar_f);
-        if (ok && at_wait_warp(&sh.bar_o, 0, ab, err)) {
+        if (ok && at_wait_warp(&sh.bar_o, 0, ab, w)) {
             if (live) w.finish(it, row, m, l);
         }
     } else if (warp < 20) {
@@ -487,9 +486,9 @@ __device__ __forceinline__ void attn_wide_core(const W w) {
             // when the scores two tiles before are (the second place: when the
             // queries' first plane has left it)
             if (is_v) {
-                if (j > 0 && !at_wait_warp(&sh.bar_vf, (j - 1) & 1, ab, err)) break;
+                if (j > 0 && !at_wait_warp(&sh.bar_vf, (j - 1) & 1, ab, w)) break;
             } else if (j > 0) {
-                if (!at_wait_warp(j > 1 ? &sh.bar_s[j & 1] : &sh.bar_q1, j > 1 ? ((j >> 1) - 1) & 1 : 0, ab, err)) break;
+                if (!at_wait_warp(j > 1 ? &sh.bar_s[j & 1] : &sh.bar_q1, j > 1 ? ((j >> 1) - 1) & 1 : 0, ab, w)) break;
             }
             uint8_t* const tile = sm + (is_v ? kWdV : kWdK + (j & 1) * 3 * kWdPlane) + half * kWdHalf;
             float top = 0.f;
@@ -523,7 +522,7 @@ __device__ __forceinline__ void attn_wide_core(const W w) {
         }
         // the outputs: sixteen warps, 32 rows x 32 columns each (the query
         // planes' place is free)
-        if (at_wait_warp(&sh.bar_f, 0, ab, err) && at_wait_warp(&sh.bar_o, 0, ab, err)) {
+        if (at_wait_warp(&sh.bar_f, 0, ab, w) && at_wait_warp(&sh.bar_o, 0, ab, w)) {
             tc_fence_after();
             const int first = 32 * (warp & 3), col = 32 * ((warp - 4) >> 2);
             const uint32_t at = tmem + ((uint32_t)first << 16) + col;
@@ -582,8 +581,8 @@ __device__ __forceinline__ void attn_wide_core(const W w) {
                 }
                 umma_commit(&sh.bar_vf);
             };
-            bool ok = at_wait(&sh.bar_q, 0, ab, err) && at_wait(&sh.bar_q1, 0, ab, err) &&
-                      at_wait(&sh.bar_k[0], 0, ab, err);
+            bool ok = at_wait_start(&sh.bar_q, 0, ab, w) && at_wait(&sh.bar_q1, 0, ab, w) &&
+                      at_wait(&sh.bar_k[0], 0, ab, w);
             if (ok) {
                 tc_fence_after();
                 scores(0);
@@ -591,13 +590,13 @@ __device__ __forceinline__ void attn_wide_core(const W w) {
             #pragma unroll 1
             for (int j = 0; j < n && ok; ++j) {
                 if (j + 1 < n) {
-                    if (!(ok = at_wait(&sh.bar_k[(j + 1) & 1], ((j + 1) >> 1) & 1, ab, err) &&
-                               at_wait(&sh.bar_sf, j & 1, ab, err)))
+                    if (!(ok = at_wait(&sh.bar_k[(j + 1) & 1], ((j + 1) >> 1) & 1, ab, w) &&
+                               at_wait(&sh.bar_sf, j & 1, ab, w)))
                         break;
                     tc_fence_after();
                     scores(j + 1);
                 }
-                if (!(ok = at_wait(&sh.bar_v, j & 1, ab, err) && at_wait(&sh.bar_p, j & 1, ab, err))) break;
+                if (!(ok = at_wait(&sh.bar_v, j & 1, ab, w) && at_wait(&sh.bar_p, j & 1, ab, w))) break;
                 tc_fence_after();
                 outputs(j);
             }

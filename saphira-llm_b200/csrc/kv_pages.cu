@@ -653,10 +653,10 @@ cudaError_t launch_copies(const sllm_cuda_kv_pages& p, long long most, void* wor
 
 }  // namespace
 
-static std::atomic<unsigned long long> g_attn_wait_ns{0};
-unsigned long long attn_wait_ns() {
-    const unsigned long long ns = g_attn_wait_ns.load(std::memory_order_relaxed);
-    return ns != 0 ? ns : 2000000000ull;
+static std::atomic<uint32_t> g_attn_wait_ns{0};
+WaitLimit attn_wait_limit() {
+    const uint32_t set = g_attn_wait_ns.load(std::memory_order_relaxed), ns = set != 0 ? set : 2000000000u;
+    return WaitLimit{ns, ns < 65536u ? ns : 65536u};
 }
 
 int current_sms() {
@@ -711,7 +711,7 @@ extern "C" int sllm_cuda_test_attn_error(void) {
     return a != 0 ? a : b;
 }
 
-extern "C" void sllm_cuda_test_attn_wait(unsigned long long ns) { g_attn_wait_ns.store(ns, std::memory_order_relaxed); }
+extern "C" void sllm_cuda_test_attn_wait(uint32_t ns) { g_attn_wait_ns.store(ns, std::memory_order_relaxed); }
 
 extern "C" size_t sllm_cuda_kv_work_bytes(const sllm_cuda_kv_pages* p) {
     if (check_pages(p, "kv_work_bytes") != SLLM_CUDA_OK) return 0;

@@ -25,8 +25,12 @@ int check_pages(const sllm_cuda_kv_pages* p, const char* who);
 // the error words of the attention kernels' bounded waits, read and cleared
 int take_prompt_error();
 int take_prefix_error();
-// the limit of those waits for the next launches (2 s; tests set a short one)
-unsigned long long attn_wait_ns();
+// the limit of those waits for the next launches (2 s; tests set a short one), and
+// of one try's sleep, ns
+struct WaitLimit {
+    uint32_t ns, nap;
+};
+WaitLimit attn_wait_limit();
 
 int current_sms();
 
