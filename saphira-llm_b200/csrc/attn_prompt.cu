@@ -46,23 +46,41 @@ __device__ __forceinline__ int seq_len(const PromptParams& p, int s, int* start)
     return min(max(p.cu[s + 1], *start), p.n_tokens) - *start;
 }
 
+// the place of the n-th bit (from 0) that is set, by a whole warp; it is there
+__device__ __forceinline__ int nth_bit(unsigned bits, int n) {
+    const unsigned lane = threadIdx.x & 31, below = bits & ((1u << lane) - 1u);
+    return __ffs(__ballot_sync(0xffffffffu, (bits >> lane & 1u) != 0 && __popc(below) == n)) - 1;
+}
+
 // The call's tiles of R rows in descending order of their position in their
 // sequence (the later, the more keys they see): the longest work first. One
 // warp; what it asks for only ever rises, so all of a CTA's searches together
 // walk the sequences once per position. (With a search from the start for each
 // item 256 prompts of 100 to 200 tokens, 20 heads, took 270 us instead of 198,
-// 2048 of 32 to 64 tokens 6.0 ms instead of 1.05.)
+// 2048 of 32 to 64 tokens 6.0 ms instead of 1.05.) Positions that the same
+// sequences reach are passed over after one walk: 65535 prompts of 8 tokens and
+// one of 131072 take 6.6 ms; with a walk for each of its tiles, behind which the
+// other warps wait, 256 ms.
 template <int R>
 struct LongFirst {
     int pos;                        // the position
     int before;                     // tiles at later positions, and at this one in sequences below s0
     int s0;
+    int at, below;                  // `before` at this walk's start; the most tiles of sequences that end before pos (by lanes)
+    int2 cur, nxt;                  // the offsets of sequences s0 .. s0 + 31, and of the 32 that are looked at after them
+    __device__ __forceinline__ int2 offsets(const PromptParams& p, int s) const {
+        s = min(s + (int)(threadIdx.x & 31), p.n_seq - 1);
+        return make_int2(p.cu[s], p.cu[s + 1]);
+    }
+    __device__ __forceinline__ int after(const PromptParams& p, int s) const { return s + 32 < p.n_seq ? s + 32 : 0; }
     __device__ __forceinline__ void start(const PromptParams& p) {
         int most = 0, a;
-        before = s0 = pos = 0;
+        before = s0 = pos = at = below = 0;
         if (p.n_seq == 1) return;
         for (int s = threadIdx.x & 31; s < p.n_seq; s += 32) most = max(most, (seq_len(p, s, &a) + R - 1) / R);
         pos = __reduce_max_sync(0xffffffffu, most) - 1;
+        cur = offsets(p, 0);
+        nxt = offsets(p, after(p, 0));
     }
     // tile x; false: there is none, nor any after it
     __device__ __forceinline__ bool find(const PromptParams& p, int x, int* start, int* len, int* tile) {
@@ -73,21 +91,30 @@ struct LongFirst {
             return *tile >= 0;
         }
         if (x >= p.n_tokens / R + p.n_seq) return false;        // ascending offsets have no more
-        for (; pos >= 0; --pos, s0 = 0) {
-            for (; s0 < p.n_seq; s0 += 32) {
-                int a = 0, n = 0;
-                if (s0 + lane < p.n_seq) n = seq_len(p, s0 + lane, &a);
-                const unsigned has = __ballot_sync(0xffffffffu, (n + R - 1) / R > pos);
-                const int c = __popc(has), r = x - before;
-                if (r < c) {
-                    const int l = __fns(has, 0, r + 1);
-                    *start = __shfl_sync(0xffffffffu, a, l);
-                    *len = __shfl_sync(0xffffffffu, n, l);
-                    *tile = pos;
-                    return true;
-                }
-                before += c;
+        while (pos >= 0) {
+            const int a = min(max(cur.x, 0), p.n_tokens);
+            const int n = s0 + lane < p.n_seq ? min(max(cur.y, a), p.n_tokens) - a : 0, tiles = (n + R - 1) / R;
+            const unsigned has = __ballot_sync(0xffffffffu, tiles > pos);
+            const int c = __popc(has), r = x - before;
+            if (r < c) {
+                const int l = nth_bit(has, r);
+                *start = __shfl_sync(0xffffffffu, a, l);
+                *len = __shfl_sync(0xffffffffu, n, l);
+                *tile = pos;
+                return true;
             }
+            before += c;
+            if (tiles <= pos) below = max(below, tiles);
+            s0 = after(p, s0);
+            cur = nxt;
+            if (p.n_seq > 32) nxt = offsets(p, after(p, s0));
+            if (s0 != 0) continue;
+            const int each = before - at, same = pos - __reduce_max_sync(0xffffffffu, below);
+            const int skip = min(same, (x - before) / each);
+            pos -= skip + 1;
+            before += skip * each;
+            at = before;
+            below = 0;
         }
         return false;
     }
@@ -112,7 +139,7 @@ __device__ __forceinline__ bool find_long_first(const PromptParams& p, int x, in
             f_hi = f;
         }
     }
-    const int l = __fns(__ballot_sync(0xffffffffu, tiles > lo), 0, x - f_hi + 1);
+    const int l = nth_bit(__ballot_sync(0xffffffffu, tiles > lo), x - f_hi);
     *start = __shfl_sync(0xffffffffu, a, l);
     *len = __shfl_sync(0xffffffffu, n, l);
     *tile = lo;

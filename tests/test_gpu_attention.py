@@ -333,3 +333,39 @@ def test_prefix_f32_is_as_good_as_32_bits(cuda, prefix, owns, nq, heads):
             x = (q[b, :, rows].reshape(-1, 128), c.rows(b)[:, 1, g], c.rows(b, c.v)[:, 1, g], lim)
             big, rms = as_good_as_32_bits(out[b, :, rows].reshape(-1, 128), *x)
             assert big <= 3 and rms <= 3, (b, g, big, rms)
+
+
+def test_prompt_one_long_sequence_among_very_many(cuda):
+    """The search for the next item passes over positions that the same
+    sequences reach: the others wait behind it (7 ms; 256 ms when it walked all
+    sequences once for each of the long one's tiles)."""
+    import torch
+    short, long = 8, 1 << 17
+    lens = [short] * 60000 + [long] + [0, short] * 2767 + [1]
+    T, at = sum(lens), short * 60000
+    q, k, v = (_rand(s, T, 1, 128, dt=torch.float16) for s in (1, 2, 3))
+    out, status = torch.empty_like(q), _i32([0])
+    cu = _i32(np.concatenate([[0], np.cumsum(lens)]).tolist())
+    ms = []
+    for _ in range(3):
+        out.fill_(7.0)
+        a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        a.record()
+        cuda.attn_prompt(q, k, v, out, cu, status=status)
+        b.record()
+        torch.cuda.synchronize()
+        ms.append(a.elapsed_time(b))
+    assert status.item() == 0 and cuda.attn_error() == 0
+    # the short ones all at once, the long one's rows here and there
+    n = T - long
+    keep = torch.cat([torch.arange(at, device="cuda"), torch.arange(at + long, T, device="cuda")])[:n - 1].view(-1, short)
+    qq, kk, vv = (t[keep, 0].double() for t in (q, k, v))
+    s = (qq @ kk.transpose(1, 2) / math.sqrt(128.0)).masked_fill(torch.ones(short, short, device="cuda").triu(1).bool(), -math.inf)
+    want = torch.softmax(s, -1) @ vv
+    assert float((out[keep, 0].double() - want).abs().max()) < 0.01     # (another sequence's keys would be off by about 1)
+    assert torch.equal(out[-1], v[-1])
+    rows = torch.tensor([0, 255, 256, 70000, long - 1], device="cuda")
+    x = (k[at:at + long, 0].double(), v[at:at + long, 0].double())
+    want, pv, big, va = attention(q[at + rows, 0].double(), *x, rows + 1)
+    assert bool(((out[at + rows, 0].double() - want).abs() <= attention_bound(want, pv, big, va, long, True, True)).all())
+    assert min(ms) < 60.0, ms
