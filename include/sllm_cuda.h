@@ -322,7 +322,7 @@ SLLM_CUDA_API int sllm_cuda_kv_compact(const sllm_cuda_kv_pages * p, void * work
  * to the next. A token with slot[t] < 0 is padding: nothing of it is
  * written. A token whose slot, position or page is wrong, or whose
  * page has other owners, sets SLLM_CUDA_ERR_ARG in *status and is left out.
- * Two tokens for one place leave either of them.
+ * Two tokens for one place leave a mix of both there.
  */
 SLLM_CUDA_API int sllm_cuda_kv_append(const sllm_cuda_kv_pages * p, int32_t layer, int32_t n_tokens,
                                       const int32_t * slot, const int32_t * pos, int32_t n_head,
