@@ -41,7 +41,7 @@
 // 2.4 us, with the products cut to a sixth besides 1.7 us. An item's start and
 // end cost about 9 us: 1.2 to find it among several prompts, 2.6 to read and
 // split Q and the first tile, 2.6 for the first scores and softmax, 1.6 for the
-// last products, 1.4 to store. Four prompts of 320, 1, 777 and 256 tokens: 43.6
+// last products, 1.4 to store. Four prompts of 320, 1, 777 and 256 tokens: 42.4
 // us, the longest row tile's 36 us among them. 32 heads of 8 against a prefix of
 // 16384: 59 us.
 //

@@ -15,10 +15,11 @@
 // What is rare costs another pass: a residual without mass (p stands in), and
 // infinities, which count as nothing.
 //
-// Bound: HBM for many sequences (64 of 128256 words: 10.2 us for the two rows
-// that each needs; measured 17.3 us, 3.8 TB/s); for one, the chain of dependent
-// reads: lengths and tokens, their probabilities, the rows, the run again
-// (measured 9.5 us).
+// Bound: for one sequence the chain of dependent reads: lengths and tokens,
+// their probabilities, the rows, the run again (measured 9.5 us); for many the
+// loads of a row's pass, four of each row in flight a warp, summed before the next
+// (64 of 128256 words: 17.3 us, 3.8 TB/s, 10.2 us for the two rows that each needs
+// at the memory's rate; 256: 57.5 us, 4.6 TB/s, 41 us).
 
 #include <cooperative_groups.h>
 
