@@ -223,7 +223,7 @@ SLLM_CUDA_API int sllm_cuda_i2s_gemm_silu(const uint8_t * w_gate, const uint8_t 
  * Q/K/V array can be passed as they are. Rows of `out` behind the last
  * sequence are not written. A key that a row does not see leaves no trace in
  * it, not even as an infinity or a NaN; in a row that does see it, a value that
- * is no finite number leaves no number in its dimension, a key none in all
+ * is no finite number leaves none in its dimension, a key may leave none in all
  * (in f16 a score of -inf only has weight 0). q, k and v have type `type`; out is
  * f32 or, from f16, f16. f16 inputs are multiplied on the tensor cores with
  * f32 sums and softmax; the softmax weights are rounded to f16 there (11 bits

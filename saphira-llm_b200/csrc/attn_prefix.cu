@@ -387,7 +387,7 @@ attn_prefix_join_kernel(const __grid_constant__ PagesDev pg, const __grid_consta
             #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const float g = __shfl_sync(0xffffffffu, f, (i + e) & 31);
-                if (i + e < n && g != 0.f) {
+                if (i + e < n) {        // (a part too small to count still brings its infinities)
                     o.x = fmaf(g, v[e].x, o.x);
                     o.y = fmaf(g, v[e].y, o.y);
                     o.z = fmaf(g, v[e].z, o.z);

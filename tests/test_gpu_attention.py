@@ -166,6 +166,31 @@ def test_prefix_odd_values_one_by_one(cuda, dt, prefix, owns, page, heads, nq):
     assert bool(torch.isnan(b[:, :, :, 90][mask[:, :, :, 90]]).all())
 
 
+@pytest.mark.parametrize("dt", ["f32", "f16"])
+def test_prefix_odd_value_of_a_vanishing_part(cuda, dt):
+    """Scores of the own tokens 250 below the prefix's, so that their part weighs
+    e^-250: 0 in 32 bits, but an infinity among its values is still one."""
+    import torch
+    c = shared_cache(cuda, 256, [40, 70], 16, (4, 2), dt)
+    c.k *= 0.1
+    c.k[c.m.tables[0][0], :, :, 5] = 22.0
+    q = _rand(3, 2, 2, 4, 128, dt=_dt(dt), scale=0.1).add_(1.0)
+    for s in (0, 1):
+        n = c.m.lens[s]
+        c.v[c.m.tables[s][(n - 1) // 16], :, :, (n - 1) % 16, 9] = math.inf
+        c.v[c.m.tables[s][(n - 7) // 16], :, :, (n - 7) % 16, 70] = math.nan
+    out = torch.empty(2, 2, 4, 128, device="cuda")
+    work = torch.empty(c.p.attn_prefix_work_bytes(2, 2, 4, 256), dtype=torch.uint8, device="cuda")
+    c.p.attn_prefix(1, q, out, _i32([0, 1]), 256, work, c.status)
+    torch.cuda.synchronize()
+    assert c.take_status() == 0
+    assert not bool(torch.isfinite(out[:, 1, :, 9]).any()) and bool(torch.isfinite(out[:, 0, :, 9]).all())
+    assert bool(torch.isnan(out[:, :, :, 70]).all())
+    v = c.v[c.m.tables[0][0], 1, :, 5].float().repeat_interleave(2, 0)      # the one key that counts
+    rest = [d for d in range(128) if d not in (9, 70)]
+    assert float((out - v)[..., rest].abs().max()) < 1e-3
+
+
 def test_prompt_odd_value_at_the_end_of_a_long_sequence(cuda):
     """No work grows with the sequence where a value is no number: no bounded
     wait runs out, and the rows before it are those of the run without it."""
