@@ -109,7 +109,8 @@ struct LongFirst {
             cur = nxt;
             if (p.n_seq > 32) nxt = offsets(p, after(p, s0));
             if (s0 != 0) continue;
-            const int each = before - at, same = pos - __reduce_max_sync(0xffffffffu, below);
+            // (never 0, unless somebody writes the offsets meanwhile; the search ends all the same)
+            const int each = max(before - at, 1), same = pos - __reduce_max_sync(0xffffffffu, below);
             const int skip = min(same, (x - before) / each);
             pos -= skip + 1;
             before += skip * each;
