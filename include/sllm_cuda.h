@@ -231,7 +231,8 @@ SLLM_CUDA_API int sllm_cuda_i2s_gemm_silu(const uint8_t * w_gate, const uint8_t 
  * infinite from 2^128 - 2^119 on.
  * The first form has no status word: wrong offsets stay inside the arrays, but
  * nobody hears of them, nor of a bounded wait that ran out. The second reports
- * both in `*status`.
+ * both in `*status`. n_seq <= 2^20, n_tokens <= 2^24, n_head <= 1024, strides <=
+ * 2^30.
  */
 SLLM_CUDA_API int sllm_cuda_attn_prompt(const void * q, size_t q_stride, const void * k, size_t k_stride,
                                         const void * v, size_t v_stride, int32_t type,
@@ -251,7 +252,8 @@ SLLM_CUDA_API int sllm_cuda_attn_prompt_checked(const void * q, size_t q_stride,
  * tables[s * table_width + t / page_size]. refs[p] is the number of table
  * entries that name page p; 0 means free. Entries behind a slot's last page
  * mean nothing. An empty cache is all zeros in refs and lens. Slots may share
- * pages (kv_fork); only a page with one owner is ever written.
+ * pages (kv_fork); only a page with one owner is ever written. At most 2^24
+ * pages, 65536 slots, 1024 layers and kv heads, 2^31 - 256 tokens a slot.
  */
 typedef struct sllm_cuda_kv_pages {
     void    * k;
@@ -374,7 +376,7 @@ SLLM_CUDA_API int sllm_cuda_attn_prefix(const sllm_cuda_kv_pages * p, int32_t la
  * drawn one and -1 behind it, count [n] their number; the drawn token is -1
  * where p has no mass either. A drafted id out of range is refused, a draft
  * length out of range clamped, with SLLM_CUDA_ERR_ARG in *status.
- * k <= 64, n <= 65536.
+ * 1 <= k <= 64, n <= 65536, n_vocab <= 2^24.
  */
 SLLM_CUDA_API int sllm_cuda_spec_verify(const float * p, const float * q, const int32_t * draft,
                                         const int32_t * n_draft, const float * u_accept, const float * u_draw,
