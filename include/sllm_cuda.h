@@ -41,6 +41,7 @@ extern "C" {
 /* the types of a KV cache (sllm_cuda_ctx_new_kv, sllm_cuda_kv_pages) */
 #define SLLM_CUDA_KV_F32 0
 #define SLLM_CUDA_KV_F16 1
+#define SLLM_CUDA_KV_I8  2      /* paged caches only (sllm_cuda_kv_pages) */
 
 /* ------------------------------------------------------------------ */
 /* status codes                                                        */
@@ -193,8 +194,8 @@ SLLM_CUDA_API int sllm_cuda_i2s_gemm_silu(const uint8_t * w_gate, const uint8_t 
  * 32-bit sums, not bit for bit.
  *
  * Rules for all of them:
- *   - head dim 128, as everywhere in this library; types are the cache types
- *     SLLM_CUDA_KV_F32 / _F16;
+ *   - head dim 128, as everywhere in this library; types are
+ *     SLLM_CUDA_KV_F32 / _F16, and of a paged cache SLLM_CUDA_KV_I8 besides;
  *   - every array is memory of the current device (anything else is refused
  *     with SLLM_CUDA_ERR_ARG); `stream` belongs to that device;
  *   - asynchronous on `stream`, no allocation, no synchronisation: they can
@@ -264,8 +265,18 @@ typedef struct sllm_cuda_kv_pages {
     int32_t   n_pages, n_layer, n_head_kv;
     int32_t   page_size;    /* 16, 32, 64 or 128 tokens */
     int32_t   n_slots, table_width;
-    int32_t   kv_type;      /* SLLM_CUDA_KV_F32 or SLLM_CUDA_KV_F16 */
+    int32_t   kv_type;      /* SLLM_CUDA_KV_F32, _F16 or _I8 */
+    float   * k_scale;      /* SLLM_CUDA_KV_I8 alone (not read otherwise): */
+    float   * v_scale;      /* [n_pages][n_layer][n_head_kv][page_size / 16], 16-byte aligned */
 } sllm_cuda_kv_pages;
+
+/*
+ * SLLM_CUDA_KV_I8: pools of int8 codes c in [-127, 127] and one scale s for 16
+ * tokens of a head (tokens 16 b .. 16 b + 15 of a sequence, a block); a value is
+ * c * s. sllm_cuda_kv8_append writes such a cache, sllm_cuda_kv8_read reads it back,
+ * sllm_cuda_attn_kv8 attends over it; kv_fork, kv_reserve, kv_release and kv_compact
+ * take it as they take the others. kv_append and attn_prefix refuse it.
+ */
 
 /* Bytes of the workspace that the four calls below take; 0 for a bad cache. */
 SLLM_CUDA_API size_t sllm_cuda_kv_work_bytes(const sllm_cuda_kv_pages * p);
@@ -360,6 +371,89 @@ SLLM_CUDA_API int sllm_cuda_attn_prefix(const sllm_cuda_kv_pages * p, int32_t la
                                         const int32_t * slots, int32_t n, int32_t n_q, int32_t n_head,
                                         int32_t prefix_len, void * out, int32_t out_type, void * work,
                                         size_t work_bytes, int32_t * status, void * stream);
+
+/*
+ * Stores the K and V of n_tokens tokens in one layer of an 8-bit cache, rotated
+ * and placed as kv_append does it. A block's scale is the largest |value| that was
+ * stored in it, divided by 127 (at least 2^-100; 0 while all are 0), and a code is
+ * value / scale rounded to the nearest, ties to even. Where a token needs a larger
+ * scale, the codes of the block's earlier tokens (the rows before the first that
+ * this call stores there) are rounded to it: each such step costs them up to half
+ * a step of the new scale. Rows behind the last token stored mean nothing
+ * afterwards, so tokens go in ascending order of their positions, and a position
+ * may be stored again after kv_release. The call's tokens of one block
+ * stand together in its lists, in ascending order; one that does not come after
+ * the token before it of the same block sets SLLM_CUDA_ERR_ARG in *status and is
+ * left out of the cache. A block that the lists come back to later leaves a mix
+ * of both. A NaN is stored as 0, an infinity as 127 times the scale of the finite
+ * values, both with SLLM_CUDA_ERR_ARG in *status.
+ * q_out [n_tokens][n_head][128] and k_out, v_out [n_tokens][n_head_kv][128], of
+ * type out_type, receive the rotated q, k and v before quantisation (k_out and
+ * v_out may be NULL; q and q_out may both be NULL). Padding, wrong tokens and
+ * strides as in kv_append.
+ */
+SLLM_CUDA_API int sllm_cuda_kv8_append(const sllm_cuda_kv_pages * p, int32_t layer, int32_t n_tokens,
+                                       const int32_t * slot, const int32_t * pos, int32_t n_head,
+                                       const float * q, size_t q_stride, const float * k, size_t k_stride,
+                                       const float * v, size_t v_stride, const float * rope_cos,
+                                       const float * rope_sin, int32_t n_ctx, void * q_out, void * k_out,
+                                       void * v_out, int32_t out_type, int32_t * status, void * stream);
+
+/*
+ * Reads n_tokens tokens of one layer of an 8-bit cache back: k_out[t], v_out[t]
+ * ([n_head_kv][128] each, of type out_type; either may be NULL) are the stored
+ * values of position pos[t] of slot slot[t], in any order, rounded once to
+ * out_type. A token with slot[t] < 0 is padding, and its rows are left as they
+ * are; so are those of a token whose slot, position or page is wrong, which sets
+ * SLLM_CUDA_ERR_ARG in *status. n_tokens <= 2^24.
+ */
+SLLM_CUDA_API int sllm_cuda_kv8_read(const sllm_cuda_kv_pages * p, int32_t layer, int32_t n_tokens,
+                                     const int32_t * slot, const int32_t * pos, void * k_out, void * v_out,
+                                     int32_t out_type, int32_t * status, void * stream);
+
+/*
+ * Decode attention of n sequences over an 8-bit cache: attn_prefix without a
+ * shared prefix. Sequence b's n_q query tokens are the last n_q tokens of
+ * slots[b]; query j sees the slot's first lens - n_q + 1 + j tokens (zeros come
+ * out where that is none). q and out are [n][n_q][n_head][128]; q is of type
+ * q_type, out f32 or, from f16 queries, f16. Codes are multiplied on the tensor
+ * cores exactly, in f32 sums; f16 queries are taken as they are, f32 queries and
+ * their softmax weights as pairs of f16 (22 bits), the weights of f16 queries
+ * rounded to f16 (against the running maximum: 11 bits down to 2^-20 of a row's
+ * largest). A sequence whose slot, length or table is wrong sets
+ * SLLM_CUDA_ERR_ARG in *status, and its rows of out mean nothing. n <= 4096, n_q
+ * <= 16, n_head <= 1024. A workspace of work_bytes(n, n_q, n_head) serves every
+ * call over this cache with that n_head and no more sequences and query tokens.
+ */
+SLLM_CUDA_API size_t sllm_cuda_attn_kv8_work_bytes(const sllm_cuda_kv_pages * p, int32_t n, int32_t n_q,
+                                                   int32_t n_head);
+SLLM_CUDA_API int sllm_cuda_attn_kv8(const sllm_cuda_kv_pages * p, int32_t layer, const void * q, int32_t q_type,
+                                     const int32_t * slots, int32_t n, int32_t n_q, int32_t n_head, void * out,
+                                     int32_t out_type, void * work, size_t work_bytes, int32_t * status,
+                                     void * stream);
+
+/*
+ * One step of n beam searches of `beams` beams each. Request i's candidates are
+ * (b, x): beam b continued by word x, of value
+ *     score[i][b] + logits[i][b][x] - ln sum_y exp(logits[i][b][y])
+ * (64 bits; the exponentials 32, their sum 64); a beam with done[i][b] != 0 has
+ * one candidate, eos, of its own score (done NULL: none is). The `beams` best come out
+ * in descending order: parent, token and score_out [n][beams]. Equal values: the
+ * lower beam first, then the larger logit, then the lower word. Row (i, b) of the logits lies
+ * at logits + (i * beams + b) * row_stride. A score or logit of -inf makes
+ * candidates of value -inf, which are chosen, lowest (b, x) first, only when
+ * there are no others; NaN and +inf count as -inf and set SLLM_CUDA_ERR_ARG in
+ * *status. done_out[i][j] (may be NULL) is 1 when the parent was done or the
+ * token is eos. src[i][j] = slots[i][parent[i][j]] (both NULL or neither): with them
+ * sllm_cuda_kv_fork(src, dst = slots) lets every beam's slot hold its parent's
+ * tokens. eos < 0: no such word (then done and done_out must be NULL). The outputs may
+ * not overlap score or done. beams <= 16, n <= 65536, n_vocab <= 2^20.
+ */
+SLLM_CUDA_API int sllm_cuda_beam_select(const float * logits, size_t row_stride, const float * score,
+                                        const int32_t * done, const int32_t * slots, int32_t n, int32_t beams,
+                                        int32_t n_vocab, int32_t eos, float * score_out, int32_t * parent,
+                                        int32_t * token, int32_t * done_out, int32_t * src, int32_t * status,
+                                        void * stream);
 
 /*
  * Verification of drafted tokens, so that what comes out is distributed as

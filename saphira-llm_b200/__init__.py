@@ -138,6 +138,12 @@ def lib():
     L.sllm_cuda_attn_prefix_work_bytes.argtypes = [pg, i32, i32, i32, i32]
     L.sllm_cuda_attn_prefix_work_bytes.restype = sz
     L.sllm_cuda_attn_prefix.argtypes = [pg, i32, vp, vp, i32, i32, i32, i32, vp, i32, vp, sz, vp, vp]
+    L.sllm_cuda_kv8_append.argtypes = L.sllm_cuda_kv_append.argtypes[:-2] + [i32, vp, vp]
+    L.sllm_cuda_kv8_read.argtypes = [pg, i32, i32, vp, vp, vp, vp, i32, vp, vp]
+    L.sllm_cuda_attn_kv8_work_bytes.argtypes = [pg, i32, i32, i32]
+    L.sllm_cuda_attn_kv8_work_bytes.restype = sz
+    L.sllm_cuda_attn_kv8.argtypes = [pg, i32, vp, i32, vp, i32, i32, i32, vp, i32, vp, sz, vp, vp]
+    L.sllm_cuda_beam_select.argtypes = [vp, sz, vp, vp, vp, i32, i32, i32, i32, vp, vp, vp, vp, vp, vp, vp]
     L.sllm_cuda_spec_verify.argtypes = [vp, vp, vp, vp, vp, vp, i32, i32, i32, vp, vp, vp, vp]
     _lib = L
     return L
@@ -260,7 +266,7 @@ def _kind(dtype):
     kind = _DTYPES.get(dtype)
     if kind is None:
         name = str(dtype).rpartition(".")[2]
-        kind = _DTYPES[dtype] = {"float32": "f32", "float16": "f16", "int32": "i32"}.get(name, "")
+        kind = _DTYPES[dtype] = {"float32": "f32", "float16": "f16", "int32": "i32", "int8": "i8"}.get(name, "")
     return kind
 
 
@@ -330,21 +336,30 @@ def rope_table(n_ctx, base):
 
 class KvPages:
     """A paged KV cache over the caller's tensors (sllm_cuda_kv_pages): k, v
-    [pages][layers][kv heads][page size][128] float32 or float16, refs int32
-    [pages], tables int32 [slots][width], lens int32 [slots]. The tensors are
-    kept, not copied."""
+    [pages][layers][kv heads][page size][128] float32, float16 or int8, refs
+    int32 [pages], tables int32 [slots][width], lens int32 [slots]; with int8,
+    k_scale and v_scale float32 [pages][layers][kv heads][page size / 16]. The
+    tensors are kept, not copied."""
 
-    def __init__(self, k, v, refs, tables, lens):
+    def __init__(self, k, v, refs, tables, lens, k_scale=None, v_scale=None):
         w = "KvPages"
         if not (k.dim() == 5 and k.shape == v.shape and k.shape[4] == abi.HEAD_DIM and k.is_contiguous() and
-                v.is_contiguous() and _type(k) == _type(v)):
+                v.is_contiguous() and k.dtype == v.dtype):
             raise ValueError("KvPages: k and v must be [pages][layers][heads][size][128]")
+        kv_type = abi.KV_I8 if _kind(k.dtype) == "i8" else _type(k)
+        if (kv_type == abi.KV_I8) != (k_scale is not None) or (k_scale is None) != (v_scale is None):
+            raise ValueError("KvPages: int8 pools, and they alone, have k_scale and v_scale")
+        for t in (k_scale, v_scale):
+            if t is not None and not (tuple(t.shape) == tuple(k.shape[:3]) + (k.shape[3] // abi.KV_BLOCK,) and
+                                      t.is_contiguous() and _kind(t.dtype) == "f32"):
+                raise ValueError("KvPages: scales must be contiguous float32 [pages][layers][heads][size / 16]")
         if not (tables.dim() == 2 and tables.shape[0] == lens.numel() and refs.numel() == k.shape[0]):
             raise ValueError("KvPages: refs, tables and lens must match the pools and each other")
-        self._keep = (k, v, refs, tables, lens)
+        self._keep = (k, v, refs, tables, lens, k_scale, v_scale)
         self.c = abi.KvPages(k.data_ptr(), v.data_ptr(), _ints(refs, refs.numel(), w, "refs"),
                              _ints(tables, tables.numel(), w, "tables"), _ints(lens, lens.numel(), w, "lens"),
-                             k.shape[0], k.shape[1], k.shape[2], k.shape[3], tables.shape[0], tables.shape[1], _type(k))
+                             k.shape[0], k.shape[1], k.shape[2], k.shape[3], tables.shape[0], tables.shape[1], kv_type,
+                             _ptr(k_scale), _ptr(v_scale))
         self._p = C.byref(self.c)
         self._kv_type, self._kv_heads = self.c.kv_type, self.c.n_head_kv
 
@@ -389,37 +404,87 @@ class KvPages:
         if rc:
             _check(rc, "kv_compact")
 
-    def _out(self, t, n, h):
-        if t.shape != (n, h, abi.HEAD_DIM) or not t.is_contiguous() or _type(t) != self._kv_type:
-            raise ValueError("kv_append: outputs must be contiguous, of the cache's type")
+    def _out(self, t, n, h, kind, w):
+        if t.shape != (n, h, abi.HEAD_DIM) or not t.is_contiguous() or _type(t) != kind:
+            raise ValueError(f"{w}: outputs must be contiguous [tokens][heads][128], of the cache's type (8 bits: of one)")
         return t.data_ptr()
 
     def append(self, layer, slot, pos, q, k, v, cos, sin, q_out=None, k_out=None, v_out=None, status=None,
                stream=None):
-        w = "kv_append"
+        """sllm_cuda_kv_append: q [tokens][heads][128], k, v [tokens][kv heads][128] float32, cos and sin
+        [positions][64]; the outputs are contiguous and of the cache's type."""
+        self._append("kv_append", layer, slot, pos, q, k, v, cos, sin, q_out, k_out, v_out, status, stream)
+
+    def append8(self, layer, slot, pos, q, k, v, cos, sin, q_out=None, k_out=None, v_out=None, status=None,
+                stream=None):
+        """sllm_cuda_kv8_append, likewise; the outputs are all float32 or all float16."""
+        self._append("kv8_append", layer, slot, pos, q, k, v, cos, sin, q_out, k_out, v_out, status, stream)
+
+    def _append(self, w, layer, slot, pos, q, k, v, cos, sin, q_out, k_out, v_out, status, stream):
+        eight = w == "kv8_append"
+        kind = self._kv_type
+        if eight:
+            out = q_out if q_out is not None else k_out if k_out is not None else v_out
+            kind = abi.KV_F32 if out is None else _type(out)
         kp, ks, n, hk = _heads(k, w, "k")
         vp, vs, nv, hv = _heads(v, w, "v")
         qp, qs, nq, h = _heads(q, w, "q") if q is not None else (None, 0, n, 0)
         if not (n == nv == nq and hk == hv == self._kv_heads):
-            raise ValueError("kv_append: q, k, v disagree in tokens, or with the cache's heads")
+            raise ValueError(f"{w}: q, k, v disagree in tokens, or with the cache's heads")
         if (q is None) != (q_out is None):
-            raise ValueError("kv_append: q and q_out go together")
+            raise ValueError(f"{w}: q and q_out go together")
         f32 = k.dtype
         if _kind(f32) != "f32" or v.dtype != f32 or cos.dtype != f32 or sin.dtype != f32 or (
                 q is not None and q.dtype != f32):
-            raise ValueError("kv_append: q, k, v, cos and sin must be float32")
-        qo = None if q_out is None else self._out(q_out, n, h)
-        ko = None if k_out is None else self._out(k_out, n, hk)
-        vo = None if v_out is None else self._out(v_out, n, hk)
+            raise ValueError(f"{w}: q, k, v, cos and sin must be float32")
+        qo = None if q_out is None else self._out(q_out, n, h, kind, w)
+        ko = None if k_out is None else self._out(k_out, n, hk, kind, w)
+        vo = None if v_out is None else self._out(v_out, n, hk, kind, w)
         shape = cos.shape
         if not (len(shape) == 2 and shape[1] == 64 and sin.shape == shape and cos.is_contiguous() and
                 sin.is_contiguous()):
-            raise ValueError("kv_append: cos and sin must be [positions][64]")
+            raise ValueError(f"{w}: cos and sin must be [positions][64]")
         if n == 0:
             return
-        rc = lib().sllm_cuda_kv_append(self._p, layer, n, _ints(slot, n, w, "slot"), _ints(pos, n, w, "pos"), h, qp, qs,
-                                       kp, ks, vp, vs, cos.data_ptr(), sin.data_ptr(), shape[0], qo, ko, vo,
-                                       _ints(status, 1, w, "status"), _stream(stream))
+        args = (self._p, layer, n, _ints(slot, n, w, "slot"), _ints(pos, n, w, "pos"), h, qp, qs, kp, ks, vp, vs,
+                cos.data_ptr(), sin.data_ptr(), shape[0], qo, ko, vo)
+        tail = (_ints(status, 1, w, "status"), _stream(stream))
+        rc = lib().sllm_cuda_kv8_append(*args, kind, *tail) if eight else lib().sllm_cuda_kv_append(*args, *tail)
+        if rc:
+            _check(rc, w)
+
+    def read8(self, layer, slot, pos, k_out=None, v_out=None, status=None, stream=None):
+        """sllm_cuda_kv8_read: k_out, v_out contiguous [tokens][kv heads][128], float32 or float16 (either may
+        be None)."""
+        w = "kv8_read"
+        n, out = slot.numel(), k_out if k_out is not None else v_out
+        if out is None:
+            raise ValueError("kv8_read: nothing to write to")
+        kind = _type(out)
+        ko = None if k_out is None else self._out(k_out, n, self._kv_heads, kind, w)
+        vo = None if v_out is None else self._out(v_out, n, self._kv_heads, kind, w)
+        if n == 0:
+            return
+        rc = lib().sllm_cuda_kv8_read(self._p, layer, n, _ints(slot, n, w, "slot"), _ints(pos, n, w, "pos"), ko, vo, kind,
+                                      _ints(status, 1, w, "status"), _stream(stream))
+        if rc:
+            _check(rc, w)
+
+    def attn8_work_bytes(self, n, n_q, n_head):
+        return self._bytes(lib().sllm_cuda_attn_kv8_work_bytes(self._p, n, n_q, n_head), "attn_kv8_work_bytes")
+
+    def attn8(self, layer, q, out, slots, work, status=None, stream=None):
+        """sllm_cuda_attn_kv8: q, out [sequences][query tokens][heads][128], float32 or float16."""
+        w, shape = "attn_kv8", q.shape
+        if not (len(shape) == 4 and shape == out.shape and shape[3] == abi.HEAD_DIM and q.is_contiguous() and
+                out.is_contiguous()):
+            raise ValueError("attn_kv8: q and out must be contiguous [sequences][query tokens][heads][128]")
+        n, nq, h, _ = shape
+        if n == 0:
+            return
+        rc = lib().sllm_cuda_attn_kv8(self._p, layer, q.data_ptr(), _type(q), _ints(slots, n, w, "slots"), n, nq, h,
+                                      out.data_ptr(), _type(out), work.data_ptr(), work.nbytes,
+                                      _ints(status, 1, w, "status"), _stream(stream))
         if rc:
             _check(rc, w)
 
@@ -464,6 +529,35 @@ def spec_verify(p, q, draft, n_draft, u_accept, u_draw, tokens, count, status=No
     rc = lib().sllm_cuda_spec_verify(p.data_ptr(), None if q is None else q.data_ptr(), _ints(draft, n * k, w, "draft"),
                                      _ints(n_draft, n, w, "n_draft"), u_accept.data_ptr(), u_draw.data_ptr(), n, k, nv,
                                      _ints(tokens, n * (k + 1), w, "tokens"), _ints(count, n, w, "count"),
+                                     _ints(status, 1, w, "status"), _stream(stream))
+    if rc:
+        _check(rc, w)
+
+
+def beam_select(logits, score, score_out, parent, token, done=None, eos=-1, done_out=None, slots=None, src=None,
+                status=None, stream=None):
+    """sllm_cuda_beam_select: logits float32 [requests][beams][vocab] (rows may lie apart), score and score_out
+    float32, parent, token, done, done_out, slots and src int32 [requests][beams]."""
+    w, shape = "beam_select", logits.shape
+    if len(shape) != 3 or _kind(logits.dtype) != "f32":
+        raise ValueError("beam_select: logits must be float32 [requests][beams][vocab]")
+    n, b, nv = shape
+    s0, s1, s2 = logits.stride()
+    if b > 1:
+        row = s1
+    else:
+        row = s0 if n > 1 else nv
+    if n > 0 and ((nv > 1 and s2 != 1) or (n > 1 and s0 != b * row)):
+        raise ValueError("beam_select: the rows of the logits must be evenly apart")
+    for t in (score, score_out):
+        if not (t.is_contiguous() and t.numel() == n * b and _kind(t.dtype) == "f32"):
+            raise ValueError("beam_select: score and score_out must be float32 [requests][beams]")
+    if n == 0:
+        return
+    rc = lib().sllm_cuda_beam_select(logits.data_ptr(), row, score.data_ptr(), _ints(done, n * b, w, "done"),
+                                     _ints(slots, n * b, w, "slots"), n, b, nv, eos, score_out.data_ptr(),
+                                     _ints(parent, n * b, w, "parent"), _ints(token, n * b, w, "token"),
+                                     _ints(done_out, n * b, w, "done_out"), _ints(src, n * b, w, "src"),
                                      _ints(status, 1, w, "status"), _stream(stream))
     if rc:
         _check(rc, w)

@@ -69,10 +69,12 @@ class KvPages(C.Structure):
         ("refs", C.c_void_p), ("tables", C.c_void_p), ("lens", C.c_void_p),
         ("n_pages", C.c_int32), ("n_layer", C.c_int32), ("n_head_kv", C.c_int32), ("page_size", C.c_int32),
         ("n_slots", C.c_int32), ("table_width", C.c_int32), ("kv_type", C.c_int32),
+        ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
     ]
 
 
-KV_F32, KV_F16 = 0, 1
+KV_F32, KV_F16, KV_I8 = 0, 1, 2
+KV_BLOCK = 16           # tokens that share a scale of an 8-bit cache
 HEAD_DIM = 128
 
 TP_ID_BYTES = 128

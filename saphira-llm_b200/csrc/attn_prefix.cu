@@ -535,7 +535,7 @@ cudaError_t launch_32(const PagesDev& pg, const PrefixParams& p, cudaStream_t st
 }
 
 int check_shape(const sllm_cuda_kv_pages* p, int n, int n_q, int n_head, int prefix, const char* who) {
-    const int rc = check_pages(p, who);
+    const int rc = check_pages(p, who, false);
     if (rc != SLLM_CUDA_OK) return rc;
     if (n < 0 || n > 4096 || n_q < 1 || n_q > 16 || n_head < 1 || n_head > 1024 || n_head % p->n_head_kv != 0 ||
         prefix < 0 || prefix % p->page_size != 0 || prefix / p->page_size > p->table_width)

@@ -492,12 +492,14 @@ kv_compact_kernel(const PagesDev p, void* work, int32_t* status) {
 // ---------------------------------------------------------------------------
 // the copies: one warp per run of rows (a page's rows of one layer and kv
 // head are contiguous), 4 KB in flight per warp. Only the rows a copy names
-// move. For compact the same launch rewrites the tables. Bound by HBM: 48 slots
+// move (and of an 8-bit cache the scales of their blocks). For compact the same
+// launch rewrites the tables. Bound by HBM: 48 slots
 // of up to 200 tokens, 30 layers and 1024 pages of f16 compacted in 90 us, 5.6
 // TB/s of reads and writes, the bookkeeping before it included.
 // ---------------------------------------------------------------------------
 __global__ void __launch_bounds__(256)
-kv_copy_kernel(const PagesDev p, uint8_t* k, uint8_t* v, int runs, int row_bytes, void* work, int remap) {
+kv_copy_kernel(const PagesDev p, uint8_t* k, uint8_t* v, float* ks, float* vs, int runs, int row_bytes, void* work,
+               int remap) {
     pdl_wait();
     const Work w = work_of(work, p.n_pages, p.n_slots, p.width);
     const int count = *w.count;
@@ -523,6 +525,11 @@ kv_copy_kernel(const PagesDev p, uint8_t* k, uint8_t* v, int runs, int row_bytes
             #pragma unroll
             for (int j = 0; j < 8; ++j)
                 if (x + 32 * j < nv) __stcs(b + x + 32 * j, r8[j]);
+        }
+        if (ks != nullptr && lane < (m.z + kKvBlock - 1) / kKvBlock) {
+            float* const sc = (r < runs ? ks : vs) + (size_t)(r < runs ? r : r - runs) * (p.page / kKvBlock) + lane;
+            const size_t page = (size_t)runs * (p.page / kKvBlock);
+            sc[(size_t)m.y * page] = sc[(size_t)m.x * page];
         }
     }
     if (remap) {
@@ -638,9 +645,12 @@ int check_call(const sllm_cuda_kv_pages* p, const char* who, int n, const void* 
     if (work == nullptr || !aligned16(work) || work_bytes < sllm_cuda_kv_work_bytes(p))
         return fail(SLLM_CUDA_ERR_ARG, "%s: workspace of %zu bytes, %zu needed, 16-byte aligned", who, work_bytes,
                     sllm_cuda_kv_work_bytes(p));
-    const void* ptr[] = {p->k, p->v, p->refs, p->tables, p->lens, work, a, b, status};
-    const char* name[] = {"k", "v", "refs", "tables", "lens", "work", "slots", "slots or lengths", "status"};
-    for (int i = 0; i < 9; ++i)
+    const bool eight = p->kv_type == SLLM_CUDA_KV_I8;
+    const void* ptr[] = {p->k, p->v, p->refs, p->tables, p->lens, work, a, b, status, eight ? p->k_scale : nullptr,
+                         eight ? p->v_scale : nullptr};
+    const char* name[] = {"k", "v", "refs", "tables", "lens", "work", "slots", "slots or lengths", "status", "k_scale",
+                          "v_scale"};
+    for (int i = 0; i < 11; ++i)
         if (ptr[i] != nullptr && (rc = need_device(ptr[i], who, name[i])) != SLLM_CUDA_OK) return rc;
     return SLLM_CUDA_OK;
 }
@@ -650,7 +660,8 @@ cudaError_t launch_copies(const sllm_cuda_kv_pages& p, long long most, void* wor
     const long long units = most * 2 * runs + (remap ? p.n_slots : 0);
     const long long blocks = (units + 7) / 8, cap = 8LL * current_sms();
     return launch(kv_copy_kernel, dim3((unsigned)(blocks < 1 ? 1 : blocks < cap ? blocks : cap)), dim3(256), 0, st, true,
-                  pages_dev(p), static_cast<uint8_t*>(p.k), static_cast<uint8_t*>(p.v), runs,
+                  pages_dev(p), static_cast<uint8_t*>(p.k), static_cast<uint8_t*>(p.v),
+                  p.kv_type == SLLM_CUDA_KV_I8 ? p.k_scale : nullptr, p.kv_type == SLLM_CUDA_KV_I8 ? p.v_scale : nullptr, runs,
                   (int)(kServeDim * kv_elt_bytes(p.kv_type)), work, remap);
 }
 
@@ -689,8 +700,11 @@ int check_pages(const sllm_cuda_kv_pages* p, const char* who) {
     if (p == nullptr || p->k == nullptr || p->v == nullptr || p->refs == nullptr || p->tables == nullptr ||
         p->lens == nullptr)
         return fail(SLLM_CUDA_ERR_ARG, "%s: a NULL cache or array", who);
-    if (p->kv_type != SLLM_CUDA_KV_F32 && p->kv_type != SLLM_CUDA_KV_F16)
+    if (p->kv_type != SLLM_CUDA_KV_F32 && p->kv_type != SLLM_CUDA_KV_F16 && p->kv_type != SLLM_CUDA_KV_I8)
         return fail(SLLM_CUDA_ERR_ARG, "%s: unknown cache type %d", who, p->kv_type);
+    if (p->kv_type == SLLM_CUDA_KV_I8 && (p->k_scale == nullptr || p->v_scale == nullptr || !aligned16(p->k_scale) ||
+                                          !aligned16(p->v_scale)))
+        return fail(SLLM_CUDA_ERR_ARG, "%s: an 8-bit cache needs k_scale and v_scale, 16-byte aligned", who);
     if (p->page_size != 16 && p->page_size != 32 && p->page_size != 64 && p->page_size != 128)
         return fail(SLLM_CUDA_ERR_UNSUPPORTED, "%s: pages of %d tokens (16, 32, 64 or 128)", who, p->page_size);
     if (p->n_pages < 1 || p->n_pages > (1 << 24) || p->n_layer < 1 || p->n_layer > 1024 || p->n_head_kv < 1 ||
@@ -702,6 +716,13 @@ int check_pages(const sllm_cuda_kv_pages* p, const char* who) {
     if (!aligned16(p->k) || !aligned16(p->v) || !aligned16(p->refs))
         return fail(SLLM_CUDA_ERR_ARG, "%s: k, v and refs must be 16-byte aligned", who);
     return SLLM_CUDA_OK;
+}
+
+int check_pages(const sllm_cuda_kv_pages* p, const char* who, bool eight) {
+    const int rc = check_pages(p, who);
+    if (rc != SLLM_CUDA_OK || (p->kv_type == SLLM_CUDA_KV_I8) == eight) return rc;
+    return fail(SLLM_CUDA_ERR_ARG, eight ? "%s: takes an 8-bit cache" : "%s: does not take an 8-bit cache (kv8_append, kv8_read, "
+                                                                       "attn_kv8 do)", who);
 }
 
 }  // namespace sllm
@@ -774,7 +795,7 @@ extern "C" int sllm_cuda_kv_append(const sllm_cuda_kv_pages* p, int32_t layer, i
                                    const float* k, size_t k_stride, const float* v, size_t v_stride,
                                    const float* rope_cos, const float* rope_sin, int32_t n_ctx, void* q_out,
                                    void* k_out, void* v_out, int32_t* status, void* stream) {
-    int rc = check_pages(p, "kv_append");
+    int rc = check_pages(p, "kv_append", false);
     if (rc != SLLM_CUDA_OK) return rc;
     if (slot == nullptr || pos == nullptr || k == nullptr || v == nullptr || rope_cos == nullptr ||
         rope_sin == nullptr || (q == nullptr) != (q_out == nullptr))

@@ -1,5 +1,5 @@
-// serve.cuh -- shared by the serving operators' files (kv_pages.cu,
-// attn_prompt.cu, attn_prefix.cu, spec_verify.cu): argument checks, the
+// serve.cuh -- shared by the serving operators' files (kv_pages.cu, kv8.cu,
+// attn_prompt.cu, attn_prefix.cu, attn_kv8.cu, spec_verify.cu, beam_select.cu): argument checks, the
 // device's view of a paged cache, launches.
 #pragma once
 
@@ -19,8 +19,10 @@ constexpr float kServeScale = 0.08838834764831845f;     // 1 / sqrt(128)
 // another device's would fault); the message names the argument.
 int need_device(const void* p, const char* who, const char* arg);
 
-// the fields of a sllm_cuda_kv_pages, checked (no device call)
+// the fields of a sllm_cuda_kv_pages, checked (no device call); and whether its
+// values are 8-bit codes or not, as the caller takes them
 int check_pages(const sllm_cuda_kv_pages* p, const char* who);
+int check_pages(const sllm_cuda_kv_pages* p, const char* who, bool eight);
 
 // the error words of the attention kernels' bounded waits, read and cleared
 int take_prompt_error();
@@ -66,7 +68,9 @@ inline PagesDev pages_dev(const sllm_cuda_kv_pages& p) {
                     p.table_width * p.page_size};
 }
 
-inline size_t kv_elt_bytes(int type) { return type == SLLM_CUDA_KV_F16 ? 2 : 4; }
+inline size_t kv_elt_bytes(int type) { return type == SLLM_CUDA_KV_I8 ? 1 : type == SLLM_CUDA_KV_F16 ? 2 : 4; }
+
+constexpr int kKvBlock = 16;        // tokens that share a scale of an 8-bit cache
 
 // sets *status (nullable) to an error; it is never cleared here
 __device__ __forceinline__ void raise(int32_t* status, int code) {

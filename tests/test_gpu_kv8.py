@@ -1,0 +1,517 @@
+"""The 8-bit paged cache on a GPU: stores, reading back, attention, and the page
+operations over it, against plain restatements (kv8_ref.py, serving_ref.py).
+Codes and scales have to be equal; attention's tolerance is derived below."""
+import math
+
+import numpy as np
+import pytest
+
+from kv8_ref import BLOCK, Cache8
+from serving_ref import PageModel, attention, attention_bound
+
+pytestmark = pytest.mark.gpu
+
+
+def _dt(name):
+    import torch
+    return {"f32": torch.float32, "f16": torch.float16}[name]
+
+
+def _i32(a):
+    import torch
+    return torch.tensor(a, dtype=torch.int32, device="cuda")
+
+
+def _t(a):
+    import torch
+    return torch.from_numpy(np.ascontiguousarray(a)).cuda()
+
+
+class Eight:
+    """A cache on the device beside its host model."""
+
+    def __init__(self, cuda, pages, slots, width, page, layers, heads, seed=None):
+        import torch
+        self.cuda, self.m = cuda, PageModel(pages, slots, width, page)
+        self.host = Cache8(pages, layers, heads, page, seed)
+        self.k, self.v = (_t(x) for x in self.host.codes)
+        self.ks, self.vs = (_t(x) for x in self.host.scales)
+        self.refs, self.lens = _i32([0] * pages), _i32([0] * slots)
+        self.tables = _i32(self.m.tables)
+        self.p = cuda.KvPages(self.k, self.v, self.refs, self.tables, self.lens, self.ks, self.vs)
+        self.work = torch.empty(self.p.work_bytes(), dtype=torch.uint8, device="cuda")
+        self.status = torch.zeros(1, dtype=torch.int32, device="cuda")
+
+    def take_status(self):
+        v = int(self.status.item())
+        self.status.zero_()
+        return v
+
+    def reserve(self, slots, new):
+        self.p.reserve(_i32(slots), _i32(new), self.work, self.status)
+        want, copies = self.m.reserve(slots, new)
+        for a, b, rows in copies:
+            self.copy(a, b, rows)
+        return want
+
+    def copy(self, a, b, rows):
+        for c, s in zip(self.host.codes, self.host.scales):
+            c[b, :, :, :rows] = c[a, :, :, :rows]
+            blocks = -(-rows // BLOCK)
+            s[b, :, :, :blocks] = s[a, :, :, :blocks]
+
+    def place(self, lens, seed=0):
+        """Slots of these lengths, in pages of no order."""
+        r = np.random.default_rng(seed)
+        ids = r.permutation(self.m.n_pages).tolist()
+        for s, n in enumerate(lens):
+            for j in range(self.m.used(n)):
+                p = ids.pop()
+                self.m.tables[s][j] = p
+                self.m.refs[p] = 1
+            self.m.lens[s] = n
+        self.refs.copy_(_i32(self.m.refs))
+        self.tables.copy_(_i32(self.m.tables))
+        self.lens.copy_(_i32(self.m.lens))
+
+    def same(self):
+        got = [x.cpu().numpy() for x in (self.k, self.v, self.ks, self.vs)]
+        want = self.host.codes + self.host.scales
+        return [bool(np.array_equal(a, b)) for a, b in zip(got, want)]
+
+
+def _angles(n):
+    ang = np.arange(n)[:, None] * (500000.0 ** (-np.arange(64) / 64))[None]
+    return np.cos(ang).astype(np.float32), np.sin(ang).astype(np.float32)
+
+
+# ---------------------------------------------------------------------------
+# append
+# ---------------------------------------------------------------------------
+def _random_call(r, c, S, n_ctx):
+    """Lists for one call: runs of several slots, some of them padded, wrong or out of order."""
+    slot, pos = [], []
+    for s in r.permutation(S):
+        n = int(r.integers(0, 40))
+        a = int(r.integers(0, max(1, c.m.lens[s] + 6)))
+        slot += [int(s)] * n
+        pos += list(range(a, a + n))
+        if r.random() < 0.3:
+            slot += [-1] * int(r.integers(1, 4))
+            pos += [5] * (len(slot) - len(pos))
+    if slot and r.random() < 0.5:                            # (between slots: a block's tokens stay together)
+        i = int(r.choice([0] + [j for j in range(1, len(slot)) if slot[j] != slot[j - 1]]))
+        slot.insert(i, S + 3)
+        pos.insert(i, 0)
+    if len(slot) > 3 and r.random() < 0.5:                   # one token twice, one position negative
+        i = int(r.integers(len(slot)))
+        slot.insert(i, slot[i])
+        pos.insert(i, pos[i])
+        slot.append(0)
+        pos.append(-3)
+    return slot, pos
+
+
+@pytest.mark.parametrize("page", [16, 32, 64, 128])
+@pytest.mark.parametrize("heads,layers", [((4, 4), 1), ((5, 1), 2), ((20, 5), 1), ((16, 2), 3)])
+@pytest.mark.parametrize("out", ["f32", "f16"])
+def test_append8(cuda, page, heads, layers, out):
+    """Several calls on one cache: blocks begun, gone on with, grown and written again; tokens out of order,
+    wrong ones and padding among them. Codes and scales are equal to the definition's, whole pools."""
+    import torch
+    H, Hkv = heads
+    S, n_ctx = 5, 150
+    c = Eight(cuda, 60, S, -(-160 // page) + 1, page, layers, Hkv, seed=3)
+    c.place([37, 150, 0, 64, 15], seed=page)
+    cos, sin = _angles(n_ctx)
+    r = np.random.default_rng(page + H)
+    for step in range(6):
+        layer = int(r.integers(layers))
+        slot, pos = _random_call(r, c, S, n_ctx)
+        T = len(slot)
+        qkv = r.standard_normal((T, H + 2 * Hkv, 128)).astype(np.float32)
+        qkv *= np.exp(r.normal(0, 1, (T, 1, 1))).astype(np.float32)
+        d = _t(qkv)
+        q, k, v = d[:, :H], d[:, H:H + Hkv], d[:, H + Hkv:]
+        qo = torch.full((T, H, 128), 7.0, dtype=_dt(out), device="cuda")
+        ko, vo = (torch.full((T, Hkv, 128), 7.0, dtype=_dt(out), device="cuda") for _ in range(2))
+        c.p.append8(layer, _i32(slot), _i32(pos), q, k, v, _t(cos), _t(sin), qo, ko, vo, c.status)
+        torch.cuda.synchronize()
+        bad, left = c.host.append(layer, c.m.tables, c.m.lens, c.m.refs, slot, pos, qkv[:, H:H + Hkv], qkv[:, H + Hkv:],
+                                  cos, sin)
+        assert c.take_status() == (-1 if bad else 0)
+        assert all(c.same()), (step, c.same())
+        for t in range(T):
+            if slot[t] < 0:
+                assert bool((qo[t] == 7).all() and (ko[t] == 7).all() and (vo[t] == 7).all())
+            elif t not in left:
+                from kv8_ref import rope
+                for got, x, rot in ((qo, qkv[t, :H], True), (ko, qkv[t, H:H + Hkv], True), (vo, qkv[t, H + Hkv:], False)):
+                    want = rope(x, cos[pos[t]], sin[pos[t]]) if rot else x
+                    assert np.array_equal(got[t].cpu().numpy(), want.astype(got[t].cpu().numpy().dtype))
+
+
+def test_append8_odd_values(cuda):
+    """Zeros, values too small or large for an ordinary scale, NaN and infinities."""
+    import torch
+    c = Eight(cuda, 6, 1, 6, 16, 1, 2, seed=1)
+    c.place([96])
+    cos, sin = np.ones((96, 64), np.float32), np.zeros((96, 64), np.float32)
+    x = np.zeros((96, 2, 128), np.float32)
+    x[16:32, 0, :5] = 1e-38                                  # below the least scale's step
+    x[16:32, 1, 7] = 3e-30
+    x[32:48, 0] = 3.3e38
+    x[32, 1, 3], x[33, 1, 4], x[34, 1, 5], x[35, 1, 6] = np.nan, np.inf, -np.inf, 2.0
+    x[48, :, 1], x[49, :, 2], x[60, :, 3] = 1e-20, 1.0, 1e30         # steps up by many orders
+    x[64, 0, 0] = np.inf                                     # nothing finite but zeros
+    x[80:] = np.random.default_rng(0).standard_normal((16, 2, 128))
+    for a in range(0, 96, 1):                                # one token at a time
+        d = _t(x[a:a + 1])
+        c.p.append8(0, _i32([0]), _i32([a]), None, d, d, _t(cos), _t(sin), status=c.status)
+        bad, _ = c.host.append(0, c.m.tables, c.m.lens, c.m.refs, [0], [a], x[a:a + 1], x[a:a + 1], cos, sin)
+        assert c.take_status() == (-1 if bad else 0), a
+    torch.cuda.synchronize()
+    assert all(c.same())
+    assert bool(torch.isfinite(c.ks).all() and torch.isfinite(c.vs).all())
+
+
+def test_append8_leaves_shared_pages_alone(cuda):
+    import torch
+    c = Eight(cuda, 8, 3, 4, 16, 1, 1, seed=1)
+    c.place([20, 0, 20])
+    c.p.fork(_i32([0]), _i32([1]), c.work, c.status)
+    c.m.fork([0], [1])
+    cos, sin = _angles(64)
+    x = np.random.default_rng(0).standard_normal((3, 1, 128)).astype(np.float32)
+    d = _t(x)
+    c.p.append8(0, _i32([0, 1, 2]), _i32([19, 19, 19]), None, d, d, _t(cos), _t(sin), status=c.status)
+    torch.cuda.synchronize()
+    bad, left = c.host.append(0, c.m.tables, c.m.lens, c.m.refs, [0, 1, 2], [19, 19, 19], x, x, cos, sin)
+    assert left == {0, 1} and c.take_status() == -1 and all(c.same())
+
+
+# ---------------------------------------------------------------------------
+# read
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("page", [16, 64, 128])
+@pytest.mark.parametrize("heads", [1, 3, 5, 8])
+@pytest.mark.parametrize("out", ["f32", "f16"])
+def test_read8(cuda, page, heads, out):
+    """Tokens in any order, twice, wrong and padded: one product and one rounding a value."""
+    import torch
+    c = Eight(cuda, 40, 4, 9, page, 2, heads, seed=heads)
+    c.place([100, 1, 0, 130], seed=2)
+    r = np.random.default_rng(5)
+    slot = r.integers(-1, 5, 300).tolist()
+    pos = r.integers(-2, 140, 300).tolist()
+    n = len(slot)
+    ok = [0 <= s < 4 and 0 <= p < c.m.lens[s] for s, p in zip(slot, pos)]
+    for which in ("kv", "k", "v"):
+        ko = torch.full((n, heads, 128), 7.0, dtype=_dt(out), device="cuda") if "k" in which else None
+        vo = torch.full((n, heads, 128), 7.0, dtype=_dt(out), device="cuda") if "v" in which else None
+        c.p.read8(1, _i32(slot), _i32(pos), ko, vo, c.status)
+        torch.cuda.synchronize()
+        assert c.take_status() == -1
+        for w, o in ((0, ko), (1, vo)):
+            if o is None:
+                continue
+            got = o.cpu().numpy()
+            for t in range(n):
+                if not ok[t]:
+                    assert (got[t] == 7).all()
+                    continue
+                pg, row = c.m.tables[slot[t]][pos[t] // page], pos[t] % page
+                want = c.host.codes[w][pg, 1, :, row].astype(np.float32) * c.host.scales[w][pg, 1, :, row // BLOCK][:, None]
+                assert np.array_equal(got[t], want.astype(got.dtype))
+
+
+# ---------------------------------------------------------------------------
+# attention
+# ---------------------------------------------------------------------------
+def attn8_bound(o, pv, big, va, n, f16, out_f16):
+    """serving_ref's bound, with the stored values as the exact inputs: code times scale is applied to sums of
+    exact products (one more unit, inside its 8), f32 queries and weights are pairs of f16, 2^-22 of each
+    lost at most: of a score 2^-22 big, so 2 * 2^-22 big of a weight, and 2^-22 of the weight itself. One half
+    as much again for the products of the second with the first."""
+    b = attention_bound(o, pv, big, va, n, f16, out_f16)
+    return b if f16 else b + 1.5 * pv * (2 * 2.0 ** -22 * big + 2.0 ** -22)
+
+
+def check_attn8(c, layer, q, out, slots, f16):
+    import torch
+    n, nq, H, _ = q.shape
+    Hkv = c.host.codes[0].shape[2]
+    for b, s in enumerate(slots):
+        L = c.m.lens[s]
+        k, v = (torch.from_numpy(c.host.values(w, layer, c.m.tables[s], L)).cuda() for w in range(2))
+        for h in range(H):
+            lim = torch.tensor([max(0, L - nq + 1 + j) for j in range(nq)], device="cuda")
+            o, pv, big, va = attention(q[b, :, h].double(), k[h * Hkv // H], v[h * Hkv // H], lim)
+            tol = attn8_bound(o, pv, big, va, L, f16, out.dtype == torch.float16)
+            err = (out[b, :, h].double() - o).abs()
+            assert bool((err <= tol).all()), (b, h, L, float((err / tol).nan_to_num(math.inf).max()))
+
+
+def run_attn8(c, layer, q, slots, odt, stream=None):
+    import torch
+    n, nq, H, _ = q.shape
+    out = torch.full(q.shape, 7.0, dtype=odt, device="cuda")
+    work = torch.empty(c.p.attn8_work_bytes(n, nq, H), dtype=torch.uint8, device="cuda")
+    c.p.attn8(layer, q, out, _i32(slots), work, c.status, stream=stream)
+    torch.cuda.synchronize()
+    return out
+
+
+def _q(seed, n, nq, H, dt, scale=1.5):
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn((n, nq, H, 128), generator=g, device="cuda") * scale).to(dt)
+
+
+# heads (query, key), query tokens, lengths
+CASES = [
+    ((1, 1), 1, [1]),
+    ((8, 1), 1, [1, 15, 16, 17, 0, 63, 64, 65]),
+    ((20, 5), 1, [300, 1, 128, 129]),
+    ((4, 4), 3, [2, 3, 4, 70]),
+    ((14, 2), 2, [127, 1, 33]),
+    ((64, 8), 1, [513, 64]),
+    ((6, 2), 16, [16, 15, 200, 1]),
+    ((32, 4), 4, [77, 4, 260]),
+    ((24, 1), 1, [190, 7]),
+    ((40, 1), 2, [100, 65, 1]),
+    ((128, 1), 1, [90, 257]),
+    ((16, 2), 16, [300, 31]),
+    ((66, 1), 3, [129, 2]),
+    ((8, 8), 1, [1500, 0, 3]),
+]
+
+
+@pytest.mark.parametrize("case", CASES, ids=str)
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("types", [("f32", "f32"), ("f16", "f16"), ("f16", "f32")])
+def test_attn8(cuda, case, page, types):
+    (H, Hkv), nq, lens = case
+    width = max(lens) // page + 2
+    c = Eight(cuda, sum(x // page + 1 for x in lens) + 9, len(lens) + 2, width, page, 2, Hkv, seed=H + nq)
+    c.place([9] + lens + [40 if width * page >= 40 else 1], seed=nq)
+    slots = np.random.default_rng(H).permutation(np.arange(1, len(lens) + 1)).tolist()
+    q = _q(H + nq, len(lens), nq, H, _dt(types[0]))
+    out = run_attn8(c, 1, q, slots, _dt(types[1]))
+    assert c.take_status() == 0
+    check_attn8(c, 1, q, out, slots, types[0] == "f16")
+    for b, s in enumerate(slots):                            # rows that see nothing are zeros
+        for j in range(nq):
+            if c.m.lens[s] - nq + 1 + j <= 0:
+                assert bool((out[b, j] == 0).all())
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16"])
+@pytest.mark.parametrize("page", [16, 128])
+def test_attn8_long_and_short(cuda, dt, page):
+    """Many sequences of very different lengths, one of them far longer than the others."""
+    r = np.random.default_rng(4)
+    lens = [int(x) for x in np.exp(r.uniform(0, 6, 70))] + [20000, 0, 1]
+    c = Eight(cuda, sum(x // page + 1 for x in lens) + 3, len(lens), max(lens) // page + 1, page, 1, 2, seed=8)
+    c.place(lens, seed=1)
+    slots = r.permutation(len(lens)).tolist()
+    q = _q(3, len(lens), 2, 8, _dt(dt))
+    out = run_attn8(c, 0, q, slots, _dt(dt))
+    assert c.take_status() == 0
+    check_attn8(c, 0, q, out, slots, dt == "f16")
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16"])
+def test_attn8_one_slot_twice(cuda, dt):
+    import torch
+    c = Eight(cuda, 20, 2, 12, 16, 1, 2, seed=8)
+    c.place([150, 33], seed=1)
+    q = _q(3, 3, 1, 4, _dt(dt))
+    q[2] = q[0]
+    out = run_attn8(c, 0, q, [0, 1, 0], _dt(dt))
+    check_attn8(c, 0, q, out, [0, 1, 0], dt == "f16")
+    assert torch.equal(out[0], out[2])
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16"])
+def test_attn8_peaked_rows(cuda, dt):
+    """Scores up to some hundreds, the largest late, early, and alone; scales that differ by many orders
+    between neighbouring blocks."""
+    import torch
+    lens = [700, 333]
+    c = Eight(cuda, 70, 2, 45, 16, 1, 2, seed=2)
+    c.place(lens, seed=3)
+    r = np.random.default_rng(3)
+    c.host.scales[0][:] = np.exp(r.uniform(-8, 1.5, c.host.scales[0].shape)).astype(np.float32)
+    c.host.scales[1][:] = np.exp(r.uniform(-25, 25, c.host.scales[1].shape)).astype(np.float32)
+    c.ks.copy_(_t(c.host.scales[0]))
+    c.vs.copy_(_t(c.host.scales[1]))
+    q = _q(5, 2, 2, 8, _dt(dt), 0.2)
+    out = run_attn8(c, 0, q, [0, 1], torch.float32)
+    check_attn8(c, 0, q, out, [0, 1], dt == "f16")
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16"])
+def test_attn8_unseen_places_leave_no_trace(cuda, dt):
+    """Codes, scales that are no numbers and page ids behind a sequence's end reach nothing."""
+    import torch
+    lens = [100, 7, 64]
+    c = Eight(cuda, 30, 3, 12, 32, 1, 2, seed=2)
+    c.place(lens, seed=3)
+    q = _q(5, 3, 2, 8, _dt(dt))
+    a = run_attn8(c, 0, q, [0, 1, 2], _dt(dt))
+    seen = {(c.m.tables[s][t // 32], t % 32) for s in range(3) for t in range(lens[s])}
+    blocks = {(p, row // BLOCK) for p, row in seen}
+    for p in range(30):
+        for b in range(2):
+            if (p, b) not in blocks:
+                c.ks[p, :, :, b], c.vs[p, :, :, b] = math.nan, math.inf
+        for row in range(32):
+            if (p, row) not in seen:
+                c.k[p, :, :, row], c.v[p, :, :, row] = 127, -128
+    for s in range(3):
+        c.tables[s, -(-lens[s] // 32):] = 1 << 30
+    b = run_attn8(c, 0, q, [0, 1, 2], _dt(dt))
+    assert c.take_status() == 0 and torch.equal(a, b)
+
+
+def test_attn8_bad_sequences_are_reported(cuda):
+    """Wrong slots, lengths and pages: *status says so, and the other sequences come out right."""
+    import torch
+    lens = [90, 40, 64, 200]
+    c = Eight(cuda, 40, 4, 14, 16, 1, 2, seed=2)
+    c.place(lens, seed=3)
+    for dt in (torch.float32, torch.float16):
+        q = _q(5, 4, 1, 8, dt)
+        good = run_attn8(c, 0, q, [0, 1, 2, 3], dt)
+        assert c.take_status() == 0
+        for slots in ([0, 4, 2, 3], [0, -1, 2, 3]):
+            out = run_attn8(c, 0, q, slots, dt)
+            assert c.take_status() == -1
+            for b in (0, 2, 3):
+                assert torch.equal(out[b], good[b]) or bool(torch.allclose(out[b].float(), good[b].float(), atol=2e-3))
+        for bad in (-1, 14 * 16 + 1):
+            c.lens[1] = bad
+            out = run_attn8(c, 0, q, [0, 1, 2, 3], dt)
+            assert c.take_status() == -1
+            assert bool(torch.allclose(out[[0, 2, 3]].float(), good[[0, 2, 3]].float(), atol=2e-3))
+        c.lens[1] = 40
+        for bad in (-1, 40, 1 << 30):
+            keep = int(c.tables[1, 1])
+            c.tables[1, 1] = bad
+            out = run_attn8(c, 0, q, [0, 1, 2, 3], dt)
+            assert c.take_status() == -1
+            assert torch.equal(out[[0, 2, 3]], good[[0, 2, 3]])
+            c.tables[1, 1] = keep
+        assert torch.equal(run_attn8(c, 0, q, [0, 1, 2, 3], dt), good) and c.take_status() == 0
+
+
+def test_attn8_same_result_every_time(cuda):
+    import torch
+    lens = [5000, 77, 300]
+    c = Eight(cuda, 400, 3, 340, 16, 1, 2, seed=2)
+    c.place(lens, seed=3)
+    q = _q(5, 3, 1, 8, torch.float16)
+    a = run_attn8(c, 0, q, [0, 1, 2], torch.float16)
+    for _ in range(5):
+        assert torch.equal(run_attn8(c, 0, q, [0, 1, 2], torch.float16), a)
+
+
+# ---------------------------------------------------------------------------
+# page operations, offsets, streams, graphs
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("page", [16, 64, 128])
+def test_copies_take_the_scales_along(cuda, page):
+    """Copy on write moves a page's live rows and their blocks' scales; compaction whole pages."""
+    import torch
+    c = Eight(cuda, 40, 6, 8, page, 3, 2, seed=4)
+    c.place([page + page // 2 + 1, 3 * page, 5, 0, 0, 0], seed=1)
+    for src, dst in (([0, 0, 2], [3, 4, 5]),):
+        c.p.fork(_i32(src), _i32(dst), c.work, c.status)
+        assert c.m.fork(src, dst) == 0
+    want = c.reserve([0, 3, 4, 2, 5], [1, 2, 1, 1, page])
+    assert c.take_status() == want == 0
+    assert all(c.same())
+    c.p.release(_i32([1, 3]), None, c.work, c.status)
+    assert c.m.release([1, 3], None) == 0
+    c.p.compact(c.work, c.status)
+    rc, moves = c.m.compact()
+    for a, b, rows in moves:
+        c.copy(a, b, rows)
+    assert c.take_status() == rc == 0 and len(moves) > 0
+    assert all(c.same()) and torch.equal(c.tables.cpu()[0, :2], torch.tensor(c.m.tables[0][:2], dtype=torch.int32))
+
+
+def test_offsets_beyond_32_bits(cuda):
+    """Pools of more than 2^32 bytes: the last pages are stored to, read and attended over."""
+    import torch
+    heads, page, layers = 8, 128, 2
+    n_pages = (1 << 32) // (layers * heads * page * 128) + 3
+    k, v = (torch.zeros((n_pages, layers, heads, page, 128), dtype=torch.int8, device="cuda") for _ in range(2))
+    ks, vs = (torch.zeros((n_pages, layers, heads, page // 16), device="cuda") for _ in range(2))
+    tab = _i32([[n_pages - 1, n_pages - 3, 0]])
+    refs = torch.zeros(n_pages, dtype=torch.int32, device="cuda")
+    refs[n_pages - 1] = refs[n_pages - 3] = 1
+    lens, status = _i32([200]), _i32([0])
+    p = cuda.KvPages(k, v, refs, tab, lens, ks, vs)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn((200, 3 * heads, 128), generator=g, device="cuda")
+    cos, sin = torch.ones((200, 64), device="cuda"), torch.zeros((200, 64), device="cuda")
+    slot, pos = _i32([0] * 200), _i32(list(range(200)))
+    p.append8(1, slot, pos, None, x[:, :heads], x[:, heads:2 * heads], cos, sin, status=status)
+    ko, vo = (torch.empty((200, heads, 128), device="cuda") for _ in range(2))
+    p.read8(1, slot, pos, ko, vo, status)
+    q = x[199:, 2 * heads:].contiguous().view(1, 1, heads, 128)
+    out = torch.empty_like(q)
+    work = torch.empty(p.attn8_work_bytes(1, 1, heads), dtype=torch.uint8, device="cuda")
+    p.attn8(1, q, out, _i32([0]), work, status)
+    assert int(status.item()) == 0
+    for got, want in ((ko, x[:, :heads]), (vo, x[:, heads:2 * heads])):
+        blocks = want.abs().amax(-1)
+        step = torch.stack([blocks[i // 16 * 16:min(200, i // 16 * 16 + 16)].amax(0) for i in range(200)])[..., None] / 127
+        assert bool(((got - want).abs() <= step * 0.5001).all())
+    for h in range(heads):
+        o, pv, big, va = attention(q[0, :, h].double(), ko[:, h].double(), vo[:, h].double(), torch.tensor([200], device="cuda"))
+        assert bool(((out[0, :, h].double() - o).abs() <= attn8_bound(o, pv, big, va, 200, False, False)).all())
+    assert int(k[0].abs().max()) == 0 and int(k[n_pages - 2].abs().max()) == 0
+
+
+def test_stream_and_graph(cuda):
+    """Store, attention and reading back on a stream of their own, captured and replayed on new inputs."""
+    import torch
+    c = Eight(cuda, 30, 3, 10, 16, 1, 2, seed=2)
+    c.place([50, 17, 100], seed=3)
+    cos, sin = _angles(160)
+    dc, ds = _t(cos), _t(sin)
+    r = np.random.default_rng(0)
+    q = torch.empty((3, 4, 128), device="cuda")
+    kv = torch.empty((3, 4, 128), device="cuda")
+    slot, pos = _i32([0, 1, 2]), _i32([49, 16, 99])
+    qo = torch.empty((3, 4, 128), dtype=torch.float16, device="cuda")
+    out = torch.empty((3, 1, 4, 128), dtype=torch.float16, device="cuda")
+    ko, vo = (torch.empty((3, 2, 128), device="cuda") for _ in range(2))
+    work = torch.empty(c.p.attn8_work_bytes(3, 1, 4), dtype=torch.uint8, device="cuda")
+    s = torch.cuda.Stream()
+
+    def calls():
+        c.p.append8(0, slot, pos, q, kv[:, :2], kv[:, 2:], dc, ds, qo, status=c.status, stream=s)
+        c.p.attn8(0, qo.view(3, 1, 4, 128), out, slot, work, c.status, stream=s)
+        c.p.read8(0, slot, pos, ko, vo, c.status, stream=s)
+
+    g = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g, stream=s):
+        calls()
+    for step in range(3):
+        x = r.standard_normal((3, 8, 128)).astype(np.float32)
+        q.copy_(_t(x[:, :4]))
+        kv.copy_(_t(x[:, 4:]))
+        torch.cuda.synchronize()
+        g.replay() if step else (calls(), s.synchronize())
+        torch.cuda.synchronize()
+        c.host.append(0, c.m.tables, c.m.lens, c.m.refs, [0, 1, 2], [49, 16, 99], x[:, 4:6], x[:, 6:], cos, sin)
+        assert c.take_status() == 0 and all(c.same())
+        check_attn8(c, 0, qo.view(3, 1, 4, 128), out, [0, 1, 2], True)
+        for b, n in enumerate((50, 17, 100)):
+            assert np.array_equal(ko[b].cpu().numpy(),
+                                  c.host.values(0, 0, c.m.tables[b], n)[:, -1].astype(np.float32))
