@@ -731,8 +731,8 @@ using namespace sllm;
 
 extern "C" int sllm_cuda_test_attn_error(void) {
     if (cudaDeviceSynchronize() != cudaSuccess) return -1;
-    const int a = take_prompt_error(), b = take_prefix_error();
-    return a != 0 ? a : b;
+    const int a = take_prompt_error(), b = take_prefix_error(), c = take_kv8_error();
+    return a != 0 ? a : b != 0 ? b : c;
 }
 
 extern "C" void sllm_cuda_test_attn_wait(uint32_t ns) { g_attn_wait_ns.store(ns, std::memory_order_relaxed); }

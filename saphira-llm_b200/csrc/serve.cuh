@@ -27,6 +27,7 @@ int check_pages(const sllm_cuda_kv_pages* p, const char* who, bool eight);
 // the error words of the attention kernels' bounded waits, read and cleared
 int take_prompt_error();
 int take_prefix_error();
+int take_kv8_error();
 // the limit of those waits for the next launches (2 s; tests set a short one), and
 // of one try's sleep, ns
 struct WaitLimit {

@@ -232,9 +232,11 @@ def attn8_bound(o, pv, big, va, n, f16, out_f16):
     """serving_ref's bound, with the stored values as the exact inputs: code times scale is applied to sums of
     exact products (one more unit, inside its 8), f32 queries and weights are pairs of f16, 2^-22 of each
     lost at most: of a score 2^-22 big, so 2 * 2^-22 big of a weight, and 2^-22 of the weight itself. One half
-    as much again for the products of the second with the first."""
+    as much again for the products of the second with the first. Where the first of a pair is subnormal the
+    second is rounded to 2^-25 of its own scale, 2^-36, on weights that are 2^15 at most: 2^-51 of the largest
+    weight, which is at most 1."""
     b = attention_bound(o, pv, big, va, n, f16, out_f16)
-    return b if f16 else b + 1.5 * pv * (2 * 2.0 ** -22 * big + 2.0 ** -22)
+    return b if f16 else b + 1.5 * pv * (2 * 2.0 ** -22 * big + 2.0 ** -22) + 2.0 ** -51 * va
 
 
 def check_attn8(c, layer, q, out, slots, f16):
