@@ -16,14 +16,13 @@
 // f32 queries and weights are pairs of f16, x = hi + 2^-11 lo, with a power of
 // two per query row; two products then, 22 bits.
 //
-// The work is cut by the device: the tiles of 64 keys of all (sequence, kv
+// The work is cut by the device: the tiles of 128 keys of all (sequence, kv
 // head) pairs, in order, are dealt to the CTAs in equal runs. A pair inside one
 // run is written at once; of a pair that runs share each leaves its part
 // (maximum, sum, outputs), at most two a CTA, and a second launch joins them.
 // So the split follows the lengths, whatever they are, and the workspace does not
 // depend on them.
 
-#include <algorithm>
 #include <type_traits>
 
 #include "attn_mma.cuh"
@@ -34,12 +33,13 @@ namespace {
 
 constexpr int kE8Warps = 4;                         // that multiply; one more loads
 constexpr int kE8Threads = 32 * (kE8Warps + 1);
-constexpr int kE8Keys = 64;                         // keys of a tile
+constexpr int kE8Keys = 128;                        // keys of a tile
+constexpr int kE8Blocks = kE8Keys / kKvBlock;
 constexpr int kE8Tile = kE8Keys * kServeDim;        // bytes of one of K or V
 constexpr float kE8Lift = 15.f;                     // weights are up to 2^15: f16 keeps 11 bits of them down to 2^-29 of the largest
 constexpr float kE8Log2 = kServeScale * 1.4426950408889634f;
 
-__host__ __device__ constexpr int e8_stages(int nt) { return nt == 1 ? 4 : 5; }
+__host__ __device__ constexpr int e8_stages(int) { return 2; }
 __host__ __device__ constexpr int e8_ctas(int nt) { return nt == 1 ? 3 : 2; }      // per SM
 
 struct Attn8Params {
@@ -51,7 +51,7 @@ struct Attn8Params {
     const int32_t* slots;
     int n, n_q, n_head, n_kv, group, rows;          // rows: n_q * group
     int rg, row_blocks, block_rows;                 // row groups of a CTA; row blocks of a pair, and rows of one
-    int box;                        // rows of a load
+    int page_log2;                  // rows of a page, and of a load
     WaitLimit wait;
     int32_t* status;
     float* part_o;                  // [2 * CTAs][block_rows][128]
@@ -60,7 +60,7 @@ struct Attn8Params {
 };
 
 struct Meta {                       // of a tile in a stage
-    int b, pair, len, key0, flags;  // pair: kv head * row blocks + row block
+    int b, head, row_block, len, key0, flags;
 };
 enum { E8_FIRST = 1, E8_LAST = 2, E8_PART0 = 4, E8_PART1 = 8, E8_END = 16 };
 
@@ -69,7 +69,7 @@ struct __align__(1024) Shared8 {
     uint8_t k[e8_stages(NT)][kE8Tile];
     uint8_t v[e8_stages(NT)][kE8Tile];
     float4 merge[2][NT * 9][32];                    // outputs, maximum and sum of a warp, a lane apart
-    float sc[e8_stages(NT)][8];                     // four blocks of K, four of V
+    float sc[e8_stages(NT)][2 * kE8Blocks];         // of K's blocks, of V's
     Meta meta[e8_stages(NT)];
     uint64_t full[e8_stages(NT)], empty[e8_stages(NT)], merged[2], taken[2], passed;
     unsigned long long scan[kE8Threads / 32];
@@ -93,6 +93,13 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// ... from zero
+__device__ __forceinline__ void mma_f16_new(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
@@ -197,72 +204,82 @@ struct Rows8 {
         }
     }
 
-    // 16 keys, the first of them number j0
-    __device__ __forceinline__ void block(const uint8_t* kt, const uint8_t* vt, float ks, float vs, bool masked, int j0) {
+    // Two blocks of 16 keys, the first keys of each number j0 and j0 + dj; the second
+    // counts for nothing where its scales are 0 and its keys are masked.
+    __device__ __forceinline__ void blocks(const uint8_t* kt, const uint8_t* vt, int apart, const float (&ks)[2],
+                                           const float (&vs)[2], bool masked, int j0, int dj) {
         const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-        float s[P][NT][4];
-        #pragma unroll
-        for (int x = 0; x < P; ++x)
-            #pragma unroll
-            for (int n = 0; n < NT; ++n)
-                #pragma unroll
-                for (int c = 0; c < 4; ++c) s[x][n][c] = 0.f;
+        float s[2][P][NT][4];
         #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const uint8_t* at = kt + g * 128 + (((2 * t + i) ^ g) << 4);
-            const uint4 ua = lds16(at), ub = lds16(at + 1024);
-            const uint32_t wa[4] = {ua.x, ua.y, ua.z, ua.w}, wb[4] = {ub.x, ub.y, ub.z, ub.w};
             #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                const uint32_t xa = wa[w] ^ 0x80808080u, xb = wb[w] ^ 0x80808080u;
-                const uint32_t a[4] = {two_codes(xa, false), two_codes(xb, false), two_codes(xa, true), two_codes(xb, true)};
+            for (int k = 0; k < 2; ++k) {
+                const uint8_t* at = kt + k * apart + g * 128 + (((2 * t + i) ^ g) << 4);
+                const uint4 ua = lds16(at), ub = lds16(at + 1024);
+                const uint32_t wa[4] = {ua.x, ua.y, ua.z, ua.w}, wb[4] = {ub.x, ub.y, ub.z, ub.w};
                 #pragma unroll
-                for (int n = 0; n < NT; ++n)
+                for (int w = 0; w < 4; ++w) {
+                    const uint32_t xa = wa[w] ^ 0x80808080u, xb = wb[w] ^ 0x80808080u;
+                    const uint32_t a[4] = {two_codes(xa, false), two_codes(xb, false), two_codes(xa, true), two_codes(xb, true)};
                     #pragma unroll
-                    for (int x = 0; x < P; ++x) mma_f16(s[x][n], a, q[x][n][8 * i + 2 * w], q[x][n][8 * i + 2 * w + 1]);
+                    for (int n = 0; n < NT; ++n)
+                        #pragma unroll
+                        for (int x = 0; x < P; ++x) {
+                            if (i == 0 && w == 0) mma_f16_new(s[k][x][n], a, q[x][n][0], q[x][n][1]);
+                            else mma_f16(s[k][x][n], a, q[x][n][8 * i + 2 * w], q[x][n][8 * i + 2 * w + 1]);
+                        }
+                }
             }
         }
-        const float base = ks * kE8Log2;
-        uint32_t pb[P][NT][2];
+        const float base[2] = {ks[0] * kE8Log2, ks[1] * kE8Log2};
+        uint32_t pb[2][P][NT][2];
         bool moved = false;
         float alpha[NT][2];
         #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            float y[4];
+            float y[2][4];
             #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                y[c] = P == 1 ? s[0][n][c] * base : __fmaf_rn(s[P - 1][n][c], 0x1p-11f, s[0][n][c]) * (base * mul[n][c & 1]);
-                if (masked && j0 + g + 8 * (c >> 1) >= lim[n][c & 1]) y[c] = -INFINITY;
-            }
-            float mx[2] = {fmaxf(y[0], y[2]), fmaxf(y[1], y[3])};
-            #pragma unroll
-            for (int z = 4; z < 32; z <<= 1) {
-                mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], z));
-                mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], z));
+            for (int k = 0; k < 2; ++k)
+                #pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    y[k][c] = P == 1 ? s[k][0][n][c] * base[k]
+                                     : __fmaf_rn(s[k][P - 1][n][c], 0x1p-11f, s[k][0][n][c]) * (base[k] * mul[n][c & 1]);
+            if (masked) {
+                #pragma unroll
+                for (int k = 0; k < 2; ++k)
+                    #pragma unroll
+                    for (int c = 0; c < 4; ++c)
+                        if (j0 + k * dj + g + 8 * (c >> 1) >= lim[n][c & 1]) y[k][c] = -INFINITY;
             }
             float ref[2];
             #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                const float now = fmaxf(m[n][c], mx[c]);
+                float now = fmaxf(fmaxf(y[0][c], y[0][c + 2]), fmaxf(y[1][c], y[1][c + 2]));
+                #pragma unroll
+                for (int z = 4; z < 32; z <<= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, z));
+                now = fmaxf(m[n][c], now);
                 ref[c] = (now == -INFINITY ? 0.f : now) - kE8Lift;
                 alpha[n][c] = ex2(m[n][c] - kE8Lift - ref[c]);
                 moved = moved || now != m[n][c];
                 m[n][c] = now;
             }
-            float e[4];
             #pragma unroll
-            for (int c = 0; c < 4; ++c) e[c] = ex2(y[c] - ref[c & 1]);
-            #pragma unroll
-            for (int c = 0; c < 2; ++c) l[n][c] = __fmaf_rn(l[n][c], alpha[n][c], e[c] + e[c + 2]);
-            #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const uint32_t hi = pack2(e[2 * c], e[2 * c + 1]);
-                pb[0][n][c] = transpose8(hi);
-                if constexpr (P == 2) {
-                    const float2 z = unpack2(hi);
-                    pb[P - 1][n][c] = transpose8(pack2((e[2 * c] - z.x) * 2048.f, (e[2 * c + 1] - z.y) * 2048.f));
+            for (int k = 0; k < 2; ++k) {
+                #pragma unroll
+                for (int c = 0; c < 4; ++c) y[k][c] = ex2(y[k][c] - ref[c & 1]);
+                #pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const uint32_t hi = pack2(y[k][2 * c], y[k][2 * c + 1]);
+                    pb[k][0][n][c] = transpose8(hi);
+                    if constexpr (P == 2) {
+                        const float2 z = unpack2(hi);
+                        pb[k][P - 1][n][c] = transpose8(pack2((y[k][2 * c] - z.x) * 2048.f, (y[k][2 * c + 1] - z.y) * 2048.f));
+                    }
                 }
             }
+            #pragma unroll
+            for (int c = 0; c < 2; ++c)
+                l[n][c] = __fmaf_rn(l[n][c], alpha[n][c], (y[0][c] + y[0][c + 2]) + (y[1][c] + y[1][c + 2]));
         }
         if (__any_sync(0xffffffffu, moved)) {
             #pragma unroll
@@ -272,36 +289,35 @@ struct Rows8 {
                     #pragma unroll
                     for (int c = 0; c < 4; ++c) o[n][j][c] *= alpha[n][c & 1];
         }
-        uint32_t wv[4][4];
         #pragma unroll
-        for (int i = 0; i < 4; ++i) {               // keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
-            const int r = 2 * t + (i & 1);
-            const uint4 u = lds16(vt + (r + 8 * (i >> 1)) * 128 + ((g ^ r) << 4));
-            wv[i][0] = u.x ^ 0x80808080u;
-            wv[i][1] = u.y ^ 0x80808080u;
-            wv[i][2] = u.z ^ 0x80808080u;
-            wv[i][3] = u.w ^ 0x80808080u;
-        }
-        #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+        for (int k = 0; k < 2; ++k) {
+            uint32_t wv[4][4];
             #pragma unroll
-            for (int hi = 0; hi < 2; ++hi) {
-                const uint32_t x = __byte_perm(wv[0][w], wv[1][w], hi ? 0x7362 : 0x5140);
-                const uint32_t y = __byte_perm(wv[2][w], wv[3][w], hi ? 0x7362 : 0x5140);
-                const uint32_t a[4] = {two_codes(x, false), two_codes(x, true), two_codes(y, false), two_codes(y, true)};
-                const int j = 2 * w + hi;
+            for (int i = 0; i < 4; ++i) {           // keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
+                const int r = 2 * t + (i & 1);
+                const uint4 u = lds16(vt + k * apart + (r + 8 * (i >> 1)) * 128 + ((g ^ r) << 4));
+                wv[i][0] = u.x ^ 0x80808080u;
+                wv[i][1] = u.y ^ 0x80808080u;
+                wv[i][2] = u.z ^ 0x80808080u;
+                wv[i][3] = u.w ^ 0x80808080u;
+            }
+            #pragma unroll
+            for (int w = 0; w < 4; ++w) {
                 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    float d[P][4];
+                for (int hi = 0; hi < 2; ++hi) {
+                    const uint32_t x = __byte_perm(wv[0][w], wv[1][w], hi ? 0x7362 : 0x5140);
+                    const uint32_t y = __byte_perm(wv[2][w], wv[3][w], hi ? 0x7362 : 0x5140);
+                    const uint32_t a[4] = {two_codes(x, false), two_codes(x, true), two_codes(y, false), two_codes(y, true)};
+                    const int j = 2 * w + hi;
                     #pragma unroll
-                    for (int z = 0; z < P; ++z) {
+                    for (int n = 0; n < NT; ++n) {
+                        float d[P][4];
                         #pragma unroll
-                        for (int c = 0; c < 4; ++c) d[z][c] = 0.f;
-                        mma_f16(d[z], a, pb[z][n][0], pb[z][n][1]);
+                        for (int z = 0; z < P; ++z) mma_f16_new(d[z], a, pb[k][z][n][0], pb[k][z][n][1]);
+                        #pragma unroll
+                        for (int c = 0; c < 4; ++c)
+                            o[n][j][c] = __fmaf_rn(P == 1 ? d[0][c] : __fmaf_rn(d[P - 1][c], 0x1p-11f, d[0][c]), vs[k], o[n][j][c]);
                     }
-                    #pragma unroll
-                    for (int c = 0; c < 4; ++c)
-                        o[n][j][c] = __fmaf_rn(P == 1 ? d[0][c] : __fmaf_rn(d[P - 1][c], 0x1p-11f, d[0][c]), vs, o[n][j][c]);
                 }
             }
         }
@@ -403,7 +419,7 @@ __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
 
 // The loading warp's place: unit by unit through its run.
 struct Place {
-    int b, slot, len, tiles, pair, tile;
+    int b, slot, len, tiles, pair, head, row_block, tile;    // pair: head * row blocks + row block
 };
 
 template <class Q, class O, int NT>
@@ -425,7 +441,7 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
     }
     if (t == 0) {
         for (int i = 0; i < STAGES; ++i) {
-            mbar_init(&sh.full[i], 1 + 8);
+            mbar_init(&sh.full[i], 1 + 2 * kE8Blocks);
             mbar_init(&sh.empty[i], kE8Warps);
         }
         for (int i = 0; i < 2; ++i) {
@@ -498,10 +514,10 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
         };
         // lane i: the page of the tile's i-th load
         auto ids = [&](const Place& x) {
-            const int key = x.tile * kE8Keys + lane * p.box;
+            const int key = x.tile * kE8Keys + (lane << p.page_log2);
             int id = 0;
-            if (lane < kE8Keys / p.box && key < x.len) {
-                id = pg.tables[(size_t)x.slot * pg.width + key / pg.page];
+            if (lane < (kE8Keys >> p.page_log2) && key < x.len) {
+                id = pg.tables[(size_t)x.slot * pg.width + (key >> p.page_log2)];
                 if (id < 0 || id >= pg.n_pages) {
                     raise(p.status, SLLM_CUDA_ERR_ARG);
                     id = 0;
@@ -512,12 +528,14 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
         Place cur;
         unsigned long long left = u1 - u0;
         // (lengths that somebody writes to meanwhile end the run early, inside the arrays)
-        cur.pair = cur.tile = 0;
+        cur.pair = cur.tile = cur.head = cur.row_block = 0;
         if (!enter(cur, sh.start_b) || sh.start_rest >= (unsigned long long)cur.tiles * pairs) {
             left = 0;
         } else {
             cur.pair = (int)(sh.start_rest / cur.tiles);
             cur.tile = (int)(sh.start_rest % cur.tiles);
+            cur.head = cur.pair / p.row_blocks;
+            cur.row_block = cur.pair % p.row_blocks;
         }
         int id = left > 0 ? ids(cur) : 0;
         int first = 1, started = cur.tile == 0;     // of the segment: its first tile here; whether the pair starts here
@@ -529,8 +547,12 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
             if (left > 1) {
                 if (++nxt.tile == nxt.tiles) {
                     nxt.tile = 0;
+                    if (++nxt.row_block == p.row_blocks) {
+                        nxt.row_block = 0;
+                        ++nxt.head;
+                    }
                     if (++nxt.pair == pairs) {
-                        nxt.pair = 0;
+                        nxt.pair = nxt.head = 0;
                         if (!enter(nxt, cur.b + 1)) left = 1;
                     }
                 }
@@ -539,29 +561,31 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
             const int slot = n % STAGES;
             if (n >= STAGES && !(ok = at_wait_warp(&sh.empty[slot], (n / STAGES - 1) & 1, ab, w))) break;
             const bool ends = cur.tile + 1 == cur.tiles, last = ends || left == 1;
-            const int keys = min(kE8Keys, cur.len - cur.tile * kE8Keys), loads = (keys + p.box - 1) / p.box;
-            const int key0 = cur.tile * kE8Keys, h = cur.pair / p.row_blocks;
+            const int key0 = cur.tile * kE8Keys, keys = min(kE8Keys, cur.len - key0);
+            const int loads = (keys + (1 << p.page_log2) - 1) >> p.page_log2;
             if (lane == 0) {
                 const int flags = (first ? E8_FIRST : 0) | (last ? E8_LAST : 0) |
                                   (!last || (ends && started) ? 0 : started ? E8_PART1 : E8_PART0);
-                sh.meta[slot] = Meta{cur.b, cur.pair, cur.len, key0, flags};
-                mbar_expect_tx(&sh.full[slot], (uint32_t)(loads * p.box) * 2 * kServeDim);
+                sh.meta[slot] = Meta{cur.b, cur.head, cur.row_block, cur.len, key0, flags};
+                mbar_expect_tx(&sh.full[slot], (uint32_t)(loads << p.page_log2) * 2 * kServeDim);
             }
             __syncwarp();
             if (lane < loads) {
-                tma_load_4d(sh.k[slot] + lane * p.box * kServeDim, &tm_k, 0, key0 % pg.page, h, id, &sh.full[slot]);
-                tma_load_4d(sh.v[slot] + lane * p.box * kServeDim, &tm_v, 0, key0 % pg.page, h, id, &sh.full[slot]);
+                const int at = lane * kServeDim << p.page_log2;
+                tma_load_4d(sh.k[slot] + at, &tm_k, 0, 0, cur.head, id, &sh.full[slot]);
+                tma_load_4d(sh.v[slot] + at, &tm_v, 0, 0, cur.head, id, &sh.full[slot]);
             }
-            const int blk = lane & 3, from = __shfl_sync(0xffffffffu, id, blk * kKvBlock / p.box);
-            if (lane < 8) {
+            const int blk = lane & (kE8Blocks - 1), from = __shfl_sync(0xffffffffu, id, (blk * kKvBlock) >> p.page_log2);
+            if (lane < 2 * kE8Blocks) {
                 if (blk * kKvBlock < keys)
-                    cp_async4(&sh.sc[slot][lane], (lane < 4 ? p.ksc : p.vsc) + (size_t)from * p.scale_stride +
-                                                      (size_t)h * (pg.page / kKvBlock) + (key0 + blk * kKvBlock) % pg.page / kKvBlock);
+                    cp_async4(&sh.sc[slot][lane], (lane < kE8Blocks ? p.ksc : p.vsc) + (size_t)from * p.scale_stride +
+                                                      cur.head * (pg.page / kKvBlock) +
+                                                      ((key0 + blk * kKvBlock) & (pg.page - 1)) / kKvBlock);
                 cp_async_arrive(&sh.full[slot]);
             }
             if (last && !ends && started) {         // other runs go on with this pair
                 const unsigned long long end = u1 + (unsigned long long)(cur.tiles - cur.tile - 1);
-                note = make_int4(cur.b, cur.pair, (int)min((end * G - 1) / all, G - 1), 0);
+                note = make_int4(cur.b, cur.head, (int)min((end * G - 1) / all, G - 1), cur.row_block);
             }
             first = last;
             started = last ? 1 : started;
@@ -573,10 +597,10 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
             ok = n < STAGES || at_wait_warp(&sh.empty[slot], (n / STAGES - 1) & 1, ab, w);
             if (ok) {
                 if (lane == 0) {
-                    sh.meta[slot] = Meta{0, 0, 0, 0, E8_END};
+                    sh.meta[slot] = Meta{0, 0, 0, 0, 0, E8_END};
                     mbar_arrive(&sh.full[slot]);
                 }
-                if (lane < 8) mbar_arrive(&sh.full[slot]);
+                if (lane < 2 * kE8Blocks) mbar_arrive(&sh.full[slot]);
                 ++n;
             }
         }
@@ -597,17 +621,22 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
             if (!ok) break;
             const Meta mt = sh.meta[slot];
             if (mt.flags & E8_END) break;
-            const int h = mt.pair / p.row_blocks, rb = mt.pair % p.row_blocks;
             if (mt.flags & E8_FIRST) {
                 rows.clear();
-                rows.template load<Q>(p, mt.b, h, rb * p.block_rows + rgrp * 8 * NT, mt.len);
+                rows.template load<Q>(p, mt.b, mt.head, mt.row_block * p.block_rows + rgrp * 8 * NT, mt.len);
             }
             const int keys = min(kE8Keys, mt.len - mt.key0);
             const bool masked = mt.key0 + kE8Keys > mt.len - p.n_q + 1;
+            const float* const sc = sh.sc[slot];
+            // blocks kg and kg + KG, and so on: a short tile's are shared out, too
             #pragma unroll 1
-            for (int blk = kg; blk * kKvBlock < keys; blk += KG)
-                rows.block(sh.k[slot] + blk * kKvBlock * kServeDim, sh.v[slot] + blk * kKvBlock * kServeDim, sh.sc[slot][blk],
-                           sh.sc[slot][4 + blk], masked, mt.key0 + blk * kKvBlock);
+            for (int blk = kg; blk * kKvBlock < keys; blk += 2 * KG) {
+                const bool two = (blk + KG) * kKvBlock < keys;
+                const float ks[2] = {sc[blk], two ? sc[blk + KG] : 0.f};
+                const float vs[2] = {sc[kE8Blocks + blk], two ? sc[kE8Blocks + blk + KG] : 0.f};
+                rows.blocks(sh.k[slot] + blk * kKvBlock * kServeDim, sh.v[slot] + blk * kKvBlock * kServeDim,
+                            KG * kKvBlock * kServeDim, ks, vs, masked, mt.key0 + blk * kKvBlock, KG * kKvBlock);
+            }
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.empty[slot]);
             if (!(mt.flags & E8_LAST)) continue;
@@ -642,7 +671,7 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
                 }
             }
             const int part = mt.flags & E8_PART0 ? 2 * (int)c : mt.flags & E8_PART1 ? 2 * (int)c + 1 : -1;
-            rows.template store<O>(p, mt.b, h, rb, rgrp * 8 * NT, part);
+            rows.template store<O>(p, mt.b, mt.head, mt.row_block, rgrp * 8 * NT, part);
         }
     }
     if (!ok && lane == 0) raise(p.status, SLLM_CUDA_ERR_TIMEOUT);
@@ -663,7 +692,7 @@ attn_kv8_join_kernel(const __grid_constant__ Attn8Params p, int per_row) {
     pdl_wait();
     const int4 note = p.shared[c];
     if (note.x < 0) return;
-    const int h = note.y / p.row_blocks, r = note.y % p.row_blocks * p.block_rows + in;
+    const int h = note.y, r = note.w * p.block_rows + in;
     const bool live = in < p.block_rows && r < p.rows;
     // parts: the second of this CTA's, then the first of the following CTAs'
     const int parts = note.z - c + 1;
@@ -748,14 +777,14 @@ size_t work8_bytes(const Cut8& x) {
     return (size_t)x.ctas * (2 * x.block_rows * (kServeDim * sizeof(float) + sizeof(float2)) + sizeof(int4));
 }
 
-// one layer of a pool: `box` rows of one page and kv head
-bool encode_codes(CUtensorMap* tm, const void* base, const sllm_cuda_kv_pages& p, int box_rows) {
+// one layer of a pool: a page's rows of one kv head per box
+bool encode_codes(CUtensorMap* tm, const void* base, const sllm_cuda_kv_pages& p) {
     PFN_cuTensorMapEncodeTiled_v12000 enc = tensor_map_encoder();
     if (enc == nullptr) return false;
     const cuuint64_t row = kServeDim, head = row * p.page_size, page = head * p.n_head_kv * p.n_layer;
     const cuuint64_t dims[4] = {(cuuint64_t)kServeDim, (cuuint64_t)p.page_size, (cuuint64_t)p.n_head_kv, (cuuint64_t)p.n_pages};
     const cuuint64_t strides[3] = {row, head, page};
-    const cuuint32_t box[4] = {(cuuint32_t)kServeDim, (cuuint32_t)box_rows, 1, 1}, estr[4] = {1, 1, 1, 1};
+    const cuuint32_t box[4] = {(cuuint32_t)kServeDim, (cuuint32_t)p.page_size, 1, 1}, estr[4] = {1, 1, 1, 1};
     return enc(tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(base), dims, strides, box, estr,
                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -821,7 +850,7 @@ extern "C" int sllm_cuda_attn_kv8(const sllm_cuda_kv_pages* p, int32_t layer, co
     a.n = n; a.n_q = n_q; a.n_head = n_head; a.n_kv = p->n_head_kv; a.group = n_head / p->n_head_kv;
     a.rows = n_q * a.group;
     a.rg = cut.rg; a.row_blocks = cut.row_blocks; a.block_rows = cut.block_rows;
-    a.box = std::min(p->page_size, kE8Keys);
+    while ((1 << a.page_log2) < p->page_size) ++a.page_log2;
     a.wait = attn_wait_limit();
     a.status = status;
     a.part_o = static_cast<float*>(work);
@@ -830,8 +859,8 @@ extern "C" int sllm_cuda_attn_kv8(const sllm_cuda_kv_pages* p, int32_t layer, co
     const PagesDev pg = pages_dev(*p);
     const cudaStream_t st = (cudaStream_t)stream;
     CUtensorMap tk, tv;
-    if (!encode_codes(&tk, static_cast<const int8_t*>(p->k) + layer * layer_codes, *p, a.box) ||
-        !encode_codes(&tv, static_cast<const int8_t*>(p->v) + layer * layer_codes, *p, a.box))
+    if (!encode_codes(&tk, static_cast<const int8_t*>(p->k) + layer * layer_codes, *p) ||
+        !encode_codes(&tv, static_cast<const int8_t*>(p->v) + layer * layer_codes, *p))
         return fail(SLLM_CUDA_ERR_DEVICE, "attn_kv8: a tensor map could not be made");
     const bool f32 = q_type == SLLM_CUDA_KV_F32, out32 = out_type == SLLM_CUDA_KV_F32;
     cudaError_t e;
