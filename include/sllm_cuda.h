@@ -419,8 +419,7 @@ SLLM_CUDA_API int sllm_cuda_kv8_read(const sllm_cuda_kv_pages * p, int32_t layer
  * q_type, out f32 or, from f16 queries, f16. Codes are multiplied on the tensor
  * cores exactly, in f32 sums; f16 queries are taken as they are, f32 queries and
  * their softmax weights as pairs of f16 (22 bits), the weights of f16 queries
- * rounded to f16 (against the running maximum: 11 bits down to 2^-29 of a row's
- * largest). A sequence whose slot, length or table is wrong sets
+ * rounded to f16 (11 bits down to 2^-21 of a row's largest). A sequence whose slot, length or table is wrong sets
  * SLLM_CUDA_ERR_ARG in *status, and its rows of out mean nothing. n <= 4096, n_q
  * <= 16, n_head <= 1024. A workspace of work_bytes(n, n_q, n_head) serves every
  * call over this cache with that n_head and no more sequences and query tokens.

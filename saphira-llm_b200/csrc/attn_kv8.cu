@@ -36,10 +36,14 @@ constexpr int kE8Threads = 32 * (kE8Warps + 1);
 constexpr int kE8Keys = 128;                        // keys of a tile
 constexpr int kE8Blocks = kE8Keys / kKvBlock;
 constexpr int kE8Tile = kE8Keys * kServeDim;        // bytes of one of K or V
-constexpr float kE8Lift = 15.f;                     // weights are up to 2^15: f16 keeps 11 bits of them down to 2^-29 of the largest
+// Weights stand against 2^-lift of a reference. Pairs of f16: the running maximum,
+// so weights are up to 2^15. One f16: the maximum when it last grew by more than
+// 2^8, so that the outputs are seldom rescaled; weights are up to 2^15, too, and
+// keep 11 bits down to 2^-21 of the largest.
+constexpr float kE8Grow = 8.f;
+__host__ __device__ constexpr float e8_lift(int planes) { return planes == 1 ? 15.f - kE8Grow : 15.f; }
 constexpr float kE8Log2 = kServeScale * 1.4426950408889634f;
 
-__host__ __device__ constexpr int e8_stages(int) { return 2; }
 __host__ __device__ constexpr int e8_ctas(int nt) { return nt == 1 ? 3 : 2; }      // per SM
 
 struct Attn8Params {
@@ -51,12 +55,25 @@ struct Attn8Params {
     const int32_t* slots;
     int n, n_q, n_head, n_kv, group, rows;          // rows: n_q * group
     int rg, row_blocks, block_rows;                 // row groups of a CTA; row blocks of a pair, and rows of one
+    int q_bufs;                     // buffers of a row block's queries
     int page_log2;                  // rows of a page, and of a load
     WaitLimit wait;
     int32_t* status;
     float* part_o;                  // [2 * CTAs][block_rows][128]
     float2* part_ml;                // [2 * CTAs][block_rows]
-    int4* shared;                   // [CTAs]: the pair that starts in this CTA's run and ends in another's
+    // notes for the join: sequence (-1: nothing to join), pair, first and last CTA. Of each
+    // pair where there are no more pairs than CTAs (by_pair), else of the pair that starts
+    // in a CTA's run and ends in another's
+    int4* notes;
+    int by_pair, n_notes;
+    uint32_t over_group;            // ceil(2^32 / group), 0 for 1: exact below 2^22 (rows are under 2^14, groups up to 2^10)
+
+    __device__ __forceinline__ int token(int row) const { return over_group == 0 ? row : (int)__umulhi((uint32_t)row, over_group); }
+    // row `row` of a sequence's kv head, in q and out
+    __device__ __forceinline__ size_t row_at(int b, int head, int row) const {
+        const int j = token(row);
+        return (((size_t)b * n_q + j) * n_head + (size_t)head * group + (row - j * group)) * kServeDim;
+    }
 };
 
 struct Meta {                       // of a tile in a stage
@@ -64,18 +81,28 @@ struct Meta {                       // of a tile in a stage
 };
 enum { E8_FIRST = 1, E8_LAST = 2, E8_PART0 = 4, E8_PART1 = 8, E8_END = 16 };
 
-template <int NT>
-struct __align__(1024) Shared8 {
-    uint8_t k[e8_stages(NT)][kE8Tile];
-    uint8_t v[e8_stages(NT)][kE8Tile];
-    float4 merge[2][NT * 9][32];                    // outputs, maximum and sum of a warp, a lane apart
-    float sc[e8_stages(NT)][2 * kE8Blocks];         // of K's blocks, of V's
-    Meta meta[e8_stages(NT)];
-    uint64_t full[e8_stages(NT)], empty[e8_stages(NT)], merged[2], taken[2], passed;
+struct __align__(1024) Stage8 {
+    uint8_t k[kE8Tile], v[kE8Tile];
+};
+constexpr int kE8Stages = 2;
+
+// The loading warp's place in its run, tile by tile; pair: head * row blocks + row
+// block of a sequence
+struct Place {
+    int b, slot, len, tiles, pair, head, row_block, tile;
+};
+
+struct __align__(1024) Shared8 {    // and the queries' buffers behind it
+    Stage8 stage[kE8Stages];
+    float sc[kE8Stages][2 * kE8Blocks];             // of K's blocks, of V's
+    Meta meta[kE8Stages];
+    uint64_t full[kE8Stages], empty[kE8Stages];
+    uint64_t q_free[2], done, merged;
     unsigned long long scan[kE8Threads / 32];
     unsigned long long start_rest;
-    int start_b;
+    Place start;
     int abort;
+    float2 ml[kE8Warps][16];
 };
 
 struct Waits {                      // for the bounded waits
@@ -95,11 +122,11 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// ... from zero
-__device__ __forceinline__ void mma_f16_new(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+// ... from c0 in the even columns, c1 in the odd ones
+__device__ __forceinline__ void mma_f16_from(float (&d)[4], float c0, float c1, const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %10, %11};"
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
 }
 
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
@@ -109,10 +136,13 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 }
 
 // two codes, of bytes 0 and 1 or 2 and 3 of u (with 128 added to each), as f16:
-// 0x6400 + byte is 1024 + byte
+// 0x6400 + byte is 1024 + byte; `raw`: with the 1152 that this is too much
+constexpr float kE8Raw = 1152.f;
+template <bool RAW>
 __device__ __forceinline__ uint32_t two_codes(uint32_t u, bool upper) {
     const uint32_t x = __byte_perm(u, 0x64646464u, upper ? 0x4342 : 0x4140);
-    const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&x), __half2half2(__ushort_as_half(0x6480)));     // 1152
+    if (RAW) return x;
+    const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&x), __half2half2(__ushort_as_half(0x6480)));
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
@@ -130,7 +160,8 @@ __device__ __forceinline__ uint4 lds16(const uint8_t* p) { return *reinterpret_c
 template <int P, int NT>
 struct Rows8 {
     uint32_t q[P][NT][16];
-    float o[NT][8][4], m[NT][2], l[NT][2], mul[NT][2];
+    float o[NT][8][4], m[NT][2], l[NT][2];
+    float mul[NT][2];               // pairs: the row's power of two. One f16: what its scores start from, see below
     int lim[NT][2];
 
     __device__ __forceinline__ void clear() {
@@ -149,31 +180,43 @@ struct Rows8 {
         }
     }
 
-    // query rows r0 .. of sequence b and kv head h
+    // query rows r0 .. of the row block that starts at row `first`, from its buffer
     template <class Q>
-    __device__ __forceinline__ void load(const Attn8Params& p, int b, int h, int r0, int len) {
+    __device__ __forceinline__ void load(const Attn8Params& p, const uint8_t* buf, int r0, int first, int len) {
         const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
         #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            const int r = r0 + 8 * n + g;
-            const bool in = r < p.rows;
-            const Q* x = static_cast<const Q*>(p.q) +
-                         (((size_t)b * p.n_q + (in ? r / p.group : 0)) * p.n_head + (size_t)h * p.group + (in ? r % p.group : 0)) * kServeDim + 32 * t;
+            const Q* x = reinterpret_cast<const Q*>(buf) + (r0 + 8 * n + g) * kServeDim + 32 * t;
             if constexpr (P == 1) {
                 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const uint4 u = in ? __ldg(reinterpret_cast<const uint4*>(x) + i) : make_uint4(0, 0, 0, 0);
+                    const uint4 u = *(reinterpret_cast<const uint4*>(x) + i);
                     q[0][n][4 * i] = u.x;
                     q[0][n][4 * i + 1] = u.y;
                     q[0][n][4 * i + 2] = u.z;
                     q[0][n][4 * i + 3] = u.w;
                 }
+                // K's codes go in 1152 too large, and 1152 times the row's sum less is
+                // where its scores start: half an instruction a code less, for
+                // 2^-24 of that sum, which is a hundredth of what half a step of a
+                // code is
+                float part[4] = {0.f, 0.f, 0.f, 0.f};
+                #pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float2 z = unpack2(q[0][n][i]);
+                    part[i & 3] += z.x + z.y;
+                }
+                float sum = (part[0] + part[1]) + (part[2] + part[3]);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                #pragma unroll
+                for (int c = 0; c < 2; ++c) mul[n][c] = -kE8Raw * __shfl_sync(0xffffffffu, sum, 8 * t + 4 * c);
             } else {
                 float4 f[8];
                 float most = 0.f;
                 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    f[i] = in ? __ldg(reinterpret_cast<const float4*>(x) + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    f[i] = *(reinterpret_cast<const float4*>(x) + i);
                     most = fmaxf(most, fmaxf(fmaxf(fabsf(f[i].x), fabsf(f[i].y)), fmaxf(fabsf(f[i].z), fabsf(f[i].w))));
                 }
                 most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
@@ -198,8 +241,8 @@ struct Rows8 {
             }
             #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                const int row = r0 + 8 * n + 2 * t + c;
-                lim[n][c] = len - p.n_q + 1 + (row < p.rows ? row / p.group : p.n_q - 1);
+                const int row = first + r0 + 8 * n + 2 * t + c;
+                lim[n][c] = len - p.n_q + 1 + (row < p.rows ? p.token(row) : p.n_q - 1);
             }
         }
     }
@@ -220,12 +263,14 @@ struct Rows8 {
                 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
                     const uint32_t xa = wa[w] ^ 0x80808080u, xb = wb[w] ^ 0x80808080u;
-                    const uint32_t a[4] = {two_codes(xa, false), two_codes(xb, false), two_codes(xa, true), two_codes(xb, true)};
+                    const uint32_t a[4] = {two_codes<P == 1>(xa, false), two_codes<P == 1>(xb, false), two_codes<P == 1>(xa, true),
+                                           two_codes<P == 1>(xb, true)};
                     #pragma unroll
                     for (int n = 0; n < NT; ++n)
                         #pragma unroll
                         for (int x = 0; x < P; ++x) {
-                            if (i == 0 && w == 0) mma_f16_new(s[k][x][n], a, q[x][n][0], q[x][n][1]);
+                            if (i == 0 && w == 0)
+                                mma_f16_from(s[k][x][n], P == 1 ? mul[n][0] : 0.f, P == 1 ? mul[n][1] : 0.f, a, q[x][n][0], q[x][n][1]);
                             else mma_f16(s[k][x][n], a, q[x][n][8 * i + 2 * w], q[x][n][8 * i + 2 * w + 1]);
                         }
                 }
@@ -233,61 +278,68 @@ struct Rows8 {
         }
         const float base[2] = {ks[0] * kE8Log2, ks[1] * kE8Log2};
         uint32_t pb[2][P][NT][2];
-        bool moved = false;
-        float alpha[NT][2];
+        constexpr float LIFT = e8_lift(P), GROW = P == 1 ? kE8Grow : 0.f;
+        float y[NT][2][4], most[NT][2];
+        bool grown = false;
         #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            float y[2][4];
             #pragma unroll
             for (int k = 0; k < 2; ++k)
                 #pragma unroll
                 for (int c = 0; c < 4; ++c)
-                    y[k][c] = P == 1 ? s[k][0][n][c] * base[k]
-                                     : __fmaf_rn(s[k][P - 1][n][c], 0x1p-11f, s[k][0][n][c]) * (base[k] * mul[n][c & 1]);
+                    y[n][k][c] = P == 1 ? s[k][0][n][c] * base[k]
+                                        : __fmaf_rn(s[k][P - 1][n][c], 0x1p-11f, s[k][0][n][c]) * (base[k] * mul[n][c & 1]);
             if (masked) {
                 #pragma unroll
                 for (int k = 0; k < 2; ++k)
                     #pragma unroll
                     for (int c = 0; c < 4; ++c)
-                        if (j0 + k * dj + g + 8 * (c >> 1) >= lim[n][c & 1]) y[k][c] = -INFINITY;
+                        if (j0 + k * dj + g + 8 * (c >> 1) >= lim[n][c & 1]) y[n][k][c] = -INFINITY;
             }
-            float ref[2];
             #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                float now = fmaxf(fmaxf(y[0][c], y[0][c + 2]), fmaxf(y[1][c], y[1][c + 2]));
+                float now = fmaxf(fmaxf(y[n][0][c], y[n][0][c + 2]), fmaxf(y[n][1][c], y[n][1][c + 2]));
                 #pragma unroll
                 for (int z = 4; z < 32; z <<= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, z));
-                now = fmaxf(m[n][c], now);
-                ref[c] = (now == -INFINITY ? 0.f : now) - kE8Lift;
-                alpha[n][c] = ex2(m[n][c] - kE8Lift - ref[c]);
-                moved = moved || now != m[n][c];
-                m[n][c] = now;
+                most[n][c] = now;
+                grown = grown || now > m[n][c] + GROW;
             }
+        }
+        if (__any_sync(0xffffffffu, grown)) {
+            #pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                float alpha[2];
+                #pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const float now = fmaxf(m[n][c], most[n][c]);
+                    alpha[c] = now == -INFINITY ? 1.f : ex2(m[n][c] - now);
+                    m[n][c] = now;
+                    l[n][c] *= alpha[c];
+                }
+                #pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    #pragma unroll
+                    for (int c = 0; c < 4; ++c) o[n][j][c] *= alpha[c & 1];
+            }
+        }
+        #pragma unroll
+        for (int n = 0; n < NT; ++n) {
             #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 #pragma unroll
-                for (int c = 0; c < 4; ++c) y[k][c] = ex2(y[k][c] - ref[c & 1]);
+                for (int c = 0; c < 4; ++c) y[n][k][c] = ex2(y[n][k][c] - ((m[n][c & 1] == -INFINITY ? 0.f : m[n][c & 1]) - LIFT));
                 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                    const uint32_t hi = pack2(y[k][2 * c], y[k][2 * c + 1]);
+                    const uint32_t hi = pack2(y[n][k][2 * c], y[n][k][2 * c + 1]);
                     pb[k][0][n][c] = transpose8(hi);
                     if constexpr (P == 2) {
                         const float2 z = unpack2(hi);
-                        pb[k][P - 1][n][c] = transpose8(pack2((y[k][2 * c] - z.x) * 2048.f, (y[k][2 * c + 1] - z.y) * 2048.f));
+                        pb[k][P - 1][n][c] = transpose8(pack2((y[n][k][2 * c] - z.x) * 2048.f, (y[n][k][2 * c + 1] - z.y) * 2048.f));
                     }
                 }
             }
             #pragma unroll
-            for (int c = 0; c < 2; ++c)
-                l[n][c] = __fmaf_rn(l[n][c], alpha[n][c], (y[0][c] + y[0][c + 2]) + (y[1][c] + y[1][c + 2]));
-        }
-        if (__any_sync(0xffffffffu, moved)) {
-            #pragma unroll
-            for (int n = 0; n < NT; ++n)
-                #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    #pragma unroll
-                    for (int c = 0; c < 4; ++c) o[n][j][c] *= alpha[n][c & 1];
+            for (int c = 0; c < 2; ++c) l[n][c] += (y[n][0][c] + y[n][0][c + 2]) + (y[n][1][c] + y[n][1][c + 2]);
         }
         #pragma unroll
         for (int k = 0; k < 2; ++k) {
@@ -306,14 +358,15 @@ struct Rows8 {
                 #pragma unroll
                 for (int hi = 0; hi < 2; ++hi) {
                     const uint32_t x = __byte_perm(wv[0][w], wv[1][w], hi ? 0x7362 : 0x5140);
-                    const uint32_t y = __byte_perm(wv[2][w], wv[3][w], hi ? 0x7362 : 0x5140);
-                    const uint32_t a[4] = {two_codes(x, false), two_codes(x, true), two_codes(y, false), two_codes(y, true)};
+                    const uint32_t z = __byte_perm(wv[2][w], wv[3][w], hi ? 0x7362 : 0x5140);
+                    const uint32_t a[4] = {two_codes<false>(x, false), two_codes<false>(x, true), two_codes<false>(z, false),
+                                           two_codes<false>(z, true)};
                     const int j = 2 * w + hi;
                     #pragma unroll
                     for (int n = 0; n < NT; ++n) {
                         float d[P][4];
                         #pragma unroll
-                        for (int z = 0; z < P; ++z) mma_f16_new(d[z], a, pb[k][z][n][0], pb[k][z][n][1]);
+                        for (int e = 0; e < P; ++e) mma_f16_from(d[e], 0.f, 0.f, a, pb[k][e][n][0], pb[k][e][n][1]);
                         #pragma unroll
                         for (int c = 0; c < 4; ++c)
                             o[n][j][c] = __fmaf_rn(P == 1 ? d[0][c] : __fmaf_rn(d[P - 1][c], 0x1p-11f, d[0][c]), vs[k], o[n][j][c]);
@@ -333,69 +386,75 @@ struct Rows8 {
                 for (int z = 4; z < 32; z <<= 1) l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], z);
     }
 
-    __device__ __forceinline__ void give(float4 (*to)[32]) const {
-        const int lane = threadIdx.x & 31;
-        #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            #pragma unroll
-            for (int j = 0; j < 8; ++j) to[n * 9 + j][lane] = make_float4(o[n][j][0], o[n][j][1], o[n][j][2], o[n][j][3]);
-            to[n * 9 + 8][lane] = make_float4(m[n][0], m[n][1], l[n][0], l[n][1]);
-        }
-    }
-    __device__ __forceinline__ void take(const float4 (*from)[32]) {
-        const int lane = threadIdx.x & 31;
-        #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const float4 ml = from[n * 9 + 8][lane];
-            const float om[2] = {ml.x, ml.y}, ol[2] = {ml.z, ml.w};
-            float fa[2], fb[2];
-            #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const float now = fmaxf(m[n][c], om[c]), ref = now == -INFINITY ? 0.f : now;
-                fa[c] = ex2(m[n][c] - ref);
-                fb[c] = ex2(om[c] - ref);
-                m[n][c] = now;
-                l[n][c] = __fmaf_rn(l[n][c], fa[c], ol[c] * fb[c]);
-            }
-            #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float4 v = from[n * 9 + j][lane];
-                o[n][j][0] = __fmaf_rn(o[n][j][0], fa[0], v.x * fb[0]);
-                o[n][j][1] = __fmaf_rn(o[n][j][1], fa[1], v.y * fb[1]);
-                o[n][j][2] = __fmaf_rn(o[n][j][2], fa[0], v.z * fb[0]);
-                o[n][j][3] = __fmaf_rn(o[n][j][3], fa[1], v.w * fb[1]);
-            }
-        }
-    }
-
-    // rows r0 .. of the pair as results, or as the part `part` (>= 0)
-    template <class O>
-    __device__ __forceinline__ void store(const Attn8Params& p, int b, int h, int row_block, int r0, int part) const {
+    // This warp's outputs [row][128] into `to`, its maxima and sums into `ml`. The 16-byte
+    // columns of row r are permuted by (r / 2) % 4: no two of the lanes that store
+    // at once meet in a bank.
+    __device__ __forceinline__ void give(float4* to, float2* ml) const {
         const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
         #pragma unroll
         for (int n = 0; n < NT; ++n)
             #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                const int in = r0 + 8 * n + 2 * t + c, r = row_block * p.block_rows + in;
-                if (r >= p.rows) continue;
-                if (part >= 0) {
-                    const size_t at = (size_t)part * p.block_rows + in;
-                    float4* to = reinterpret_cast<float4*>(p.part_o + at * kServeDim + 16 * g);
-                    #pragma unroll
-                    for (int j = 0; j < 8; j += 2)
-                        to[j / 2] = make_float4(o[n][j][c], o[n][j][c + 2], o[n][j + 1][c], o[n][j + 1][c + 2]);
-                    if (g == 0) p.part_ml[at] = make_float2(m[n][c], l[n][c]);
-                    continue;
-                }
-                const float inv = m[n][c] == -INFINITY && l[n][c] == 0.f ? 0.f : __fdiv_rn(1.f, l[n][c]);
-                O* to = static_cast<O*>(p.out) +
-                        (((size_t)b * p.n_q + r / p.group) * p.n_head + (size_t)h * p.group + r % p.group) * kServeDim + 16 * g;
+                const int r = 8 * n + 2 * t + c;
                 #pragma unroll
-                for (int j = 0; j < 8; j += 2)
-                    st4(to + 2 * j, make_float4(o[n][j][c] * inv, o[n][j][c + 2] * inv, o[n][j + 1][c] * inv, o[n][j + 1][c + 2] * inv));
+                for (int j = 0; j < 4; ++j)
+                    to[r * 32 + ((4 * g + j) ^ t)] =
+                        make_float4(o[n][2 * j][c], o[n][2 * j][c + 2], o[n][2 * j + 1][c], o[n][2 * j + 1][c + 2]);
+                if (g == 0) ml[r] = make_float2(m[n][c], l[n][c]);
             }
     }
 };
+
+// The rows of a row group from its key groups' warps (`from`: the first warp's, `step`
+// float4 from one key group to the next), a share of the rows each: results, or
+// the part `part` (>= 0). Lane i weighs row i of the share; then row by row.
+template <class O, int NT, int KG>
+__device__ __forceinline__ void finish(const Attn8Params& p, const Meta& mt, const float4* from, int step, const float2 (*ml)[16],
+                                       int ml_step, int kg, int r0, int part) {
+    constexpr int SHARE = 8 * NT / KG;
+    const int lane = threadIdx.x & 31, r = kg * SHARE + (lane < SHARE ? lane : 0), row = mt.row_block * p.block_rows + r0 + r;
+    float w[KG], M = -INFINITY, l = 0.f;
+    float2 x[KG];
+    #pragma unroll
+    for (int k = 0; k < KG; ++k) {
+        x[k] = ml[k * ml_step][r];
+        M = fmaxf(M, x[k].x);
+    }
+    #pragma unroll
+    for (int k = 0; k < KG; ++k) {
+        w[k] = ex2(x[k].x - (M == -INFINITY ? 0.f : M));
+        l = __fmaf_rn(w[k], x[k].y, l);
+    }
+    const int live = min(max(p.rows - (mt.row_block * p.block_rows + r0 + kg * SHARE), 0), SHARE);
+    size_t at;                                      // of this lane's row, in floats of a part or elements of the output
+    if (part >= 0) {
+        at = ((size_t)part * p.block_rows + r0 + r) * kServeDim;
+        if (lane < live) p.part_ml[(size_t)part * p.block_rows + r0 + r] = make_float2(M, l);
+    } else {
+        const float inv = M == -INFINITY && l == 0.f ? 0.f : __fdiv_rn(1.f, l);
+        #pragma unroll
+        for (int k = 0; k < KG; ++k) w[k] *= inv;
+        at = p.row_at(mt.b, mt.head, row);
+    }
+    #pragma unroll
+    for (int i = 0; i < SHARE; ++i) {
+        const int ri = kg * SHARE + i;
+        const size_t to = __shfl_sync(0xffffffffu, (unsigned long long)at, i) + 4 * lane;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        #pragma unroll
+        for (int k = 0; k < KG; ++k) {
+            const float4 v = from[(size_t)k * step + ri * 32 + (lane ^ ((ri >> 1) & 3))];
+            const float f = __shfl_sync(0xffffffffu, w[k], i);
+            o.x = __fmaf_rn(f, v.x, o.x);
+            o.y = __fmaf_rn(f, v.y, o.y);
+            o.z = __fmaf_rn(f, v.z, o.z);
+            o.w = __fmaf_rn(f, v.w, o.w);
+        }
+        if (i >= live) continue;
+        if (part >= 0) st4(p.part_o + to, o);
+        else st4(static_cast<O*>(p.out) + to, o);
+    }
+}
 
 // the tiles of a sequence (one at least: without keys it has zeros to write); 0
 // where its slot or length is wrong
@@ -413,57 +472,64 @@ __device__ __forceinline__ int seq_tiles(const PagesDev& pg, const Attn8Params& 
 __device__ __forceinline__ void cp_async4(void* dst, const void* src) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
 }
+__device__ __forceinline__ void cp_async16(void* dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
 __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-
-// The loading warp's place: unit by unit through its run.
-struct Place {
-    int b, slot, len, tiles, pair, head, row_block, tile;    // pair: head * row blocks + row block
-};
 
 template <class Q, class O, int NT>
 __global__ void __launch_bounds__(kE8Threads, e8_ctas(NT))
 attn_kv8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                 const __grid_constant__ PagesDev pg, const __grid_constant__ Attn8Params p) {
-    constexpr int P = std::is_same<Q, float>::value ? 2 : 1, STAGES = e8_stages(NT);
+    constexpr int P = std::is_same<Q, float>::value ? 2 : 1, STAGES = kE8Stages;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
-    Shared8<NT>& sh = *reinterpret_cast<Shared8<NT>*>(smem_raw);
+    Shared8& sh = *reinterpret_cast<Shared8*>(smem_raw);
+    uint8_t* const q_buf = smem_raw + sizeof(Shared8);
+    const int q_bytes = p.block_rows * kServeDim * (int)sizeof(Q);
     pdl_trigger();
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     volatile int* const ab = &sh.abort;
     if ((smem_u32(smem_raw) & 1023u) != 0) {        // (the swizzle counts from a 1024-byte boundary)
         if (t == 0) {
             raise(p.status, SLLM_CUDA_ERR_DEVICE);
-            p.shared[blockIdx.x] = make_int4(-1, 0, 0, 0);
+            if ((int)blockIdx.x < p.n_notes) p.notes[blockIdx.x] = make_int4(-1, 0, 0, 0);
         }
         return;
     }
     if (t == 0) {
         for (int i = 0; i < STAGES; ++i) {
-            mbar_init(&sh.full[i], 1 + 2 * kE8Blocks);
+            mbar_init(&sh.full[i], 1 + 32);
             mbar_init(&sh.empty[i], kE8Warps);
         }
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(&sh.merged[i], 1);
-            mbar_init(&sh.taken[i], 1);
-        }
-        mbar_init(&sh.passed, 1);
+        mbar_init(&sh.q_free[0], kE8Warps);
+        mbar_init(&sh.q_free[1], kE8Warps);
+        mbar_init(&sh.done, kE8Warps);
+        mbar_init(&sh.merged, kE8Warps);
         sh.abort = 0;
-        sh.start_b = p.n;
-        sh.start_rest = 0;
+        sh.start.tiles = 0;
         fence_proxy_async_smem();
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    // this CTA's run of units: a prefix sum over the sequences, each thread some of them
+    if (t == 32 * kE8Warps) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tm_k)) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tm_v)) : "memory");
+    }
+    // This CTA's run: a prefix sum over the sequences, each thread some of them. A pair
+    // counts a tile more than it has, at its end: what its start and end cost.
     const int pairs = p.n_kv * p.row_blocks, per = (p.n + kE8Threads - 1) / kE8Threads;
     const int b0 = min(t * per, p.n), b1 = min(b0 + per, p.n);
     unsigned long long mine = 0;
     for (int b = b0; b < b1; ++b) {
         int slot, len;
         const int tiles = seq_tiles(pg, p, b, &slot, &len);
-        if (tiles == 0 && blockIdx.x == 0) raise(p.status, SLLM_CUDA_ERR_ARG);
-        mine += (unsigned long long)tiles * pairs;
+        if (tiles == 0 && blockIdx.x == 0) {
+            raise(p.status, SLLM_CUDA_ERR_ARG);
+            if (p.by_pair)
+                for (int i = 0; i < pairs; ++i) p.notes[b * pairs + i] = make_int4(-1, 0, 0, 0);
+        }
+        if (tiles > 0) mine += (unsigned long long)(tiles + 1) * pairs;
     }
     unsigned long long upto = mine;
     #pragma unroll
@@ -482,17 +548,19 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
     const unsigned long long G = gridDim.x < all ? gridDim.x : all;     // runs
     const unsigned long long c = blockIdx.x;
     if (c >= G) {
-        if (t == 0) p.shared[c] = make_int4(-1, 0, 0, 0);
+        if (t == 0 && !p.by_pair) p.notes[c] = make_int4(-1, 0, 0, 0);
         return;
     }
     const unsigned long long u0 = c * all / G, u1 = (c + 1) * all / G;
     if (u0 >= upto - mine && u0 < upto) {
         unsigned long long rest = u0 - (upto - mine);
         for (int b = b0; b < b1; ++b) {
-            int slot, len;
-            const unsigned long long units = (unsigned long long)seq_tiles(pg, p, b, &slot, &len) * pairs;
+            Place x;
+            x.tiles = seq_tiles(pg, p, b, &x.slot, &x.len);
+            const unsigned long long units = x.tiles > 0 ? (unsigned long long)(x.tiles + 1) * pairs : 0;
             if (rest < units) {
-                sh.start_b = b;
+                x.b = b;
+                sh.start = x;
                 sh.start_rest = rest;
                 break;
             }
@@ -525,42 +593,47 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
             }
             return id;
         };
-        Place cur;
-        unsigned long long left = u1 - u0;
+        auto next_pair = [&](Place& x) {
+            x.tile = 0;
+            if (++x.row_block == p.row_blocks) {
+                x.row_block = 0;
+                ++x.head;
+            }
+            if (++x.pair < pairs) return true;
+            x.pair = x.head = 0;
+            return enter(x, x.b + 1);
+        };
         // (lengths that somebody writes to meanwhile end the run early, inside the arrays)
-        cur.pair = cur.tile = cur.head = cur.row_block = 0;
-        if (!enter(cur, sh.start_b) || sh.start_rest >= (unsigned long long)cur.tiles * pairs) {
-            left = 0;
-        } else {
-            cur.pair = (int)(sh.start_rest / cur.tiles);
-            cur.tile = (int)(sh.start_rest % cur.tiles);
+        Place cur = sh.start;
+        unsigned long long left = u1 - u0;
+        bool more = cur.tiles > 0;
+        if (more) {
+            cur.pair = (int)(sh.start_rest / (cur.tiles + 1));
+            cur.tile = (int)(sh.start_rest % (cur.tiles + 1));
             cur.head = cur.pair / p.row_blocks;
             cur.row_block = cur.pair % p.row_blocks;
+            if (cur.tile == cur.tiles) more = --left > 0 && next_pair(cur);
         }
-        int id = left > 0 ? ids(cur) : 0;
-        int first = 1, started = cur.tile == 0;     // of the segment: its first tile here; whether the pair starts here
+        int id = more ? ids(cur) : 0;
+        int first = 1, started = more && cur.tile == 0;     // of the segment: its first tile here; whether the pair starts here
         int4 note = make_int4(-1, 0, 0, 0);
-        uint32_t n = 0;
-        for (; left > 0 && ok; --left, ++n) {
+        uint32_t n = 0, seg = 0;
+        while (more) {
+            const bool ends = cur.tile + 1 == cur.tiles;
+            const unsigned step = ends ? 2 : 1;
             Place nxt = cur;
             int nid = 0;
-            if (left > 1) {
-                if (++nxt.tile == nxt.tiles) {
-                    nxt.tile = 0;
-                    if (++nxt.row_block == p.row_blocks) {
-                        nxt.row_block = 0;
-                        ++nxt.head;
-                    }
-                    if (++nxt.pair == pairs) {
-                        nxt.pair = nxt.head = 0;
-                        if (!enter(nxt, cur.b + 1)) left = 1;
-                    }
-                }
-                if (left > 1) nid = ids(nxt);
+            more = left > step;
+            if (more) {
+                if (ends) more = next_pair(nxt);
+                else ++nxt.tile;
+                if (more) nid = ids(nxt);
             }
             const int slot = n % STAGES;
             if (n >= STAGES && !(ok = at_wait_warp(&sh.empty[slot], (n / STAGES - 1) & 1, ab, w))) break;
-            const bool ends = cur.tile + 1 == cur.tiles, last = ends || left == 1;
+            const int qb = seg % p.q_bufs;
+            if (first && seg >= p.q_bufs && !(ok = at_wait_warp(&sh.q_free[qb], (seg / p.q_bufs - 1) & 1, ab, w))) break;
+            const bool last = ends || !more;
             const int key0 = cur.tile * kE8Keys, keys = min(kE8Keys, cur.len - key0);
             const int loads = (keys + (1 << p.page_log2) - 1) >> p.page_log2;
             if (lane == 0) {
@@ -572,8 +645,8 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
             __syncwarp();
             if (lane < loads) {
                 const int at = lane * kServeDim << p.page_log2;
-                tma_load_4d(sh.k[slot] + at, &tm_k, 0, 0, cur.head, id, &sh.full[slot]);
-                tma_load_4d(sh.v[slot] + at, &tm_v, 0, 0, cur.head, id, &sh.full[slot]);
+                tma_load_4d(sh.stage[slot].k + at, &tm_k, 0, 0, cur.head, id, &sh.full[slot]);
+                tma_load_4d(sh.stage[slot].v + at, &tm_v, 0, 0, cur.head, id, &sh.full[slot]);
             }
             const int blk = lane & (kE8Blocks - 1), from = __shfl_sync(0xffffffffu, id, (blk * kKvBlock) >> p.page_log2);
             if (lane < 2 * kE8Blocks) {
@@ -581,16 +654,30 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
                     cp_async4(&sh.sc[slot][lane], (lane < kE8Blocks ? p.ksc : p.vsc) + (size_t)from * p.scale_stride +
                                                       cur.head * (pg.page / kKvBlock) +
                                                       ((key0 + blk * kKvBlock) & (pg.page - 1)) / kKvBlock);
-                cp_async_arrive(&sh.full[slot]);
             }
-            if (last && !ends && started) {         // other runs go on with this pair
-                const unsigned long long end = u1 + (unsigned long long)(cur.tiles - cur.tile - 1);
-                note = make_int4(cur.b, cur.head, (int)min((end * G - 1) / all, G - 1), cur.row_block);
+            if (first) {                            // the pair's queries come with its first tile
+                const int r0 = cur.row_block * p.block_rows, rows = min(p.block_rows, p.rows - r0);
+                constexpr int PER = kServeDim * (int)sizeof(Q) / 16;
+                for (int i = lane; i < rows * PER; i += 32) {
+                    cp_async16(q_buf + qb * q_bytes + i * 16,
+                               static_cast<const Q*>(p.q) + p.row_at(cur.b, cur.head, r0 + i / PER) + i % PER * (16 / (int)sizeof(Q)));
+                }
+                ++seg;
+            }
+            cp_async_arrive(&sh.full[slot]);
+            if (last && started) {
+                // other runs go on with this pair: up to its last tile's
+                const unsigned long long end = u1 - left + (unsigned long long)(cur.tiles - cur.tile);
+                const int4 x = make_int4(ends ? -1 : cur.b, cur.pair, (int)c, (int)min((end * G - 1) / all, G - 1));
+                if (!ends) note = x;
+                if (p.by_pair && lane == 0) p.notes[cur.b * pairs + cur.pair] = x;
             }
             first = last;
             started = last ? 1 : started;
+            left -= step;
             cur = nxt;
             id = nid;
+            ++n;
         }
         if (ok) {
             const int slot = n % STAGES;
@@ -600,17 +687,17 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
                     sh.meta[slot] = Meta{0, 0, 0, 0, 0, E8_END};
                     mbar_arrive(&sh.full[slot]);
                 }
-                if (lane < 2 * kE8Blocks) mbar_arrive(&sh.full[slot]);
+                mbar_arrive(&sh.full[slot]);
                 ++n;
             }
         }
-        if (lane == 0) p.shared[c] = note;
+        if (lane == 0 && !p.by_pair) p.notes[c] = note;
         // copies in flight end before the CTA does, also where the others gave up
         for (uint32_t i = n > STAGES ? n - STAGES : 0; i < n; ++i) at_drain(&sh.full[i % STAGES], (i / STAGES) & 1);
     } else {
         // ---- products. A warp has its share of the blocks of a tile (key group
         // kg) for its share of the rows (row group)
-        const int RG = p.rg, KG = kE8Warps / RG, rgrp = warp % RG, kg = warp / RG, half = KG / 2;
+        const int RG = p.rg, KG = kE8Warps / RG, rgrp = warp % RG, kg = warp / RG;
         Rows8<P, NT> rows;
         rows.clear();
         uint32_t seg = 0;
@@ -622,8 +709,11 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
             const Meta mt = sh.meta[slot];
             if (mt.flags & E8_END) break;
             if (mt.flags & E8_FIRST) {
+                const int qb = seg % p.q_bufs;
                 rows.clear();
-                rows.template load<Q>(p, mt.b, mt.head, mt.row_block * p.block_rows + rgrp * 8 * NT, mt.len);
+                rows.template load<Q>(p, q_buf + qb * q_bytes, rgrp * 8 * NT, mt.row_block * p.block_rows, mt.len);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.q_free[qb]);
             }
             const int keys = min(kE8Keys, mt.len - mt.key0);
             const bool masked = mt.key0 + kE8Keys > mt.len - p.n_q + 1;
@@ -634,44 +724,34 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
                 const bool two = (blk + KG) * kKvBlock < keys;
                 const float ks[2] = {sc[blk], two ? sc[blk + KG] : 0.f};
                 const float vs[2] = {sc[kE8Blocks + blk], two ? sc[kE8Blocks + blk + KG] : 0.f};
-                rows.blocks(sh.k[slot] + blk * kKvBlock * kServeDim, sh.v[slot] + blk * kKvBlock * kServeDim,
+                rows.blocks(sh.stage[slot].k + blk * kKvBlock * kServeDim, sh.stage[slot].v + blk * kKvBlock * kServeDim,
                             KG * kKvBlock * kServeDim, ks, vs, masked, mt.key0 + blk * kKvBlock, KG * kKvBlock);
             }
             __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.empty[slot]);
-            if (!(mt.flags & E8_LAST)) continue;
-            rows.total();
+            if (!(mt.flags & E8_LAST)) {
+                if (lane == 0) mbar_arrive(&sh.empty[slot]);
+                continue;
+            }
+            // the key groups' parts into one, through the tile that nobody needs any more
             const uint32_t par = seg & 1;
             ++seg;
-            // the key groups' parts into one: the upper half gives, the lower takes
-            if (KG > 1) {
-                const int at = (kg >= half ? kg - half : kg) * RG + rgrp;
-                if (kg >= half) {
-                    if (seg > 1 && !(ok = at_wait_warp(&sh.taken[at], par ^ 1, ab, w))) break;
-                    rows.give(sh.merge[at]);
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&sh.merged[at]);
-                    continue;
-                }
-                if (!(ok = at_wait_warp(&sh.merged[at], par, ab, w))) break;
-                rows.take(sh.merge[at]);
-                __syncwarp();
-                if (KG == 4 && kg == 1) {           // (its place is free again when warp 0 has read it)
-                    rows.give(sh.merge[1]);
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&sh.passed);
-                    continue;
-                }
-                if (lane == 0) mbar_arrive(&sh.taken[at]);
-                if (KG == 4) {
-                    if (!(ok = at_wait_warp(&sh.passed, par, ab, w))) break;
-                    rows.take(sh.merge[1]);
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&sh.taken[1]);
-                }
-            }
+            if (lane == 0) mbar_arrive(&sh.done);
+            rows.total();
+            if (!(ok = at_wait_warp(&sh.done, par, ab, w))) break;
+            float4* const area = reinterpret_cast<float4*>(sh.stage[slot].k);
+            rows.give(area + warp * (8 * NT * 32), sh.ml[warp]);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.merged);
+            if (!(ok = at_wait_warp(&sh.merged, par, ab, w))) break;
             const int part = mt.flags & E8_PART0 ? 2 * (int)c : mt.flags & E8_PART1 ? 2 * (int)c + 1 : -1;
-            rows.template store<O>(p, mt.b, mt.head, mt.row_block, rgrp * 8 * NT, part);
+            const float4* const from = area + rgrp * (8 * NT * 32);
+            const int step = RG * 8 * NT * 32, r0 = rgrp * 8 * NT;
+            if (NT == 1 || KG == 4) finish<O, NT, 4>(p, mt, from, step, sh.ml + rgrp, RG, kg, r0, part);
+            else if (KG == 2) finish<O, NT, NT == 1 ? 4 : 2>(p, mt, from, step, sh.ml + rgrp, RG, kg, r0, part);
+            else finish<O, NT, NT == 1 ? 4 : 1>(p, mt, from, step, sh.ml + rgrp, RG, kg, r0, part);
+            fence_proxy_async_smem();               // before the next tile is copied over it
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.empty[slot]);
         }
     }
     if (!ok && lane == 0) raise(p.status, SLLM_CUDA_ERR_TIMEOUT);
@@ -681,21 +761,22 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
 // the join of pairs that several runs share: a row per warp, or per several
 // where rows are few
 // ---------------------------------------------------------------------------
-constexpr int kJoinWarps = 4;
+constexpr int kJoinWarps = 8;
 template <class O>
 __global__ void __launch_bounds__(32 * kJoinWarps)
 attn_kv8_join_kernel(const __grid_constant__ Attn8Params p, int per_row) {
     __shared__ float4 so[kJoinWarps][32];
     __shared__ float2 sm[kJoinWarps];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int sub = warp % per_row, in = blockIdx.y * (kJoinWarps / per_row) + warp / per_row;
     pdl_wait();
-    const int4 note = p.shared[c];
+    const int4 note = p.notes[blockIdx.x];
+    const int c = note.z;
     if (note.x < 0) return;
-    const int h = note.y, r = note.w * p.block_rows + in;
+    const int h = note.y / p.row_blocks, r = note.y % p.row_blocks * p.block_rows + in;
     const bool live = in < p.block_rows && r < p.rows;
-    // parts: the second of this CTA's, then the first of the following CTAs'
-    const int parts = note.z - c + 1;
+    // parts: the second of the first CTA's, then the first of the following CTAs'
+    const int parts = note.w - c + 1;
     auto at = [&](int i) { return (size_t)(i == 0 ? 2 * c + 1 : 2 * (c + i)) * p.block_rows + in; };
     float M = -INFINITY, l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -750,8 +831,7 @@ attn_kv8_join_kernel(const __grid_constant__ Attn8Params p, int per_row) {
     }
     if (!live) return;
     const float inv = M == -INFINITY && l == 0.f ? 0.f : __fdiv_rn(1.f, l);
-    st4(static_cast<O*>(p.out) + (((size_t)note.x * p.n_q + r / p.group) * p.n_head + (size_t)h * p.group + r % p.group) * kServeDim + 4 * lane,
-        make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+    st4(static_cast<O*>(p.out) + p.row_at(note.x, h, r) + 4 * lane, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
 }
 
 // ---------------------------------------------------------------------------
@@ -777,6 +857,9 @@ size_t work8_bytes(const Cut8& x) {
     return (size_t)x.ctas * (2 * x.block_rows * (kServeDim * sizeof(float) + sizeof(float2)) + sizeof(int4));
 }
 
+// two buffers of queries up to 32 rows, one of 64: 16 KB of f16, 32 KB of f32
+constexpr int kE8QBytes = 64 * kServeDim * 2;
+
 // one layer of a pool: a page's rows of one kv head per box
 bool encode_codes(CUtensorMap* tm, const void* base, const sllm_cuda_kv_pages& p) {
     PFN_cuTensorMapEncodeTiled_v12000 enc = tensor_map_encoder();
@@ -793,9 +876,10 @@ bool encode_codes(CUtensorMap* tm, const void* base, const sllm_cuda_kv_pages& p
 template <class Q, class O, int NT>
 cudaError_t launch8(const CUtensorMap& tk, const CUtensorMap& tv, const PagesDev& pg, const Attn8Params& a, int ctas,
                     cudaStream_t st) {
-    constexpr int kBytes = (int)sizeof(Shared8<NT>);
-    const cudaError_t e = allow_smem<attn_kv8_kernel<Q, O, NT>>(kBytes);
-    return e != cudaSuccess ? e : launch(attn_kv8_kernel<Q, O, NT>, dim3(ctas), dim3(kE8Threads), kBytes, st, false, tk, tv, pg, a);
+    constexpr int kMost = (int)sizeof(Shared8) + kE8QBytes * (int)sizeof(Q) / 2;
+    const cudaError_t e = allow_smem<attn_kv8_kernel<Q, O, NT>>(kMost);
+    const int bytes = (int)sizeof(Shared8) + a.q_bufs * a.block_rows * kServeDim * (int)sizeof(Q);
+    return e != cudaSuccess ? e : launch(attn_kv8_kernel<Q, O, NT>, dim3(ctas), dim3(kE8Threads), bytes, st, false, tk, tv, pg, a);
 }
 
 int check_shape8(const sllm_cuda_kv_pages* p, int n, int n_q, int n_head, const char* who) {
@@ -849,13 +933,18 @@ extern "C" int sllm_cuda_attn_kv8(const sllm_cuda_kv_pages* p, int32_t layer, co
     a.slots = slots;
     a.n = n; a.n_q = n_q; a.n_head = n_head; a.n_kv = p->n_head_kv; a.group = n_head / p->n_head_kv;
     a.rows = n_q * a.group;
+    a.over_group = a.group == 1 ? 0 : (uint32_t)(((1ull << 32) + a.group - 1) / a.group);
+    a.q_bufs = cut.block_rows <= 32 ? 2 : 1;
     a.rg = cut.rg; a.row_blocks = cut.row_blocks; a.block_rows = cut.block_rows;
     while ((1 << a.page_log2) < p->page_size) ++a.page_log2;
     a.wait = attn_wait_limit();
     a.status = status;
     a.part_o = static_cast<float*>(work);
     a.part_ml = reinterpret_cast<float2*>(a.part_o + (size_t)2 * cut.ctas * cut.block_rows * kServeDim);
-    a.shared = reinterpret_cast<int4*>(a.part_ml + (size_t)2 * cut.ctas * cut.block_rows);
+    a.notes = reinterpret_cast<int4*>(a.part_ml + (size_t)2 * cut.ctas * cut.block_rows);
+    const long long pairs = (long long)n * p->n_head_kv * cut.row_blocks;
+    a.by_pair = pairs <= cut.ctas;
+    a.n_notes = a.by_pair ? (int)pairs : cut.ctas;
     const PagesDev pg = pages_dev(*p);
     const cudaStream_t st = (cudaStream_t)stream;
     CUtensorMap tk, tv;
@@ -873,8 +962,9 @@ extern "C" int sllm_cuda_attn_kv8(const sllm_cuda_kv_pages* p, int32_t layer, co
             : out32 ? launch8<__half, float, 2>(tk, tv, pg, a, cut.ctas, st)
                     : launch8<__half, __half, 2>(tk, tv, pg, a, cut.ctas, st);
     CK(e, "attn_kv8 launch");
-    const int per_row = cut.block_rows <= 8 ? 4 : cut.block_rows <= 16 ? 2 : 1;
-    const dim3 grid(cut.ctas, (cut.block_rows * per_row + kJoinWarps - 1) / kJoinWarps);
+    // few pairs have many parts each: warps share a row's
+    const int share = cut.ctas / a.n_notes, per_row = !a.by_pair ? 1 : share >= 16 ? 8 : share >= 8 ? 4 : share >= 4 ? 2 : 1;
+    const dim3 grid(a.n_notes, (cut.block_rows * per_row + kJoinWarps - 1) / kJoinWarps);
     CK(out32 ? launch(attn_kv8_join_kernel<float>, grid, dim3(32 * kJoinWarps), 0, st, true, a, per_row)
              : launch(attn_kv8_join_kernel<__half>, grid, dim3(32 * kJoinWarps), 0, st, true, a, per_row),
        "attn_kv8 join");
