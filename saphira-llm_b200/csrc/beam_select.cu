@@ -6,13 +6,16 @@
 // logits, so each beam needs its own best `beams` logits only, and its lse.
 //
 // One cluster of CTAs per request; each CTA has a share of the vocabulary of
-// all beams, 8192 words of one beam at a time, 16 in the registers of a thread.
-// One pass gives the sum of exponentials (against the running maximum; terms
-// in 32 bits, sums of four of them in 64) and the few words that can be among
-// the best: those not below the least of `beams` or more disjoint parts' maxima,
-// about three per part for random logits. A list that overflows all the same
-// (many equal logits) is made again word by word. The first CTA of the cluster
-// gets the lists through distributed shared memory and merges them.
+// all beams, a piece of 8192 words of one beam at a time, 16 in the registers of
+// a thread, the pieces behind it on their way into shared memory (a thread
+// copies and reads its own words, so that needs no barrier, and 4-byte copies
+// where rows are not aligned). One pass gives the sum of exponentials (against
+// the warp's running maximum; terms in 32 bits, sums of more than 16 in 64) and
+// the few words that can be among the best: those not below the least of
+// `beams` or more disjoint parts' maxima, about three per part for random
+// logits. A list that overflows all the same (many equal logits) is made again
+// word by word. The first CTA of the cluster gets the lists through distributed
+// shared memory and merges them.
 //
 // Bound: HBM, the logits once; for one request the chain load, maximum, list,
 // merge.
@@ -32,7 +35,7 @@ constexpr int kBmPer = 16;                          // words of a thread
 constexpr int kBmPiece = kBmThreads * kBmPer;
 constexpr int kBmMost = 16;                         // beams
 constexpr int kBmList = 256;                        // words kept of a beam by a CTA
-constexpr int kBmNone = 0x7fffffff;
+constexpr int kBmRing = 2;                          // pieces in shared memory or on their way
 
 struct BeamParams {
     const float* logits;
@@ -49,26 +52,65 @@ struct BeamParams {
     int32_t* status;
 };
 
-struct Word {
-    float v;
-    int x;
-};
+// A word of a beam as one integer: its logit's order, then the words before it first.
+// 0 is none.
+using Word = unsigned long long;
+__device__ __forceinline__ uint32_t key_of(float v) {       // (+0 and -0 are equal)
+    const uint32_t u = __float_as_uint(v + 0.f);
+    return (u & 0x80000000u) != 0 ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float logit_of(uint32_t key) {
+    return __uint_as_float((key & 0x80000000u) != 0 ? key ^ 0x80000000u : ~key);
+}
+__device__ __forceinline__ Word word_of(float v, int x) { return (Word)key_of(v) << 32 | (0xffffffffu - (uint32_t)x); }
+__device__ __forceinline__ int index_of(Word w) { return (int)(0xffffffffu - (uint32_t)w); }
 
 struct BeamShared {
-    float wmax[2][kBmWarps];
-    double part[kBmMost][kBmWarps];                 // a warp's sum of exponentials, against top[b]
-    float top[kBmMost];                             // the largest logit of this CTA's share
+    uint32_t wmax[2][kBmWarps];                     // keys of the warps' largest logits of the beam so far
+    double part[kBmMost][kBmWarps];                 // a warp's sum of e^(x - ref)
+    float ref[kBmMost][kBmWarps];                   // and that ref, whole; -inf: no words
+    uint32_t floor[kBmMost];                        // key: at least `beams` words reach it
     int count[kBmMost];
     int odd;
-    Word list[kBmMost][kBmList];
-    Word best[16][kBmMost][kBmMost];                // [CTA][beam][rank], of the cluster's first CTA
-    double sum[16][kBmMost];
-    float tops[16][kBmMost];
+    float score[kBmMost];
+    int done[kBmMost], slots[kBmMost];
+    double sum[16][kBmMost];                        // [CTA][beam], of the cluster's first CTA, as are `best` and what follows
+    float refs[16][kBmMost];
     Word merged[kBmMost][kBmMost];
-    double lse[kBmMost];
+    double value[kBmMost * kBmMost];
+    double powers[96];                              // of kPowers
+
+    __device__ __forceinline__ double down_by(float d) const { return d < 96.f ? powers[(int)d] : 0.0; }
+    int pick[kBmMost];                              // the chosen: beam * beams + rank
+    Word list[kBmMost][kBmList];
+    union {
+        float4 ring[kBmRing][kBmPiece / 4];
+        Word best[16][kBmMost][kBmMost];            // [CTA][beam][rank]
+    };
 };
 
-__device__ __forceinline__ bool before(float av, int ax, float bv, int bx) { return av > bv || (av == bv && ax < bx); }
+// e^-i: references are whole, so sums against two of them differ by such a factor
+struct Powers {
+    double v[96];
+    constexpr Powers() : v() {
+        v[0] = 1.0;
+        for (int i = 1; i < 96; ++i) v[i] = v[i - 1] * 0.36787944117144232160;
+    }
+};
+__device__ const Powers kPowers;
+
+// the sum of e^(x - ref) over a thread's words
+__device__ __forceinline__ float sum_exp(const float (&x)[kBmPer], float ref) {
+    float e[kBmPer];
+    #pragma unroll
+    for (int i = 0; i < kBmPer; ++i)
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e[i]) : "f"((x[i] - ref) * 1.4426950408889634f));
+    #pragma unroll
+    for (int n = kBmPer / 2; n > 0; n >>= 1)
+        #pragma unroll
+        for (int i = 0; i < n; ++i) e[i] += e[i + n];
+    return e[0];
+}
 
 // 16 words of a thread: by fours where rows are 16-byte aligned, one by one
 // where not; a share of under 2048 words dealt out among the warps, so that each
@@ -82,47 +124,59 @@ __device__ __forceinline__ int word_at(int e, int t) {
     return (t >> 5) + kBmWarps * (t & 31) + kBmThreads * e;
 }
 
+// a thread's words of the piece at `lo`, on their way into its places of a ring entry
 template <int MODE>
-__device__ __forceinline__ void load_piece(const float* row, int lo, int hi, float (&x)[kBmPer]) {
-    constexpr bool VEC = MODE == BM_VEC;
+__device__ __forceinline__ void fetch_piece(const float* row, int lo, int hi, float4* to) {
     const int t = threadIdx.x;
     #pragma unroll
-    for (int e = 0; e < kBmPer; e += VEC ? 4 : 1) {
+    for (int e = 0; e < kBmPer; e += MODE == BM_VEC ? 4 : 1) {
         const int i = lo + word_at<MODE>(e, t);
-        if (VEC && i + 4 <= hi) {
-            const float4 v = __ldcs(reinterpret_cast<const float4*>(row + i));
-            x[e] = v.x;
-            x[e + (VEC ? 1 : 0)] = v.y;
-            x[e + (VEC ? 2 : 0)] = v.z;
-            x[e + (VEC ? 3 : 0)] = v.w;
-        } else {
+        const uint32_t dst = (uint32_t)__cvta_generic_to_shared(to + (e / 4) * kBmThreads + t) + 4 * (e & 3);
+        if (MODE == BM_VEC && i + 4 <= hi)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(row + i) : "memory");
+        else
             #pragma unroll
-            for (int j = 0; j < (VEC ? 4 : 1); ++j) x[e + j] = i + j < hi ? __ldg(row + i + j) : -INFINITY;
-        }
+            for (int j = 0; j < (MODE == BM_VEC ? 4 : 1); ++j)
+                if (i + j < hi) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst + 4 * j), "l"(row + i + j) : "memory");
+    }
+}
+__device__ __forceinline__ void fetch_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void fetch_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+template <int MODE>
+__device__ __forceinline__ void take_piece(const float4* from, int lo, int hi, float (&x)[kBmPer]) {
+    const int t = threadIdx.x;
+    #pragma unroll
+    for (int e = 0; e < kBmPer; e += 4) {
+        const float4 v = from[(e / 4) * kBmThreads + t];
+        x[e] = v.x;
+        x[e + 1] = v.y;
+        x[e + 2] = v.z;
+        x[e + 3] = v.w;
+    }
+    if (lo + kBmPiece > hi) {
+        #pragma unroll
+        for (int e = 0; e < kBmPer; ++e)
+            if (lo + word_at<MODE>(e, t) >= hi) x[e] = -INFINITY;
     }
 }
 
-// the best of a row's words that come after (pv, px), over the CTA; for lists
-// that overflowed
-__device__ Word next_word(const float* row, int lo, int hi, float pv, int px, Word* scratch) {
+// the best of a row's words behind `last`, over the CTA; for lists that overflowed
+__device__ Word next_word(const float* row, int lo, int hi, Word last, Word* scratch) {
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-    Word w{-INFINITY, kBmNone};
+    Word w = 0;
     for (int i = lo + t; i < hi; i += kBmThreads) {
-        float v = row[i];
-        if (!(v < INFINITY)) v = -INFINITY;
-        if (v > -INFINITY && before(pv, px, v, i) && before(v, i, w.v, w.x)) w = Word{v, i};
+        const float v = row[i];
+        if (!(v < INFINITY && v > -INFINITY)) continue;
+        const Word x = word_of(v, i);
+        if (x < last && x > w) w = x;
     }
     #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const float v = __shfl_xor_sync(0xffffffffu, w.v, o);
-        const int x = __shfl_xor_sync(0xffffffffu, w.x, o);
-        if (before(v, x, w.v, w.x)) w = Word{v, x};
-    }
+    for (int o = 16; o > 0; o >>= 1) w = max(w, __shfl_xor_sync(0xffffffffu, w, o));
     if (lane == 0) scratch[warp] = w;
     __syncthreads();
-    w = scratch[0];
-    for (int i = 1; i < kBmWarps; ++i)
-        if (before(scratch[i].v, scratch[i].x, w.v, w.x)) w = scratch[i];
+    for (int i = 0; i < kBmWarps; ++i) w = max(w, scratch[i]);
     __syncthreads();
     return w;
 }
@@ -137,203 +191,257 @@ beam_select_kernel(const __grid_constant__ BeamParams a) {
     const int req = blockIdx.x / C, t = threadIdx.x, lane = t & 31, warp = t >> 5, B = a.beams;
     const int lo = (int)min((long long)rank * a.per, (long long)a.V), hi = min(a.V, lo + a.per);
     const float* const rows = a.logits + (size_t)req * B * a.stride;
-    if (t < kBmMost) {
-        sh.count[t] = 0;
-        sh.top[t] = -INFINITY;
-    }
+    if (t < kBmMost) sh.count[t] = 0;
+    if (t >= kBmThreads - 96) sh.powers[t - (kBmThreads - 96)] = kPowers.v[t - (kBmThreads - 96)];
+    if (t < kBmMost * kBmWarps) sh.ref[t / kBmWarps][t % kBmWarps] = -INFINITY;
     if (t == 0) sh.odd = 0;
     // beams that have words to offer: not done, of a score above -inf
-    unsigned live = 0;
-    bool odd = false;
-    for (int b = 0; b < B; ++b) {
-        const float s = a.score[(size_t)req * B + b];
-        odd = odd || !(s < INFINITY);
-        if (s > -INFINITY && s < INFINITY && (a.done == nullptr || a.done[(size_t)req * B + b] == 0)) live |= 1u << b;
+    float my_score = 0.f;
+    int my_done = 0, my_slot = 0;
+    if (lane < B) {
+        my_score = a.score[(size_t)req * B + lane];
+        if (a.done != nullptr) my_done = a.done[(size_t)req * B + lane];
+        if (warp == 0 && a.slots != nullptr) my_slot = a.slots[(size_t)req * B + lane];
     }
-    // parts of 32 to 512 threads whose maxima bound the beams-th best
-    const int span = B <= 4 ? 128 : B <= 8 ? 64 : 32;
-    float x[kBmPer], next[kBmPer];
-    int b = live != 0 ? __ffs(live) - 1 : B, at = lo, buf = 0;
-    if (b < B && lo < hi) load_piece<MODE>(rows + (size_t)b * a.stride, lo, hi, x);
-    float top = -INFINITY, floor = -INFINITY;       // of the beam so far: its largest; what `beams` of its words reach
+    const unsigned live = __ballot_sync(0xffffffffu, lane < B && my_done == 0 && my_score > -INFINITY && my_score < INFINITY);
+    bool odd = lane < B && !(my_score < INFINITY);
+    if (warp == 0 && lane < B) {
+        sh.score[lane] = my_score;
+        sh.done[lane] = my_done;
+        sh.slots[lane] = my_slot;
+    }
+    // parts of 1 to 4 warps whose maxima bound the beams-th best
+    const int parts = B <= 4 ? 4 : B <= 8 ? 8 : 16, span = kBmWarps / parts;
+    // the pieces of this CTA in order: beam by beam
+    struct Piece {
+        int b, at;
+    };
+    auto after = [&](Piece p) {
+        p.at += kBmPiece;
+        if (p.at >= hi) {
+            const unsigned rest = live >> p.b >> 1;
+            p.b = rest != 0 ? p.b + __ffs(rest) : B;
+            p.at = lo;
+        }
+        return p;
+    };
+    float x[kBmPer];
+    Piece cur{live != 0 && lo < hi ? __ffs(live) - 1 : B, lo}, ahead = cur;
+    int buf = 0, entry = 0, fill = 0;
+    #pragma unroll
+    for (int i = 0; i < kBmRing - 1; ++i) {
+        if (ahead.b < B) {
+            fetch_piece<MODE>(rows + (size_t)ahead.b * a.stride, ahead.at, hi, sh.ring[fill]);
+            ahead = after(ahead);
+        }
+        fetch_end();
+        fill = i + 1;
+    }
+    // of the beam so far: this warp's reference, its sum, its largest logit
+    float ref = -INFINITY;
     double sum = 0.0;
+    uint32_t run = 0;
     __syncthreads();
-    while (b < B && lo < hi) {
-        int nb = b, nat = at + kBmPiece;
-        if (nat >= hi) {
-            const unsigned rest = live >> b >> 1;
-            nb = rest != 0 ? b + __ffs(rest) : B;
-            nat = lo;
+    while (cur.b < B) {
+        const int b = cur.b, at = cur.at;
+        fetch_wait<kBmRing - 2>();
+        const float4* const here = sh.ring[entry];
+        take_piece<MODE>(here, at, hi, x);
+        // (this thread's places of the entry that it read last are free)
+        if (ahead.b < B) {
+            fetch_piece<MODE>(rows + (size_t)ahead.b * a.stride, ahead.at, hi, sh.ring[fill]);
+            ahead = after(ahead);
         }
-        if (nb < B) load_piece<MODE>(rows + (size_t)nb * a.stride, nat, hi, next);
-        float m = -INFINITY;
+        fetch_end();
+        entry = entry + 1 == kBmRing ? 0 : entry + 1;
+        fill = fill + 1 == kBmRing ? 0 : fill + 1;
+        cur = after(cur);
+        float mine = x[0];
         #pragma unroll
-        for (int e = 0; e < kBmPer; ++e) {
-            const bool fine = x[e] < INFINITY;      // NaN and +inf count as -inf
-            odd = odd || !fine;
-            x[e] = fine ? x[e] : -INFINITY;
-            m = fmaxf(m, x[e]);
+        for (int e = 1; e < kBmPer; ++e) mine = fmaxf(mine, x[e]);
+        if (!(mine < INFINITY)) {                   // +inf counts as -inf, as a NaN does
+            odd = true;
+            mine = -INFINITY;
+            #pragma unroll
+            for (int e = 0; e < kBmPer; ++e) {
+                x[e] = x[e] < INFINITY ? x[e] : -INFINITY;
+                mine = fmaxf(mine, x[e]);
+            }
         }
-        const float mine = m;
-        m = warp_max(m);
-        if (lane == 0) sh.wmax[buf][warp] = m;
+        run = max(run, __reduce_max_sync(0xffffffffu, key_of(mine)));
+        if (lane == 0) sh.wmax[buf][warp] = run;
+        // this warp's exponentials, while the maxima of the others come in
+        const float want = ceilf(logit_of(run));
+        if (want > ref) {
+            sum = ref > -INFINITY ? sum * sh.down_by(want - ref) : 0.0;
+            ref = want;
+        }
+        if (ref > -INFINITY) {
+            float e = sum_exp(x, ref);
+            if (e != e) {                           // a NaN among them
+                odd = true;
+                #pragma unroll
+                for (int i = 0; i < kBmPer; ++i) x[i] = x[i] == x[i] ? x[i] : -INFINITY;
+                e = sum_exp(x, ref);
+            }
+            sum += (double)e;
+        } else {                                    // only -inf so far, and perhaps NaN
+            #pragma unroll
+            for (int i = 0; i < kBmPer; ++i) odd = odd || x[i] != x[i];
+        }
         __syncthreads();
-        // parts of span threads: span / 32 warps each
-        float w = sh.wmax[buf][lane & (kBmWarps - 1)];
-        for (int o = 1; o < span / 32; o <<= 1) w = fmaxf(w, __shfl_xor_sync(0xffffffffu, w, o));
-        float least = w, most = w;
-        #pragma unroll
-        for (int o = 1; o < kBmWarps; o <<= 1) {
-            least = fminf(least, __shfl_xor_sync(0xffffffffu, least, o));
-            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+        // the least of the parts' maxima is reached by as many words as there are parts
+        uint32_t least = 0xffffffffu;
+        if (lane < parts) {
+            least = sh.wmax[buf][lane * span];
+            if (span > 1) least = max(least, sh.wmax[buf][lane * span + 1]);
+            if (span > 2) least = max(least, max(sh.wmax[buf][lane * span + 2], sh.wmax[buf][lane * span + 3]));
         }
-        floor = fmaxf(floor, least);
+        least = __reduce_min_sync(0xffffffffu, least);
+        const float floor = logit_of(least);
         if (mine >= floor && mine > -INFINITY) {
+            unsigned hits = 0;
             #pragma unroll
-            for (int e = 0; e < kBmPer; ++e)
-                if (x[e] >= floor && x[e] > -INFINITY) {
-                    const int i = atomicAdd(&sh.count[b], 1);
-                    if (i < kBmList) sh.list[b][i] = Word{x[e], at + word_at<MODE>(e, t)};
-                }
+            for (int e = 0; e < kBmPer; ++e) hits |= x[e] >= floor && x[e] > -INFINITY ? 1u << e : 0u;
+            int i = atomicAdd(&sh.count[b], __popc(hits));
+            // (few as a rule, and still where they were read from)
+            for (; hits != 0 && i < kBmList; hits &= hits - 1, ++i) {
+                const int e = __ffs(hits) - 1;
+                const float v = reinterpret_cast<const float*>(&here[(e >> 2) * kBmThreads + t])[e & 3];
+                sh.list[b][i] = word_of(v, at + word_at<MODE>(e, t));
+            }
         }
-        if (most > top) {
-            sum = top > -INFINITY ? sum * exp((double)top - (double)most) : 0.0;
-            top = most;
-        }
-        if (top > -INFINITY) {
-            #pragma unroll
-            for (int e = 0; e < kBmPer; e += 4)
-                sum += (double)((expf(x[e] - top) + expf(x[e + 1] - top)) + (expf(x[e + 2] - top) + expf(x[e + 3] - top)));
-        }
-        if (nb != b) {
+        if (cur.b != b) {
             const double all = warp_sum_d(sum);
-            if (lane == 0) sh.part[b][warp] = all;
-            if (t == 0) sh.top[b] = top;
+            if (lane == 0) {
+                sh.part[b][warp] = all;
+                sh.ref[b][warp] = ref;
+                if (warp == 0) sh.floor[b] = least;
+            }
             sum = 0.0;
-            top = floor = -INFINITY;
+            ref = -INFINITY;
+            run = 0;
         }
         buf ^= 1;
-        b = nb;
-        at = nat;
-        #pragma unroll
-        for (int e = 0; e < kBmPer; ++e) x[e] = next[e];
     }
+    fetch_wait<0>();
     if (odd) sh.odd = 1;
     __syncthreads();
     if (t == 0 && sh.odd != 0) raise(a.status, SLLM_CUDA_ERR_ARG);
     // this CTA's best words of each beam, in order, into the first CTA's memory
     BeamShared& sh0 = *cl.map_shared_rank(&sh, 0);
-    cl.sync();                      // (the first CTA runs)
+    cl.sync();                      // the first CTA no longer needs its ring
     for (int r = warp; r < B; r += kBmWarps) {
-        const int c = sh.count[r];
+        int c = sh.count[r];
+        const float mine = lane < kBmWarps ? sh.ref[r][lane] : -INFINITY, all = warp_max(mine);
+        const double s = warp_sum_d(mine > -INFINITY ? sh.part[r][lane] * sh.down_by(all - mine) : 0.0);
         if (lane == 0) {
-            double s = 0.0;
-            if (sh.top[r] > -INFINITY)
-                for (int i = 0; i < kBmWarps; ++i) s += sh.part[r][i];
             sh0.sum[rank][r] = s;
-            sh0.tops[rank][r] = sh.top[r];
+            sh0.refs[rank][r] = all;
         }
         if (c > kBmList) continue;
+        // those that the last floor leaves, then each one's place
+        Word* const list = sh.list[r];
+        const Word least = (Word)sh.floor[r] << 32;
+        int kept = 0;
+        for (int i0 = 0; i0 < c; i0 += 32) {
+            const Word w = i0 + lane < c ? list[i0 + lane] : 0;
+            const unsigned m = __ballot_sync(0xffffffffu, w > least && w != 0);
+            __syncwarp();
+            if (w > least && w != 0) list[kept + __popc(m & ((1u << lane) - 1u))] = w;
+            kept += __popc(m);
+            __syncwarp();
+        }
+        c = kept;
         for (int i = lane; i < c || i < B; i += 32) {
             if (i >= c) {
-                sh0.best[rank][r][i] = Word{-INFINITY, kBmNone};
+                sh0.best[rank][r][i] = 0;
                 continue;
             }
-            const Word w = sh.list[r][i];
+            const Word w = list[i];
             int place = 0;
-            for (int j = 0; j < c; ++j) {
-                const Word o = sh.list[r][j];
-                place += before(o.v, o.x, w.v, w.x) ? 1 : 0;
-            }
+            #pragma unroll 4
+            for (int j = 0; j < c; ++j) place += list[j] > w ? 1 : 0;
             if (place < B) sh0.best[rank][r][place] = w;
         }
     }
     __syncthreads();
     for (int r = 0; r < B; ++r) {
         if (sh.count[r] <= kBmList) continue;       // the same for every thread
-        float pv = INFINITY;
-        int px = -1;
+        Word last = ~0ull;
         for (int i = 0; i < B; ++i) {
-            const Word w = next_word(rows + (size_t)r * a.stride, lo, hi, pv, px, sh.list[r]);
-            if (t == 0) sh0.best[rank][r][i] = w;
-            pv = w.v;
-            px = w.x;
+            last = next_word(rows + (size_t)r * a.stride, lo, hi, last, sh.list[r]);
+            if (t == 0) sh0.best[rank][r][i] = last;
         }
     }
     cl.sync();
     if (rank != 0) return;
-    // merge: a warp per beam, a lane per CTA's list
+    // merge: a warp per beam, a lane per CTA's list; then the candidates' values
     for (int r = warp; r < B; r += kBmWarps) {
-        if ((live >> r & 1) == 0) continue;
+        const bool on = (live >> r & 1) != 0;
+        const float mine = on && lane < C ? sh.refs[lane][r] : -INFINITY, all = warp_max(mine);
+        const double s = warp_sum_d(mine > -INFINITY ? sh.sum[lane][r] * sh.down_by(all - mine) : 0.0);
+        const double lse = (double)all + log(s);
         int head = 0;
+        Word w = on && lane < C ? sh.best[lane][r][0] : 0;
         for (int i = 0; i < B; ++i) {
-            Word w{-INFINITY, kBmNone};
-            if (lane < C && head < B) w = sh.best[lane][r][head];
-            Word m = w;
-            #pragma unroll
-            for (int o = 8; o > 0; o >>= 1) {
-                const float v = __shfl_xor_sync(0xffffffffu, m.v, o);
-                const int y = __shfl_xor_sync(0xffffffffu, m.x, o);
-                if (before(v, y, m.v, m.x)) m = Word{v, y};
+            // of equal logits the first CTA's: its words come first
+            const uint32_t key = (uint32_t)(w >> 32), top = __reduce_max_sync(0xffffffffu, key);
+            const int who = __ffs(__ballot_sync(0xffffffffu, key == top)) - 1;
+            if (lane == who) {
+                sh.merged[r][i] = w;
+                ++head;
+                w = w != 0 && head < B ? sh.best[lane][r][head] : 0;
             }
-            if (w.x == m.x && w.x != kBmNone) ++head;
-            if (lane == 0) sh.merged[r][i] = m;
         }
-        float top_r = lane < C ? sh.tops[lane][r] : -INFINITY;
-        const float all = warp_max(top_r);
-        double s = lane < C && top_r > -INFINITY ? sh.sum[lane][r] * exp((double)top_r - (double)all) : 0.0;
-        s = warp_sum_d(s);
-        if (lane == 0) sh.lse[r] = (double)all + log(s);
+        __syncwarp();
+        if (lane < B) {
+            double v = -INFINITY;
+            const Word m = sh.merged[r][lane];
+            if (m != 0) v = (double)sh.score[r] + ((double)logit_of((uint32_t)(m >> 32)) - lse);
+            if (!on && lane == 0 && sh.done[r] != 0 && sh.score[r] < INFINITY) v = (double)sh.score[r];
+            sh.value[r * B + lane] = v;
+        }
+    }
+    if (t < B) sh.pick[t] = -1;
+    __syncthreads();
+    // Each candidate's place among them: its beam's order is its rank's, so equal ones
+    // go by number. 2^share threads count for one.
+    const int all = B * B;
+    int share = 0;
+    while (share < 5 && all << (share + 1) <= kBmThreads) ++share;
+    const int sub = 1 << share;
+    if (t >> share < all) {
+        const int i = t >> share;
+        const double v = sh.value[i];
+        int place = 0;
+        for (int j = t & (sub - 1); j < all; j += sub) {
+            const double o = sh.value[j];
+            place += o > v || (o == v && j < i) ? 1 : 0;
+        }
+        const int in = all * sub - 32 * warp;       // of this warp's threads
+        const unsigned m = in >= 32 ? 0xffffffffu : (1u << in) - 1u;
+        for (int o = 1; o < sub; o <<= 1) place += __shfl_xor_sync(m, place, o);
+        if ((t & (sub - 1)) == 0 && place < B && v > -INFINITY) sh.pick[place] = i;
     }
     __syncthreads();
     if (warp != 0) return;
-    // the best of the beams' heads, `beams` times: a lane per beam
     const bool mine = lane < B;
-    const float score = mine ? a.score[(size_t)req * B + lane] : -INFINITY;
-    const bool is_done = mine && a.done != nullptr && a.done[(size_t)req * B + lane] != 0;
-    const bool offers = (live >> (lane & 31) & 1) != 0 && mine;
-    const bool one = is_done && score > -INFINITY && score < INFINITY;
-    int head = 0, px = -1, pb = -1;
-    double pv = 0.0;
-    int got = 0;
-    auto value = [&](int i) -> double {             // of this lane's i-th candidate
-        if (one) return i == 0 ? (double)score : -INFINITY;
-        if (!offers || i >= B || sh.merged[lane][i].x == kBmNone) return -INFINITY;
-        return (double)score + ((double)sh.merged[lane][i].v - sh.lse[lane]);
-    };
-    for (int i = 0; i < B; ++i) {
-        const double v = value(head);
-        double m = v;
-        int who = lane;
-        #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const double ov = __shfl_xor_sync(0xffffffffu, m, o);
-            const int ow = __shfl_xor_sync(0xffffffffu, who, o);
-            if (ov > m || (ov == m && ow < who)) {
-                m = ov;
-                who = ow;
-            }
-        }
-        if (!(m > -INFINITY)) break;
-        int word = 0;
-        if (lane == who) {
-            word = one ? a.eos : sh.merged[lane][head].x;
-            ++head;
-        }
-        word = __shfl_sync(0xffffffffu, word, who);
-        if (lane == i) {
-            pv = m;
-            pb = who;
-            px = word;
-        }
-        got = i + 1;
+    const int won = mine ? sh.pick[lane] : -1;
+    const int got = __popc(__ballot_sync(0xffffffffu, won >= 0));
+    double pv = -INFINITY;
+    int pb = -1, px = -1;
+    if (won >= 0) {
+        pb = won / B;
+        pv = sh.value[won];
+        px = sh.done[pb] != 0 ? a.eos : index_of(sh.merged[pb][won % B]);
     }
     // too few of weight: the first candidates of value -inf
     if (got < B) {
         int cb = 0, cx = 0;
         for (int i = got; i < B; ++i) {
             for (;;) {
-                const bool d = a.done != nullptr && a.done[(size_t)req * B + cb] != 0;
+                const bool d = sh.done[cb] != 0;
                 if (d && cx <= a.eos) cx = a.eos;
                 else if (d) cx = a.V;
                 if (cx >= a.V) {
@@ -359,15 +467,25 @@ beam_select_kernel(const __grid_constant__ BeamParams a) {
         a.parent[o] = pb;
         a.token[o] = px;
         if (a.done_out != nullptr)
-            a.done_out[o] = (a.done != nullptr && a.done[(size_t)req * B + pb] != 0) || px == a.eos ? 1 : 0;
-        if (a.src != nullptr) a.src[o] = a.slots[(size_t)req * B + pb];
+            a.done_out[o] = sh.done[pb] != 0 || px == a.eos ? 1 : 0;
+        if (a.src != nullptr) a.src[o] = sh.slots[pb];
     }
 }
 
+// The CTAs of a request: what ends first when a piece takes 0.6 us, the rest of a
+// CTA 6 us, and two CTAs are on an SM at a time.
 int beam_cluster(int n, int beams, int n_vocab, int sms) {
-    int C = 1;
-    while (C < 16 && (long long)n * C * 2 <= 4LL * sms && n_vocab / C > kBmPiece) C *= 2;
-    return C;
+    int best = 1;
+    double least = 0.0;
+    for (int C = 1; C <= 16; C *= 2) {
+        const int per = (n_vocab + C - 1) / C, pieces = (per + kBmPiece - 1) / kBmPiece;
+        const double cost = (double)(((long long)n * C + 2 * sms - 1) / (2 * sms)) * (0.6 * pieces * beams + 6.0);
+        if (C == 1 || cost < least) {
+            least = cost;
+            best = C;
+        }
+    }
+    return best;
 }
 
 }  // namespace
