@@ -6,18 +6,21 @@
 // logits, so each beam needs its own best `beams` logits only, and its lse.
 //
 // One cluster of CTAs per request; each CTA has a share of the vocabulary of
-// all beams, a piece of 8192 words of one beam at a time, 16 in the registers of
-// a thread, the pieces behind it on their way into shared memory (a thread
-// copies and reads its own words, so that needs no barrier, and 4-byte copies
-// where rows are not aligned). One pass gives the sum of exponentials (against
-// the warp's running maximum; terms in 32 bits, sums of more than 16 in 64) and
-// the few words that can be among the best: those not below the least of
-// `beams` or more disjoint parts' maxima, about three per part for random
-// logits. A list that overflows all the same (many equal logits) is made again
-// word by word. The first CTA of the cluster gets the lists through distributed
-// shared memory and merges them.
+// all beams and streams it once, a piece of 4096 words of one beam at a time, 16
+// in the registers of a thread, the pieces behind it on their way into shared
+// memory. A thread copies and reads its own words (4-byte copies where rows are
+// not aligned), and keeps of a beam its largest logit and its sum of
+// exponentials (terms and sums of 16 in 32 bits, else 64, against its own running
+// maximum rounded up), so the stream has no barrier in it. What follows is short: of a
+// beam's 256 largest-of-a-thread the `beams`-th best is a bound that at least as
+// many words reach; the few threads that reach it have their words read again
+// (from L2), those words are put in order, and the first CTA of the cluster gets
+// the lists through distributed shared memory and merges them. A list that overflows
+// (many equal logits) is made word by word instead. Keeping lists while
+// streaming, against bounds that the warps exchanged at a barrier per piece, took
+// more clocks than the exponentials: 51 us for 32 requests of 8 beams.
 //
-// Bound: HBM, the logits once; for one request the chain load, maximum, list,
+// Bound: HBM, the logits once; for one request the chain load, bound, second look,
 // merge.
 
 #include <cooperative_groups.h>
@@ -29,13 +32,12 @@ namespace cg = cooperative_groups;
 namespace sllm {
 namespace {
 
-constexpr int kBmThreads = 512;
+constexpr int kBmThreads = 256;
 constexpr int kBmWarps = kBmThreads / 32;
 constexpr int kBmPer = 16;                          // words of a thread
 constexpr int kBmPiece = kBmThreads * kBmPer;
 constexpr int kBmMost = 16;                         // beams
-constexpr int kBmList = 256;                        // words kept of a beam by a CTA
-constexpr int kBmRing = 2;                          // pieces in shared memory or on their way
+constexpr int kBmList = 128;                        // words kept of a beam by a CTA
 
 struct BeamParams {
     const float* logits;
@@ -65,12 +67,10 @@ __device__ __forceinline__ float logit_of(uint32_t key) {
 __device__ __forceinline__ Word word_of(float v, int x) { return (Word)key_of(v) << 32 | (0xffffffffu - (uint32_t)x); }
 __device__ __forceinline__ int index_of(Word w) { return (int)(0xffffffffu - (uint32_t)w); }
 
-struct BeamShared {
-    uint32_t wmax[2][kBmWarps];                     // keys of the warps' largest logits of the beam so far
+struct __align__(16) BeamShared {                 // behind it: most and list of each beam, then the ring
     double part[kBmMost][kBmWarps];                 // a warp's sum of e^(x - ref)
     float ref[kBmMost][kBmWarps];                   // and that ref, whole; -inf: no words
-    uint32_t floor[kBmMost];                        // key: at least `beams` words reach it
-    int count[kBmMost];
+    int count[kBmMost];                             // words in the list
     int odd;
     float score[kBmMost];
     int done[kBmMost], slots[kBmMost];
@@ -79,15 +79,16 @@ struct BeamShared {
     Word merged[kBmMost][kBmMost];
     double value[kBmMost * kBmMost];
     double powers[96];                              // of kPowers
+    int pick[kBmMost];                              // the chosen: beam * beams + rank
 
     __device__ __forceinline__ double down_by(float d) const { return d < 96.f ? powers[(int)d] : 0.0; }
-    int pick[kBmMost];                              // the chosen: beam * beams + rank
-    Word list[kBmMost][kBmList];
-    union {
-        float4 ring[kBmRing][kBmPiece / 4];
-        Word best[16][kBmMost][kBmMost];            // [CTA][beam][rank]
-    };
 };
+struct __align__(16) BeamRow {
+    Word list[kBmList];
+    uint32_t most[kBmThreads];      // keys of the threads' largest logits
+};
+// [CTA][beam][rank], where the first CTA's ring was
+using BeamBest = Word[kBmMost][kBmMost];
 
 // e^-i: references are whole, so sums against two of them differ by such a factor
 struct Powers {
@@ -112,31 +113,25 @@ __device__ __forceinline__ float sum_exp(const float (&x)[kBmPer], float ref) {
     return e[0];
 }
 
-// 16 words of a thread: by fours where rows are 16-byte aligned, one by one
-// where not; a share of under 2048 words dealt out among the warps, so that each
-// has some (parts without words give no bound)
-enum { BM_VEC = 0, BM_WORDS = 1, BM_DEALT = 2 };
-constexpr int kBmDealt = 4 * kBmThreads;
-template <int MODE>
+// 16 words of a thread: by fours where rows are 16-byte aligned, else one by one
+template <bool VEC>
 __device__ __forceinline__ int word_at(int e, int t) {
-    if (MODE == BM_VEC) return 4 * (t + kBmThreads * (e >> 2)) + (e & 3);
-    if (MODE == BM_WORDS) return t + kBmThreads * e;
-    return (t >> 5) + kBmWarps * (t & 31) + kBmThreads * e;
+    return VEC ? 4 * (t + kBmThreads * (e >> 2)) + (e & 3) : t + kBmThreads * e;
 }
 
 // a thread's words of the piece at `lo`, on their way into its places of a ring entry
-template <int MODE>
+template <bool VEC>
 __device__ __forceinline__ void fetch_piece(const float* row, int lo, int hi, float4* to) {
     const int t = threadIdx.x;
     #pragma unroll
-    for (int e = 0; e < kBmPer; e += MODE == BM_VEC ? 4 : 1) {
-        const int i = lo + word_at<MODE>(e, t);
+    for (int e = 0; e < kBmPer; e += VEC ? 4 : 1) {
+        const int i = lo + word_at<VEC>(e, t);
         const uint32_t dst = (uint32_t)__cvta_generic_to_shared(to + (e / 4) * kBmThreads + t) + 4 * (e & 3);
-        if (MODE == BM_VEC && i + 4 <= hi)
+        if (VEC && i + 4 <= hi)
             asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(row + i) : "memory");
         else
             #pragma unroll
-            for (int j = 0; j < (MODE == BM_VEC ? 4 : 1); ++j)
+            for (int j = 0; j < (VEC ? 4 : 1); ++j)
                 if (i + j < hi) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst + 4 * j), "l"(row + i + j) : "memory");
     }
 }
@@ -144,7 +139,7 @@ __device__ __forceinline__ void fetch_end() { asm volatile("cp.async.commit_grou
 template <int N>
 __device__ __forceinline__ void fetch_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-template <int MODE>
+template <bool VEC>
 __device__ __forceinline__ void take_piece(const float4* from, int lo, int hi, float (&x)[kBmPer]) {
     const int t = threadIdx.x;
     #pragma unroll
@@ -158,7 +153,7 @@ __device__ __forceinline__ void take_piece(const float4* from, int lo, int hi, f
     if (lo + kBmPiece > hi) {
         #pragma unroll
         for (int e = 0; e < kBmPer; ++e)
-            if (lo + word_at<MODE>(e, t) >= hi) x[e] = -INFINITY;
+            if (lo + word_at<VEC>(e, t) >= hi) x[e] = -INFINITY;
     }
 }
 
@@ -181,20 +176,96 @@ __device__ Word next_word(const float* row, int lo, int hi, Word last, Word* scr
     return w;
 }
 
-template <int MODE>
+// the words of one beam that are among this CTA's best: a warp
+template <bool VEC>
+__device__ __forceinline__ int collect(const float* row, int lo, int hi, BeamRow& sr, int B) {
+    constexpr uint32_t NONE = 0x007fffffu;          // the key of -inf
+    const int lane = threadIdx.x & 31;
+    uint32_t k[kBmWarps], left[kBmWarps];
+    #pragma unroll
+    for (int i = 0; i < kBmWarps; ++i) left[i] = k[i] = sr.most[32 * i + lane];
+    // the B-th largest; any number where there are not so many
+    uint32_t floor = 0;
+    for (int i = 0; i < B; ++i) {
+        uint32_t m = left[0];
+        #pragma unroll
+        for (int j = 1; j < kBmWarps; ++j) m = max(m, left[j]);
+        const uint32_t top = __reduce_max_sync(0xffffffffu, m);
+        floor = max(top, NONE + 1);
+        if (top <= NONE) break;
+        if (lane == __ffs(__ballot_sync(0xffffffffu, m == top)) - 1) {
+            bool gone = false;
+            #pragma unroll
+            for (int j = 0; j < kBmWarps; ++j)
+                if (!gone && left[j] == top) {
+                    left[j] = 0;
+                    gone = true;
+                }
+        }
+    }
+    // the threads that reach it, into the list's place for now
+    int* const who = reinterpret_cast<int*>(sr.list);
+    int threads = 0;
+    #pragma unroll
+    for (int i = 0; i < kBmWarps; ++i) {
+        const unsigned m = __ballot_sync(0xffffffffu, k[i] >= floor);
+        if (k[i] >= floor) who[threads + __popc(m & ((1u << lane) - 1u))] = 32 * i + lane;
+        threads += __popc(m);
+    }
+    __syncwarp();
+    if (threads > 64) return kBmList + 1;           // many equal ones
+    const int w0 = lane < threads ? who[lane] : 0, w1 = 32 + lane < threads ? who[32 + lane] : 0;
+    __syncwarp();
+    // their words again, a piece of one thread to a lane
+    const float bound = logit_of(floor);
+    const int pieces = (hi - lo + kBmPiece - 1) / kBmPiece;
+    int count = 0;
+    for (int i0 = 0; i0 < threads * pieces; i0 += 32) {
+        const int i = i0 + lane, h = i / pieces, at = lo + (i - h * pieces) * kBmPiece;
+        const int x0 = __shfl_sync(0xffffffffu, w0, h & 31), x1 = __shfl_sync(0xffffffffu, w1, h & 31), t = h < 32 ? x0 : x1;
+        float v[kBmPer];
+        #pragma unroll
+        for (int e = 0; e < kBmPer; e += VEC ? 4 : 1) {
+            const int x = at + word_at<VEC>(e, t);
+            const bool in = h < threads;
+            if (VEC && in && x + 4 <= hi) {
+                const float4 f = __ldg(reinterpret_cast<const float4*>(row + x));
+                v[e] = f.x;
+                v[e + (VEC ? 1 : 0)] = f.y;
+                v[e + (VEC ? 2 : 0)] = f.z;
+                v[e + (VEC ? 3 : 0)] = f.w;
+            } else {
+                #pragma unroll
+                for (int j = 0; j < (VEC ? 4 : 1); ++j) v[e + j] = in && x + j < hi ? __ldg(row + x + j) : -INFINITY;
+            }
+        }
+        #pragma unroll
+        for (int e = 0; e < kBmPer; ++e) {
+            const bool hit = v[e] >= bound && v[e] < INFINITY;
+            const unsigned m = __ballot_sync(0xffffffffu, hit);
+            const int to = count + __popc(m & ((1u << lane) - 1u));
+            if (hit && to < kBmList) sr.list[to] = word_of(v[e], at + word_at<VEC>(e, t));
+            count += __popc(m);
+        }
+    }
+    __syncwarp();
+    return count;
+}
+
+// RING: pieces in shared memory or on their way
+template <bool VEC, int RING>
 __global__ void __launch_bounds__(kBmThreads, 2)
 beam_select_kernel(const __grid_constant__ BeamParams a) {
     extern __shared__ __align__(16) uint8_t smem[];
     BeamShared& sh = *reinterpret_cast<BeamShared*>(smem);
+    BeamRow* const by_row = reinterpret_cast<BeamRow*>(smem + sizeof(BeamShared));
+    const int B = a.beams;
+    float4 (*const ring)[kBmPiece / 4] = reinterpret_cast<float4 (*)[kBmPiece / 4]>(by_row + B);
     cg::cluster_group cl = cg::this_cluster();
     const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank();
-    const int req = blockIdx.x / C, t = threadIdx.x, lane = t & 31, warp = t >> 5, B = a.beams;
+    const int req = blockIdx.x / C, t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const int lo = (int)min((long long)rank * a.per, (long long)a.V), hi = min(a.V, lo + a.per);
     const float* const rows = a.logits + (size_t)req * B * a.stride;
-    if (t < kBmMost) sh.count[t] = 0;
-    if (t >= kBmThreads - 96) sh.powers[t - (kBmThreads - 96)] = kPowers.v[t - (kBmThreads - 96)];
-    if (t < kBmMost * kBmWarps) sh.ref[t / kBmWarps][t % kBmWarps] = -INFINITY;
-    if (t == 0) sh.odd = 0;
     // beams that have words to offer: not done, of a score above -inf
     float my_score = 0.f;
     int my_done = 0, my_slot = 0;
@@ -203,6 +274,9 @@ beam_select_kernel(const __grid_constant__ BeamParams a) {
         if (a.done != nullptr) my_done = a.done[(size_t)req * B + lane];
         if (warp == 0 && a.slots != nullptr) my_slot = a.slots[(size_t)req * B + lane];
     }
+    if (t >= kBmThreads - 96) sh.powers[t - (kBmThreads - 96)] = kPowers.v[t - (kBmThreads - 96)];
+    for (int i = t; i < kBmMost * kBmWarps; i += kBmThreads) sh.ref[i / kBmWarps][i % kBmWarps] = -INFINITY;
+    if (t == 0) sh.odd = 0;
     const unsigned live = __ballot_sync(0xffffffffu, lane < B && my_done == 0 && my_score > -INFINITY && my_score < INFINITY);
     bool odd = lane < B && !(my_score < INFINITY);
     if (warp == 0 && lane < B) {
@@ -210,8 +284,6 @@ beam_select_kernel(const __grid_constant__ BeamParams a) {
         sh.done[lane] = my_done;
         sh.slots[lane] = my_slot;
     }
-    // parts of 1 to 4 warps whose maxima bound the beams-th best
-    const int parts = B <= 4 ? 4 : B <= 8 ? 8 : 16, span = kBmWarps / parts;
     // the pieces of this CTA in order: beam by beam
     struct Piece {
         int b, at;
@@ -225,36 +297,33 @@ beam_select_kernel(const __grid_constant__ BeamParams a) {
         }
         return p;
     };
-    float x[kBmPer];
     Piece cur{live != 0 && lo < hi ? __ffs(live) - 1 : B, lo}, ahead = cur;
-    int buf = 0, entry = 0, fill = 0;
+    int entry = 0, fill = 0;
     #pragma unroll
-    for (int i = 0; i < kBmRing - 1; ++i) {
+    for (int i = 0; i < RING - 1; ++i) {
         if (ahead.b < B) {
-            fetch_piece<MODE>(rows + (size_t)ahead.b * a.stride, ahead.at, hi, sh.ring[fill]);
+            fetch_piece<VEC>(rows + (size_t)ahead.b * a.stride, ahead.at, hi, ring[fill]);
             ahead = after(ahead);
         }
         fetch_end();
         fill = i + 1;
     }
-    // of the beam so far: this warp's reference, its sum, its largest logit
-    float ref = -INFINITY;
+    __syncthreads();                // (the powers)
+    float ref = -INFINITY, most = -INFINITY;        // of the beam so far
     double sum = 0.0;
-    uint32_t run = 0;
-    __syncthreads();
     while (cur.b < B) {
-        const int b = cur.b, at = cur.at;
-        fetch_wait<kBmRing - 2>();
-        const float4* const here = sh.ring[entry];
-        take_piece<MODE>(here, at, hi, x);
+        const int b = cur.b;
+        float x[kBmPer];
+        fetch_wait<RING - 2>();
+        take_piece<VEC>(ring[entry], cur.at, hi, x);
         // (this thread's places of the entry that it read last are free)
         if (ahead.b < B) {
-            fetch_piece<MODE>(rows + (size_t)ahead.b * a.stride, ahead.at, hi, sh.ring[fill]);
+            fetch_piece<VEC>(rows + (size_t)ahead.b * a.stride, ahead.at, hi, ring[fill]);
             ahead = after(ahead);
         }
         fetch_end();
-        entry = entry + 1 == kBmRing ? 0 : entry + 1;
-        fill = fill + 1 == kBmRing ? 0 : fill + 1;
+        entry = entry + 1 == RING ? 0 : entry + 1;
+        fill = fill + 1 == RING ? 0 : fill + 1;
         cur = after(cur);
         float mine = x[0];
         #pragma unroll
@@ -268,10 +337,8 @@ beam_select_kernel(const __grid_constant__ BeamParams a) {
                 mine = fmaxf(mine, x[e]);
             }
         }
-        run = max(run, __reduce_max_sync(0xffffffffu, key_of(mine)));
-        if (lane == 0) sh.wmax[buf][warp] = run;
-        // this warp's exponentials, while the maxima of the others come in
-        const float want = ceilf(logit_of(run));
+        most = fmaxf(most, mine);
+        const float want = ceilf(most);
         if (want > ref) {
             sum = ref > -INFINITY ? sum * sh.down_by(want - ref) : 0.0;
             ref = want;
@@ -289,80 +356,48 @@ beam_select_kernel(const __grid_constant__ BeamParams a) {
             #pragma unroll
             for (int i = 0; i < kBmPer; ++i) odd = odd || x[i] != x[i];
         }
-        __syncthreads();
-        // the least of the parts' maxima is reached by as many words as there are parts
-        uint32_t least = 0xffffffffu;
-        if (lane < parts) {
-            least = sh.wmax[buf][lane * span];
-            if (span > 1) least = max(least, sh.wmax[buf][lane * span + 1]);
-            if (span > 2) least = max(least, max(sh.wmax[buf][lane * span + 2], sh.wmax[buf][lane * span + 3]));
-        }
-        least = __reduce_min_sync(0xffffffffu, least);
-        const float floor = logit_of(least);
-        if (mine >= floor && mine > -INFINITY) {
-            unsigned hits = 0;
-            #pragma unroll
-            for (int e = 0; e < kBmPer; ++e) hits |= x[e] >= floor && x[e] > -INFINITY ? 1u << e : 0u;
-            int i = atomicAdd(&sh.count[b], __popc(hits));
-            // (few as a rule, and still where they were read from)
-            for (; hits != 0 && i < kBmList; hits &= hits - 1, ++i) {
-                const int e = __ffs(hits) - 1;
-                const float v = reinterpret_cast<const float*>(&here[(e >> 2) * kBmThreads + t])[e & 3];
-                sh.list[b][i] = word_of(v, at + word_at<MODE>(e, t));
-            }
-        }
         if (cur.b != b) {
-            const double all = warp_sum_d(sum);
+            by_row[b].most[t] = key_of(most);
+            const float top = logit_of(__reduce_max_sync(0xffffffffu, key_of(ref)));
+            const double all = warp_sum_d(ref > -INFINITY ? sum * sh.down_by(top - ref) : 0.0);
             if (lane == 0) {
                 sh.part[b][warp] = all;
-                sh.ref[b][warp] = ref;
-                if (warp == 0) sh.floor[b] = least;
+                sh.ref[b][warp] = top;
             }
             sum = 0.0;
-            ref = -INFINITY;
-            run = 0;
+            ref = most = -INFINITY;
         }
-        buf ^= 1;
     }
     fetch_wait<0>();
     if (odd) sh.odd = 1;
-    __syncthreads();
+    cl.sync();                      // the first CTA no longer needs its ring (and this CTA's shared memory is written)
     if (t == 0 && sh.odd != 0) raise(a.status, SLLM_CUDA_ERR_ARG);
     // this CTA's best words of each beam, in order, into the first CTA's memory
     BeamShared& sh0 = *cl.map_shared_rank(&sh, 0);
-    cl.sync();                      // the first CTA no longer needs its ring
+    BeamBest* const best = reinterpret_cast<BeamBest*>(ring);
+    BeamBest& best0 = *cl.map_shared_rank(best + rank, 0);
     for (int r = warp; r < B; r += kBmWarps) {
-        int c = sh.count[r];
+        const bool on = (live >> r & 1) != 0 && lo < hi;
+        const int c = on ? collect<VEC>(rows + (size_t)r * a.stride, lo, hi, by_row[r], B) : 0;
         const float mine = lane < kBmWarps ? sh.ref[r][lane] : -INFINITY, all = warp_max(mine);
         const double s = warp_sum_d(mine > -INFINITY ? sh.part[r][lane] * sh.down_by(all - mine) : 0.0);
         if (lane == 0) {
+            sh.count[r] = c;
             sh0.sum[rank][r] = s;
             sh0.refs[rank][r] = all;
         }
         if (c > kBmList) continue;
-        // those that the last floor leaves, then each one's place
-        Word* const list = sh.list[r];
-        const Word least = (Word)sh.floor[r] << 32;
-        int kept = 0;
-        for (int i0 = 0; i0 < c; i0 += 32) {
-            const Word w = i0 + lane < c ? list[i0 + lane] : 0;
-            const unsigned m = __ballot_sync(0xffffffffu, w > least && w != 0);
-            __syncwarp();
-            if (w > least && w != 0) list[kept + __popc(m & ((1u << lane) - 1u))] = w;
-            kept += __popc(m);
-            __syncwarp();
-        }
-        c = kept;
+        const Word* const list = by_row[r].list;
         for (int i = lane; i < c || i < B; i += 32) {
             if (i >= c) {
-                sh0.best[rank][r][i] = 0;
+                best0[r][i] = 0;
                 continue;
             }
             const Word w = list[i];
             int place = 0;
             #pragma unroll 4
             for (int j = 0; j < c; ++j) place += list[j] > w ? 1 : 0;
-            if (place < B) sh0.best[rank][r][place] = w;
+            if (place < B) best0[r][place] = w;
         }
     }
     __syncthreads();
@@ -370,8 +405,8 @@ beam_select_kernel(const __grid_constant__ BeamParams a) {
         if (sh.count[r] <= kBmList) continue;       // the same for every thread
         Word last = ~0ull;
         for (int i = 0; i < B; ++i) {
-            last = next_word(rows + (size_t)r * a.stride, lo, hi, last, sh.list[r]);
-            if (t == 0) sh0.best[rank][r][i] = last;
+            last = next_word(rows + (size_t)r * a.stride, lo, hi, last, by_row[r].list);
+            if (t == 0) best0[r][i] = last;
         }
     }
     cl.sync();
@@ -383,7 +418,7 @@ beam_select_kernel(const __grid_constant__ BeamParams a) {
         const double s = warp_sum_d(mine > -INFINITY ? sh.sum[lane][r] * sh.down_by(all - mine) : 0.0);
         const double lse = (double)all + log(s);
         int head = 0;
-        Word w = on && lane < C ? sh.best[lane][r][0] : 0;
+        Word w = on && lane < C ? best[lane][r][0] : 0;
         for (int i = 0; i < B; ++i) {
             // of equal logits the first CTA's: its words come first
             const uint32_t key = (uint32_t)(w >> 32), top = __reduce_max_sync(0xffffffffu, key);
@@ -391,7 +426,7 @@ beam_select_kernel(const __grid_constant__ BeamParams a) {
             if (lane == who) {
                 sh.merged[r][i] = w;
                 ++head;
-                w = w != 0 && head < B ? sh.best[lane][r][head] : 0;
+                w = w != 0 && head < B ? best[lane][r][head] : 0;
             }
         }
         __syncwarp();
@@ -472,20 +507,46 @@ beam_select_kernel(const __grid_constant__ BeamParams a) {
     }
 }
 
-// The CTAs of a request: what ends first when a piece takes 0.6 us, the rest of a
+// The CTAs of a request: what ends first when a piece takes 0.25 us, the rest of a
 // CTA 6 us, and two CTAs are on an SM at a time.
 int beam_cluster(int n, int beams, int n_vocab, int sms) {
     int best = 1;
     double least = 0.0;
     for (int C = 1; C <= 16; C *= 2) {
         const int per = (n_vocab + C - 1) / C, pieces = (per + kBmPiece - 1) / kBmPiece;
-        const double cost = (double)(((long long)n * C + 2 * sms - 1) / (2 * sms)) * (0.6 * pieces * beams + 6.0);
+        const double cost = (double)(((long long)n * C + 2 * sms - 1) / (2 * sms)) * (0.25 * pieces * beams + 6.0);
         if (C == 1 || cost < least) {
             least = cost;
             best = C;
         }
     }
     return best;
+}
+
+template <bool VEC, int RING>
+cudaError_t launch_ring(const BeamParams& a, int C, cudaStream_t st) {
+    constexpr int kRing = RING * kBmPiece * (int)sizeof(float), kMost = (int)sizeof(BeamShared) + kBmMost * (int)sizeof(BeamRow) + kRing;
+    static_assert(kRing >= (int)(16 * sizeof(BeamBest)) && sizeof(BeamShared) % 16 == 0 && sizeof(BeamRow) % 16 == 0, "");
+    const cudaError_t e1 = allow_smem<beam_select_kernel<VEC, RING>>(kMost), e2 = allow_cluster<beam_select_kernel<VEC, RING>>();
+    if (e1 != cudaSuccess || e2 != cudaSuccess) return e1 != cudaSuccess ? e1 : e2;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(a.n * C));
+    cfg.blockDim = dim3(kBmThreads);
+    cfg.dynamicSmemBytes = sizeof(BeamShared) + a.beams * sizeof(BeamRow) + kRing;
+    cfg.stream = st;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = C;
+    at.val.clusterDim.y = 1;
+    at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, beam_select_kernel<VEC, RING>, a);
+}
+// where each CTA has an SM of its own, more of its pieces are on their way
+template <bool VEC>
+cudaError_t launch_beam(const BeamParams& a, int C, int sms, cudaStream_t st) {
+    return (long long)a.n * C <= sms ? launch_ring<VEC, 8>(a, C, st) : launch_ring<VEC, 4>(a, C, st);
 }
 
 }  // namespace
@@ -520,30 +581,11 @@ extern "C" int sllm_cuda_beam_select(const float* logits, size_t row_stride, con
     a.n = n; a.beams = beams; a.V = n_vocab; a.eos = eos < 0 ? -1 : eos;
     a.score_out = score_out; a.parent = parent; a.token = token; a.done_out = done_out; a.src = src;
     a.status = status;
-    const int C = beam_cluster(n, beams, n_vocab, current_sms());
+    const int sms = current_sms(), C = beam_cluster(n, beams, n_vocab, sms);
     a.per = ((n_vocab + C - 1) / C + 3) / 4 * 4;
-    const int mode = a.per < kBmDealt ? BM_DEALT : row_stride % 4 == 0 && aligned16(logits) ? BM_VEC : BM_WORDS;
-    constexpr int kBytes = (int)sizeof(BeamShared);
-    const cudaError_t e[6] = {allow_smem<beam_select_kernel<BM_VEC>>(kBytes), allow_smem<beam_select_kernel<BM_WORDS>>(kBytes),
-                              allow_smem<beam_select_kernel<BM_DEALT>>(kBytes), allow_cluster<beam_select_kernel<BM_VEC>>(),
-                              allow_cluster<beam_select_kernel<BM_WORDS>>(), allow_cluster<beam_select_kernel<BM_DEALT>>()};
-    for (int i = 0; i < 6; ++i) CK(e[i], "beam_select attributes");
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(n * C));
-    cfg.blockDim = dim3(kBmThreads);
-    cfg.dynamicSmemBytes = kBytes;
-    cfg.stream = (cudaStream_t)stream;
-    cudaLaunchAttribute at{};
-    at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = C;
-    at.val.clusterDim.y = 1;
-    at.val.clusterDim.z = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
-    CK(mode == BM_VEC     ? cudaLaunchKernelEx(&cfg, beam_select_kernel<BM_VEC>, a)
-       : mode == BM_WORDS ? cudaLaunchKernelEx(&cfg, beam_select_kernel<BM_WORDS>, a)
-                          : cudaLaunchKernelEx(&cfg, beam_select_kernel<BM_DEALT>, a),
-       "beam_select launch");
+    const bool vec = row_stride % 4 == 0 && aligned16(logits);
+    const cudaStream_t st = (cudaStream_t)stream;
+    CK(vec ? launch_beam<true>(a, C, sms, st) : launch_beam<false>(a, C, sms, st), "beam_select launch");
     count_launches(1);
     return SLLM_CUDA_OK;
 }
