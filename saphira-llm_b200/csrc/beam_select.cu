@@ -11,7 +11,7 @@
 // memory. A thread copies and reads its own words (4-byte copies where rows are
 // not aligned), and keeps of a beam its largest logit and its sum of
 // exponentials (terms and sums of 16 in 32 bits, else 64, against its own running
-// maximum rounded up), so the stream has no barrier in it. What follows is short: of a
+// maximum, rounded up to a power of two), so the stream has no barrier in it. What follows is short: of a
 // beam's 256 largest-of-a-thread the `beams`-th best is a bound that at least as
 // many words reach; the few threads that reach it have their words read again
 // (from L2), those words are put in order, and the first CTA of the cluster gets
@@ -78,10 +78,7 @@ struct __align__(16) BeamShared {                 // behind it: most and list of
     float refs[16][kBmMost];
     Word merged[kBmMost][kBmMost];
     double value[kBmMost * kBmMost];
-    double powers[96];                              // of kPowers
     int pick[kBmMost];                              // the chosen: beam * beams + rank
-
-    __device__ __forceinline__ double down_by(float d) const { return d < 96.f ? powers[(int)d] : 0.0; }
 };
 struct __align__(16) BeamRow {
     Word list[kBmList];
@@ -90,27 +87,55 @@ struct __align__(16) BeamRow {
 // [CTA][beam][rank], where the first CTA's ring was
 using BeamBest = Word[kBmMost][kBmMost];
 
-// e^-i: references are whole, so sums against two of them differ by such a factor
-struct Powers {
-    double v[96];
-    constexpr Powers() : v() {
-        v[0] = 1.0;
-        for (int i = 1; i < 96; ++i) v[i] = v[i - 1] * 0.36787944117144232160;
-    }
-};
-__device__ const Powers kPowers;
+// Sums are of 2^(x log2 e - ref) with a whole ref, so those against two references
+// differ by a power of two. log2 e is an f32, off by kBmLog2eOff of itself: what that
+// makes of the largest logit is put right at the end. Logits beyond 2^100 count as that.
+constexpr float kBmLog2e = 1.44269502162933349609375f, kBmHuge = 0x1p100f;
+constexpr double kBmLog2eOff = 1.44269502162933349609375 / 1.4426950408889634074 - 1.0;
+__device__ __forceinline__ double down_by(float d) {        // 2^-d, d whole and not negative
+    return d < 1000.f ? __hiloint2double((1023 - (int)d) << 20, 0) : 0.0;
+}
 
-// the sum of e^(x - ref) over a thread's words
+__device__ __forceinline__ double limited(uint32_t key) { return (double)fminf(fmaxf(logit_of(key), -kBmHuge), kBmHuge); }
+
+// x += a, y += b in one instruction
+__device__ __forceinline__ void add2(float& x, float& y, float a, float b) {
+    asm("{\n\t.reg .b64 d, a;\n\t"
+        "mov.b64 d, {%0, %1};\n\tmov.b64 a, {%2, %3};\n\t"
+        "add.rn.f32x2 d, d, a;\n\t"
+        "mov.b64 {%0, %1}, d;\n\t}"
+        : "+f"(x), "+f"(y)
+        : "f"(a), "f"(b));
+}
+
+// the sum of 2^(x log2 e - ref) over a thread's words, two at a time
 __device__ __forceinline__ float sum_exp(const float (&x)[kBmPer], float ref) {
     float e[kBmPer];
     #pragma unroll
-    for (int i = 0; i < kBmPer; ++i)
-        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e[i]) : "f"((x[i] - ref) * 1.4426950408889634f));
+    for (int i = 0; i < kBmPer; i += 2) {
+        asm("{\n\t.reg .b64 x, l, r;\n\t"
+            "mov.b64 x, {%2, %3};\n\tmov.b64 l, {%4, %4};\n\tmov.b64 r, {%5, %5};\n\t"
+            "fma.rn.f32x2 x, x, l, r;\n\t"
+            "mov.b64 {%0, %1}, x;\n\t}"
+            : "=f"(e[i]), "=f"(e[i + 1])
+            : "f"(x[i]), "f"(x[i + 1]), "f"(kBmLog2e), "f"(-ref));
+        asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e[i]));
+        asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e[i + 1]));
+    }
     #pragma unroll
-    for (int n = kBmPer / 2; n > 0; n >>= 1)
+    for (int n = kBmPer / 2; n > 1; n >>= 1)
         #pragma unroll
-        for (int i = 0; i < n; ++i) e[i] += e[i + n];
-    return e[0];
+        for (int i = 0; i < n; i += 2) add2(e[i], e[i + 1], e[i + n], e[i + n + 1]);
+    return e[0] + e[1];
+}
+
+// the largest of a thread's words, NaN if there is one
+__device__ __forceinline__ float max_of(const float (&x)[kBmPer]) {
+    float m = x[0];
+    #pragma unroll
+    for (int i = 1; i + 1 < kBmPer; i += 2) asm("max.NaN.f32 %0, %0, %1, %2;" : "+f"(m) : "f"(x[i]), "f"(x[i + 1]));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(x[kBmPer - 1]));
+    return m;
 }
 
 // 16 words of a thread: by fours where rows are 16-byte aligned, else one by one
@@ -216,37 +241,46 @@ __device__ __forceinline__ int collect(const float* row, int lo, int hi, BeamRow
     if (threads > 64) return kBmList + 1;           // many equal ones
     const int w0 = lane < threads ? who[lane] : 0, w1 = 32 + lane < threads ? who[32 + lane] : 0;
     __syncwarp();
-    // their words again, a piece of one thread to a lane
+    // their words again, four of one thread's piece to a lane
     const float bound = logit_of(floor);
-    const int pieces = (hi - lo + kBmPiece - 1) / kBmPiece;
+    const int pieces = (hi - lo + kBmPiece - 1) / kBmPiece, all = threads * pieces * (kBmPer / 4);
     int count = 0;
-    for (int i0 = 0; i0 < threads * pieces; i0 += 32) {
-        const int i = i0 + lane, h = i / pieces, at = lo + (i - h * pieces) * kBmPiece;
-        const int x0 = __shfl_sync(0xffffffffu, w0, h & 31), x1 = __shfl_sync(0xffffffffu, w1, h & 31), t = h < 32 ? x0 : x1;
-        float v[kBmPer];
-        #pragma unroll
-        for (int e = 0; e < kBmPer; e += VEC ? 4 : 1) {
-            const int x = at + word_at<VEC>(e, t);
-            const bool in = h < threads;
-            if (VEC && in && x + 4 <= hi) {
-                const float4 f = __ldg(reinterpret_cast<const float4*>(row + x));
-                v[e] = f.x;
-                v[e + (VEC ? 1 : 0)] = f.y;
-                v[e + (VEC ? 2 : 0)] = f.z;
-                v[e + (VEC ? 3 : 0)] = f.w;
-            } else {
-                #pragma unroll
-                for (int j = 0; j < (VEC ? 4 : 1); ++j) v[e + j] = in && x + j < hi ? __ldg(row + x + j) : -INFINITY;
-            }
+    auto place = [&](int i, int* x) {               // the first of lane's four words of batch i, or none
+        const int u = (i + lane) / (kBmPer / 4), h = u / pieces;
+        const int x0 = __shfl_sync(0xffffffffu, w0, h & 31), x1 = __shfl_sync(0xffffffffu, w1, h & 31);
+        *x = lo + (u - h * pieces) * kBmPiece + word_at<VEC>(lane % (kBmPer / 4) * 4, h < 32 ? x0 : x1);
+        return i + lane < all;
+    };
+    auto load = [&](int x, bool in) {
+        float4 v = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        constexpr int STEP = VEC ? 1 : kBmThreads;
+        if (VEC && in && x + 4 <= hi) return __ldg(reinterpret_cast<const float4*>(row + x));
+        if (in && x < hi) v.x = __ldg(row + x);
+        if (in && x + STEP < hi) v.y = __ldg(row + x + STEP);
+        if (in && x + 2 * STEP < hi) v.z = __ldg(row + x + 2 * STEP);
+        if (in && x + 3 * STEP < hi) v.w = __ldg(row + x + 3 * STEP);
+        return v;
+    };
+    int x, nx = 0;
+    bool in = place(0, &x);
+    float4 v = load(x, in), nv = v;
+    #pragma unroll 1
+    for (int i = 0; i < all; i += 32) {
+        if (i + 32 < all) {
+            in = place(i + 32, &nx);
+            nv = load(nx, in);
         }
         #pragma unroll
-        for (int e = 0; e < kBmPer; ++e) {
-            const bool hit = v[e] >= bound && v[e] < INFINITY;
+        for (int e = 0; e < 4; ++e) {
+            const float f = e == 0 ? v.x : e == 1 ? v.y : e == 2 ? v.z : v.w;
+            const bool hit = f >= bound && f < INFINITY;
             const unsigned m = __ballot_sync(0xffffffffu, hit);
             const int to = count + __popc(m & ((1u << lane) - 1u));
-            if (hit && to < kBmList) sr.list[to] = word_of(v[e], at + word_at<VEC>(e, t));
+            if (hit && to < kBmList) sr.list[to] = word_of(f, x + e * (VEC ? 1 : kBmThreads));
             count += __popc(m);
         }
+        x = nx;
+        v = nv;
     }
     __syncwarp();
     return count;
@@ -274,7 +308,6 @@ beam_select_kernel(const __grid_constant__ BeamParams a) {
         if (a.done != nullptr) my_done = a.done[(size_t)req * B + lane];
         if (warp == 0 && a.slots != nullptr) my_slot = a.slots[(size_t)req * B + lane];
     }
-    if (t >= kBmThreads - 96) sh.powers[t - (kBmThreads - 96)] = kPowers.v[t - (kBmThreads - 96)];
     for (int i = t; i < kBmMost * kBmWarps; i += kBmThreads) sh.ref[i / kBmWarps][i % kBmWarps] = -INFINITY;
     if (t == 0) sh.odd = 0;
     const unsigned live = __ballot_sync(0xffffffffu, lane < B && my_done == 0 && my_score > -INFINITY && my_score < INFINITY);
@@ -308,7 +341,6 @@ beam_select_kernel(const __grid_constant__ BeamParams a) {
         fetch_end();
         fill = i + 1;
     }
-    __syncthreads();                // (the powers)
     float ref = -INFINITY, most = -INFINITY;        // of the beam so far
     double sum = 0.0;
     while (cur.b < B) {
@@ -325,41 +357,30 @@ beam_select_kernel(const __grid_constant__ BeamParams a) {
         entry = entry + 1 == RING ? 0 : entry + 1;
         fill = fill + 1 == RING ? 0 : fill + 1;
         cur = after(cur);
-        float mine = x[0];
-        #pragma unroll
-        for (int e = 1; e < kBmPer; ++e) mine = fmaxf(mine, x[e]);
-        if (!(mine < INFINITY)) {                   // +inf counts as -inf, as a NaN does
+        float mine = max_of(x);
+        if (!(mine < INFINITY)) {                   // +inf and NaN count as -inf
             odd = true;
-            mine = -INFINITY;
             #pragma unroll
-            for (int e = 0; e < kBmPer; ++e) {
-                x[e] = x[e] < INFINITY ? x[e] : -INFINITY;
-                mine = fmaxf(mine, x[e]);
-            }
+            for (int e = 0; e < kBmPer; ++e) x[e] = x[e] < INFINITY ? x[e] : -INFINITY;
+            mine = max_of(x);
         }
         most = fmaxf(most, mine);
-        const float want = ceilf(most);
-        if (want > ref) {
-            sum = ref > -INFINITY ? sum * sh.down_by(want - ref) : 0.0;
-            ref = want;
-        }
-        if (ref > -INFINITY) {
-            float e = sum_exp(x, ref);
-            if (e != e) {                           // a NaN among them
-                odd = true;
-                #pragma unroll
-                for (int i = 0; i < kBmPer; ++i) x[i] = x[i] == x[i] ? x[i] : -INFINITY;
-                e = sum_exp(x, ref);
-            }
-            sum += (double)e;
-        } else {                                    // only -inf so far, and perhaps NaN
+        if (!(fabsf(most) <= kBmHuge)) {
             #pragma unroll
-            for (int i = 0; i < kBmPer; ++i) odd = odd || x[i] != x[i];
+            for (int e = 0; e < kBmPer; ++e) x[e] = x[e] > -INFINITY ? fminf(fmaxf(x[e], -kBmHuge), kBmHuge) : x[e];
+        }
+        if (most > -INFINITY) {
+            const float want = ceilf(fminf(fmaxf(most, -kBmHuge), kBmHuge) * kBmLog2e);
+            if (want > ref) {
+                sum = ref > -INFINITY ? sum * down_by(want - ref) : 0.0;
+                ref = want;
+            }
+            sum += (double)sum_exp(x, ref);
         }
         if (cur.b != b) {
             by_row[b].most[t] = key_of(most);
             const float top = logit_of(__reduce_max_sync(0xffffffffu, key_of(ref)));
-            const double all = warp_sum_d(ref > -INFINITY ? sum * sh.down_by(top - ref) : 0.0);
+            const double all = warp_sum_d(ref > -INFINITY ? sum * down_by(top - ref) : 0.0);
             if (lane == 0) {
                 sh.part[b][warp] = all;
                 sh.ref[b][warp] = top;
@@ -380,7 +401,7 @@ beam_select_kernel(const __grid_constant__ BeamParams a) {
         const bool on = (live >> r & 1) != 0 && lo < hi;
         const int c = on ? collect<VEC>(rows + (size_t)r * a.stride, lo, hi, by_row[r], B) : 0;
         const float mine = lane < kBmWarps ? sh.ref[r][lane] : -INFINITY, all = warp_max(mine);
-        const double s = warp_sum_d(mine > -INFINITY ? sh.part[r][lane] * sh.down_by(all - mine) : 0.0);
+        const double s = warp_sum_d(mine > -INFINITY ? sh.part[r][lane] * down_by(all - mine) : 0.0);
         if (lane == 0) {
             sh.count[r] = c;
             sh0.sum[rank][r] = s;
@@ -415,8 +436,7 @@ beam_select_kernel(const __grid_constant__ BeamParams a) {
     for (int r = warp; r < B; r += kBmWarps) {
         const bool on = (live >> r & 1) != 0;
         const float mine = on && lane < C ? sh.refs[lane][r] : -INFINITY, all = warp_max(mine);
-        const double s = warp_sum_d(mine > -INFINITY ? sh.sum[lane][r] * sh.down_by(all - mine) : 0.0);
-        const double lse = (double)all + log(s);
+        const double s = warp_sum_d(mine > -INFINITY ? sh.sum[lane][r] * down_by(all - mine) : 0.0);
         int head = 0;
         Word w = on && lane < C ? best[lane][r][0] : 0;
         for (int i = 0; i < B; ++i) {
@@ -430,10 +450,11 @@ beam_select_kernel(const __grid_constant__ BeamParams a) {
             }
         }
         __syncwarp();
+        const double lse = ((double)all + log2(s)) * 0.69314718055994530942 - limited((uint32_t)(sh.merged[r][0] >> 32)) * kBmLog2eOff;
         if (lane < B) {
             double v = -INFINITY;
             const Word m = sh.merged[r][lane];
-            if (m != 0) v = (double)sh.score[r] + ((double)logit_of((uint32_t)(m >> 32)) - lse);
+            if (m != 0) v = (double)sh.score[r] + (limited((uint32_t)(m >> 32)) - lse);
             if (!on && lane == 0 && sh.done[r] != 0 && sh.score[r] < INFINITY) v = (double)sh.score[r];
             sh.value[r * B + lane] = v;
         }
