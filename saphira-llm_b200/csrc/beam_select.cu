@@ -37,7 +37,7 @@ constexpr int kBmWarps = kBmThreads / 32;
 constexpr int kBmPer = 16;                          // words of a thread
 constexpr int kBmPiece = kBmThreads * kBmPer;
 constexpr int kBmMost = 16;                         // beams
-constexpr int kBmList = 128;                        // words kept of a beam by a CTA
+constexpr int kBmList = 64;                         // words kept of a beam by a CTA
 
 struct BeamParams {
     const float* logits;
@@ -82,7 +82,8 @@ struct __align__(16) BeamShared {                 // behind it: most and list of
 };
 struct __align__(16) BeamRow {
     Word list[kBmList];
-    uint32_t most[kBmThreads];      // keys of the threads' largest logits
+    uint32_t most[kBmThreads];      // keys of the threads' largest logits; later the pieces to look at again
+    uint32_t next[kBmThreads];      // the piece that has it, and 16 bits of the largest key of the others
 };
 // [CTA][beam][rank], where the first CTA's ring was
 using BeamBest = Word[kBmMost][kBmMost];
@@ -209,47 +210,63 @@ __device__ __forceinline__ int collect(const float* row, int lo, int hi, BeamRow
     uint32_t k[kBmWarps], left[kBmWarps];
     #pragma unroll
     for (int i = 0; i < kBmWarps; ++i) left[i] = k[i] = sr.most[32 * i + lane];
+    static_assert(kBmWarps == 8, "a sorting network of eight");
+    constexpr int NET[19][2] = {{0, 1}, {2, 3}, {4, 5}, {6, 7}, {0, 2}, {1, 3}, {4, 6}, {5, 7}, {1, 2}, {5, 6},
+                                {0, 4}, {1, 5}, {2, 6}, {3, 7}, {2, 4}, {3, 5}, {1, 2}, {3, 4}, {5, 6}};
+    #pragma unroll
+    for (int i = 0; i < 19; ++i) {
+        const uint32_t x = left[NET[i][0]], y = left[NET[i][1]];
+        left[NET[i][0]] = max(x, y);
+        left[NET[i][1]] = min(x, y);
+    }
     // the B-th largest; any number where there are not so many
     uint32_t floor = 0;
     for (int i = 0; i < B; ++i) {
-        uint32_t m = left[0];
-        #pragma unroll
-        for (int j = 1; j < kBmWarps; ++j) m = max(m, left[j]);
-        const uint32_t top = __reduce_max_sync(0xffffffffu, m);
+        const uint32_t top = __reduce_max_sync(0xffffffffu, left[0]);
         floor = max(top, NONE + 1);
         if (top <= NONE) break;
-        if (lane == __ffs(__ballot_sync(0xffffffffu, m == top)) - 1) {
-            bool gone = false;
-            #pragma unroll
-            for (int j = 0; j < kBmWarps; ++j)
-                if (!gone && left[j] == top) {
-                    left[j] = 0;
-                    gone = true;
-                }
-        }
+        const bool mine = lane == __ffs(__ballot_sync(0xffffffffu, left[0] == top)) - 1;
+        #pragma unroll
+        for (int j = 0; j < kBmWarps; ++j) left[j] = mine ? (j + 1 < kBmWarps ? left[j + 1] : 0u) : left[j];
     }
-    // the threads that reach it, into the list's place for now
-    int* const who = reinterpret_cast<int*>(sr.list);
-    int threads = 0;
+    // the pieces that may hold words as large: of each thread that reaches it the one
+    // with its largest, all where another may reach it, too
+    const int pieces = (hi - lo + kBmPiece - 1) / kBmPiece;
+    int tasks = 0;
+    __syncwarp();                                   // (all keys are in registers)
     #pragma unroll
     for (int i = 0; i < kBmWarps; ++i) {
-        const unsigned m = __ballot_sync(0xffffffffu, k[i] >= floor);
-        if (k[i] >= floor) who[threads + __popc(m & ((1u << lane) - 1u))] = 32 * i + lane;
-        threads += __popc(m);
+        const bool in = k[i] >= floor;
+        const unsigned m = __ballot_sync(0xffffffffu, in);
+        if (m == 0) continue;
+        const uint32_t nx = sr.next[32 * i + lane], who = (uint32_t)(32 * i + lane) << 16;
+        const bool many = in && (nx >> 16) >= (floor >> 16);
+        const int n = !in ? 0 : many ? pieces : 1;
+        int before = __popc(m & ((1u << lane) - 1u)), total = __popc(m);
+        if (__any_sync(0xffffffffu, many)) {
+            int upto = n;
+            #pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += y;
+            }
+            before = upto - n;
+            total = __shfl_sync(0xffffffffu, upto, 31);
+        }
+        if (tasks + total > kBmThreads) return kBmList + 1;              // many equal ones
+        for (int j = 0; j < n; ++j) sr.most[tasks + before + j] = who | (many ? (uint32_t)j : nx & 0xffffu);
+        tasks += total;
     }
     __syncwarp();
-    if (threads > 64) return kBmList + 1;           // many equal ones
-    const int w0 = lane < threads ? who[lane] : 0, w1 = 32 + lane < threads ? who[32 + lane] : 0;
-    __syncwarp();
-    // their words again, four of one thread's piece to a lane
+    // their words again, four to a lane
     const float bound = logit_of(floor);
-    const int pieces = (hi - lo + kBmPiece - 1) / kBmPiece, all = threads * pieces * (kBmPer / 4);
+    const int all = tasks * (kBmPer / 4);
     int count = 0;
     auto place = [&](int i, int* x) {               // the first of lane's four words of batch i, or none
-        const int u = (i + lane) / (kBmPer / 4), h = u / pieces;
-        const int x0 = __shfl_sync(0xffffffffu, w0, h & 31), x1 = __shfl_sync(0xffffffffu, w1, h & 31);
-        *x = lo + (u - h * pieces) * kBmPiece + word_at<VEC>(lane % (kBmPer / 4) * 4, h < 32 ? x0 : x1);
-        return i + lane < all;
+        const bool in = i + lane < all;
+        const uint32_t task = in ? sr.most[(i + lane) / (kBmPer / 4)] : 0;
+        *x = lo + (int)(task & 0xffffu) * kBmPiece + word_at<VEC>(lane % (kBmPer / 4) * 4, (int)(task >> 16));
+        return in;
     };
     auto load = [&](int x, bool in) {
         float4 v = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
@@ -288,7 +305,7 @@ __device__ __forceinline__ int collect(const float* row, int lo, int hi, BeamRow
 
 // RING: pieces in shared memory or on their way
 template <bool VEC, int RING>
-__global__ void __launch_bounds__(kBmThreads, 2)
+__global__ void __launch_bounds__(kBmThreads, 3)
 beam_select_kernel(const __grid_constant__ BeamParams a) {
     extern __shared__ __align__(16) uint8_t smem[];
     BeamShared& sh = *reinterpret_cast<BeamShared*>(smem);
@@ -341,7 +358,10 @@ beam_select_kernel(const __grid_constant__ BeamParams a) {
         fetch_end();
         fill = i + 1;
     }
-    float ref = -INFINITY, most = -INFINITY;        // of the beam so far
+    // of the beam so far: the reference, this thread's largest logit, the piece that
+    // has it, the largest of the other pieces
+    float ref = -INFINITY, most = -INFINITY, other = -INFINITY;
+    int piece = 0, at_piece = 0;
     double sum = 0.0;
     while (cur.b < B) {
         const int b = cur.b;
@@ -364,7 +384,12 @@ beam_select_kernel(const __grid_constant__ BeamParams a) {
             for (int e = 0; e < kBmPer; ++e) x[e] = x[e] < INFINITY ? x[e] : -INFINITY;
             mine = max_of(x);
         }
-        most = fmaxf(most, mine);
+        other = fmaxf(other, fminf(most, mine));
+        if (mine > most) {
+            most = mine;
+            at_piece = piece;
+        }
+        ++piece;
         if (!(fabsf(most) <= kBmHuge)) {
             #pragma unroll
             for (int e = 0; e < kBmPer; ++e) x[e] = x[e] > -INFINITY ? fminf(fmaxf(x[e], -kBmHuge), kBmHuge) : x[e];
@@ -379,6 +404,7 @@ beam_select_kernel(const __grid_constant__ BeamParams a) {
         }
         if (cur.b != b) {
             by_row[b].most[t] = key_of(most);
+            by_row[b].next[t] = (key_of(other) & 0xffff0000u) | (uint32_t)at_piece;
             const float top = logit_of(__reduce_max_sync(0xffffffffu, key_of(ref)));
             const double all = warp_sum_d(ref > -INFINITY ? sum * down_by(top - ref) : 0.0);
             if (lane == 0) {
@@ -386,7 +412,8 @@ beam_select_kernel(const __grid_constant__ BeamParams a) {
                 sh.ref[b][warp] = top;
             }
             sum = 0.0;
-            ref = most = -INFINITY;
+            ref = most = other = -INFINITY;
+            piece = at_piece = 0;
         }
     }
     fetch_wait<0>();
@@ -529,13 +556,13 @@ beam_select_kernel(const __grid_constant__ BeamParams a) {
 }
 
 // The CTAs of a request: what ends first when a piece takes 0.25 us, the rest of a
-// CTA 6 us, and two CTAs are on an SM at a time.
+// CTA 6 us, and three CTAs are on an SM at a time.
 int beam_cluster(int n, int beams, int n_vocab, int sms) {
     int best = 1;
     double least = 0.0;
     for (int C = 1; C <= 16; C *= 2) {
         const int per = (n_vocab + C - 1) / C, pieces = (per + kBmPiece - 1) / kBmPiece;
-        const double cost = (double)(((long long)n * C + 2 * sms - 1) / (2 * sms)) * (0.25 * pieces * beams + 6.0);
+        const double cost = (double)(((long long)n * C + 3 * sms - 1) / (3 * sms)) * (0.25 * pieces * beams + 6.0);
         if (C == 1 || cost < least) {
             least = cost;
             best = C;
@@ -547,7 +574,7 @@ int beam_cluster(int n, int beams, int n_vocab, int sms) {
 template <bool VEC, int RING>
 cudaError_t launch_ring(const BeamParams& a, int C, cudaStream_t st) {
     constexpr int kRing = RING * kBmPiece * (int)sizeof(float), kMost = (int)sizeof(BeamShared) + kBmMost * (int)sizeof(BeamRow) + kRing;
-    static_assert(kRing >= (int)(16 * sizeof(BeamBest)) && sizeof(BeamShared) % 16 == 0 && sizeof(BeamRow) % 16 == 0, "");
+    static_assert(kRing >= (int)(16 * sizeof(BeamBest)) && kBmPiece * 256 >= 1 << 20 && sizeof(BeamShared) % 16 == 0 && sizeof(BeamRow) % 16 == 0, "");
     const cudaError_t e1 = allow_smem<beam_select_kernel<VEC, RING>>(kMost), e2 = allow_cluster<beam_select_kernel<VEC, RING>>();
     if (e1 != cudaSuccess || e2 != cudaSuccess) return e1 != cudaSuccess ? e1 : e2;
     cudaLaunchConfig_t cfg{};
@@ -564,10 +591,10 @@ cudaError_t launch_ring(const BeamParams& a, int C, cudaStream_t st) {
     cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, beam_select_kernel<VEC, RING>, a);
 }
-// where each CTA has an SM of its own, more of its pieces are on their way
+// where each CTA has an SM of its own (and clusters find room), more of its pieces are on their way
 template <bool VEC>
 cudaError_t launch_beam(const BeamParams& a, int C, int sms, cudaStream_t st) {
-    return (long long)a.n * C <= sms ? launch_ring<VEC, 8>(a, C, st) : launch_ring<VEC, 4>(a, C, st);
+    return 2LL * a.n * C <= sms ? launch_ring<VEC, 8>(a, C, st) : launch_ring<VEC, 3>(a, C, st);
 }
 
 }  // namespace
