@@ -37,7 +37,7 @@ struct Append8Params {
     float* vsc;
     size_t page_stride, scale_stride;       // codes, scales from a page to the next
     int n_tokens, n_head, n_kv, n_ctx;
-    int kv_ctas;                    // CTAs of k and v; those of q behind them
+    int kv_ctas, kv_rows;           // CTAs of k and v (those of q behind them), and the heads of k and v that one has
     int32_t* status;
 };
 
@@ -104,32 +104,39 @@ __device__ __forceinline__ int page_at(const PagesDev& p, int slot, int pos) {
 // append. Of the list's tokens those of one block are a run; a warp takes one
 // run of one head of k or of v, all of its (up to 16) tokens in registers: lane
 // l of a half-warp holds elements 4l .. and 64 + 4l .. of a token, the
-// rotation's pairs. A CTA has 16 entries of the list and one head; whether they
-// hold one run (a prompt) or 16 (a decode step) its eight warps share what there
-// is. The q rows are rotated by CTAs of their own, eight rows a warp.
+// rotation's pairs. A CTA has 16 entries of the list and some heads, and its eight
+// warps share the runs times heads: one or two runs in a prompt, 16 in a
+// decode step. With one head a CTA a step of few tokens has one such pair a warp;
+// with eight a long prompt has (one head a CTA left six warps of eight idle: 67 us
+// for 4099 tokens of 8 heads). The pages are looked up once for all pairs, a lane
+// per entry, behind the first pair's loads. The q rows are rotated by CTAs of
+// their own, eight rows a warp.
 // ---------------------------------------------------------------------------
-template <class O>
-__device__ __forceinline__ void append_run(const PagesDev& p, const Append8Params& a, int e0, int count, int slot, int pos0,
-                                           int h, bool is_v) {
-    const int lane = threadIdx.x & 31, half = lane >> 4, l4 = 4 * (lane & 15);
-    const float* const x = is_v ? a.v + h * kServeDim : a.k + h * kServeDim;
-    const size_t xs = is_v ? a.vs : a.ks;
+struct Run {
     RotPair r[8];
-    #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int t = 2 * i + half;
-        if (t < count) {
-            const float* row = x + (size_t)(e0 + t) * xs + l4;
-            r[i].lo = __ldcs(reinterpret_cast<const float4*>(row));
-            r[i].hi = __ldcs(reinterpret_cast<const float4*>(row + 64));
+
+    __device__ __forceinline__ void load(const Append8Params& a, int e0, int count, int h, bool is_v) {
+        const int lane = threadIdx.x & 31, half = lane >> 4, l4 = 4 * (lane & 15);
+        const float* const x = (is_v ? a.v : a.k) + h * kServeDim + l4;
+        const size_t xs = is_v ? a.vs : a.ks;
+        #pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int t = 2 * i + half;
+            if (t < count) {
+                const float* row = x + (size_t)(e0 + t) * xs;
+                r[i].lo = __ldcs(reinterpret_cast<const float4*>(row));
+                r[i].hi = __ldcs(reinterpret_cast<const float4*>(row + 64));
+            }
         }
     }
-    const int id = page_at(p, slot, pos0);
-    // a shared page is never written: its other owners would change
-    if (id < 0 || p.refs[id] != 1) {
-        if (lane == 0) raise(a.status, SLLM_CUDA_ERR_ARG);
-        return;
-    }
+};
+
+// tokens e0 .. e0 + count - 1 into page `id`, their first position pos0
+template <class O>
+__device__ __forceinline__ void append_run(const PagesDev& p, const Append8Params& a, Run& run, int e0, int count, int id, int pos0,
+                                           int h, bool is_v) {
+    RotPair (&r)[8] = run.r;
+    const int lane = threadIdx.x & 31, half = lane >> 4, l4 = 4 * (lane & 15);
     const int block = pos0 % p.page / kKvBlock, row0 = pos0 % kKvBlock;
     float* const sc = (is_v ? a.vsc : a.ksc) + (size_t)id * a.scale_stride + (size_t)h * (p.page / kKvBlock) + block;
     int8_t* const codes = (is_v ? a.vp : a.kp) + (size_t)id * a.page_stride + ((size_t)h * p.page + block * kKvBlock) * kServeDim;
@@ -188,7 +195,9 @@ __global__ void __launch_bounds__(32 * kK8Warps)
 kv8_append_kernel(const __grid_constant__ PagesDev p, const __grid_constant__ Append8Params a) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if ((int)blockIdx.x < a.kv_ctas) {
-        const int row = (int)blockIdx.x % (2 * a.n_kv), e0 = (int)blockIdx.x / (2 * a.n_kv) * kK8Entries;
+        const int groups = (2 * a.n_kv + a.kv_rows - 1) / a.kv_rows;
+        const int row0 = (int)blockIdx.x % groups * a.kv_rows, e0 = (int)blockIdx.x / groups * kK8Entries;
+        const int heads = min(a.kv_rows, 2 * a.n_kv - row0);
         // lane l looks at entry e0 + l: a run starts at one of the first 16 and
         // ends among all 32
         const int e = e0 + lane;
@@ -200,26 +209,40 @@ kv8_append_kernel(const __grid_constant__ PagesDev p, const __grid_constant__ Ap
             bpos = e0 > 0 ? a.pos[e0 - 1] : 0;
         }
         const bool same = slot >= 0 && slot == before && (pos >> 4) == (bpos >> 4);
-        const bool follows = same && pos > bpos;
         const unsigned starts = __ballot_sync(0xffffffffu, in && slot >= 0 && !same && lane < kK8Entries);
-        const unsigned goes_on = __ballot_sync(0xffffffffu, follows), again = __ballot_sync(0xffffffffu, same);
-        int j = 0;
-        for (unsigned m = starts; m != 0; m &= m - 1, ++j) {
-            if (j % kK8Warps != warp) continue;
-            const int l = __ffs(m) - 1;
-            const unsigned rest = goes_on >> 1 >> l;            // bit i: entry l + 1 + i follows its predecessor
-            int count = 1 + __ffs(~rest) - 1;                   // (at most 16: positions ascend in a block)
-            const int s = __shfl_sync(0xffffffffu, slot, l), p0 = __shfl_sync(0xffffffffu, pos, l);
-            bool wrong = l + count < 32 && (again >> (l + count) & 1) != 0;      // not after its predecessor
-            // the tokens behind the slot's end or the table's are left out
-            const int len = s < p.n_slots ? p.lens[s] : 0, limit = min(min(len, p.cap), a.n_ctx);
-            const int mine = __shfl_sync(0xffffffffu, pos, (l + lane) & 31);
-            const unsigned fine = __ballot_sync(0xffffffffu, lane < count && mine >= 0 && mine < limit);
-            const int live = __popc(fine);
-            wrong = wrong || live < count;
+        const unsigned goes_on = __ballot_sync(0xffffffffu, same && pos > bpos), again = __ballot_sync(0xffffffffu, same);
+        const int pairs = __popc(starts) * heads;
+        // pair w of this CTA: run w / heads, head w % heads
+        auto run_of = [&](int w, int* l, int* count) {
+            *l = (int)__fns(starts, 0, w / heads + 1);
+            const unsigned rest = goes_on >> 1 >> *l;           // bit i: entry l + 1 + i follows its predecessor
+            *count = __ffs(~rest);                              // (at most 16: positions ascend in a block)
+        };
+        if (warp >= pairs) return;
+        int l, count;
+        run_of(warp, &l, &count);
+        Run run;
+        run.load(a, e0 + l, count, (row0 + warp % heads) % a.n_kv, row0 + warp % heads >= a.n_kv);
+        // Each entry's page, -1: none, or a shared one, which is never written (its other
+        // owners would change). Tokens behind the slot's end or the angles' are left out.
+        const bool fine = slot >= 0 && slot < p.n_slots && pos >= 0 && pos < a.n_ctx && pos < p.cap && pos < p.lens[slot];
+        int id = fine ? p.tables[(size_t)slot * p.width + pos / p.page] : -1;
+        if (id < 0 || id >= p.n_pages || p.refs[id] != 1) id = -1;
+        const unsigned good = __ballot_sync(0xffffffffu, fine && id >= 0);
+        for (int w = warp; w < pairs; w += kK8Warps) {
+            if (w != warp) run_of(w, &l, &count);
+            const int row = row0 + w % heads;
+            const unsigned mine = (count < 32 ? (1u << count) - 1u : 0xffffffffu) << l;
+            // those that count end where the positions pass a limit; what comes after
+            // its place in the list is wrong, too
+            const int live = __popc(good & mine);
+            const bool wrong = live < count || (l + count < 32 && (again >> (l + count) & 1) != 0);
             if (wrong && lane == 0) raise(a.status, SLLM_CUDA_ERR_ARG);
-            if (live > 0)
-                append_run<O>(p, a, e0 + l, live, s, p0, row < a.n_kv ? row : row - a.n_kv, row >= a.n_kv);
+            const int page = __shfl_sync(0xffffffffu, id, l), p0 = __shfl_sync(0xffffffffu, pos, l);
+            if (live == 0) continue;
+            const bool is_v = row >= a.n_kv;
+            if (w != warp) run.load(a, e0 + l, live, row - (is_v ? a.n_kv : 0), is_v);
+            append_run<O>(p, a, run, e0 + l, live, page, p0, row - (is_v ? a.n_kv : 0), is_v);
         }
         return;
     }
@@ -381,7 +404,10 @@ extern "C" int sllm_cuda_kv8_append(const sllm_cuda_kv_pages* p, int32_t layer, 
     a.scale_stride = p->n_layer * layer_scales;
     a.n_tokens = n_tokens; a.n_head = n_head; a.n_kv = p->n_head_kv; a.n_ctx = n_ctx;
     a.status = status;
-    const long long kv = (long long)((n_tokens + kK8Entries - 1) / kK8Entries) * 2 * p->n_head_kv;
+    // one head of k or v a CTA while that makes no more than four CTAs an SM, else eight
+    const long long chunks = (n_tokens + kK8Entries - 1) / kK8Entries;
+    a.kv_rows = chunks * 2 * p->n_head_kv <= 4LL * current_sms() ? 1 : 8;
+    const long long kv = chunks * ((2 * p->n_head_kv + a.kv_rows - 1) / a.kv_rows);
     const long long units = q != nullptr ? (long long)n_tokens * ((n_head + 7) / 8) : 0;
     const long long ctas = kv + (units + kK8Warps - 1) / kK8Warps;
     if (ctas > 0x7fffffffLL) return fail(SLLM_CUDA_ERR_TOO_LARGE, "kv8_append: %d tokens", n_tokens);
