@@ -279,11 +279,11 @@ kv8_append_kernel(const __grid_constant__ PagesDev p, const __grid_constant__ Ap
 }
 
 // ---------------------------------------------------------------------------
-// read. A warp takes eight rows (k heads, then v heads) of a token; a lane's
-// values leave in 16 bytes, so 16 lanes share an f16 row and 32 an f32 one.
+// read. A warp takes one head of k or of v of up to 32 tokens of the list; the
+// tokens' pages are looked up first, a lane each. A lane's values leave in 16
+// bytes, so 16 lanes share an f16 row and 32 an f32 one; eight such loads are in
+// flight.
 // ---------------------------------------------------------------------------
-constexpr int kRdRows = 8;
-
 struct Read8Params {
     const int32_t* slot;
     const int32_t* pos;
@@ -295,6 +295,7 @@ struct Read8Params {
     void* ko;
     void* vo;
     int n_tokens, n_kv;
+    int per, first, rows;           // tokens of a warp; the first row (k heads, then v heads) and their number
     int32_t* status;
 };
 
@@ -305,54 +306,62 @@ __device__ __forceinline__ float value_of(uint32_t u, int i, float s) {
 template <class O>
 __global__ void __launch_bounds__(32 * kK8Warps)
 kv8_read_kernel(const __grid_constant__ PagesDev p, const __grid_constant__ Read8Params a) {
-    constexpr int PER = 16 / (int)sizeof(O), ROWS = PER / 4;           // elements of a lane; rows at once
+    constexpr int PER = 16 / (int)sizeof(O), ROWS = PER / 4, FLY = 8;  // elements of a lane; tokens at once; loads in flight
     const int lane = threadIdx.x & 31;
-    const int first = a.ko != nullptr ? 0 : a.n_kv, rows = (a.vo != nullptr ? 2 * a.n_kv : a.n_kv) - first;
-    const int units = (rows + kRdRows - 1) / kRdRows;
     const long long u = (long long)blockIdx.x * kK8Warps + (threadIdx.x >> 5);
-    const int tok = (int)(u / units);
-    if (tok >= a.n_tokens) return;
-    const int slot = a.slot[tok], pos = a.pos[tok];
-    if (slot < 0) return;
-    const int id = page_at(p, slot, pos);
-    if (id < 0) {
-        if (lane == 0) raise(a.status, SLLM_CUDA_ERR_ARG);
-        return;
-    }
-    const int r0 = (int)(u - (long long)tok * units) * kRdRows + lane / (32 / ROWS), col = lane % (32 / ROWS) * PER;
-    const int in = pos % p.page;
-    uint2 c[kRdRows / ROWS];
-    float s[kRdRows / ROWS];
-    #pragma unroll
-    for (int i = 0; i < kRdRows / ROWS; ++i) {
-        const int r = r0 + i * ROWS;
-        if (r < rows) {
-            const bool is_v = r + first >= a.n_kv;
-            const int h = r + first - (is_v ? a.n_kv : 0);
-            const int8_t* x = (is_v ? a.vp : a.kp) + (size_t)id * a.page_stride + ((size_t)h * p.page + in) * kServeDim + col;
-            if (PER == 8) c[i] = __ldg(reinterpret_cast<const uint2*>(x));
-            else c[i].x = __ldg(reinterpret_cast<const uint32_t*>(x));
-            s[i] = __ldg((is_v ? a.vsc : a.ksc) + (size_t)id * a.scale_stride + (size_t)h * (p.page / kKvBlock) + in / kKvBlock);
+    const long long c = u / a.rows;
+    const int row = a.first + (int)(u - c * a.rows), h = row < a.n_kv ? row : row - a.n_kv;
+    if (c * a.per >= a.n_tokens) return;
+    const int e0 = (int)c * a.per, n = min(a.per, a.n_tokens - e0);
+    // this lane's token: where its row of head 0 and the scale of that are, -1: nowhere
+    int id = -1, in = 0;
+    bool wrong = false;
+    if (lane < n) {
+        const int slot = a.slot[e0 + lane], pos = a.pos[e0 + lane];
+        if (slot >= 0) {
+            id = page_at(p, slot, pos);
+            wrong = id < 0;
+            in = pos & (p.page - 1);
         }
     }
-    #pragma unroll
-    for (int i = 0; i < kRdRows / ROWS; ++i) {
-        const int r = r0 + i * ROWS;
-        if (r >= rows) continue;
-        const bool is_v = r + first >= a.n_kv;
-        const int h = r + first - (is_v ? a.n_kv : 0);
-        O* const out = static_cast<O*>(is_v ? a.vo : a.ko) + ((size_t)tok * a.n_kv + h) * kServeDim + col;
-        if constexpr (PER == 8) {
-            __half2 x[4];
-            #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const uint32_t w = e < 2 ? c[i].x : c[i].y;
-                x[e] = __floats2half2_rn(value_of(w, 2 * (e & 1), s[i]), value_of(w, 2 * (e & 1) + 1, s[i]));
+    if (__any_sync(0xffffffffu, wrong) && lane == 0) raise(a.status, SLLM_CUDA_ERR_ARG);
+    const bool is_v = row >= a.n_kv;
+    const int sub = lane / (32 / ROWS), col = lane % (32 / ROWS) * PER;
+    const int8_t* const codes = (is_v ? a.vp : a.kp) + (size_t)h * p.page * kServeDim + col;
+    const float* const scales = (is_v ? a.vsc : a.ksc) + (size_t)h * (p.page / kKvBlock);
+    O* const out = static_cast<O*>(is_v ? a.vo : a.ko) + ((size_t)e0 * a.n_kv + h) * kServeDim + col;
+    for (int i0 = 0; i0 < n; i0 += ROWS * FLY) {
+        uint2 x[FLY];
+        float s[FLY];
+        bool live[FLY];
+        #pragma unroll
+        for (int i = 0; i < FLY; ++i) {
+            const int t = i0 + i * ROWS + sub;
+            const int page = __shfl_sync(0xffffffffu, id, t & 31), at = __shfl_sync(0xffffffffu, in, t & 31);
+            live[i] = t < n && page >= 0;
+            if (live[i]) {
+                const int8_t* from = codes + (size_t)page * a.page_stride + at * kServeDim;
+                if (PER == 8) x[i] = __ldg(reinterpret_cast<const uint2*>(from));
+                else x[i].x = __ldg(reinterpret_cast<const uint32_t*>(from));
+                s[i] = __ldg(scales + (size_t)page * a.scale_stride + at / kKvBlock);
             }
-            __stcs(reinterpret_cast<uint4*>(out), *reinterpret_cast<const uint4*>(x));
-        } else {
-            __stcs(reinterpret_cast<float4*>(out), make_float4(value_of(c[i].x, 0, s[i]), value_of(c[i].x, 1, s[i]),
-                                                               value_of(c[i].x, 2, s[i]), value_of(c[i].x, 3, s[i])));
+        }
+        #pragma unroll
+        for (int i = 0; i < FLY; ++i) {
+            if (!live[i]) continue;
+            O* const to = out + (size_t)(i0 + i * ROWS + sub) * a.n_kv * kServeDim;
+            if constexpr (PER == 8) {
+                __half2 y[4];
+                #pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t w = e < 2 ? x[i].x : x[i].y;
+                    y[e] = __floats2half2_rn(value_of(w, 2 * (e & 1), s[i]), value_of(w, 2 * (e & 1) + 1, s[i]));
+                }
+                __stcs(reinterpret_cast<uint4*>(to), *reinterpret_cast<const uint4*>(y));
+            } else {
+                __stcs(reinterpret_cast<float4*>(to), make_float4(value_of(x[i].x, 0, s[i]), value_of(x[i].x, 1, s[i]),
+                                                                  value_of(x[i].x, 2, s[i]), value_of(x[i].x, 3, s[i])));
+            }
         }
     }
 }
@@ -449,8 +458,11 @@ extern "C" int sllm_cuda_kv8_read(const sllm_cuda_kv_pages* p, int32_t layer, in
     a.ko = k_out; a.vo = v_out;
     a.n_tokens = n_tokens; a.n_kv = p->n_head_kv;
     a.status = status;
-    const int rows = ((k_out != nullptr) + (v_out != nullptr)) * p->n_head_kv;
-    const long long units = (long long)n_tokens * ((rows + kRdRows - 1) / kRdRows);
+    a.first = k_out != nullptr ? 0 : p->n_head_kv;
+    a.rows = ((k_out != nullptr) + (v_out != nullptr)) * p->n_head_kv;
+    // 32 tokens a warp where that still makes 16 warps an SM, else eight
+    a.per = (long long)n_tokens * a.rows / 32 >= 16LL * current_sms() ? 32 : 8;
+    const long long units = ((long long)n_tokens + a.per - 1) / a.per * a.rows;
     const long long ctas = (units + kK8Warps - 1) / kK8Warps;
     if (ctas > 0x7fffffffLL) return fail(SLLM_CUDA_ERR_TOO_LARGE, "kv8_read: %d tokens", n_tokens);
     if (out_type == SLLM_CUDA_KV_F16)
