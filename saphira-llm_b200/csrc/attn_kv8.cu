@@ -36,10 +36,11 @@ constexpr int kE8Threads = 32 * (kE8Warps + 1);
 constexpr int kE8Keys = 128;                        // keys of a tile
 constexpr int kE8Blocks = kE8Keys / kKvBlock;
 constexpr int kE8Tile = kE8Keys * kServeDim;        // bytes of one of K or V
-// Weights stand against 2^-lift of a reference. Pairs of f16: the running maximum,
-// so weights are up to 2^15. One f16: the maximum when it last grew by more than
-// 2^8, so that the outputs are seldom rescaled; weights are up to 2^15, too, and
-// keep 11 bits down to 2^-21 of the largest.
+// Weights stand against 2^-lift of a reference and are 2^15 at most. Pairs of f16: the
+// reference is the running maximum. One f16: the maximum when it last grew by more
+// than 2^8, so that the outputs are seldom rescaled; weights keep 11 bits down to
+// 2^-21 of the largest. A row that has seen nothing has the reference kE8None.
+constexpr float kE8None = -1e30f;
 constexpr float kE8Grow = 8.f;
 __host__ __device__ constexpr float e8_lift(int planes) { return planes == 1 ? 15.f - kE8Grow : 15.f; }
 constexpr float kE8Log2 = kServeScale * 1.4426950408889634f;
@@ -173,7 +174,7 @@ struct Rows8 {
                 for (int c = 0; c < 4; ++c) o[n][j][c] = 0.f;
             #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                m[n][c] = -INFINITY;
+                m[n][c] = kE8None;
                 l[n][c] = 0.f;
                 mul[n][c] = 1.f;
             }
@@ -276,45 +277,56 @@ struct Rows8 {
                 }
             }
         }
+        // Exponents against the rows' references, no shuffles: one that is too large is
+        // seen by its own lane, and then only the row's maximum is looked for. (With it
+        // each time, a tile of eight rows took 206 instructions for the 32 keys, not 141.)
         const float base[2] = {ks[0] * kE8Log2, ks[1] * kE8Log2};
-        uint32_t pb[2][P][NT][2];
-        constexpr float LIFT = e8_lift(P), GROW = P == 1 ? kE8Grow : 0.f;
-        float y[NT][2][4], most[NT][2];
-        bool grown = false;
+        constexpr float LIFT = e8_lift(P), MOST = 15.f;
+        float z[NT][2][4], top = -INFINITY;
         #pragma unroll
         for (int n = 0; n < NT; ++n) {
+            const float ref[2] = {LIFT - m[n][0], LIFT - m[n][1]};
             #pragma unroll
             for (int k = 0; k < 2; ++k)
                 #pragma unroll
-                for (int c = 0; c < 4; ++c)
-                    y[n][k][c] = P == 1 ? s[k][0][n][c] * base[k]
-                                        : __fmaf_rn(s[k][P - 1][n][c], 0x1p-11f, s[k][0][n][c]) * (base[k] * mul[n][c & 1]);
+                for (int c = 0; c < 4; ++c) {
+                    if constexpr (P == 2) s[k][0][n][c] = __fmaf_rn(s[k][P - 1][n][c], 0x1p-11f, s[k][0][n][c]);
+                    z[n][k][c] = __fmaf_rn(s[k][0][n][c], P == 1 ? base[k] : base[k] * mul[n][c & 1], ref[c & 1]);
+                }
             if (masked) {
                 #pragma unroll
                 for (int k = 0; k < 2; ++k)
                     #pragma unroll
                     for (int c = 0; c < 4; ++c)
-                        if (j0 + k * dj + g + 8 * (c >> 1) >= lim[n][c & 1]) y[n][k][c] = -INFINITY;
+                        if (j0 + k * dj + g + 8 * (c >> 1) >= lim[n][c & 1]) z[n][k][c] = -INFINITY;
             }
             #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                float now = fmaxf(fmaxf(y[n][0][c], y[n][0][c + 2]), fmaxf(y[n][1][c], y[n][1][c + 2]));
-                #pragma unroll
-                for (int z = 4; z < 32; z <<= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, z));
-                most[n][c] = now;
-                grown = grown || now > m[n][c] + GROW;
-            }
+            for (int k = 0; k < 2; ++k) top = fmaxf(fmaxf(fmaxf(top, z[n][k][0]), fmaxf(z[n][k][1], z[n][k][2])), z[n][k][3]);
         }
-        if (__any_sync(0xffffffffu, grown)) {
+        if (__any_sync(0xffffffffu, top > MOST)) {
             #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 float alpha[2];
                 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                    const float now = fmaxf(m[n][c], most[n][c]);
-                    alpha[c] = now == -INFINITY ? 1.f : ex2(m[n][c] - now);
+                    float now = kE8None;
+                    #pragma unroll
+                    for (int k = 0; k < 2; ++k)
+                        #pragma unroll
+                        for (int i = c; i < 4; i += 2)
+                            if (z[n][k][i] > -INFINITY) now = fmaxf(now, s[k][0][n][i] * (P == 1 ? base[k] : base[k] * mul[n][c]));
+                    #pragma unroll
+                    for (int y = 4; y < 32; y <<= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, y));
+                    now = fmaxf(m[n][c], now);
+                    alpha[c] = ex2(m[n][c] - now);
                     m[n][c] = now;
                     l[n][c] *= alpha[c];
+                    #pragma unroll
+                    for (int k = 0; k < 2; ++k)
+                        #pragma unroll
+                        for (int i = c; i < 4; i += 2)
+                            if (z[n][k][i] != -INFINITY)
+                                z[n][k][i] = __fmaf_rn(s[k][0][n][i], P == 1 ? base[k] : base[k] * mul[n][c], LIFT - now);
                 }
                 #pragma unroll
                 for (int j = 0; j < 8; ++j)
@@ -322,24 +334,25 @@ struct Rows8 {
                     for (int c = 0; c < 4; ++c) o[n][j][c] *= alpha[c & 1];
             }
         }
+        uint32_t pb[2][P][NT][2];
         #pragma unroll
         for (int n = 0; n < NT; ++n) {
             #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 #pragma unroll
-                for (int c = 0; c < 4; ++c) y[n][k][c] = ex2(y[n][k][c] - ((m[n][c & 1] == -INFINITY ? 0.f : m[n][c & 1]) - LIFT));
+                for (int c = 0; c < 4; ++c) z[n][k][c] = ex2(z[n][k][c]);
                 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                    const uint32_t hi = pack2(y[n][k][2 * c], y[n][k][2 * c + 1]);
+                    const uint32_t hi = pack2(z[n][k][2 * c], z[n][k][2 * c + 1]);
                     pb[k][0][n][c] = transpose8(hi);
                     if constexpr (P == 2) {
-                        const float2 z = unpack2(hi);
-                        pb[k][P - 1][n][c] = transpose8(pack2((y[n][k][2 * c] - z.x) * 2048.f, (y[n][k][2 * c + 1] - z.y) * 2048.f));
+                        const float2 y = unpack2(hi);
+                        pb[k][P - 1][n][c] = transpose8(pack2((z[n][k][2 * c] - y.x) * 2048.f, (z[n][k][2 * c + 1] - y.y) * 2048.f));
                     }
                 }
             }
             #pragma unroll
-            for (int c = 0; c < 2; ++c) l[n][c] += (y[n][0][c] + y[n][0][c + 2]) + (y[n][1][c] + y[n][1][c + 2]);
+            for (int c = 0; c < 2; ++c) l[n][c] += (z[n][0][c] + z[n][0][c + 2]) + (z[n][1][c] + z[n][1][c + 2]);
         }
         #pragma unroll
         for (int k = 0; k < 2; ++k) {
@@ -413,7 +426,7 @@ __device__ __forceinline__ void finish(const Attn8Params& p, const Meta& mt, con
                                        int ml_step, int kg, int r0, int part) {
     constexpr int SHARE = 8 * NT / KG;
     const int lane = threadIdx.x & 31, r = kg * SHARE + (lane < SHARE ? lane : 0), row = mt.row_block * p.block_rows + r0 + r;
-    float w[KG], M = -INFINITY, l = 0.f;
+    float w[KG], M = kE8None, l = 0.f;
     float2 x[KG];
     #pragma unroll
     for (int k = 0; k < KG; ++k) {
@@ -422,7 +435,7 @@ __device__ __forceinline__ void finish(const Attn8Params& p, const Meta& mt, con
     }
     #pragma unroll
     for (int k = 0; k < KG; ++k) {
-        w[k] = ex2(x[k].x - (M == -INFINITY ? 0.f : M));
+        w[k] = ex2(x[k].x - M);
         l = __fmaf_rn(w[k], x[k].y, l);
     }
     const int live = min(max(p.rows - (mt.row_block * p.block_rows + r0 + kg * SHARE), 0), SHARE);
@@ -431,7 +444,7 @@ __device__ __forceinline__ void finish(const Attn8Params& p, const Meta& mt, con
         at = ((size_t)part * p.block_rows + r0 + r) * kServeDim;
         if (lane < live) p.part_ml[(size_t)part * p.block_rows + r0 + r] = make_float2(M, l);
     } else {
-        const float inv = M == -INFINITY && l == 0.f ? 0.f : __fdiv_rn(1.f, l);
+        const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);     // (0: the row has seen nothing)
         #pragma unroll
         for (int k = 0; k < KG; ++k) w[k] *= inv;
         at = p.row_at(mt.b, mt.head, row);
@@ -778,7 +791,7 @@ attn_kv8_join_kernel(const __grid_constant__ Attn8Params p, int per_row) {
     // parts: the second of the first CTA's, then the first of the following CTAs'
     const int parts = note.w - c + 1;
     auto at = [&](int i) { return (size_t)(i == 0 ? 2 * c + 1 : 2 * (c + i)) * p.block_rows + in; };
-    float M = -INFINITY, l = 0.f;
+    float M = kE8None, l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     if (live) {
         for (int i0 = sub; i0 < parts; i0 += 8 * per_row) {
@@ -787,7 +800,7 @@ attn_kv8_join_kernel(const __grid_constant__ Attn8Params p, int per_row) {
             #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const int i = i0 + e * per_row;
-                ml[e] = make_float2(-INFINITY, 0.f);
+                ml[e] = make_float2(kE8None, 0.f);
                 if (i < parts) {
                     ml[e] = __ldcg(p.part_ml + at(i));
                     v[e] = __ldcg(reinterpret_cast<const float4*>(p.part_o + at(i) * kServeDim) + lane);
@@ -796,14 +809,14 @@ attn_kv8_join_kernel(const __grid_constant__ Attn8Params p, int per_row) {
             float now = M;
             #pragma unroll
             for (int e = 0; e < 8; ++e) now = fmaxf(now, ml[e].x);
-            const float ref = now == -INFINITY ? 0.f : now, f0 = ex2(M - ref);
+            const float f0 = ex2(M - now);
             M = now;
             l *= f0;
             o.x *= f0; o.y *= f0; o.z *= f0; o.w *= f0;
             #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 if (i0 + e * per_row >= parts) continue;
-                const float f = ex2(ml[e].x - ref);
+                const float f = ex2(ml[e].x - M);
                 l = __fmaf_rn(f, ml[e].y, l);
                 o.x = __fmaf_rn(f, v[e].x, o.x);
                 o.y = __fmaf_rn(f, v[e].y, o.y);
@@ -820,7 +833,7 @@ attn_kv8_join_kernel(const __grid_constant__ Attn8Params p, int per_row) {
         for (int i = 1; i < per_row; ++i) {
             const float2 b = sm[warp + i];
             const float4 v = so[warp + i][lane];
-            const float now = fmaxf(M, b.x), ref = now == -INFINITY ? 0.f : now, f0 = ex2(M - ref), f1 = ex2(b.x - ref);
+            const float now = fmaxf(M, b.x), f0 = ex2(M - now), f1 = ex2(b.x - now);
             M = now;
             l = __fmaf_rn(l, f0, b.y * f1);
             o.x = __fmaf_rn(o.x, f0, v.x * f1);
@@ -830,7 +843,7 @@ attn_kv8_join_kernel(const __grid_constant__ Attn8Params p, int per_row) {
         }
     }
     if (!live) return;
-    const float inv = M == -INFINITY && l == 0.f ? 0.f : __fdiv_rn(1.f, l);
+    const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);
     st4(static_cast<O*>(p.out) + p.row_at(note.x, h, r) + 4 * lane, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
 }
 
