@@ -16,6 +16,8 @@
 // f32 queries and weights are pairs of f16, x = hi + 2^-11 lo, with a power of
 // two per query row; two products then, 22 bits.
 //
+// 17 rows and more of f16 queries go to attn_kv8_wide.cuh.
+//
 // The work is cut by the device: the tiles of 128 keys of all (sequence, kv
 // head) pairs, in order, are dealt to the CTAs in equal runs. A pair inside one
 // run is written at once; of a pair that runs share each leaves its part
@@ -25,73 +27,20 @@
 
 #include <type_traits>
 
-#include "attn_mma.cuh"
-#include "serve.cuh"
+#include "attn_kv8.cuh"
+#include "attn_kv8_wide.cuh"
 
 namespace sllm {
 namespace {
 
 constexpr int kE8Warps = 4;                         // that multiply; one more loads
 constexpr int kE8Threads = 32 * (kE8Warps + 1);
-constexpr int kE8Keys = 128;                        // keys of a tile
-constexpr int kE8Blocks = kE8Keys / kKvBlock;
-constexpr int kE8Tile = kE8Keys * kServeDim;        // bytes of one of K or V
-// Weights stand against 2^-lift of a reference and are 2^15 at most. Pairs of f16: the
-// reference is the running maximum. One f16: the maximum when it last grew by more
-// than 2^8, so that the outputs are seldom rescaled; weights keep 11 bits down to
-// 2^-21 of the largest. A row that has seen nothing has the reference kE8None.
-constexpr float kE8None = -1e30f;
-constexpr float kE8Grow = 8.f;
-__host__ __device__ constexpr float e8_lift(int planes) { return planes == 1 ? 15.f - kE8Grow : 15.f; }
-constexpr float kE8Log2 = kServeScale * 1.4426950408889634f;
-
 __host__ __device__ constexpr int e8_ctas(int nt) { return nt == 1 ? 3 : 2; }      // per SM
-
-struct Attn8Params {
-    const void* q;                  // [n][n_q][n_head][128]
-    void* out;
-    const float* ksc;               // the layer's slice of page 0
-    const float* vsc;
-    size_t scale_stride;
-    const int32_t* slots;
-    int n, n_q, n_head, n_kv, group, rows;          // rows: n_q * group
-    int rg, row_blocks, block_rows;                 // row groups of a CTA; row blocks of a pair, and rows of one
-    int q_bufs;                     // buffers of a row block's queries
-    int page_log2;                  // rows of a page, and of a load
-    WaitLimit wait;
-    int32_t* status;
-    float* part_o;                  // [2 * CTAs][block_rows][128]
-    float2* part_ml;                // [2 * CTAs][block_rows]
-    // notes for the join: sequence (-1: nothing to join), pair, first and last CTA. Of each
-    // pair where there are no more pairs than CTAs (by_pair), else of the pair that starts
-    // in a CTA's run and ends in another's
-    int4* notes;
-    int by_pair, n_notes;
-    uint32_t over_group;            // ceil(2^32 / group), 0 for 1: exact below 2^22 (rows are under 2^14, groups up to 2^10)
-
-    __device__ __forceinline__ int token(int row) const { return over_group == 0 ? row : (int)__umulhi((uint32_t)row, over_group); }
-    // row `row` of a sequence's kv head, in q and out
-    __device__ __forceinline__ size_t row_at(int b, int head, int row) const {
-        const int j = token(row);
-        return (((size_t)b * n_q + j) * n_head + (size_t)head * group + (row - j * group)) * kServeDim;
-    }
-};
-
-struct Meta {                       // of a tile in a stage
-    int b, head, row_block, len, key0, flags;
-};
-enum { E8_FIRST = 1, E8_LAST = 2, E8_PART0 = 4, E8_PART1 = 8, E8_END = 16 };
 
 struct __align__(1024) Stage8 {
     uint8_t k[kE8Tile], v[kE8Tile];
 };
 constexpr int kE8Stages = 2;
-
-// The loading warp's place in its run, tile by tile; pair: head * row blocks + row
-// block of a sequence
-struct Place {
-    int b, slot, len, tiles, pair, head, row_block, tile;
-};
 
 struct __align__(1024) Shared8 {    // and the queries' buffers behind it
     Stage8 stage[kE8Stages];
@@ -99,23 +48,10 @@ struct __align__(1024) Shared8 {    // and the queries' buffers behind it
     Meta meta[kE8Stages];
     uint64_t full[kE8Stages], empty[kE8Stages];
     uint64_t q_free[2], done, merged;
-    unsigned long long scan[kE8Threads / 32];
-    unsigned long long start_rest;
-    Place start;
+    RunStart run;
     int abort;
     float2 ml[kE8Warps][16];
 };
-
-struct Waits {                      // for the bounded waits
-    const Attn8Params& p;
-    __device__ __forceinline__ WaitLimit wait_limit() const { return p.wait; }
-};
-
-__device__ __forceinline__ float ex2(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -135,23 +71,6 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
     return r;
 }
-
-// two codes, of bytes 0 and 1 or 2 and 3 of u (with 128 added to each), as f16:
-// 0x6400 + byte is 1024 + byte; `raw`: with the 1152 that this is too much
-constexpr float kE8Raw = 1152.f;
-template <bool RAW>
-__device__ __forceinline__ uint32_t two_codes(uint32_t u, bool upper) {
-    const uint32_t x = __byte_perm(u, 0x64646464u, upper ? 0x4342 : 0x4140);
-    if (RAW) return x;
-    const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&x), __half2half2(__ushort_as_half(0x6480)));
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-
-__device__ __forceinline__ uint32_t pack2(float x, float y) {
-    const __half2 h = __floats2half2_rn(x, y);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-__device__ __forceinline__ float2 unpack2(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
 
 __device__ __forceinline__ uint4 lds16(const uint8_t* p) { return *reinterpret_cast<const uint4*>(p); }
 
@@ -469,29 +388,6 @@ __device__ __forceinline__ void finish(const Attn8Params& p, const Meta& mt, con
     }
 }
 
-// the tiles of a sequence (one at least: without keys it has zeros to write); 0
-// where its slot or length is wrong
-__device__ __forceinline__ int seq_tiles(const PagesDev& pg, const Attn8Params& p, int b, int* slot, int* len) {
-    const int s = p.slots[b];
-    *slot = s;
-    *len = 0;
-    if (s < 0 || s >= pg.n_slots) return 0;
-    const int n = pg.lens[s];
-    if (n < 0 || n > pg.cap) return 0;
-    *len = n;
-    return max(1, (n + kE8Keys - 1) / kE8Keys);
-}
-
-__device__ __forceinline__ void cp_async4(void* dst, const void* src) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async16(void* dst, const void* src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
-    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-
 template <class Q, class O, int NT>
 __global__ void __launch_bounds__(kE8Threads, e8_ctas(NT))
 attn_kv8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
@@ -521,7 +417,7 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
         mbar_init(&sh.done, kE8Warps);
         mbar_init(&sh.merged, kE8Warps);
         sh.abort = 0;
-        sh.start.tiles = 0;
+        sh.run.at.tiles = 0;
         fence_proxy_async_smem();
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -529,70 +425,13 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tm_k)) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tm_v)) : "memory");
     }
-    // This CTA's run: a prefix sum over the sequences, each thread some of them. A pair
-    // counts a tile more than it has, at its end: what its start and end cost.
-    const int pairs = p.n_kv * p.row_blocks, per = (p.n + kE8Threads - 1) / kE8Threads;
-    const int b0 = min(t * per, p.n), b1 = min(b0 + per, p.n);
-    unsigned long long mine = 0;
-    for (int b = b0; b < b1; ++b) {
-        int slot, len;
-        const int tiles = seq_tiles(pg, p, b, &slot, &len);
-        if (tiles == 0 && blockIdx.x == 0) {
-            raise(p.status, SLLM_CUDA_ERR_ARG);
-            if (p.by_pair)
-                for (int i = 0; i < pairs; ++i) p.notes[b * pairs + i] = make_int4(-1, 0, 0, 0);
-        }
-        if (tiles > 0) mine += (unsigned long long)(tiles + 1) * pairs;
-    }
-    unsigned long long upto = mine;
-    #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const unsigned long long y = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += y;
-    }
-    if (lane == 31) sh.scan[warp] = upto;
-    __syncthreads();
-    unsigned long long all = 0;
-    #pragma unroll
-    for (int w = 0; w < kE8Threads / 32; ++w) {
-        if (w < warp) upto += sh.scan[w];
-        all += sh.scan[w];
-    }
-    const unsigned long long G = gridDim.x < all ? gridDim.x : all;     // runs
-    const unsigned long long c = blockIdx.x;
-    if (c >= G) {
-        if (t == 0 && !p.by_pair) p.notes[c] = make_int4(-1, 0, 0, 0);
-        return;
-    }
-    const unsigned long long u0 = c * all / G, u1 = (c + 1) * all / G;
-    if (u0 >= upto - mine && u0 < upto) {
-        unsigned long long rest = u0 - (upto - mine);
-        for (int b = b0; b < b1; ++b) {
-            Place x;
-            x.tiles = seq_tiles(pg, p, b, &x.slot, &x.len);
-            const unsigned long long units = x.tiles > 0 ? (unsigned long long)(x.tiles + 1) * pairs : 0;
-            if (rest < units) {
-                x.b = b;
-                sh.start = x;
-                sh.start_rest = rest;
-                break;
-            }
-            rest -= units;
-        }
-    }
-    __syncthreads();
+    Walk8<1> walk(pg, p);
+    if (!walk.find<kE8Threads>(sh.run)) return;
 
     const Waits w{p};
     bool ok = true;
     if (warp == kE8Warps) {
         // ---- loads
-        auto enter = [&](Place& x, int b) {         // the next sequence that has tiles; false: none
-            for (x.tiles = 0; b < p.n && x.tiles == 0; ++b) {
-                x.b = b;
-                x.tiles = seq_tiles(pg, p, b, &x.slot, &x.len);
-            }
-            return x.tiles > 0;
-        };
         // lane i: the page of the tile's i-th load
         auto ids = [&](const Place& x) {
             const int key = x.tile * kE8Keys + (lane << p.page_log2);
@@ -606,42 +445,16 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
             }
             return id;
         };
-        auto next_pair = [&](Place& x) {
-            x.tile = 0;
-            if (++x.row_block == p.row_blocks) {
-                x.row_block = 0;
-                ++x.head;
-            }
-            if (++x.pair < pairs) return true;
-            x.pair = x.head = 0;
-            return enter(x, x.b + 1);
-        };
-        // (lengths that somebody writes to meanwhile end the run early, inside the arrays)
-        Place cur = sh.start;
-        unsigned long long left = u1 - u0;
-        bool more = cur.tiles > 0;
-        if (more) {
-            cur.pair = (int)(sh.start_rest / (cur.tiles + 1));
-            cur.tile = (int)(sh.start_rest % (cur.tiles + 1));
-            cur.head = cur.pair / p.row_blocks;
-            cur.row_block = cur.pair % p.row_blocks;
-            if (cur.tile == cur.tiles) more = --left > 0 && next_pair(cur);
-        }
-        int id = more ? ids(cur) : 0;
-        int first = 1, started = more && cur.tile == 0;     // of the segment: its first tile here; whether the pair starts here
+        bool more = walk.start(sh.run);
+        int id = more ? ids(walk.cur) : 0;
+        int first = 1, started = more && walk.cur.tile == 0;    // of the segment: its first tile here; whether the pair starts here
         int4 note = make_int4(-1, 0, 0, 0);
         uint32_t n = 0, seg = 0;
         while (more) {
+            const Place cur = walk.cur;
             const bool ends = cur.tile + 1 == cur.tiles;
-            const unsigned step = ends ? 2 : 1;
-            Place nxt = cur;
-            int nid = 0;
-            more = left > step;
-            if (more) {
-                if (ends) more = next_pair(nxt);
-                else ++nxt.tile;
-                if (more) nid = ids(nxt);
-            }
+            more = walk.advance();
+            const int nid = more ? ids(walk.cur) : 0;
             const int slot = n % STAGES;
             if (n >= STAGES && !(ok = at_wait_warp(&sh.empty[slot], (n / STAGES - 1) & 1, ab, w))) break;
             const int qb = seg % p.q_bufs;
@@ -679,16 +492,12 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
             }
             cp_async_arrive(&sh.full[slot]);
             if (last && started) {
-                // other runs go on with this pair: up to its last tile's
-                const unsigned long long end = u1 - left + (unsigned long long)(cur.tiles - cur.tile);
-                const int4 x = make_int4(ends ? -1 : cur.b, cur.pair, (int)c, (int)min((end * G - 1) / all, G - 1));
+                const int4 x = walk.note(cur);
                 if (!ends) note = x;
-                if (p.by_pair && lane == 0) p.notes[cur.b * pairs + cur.pair] = x;
+                if (p.by_pair && lane == 0) p.notes[cur.b * walk.pairs + cur.pair] = x;
             }
             first = last;
             started = last ? 1 : started;
-            left -= step;
-            cur = nxt;
             id = nid;
             ++n;
         }
@@ -704,7 +513,7 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
                 ++n;
             }
         }
-        if (lane == 0 && !p.by_pair) p.notes[c] = note;
+        if (lane == 0 && !p.by_pair) p.notes[blockIdx.x] = note;
         // copies in flight end before the CTA does, also where the others gave up
         for (uint32_t i = n > STAGES ? n - STAGES : 0; i < n; ++i) at_drain(&sh.full[i % STAGES], (i / STAGES) & 1);
     } else {
@@ -756,7 +565,7 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.merged);
             if (!(ok = at_wait_warp(&sh.merged, par, ab, w))) break;
-            const int part = mt.flags & E8_PART0 ? 2 * (int)c : mt.flags & E8_PART1 ? 2 * (int)c + 1 : -1;
+            const int part = mt.flags & E8_PART0 ? 2 * (int)blockIdx.x : mt.flags & E8_PART1 ? 2 * (int)blockIdx.x + 1 : -1;
             const float4* const from = area + rgrp * (8 * NT * 32);
             const int step = RG * 8 * NT * 32, r0 = rgrp * 8 * NT;
             if (NT == 1 || KG == 4) finish<O, NT, 4>(p, mt, from, step, sh.ml + rgrp, RG, kg, r0, part);
@@ -853,10 +662,19 @@ attn_kv8_join_kernel(const __grid_constant__ Attn8Params p, int per_row) {
 // Rows of a CTA: 8 NT a warp, and row groups so that the four warps share them
 // and the keys; beyond 64 rows a pair is read once for every 64.
 struct Cut8 {
+    bool wide;
     int nt, rg, block_rows, row_blocks, ctas;
 };
-Cut8 cut8(int rows, int sms) {
+Cut8 cut8(int rows, bool f16, int sms) {
     Cut8 x;
+    x.wide = f16 && rows > 16;
+    if (x.wide) {
+        x.nt = x.rg = 0;
+        x.block_rows = kW8Rows;
+        x.row_blocks = (rows + kW8Rows - 1) / kW8Rows;
+        x.ctas = sms * kW8Ctas;
+        return x;
+    }
     x.nt = rows <= 8 ? 1 : 2;
     x.rg = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
     x.block_rows = 8 * x.nt * x.rg;
@@ -865,7 +683,7 @@ Cut8 cut8(int rows, int sms) {
     return x;
 }
 
-// (rises with the rows: 8 * 3, 16 * 2, 32 * 2, 64 * 2 a SM)
+// (f32 rises with the rows: 8 * 3, 16 * 2, 32 * 2, 64 * 2 a SM, and the wide form needs 32 * 2)
 size_t work8_bytes(const Cut8& x) {
     return (size_t)x.ctas * (2 * x.block_rows * (kServeDim * sizeof(float) + sizeof(float2)) + sizeof(int4));
 }
@@ -895,6 +713,13 @@ cudaError_t launch8(const CUtensorMap& tk, const CUtensorMap& tv, const PagesDev
     return e != cudaSuccess ? e : launch(attn_kv8_kernel<Q, O, NT>, dim3(ctas), dim3(kE8Threads), bytes, st, false, tk, tv, pg, a);
 }
 
+template <class O>
+cudaError_t launch_wide8(const CUtensorMap& tk, const CUtensorMap& tv, const PagesDev& pg, const Attn8Params& a, int ctas, cudaStream_t st) {
+    constexpr int kBytes = (int)sizeof(SharedW8);
+    const cudaError_t e = allow_smem<attn_kv8_wide_kernel<O>>(kBytes);
+    return e != cudaSuccess ? e : launch(attn_kv8_wide_kernel<O>, dim3(ctas), dim3(kW8Threads), kBytes, st, false, tk, tv, pg, a);
+}
+
 int check_shape8(const sllm_cuda_kv_pages* p, int n, int n_q, int n_head, const char* who) {
     const int rc = check_pages(p, who, true);
     if (rc != SLLM_CUDA_OK) return rc;
@@ -913,7 +738,7 @@ int sllm::take_kv8_error() { return take_attn_error(); }
 
 extern "C" size_t sllm_cuda_attn_kv8_work_bytes(const sllm_cuda_kv_pages* p, int32_t n, int32_t n_q, int32_t n_head) {
     if (check_shape8(p, n, n_q, n_head, "attn_kv8_work_bytes") != SLLM_CUDA_OK) return 0;
-    return work8_bytes(cut8(n_q * (n_head / p->n_head_kv), current_sms()));
+    return work8_bytes(cut8(n_q * (n_head / p->n_head_kv), false, current_sms()));
 }
 
 extern "C" int sllm_cuda_attn_kv8(const sllm_cuda_kv_pages* p, int32_t layer, const void* q, int32_t q_type,
@@ -927,8 +752,9 @@ extern "C" int sllm_cuda_attn_kv8(const sllm_cuda_kv_pages* p, int32_t layer, co
         (out_type != SLLM_CUDA_KV_F32 && out_type != SLLM_CUDA_KV_F16) ||
         (q_type == SLLM_CUDA_KV_F32 && out_type == SLLM_CUDA_KV_F16))
         return fail(SLLM_CUDA_ERR_ARG, "attn_kv8: query type %d, output type %d (f32, or f16 from f16)", q_type, out_type);
-    const Cut8 cut = cut8(n_q * (n_head / p->n_head_kv), current_sms());
-    const size_t need = work8_bytes(cut);
+    const int sms = current_sms(), rows = n_q * (n_head / p->n_head_kv);
+    const Cut8 cut = cut8(rows, q_type == SLLM_CUDA_KV_F16, sms);
+    const size_t need = work8_bytes(cut8(rows, false, sms));
     if (!aligned16(q) || !aligned16(out) || !aligned16(work) || work_bytes < need)
         return fail(SLLM_CUDA_ERR_ARG, "attn_kv8: workspace of %zu bytes (%zu needed), arrays 16-byte aligned", work_bytes, need);
     const void* ptr[] = {p->k, p->v, p->tables, p->lens, p->k_scale, p->v_scale, q, slots, out, work, status};
@@ -940,6 +766,9 @@ extern "C" int sllm_cuda_attn_kv8(const sllm_cuda_kv_pages* p, int32_t layer, co
     a.q = q; a.out = out;
     const size_t layer_codes = (size_t)p->n_head_kv * kServeDim * p->page_size;
     const size_t layer_scales = (size_t)p->n_head_kv * (p->page_size / kKvBlock);
+    a.kp = static_cast<const int8_t*>(p->k) + layer * layer_codes;
+    a.vp = static_cast<const int8_t*>(p->v) + layer * layer_codes;
+    a.page_codes = p->n_layer * layer_codes;
     a.ksc = p->k_scale + layer * layer_scales;
     a.vsc = p->v_scale + layer * layer_scales;
     a.scale_stride = p->n_layer * layer_scales;
@@ -960,13 +789,14 @@ extern "C" int sllm_cuda_attn_kv8(const sllm_cuda_kv_pages* p, int32_t layer, co
     a.n_notes = a.by_pair ? (int)pairs : cut.ctas;
     const PagesDev pg = pages_dev(*p);
     const cudaStream_t st = (cudaStream_t)stream;
-    CUtensorMap tk, tv;
-    if (!encode_codes(&tk, static_cast<const int8_t*>(p->k) + layer * layer_codes, *p) ||
-        !encode_codes(&tv, static_cast<const int8_t*>(p->v) + layer * layer_codes, *p))
-        return fail(SLLM_CUDA_ERR_DEVICE, "attn_kv8: a tensor map could not be made");
     const bool f32 = q_type == SLLM_CUDA_KV_F32, out32 = out_type == SLLM_CUDA_KV_F32;
     cudaError_t e;
-    if (cut.nt == 1)
+    CUtensorMap tk, tv;
+    if (!encode_codes(&tk, a.kp, *p) || !encode_codes(&tv, a.vp, *p))
+        return fail(SLLM_CUDA_ERR_DEVICE, "attn_kv8: a tensor map could not be made");
+    if (cut.wide)
+        e = out32 ? launch_wide8<float>(tk, tv, pg, a, cut.ctas, st) : launch_wide8<__half>(tk, tv, pg, a, cut.ctas, st);
+    else if (cut.nt == 1)
         e = f32     ? launch8<float, float, 1>(tk, tv, pg, a, cut.ctas, st)
             : out32 ? launch8<__half, float, 1>(tk, tv, pg, a, cut.ctas, st)
                     : launch8<__half, __half, 1>(tk, tv, pg, a, cut.ctas, st);
