@@ -594,7 +594,8 @@ attn_kv8_join_kernel(const __grid_constant__ Attn8Params p, int per_row) {
     pdl_wait();
     const int4 note = p.notes[blockIdx.x];
     const int c = note.z;
-    if (note.x < 0) return;
+    // (a run that gave up leaves notes unwritten: what stood there stays inside the arrays)
+    if (note.x < 0 || note.x >= p.n || note.y < 0 || note.y >= p.n_kv * p.row_blocks || c < 0 || note.w < c || note.w >= p.ctas) return;
     const int h = note.y / p.row_blocks, r = note.y % p.row_blocks * p.block_rows + in;
     const bool live = in < p.block_rows && r < p.rows;
     // parts: the second of the first CTA's, then the first of the following CTAs'
@@ -777,6 +778,7 @@ extern "C" int sllm_cuda_attn_kv8(const sllm_cuda_kv_pages* p, int32_t layer, co
     a.rows = n_q * a.group;
     a.over_group = a.group == 1 ? 0 : (uint32_t)(((1ull << 32) + a.group - 1) / a.group);
     a.q_bufs = cut.block_rows <= 32 ? 2 : 1;
+    a.ctas = cut.ctas;
     a.rg = cut.rg; a.row_blocks = cut.row_blocks; a.block_rows = cut.block_rows;
     while ((1 << a.page_log2) < p->page_size) ++a.page_log2;
     a.wait = attn_wait_limit();

@@ -41,7 +41,7 @@ struct Attn8Params {
     // pair where there are no more pairs than CTAs (by_pair), else of the pair that starts
     // in a CTA's run and ends in another's
     int4* notes;
-    int by_pair, n_notes;
+    int by_pair, n_notes, ctas;
     uint32_t over_group;            // ceil(2^32 / group), 0 for 1: exact below 2^22 (rows are under 2^14, groups up to 2^10)
 
     __device__ __forceinline__ int token(int row) const { return over_group == 0 ? row : (int)__umulhi((uint32_t)row, over_group); }
