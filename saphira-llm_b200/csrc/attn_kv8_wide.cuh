@@ -37,7 +37,7 @@ constexpr uint32_t kW8Cols = 256, kW8O = 2 * kW8Rows, kW8K = 128;       // tenso
 
 struct Plan8 {
     Meta meta;
-    float ks[kE8Blocks], vs[kE8Blocks];             // of each block of 16 keys; without one 0 and 1
+    __align__(8) float ks[kE8Blocks], vs[kE8Blocks];             // of each block of 16 keys; without one 0 and 1
 };
 
 struct __align__(1024) SharedW8 {
@@ -380,18 +380,24 @@ attn_kv8_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
             if (!ok) break;
             end = (sh.plan[(n + 1) % kW8Plans].meta.flags & E8_END) != 0;
             uint8_t* const raw = sh.raw[unit % kW8Ring];
+            const float2 sv = *reinterpret_cast<const float2*>(sh.plan[n % kW8Plans].vs + 2 * cw);
             #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int row = vrow + 8 * (i >> 1), half = i & 1;
-                uint4 c = *reinterpret_cast<const uint4*>(swizzled(raw, row, 4 * half + piece));
-                // (a scale of 0 is zeros, whatever the codes are)
-                if (sh.plan[n % kW8Plans].vs[2 * cw + (i >> 2)] == 0.f) c = make_uint4(0, 0, 0, 0);
-                uint32_t f[8];
-                codes16(c, f);
+            for (int g = 0; g < 2; ++g) {           // a block of 16 keys
+                uint4 c[4];
                 #pragma unroll
-                for (int j = 0; j < 2; ++j)
-                    *reinterpret_cast<uint4*>(swizzled(sh.v + half * kW8Half, row, 2 * piece + j)) =
-                        make_uint4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
+                for (int i = 0; i < 4; ++i)
+                    c[i] = *reinterpret_cast<const uint4*>(swizzled(raw, vrow + 16 * g + 8 * (i >> 1), 4 * (i & 1) + piece));
+                // (a scale of 0 is zeros, whatever the codes are)
+                if ((g == 0 ? sv.x : sv.y) == 0.f) c[0] = c[1] = c[2] = c[3] = make_uint4(0, 0, 0, 0);
+                #pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t f[8];
+                    codes16(c[i], f);
+                    #pragma unroll
+                    for (int j = 0; j < 2; ++j)
+                        *reinterpret_cast<uint4*>(swizzled(sh.v + (i & 1) * kW8Half, vrow + 16 * g + 8 * (i >> 1), 2 * piece + j)) =
+                            make_uint4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
+                }
             }
             consumed();
             fence_proxy_async_smem();
