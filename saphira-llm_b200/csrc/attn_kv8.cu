@@ -332,7 +332,7 @@ struct Rows8 {
                 for (int j = 0; j < 4; ++j)
                     to[r * 32 + ((4 * g + j) ^ t)] =
                         make_float4(o[n][2 * j][c], o[n][2 * j][c + 2], o[n][2 * j + 1][c], o[n][2 * j + 1][c + 2]);
-                if (g == 0) ml[r] = make_float2(m[n][c], l[n][c]);
+                if (g == 0) ml[r] = make_float2(m[n][c], l[n][c] * e8_down(P));
             }
     }
 };
@@ -545,7 +545,8 @@ attn_kv8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant_
             for (int blk = kg; blk * kKvBlock < keys; blk += 2 * KG) {
                 const bool two = (blk + KG) * kKvBlock < keys;
                 const float ks[2] = {sc[blk], two ? sc[blk + KG] : 0.f};
-                const float vs[2] = {sc[kE8Blocks + blk], two ? sc[kE8Blocks + blk + KG] : 0.f};
+                // (without the weights' lift: outputs overflow no sooner than the values do)
+                const float vs[2] = {sc[kE8Blocks + blk] * e8_down(P), two ? sc[kE8Blocks + blk + KG] * e8_down(P) : 0.f};
                 rows.blocks(sh.stage[slot].k + blk * kKvBlock * kServeDim, sh.stage[slot].v + blk * kKvBlock * kServeDim,
                             KG * kKvBlock * kServeDim, ks, vs, masked, mt.key0 + blk * kKvBlock, KG * kKvBlock);
             }

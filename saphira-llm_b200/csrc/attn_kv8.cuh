@@ -18,6 +18,7 @@ constexpr int kE8Tile = kE8Keys * kServeDim;        // bytes of one of K or V
 constexpr float kE8None = -1e30f;
 constexpr float kE8Grow = 8.f;
 __host__ __device__ constexpr float e8_lift(int planes) { return planes == 1 ? 15.f - kE8Grow : 15.f; }
+__host__ __device__ constexpr float e8_down(int planes) { return planes == 1 ? 0x1p-7f : 0x1p-15f; }         // 2^-lift
 constexpr float kE8Log2 = kServeScale * 1.4426950408889634f;
 
 struct Attn8Params {

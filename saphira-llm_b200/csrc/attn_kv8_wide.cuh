@@ -8,11 +8,13 @@
 //     S^T [128 keys][32 rows] = C Q^T                 (codes: 128 lanes of tensor memory)
 //     w = 2^(s log2 e / sqrt 128 * scale_k + log2 scale_v - ref)
 //     O^T [128 dimensions][32 rows] += C'^T W         (W: f16, in shared memory)
-//     l += w / scale_v
+//     l += 2^(s log2 e / sqrt 128 * scale_k - ref)
 // so w stands for a key's weight times its value scale, against a reference per row
 // that is no lower than the row's largest such product over 2^8 (as in the form of
-// 16 rows, products keep 11 bits down to 2^-21 of the largest). A block of scale_v 0
-// has zeros for values, whatever its codes, and 1 in the exponents.
+// 16 rows, products keep 11 bits down to 2^-21 of the largest). The sums have exponents
+// of their own: w / scale_v would be lost where scales are 2^110 apart. A block of
+// scale_v 0 has zeros for values, whatever its codes, and in the exponents the lowest
+// scale there is, 2^-100, so that it moves no reference that matters.
 //
 // Two CTAs a SM. Warps 0-3 and 4-7 (a key a lane, 16 of the rows each group):
 // exponentials. 8-11 (32 keys each): codes to f16, K's into tensor memory, V's into
@@ -31,6 +33,7 @@ constexpr int kW8Products = kW8Soft + kW8Load, kW8Plan = kW8Products + 1;       
 constexpr int kW8Threads = 32 * (kW8Plan + 1), kW8Ctas = 2;                     // CTAs a SM
 constexpr int kW8Half = kE8Keys * 128;              // 64 of the dimensions of a tile, f16
 constexpr int kW8Extra = 2;                         // what a pair's start and end cost, in tiles (with 1 or 3: 72 and 70 us for 68)
+constexpr float kW8Zero = -100.f;                   // log2 of a scale of 0
 constexpr int kW8Plans = 8;                         // tiles planned ahead, some of them in use
 constexpr int kW8Ring = 3;                          // K or V of a tile each
 constexpr uint32_t kW8Cols = 256, kW8O = 2 * kW8Rows, kW8K = 128;       // tensor memory: two S tiles, the outputs, two K tiles
@@ -185,7 +188,7 @@ attn_kv8_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
                 __syncwarp();
             }
             const float ks = sh.plan[n % kW8Plans].ks[key / kKvBlock], vs = sh.plan[n % kW8Plans].vs[key / kKvBlock];
-            const float base = ks * kE8Log2, lsv = vs != 0.f ? __log2f(vs) : 0.f, isv = vs != 0.f ? __fdividef(1.f, vs) : 1.f;
+            const float base = ks * kE8Log2, lsv = vs != 0.f ? __log2f(vs) : kW8Zero;
             const bool masked = mt.key0 + kE8Keys > mt.len - p.n_q + 1;
             // exponents of two against the references
             auto exponents = [&] {
@@ -255,8 +258,8 @@ attn_kv8_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
             }
             #pragma unroll
             for (int i = 0; i < R; ++i) {
+                l[i] += ex2(z[i] - lsv);
                 z[i] = ex2(z[i]);
-                l[i] = __fmaf_rn(z[i], isv, l[i]);
             }
             if (n >= 2) ok = at_wait_warp(&sh.p_free[b], par ^ 1, ab, w) && ok;
             if (ok) {

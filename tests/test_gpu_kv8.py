@@ -377,6 +377,77 @@ def test_attn8_unseen_places_leave_no_trace(cuda, dt):
     assert c.take_status() == 0 and torch.equal(a, b)
 
 
+@pytest.mark.parametrize("rows", [(8, 1), (24, 1), (8, 4), (64, 1)])
+@pytest.mark.parametrize("dt", ["f32", "f16"])
+@pytest.mark.parametrize("low,high", [(-24, 24), (-69, 80), (-40, -38)])
+def test_attn8_scales_far_apart(cuda, dt, rows, low, high):
+    """Value scales of e^low to e^high in neighbouring blocks, and blocks of scale 0 that hold codes.
+
+    Where f16 weights are rounded together with their keys' scales, a product below 2^-14 of the range is off by
+    2^-25 of it, and the largest of a row stands at 2^7 of it at least: an absolute 2^-32 of the row's largest
+    product of weight and scale, times each key's code."""
+    import torch
+    H, nq = rows
+    lens = [300, 1000, 17]
+    c = Eight(cuda, 90, 3, 64, 16, 1, 1, seed=2)
+    c.place(lens, seed=3)
+    r = np.random.default_rng(9)
+    sv = np.exp(r.uniform(low, high, c.host.scales[1].shape)).astype(np.float32)
+    sv[r.random(sv.shape) < 0.2] = 0
+    c.host.scales[1][:] = sv
+    c.vs.copy_(_t(sv))
+    q = _q(5, 3, nq, H, _dt(dt), 0.4)
+    out = run_attn8(c, 0, q, [0, 1, 2], torch.float32)
+    assert c.take_status() == 0
+    for b, L in enumerate(lens):
+        k, v = (torch.from_numpy(c.host.values(w, 0, c.m.tables[b], L)).cuda()[0] for w in range(2))
+        scale = torch.from_numpy(np.repeat(np.concatenate([sv[p, 0, 0] for p in c.m.tables[b]]), BLOCK)[:L]).cuda().double()
+        for h in range(H):
+            lim = torch.tensor([max(0, L - nq + 1 + j) for j in range(nq)], device="cuda")
+            o, pv, big, va = attention(q[b, :, h].double(), k, v, lim)
+            tol = attn8_bound(o, pv, big, va, L, dt == "f16", False)
+            if dt == "f16":
+                s = q[b, :, h].double() @ k.T / math.sqrt(128)
+                s[torch.arange(L, device="cuda")[None] >= lim[:, None]] = -math.inf
+                top = (torch.softmax(s, -1) * scale).amax(-1, keepdim=True)
+                codes = torch.where(scale[:, None] > 0, v / scale[:, None], 0.).abs().sum(0)
+                tol = tol + 2.0 ** -32 * 1.01 * top * codes
+            err = (out[b, :, h].double() - o).abs()
+            assert bool((err <= tol).all()), (b, h, float((err / tol).nan_to_num(math.inf).max()))
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16"])
+@pytest.mark.parametrize("rows", [(8, 1), (16, 1), (24, 1), (64, 1)])
+def test_attn8_a_wait_that_runs_out_is_reported(cuda, dt, rows):
+    """With a limit of 1 ns a CTA's first wait runs out (all of them load at once, from memory): the kernels end,
+    *status and the error word say so, and the next call is as good as ever. In a workspace that an earlier call has
+    used, and in two of no good numbers."""
+    import torch
+    H, nq, n = 5 * rows[0], rows[1], 24
+    c = Eight(cuda, 800, n, 33, 16, 1, 5, seed=2)
+    c.place([500] * n, seed=3)
+    q = _q(5, n, nq, H, _dt(dt))
+    good = run_attn8(c, 0, q, list(range(n)), _dt(dt))
+    assert c.take_status() == 0 and cuda.attn_error() == 0
+    out, slots = torch.empty_like(q), _i32(list(range(n)))
+    size = c.p.attn8_work_bytes(n, nq, H)
+    flush = torch.empty(256 << 20, dtype=torch.uint8, device="cuda")
+    works = [torch.full((size // 4 + 1,), x, dtype=torch.int32, device="cuda").view(torch.uint8) for x in (0, 0x7f7f7f7f, 12345)]
+    c.p.attn8(0, q, out, slots, works[0], c.status)
+    cuda.set_attn_wait(1)
+    try:
+        for work in works:
+            flush.zero_()
+            c.p.attn8(0, q, out, slots, work, c.status)
+        torch.cuda.synchronize()
+    finally:
+        cuda.set_attn_wait(0)
+    assert c.take_status() == -61 and cuda.attn_error() != 0
+    cuda.attn_error()                                       # (one word per file)
+    assert torch.equal(run_attn8(c, 0, q, list(range(n)), _dt(dt)), good)
+    assert c.take_status() == 0 and cuda.attn_error() == 0
+
+
 def test_attn8_bad_sequences_are_reported(cuda):
     """Wrong slots, lengths and pages: *status says so, and the other sequences come out right."""
     import torch
