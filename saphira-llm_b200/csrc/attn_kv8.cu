@@ -16,7 +16,7 @@
 // f32 queries and weights are pairs of f16, x = hi + 2^-11 lo, with a power of
 // two per query row; two products then, 22 bits.
 //
-// 17 rows and more of f16 queries go to attn_kv8_wide.cuh.
+// Much work of 17 rows and more of f16 queries goes to attn_kv8_wide.cuh.
 //
 // The work is cut by the device: the tiles of 128 keys of all (sequence, kv
 // head) pairs, in order, are dealt to the CTAs in equal runs. A pair inside one
@@ -667,13 +667,24 @@ struct Cut8 {
     bool wide;
     int nt, rg, block_rows, row_blocks, ctas;
 };
-Cut8 cut8(int rows, bool f16, int sms) {
+// `keys`: the most that there may be, of all pairs. The wide form's longer chain
+// from a CTA's first load to its last result costs 4 us, and its tiles take four
+// fifths of the time. Both measured, in us, f16 (wide, this file's): 10 sequences of
+// 1000 keys at most, 4 tokens of 64/8 heads (80 thousand keys at most) 22.6, 18.8; 64
+// of 1000 (512) 49.4, 47.5; 30 of 4000, 5 tokens of 20/5 heads (600) 41.8, 43.1; one of
+// 60000 (480) 50.0, 55.6; 8 of 8000, 8 tokens (1024) 63.4, 71.2; 32 of 8192 (2097)
+// 97, 110.
+constexpr long long kE8WideKeys = 3000;             // a SM
+Cut8 cut8(int rows, bool f16, int sms, long long keys) {
     Cut8 x;
     x.wide = f16 && rows > 16;
     if (x.wide) {
         x.nt = x.rg = 0;
         x.block_rows = kW8Rows;
         x.row_blocks = (rows + kW8Rows - 1) / kW8Rows;
+        x.wide = keys * x.row_blocks >= kE8WideKeys * sms;
+    }
+    if (x.wide) {
         x.ctas = sms * kW8Ctas;
         return x;
     }
@@ -740,7 +751,7 @@ int sllm::take_kv8_error() { return take_attn_error(); }
 
 extern "C" size_t sllm_cuda_attn_kv8_work_bytes(const sllm_cuda_kv_pages* p, int32_t n, int32_t n_q, int32_t n_head) {
     if (check_shape8(p, n, n_q, n_head, "attn_kv8_work_bytes") != SLLM_CUDA_OK) return 0;
-    return work8_bytes(cut8(n_q * (n_head / p->n_head_kv), false, current_sms()));
+    return work8_bytes(cut8(n_q * (n_head / p->n_head_kv), false, current_sms(), 0));
 }
 
 extern "C" int sllm_cuda_attn_kv8(const sllm_cuda_kv_pages* p, int32_t layer, const void* q, int32_t q_type,
@@ -755,8 +766,8 @@ extern "C" int sllm_cuda_attn_kv8(const sllm_cuda_kv_pages* p, int32_t layer, co
         (q_type == SLLM_CUDA_KV_F32 && out_type == SLLM_CUDA_KV_F16))
         return fail(SLLM_CUDA_ERR_ARG, "attn_kv8: query type %d, output type %d (f32, or f16 from f16)", q_type, out_type);
     const int sms = current_sms(), rows = n_q * (n_head / p->n_head_kv);
-    const Cut8 cut = cut8(rows, q_type == SLLM_CUDA_KV_F16, sms);
-    const size_t need = work8_bytes(cut8(rows, false, sms));
+    const Cut8 cut = cut8(rows, q_type == SLLM_CUDA_KV_F16, sms, (long long)n * p->n_head_kv * p->table_width * p->page_size);
+    const size_t need = work8_bytes(cut8(rows, false, sms, 0));
     if (!aligned16(q) || !aligned16(out) || !aligned16(work) || work_bytes < need)
         return fail(SLLM_CUDA_ERR_ARG, "attn_kv8: workspace of %zu bytes (%zu needed), arrays 16-byte aligned", work_bytes, need);
     const void* ptr[] = {p->k, p->v, p->tables, p->lens, p->k_scale, p->v_scale, q, slots, out, work, status};

@@ -308,6 +308,54 @@ def test_attn8(cuda, case, page, types):
                 assert bool((out[b, j] == 0).all())
 
 
+@pytest.mark.parametrize("case", [x for x in CASES if x[0][0] // x[0][1] * x[1] > 16], ids=str)
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("out", ["f16", "f32"])
+def test_attn8_wide_tables(cuda, case, page, out):
+    """Tables with room for many keys, as of long contexts: the form for much work of 17 rows and more."""
+    (H, Hkv), nq, lens = case
+    width = (1 << 20) // page // len(lens) + max(lens) // page
+    c = Eight(cuda, sum(x // page + 1 for x in lens) + 9, len(lens) + 2, width, page, 2, Hkv, seed=H + nq)
+    c.place([9] + lens + [40], seed=nq)
+    slots = np.random.default_rng(H).permutation(np.arange(1, len(lens) + 1)).tolist()
+    q = _q(H + nq, len(lens), nq, H, _dt("f16"))
+    o = run_attn8(c, 1, q, slots, _dt(out))
+    assert c.take_status() == 0
+    check_attn8(c, 1, q, o, slots, True)
+    for b, s in enumerate(slots):
+        for j in range(nq):
+            if c.m.lens[s] - nq + 1 + j <= 0:
+                assert bool((o[b, j] == 0).all())
+    # bad ones are reported, and the others come out right
+    import torch
+    c.lens[slots[0]] = -1
+    bad = run_attn8(c, 1, q, slots, _dt(out))
+    assert c.take_status() == -1
+    assert bool(torch.allclose(bad[1:].float(), o[1:].float(), atol=2e-3))
+    c.lens[slots[0]] = c.m.lens[slots[0]]
+    c.tables[slots[0], 0] = 1 << 30
+    bad = run_attn8(c, 1, q, slots, _dt(out))
+    assert c.take_status() == (-1 if c.m.lens[slots[0]] > 0 else 0)
+    assert torch.equal(bad[1:], o[1:])
+
+
+@pytest.mark.parametrize("page", [16, 128])
+def test_attn8_wide_long_and_short(cuda, page):
+    """Much work of 17 rows and more: very different lengths, one row block and two, several times the same."""
+    import torch
+    r = np.random.default_rng(4)
+    lens = [int(x) for x in np.exp(r.uniform(0, 6, 70))] + [20000, 0, 1]
+    c = Eight(cuda, sum(x // page + 1 for x in lens) + 3, len(lens), max(lens) // page + 1, page, 1, 2, seed=8)
+    c.place(lens, seed=1)
+    slots = r.permutation(len(lens)).tolist()
+    for nq, H in ((3, 16), (7, 14), (1, 130)):
+        q = _q(3, len(lens), nq, H, torch.float16)
+        out = run_attn8(c, 0, q, slots, torch.float16)
+        assert c.take_status() == 0
+        check_attn8(c, 0, q, out, slots, True)
+        assert torch.equal(run_attn8(c, 0, q, slots, torch.float16), out)
+
+
 @pytest.mark.parametrize("dt", ["f32", "f16"])
 @pytest.mark.parametrize("page", [16, 128])
 def test_attn8_long_and_short(cuda, dt, page):
@@ -389,7 +437,7 @@ def test_attn8_scales_far_apart(cuda, dt, rows, low, high):
     import torch
     H, nq = rows
     lens = [300, 1000, 17]
-    c = Eight(cuda, 90, 3, 64, 16, 1, 1, seed=2)
+    c = Eight(cuda, 90, 3, 64 if dt == "f32" else 16384, 16, 1, 1, seed=2)
     c.place(lens, seed=3)
     r = np.random.default_rng(9)
     sv = np.exp(r.uniform(low, high, c.host.scales[1].shape)).astype(np.float32)
@@ -401,7 +449,7 @@ def test_attn8_scales_far_apart(cuda, dt, rows, low, high):
     assert c.take_status() == 0
     for b, L in enumerate(lens):
         k, v = (torch.from_numpy(c.host.values(w, 0, c.m.tables[b], L)).cuda()[0] for w in range(2))
-        scale = torch.from_numpy(np.repeat(np.concatenate([sv[p, 0, 0] for p in c.m.tables[b]]), BLOCK)[:L]).cuda().double()
+        scale = torch.from_numpy(np.repeat(np.concatenate([sv[p, 0, 0] for p in c.m.tables[b][:c.m.used(L)]]), BLOCK)[:L]).cuda().double()
         for h in range(H):
             lim = torch.tensor([max(0, L - nq + 1 + j) for j in range(nq)], device="cuda")
             o, pv, big, va = attention(q[b, :, h].double(), k, v, lim)
@@ -424,7 +472,7 @@ def test_attn8_a_wait_that_runs_out_is_reported(cuda, dt, rows):
     used, and in two of no good numbers."""
     import torch
     H, nq, n = 5 * rows[0], rows[1], 24
-    c = Eight(cuda, 800, n, 33, 16, 1, 5, seed=2)
+    c = Eight(cuda, 800, n, 33 if dt == "f32" else 1024, 16, 1, 5, seed=2)
     c.place([500] * n, seed=3)
     q = _q(5, n, nq, H, _dt(dt))
     good = run_attn8(c, 0, q, list(range(n)), _dt(dt))
