@@ -419,8 +419,11 @@ SLLM_CUDA_API int sllm_cuda_kv8_read(const sllm_cuda_kv_pages * p, int32_t layer
  * q_type, out f32 or, from f16 queries, f16. Codes are multiplied on the tensor
  * cores exactly, in f32 sums; f16 queries are taken as they are, f32 queries and
  * their softmax weights as pairs of f16 (22 bits), the weights of f16 queries
- * rounded to f16 (11 bits down to 2^-21 of a row's largest). A sequence whose slot, length or table is wrong sets
- * SLLM_CUDA_ERR_ARG in *status, and its rows of out mean nothing. n <= 4096, n_q
+ * rounded to f16 (11 bits down to 2^-21 of a row's largest; of more than 16 query
+ * rows a kv head the weights times their keys' value scales are, or the weights
+ * alone where the tables have room for little). A sequence whose slot, length or
+ * table is wrong sets SLLM_CUDA_ERR_ARG in *status, and its rows of out mean
+ * nothing; a wait that runs out (2 s) sets SLLM_CUDA_ERR_TIMEOUT. n <= 4096, n_q
  * <= 16, n_head <= 1024. A workspace of work_bytes(n, n_q, n_head) serves every
  * call over this cache with that n_head and no more sequences and query tokens.
  */
@@ -435,11 +438,11 @@ SLLM_CUDA_API int sllm_cuda_attn_kv8(const sllm_cuda_kv_pages * p, int32_t layer
  * One step of n beam searches of `beams` beams each. Request i's candidates are
  * (b, x): beam b continued by word x, of value
  *     score[i][b] + logits[i][b][x] - ln sum_y exp(logits[i][b][y])
- * (64 bits; the exponentials 32, their sum 64; logits beyond 2^100 as that); a beam with done[i][b] != 0 has
- * one candidate, eos, of its own score (done NULL: none is). The `beams` best come out
- * in descending order: parent, token and score_out [n][beams]. Equal values: the
- * lower beam first, then the larger logit, then the lower word. Row (i, b) of the logits lies
- * at logits + (i * beams + b) * row_stride. A score or logit of -inf makes
+ * (64 bits; the exponentials 32, their sum 64; logits beyond 2^100 as that); a beam
+ * with done[i][b] != 0 has one candidate, eos, of its own score (done NULL: none is).
+ * The `beams` best come out in descending order: parent, token and score_out
+ * [n][beams]. Equal values: the lower beam first, then the larger logit, then the
+ * lower word. Row (i, b) of the logits lies at logits + (i * beams + b) * row_stride. A score or logit of -inf makes
  * candidates of value -inf, which are chosen, lowest (b, x) first, only when
  * there are no others; NaN and +inf count as -inf and set SLLM_CUDA_ERR_ARG in
  * *status. done_out[i][j] (may be NULL) is 1 when the parent was done or the

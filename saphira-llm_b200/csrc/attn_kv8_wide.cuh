@@ -20,6 +20,14 @@
 // exponentials. 8-11 (32 keys each): codes to f16, K's into tensor memory, V's into
 // shared memory, K a tile ahead of V. 12: the products. 13: which tile comes next, its
 // scales, and its codes into a ring of 16 KB a half tile.
+//
+// Bound: neither memory nor the tensor cores but the chains between the roles, two
+// of them a SM, with half of the issue slots taken (32 sequences of up to 4096 keys,
+// four tokens of 64/8 heads, 139 MB: 63 us, 22 at the memory's rate). Tried, same
+// case: one CTA a SM with 18 warps and tiles double buffered 77 us; two with the
+// codes loaded into registers, a block ahead, 68 us (49 without the loads: their
+// latency was the bound, hence the ring); outputs read after the next tile's
+// weights 66 us for 62; row maxima by shuffles instead of redux 84 for 72.
 #pragma once
 
 #include "attn_kv8.cuh"
