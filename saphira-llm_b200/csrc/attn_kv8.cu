@@ -29,7 +29,7 @@
 // of codes and scales, 54 us; 64 of up to 8192, 539 MB, 96 us, 5.6 TB/s), with the
 // issue slots half taken: a block of 16 keys and eight rows is about 70 instructions
 // of a warp. For little work the chain is the bound: lengths, page ids, tile,
-// products, the parts and their join (one sequence of 300 keys 11 us, 2 of them
+// products, the parts and their join (one sequence of 320 keys 11 us, 2 of them
 // the join). Tiles of 128 keys in two stages leave room for three CTAs a SM
 // with up to eight rows, each with a warp that loads.
 

@@ -112,8 +112,8 @@ __device__ __forceinline__ int page_at(const PagesDev& p, int slot, int pos) {
 // per entry, behind the first pair's loads. The q rows are rotated by CTAs of
 // their own, eight rows a warp.
 // Bound: HBM for a prompt (4099 tokens of 64/8 heads, f16 outputs, 270 MB: 48 us, 5.6
-// TB/s), else the chain of page id, values, old scale and codes, stores (four tokens
-// of 20/5 heads: 7 us).
+// TB/s), else the chain of page id, values, old scale and codes, stores (16 tokens of
+// 20/5 heads: 7 us).
 // ---------------------------------------------------------------------------
 struct Run {
     RotPair r[8];
