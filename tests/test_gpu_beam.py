@@ -86,6 +86,11 @@ def test_select_sizes(cuda, n, B, V):
     check(cuda, _logits(n + V, n, B, V), _scores(n, n, B))
 
 
+@pytest.mark.parametrize("n,B,V", [(65536, 1, 3), (20000, 2, 2), (4, 16, 1 << 20)])
+def test_select_limits(cuda, n, B, V):
+    check(cuda, _logits(n + V, n, B, V), _scores(n, n, B))
+
+
 @pytest.mark.parametrize("V", [40, 3001, 40000])
 def test_done_beams(cuda, V):
     """Finished beams stay with their own score; all of them; one among others; of score -inf."""

@@ -636,3 +636,134 @@ def test_stream_and_graph(cuda):
         for b, n in enumerate((50, 17, 100)):
             assert np.array_equal(ko[b].cpu().numpy(),
                                   c.host.values(0, 0, c.m.tables[b], n)[:, -1].astype(np.float32))
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16"])
+def test_attn8_limits(cuda, dt):
+    """The most sequences, query tokens and heads that a call takes."""
+    import torch
+    r = np.random.default_rng(1)
+    n = 4096
+    lens = r.integers(0, 20, n).tolist()
+    c = Eight(cuda, 2 * n, n, 2, 16, 1, 1, seed=2)
+    c.place(lens, seed=3)
+    q = _q(5, n, 1, 1, _dt(dt))
+    out = run_attn8(c, 0, q, list(range(n)), _dt(dt))
+    assert c.take_status() == 0
+    check_attn8(c, 0, q, out, list(range(n)), dt == "f16")
+    c = Eight(cuda, 8, 1, 3, 16, 1, 1, seed=2)
+    c.place([40], seed=3)
+    q = _q(6, 1, 16, 1024, _dt(dt))
+    out = run_attn8(c, 0, q, [0], _dt(dt))
+    assert c.take_status() == 0
+    check_attn8(c, 0, q, out, [0], dt == "f16")
+    wide = Eight(cuda, 8, 1, 4096, 16, 1, 1, seed=2)
+    wide.place([40], seed=3)
+    out = run_attn8(wide, 0, q, [0], _dt(dt))
+    assert wide.take_status() == 0
+    check_attn8(wide, 0, q, out, [0], dt == "f16")
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16"])
+def test_attn8_workspace_of_the_largest_call_serves_the_smaller(cuda, dt):
+    """One workspace for calls of fewer and fewer sequences and query tokens; what lies behind it stays."""
+    import torch
+    H, n = 24, 20
+    c = Eight(cuda, 900, n, 1024, 16, 1, 1, seed=2)
+    c.place(np.random.default_rng(3).integers(1, 600, n).tolist(), seed=3)
+    size = c.p.attn8_work_bytes(n, 4, H)
+    work = torch.full((size + 4096,), 77, dtype=torch.uint8, device="cuda")
+    for m, nq in ((n, 4), (7, 4), (n, 1), (3, 2), (1, 1)):
+        q = _q(m + nq, m, nq, H, _dt(dt))
+        out = torch.empty_like(q)
+        assert c.p.attn8_work_bytes(m, nq, H) <= size
+        c.p.attn8(0, q, out, _i32(list(range(m))), work[:size], c.status)
+        assert c.take_status() == 0
+        check_attn8(c, 0, q, out, list(range(m)), dt == "f16")
+    assert bool((work[size:] == 77).all())
+
+
+@pytest.mark.parametrize("dt,nq,H", [("f32", 1, 8), ("f16", 1, 8), ("f16", 3, 8)])
+def test_attn8_replayed_with_other_sequences(cuda, dt, nq, H):
+    """A captured call follows the lengths and slots that stand in its arrays when it is replayed; two graphs
+    share a workspace, one after the other."""
+    import torch
+    c = Eight(cuda, 700, 6, 8192, 16, 1, 1, seed=2)
+    c.place([1000, 33, 5000, 1, 700, 64], seed=3)
+    q, slots = _q(5, 3, nq, H, _dt(dt)), _i32([0, 1, 2])
+    outs = [torch.empty_like(q) for _ in range(2)]
+    work = torch.empty(c.p.attn8_work_bytes(3, nq, H), dtype=torch.uint8, device="cuda")
+    graphs = []
+    for out in outs:
+        g = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g):
+            c.p.attn8(0, q, out, slots, work, c.status, stream=torch.cuda.current_stream())
+        graphs.append(g)
+    for names in ([0, 1, 2], [3, 4, 5], [2, 2, 0]):
+        slots.copy_(_i32(names))
+        for x in range(2):
+            q.copy_(_q(x + 7, 3, nq, H, _dt(dt)))
+            graphs[x].replay()
+            torch.cuda.synchronize()
+            assert c.take_status() == 0
+            check_attn8(c, 0, q, outs[x], names, dt == "f16")
+
+
+def test_calls_at_once(cuda):
+    """Stores, reads, both forms of attention and beam selection on four streams at once, a workspace each: as one
+    after the other."""
+    import torch
+    n, H, Hkv = 24, 16, 2
+    c = Eight(cuda, 2600, 2 * n, 1024, 16, 2, Hkv, seed=2)
+    c.place(np.random.default_rng(3).integers(100, 1000, 2 * n).tolist(), seed=3)
+    slots = _i32(list(range(n)))
+    q1, q4 = _q(5, n, 1, H, torch.float16), _q(6, n, 4, H, torch.float16)
+    q32 = _q(7, n, 2, H, torch.float32)
+    logits, score = _q(8, 8, 4, 100, torch.float32).view(8, 4, -1), torch.zeros((8, 4), device="cuda")
+    cos, sin = _angles(1024)
+    dc, ds = _t(cos), _t(sin)
+    x = torch.randn((n, 2 * Hkv, 128), generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")
+    new = _i32([n + i for i in range(n)])
+    pos = _i32([c.m.lens[n + i] - 1 for i in range(n)])
+    start = [t.clone() for t in (c.k, c.v, c.ks, c.vs)]
+
+    def calls(s, work):
+        o = {"one": torch.empty_like(q1), "four": torch.empty_like(q4), "f32": torch.empty_like(q32),
+             "ko": torch.empty((n, Hkv, 128), device="cuda"), "vo": torch.empty((n, Hkv, 128), device="cuda"),
+             "so": torch.empty((8, 4), device="cuda"), "pa": _i32([[0] * 4] * 8), "to": _i32([[0] * 4] * 8)}
+        torch.cuda.synchronize()
+
+        def go(which):
+            if which == 0:
+                c.p.append8(1, new, pos, None, x[:, :Hkv], x[:, Hkv:], dc, ds, status=c.status, stream=s[0])
+                c.p.read8(1, new, pos, o["ko"], o["vo"], c.status, stream=s[0])
+            elif which == 1:
+                c.p.attn8(0, q1, o["one"], slots, work[0], c.status, stream=s[1])
+                c.p.attn8(0, q32, o["f32"], slots, work[0], c.status, stream=s[1])
+            elif which == 2:
+                c.p.attn8(0, q4, o["four"], slots, work[1], c.status, stream=s[2])
+            else:
+                cuda.beam_select(logits, score, o["so"], o["pa"], o["to"], status=c.status, stream=s[3])
+        return o, go
+
+    work = [torch.empty(c.p.attn8_work_bytes(n, 4, H), dtype=torch.uint8, device="cuda") for _ in range(2)]
+    one = torch.cuda.current_stream()
+    want, go = calls([one] * 4, work)
+    for w in range(4):
+        go(w)
+    torch.cuda.synchronize()
+    stored = [t.clone() for t in (c.k, c.v, c.ks, c.vs)]
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    for _ in range(10):
+        for t, old in zip((c.k, c.v, c.ks, c.vs), start):
+            t.copy_(old)
+        got, go = calls(streams, work)
+        for w in (2, 0, 3, 1):
+            go(w)
+        torch.cuda.synchronize()
+        assert c.take_status() == 0
+        for name in want:
+            assert torch.equal(got[name], want[name]), name
+        for t, new_ in zip((c.k, c.v, c.ks, c.vs), stored):
+            assert torch.equal(t, new_)
