@@ -352,12 +352,13 @@ attn_kv8_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
                     #pragma unroll
                     for (int i = 0; i < kW8Rows * 16 / (32 * kW8Load); ++i) {
                         const int y = (i * kW8Load + cw) * 32 + lane, r = y >> 4, c = y & 15;
-                        uint4 u = make_uint4(0, 0, 0, 0);
-                        if (r0 + r < p.rows)
-                            u = __ldg(reinterpret_cast<const uint4*>(static_cast<const __half*>(p.q) + p.row_at(mt.b, mt.head, r0 + r)) + c);
-                        *reinterpret_cast<uint4*>(swizzled(sh.q + (c >> 3) * kW8Rows * 128, r, c & 7)) = u;
+                        const bool there = r0 + r < p.rows;         // (else zeros)
+                        const __half* const from = static_cast<const __half*>(p.q) + p.row_at(mt.b, mt.head, there ? r0 + r : r0) + 8 * c;
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                                         smem_u32(swizzled(sh.q + (c >> 3) * kW8Rows * 128, r, c & 7))),
+                                     "l"(from), "r"(there ? 16 : 0)
+                                     : "memory");
                     }
-                    fence_proxy_async_smem();
                 }
                 if (!arrived()) return false;
                 uint8_t* const raw = sh.raw[unit % kW8Ring];
@@ -373,6 +374,10 @@ attn_kv8_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
                     tmem_st32(tm + 64 * b + 32 * h, f);
                 }
                 consumed();
+                if (mt.flags & E8_FIRST) {
+                    asm volatile("cp.async.wait_all;" ::: "memory");
+                    fence_proxy_async_smem();
+                }
                 tmem_st_wait();
                 tc_fence_before();
             }
