@@ -679,10 +679,10 @@ struct Cut8 {
 // `keys`: the most that there may be, of all pairs. The wide form's longer chain
 // from a CTA's first load to its last result costs 4 us, and its tiles take four
 // fifths of the time. Both measured, in us, f16 (wide, this file's): 10 sequences of
-// 1000 keys at most, 4 tokens of 64/8 heads (80 thousand keys at most) 22.6, 18.8; 64
-// of 1000 (512) 49.4, 47.5; 30 of 4000, 5 tokens of 20/5 heads (600) 41.8, 43.1; one of
-// 60000 (480) 50.0, 55.6; 8 of 8000, 8 tokens (1024) 63.4, 71.2; 32 of 8192 (2097)
-// 97, 110.
+// 1000 keys at most, 4 tokens of 64/8 heads (80 thousand keys at most) 22.6, 18.7; 20 of
+// 2000 (320) 33.2, 32.9; 64 of 1000 (512) 49.2, 47.4; 30 of 4000, 5 tokens of 20/5 heads
+// (600) 41.3, 42.8; one of 60000 (480) 48.6, 55.7; 8 of 8000, 8 tokens (1024) 61.7,
+// 71.7; 32 of 8192 (2097) 94, 110.
 constexpr long long kE8WideKeys = 3000;             // a SM
 Cut8 cut8(int rows, bool f16, int sms, long long keys) {
     Cut8 x;

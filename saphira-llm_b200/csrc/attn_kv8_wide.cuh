@@ -23,11 +23,14 @@
 //
 // Bound: neither memory nor the tensor cores but the chains between the roles, two
 // of them a SM, with half of the issue slots taken (32 sequences of up to 4096 keys,
-// four tokens of 64/8 heads, 139 MB: 63 us, 22 at the memory's rate). Tried, same
+// four tokens of 64/8 heads, 139 MB: 60 us, 22 at the memory's rate). Tried, same
 // case: one CTA a SM with 18 warps and tiles double buffered 77 us; two with the
 // codes loaded into registers, a block ahead, 68 us (49 without the loads: their
 // latency was the bound, hence the ring); outputs read after the next tile's
-// weights 66 us for 62; row maxima by shuffles instead of redux 84 for 72.
+// weights 66 us for 62; row maxima by shuffles instead of redux 84 for 72; queries
+// loaded before a pair's first tile instead of under it 63; K's codes left 1152 too
+// large, and the exponentials correcting it, 67; sums as w / scale_v while scales are
+// within 2^50, or exponents prepared while the scores are made, 61 to 63.
 #pragma once
 
 #include "attn_kv8.cuh"
