@@ -67,11 +67,11 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// ... from c0 in the even columns, c1 in the odd ones
-__device__ __forceinline__ void mma_f16_from(float (&d)[4], float c0, float c1, const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %10, %11};"
+// ... from zero
+__device__ __forceinline__ void mma_f16_zero(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
@@ -89,7 +89,7 @@ template <int P, int NT>
 struct Rows8 {
     uint32_t q[P][NT][16];
     float o[NT][8][4], m[NT][2], l[NT][2];
-    float mul[NT][2];               // pairs: the row's power of two. One f16: what its scores start from, see below
+    float mul[NT][2];               // the row's power of two (one f16: 1)
     int lim[NT][2];
 
     __device__ __forceinline__ void clear() {
@@ -124,21 +124,6 @@ struct Rows8 {
                     q[0][n][4 * i + 2] = u.z;
                     q[0][n][4 * i + 3] = u.w;
                 }
-                // K's codes go in 1152 too large, and 1152 times the row's sum less is
-                // where its scores start: half an instruction a code less, for
-                // 2^-24 of that sum, which is a hundredth of what half a step of a
-                // code is
-                float part[4] = {0.f, 0.f, 0.f, 0.f};
-                #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float2 z = unpack2(q[0][n][i]);
-                    part[i & 3] += z.x + z.y;
-                }
-                float sum = (part[0] + part[1]) + (part[2] + part[3]);
-                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                #pragma unroll
-                for (int c = 0; c < 2; ++c) mul[n][c] = -kE8Raw * __shfl_sync(0xffffffffu, sum, 8 * t + 4 * c);
             } else {
                 float4 f[8];
                 float most = 0.f;
@@ -191,14 +176,12 @@ struct Rows8 {
                 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
                     const uint32_t xa = wa[w] ^ 0x80808080u, xb = wb[w] ^ 0x80808080u;
-                    const uint32_t a[4] = {two_codes<P == 1>(xa, false), two_codes<P == 1>(xb, false), two_codes<P == 1>(xa, true),
-                                           two_codes<P == 1>(xb, true)};
+                    const uint32_t a[4] = {two_codes(xa, false), two_codes(xb, false), two_codes(xa, true), two_codes(xb, true)};
                     #pragma unroll
                     for (int n = 0; n < NT; ++n)
                         #pragma unroll
                         for (int x = 0; x < P; ++x) {
-                            if (i == 0 && w == 0)
-                                mma_f16_from(s[k][x][n], P == 1 ? mul[n][0] : 0.f, P == 1 ? mul[n][1] : 0.f, a, q[x][n][0], q[x][n][1]);
+                            if (i == 0 && w == 0) mma_f16_zero(s[k][x][n], a, q[x][n][0], q[x][n][1]);
                             else mma_f16(s[k][x][n], a, q[x][n][8 * i + 2 * w], q[x][n][8 * i + 2 * w + 1]);
                         }
                 }
@@ -299,14 +282,13 @@ struct Rows8 {
                 for (int hi = 0; hi < 2; ++hi) {
                     const uint32_t x = __byte_perm(wv[0][w], wv[1][w], hi ? 0x7362 : 0x5140);
                     const uint32_t z = __byte_perm(wv[2][w], wv[3][w], hi ? 0x7362 : 0x5140);
-                    const uint32_t a[4] = {two_codes<false>(x, false), two_codes<false>(x, true), two_codes<false>(z, false),
-                                           two_codes<false>(z, true)};
+                    const uint32_t a[4] = {two_codes(x, false), two_codes(x, true), two_codes(z, false), two_codes(z, true)};
                     const int j = 2 * w + hi;
                     #pragma unroll
                     for (int n = 0; n < NT; ++n) {
                         float d[P][4];
                         #pragma unroll
-                        for (int e = 0; e < P; ++e) mma_f16_from(d[e], 0.f, 0.f, a, pb[k][e][n][0], pb[k][e][n][1]);
+                        for (int e = 0; e < P; ++e) mma_f16_zero(d[e], a, pb[k][e][n][0], pb[k][e][n][1]);
                         #pragma unroll
                         for (int c = 0; c < 4; ++c)
                             o[n][j][c] = __fmaf_rn(P == 1 ? d[0][c] : __fmaf_rn(d[P - 1][c], 0x1p-11f, d[0][c]), vs[k], o[n][j][c]);

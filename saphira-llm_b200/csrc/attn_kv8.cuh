@@ -87,12 +87,12 @@ __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
 }
 
 // two codes, of bytes 0 and 1 or 2 and 3 of u (with 128 added to each), as f16:
-// 0x6400 + byte is 1024 + byte; `raw`: with the 1152 that this is too much
-constexpr float kE8Raw = 1152.f;
-template <bool RAW>
+// 0x6400 + byte is 1024 + byte. (K's codes left 1152 too large, with 1152 times the
+// row's sum taken off its scores, were half an instruction a code less, but the f32
+// sums then cancelled numbers far larger than a score: scores off by 1e-3 for
+// queries of mean 10.)
 __device__ __forceinline__ uint32_t two_codes(uint32_t u, bool upper) {
     const uint32_t x = __byte_perm(u, 0x64646464u, upper ? 0x4342 : 0x4140);
-    if (RAW) return x;
     const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&x), __half2half2(__ushort_as_half(0x6480)));
     return *reinterpret_cast<const uint32_t*>(&h);
 }

@@ -100,8 +100,8 @@ __device__ __forceinline__ void codes16(const uint4& c, uint32_t* f) {
     const uint32_t w[4] = {c.x ^ 0x80808080u, c.y ^ 0x80808080u, c.z ^ 0x80808080u, c.w ^ 0x80808080u};
     #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        f[2 * i] = two_codes<false>(w[i], false);
-        f[2 * i + 1] = two_codes<false>(w[i], true);
+        f[2 * i] = two_codes(w[i], false);
+        f[2 * i + 1] = two_codes(w[i], true);
     }
 }
 

@@ -767,3 +767,37 @@ def test_calls_at_once(cuda):
             assert torch.equal(got[name], want[name]), name
         for t, new_ in zip((c.k, c.v, c.ks, c.vs), stored):
             assert torch.equal(t, new_)
+
+
+@pytest.mark.parametrize("rows", [(4, 1), (16, 1), (24, 1), (64, 1)])
+@pytest.mark.parametrize("dt", ["f32", "f16"])
+@pytest.mark.parametrize("width", [24, 16384])
+def test_attn8_queries_of_a_large_mean(cuda, dt, rows, width):
+    """Queries around 1024, keys whose codes cancel in pairs: the scores are of ordinary size. All products are
+    whole numbers below 2^14 and their sums whole below 2^21, so 32-bit sums of them are exact: a score is off by its
+    scaling, subtraction and exponential alone, the bound's `big` is the largest |score| and not sum |q| |k|."""
+    import torch
+    H, nq = rows
+    lens = [300, 33]
+    c = Eight(cuda, 30, 2, width, 16, 1, 1, seed=2)
+    c.place(lens, seed=3)
+    r = np.random.default_rng(11)
+    codes = np.repeat(r.integers(-15, 16, c.host.codes[0].shape[:-1] + (64,)), 2, -1).astype(np.int8)
+    codes[..., 1::2] *= -1
+    c.host.codes[0][:] = codes
+    c.host.scales[0][:] = 0.0625
+    c.k.copy_(_t(codes))
+    c.ks.fill_(0.0625)
+    q = _t(1024.0 + r.integers(-3, 4, (2, nq, H, 128))).to(_dt(dt))
+    out = run_attn8(c, 0, q, [0, 1], torch.float32)
+    assert c.take_status() == 0
+    for b, L in enumerate(lens):
+        k, v = (torch.from_numpy(c.host.values(w, 0, c.m.tables[b], L)).cuda()[0] for w in range(2))
+        for h in range(H):
+            x = q[b, :, h].double()
+            o, pv, _, va = attention(x, k, v, torch.tensor([max(0, L - nq + 1 + j) for j in range(nq)], device="cuda"))
+            big = (x @ k.T / math.sqrt(128)).abs().amax(-1, keepdim=True)
+            assert 1 < float(big.max()) < 30
+            tol = attn8_bound(o, pv, big, va, L, dt == "f16", False)
+            err = (out[b, :, h].double() - o).abs()
+            assert bool((err <= tol).all()), (b, h, float((err / tol).max()))
