@@ -438,7 +438,8 @@ SLLM_CUDA_API int sllm_cuda_attn_kv8(const sllm_cuda_kv_pages * p, int32_t layer
  * One step of n beam searches of `beams` beams each. Request i's candidates are
  * (b, x): beam b continued by word x, of value
  *     score[i][b] + logits[i][b][x] - ln sum_y exp(logits[i][b][y])
- * (64 bits; the exponentials 32, their sum 64; logits beyond 2^100 as that); a beam
+ * (64 bits; the exponentials 32, their sum 64; logits beyond 2^100 as that, those of a
+ * row whose largest is beyond 2^24 counted from it); a beam
  * with done[i][b] != 0 has one candidate, eos, of its own score (done NULL: none is).
  * The `beams` best come out in descending order: parent, token and score_out
  * [n][beams]. Equal values: the lower beam first, then the larger logit, then the

@@ -92,14 +92,25 @@ using BeamBest = Word[kBmMost][kBmMost];
 
 // Sums are of 2^(x log2 e - ref) with a whole ref, so those against two references
 // differ by a power of two. log2 e is an f32, off by kBmLog2eOff of itself: what that
-// makes of the largest logit is put right at the end. Logits beyond 2^100 count as that.
-constexpr float kBmLog2e = 1.44269502162933349609375f, kBmHuge = 0x1p100f;
+// makes of the largest logit is put right at the end. A largest logit beyond kBmFar is
+// its own reference, m, and sums are of e^(x - m): of x log2 e a rounded reference
+// would be off by more than an exponent holds. Such a reference is kept as 2 m,
+// beyond all near ones, so that the order is that of the logits. Logits beyond 2^100
+// count as that.
+constexpr float kBmLog2e = 1.44269502162933349609375f, kBmFar = 0x1p24f, kBmHuge = 0x1p100f;
 constexpr double kBmLog2eOff = 1.44269502162933349609375 / 1.4426950408889634074 - 1.0;
-__device__ __forceinline__ double down_by(float d) {        // 2^-d, d whole and not negative
+__device__ __forceinline__ float held(float x) { return fminf(fmaxf(x, -kBmHuge), kBmHuge); }
+__device__ __forceinline__ double limited(uint32_t key) { return (double)held(logit_of(key)); }
+__device__ __forceinline__ bool is_far(float ref) { return fabsf(ref) > 1.5f * kBmFar; }        // (a near one is below 1.4427 kBmFar)
+__device__ __forceinline__ float ref_of(float most) {
+    return fabsf(most) <= kBmFar ? ceilf(most * kBmLog2e) : 2.f * held(most);
+}
+// what sums against ref count in those against top >= ref
+__device__ __forceinline__ double down_to(float top, float ref) {
+    const float d = top - ref;
+    if (is_far(top)) return (double)exp2f(-0.5f * d * kBmLog2e);
     return d < 1000.f ? __hiloint2double((1023 - (int)d) << 20, 0) : 0.0;
 }
-
-__device__ __forceinline__ double limited(uint32_t key) { return (double)fminf(fmaxf(logit_of(key), -kBmHuge), kBmHuge); }
 
 // x += a, y += b in one instruction
 __device__ __forceinline__ void add2(float& x, float& y, float a, float b) {
@@ -130,6 +141,14 @@ __device__ __forceinline__ float sum_exp(const float (&x)[kBmPer], float ref) {
         #pragma unroll
         for (int i = 0; i < n; i += 2) add2(e[i], e[i + 1], e[i + n], e[i + n + 1]);
     return e[0] + e[1];
+}
+
+// ... of e^(x - m), with m the largest of them so far
+__device__ __forceinline__ float sum_far(const float (&x)[kBmPer], float m) {
+    float s = 0.f;
+    #pragma unroll
+    for (int i = 0; i < kBmPer; ++i) s += x[i] > -INFINITY ? exp2f((held(x[i]) - m) * kBmLog2e) : 0.f;
+    return s;
 }
 
 // the largest of a thread's words, NaN if there is one
@@ -392,23 +411,19 @@ beam_select_kernel(const __grid_constant__ BeamParams a) {
             at_piece = piece;
         }
         ++piece;
-        if (!(fabsf(most) <= kBmHuge)) {
-            #pragma unroll
-            for (int e = 0; e < kBmPer; ++e) x[e] = x[e] > -INFINITY ? fminf(fmaxf(x[e], -kBmHuge), kBmHuge) : x[e];
-        }
         if (most > -INFINITY) {
-            const float want = ceilf(fminf(fmaxf(most, -kBmHuge), kBmHuge) * kBmLog2e);
+            const float want = ref_of(most);
             if (want > ref) {
-                sum = ref > -INFINITY ? sum * down_by(want - ref) : 0.0;
+                sum = ref > -INFINITY ? sum * down_to(want, ref) : 0.0;
                 ref = want;
             }
-            sum += (double)sum_exp(x, ref);
+            sum += (double)(is_far(ref) ? sum_far(x, 0.5f * ref) : sum_exp(x, ref));
         }
         if (cur.b != b) {
             by_row[b].most[t] = key_of(most);
             by_row[b].next[t] = (key_of(other) & 0xffff0000u) | (uint32_t)at_piece;
             const float top = logit_of(__reduce_max_sync(0xffffffffu, key_of(ref)));
-            const double all = warp_sum_d(ref > -INFINITY ? sum * down_by(top - ref) : 0.0);
+            const double all = warp_sum_d(ref > -INFINITY ? sum * down_to(top, ref) : 0.0);
             if (lane == 0) {
                 sh.part[b][warp] = all;
                 sh.ref[b][warp] = top;
@@ -430,7 +445,7 @@ beam_select_kernel(const __grid_constant__ BeamParams a) {
         const bool on = (live >> r & 1) != 0 && lo < hi;
         const int c = on ? collect<VEC>(rows + (size_t)r * a.stride, lo, hi, by_row[r], B) : 0;
         const float mine = lane < kBmWarps ? sh.ref[r][lane] : -INFINITY, all = warp_max(mine);
-        const double s = warp_sum_d(mine > -INFINITY ? sh.part[r][lane] * down_by(all - mine) : 0.0);
+        const double s = warp_sum_d(mine > -INFINITY ? sh.part[r][lane] * down_to(all, mine) : 0.0);
         if (lane == 0) {
             sh.count[r] = c;
             sh0.sum[rank][r] = s;
@@ -465,7 +480,7 @@ beam_select_kernel(const __grid_constant__ BeamParams a) {
     for (int r = warp; r < B; r += kBmWarps) {
         const bool on = (live >> r & 1) != 0;
         const float mine = on && lane < C ? sh.refs[lane][r] : -INFINITY, all = warp_max(mine);
-        const double s = warp_sum_d(mine > -INFINITY ? sh.sum[lane][r] * down_by(all - mine) : 0.0);
+        const double s = warp_sum_d(mine > -INFINITY ? sh.sum[lane][r] * down_to(all, mine) : 0.0);
         int head = 0;
         Word w = on && lane < C ? best[lane][r][0] : 0;
         for (int i = 0; i < B; ++i) {
@@ -479,11 +494,14 @@ beam_select_kernel(const __grid_constant__ BeamParams a) {
             }
         }
         __syncwarp();
-        const double lse = ((double)all + log2(s)) * 0.69314718055994530942 - limited((uint32_t)(sh.merged[r][0] >> 32)) * kBmLog2eOff;
+        const double top = limited((uint32_t)(sh.merged[r][0] >> 32));
+        // (of far logits both are counted from the largest: lse would round its logarithm away)
+        const double from = is_far(all) ? top : 0.0;
+        const double lse = is_far(all) ? log(s) : ((double)all + log2(s)) * 0.69314718055994530942 - top * kBmLog2eOff;
         if (lane < B) {
             double v = -INFINITY;
             const Word m = sh.merged[r][lane];
-            if (m != 0) v = (double)sh.score[r] + (limited((uint32_t)(m >> 32)) - lse);
+            if (m != 0) v = (double)sh.score[r] + (limited((uint32_t)(m >> 32)) - from - lse);
             if (!on && lane == 0 && sh.done[r] != 0 && sh.score[r] < INFINITY) v = (double)sh.score[r];
             sh.value[r * B + lane] = v;
         }
