@@ -73,7 +73,6 @@ struct __align__(16) BeamShared {                 // behind it: most and list of
     double part[kBmMost][kBmWarps];                 // a warp's sum of e^(x - ref)
     float ref[kBmMost][kBmWarps];                   // and that ref, whole; -inf: no words
     int count[kBmMost];                             // words in the list
-    int odd;
     float score[kBmMost];
     int done[kBmMost], slots[kBmMost];
     double sum[16][kBmMost];                        // [CTA][beam], of the cluster's first CTA, as are `best` and what follows
@@ -346,8 +345,9 @@ beam_select_kernel(const __grid_constant__ BeamParams a) {
         if (a.done != nullptr) my_done = a.done[(size_t)req * B + lane];
         if (warp == 0 && a.slots != nullptr) my_slot = a.slots[(size_t)req * B + lane];
     }
-    for (int i = t; i < kBmMost * kBmWarps; i += kBmThreads) sh.ref[i / kBmWarps][i % kBmWarps] = -INFINITY;
-    if (t == 0) sh.odd = 0;
+    // (a warp's own column: the stream has no barrier)
+    if (lane < kBmMost) sh.ref[lane][warp] = -INFINITY;
+    __syncwarp();
     const unsigned live = __ballot_sync(0xffffffffu, lane < B && my_done == 0 && my_score > -INFINITY && my_score < INFINITY);
     bool odd = lane < B && !(my_score < INFINITY);
     if (warp == 0 && lane < B) {
@@ -434,9 +434,8 @@ beam_select_kernel(const __grid_constant__ BeamParams a) {
         }
     }
     fetch_wait<0>();
-    if (odd) sh.odd = 1;
+    if (__any_sync(0xffffffffu, odd) && lane == 0) raise(a.status, SLLM_CUDA_ERR_ARG);
     cl.sync();                      // the first CTA no longer needs its ring (and this CTA's shared memory is written)
-    if (t == 0 && sh.odd != 0) raise(a.status, SLLM_CUDA_ERR_ARG);
     // this CTA's best words of each beam, in order, into the first CTA's memory
     BeamShared& sh0 = *cl.map_shared_rank(&sh, 0);
     BeamBest* const best = reinterpret_cast<BeamBest*>(ring);

@@ -85,3 +85,21 @@ def test_far_and_near_in_neighbouring_words(cuda):
             lg = torch.full((1, 2, V), mask, device="cuda")
             lg[0, 0, at], lg[0, 1, V - 1 - at] = 2.0, -mask
             check_far(cuda, lg, _scores(1, 1, 2))
+
+
+@pytest.mark.parametrize("V", [3, 300, 4096])
+@pytest.mark.parametrize("B", [1, 4, 16])
+def test_short_rows_over_and_over(cuda, B, V):
+    """Many requests of one piece a beam, some with a NaN in their last word, 20 times: every warp's sums count and
+    every report arrives. (Sums and reports once passed through words that other warps might clear.)"""
+    n = 1500
+    lg, sc = _logits(V, n, B, V), _scores(V, n, B)
+    first = run(cuda, lg, sc)
+    for i in (0, 700, n - 1):
+        check_far(cuda, lg[i:i + 1], sc[i:i + 1])
+    lg[n - 1, B - 1, V - 1] = math.nan
+    for _ in range(20):
+        got = run(cuda, lg, sc)
+        assert got[5][0] == -1
+        for a, b in zip(got[:3], first[:3]):
+            assert np.array_equal(a[:-1], b[:-1])
