@@ -14,7 +14,10 @@
 // 16 rows, products keep 11 bits down to 2^-21 of the largest). The sums have exponents
 // of their own: w / scale_v would be lost where scales are 2^110 apart. A block of
 // scale_v 0 has zeros for values, whatever its codes, and in the exponents the lowest
-// scale there is, 2^-100, so that it moves no reference that matters.
+// scale there is, 2^-100, so that it moves no reference that matters. A sum's terms are
+// up to 2^115 then: sums are held 2^8 lower, so that 2^21 keys of no value fit. (The
+// other end: of keys whose scales are 2^104 and more, those count that are above 2^-21
+// of the largest. Subnormal terms as well, by exp2f, cost 5%.)
 //
 // Two CTAs a SM. Warps 0-3 and 4-7 (a key a lane, 16 of the rows each group):
 // exponentials. 8-11 (32 keys each): codes to f16, K's into tensor memory, V's into
@@ -45,6 +48,7 @@ constexpr int kW8Threads = 32 * (kW8Plan + 1), kW8Ctas = 2;                     
 constexpr int kW8Half = kE8Keys * 128;              // 64 of the dimensions of a tile, f16
 constexpr int kW8Extra = 2;                         // what a pair's start and end cost, in tiles (with 1 or 3: 72 and 70 us for 68)
 constexpr float kW8Zero = -100.f;                   // log2 of a scale of 0
+constexpr float kW8Sum = 8.f, kW8SumDown = 0x1p-8f; // what sums are held lower by, in powers of two
 constexpr int kW8Plans = 8;                         // tiles planned ahead, some of them in use
 constexpr int kW8Ring = 3;                          // K or V of a tile each
 constexpr uint32_t kW8Cols = 256, kW8O = 2 * kW8Rows, kW8K = 128;       // tensor memory: two S tiles, the outputs, two K tiles
@@ -267,9 +271,10 @@ attn_kv8_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
                 mbar_arrive(&sh.s_free[b]);
                 mbar_arrive(&sh.plan_free[n % kW8Plans]);
             }
+            const float lsum = lsv + kW8Sum;
             #pragma unroll
             for (int i = 0; i < R; ++i) {
-                l[i] += ex2(z[i] - lsv);
+                l[i] += ex2(z[i] - lsum);
                 z[i] = ex2(z[i]);
             }
             if (n >= 2) ok = at_wait_warp(&sh.p_free[b], par ^ 1, ab, w) && ok;
@@ -320,9 +325,9 @@ attn_kv8_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
                 if ((warp & 3) == 0 && lane < live) p.part_ml[at + lane] = make_float2(ref[lane], sum);
                 #pragma unroll
                 for (int i = 0; i < R; ++i)
-                    if (i < live) to[i * kServeDim] = u2f(o[i]);
+                    if (i < live) to[i * kServeDim] = u2f(o[i]) * kW8SumDown;
             } else {
-                const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);          // (0: the row has seen nothing)
+                const float inv = sum == 0.f ? 0.f : __fdiv_rn(kW8SumDown, sum);   // (0: the row has seen nothing)
                 #pragma unroll
                 for (int i = 0; i < R; ++i) {
                     const size_t at = __shfl_sync(0xffffffffu, (unsigned long long)out_at, i);

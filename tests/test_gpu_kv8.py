@@ -801,3 +801,39 @@ def test_attn8_queries_of_a_large_mean(cuda, dt, rows, width):
             tol = attn8_bound(o, pv, big, va, L, dt == "f16", False)
             err = (out[b, :, h].double() - o).abs()
             assert bool((err <= tol).all()), (b, h, float((err / tol).max()))
+
+
+@pytest.mark.parametrize("split", [False, True])
+@pytest.mark.parametrize("low", [0.0, 2.0 ** -100])
+def test_attn8_many_keys_of_no_value(cuda, split, low):
+    """16384 keys whose values are zeros or the least there are, scores 7.5 powers of two above the sequence's first
+    keys, and after them 128 keys of ordinary values, 12 above that: the sums count those without value too. One run
+    of tiles a sequence (as many sequences as two CTAs an SM), or one sequence in many parts."""
+    import torch
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    n, H, page = 1 if split else 2 * sms, 24, 128
+    reps = (4 * sms if split else 1) * 128
+    c = Eight(cuda, 3, 1, max(reps + 2, 4096), page, 1, 1, seed=2)
+    bits = 127 * math.log2(math.e) / math.sqrt(128)          # of a key of code 127 and scale 1
+    k = torch.zeros((3, page, 128))
+    k[1:, :, 0] = 127
+    c.k[:, 0, 0] = k.to(torch.int8).cuda()
+    scales = torch.tensor([1.0, 7.5 / bits, 19.5 / bits])
+    c.ks[:, 0, 0] = scales[:, None].cuda()
+    c.vs[:, 0, 0] = torch.tensor([low, low, 0.03125])[:, None].cuda()
+    c.tables[0, :reps + 2] = _i32([0] + [1] * reps + [2])
+    c.lens[0] = L = (reps + 2) * page
+    q = torch.zeros((n, 1, H, 128), dtype=torch.float16, device="cuda")
+    q[..., 0] = 1
+    out = run_attn8(c, 0, q, [0] * n, torch.float32)
+    assert c.take_status() == 0
+    # three kinds of keys: weights by 64 bits, each kind's values summed first
+    w = torch.exp2(torch.tensor([0.0, 7.5, 19.5], dtype=torch.float64)) * torch.tensor([page, reps * page, page])
+    w = (w / w.sum()).cuda()
+    mean = c.v[:, 0, 0].double().mean(1) * torch.tensor([low, low, 0.03125], dtype=torch.float64, device="cuda")[:, None]
+    o = (w[:, None] * mean).sum(0)
+    size = (w[:, None] * (c.v[:, 0, 0].double().abs().mean(1) * c.vs[:, 0, 0, :1].double())).sum(0)
+    # scores up to 20 in 32 bits, f16 weights, sums of at most 2^20 terms a part in 32 bits (cut: 2 units each), which all
+    # are of one sign and grow by halves: 32 lanes and warps, then tiles, 2^11 of them at most
+    tol = size * (2.1 * (264 + 8) * 2.0 ** -24 * 20 + 2.0 ** -11 * 1.01 + (2.0 ** 11 + 300) * 2 * 2.0 ** -24)
+    assert 0.04 < float(w[2]) and bool(((out.double() - o).abs() <= tol).all())
