@@ -191,11 +191,11 @@ struct Rows8 {
         // seen by its own lane, and then only the row's maximum is looked for. (With it
         // each time, a tile of eight rows took 206 instructions for the 32 keys, not 141.)
         const float base[2] = {ks[0] * kE8Log2, ks[1] * kE8Log2};
-        constexpr float LIFT = e8_lift(P), MOST = 15.f;
+        constexpr float LIFT = e8_lift(P), MOST = P == 1 ? kE8Most : kE8Most + 0.5f;     // (rounding alone moves no reference)
         float z[NT][2][4], top = -INFINITY;
         #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            const float ref[2] = {LIFT - m[n][0], LIFT - m[n][1]};
+            const float ref[2] = {__fsub_ru(LIFT, m[n][0]), __fsub_ru(LIFT, m[n][1])};
             #pragma unroll
             for (int k = 0; k < 2; ++k)
                 #pragma unroll
@@ -224,7 +224,7 @@ struct Rows8 {
                     for (int k = 0; k < 2; ++k)
                         #pragma unroll
                         for (int i = c; i < 4; i += 2)
-                            if (z[n][k][i] > -INFINITY) now = fmaxf(now, s[k][0][n][i] * (P == 1 ? base[k] : base[k] * mul[n][c]));
+                            if (z[n][k][i] > -INFINITY) now = fmaxf(now, __fmul_rd(s[k][0][n][i], P == 1 ? base[k] : base[k] * mul[n][c]));
                     #pragma unroll
                     for (int y = 4; y < 32; y <<= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, y));
                     now = fmaxf(m[n][c], now);
@@ -236,7 +236,7 @@ struct Rows8 {
                         #pragma unroll
                         for (int i = c; i < 4; i += 2)
                             if (z[n][k][i] != -INFINITY)
-                                z[n][k][i] = __fmaf_rn(s[k][0][n][i], P == 1 ? base[k] : base[k] * mul[n][c], LIFT - now);
+                                z[n][k][i] = ended(__fmaf_rn(s[k][0][n][i], P == 1 ? base[k] : base[k] * mul[n][c], __fsub_ru(LIFT, now)));
                 }
                 #pragma unroll
                 for (int j = 0; j < 8; ++j)

@@ -12,13 +12,19 @@ constexpr int kE8Keys = 128;                        // keys of a tile
 constexpr int kE8Blocks = kE8Keys / kKvBlock;
 constexpr int kE8Tile = kE8Keys * kServeDim;        // bytes of one of K or V
 // Weights stand against 2^-lift of a reference and are 2^15 at most. Pairs of f16: the
-// reference is the running maximum. One f16: the maximum when it last grew by more
+// reference is the running maximum, or a little below. One f16: the maximum when it last grew by more
 // than 2^8, so that the outputs are seldom rescaled; weights keep 11 bits down to
 // 2^-21 of the largest. A row that has seen nothing has the reference kE8None.
-constexpr float kE8None = -1e30f;
+// An exponent is one multiply-add of the exact product against the rounded reference.
+// References are rounded down and what is taken off up, so that a row's largest key
+// never vanishes; where a score is so far from zero (2^23) that the rounding shows,
+// exponents end at kE8Top.
+constexpr float kE8None = -3.402823466e38f;
+constexpr float kE8Most = 15.f, kE8Top = 15.9f;     // of exponents: the reference moves above the one; f16 holds the other
 constexpr float kE8Grow = 8.f;
 __host__ __device__ constexpr float e8_lift(int planes) { return planes == 1 ? 15.f - kE8Grow : 15.f; }
 __host__ __device__ constexpr float e8_down(int planes) { return planes == 1 ? 0x1p-7f : 0x1p-15f; }         // 2^-lift
+__device__ __forceinline__ float ended(float z) { return z > kE8Top ? kE8Top : z; }      // (NaN stays)
 constexpr float kE8Log2 = kServeScale * 1.4426950408889634f;
 
 struct Attn8Params {

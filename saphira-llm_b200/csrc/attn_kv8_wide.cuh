@@ -173,7 +173,7 @@ attn_kv8_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
         float* const ref = sh.ref[warp];
         float l[R];
         size_t out_at = 0;                          // of row `lane`
-        constexpr float LIFT = e8_lift(1), MOST = 15.f;
+        constexpr float LIFT = e8_lift(1);
         for (uint32_t n = 0;; ++n) {
             const int b = n & 1;
             const uint32_t par = n >> 1 & 1;
@@ -211,10 +211,10 @@ attn_kv8_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
                 #pragma unroll
                 for (int i = 0; i < R; i += 4) {
                     const float4 r = *reinterpret_cast<const float4*>(ref + i);
-                    z[i] = __fmaf_rn(z[i], base, lsv + LIFT - r.x);
-                    z[i + 1] = __fmaf_rn(z[i + 1], base, lsv + LIFT - r.y);
-                    z[i + 2] = __fmaf_rn(z[i + 2], base, lsv + LIFT - r.z);
-                    z[i + 3] = __fmaf_rn(z[i + 3], base, lsv + LIFT - r.w);
+                    z[i] = __fmaf_rn(z[i], base, __fsub_ru(lsv + LIFT, r.x));
+                    z[i + 1] = __fmaf_rn(z[i + 1], base, __fsub_ru(lsv + LIFT, r.y));
+                    z[i + 2] = __fmaf_rn(z[i + 2], base, __fsub_ru(lsv + LIFT, r.z));
+                    z[i + 3] = __fmaf_rn(z[i + 3], base, __fsub_ru(lsv + LIFT, r.w));
                 }
                 if (masked) {
                     #pragma unroll
@@ -225,7 +225,7 @@ attn_kv8_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
             exponents();
             #pragma unroll
             for (int i = 0; i < R; ++i) top = fmaxf(top, z[i]);
-            if (soft_any(group, top > MOST || stop)) {
+            if (soft_any(group, top > kE8Most || stop)) {
                 // (the group's warps leave together: they meet at barriers without a limit)
                 if (soft_any(group, stop)) break;
                 // the references move to the rows' maxima, and what stands against the
@@ -234,7 +234,7 @@ attn_kv8_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
                 float mine = kE8None;               // row `lane`
                 #pragma unroll
                 for (int i = 0; i < R; ++i) {
-                    const float m = warp_top(!masked || j < sh.lim[warp][i] ? __fmaf_rn(z[i], base, lsv) : kE8None);
+                    const float m = warp_top(!masked || j < sh.lim[warp][i] ? __fmaf_rd(z[i], base, lsv) : kE8None);
                     if (lane == i) mine = m;
                 }
                 if (lane < R) sh.most[warp][lane] = mine;
@@ -264,6 +264,8 @@ attn_kv8_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
                 #pragma unroll
                 for (int i = 0; i < R; ++i) l[i] *= alpha[i];
                 exponents();
+                #pragma unroll
+                for (int i = 0; i < R; ++i) z[i] = ended(z[i]);
             }
             tc_fence_before();
             __syncwarp();

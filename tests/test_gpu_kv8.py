@@ -837,3 +837,48 @@ def test_attn8_many_keys_of_no_value(cuda, split, low):
     # are of one sign and grow by halves: 32 lanes and warps, then tiles, 2^11 of them at most
     tol = size * (2.1 * (264 + 8) * 2.0 ** -24 * 20 + 2.0 ** -11 * 1.01 + (2.0 ** 11 + 300) * 2 * 2.0 ** -24)
     assert 0.04 < float(w[2]) and bool(((out.double() - o).abs() <= tol).all())
+
+
+FORMS = [("f32", 8, 1, 40), ("f16", 8, 1, 40), ("f32", 24, 1, 40), ("f16", 24, 1, 40), ("f16", 24, 1, 16384), ("f16", 16, 3, 16384)]
+
+
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("unit", [1e3, 1e5, 1e6, 1e8, 1e12, 1e31])
+@pytest.mark.parametrize("form", FORMS, ids=str)
+def test_attn8_scores_far_from_zero(cuda, form, unit, sign):
+    """Scores of `unit` times whole numbers, above and below zero. One key's is 10 units above all others', so its
+    weight is 1 and the others' are 0: its values come out, off by the rounding of its weight (f16: 2^-11) and by
+    some 32-bit ones. Then keys of one score, whose mean comes out: each key's weight is rounded the same way."""
+    import torch
+    dt, H, nq, width = form
+    lens = [500, 130]
+    c = Eight(cuda, 50, 2, width, 16, 1, 1, seed=2)
+    c.place(lens, seed=3)
+    r = np.random.default_rng(4)
+    bits = math.log2(math.e) / math.sqrt(128)
+    c.ks.fill_(unit / 512 / bits)
+    c.host.scales[0][:] = unit / 512 / bits
+    q = torch.zeros((2, nq, H, 128), dtype=_dt(dt), device="cuda")
+    q[..., 0] = 512.0 * sign
+    one = 2.0 ** -11 * 1.01 + 16 * 2.0 ** -24 if dt == "f16" else 2.0 ** -22 * 1.01 + 16 * 2.0 ** -24
+    for same in (False, True):
+        codes = np.zeros(c.host.codes[0].shape, np.int8)
+        codes[..., 0] = 50 if same else r.integers(-90, 91, codes.shape[:-1])
+        if same:                                             # (one scale: the wide form rounds it with the score)
+            c.host.scales[1][:] = 0.03125
+            c.vs.fill_(0.03125)
+        win = [int(r.integers(L - nq + 1)) for L in lens]
+        if not same:
+            for b, x in enumerate(win):
+                codes[c.m.tables[b][x // 16], 0, 0, x % 16, 0] = 100 * sign
+        c.k.copy_(_t(codes))
+        out = run_attn8(c, 0, q, [0, 1], torch.float32)
+        assert c.take_status() == 0
+        for b, L in enumerate(lens):
+            v = torch.from_numpy(c.host.values(1, 0, c.m.tables[b], L)).cuda()[0]
+            for j in range(nq):
+                seen = L - nq + 1 + j
+                want = v[:seen].mean(0) if same else v[win[b]]
+                size = v[:seen].abs().mean(0) if same else want.abs()
+                err = (out[b, j].double() - want).abs()
+                assert bool((err <= size * (one + 2 * seen * 2.0 ** -24) + 1e-37).all()), (same, b, j, float((err / size).max()))
