@@ -882,3 +882,84 @@ def test_attn8_scores_far_from_zero(cuda, form, unit, sign):
                 size = v[:seen].abs().mean(0) if same else want.abs()
                 err = (out[b, j].double() - want).abs()
                 assert bool((err <= size * (one + 2 * seen * 2.0 ** -24) + 1e-37).all()), (same, b, j, float((err / size).max()))
+
+
+@pytest.mark.parametrize("form", FORMS, ids=str)
+def test_attn8_rows_that_are_no_numbers(cuda, form):
+    """Query rows with a NaN or an infinity come out as NaN, where they see a key; all others as they should."""
+    import torch
+    dt, H, nq, width = form
+    lens = [200, 33, 1]
+    c = Eight(cuda, 40, 3, width, 16, 1, 1, seed=2)
+    c.place(lens, seed=3)
+    q = _q(5, 3, nq, H, _dt(dt))
+    odd = {(0, nq - 1, 3): math.nan, (0, 0, H - 1): math.inf, (1, 0, 0): -math.inf, (1, nq - 1, 5): math.nan}
+    bad = q.clone()
+    for (b, j, h), x in odd.items():
+        bad[b, j, h, 17 + h] = x
+    out = run_attn8(c, 0, bad, [0, 1, 2], torch.float32)
+    assert c.take_status() == 0
+    for b, j, h in odd:
+        assert bool(out[b, j, h].isnan().all())
+    good = run_attn8(c, 0, q, [0, 1, 2], torch.float32)
+    for b, j, h in odd:
+        out[b, j, h] = good[b, j, h]
+    check_attn8(c, 0, q, out, [0, 1, 2], dt == "f16")
+
+
+@pytest.mark.parametrize("H,nq", [(24, 1), (8, 4), (40, 1)])
+@pytest.mark.parametrize("page", [16, 32, 128])
+def test_attn8_wide_unseen_places_leave_no_trace(cuda, page, H, nq):
+    """test_attn8_unseen_places_leave_no_trace over tables with room for many keys; every place that no sequence
+    sees is poisoned, tiles end inside pages and blocks."""
+    import torch
+    lens = [100, 7, 64, 300, 0]
+    width = (1 << 20) // page // 4
+    c = Eight(cuda, 60, 5, width, page, 1, 1, seed=2)
+    c.place(lens, seed=3)
+    q = _q(5, 5, nq, H, torch.float16)
+    a = run_attn8(c, 0, q, [0, 1, 2, 3, 4], torch.float32)
+    seen = {(c.m.tables[s][t // page], t % page) for s in range(5) for t in range(lens[s])}
+    blocks = {(p, row // BLOCK) for p, row in seen}
+    for p in range(60):
+        for b in range(page // BLOCK):
+            if (p, b) not in blocks:
+                c.ks[p, :, :, b], c.vs[p, :, :, b] = math.nan, math.inf
+        for row in range(page):
+            if (p, row) not in seen:
+                c.k[p, :, :, row], c.v[p, :, :, row] = 127, -128
+    for s in range(5):
+        c.tables[s, -(-lens[s] // page):] = 1 << 30
+    b = run_attn8(c, 0, q, [0, 1, 2, 3, 4], torch.float32)
+    assert c.take_status() == 0 and torch.equal(a, b)
+    check_attn8(c, 0, q, a, [0, 1, 2, 3, 4], True)
+
+
+@pytest.mark.parametrize("H,nq", [(24, 1), (8, 4), (40, 1)])
+def test_attn8_wide_peaked_rows(cuda, H, nq):
+    """test_attn8_peaked_rows over tables with room for many keys, value scales of e^-3 to e^3. (A product of weight and
+    scale below 2^-14 of the range is off by 2^-25 of it, as test_attn8_scales_far_apart derives.)"""
+    import torch
+    lens = [700, 333]
+    c = Eight(cuda, 70, 2, 32768, 16, 1, 1, seed=2)
+    c.place(lens, seed=3)
+    r = np.random.default_rng(3)
+    c.host.scales[0][:] = np.exp(r.uniform(-8, 1.5, c.host.scales[0].shape)).astype(np.float32)
+    c.host.scales[1][:] = np.exp(r.uniform(-3, 3, c.host.scales[1].shape)).astype(np.float32)
+    c.ks.copy_(_t(c.host.scales[0]))
+    c.vs.copy_(_t(c.host.scales[1]))
+    q = _q(5, 2, nq, H, torch.float16, 0.2)
+    out = run_attn8(c, 0, q, [0, 1], torch.float32)
+    assert c.take_status() == 0
+    for b, L in enumerate(lens):
+        k, v = (torch.from_numpy(c.host.values(w, 0, c.m.tables[b], L)).cuda()[0] for w in range(2))
+        scale = torch.from_numpy(np.repeat(np.concatenate([c.host.scales[1][p, 0, 0] for p in c.m.tables[b][:c.m.used(L)]]),
+                                           BLOCK)[:L]).cuda().double()
+        for h in range(H):
+            lim = torch.tensor([max(0, L - nq + 1 + j) for j in range(nq)], device="cuda")
+            o, pv, big, va = attention(q[b, :, h].double(), k, v, lim)
+            s = q[b, :, h].double() @ k.T / math.sqrt(128)
+            s[torch.arange(L, device="cuda")[None] >= lim[:, None]] = -math.inf
+            top = (torch.softmax(s, -1) * scale).amax(-1, keepdim=True)
+            tol = attn8_bound(o, pv, big, va, L, True, False) + 2.0 ** -32 * 1.01 * top * (v / scale[:, None]).abs().sum(0)
+            assert bool(((out[b, :, h].double() - o).abs() <= tol).all()), (b, h)
