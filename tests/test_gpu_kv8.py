@@ -963,3 +963,78 @@ def test_attn8_wide_peaked_rows(cuda, H, nq):
             top = (torch.softmax(s, -1) * scale).amax(-1, keepdim=True)
             tol = attn8_bound(o, pv, big, va, L, True, False) + 2.0 ** -32 * 1.01 * top * (v / scale[:, None]).abs().sum(0)
             assert bool(((out[b, :, h].double() - o).abs() <= tol).all()), (b, h)
+
+
+@pytest.mark.parametrize("heads", [(4, 1), (6, 3), (20, 5), (16, 16)])
+@pytest.mark.parametrize("out", ["f32", "f16"])
+def test_append8_prompts(cuda, heads, out):
+    """Tokens enough for eight heads of k and v a CTA (more than four CTAs an SM with one), some of them padded, wrong
+    or repeated: codes and scales of whole pools, rotated rows, rows left alone."""
+    import torch
+    from kv8_ref import rope
+    H, Hkv = heads
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    T = 16 * (4 * sms // (2 * Hkv) + 1) + 37
+    page, S = 64, 3
+    lens = [T // 2 + 9, T - T // 2 + 40, 5]
+    c = Eight(cuda, T // page + 9, S, T // page + 2, page, 1, Hkv, seed=3)
+    c.place(lens, seed=1)
+    slot = [0] * (T // 2) + [1] * (T - T // 2)
+    pos = [9 + i for i in range(T // 2)] + [40 + i for i in range(T - T // 2)]
+    for i in range(20, 25):
+        slot[i] = -1
+    slot[103:103] = [2, S + 1, 2]                            # (between two blocks: a block's tokens stay together)
+    pos[103:103] = [4, 0, 5]                                # (the first fits, the slot ends before the last)
+    slot.insert(300, slot[300])
+    pos.insert(300, pos[300])                               # one position twice
+    n = len(slot)
+    cos, sin = _angles(max(lens))
+    r = np.random.default_rng(H)
+    qkv = r.standard_normal((n, H + 2 * Hkv, 128)).astype(np.float32) * np.exp(r.normal(0, 1, (n, 1, 1))).astype(np.float32)
+    d = _t(qkv)
+    qo = torch.full((n, H, 128), 7.0, dtype=_dt(out), device="cuda")
+    ko, vo = (torch.full((n, Hkv, 128), 7.0, dtype=_dt(out), device="cuda") for _ in range(2))
+    c.p.append8(0, _i32(slot), _i32(pos), d[:, :H], d[:, H:H + Hkv], d[:, H + Hkv:], _t(cos), _t(sin), qo, ko, vo, c.status)
+    torch.cuda.synchronize()
+    bad, left = c.host.append(0, c.m.tables, c.m.lens, c.m.refs, slot, pos, qkv[:, H:H + Hkv], qkv[:, H + Hkv:], cos, sin)
+    assert bad and c.take_status() == -1 and all(c.same())
+    got = [x.cpu().numpy() for x in (qo, ko, vo)]
+    for t in range(n):
+        if slot[t] < 0:
+            assert all((x[t] == 7).all() for x in got)
+        elif t in left:
+            assert (got[1][t] == 7).all() and (got[2][t] == 7).all()
+        else:
+            for x, a, b, rot in ((got[0], 0, H, True), (got[1], H, H + Hkv, True), (got[2], H + Hkv, H + 2 * Hkv, False)):
+                want = rope(qkv[t, a:b], cos[pos[t]], sin[pos[t]]) if rot else qkv[t, a:b]
+                assert np.array_equal(x[t], want.astype(x.dtype))
+
+
+@pytest.mark.parametrize("heads", [1, 3, 8])
+@pytest.mark.parametrize("out", ["f32", "f16"])
+@pytest.mark.parametrize("which", ["kv", "k", "v"])
+def test_read8_documents(cuda, heads, out, which):
+    """Tokens enough for 32 a warp, in any order, twice, wrong and padded."""
+    import torch
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    n = 16 * sms * 32 // (heads * len(which)) + 45
+    page = 32
+    c = Eight(cuda, 90, 3, 40, page, 2, heads, seed=heads)
+    c.place([1200, 1, 700], seed=2)
+    r = np.random.default_rng(5)
+    slot, pos = r.integers(0, 3, n), r.integers(0, 700, n)
+    odd = r.random(n) < 0.05
+    slot[odd], pos[odd] = r.integers(-1, 5, int(odd.sum())), r.integers(-2, 1400, int(odd.sum()))
+    ok = (slot >= 0) & (slot < 3)
+    ok &= (pos >= 0) & (pos < np.where(ok, np.array(c.m.lens)[np.where(ok, slot, 0)], 0))
+    ko, vo = (torch.full((n, heads, 128), 7.0, dtype=_dt(out), device="cuda") if w in which else None for w in "kv")
+    c.p.read8(1, _i32(slot.tolist()), _i32(pos.tolist()), ko, vo, c.status)
+    torch.cuda.synchronize()
+    assert c.take_status() == -1
+    pg = np.array(c.m.tables)[np.where(ok, slot, 0), np.where(ok, pos, 0) // page]
+    row = np.where(ok, pos, 0) % page
+    for w, o in ((0, ko), (1, vo)):
+        if o is not None:
+            got = o.cpu().numpy()
+            want = c.host.codes[w][pg, 1, :, row].astype(np.float32) * c.host.scales[w][pg, 1, :, row // BLOCK][..., None]
+            assert np.array_equal(got[ok], want.astype(got.dtype)[ok]) and (got[~ok] == 7).all()
