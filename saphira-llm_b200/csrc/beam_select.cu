@@ -121,17 +121,21 @@ __device__ __forceinline__ void add2(float& x, float& y, float a, float b) {
         : "f"(a), "f"(b));
 }
 
-// the sum of 2^(x log2 e - ref) over a thread's words, two at a time
-__device__ __forceinline__ float sum_exp(const float (&x)[kBmPer], float ref) {
+// the sum of 2^((x - from) log2 e - ref) over a thread's words, two at a time
+template <bool FROM>
+__device__ __forceinline__ float sum_exp(const float (&x)[kBmPer], float from, float ref) {
     float e[kBmPer];
     #pragma unroll
+    for (int i = 0; i < kBmPer; ++i) e[i] = x[i];
+    #pragma unroll
     for (int i = 0; i < kBmPer; i += 2) {
+        if (FROM) add2(e[i], e[i + 1], -from, -from);
         asm("{\n\t.reg .b64 x, l, r;\n\t"
-            "mov.b64 x, {%2, %3};\n\tmov.b64 l, {%4, %4};\n\tmov.b64 r, {%5, %5};\n\t"
+            "mov.b64 x, {%0, %1};\n\tmov.b64 l, {%2, %2};\n\tmov.b64 r, {%3, %3};\n\t"
             "fma.rn.f32x2 x, x, l, r;\n\t"
             "mov.b64 {%0, %1}, x;\n\t}"
-            : "=f"(e[i]), "=f"(e[i + 1])
-            : "f"(x[i]), "f"(x[i + 1]), "f"(kBmLog2e), "f"(-ref));
+            : "+f"(e[i]), "+f"(e[i + 1])
+            : "f"(kBmLog2e), "f"(-ref));
         asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e[i]));
         asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e[i + 1]));
     }
@@ -140,14 +144,6 @@ __device__ __forceinline__ float sum_exp(const float (&x)[kBmPer], float ref) {
         #pragma unroll
         for (int i = 0; i < n; i += 2) add2(e[i], e[i + 1], e[i + n], e[i + n + 1]);
     return e[0] + e[1];
-}
-
-// ... of e^(x - m), with m the largest of them so far
-__device__ __forceinline__ float sum_far(const float (&x)[kBmPer], float m) {
-    float s = 0.f;
-    #pragma unroll
-    for (int i = 0; i < kBmPer; ++i) s += x[i] > -INFINITY ? exp2f((held(x[i]) - m) * kBmLog2e) : 0.f;
-    return s;
 }
 
 // the largest of a thread's words, NaN if there is one
@@ -417,7 +413,19 @@ beam_select_kernel(const __grid_constant__ BeamParams a) {
                 sum = ref > -INFINITY ? sum * down_to(want, ref) : 0.0;
                 ref = want;
             }
-            sum += (double)(is_far(ref) ? sum_far(x, 0.5f * ref) : sum_exp(x, ref));
+        }
+        // (a thread without words yet: its terms are 0 against any reference; together, as
+        // far words among near ones would else take both ways)
+        const bool far = is_far(ref) && ref > -INFINITY;
+        if (!__any_sync(0xffffffffu, far)) {
+            sum += (double)sum_exp<false>(x, 0.f, ref > -INFINITY ? ref : 0.f);
+        } else {
+            const float from = far ? 0.5f * ref : 0.f;
+            if (fabsf(from) == kBmHuge) {
+                #pragma unroll
+                for (int e = 0; e < kBmPer; ++e) x[e] = x[e] > -INFINITY ? held(x[e]) : x[e];
+            }
+            sum += (double)sum_exp<true>(x, from, far || !(ref > -INFINITY) ? 0.f : ref);
         }
         if (cur.b != b) {
             by_row[b].most[t] = key_of(most);
