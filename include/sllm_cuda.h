@@ -384,9 +384,10 @@ SLLM_CUDA_API int sllm_cuda_attn_prefix(const sllm_cuda_kv_pages * p, int32_t la
  * may be stored again after kv_release. The call's tokens of one block
  * stand together in its lists, in ascending order; one that does not come after
  * the token before it of the same block sets SLLM_CUDA_ERR_ARG in *status and is
- * left out of the cache. A block that the lists come back to later leaves a mix
- * of both. A NaN is stored as 0, an infinity as 127 times the scale of the finite
- * values, both with SLLM_CUDA_ERR_ARG in *status.
+ * left out of the cache, with those of the block that stand after it. A block that
+ * the lists come back to later leaves a mix of both. A NaN is stored as 0, an
+ * infinity as 127 times the scale of the finite values, both with
+ * SLLM_CUDA_ERR_ARG in *status.
  * q_out [n_tokens][n_head][128] and k_out, v_out [n_tokens][n_head_kv][128], of
  * type out_type, receive the rotated q, k and v before quantisation (k_out and
  * v_out may be NULL; q and q_out may both be NULL). Padding, wrong tokens and
@@ -438,19 +439,20 @@ SLLM_CUDA_API int sllm_cuda_attn_kv8(const sllm_cuda_kv_pages * p, int32_t layer
  * One step of n beam searches of `beams` beams each. Request i's candidates are
  * (b, x): beam b continued by word x, of value
  *     score[i][b] + logits[i][b][x] - ln sum_y exp(logits[i][b][y])
- * (64 bits; the exponentials 32, their sum 64; logits beyond 2^100 as that, those of a
- * row whose largest is beyond 2^24 counted from it); a beam
- * with done[i][b] != 0 has one candidate, eos, of its own score (done NULL: none is).
- * The `beams` best come out in descending order: parent, token and score_out
- * [n][beams]. Equal values: the lower beam first, then the larger logit, then the
- * lower word. Row (i, b) of the logits lies at logits + (i * beams + b) * row_stride. A score or logit of -inf makes
- * candidates of value -inf, which are chosen, lowest (b, x) first, only when
- * there are no others; NaN and +inf count as -inf and set SLLM_CUDA_ERR_ARG in
- * *status. done_out[i][j] (may be NULL) is 1 when the parent was done or the
- * token is eos. src[i][j] = slots[i][parent[i][j]] (both NULL or neither): with them
- * sllm_cuda_kv_fork(src, dst = slots) lets every beam's slot hold its parent's
- * tokens. eos < 0: no such word (then done and done_out must be NULL). The outputs may
- * not overlap score or done. beams <= 16, n <= 65536, n_vocab <= 2^20.
+ * (64 bits; the exponentials 32, their sum 64; logits beyond 2^100 as that, those of
+ * a row whose largest is beyond 2^24 counted from it); a beam with done[i][b] != 0
+ * has one candidate, eos, of its own score (done NULL: none is). The `beams` best
+ * come out in descending order: parent, token and score_out [n][beams]. Equal
+ * values: the lower beam first, then the larger logit, then the lower word. Row
+ * (i, b) of the logits lies at logits + (i * beams + b) * row_stride. A score or
+ * logit of -inf makes candidates of value -inf, which are chosen, lowest (b, x)
+ * first, only when there are no others; NaN and +inf count as -inf and set
+ * SLLM_CUDA_ERR_ARG in *status (the logits of beams that are done, or have a score
+ * of -inf, are not read). done_out[i][j] (may be NULL) is 1 when the parent was done
+ * or the token is eos. src[i][j] = slots[i][parent[i][j]] (both NULL or neither):
+ * with them sllm_cuda_kv_fork(src, dst = slots) lets every beam's slot hold its
+ * parent's tokens. eos < 0: no such word (then done and done_out must be NULL). The
+ * outputs may not overlap score or done. beams <= 16, n <= 65536, n_vocab <= 2^20.
  */
 SLLM_CUDA_API int sllm_cuda_beam_select(const float * logits, size_t row_stride, const float * score,
                                         const int32_t * done, const int32_t * slots, int32_t n, int32_t beams,

@@ -1038,3 +1038,56 @@ def test_read8_documents(cuda, heads, out, which):
             got = o.cpu().numpy()
             want = c.host.codes[w][pg, 1, :, row].astype(np.float32) * c.host.scales[w][pg, 1, :, row // BLOCK][..., None]
             assert np.array_equal(got[ok], want.astype(got.dtype)[ok]) and (got[~ok] == 7).all()
+
+
+FIRST = """
+import importlib, sys
+sys.path.insert(0, %r)
+import torch
+sllm = importlib.import_module("saphira-llm_b200")
+i32 = lambda a: torch.tensor(a, dtype=torch.int32, device="cuda")
+z = lambda shape, dt=torch.float32: torch.zeros(shape, dtype=dt, device="cuda")
+k, v = (z((9, 1, 1, 16, 128), torch.int8) for _ in range(2))
+ks, vs = (z((9, 1, 1, 1)) for _ in range(2))
+tables = i32([list(range(8)) + [0] * 65528])
+refs, lens = i32([1] * 9), i32([100])
+x = torch.randn((100, 34, 128), generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")
+cos, sin = torch.ones((100, 64), device="cuda"), z((100, 64))
+slot, pos, status = i32([0] * 100), i32(list(range(100))), i32([0])
+ko, vo = z((100, 1, 128)), z((100, 1, 128))
+qs = [x[:1, 2:2 + h].reshape(1, 1, h, 128).to(dt).contiguous() for h, dt in ((8, torch.float32), (16, torch.float16), (32, torch.float16))]
+outs = [torch.zeros_like(q) for q in qs]
+lg, sc, so = torch.randn((2, 2, 500), device="cuda"), z((2, 2)), z((2, 2))
+pa, to = (z((2, 2), torch.int32) for _ in range(2))
+slots = i32([0])
+s, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+torch.cuda.synchronize()
+p = sllm.KvPages(k, v, refs, tables, lens, ks, vs)
+with torch.cuda.graph(g, stream=s):
+    works = [torch.empty(p.attn8_work_bytes(1, 1, q.shape[2]), dtype=torch.uint8, device="cuda") for q in qs]
+    p.append8(0, slot, pos, None, x[:, :1], x[:, 1:2], cos, sin, status=status, stream=s)
+    p.read8(0, slot, pos, ko, vo, status, stream=s)
+    for q, o, w in zip(qs, outs, works):
+        p.attn8(0, q, o, slots, w, status, stream=s)
+    sllm.beam_select(lg, sc, so, pa, to, status=status, stream=s)
+g.replay()
+torch.cuda.synchronize()
+assert int(status) == 0
+assert float((ko - x[:, :1]).abs().max()) < 0.05 and float((vo - x[:, 1:2]).abs().max()) < 0.05
+for q, o in zip(qs, outs):
+    w = torch.softmax(q[0, 0].double() @ ko[:, 0].double().T / 128 ** 0.5, -1)
+    assert float((o[0, 0].double() - w @ vo[:, 0].double()).abs().max()) < 0.01
+lp = torch.log_softmax(lg.double(), -1).view(2, -1).topk(2).values
+assert float((so - lp).abs().max()) < 1e-3
+print("fine")
+"""
+
+
+def test_first_calls_of_a_process_are_captured(cuda):
+    """Nothing of a call needs one outside a capture before it."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST % root], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "fine" in r.stdout, r.stderr[-2000:]
