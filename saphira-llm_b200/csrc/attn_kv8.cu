@@ -26,9 +26,8 @@
 // depend on them.
 //
 // Bound: HBM for long contexts (f16, 64/8 heads: one sequence of 131072 keys, 269 MB
-// of codes and scales, 54 us; 64 of up to 8192, 539 MB, 96 us, 5.6 TB/s), with the
-// issue slots half taken: a block of 16 keys and eight rows is about 70 instructions
-// of a warp. For little work the chain is the bound: lengths, page ids, tile,
+// of codes and scales, 54 us; 64 of up to 8192, 539 MB, 97 us, 5.6 TB/s), with the
+// issue slots half taken (53%). For little work the chain is the bound: lengths, page ids, tile,
 // products, the parts and their join (one sequence of 320 keys 11 us, 2 of them
 // the join). Tiles of 128 keys in two stages leave room for three CTAs a SM
 // with up to eight rows, each with a warp that loads.
@@ -189,7 +188,7 @@ struct Rows8 {
         }
         // Exponents against the rows' references, no shuffles: one that is too large is
         // seen by its own lane, and then only the row's maximum is looked for. (With it
-        // each time, a tile of eight rows took 206 instructions for the 32 keys, not 141.)
+        // each time, a tile of eight rows took 65 instructions more for the 32 keys.)
         const float base[2] = {ks[0] * kE8Log2, ks[1] * kE8Log2};
         constexpr float LIFT = e8_lift(P), MOST = P == 1 ? kE8Most : kE8Most + 0.5f;     // (rounding alone moves no reference)
         float z[NT][2][4], top = -INFINITY;
@@ -661,10 +660,12 @@ struct Cut8 {
 // `keys`: the most that there may be, of all pairs. The wide form's longer chain
 // from a CTA's first load to its last result costs 4 us, and its tiles take four
 // fifths of the time. Both measured, in us, f16 (wide, this file's): 10 sequences of
-// 1000 keys at most, 4 tokens of 64/8 heads (80 thousand keys at most) 22.6, 18.7; 20 of
-// 2000 (320) 33.2, 32.9; 64 of 1000 (512) 49.2, 47.4; 30 of 4000, 5 tokens of 20/5 heads
-// (600) 41.3, 42.8; one of 60000 (480) 48.6, 55.7; 8 of 8000, 8 tokens (1024) 61.7,
-// 71.7; 32 of 8192 (2097) 94, 110.
+// 1000 keys at most, 4 tokens of 64/8 heads (80 thousand keys at most) 22.4, 18.5; 20 of
+// 2000 (320) 32.9, 32.8; 64 of 1000 (512) 47.7, 47.3; 30 of 4000, 5 tokens of 20/5 heads
+// (600) 40.6, 43.1; one of 60000 (480) 48.3, 56.2; 8 of 8000, 8 tokens (1024) 61.3,
+// 71.9; 32 of 8192 (2097) 93, 112. The host knows the tables' width, not the lengths:
+// in tables with room for much, short sequences take the wide form too, 4 tokens of
+// 64/8 heads: 64 of 200 keys 30.8, 28.7; 16 of 500 22.6, 19.3.
 constexpr long long kE8WideKeys = 3000;             // a SM
 Cut8 cut8(int rows, bool f16, int sms, long long keys) {
     Cut8 x;

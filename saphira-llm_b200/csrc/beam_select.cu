@@ -11,8 +11,8 @@
 // memory. A thread copies and reads its own words (4-byte copies where rows are
 // not aligned), and keeps of a beam its largest logit and its sum of
 // exponentials (terms and sums of 16 in 32 bits, else 64, against its own running
-// maximum, rounded up to a power of two), so the stream has no barrier in it. What follows is short: of a
-// beam's 256 largest-of-a-thread the `beams`-th best is a bound that at least as
+// maximum, rounded up to a power of two, or as it is where it is far from zero), so
+// the stream has no barrier in it. What follows is short: of a beam's 256 largest-of-a-thread the `beams`-th best is a bound that at least as
 // many words reach; the few threads that reach it have their words read again
 // (from L2), those words are put in order, and the first CTA of the cluster gets
 // the lists through distributed shared memory and merges them. A list that overflows
