@@ -27,10 +27,10 @@
 //
 // Bound: HBM for long contexts (f16, 64/8 heads: one sequence of 131072 keys, 269 MB
 // of codes and scales, 54 us; 64 of up to 8192, 539 MB, 97 us, 5.6 TB/s), with the
-// issue slots half taken (53%). For little work the chain is the bound: lengths, page ids, tile,
-// products, the parts and their join (one sequence of 320 keys 11 us, 2 of them
-// the join). Tiles of 128 keys in two stages leave room for three CTAs a SM
-// with up to eight rows, each with a warp that loads.
+// issue slots half taken (53%). For little work the chain is the bound: lengths, page
+// ids, tile, products, the parts and their join (one sequence of 320 keys 11 us, 2 of
+// them the join). Tiles of 128 keys in two stages leave room for three CTAs a SM with
+// up to eight rows, each with a warp that loads.
 
 #include <type_traits>
 

@@ -12,13 +12,14 @@
 // not aligned), and keeps of a beam its largest logit and its sum of
 // exponentials (terms and sums of 16 in 32 bits, else 64, against its own running
 // maximum, rounded up to a power of two, or as it is where it is far from zero), so
-// the stream has no barrier in it. What follows is short: of a beam's 256 largest-of-a-thread the `beams`-th best is a bound that at least as
-// many words reach; the few threads that reach it have their words read again
-// (from L2), those words are put in order, and the first CTA of the cluster gets
-// the lists through distributed shared memory and merges them. A list that overflows
-// (many equal logits) is made word by word instead. Keeping lists while
-// streaming, against bounds that the warps exchanged at a barrier per piece, took
-// more clocks than the exponentials: 51 us for 32 requests of 8 beams.
+// the stream has no barrier in it. What follows is short: of a beam's 256
+// largest-of-a-thread the `beams`-th best is a bound that at least as many words
+// reach; the few threads that reach it have their words read again (from L2), those
+// words are put in order, and the first CTA of the cluster gets the lists through
+// distributed shared memory and merges them. A list that overflows (many equal logits)
+// is made word by word instead. Keeping lists while streaming, against bounds that the
+// warps exchanged at a barrier per piece, took more clocks than the exponentials: 51 us
+// for 32 requests of 8 beams.
 //
 // Bound: for many requests the exponentials and the loads together (32 of 8 beams,
 // 128256 words, 118 to 131 MB: 37 us, 3.5 TB/s, a third of the exponential pipe and 45%
